@@ -62,7 +62,9 @@ typedef enum {
   PC2D_ERR_TIMEOUT = 5           /* a device-side barrier wait gave up */
 } pc2d_status;
 
-typedef enum { PC2D_DTYPE_F32 = 0, PC2D_DTYPE_F64 = 1 } pc2d_dtype;
+/* F16 and BF16 are element types of the sequence operators (dropout, causal
+ * convolution, state space scan) only. */
+typedef enum { PC2D_DTYPE_F32 = 0, PC2D_DTYPE_F64 = 1, PC2D_DTYPE_F16 = 2, PC2D_DTYPE_BF16 = 3 } pc2d_dtype;
 
 /* Kernel families.  AUTO picks the tcgen05 tensor-core kernels (3xTF32 split
  * precision) for fp32 shapes they support and the CUDA-core kernels
@@ -210,6 +212,94 @@ int pc2d_comm_allreduce(pc2d_comm *comm, const void *src, void *dst, size_t coun
 int pc2d_param_step(int dtype, void *pars, const void *grad, void *momentum_buf, int m, int d, double lr,
                     double h_lr_factor, double p_lr_factor, double weight_decay, double wd_factor,
                     double momentum, int first_step, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Sequence operators, beside the convolution and over the maps it writes: an
+ * [N][C][H][W] map is [batch][channels][length] with length = H*W.  They have
+ * no counterpart in the reference.  All arrays are contiguous; activations,
+ * states, checkpoints and their gradients are 16-byte aligned; no output may
+ * overlap an input.  float32, float16 and bfloat16 (dropout float64 too); sums
+ * and states are held in 32 bits and rounded once to the outputs' type.  The
+ * results do not depend on the order in which blocks run.  With `lengths`
+ * (int32 on the device, one per batch row, taken as 0 .. length), the
+ * positions of a row behind its length are not read: outputs and gradients
+ * there are 0 and the states are those after the row's last token.
+ *
+ * Dropout.  Element i is kept when its 16 random bits are at least
+ * thr = round(65536 p), and multiplied by 65536/(65536 - thr); it is 0
+ * otherwise, whatever it held.  output = residual + that (residual may be
+ * NULL).  The bits are half i % 8 (low half of word 0 first) of the four words
+ * that Philox4x32-10 gives for the counter (i/8, key[1]) under the key key[0]
+ * (64-bit values, low words first); `key` is int64[2] on the device, so that
+ * a captured call can be replayed with other numbers.  The same call on the
+ * output's gradient, without residual, is the backward pass: no mask is kept.
+ * pc2d_dropout_next_key copies {state[0], state[1]} to key and adds 1 to
+ * state[1] atomically: every call of it, a replayed one too, gives another
+ * key. */
+int pc2d_dropout(int dtype, const void *input, const void *residual, const int64_t *key, double p, int64_t n,
+                 void *output, void *stream);
+int pc2d_dropout_next_key(int64_t *state, int64_t *key, void *stream);
+
+/* Causal convolution along the length, one filter of `taps` (1 to 8) per
+ * channel.  With line = [initial_state (taps-1 values; NULL: zeros) | the
+ * row's tokens]: pre_t = bias[c] + sum_k weight[c][k] line[t+k]; output = pre,
+ * or pre * sigmoid(pre) with silu; final_state = the last taps-1 values of
+ * line.  weight [channels][taps], bias [channels] (NULL: none): of the
+ * inputs' type or float32 (wdtype).  States: [batch][channels][taps-1] of the
+ * inputs' type.  final_state, grad_final, weightgrad, biasgrad and
+ * initialgrad may be NULL.  pc2d_causal_conv_step takes one token per row
+ * and moves its state on in place: `state` [places][channels][taps-1], row b
+ * uses place slots[b] (int32; NULL: b).  slots[b] = -1 marks a row without
+ * request: its output is 0 and no state changes.  A place outside the array,
+ * or one that an earlier row of the call has too, makes the row's output NaN
+ * and changes no state. */
+int pc2d_causal_conv_forward(int dtype, int wdtype, const void *input, const void *weight, const void *bias,
+                             const void *initial_state, const int *lengths, int batch, int channels, int length,
+                             int taps, int silu, void *output, void *final_state, void *stream);
+size_t pc2d_causal_conv_backward_workspace_size(int batch, int channels, int length, int taps);
+int pc2d_causal_conv_backward(int dtype, int wdtype, const void *grad, const void *grad_final, const void *input,
+                              const void *weight, const void *bias, const void *initial_state, const int *lengths,
+                              int batch, int channels, int length, int taps, int silu, void *inputgrad,
+                              void *weightgrad, void *biasgrad, void *initialgrad, void *workspace,
+                              size_t workspace_bytes, void *stream);
+int pc2d_causal_conv_step(int dtype, int wdtype, const void *input, void *state, const void *weight, const void *bias,
+                          const int *slots, int batch, int places, int channels, int taps, int silu, void *output,
+                          void *stream);
+
+/* State space scan.  Per channel c, with `states` (1 to 128) states n and the
+ * inputs B, C [batch][groups][states][length] of the channel's group (equal
+ * groups of channels/groups channels):
+ *   d_t = delta_t + delta_bias[c]        (softplus of it with delta_softplus)
+ *   h_t[n] = exp(d_t A[c][n]) h_{t-1}[n] + d_t u_t B_t[n]
+ *   output_t = (sum_n C_t[n] h_t[n] + skip[c] u_t) * (z_t sigmoid(z_t) with z)
+ * from h = initial_state (NULL: 0); final_state = h after the last token.
+ * u, delta, z and output [batch][channels][length]; A [channels][states],
+ * skip and delta_bias [channels] (NULL: 0), states [batch][channels][states]:
+ * float32.  `checkpoints` (NULL: none) receives the states that the backward
+ * pass starts its tiles from, pc2d_ssm_scan_checkpoint_size() bytes.  The
+ * backward pass gives the gradients of all inputs (skipgrad, biasgrad,
+ * initialgrad and grad_final may be NULL; zgrad goes with z).
+ * pc2d_ssm_scan_step takes one token per row (u, delta, z [batch][channels],
+ * B, C [batch][groups][states]) and moves its state [places][channels][states]
+ * on in place; slots as for pc2d_causal_conv_step. */
+size_t pc2d_ssm_scan_checkpoint_size(int batch, int channels, int length, int states);
+size_t pc2d_ssm_scan_forward_workspace_size(int batch, int channels, int length, int states, int groups);
+int pc2d_ssm_scan_forward(int dtype, const void *u, const void *delta, const float *A, const void *B, const void *C,
+                          const float *skip, const void *z, const float *delta_bias, const float *initial_state,
+                          const int *lengths, int delta_softplus, int batch, int channels, int length, int states,
+                          int groups, void *output, float *final_state, float *checkpoints, void *workspace,
+                          size_t workspace_bytes, void *stream);
+size_t pc2d_ssm_scan_backward_workspace_size(int batch, int channels, int length, int states, int groups);
+int pc2d_ssm_scan_backward(int dtype, const void *grad, const float *grad_final, const void *u, const void *delta,
+                           const float *A, const void *B, const void *C, const float *skip, const void *z,
+                           const float *delta_bias, const int *lengths, const float *checkpoints, int delta_softplus,
+                           int batch, int channels, int length, int states, int groups, void *ugrad, void *deltagrad,
+                           float *Agrad, void *Bgrad, void *Cgrad, float *skipgrad, void *zgrad, float *biasgrad,
+                           float *initialgrad, void *workspace, size_t workspace_bytes, void *stream);
+int pc2d_ssm_scan_step(int dtype, const void *u, const void *delta, float *state, const float *A, const void *B,
+                       const void *C, const float *skip, const void *z, const float *delta_bias, const int *slots,
+                       int delta_softplus, int batch, int places, int channels, int states, int groups, void *output,
+                       void *stream);
 
 /* Human-readable name of a pc2d_status. */
 const char *pc2d_status_string(int status);

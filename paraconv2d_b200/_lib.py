@@ -26,6 +26,8 @@ PC2D_ERR_CUDA = 4
 PC2D_ERR_TIMEOUT = 5
 PC2D_DTYPE_F32 = 0
 PC2D_DTYPE_F64 = 1
+PC2D_DTYPE_F16 = 2   # F16 and BF16: the sequence operators only
+PC2D_DTYPE_BF16 = 3
 PC2D_ALGO_AUTO = 0
 PC2D_ALGO_SIMT = 1
 PC2D_ALGO_TC = 2
@@ -87,6 +89,18 @@ def cabi() -> ctypes.CDLL:
             "pc2d_backward_sum": ([P, I, P, P, P, P, D] + [I] * 12 + [P, P, P, S, P], I),
             "pc2d_comm_allreduce": ([P, P, P, S, P], I),
             "pc2d_param_step": ([I, P, P, P, I, I] + [D] * 6 + [I, P], I),
+            "pc2d_dropout": ([I, P, P, P, D, L, P, P], I),
+            "pc2d_dropout_next_key": ([P, P, P], I),
+            "pc2d_causal_conv_forward": ([I, I] + [P] * 5 + [I] * 5 + [P] * 3, I),
+            "pc2d_causal_conv_backward_workspace_size": ([I] * 4, S),
+            "pc2d_causal_conv_backward": ([I, I] + [P] * 7 + [I] * 5 + [P] * 5 + [S, P], I),
+            "pc2d_causal_conv_step": ([I, I] + [P] * 5 + [I] * 5 + [P] * 2, I),
+            "pc2d_ssm_scan_checkpoint_size": ([I] * 4, S),
+            "pc2d_ssm_scan_forward_workspace_size": ([I] * 5, S),
+            "pc2d_ssm_scan_forward": ([I] + [P] * 10 + [I] * 6 + [P] * 4 + [S, P], I),
+            "pc2d_ssm_scan_backward_workspace_size": ([I] * 5, S),
+            "pc2d_ssm_scan_backward": ([I] + [P] * 12 + [I] * 6 + [P] * 10 + [S, P], I),
+            "pc2d_ssm_scan_step": ([I] + [P] * 10 + [I] * 6 + [P] * 2, I),
             "pc2d_status_string": ([I], ctypes.c_char_p),
             "pc2d_last_error": ([], ctypes.c_char_p),
             "pc2d_device_status": ([], I),

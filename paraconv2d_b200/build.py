@@ -79,9 +79,9 @@ def build_kernel_lib(force=False, verbose=False, ptxas_verbose=False):
 
 
 def build_op_lib(force=False, verbose=False):
-    src = os.path.join(CSRC, "pc2d_op.cpp")
+    srcs = [os.path.join(CSRC, "pc2d_op.cpp"), os.path.join(CSRC, "pc2d_seq_op.cpp")]
     if (not force and os.path.exists(OP_LIB)
-            and os.path.getmtime(OP_LIB) >= _newest([src, os.path.join(INCLUDE, "paraconv2d.h"), KERNEL_LIB, __file__])):
+            and os.path.getmtime(OP_LIB) >= _newest([*srcs, os.path.join(INCLUDE, "paraconv2d.h"), KERNEL_LIB, __file__])):
         return OP_LIB
     import sysconfig
 
@@ -95,7 +95,7 @@ def build_op_lib(force=False, verbose=False):
           "-isystem", os.path.join(tdir, "include"),
           "-isystem", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
           "-isystem", sysconfig.get_path("include"), "-I" + os.path.join(CUDA_HOME, "include"), "-I" + INCLUDE,
-          src, "-o", tmp,
+          *srcs, "-o", tmp,
           "-L" + PKG, "-l:libpc2d_sm100.so", "-Wl,-rpath,$ORIGIN",
           "-L" + os.path.join(tdir, "lib"), "-Wl,-rpath," + os.path.join(tdir, "lib"),
           "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_cuda",

@@ -1,0 +1,537 @@
+// Short causal convolution along the length of [batch][channels][length], one
+// filter of K <= 8 taps per channel:
+//
+//   line  = [ state (K-1 values) | x_0 ... x_{n-1} ]       n: the row's length
+//   pre_t = bias + sum_k w_k line[t + k]                   out_t = act(pre_t)
+//   final = line[n ... n+K-2]
+//
+// with act the identity or silu(v) = v sigmoid(v).  Backward, with
+// dpre = dout act'(pre):
+//
+//   dline[s] = sum_k w_k dpre[s - k]  (+ dfinal[s - n] for s >= n)
+//   dw_k = sum dpre_t line[t + k]     dbias = sum dpre_t
+//
+// All of it is a few operations per element: the kernels stream.  A warp takes
+// a run of one row, and a lane eight elements at a time, cut at the
+// 8-element boundaries of the whole array rather than of the row: every load
+// and store inside a row is then a 16-byte vector whatever the length is, and
+// only the (at most two) vectors that a row shares with its neighbours go
+// element by element.
+#include <algorithm>
+#include <initializer_list>
+#include <type_traits>
+
+#include "pc2d_seq.cuh"
+#include "pc2d_tc.cuh"
+
+namespace pc2d {
+namespace {
+
+constexpr int kConvThreads = 256;
+constexpr int kMaxTaps = 8;
+
+struct ConvArgs {
+  const void *x, *weight, *bias, *init;
+  const int *lengths;
+  int wdtype;
+  int batch, channels, length, silu;
+  int64_t rows;   // batch * channels
+  int nseg;       // warps per row
+  int seg;        // 8-element vectors per warp
+  // forward
+  void *out, *final_state;
+  // backward
+  const void *grad, *grad_final;
+  void *dx, *dinit;
+  float *part;    // [batch * nseg][K + 1][channels]
+};
+
+__device__ __forceinline__ float load_param(const void *p, int dtype, int64_t i) {
+  if (dtype == PC2D_DTYPE_F32) return static_cast<const float *>(p)[i];
+  if (dtype == PC2D_DTYPE_F16) return __half2float(static_cast<const __half *>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+__device__ __forceinline__ void store_param(void *p, int dtype, int64_t i, float v) {
+  if (dtype == PC2D_DTYPE_F32) static_cast<float *>(p)[i] = v;
+  else if (dtype == PC2D_DTYPE_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// Eight elements t0 .. t0+7 of a row: zeros outside [0, n), the kept state's
+// values (init, K-1 of them, or zeros) before 0 if kState.
+template <typename T, int K, bool kState>
+__device__ __forceinline__ void load8(const T *row, int t0, int n, const T *init, float *v) {
+  if (t0 >= 0 && t0 + 8 <= n) {
+    Pack<T, 8> p;
+    p.load(row + t0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = p.f(i);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int t = t0 + i;
+    v[i] = 0.f;
+    if (t >= 0 && t < n) v[i] = to_f(row[t]);
+    else if (kState && init && t < 0 && t >= -(K - 1)) v[i] = to_f(init[t + K - 1]);
+  }
+}
+
+// Element j (0 .. n+K-2) of a row's line.
+template <typename T, int K>
+__device__ __forceinline__ float line_at(const T *row, const T *init, int j) {
+  const int t = j - (K - 1);
+  if (t >= 0) return to_f(row[t]);
+  return init ? to_f(init[j]) : 0.f;
+}
+
+struct RowPlace {
+  int64_t row;
+  int seg, d, n;
+  int64_t base;   // first element of the row in the array
+  int e0;         // t of the first element of the row's vector 0: 0 or below
+  int nvec;       // vectors that hold elements of the row
+};
+
+__device__ __forceinline__ bool place_of(const ConvArgs &a, RowPlace *p) {
+  const int64_t w = ((int64_t)blockIdx.x * kConvThreads + threadIdx.x) >> 5;
+  p->row = w / a.nseg;
+  if (p->row >= a.rows) return false;
+  p->seg = (int)(w - p->row * a.nseg);
+  const int b = (int)(p->row / a.channels);
+  p->d = (int)(p->row - (int64_t)b * a.channels);
+  p->n = a.length;
+  if (a.lengths) p->n = min(max(a.lengths[b], 0), a.length);
+  p->base = p->row * a.length;
+  const int over = (int)(p->base & 7);
+  p->e0 = -over;
+  p->nvec = (int)(((int64_t)a.length + over + 7) >> 3);
+  return true;
+}
+
+template <typename T, int K>
+__global__ void __launch_bounds__(kConvThreads) conv_forward_kernel(ConvArgs a) {
+  RowPlace p;
+  if (!place_of(a, &p)) return;
+  const int lane = threadIdx.x & 31;
+  const T *row = static_cast<const T *>(a.x) + p.base;
+  T *out = static_cast<T *>(a.out) + p.base;
+  const T *init = a.init ? static_cast<const T *>(a.init) + p.row * (K - 1) : nullptr;
+  float w[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) w[k] = load_param(a.weight, a.wdtype, (int64_t)p.d * K + k);
+  const float bias = a.bias ? load_param(a.bias, a.wdtype, p.d) : 0.f;
+  const int v1 = min(p.nvec, (p.seg + 1) * a.seg);
+  for (int v = p.seg * a.seg + lane; v < v1; v += 32) {
+    const int t0 = p.e0 + v * 8;
+    float x[16];
+    if (K > 1) load8<T, K, true>(row, t0 - 8, p.n, init, x);
+    load8<T, K, true>(row, t0, p.n, init, x + 8);
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float s = bias;
+#pragma unroll
+      for (int k = 0; k < K; ++k) s = fmaf(w[k], x[8 + i - (K - 1) + k], s);
+      y[i] = a.silu ? s * sigmoid_f(s) : s;
+    }
+    if (t0 >= 0 && t0 + 8 <= p.n) {
+      Pack<T, 8> o;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o.v[i] = from_f<T>(y[i]);
+      o.store(out + t0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (t0 + i >= 0 && t0 + i < a.length) out[t0 + i] = t0 + i < p.n ? from_f<T>(y[i]) : from_f<T>(0.f);
+    }
+  }
+  if (a.final_state && p.seg == 0 && lane < K - 1)
+    static_cast<T *>(a.final_state)[p.row * (K - 1) + lane] = from_f<T>(line_at<T, K>(row, init, p.n + lane));
+}
+
+// dpre of the eight elements from t0 on (zeros outside [0, n)) and the 16
+// values of the line that their windows cover.
+template <typename T, int K>
+__device__ __forceinline__ void dpre8(const ConvArgs &a, const T *row, const T *grad, const T *init, int t0, int n,
+                                      const float *w, float bias, float *x, float *dp) {
+  if (K > 1) load8<T, K, true>(row, t0 - 8, n, init, x);
+  load8<T, K, true>(row, t0, n, init, x + 8);
+  load8<T, K, false>(grad, t0, n, nullptr, dp);
+  if (!a.silu) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float s = bias;
+#pragma unroll
+    for (int k = 0; k < K; ++k) s = fmaf(w[k], x[8 + i - (K - 1) + k], s);
+    const float e = sigmoid_f(s);
+    const float slope = e * fmaf(s, 1.f - e, 1.f);
+    // an element outside the row stays 0 whatever its window gives
+    dp[i] = t0 + i >= 0 && t0 + i < n ? dp[i] * slope : 0.f;
+  }
+}
+
+// A warp goes through its run from the end to the beginning: the K-1 values of
+// dpre behind a lane's eight come from the next lane, and for lane 31 from
+// lane 0 of the 32 vectors done before (for the first ones from a computation
+// of the vector behind the run).
+template <typename T, int K>
+__global__ void __launch_bounds__(kConvThreads) conv_backward_kernel(ConvArgs a) {
+  RowPlace p;
+  if (!place_of(a, &p)) return;
+  const int lane = threadIdx.x & 31;
+  const T *row = static_cast<const T *>(a.x) + p.base;
+  const T *grad = static_cast<const T *>(a.grad) + p.base;
+  const T *init = a.init ? static_cast<const T *>(a.init) + p.row * (K - 1) : nullptr;
+  const T *dfinal = a.grad_final ? static_cast<const T *>(a.grad_final) + p.row * (K - 1) : nullptr;
+  T *dx = static_cast<T *>(a.dx) + p.base;
+  float w[K], dw[K], db = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    w[k] = load_param(a.weight, a.wdtype, (int64_t)p.d * K + k);
+    dw[k] = 0.f;
+  }
+  const float bias = a.bias ? load_param(a.bias, a.wdtype, p.d) : 0.f;
+  const int va = p.seg * a.seg, vb = min(p.nvec, va + a.seg);
+  float carry[K > 1 ? K - 1 : 1];  // dpre of the first elements of the vector behind
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) carry[k] = 0.f;
+  if (K > 1 && va < vb && vb < p.nvec) {
+    float x[16], dp[8];
+    dpre8<T, K>(a, row, grad, init, p.e0 + vb * 8, p.n, w, bias, x, dp);
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) carry[k] = dp[k];
+  }
+  for (int v0 = va + ((vb - va - 1) >> 5) * 32; v0 >= va && va < vb; v0 -= 32) {
+    const int v = v0 + lane;
+    const int t0 = p.e0 + v * 8;
+    float x[16], dp[8 + K];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dp[i] = 0.f;
+    if (v < vb) dpre8<T, K>(a, row, grad, init, t0, p.n, w, bias, x, dp);
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+      // the last vector of the run may sit in any lane: lanes behind it hold
+      // zeros, so it takes the carry itself
+      const float next = __shfl_down_sync(0xffffffffu, dp[k], 1);
+      const float first = __shfl_sync(0xffffffffu, dp[k], 0);
+      dp[8 + k] = lane == 31 || v == vb - 1 ? carry[k] : next;
+      carry[k] = first;
+    }
+    if (v < vb) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        db += dp[i];
+#pragma unroll
+        for (int k = 0; k < K; ++k) dw[k] = fmaf(dp[i], x[8 + i - (K - 1) + k], dw[k]);
+      }
+      float g[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        g[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) g[i] = fmaf(w[K - 1 - k], dp[i + k], g[i]);
+        const int j = t0 + i + (K - 1) - p.n;
+        if (K > 1 && dfinal && j >= 0 && t0 + i >= 0 && t0 + i < p.n) g[i] += to_f(dfinal[j]);
+      }
+      if (t0 >= 0 && t0 + 8 <= a.length) {
+        Pack<T, 8> o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o.v[i] = from_f<T>(t0 + i < p.n ? g[i] : 0.f);
+        o.store(dx + t0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (t0 + i >= 0 && t0 + i < a.length) dx[t0 + i] = from_f<T>(t0 + i < p.n ? g[i] : 0.f);
+      }
+    }
+  }
+  // the warp's share of the parameter gradients, in a fixed order
+#pragma unroll
+  for (int k = 0; k <= K; ++k) {
+    float s = k < K ? dw[k < K ? k : 0] : db;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const int64_t b = p.row / a.channels;
+    if (lane == 0) a.part[((b * a.nseg + p.seg) * (K + 1) + k) * a.channels + p.d] = s;
+  }
+  if (K > 1 && a.dinit && p.seg == 0) {
+    // dline[s], s < K-1: lane j computes dpre[j] from its own window
+    float dpj = 0.f;
+    if (lane < K - 1 && lane < p.n) {
+      dpj = to_f(grad[lane]);
+      if (a.silu) {
+        float s = bias;
+#pragma unroll
+        for (int k = 0; k < K; ++k) s = fmaf(w[k], line_at<T, K>(row, init, lane + k), s);
+        const float e = sigmoid_f(s);
+        dpj *= e * fmaf(s, 1.f - e, 1.f);
+      }
+    }
+    float g = 0.f;
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+      const float other = __shfl_sync(0xffffffffu, dpj, (lane - k) & 31);
+      if (lane >= k) g = fmaf(w[k], other, g);
+    }
+    if (lane < K - 1) {
+      if (dfinal && lane >= p.n) g += to_f(dfinal[lane - p.n]);
+      static_cast<T *>(a.dinit)[p.row * (K - 1) + lane] = from_f<T>(g);
+    }
+  }
+}
+
+// Sums the warps' shares [groups][K+1][channels] over the groups, in 64 bits
+// and in a fixed order: 8 lanes of threads per (k, channel), then those 8.
+__global__ void __launch_bounds__(256) conv_param_kernel(const float *__restrict__ part, int groups, int taps,
+                                                        int channels, int wdtype, void *dweight, void *dbias) {
+  __shared__ double sums[8][32];
+  const int d = blockIdx.x * 32 + threadIdx.x, k = blockIdx.y;
+  double s = 0.0;
+  if (d < channels) {
+#pragma unroll 4
+    for (int g = threadIdx.y; g < groups; g += 8) s += part[((int64_t)g * (taps + 1) + k) * channels + d];
+  }
+  sums[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y != 0 || d >= channels) return;
+  for (int i = 1; i < 8; ++i) s += sums[i][threadIdx.x];
+  if (k < taps) {
+    if (dweight) store_param(dweight, wdtype, (int64_t)d * taps + k, (float)s);
+  } else if (dbias) {
+    store_param(dbias, wdtype, d, (float)s);
+  }
+}
+
+struct ConvStepArgs {
+  const void *x, *weight, *bias;
+  const int *slots;
+  void *state, *out;
+  int wdtype, batch, places, channels, silu;
+};
+
+// One token: thread = channel.  Reads and writes the K-1 kept inputs once.
+template <typename T, int K>
+__global__ void __launch_bounds__(kConvThreads) conv_step_kernel(ConvStepArgs a) {
+  const int nblk = (a.channels + kConvThreads - 1) / kConvThreads;
+  const int b = blockIdx.x / nblk;
+  bool bad;
+  const int place = step_place(a.slots, b, a.places, &bad);
+  const int d = (blockIdx.x - b * nblk) * kConvThreads + threadIdx.x;
+  if (d >= a.channels) return;
+  T *out = static_cast<T *>(a.out) + (int64_t)b * a.channels + d;
+  if (place < 0) {
+    *out = from_f<T>(bad ? __int_as_float(0x7fffffff) : 0.f);
+    return;
+  }
+  T *kept = static_cast<T *>(a.state) + ((int64_t)place * a.channels + d) * (K - 1);
+  T line[K];
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) line[k] = kept[k];
+  line[K - 1] = static_cast<const T *>(a.x)[(int64_t)b * a.channels + d];
+  float s = a.bias ? load_param(a.bias, a.wdtype, d) : 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) s = fmaf(load_param(a.weight, a.wdtype, (int64_t)d * K + k), to_f(line[k]), s);
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) kept[k] = line[k + 1];
+  *out = from_f<T>(a.silu ? s * sigmoid_f(s) : s);
+}
+
+enum ConvWhat { kConvForward, kConvBackward };
+
+// Vectors per warp: long runs amortise a warp's set-up (parameters, the vector
+// behind the run), short ones fill the GPU when there are few rows.
+void conv_split(const ConvArgs &a, int *nseg, int *seg) {
+  const int nvec = (int)(((int64_t)a.length + 7 + 7) >> 3);
+  int iters = 8;
+  while (iters > 1 && a.rows * ((nvec + 32 * iters - 1) / (32 * iters)) < (int64_t)device_sm_count() * 32) iters /= 2;
+  *seg = 32 * iters;
+  *nseg = std::max(1, (nvec + *seg - 1) / *seg);
+}
+
+template <typename T, int K>
+int launch_conv(ConvWhat what, const ConvArgs &a, cudaStream_t stream) {
+  const int64_t blocks = (a.rows * a.nseg * 32 + kConvThreads - 1) / kConvThreads;
+  if (what == kConvForward) conv_forward_kernel<T, K><<<(unsigned)blocks, kConvThreads, 0, stream>>>(a);
+  else conv_backward_kernel<T, K><<<(unsigned)blocks, kConvThreads, 0, stream>>>(a);
+  PC2D_LAUNCH_CHECK(what == kConvForward ? "conv_forward_kernel" : "conv_backward_kernel");
+  return PC2D_OK;
+}
+
+template <typename T, int K>
+int launch_conv_step(const ConvStepArgs &a, cudaStream_t stream) {
+  const int nblk = (a.channels + kConvThreads - 1) / kConvThreads;
+  conv_step_kernel<T, K><<<(unsigned)(nblk * a.batch), kConvThreads, 0, stream>>>(a);
+  PC2D_LAUNCH_CHECK("conv_step_kernel");
+  return PC2D_OK;
+}
+
+// f.template operator()<T, K>() for the call's type and taps
+template <typename F>
+int by_type_and_taps(int dtype, int taps, F &&f) {
+#define PC2D_TAPS(T)                                            \
+  switch (taps) {                                               \
+    case 1: return f(T{}, std::integral_constant<int, 1>{});    \
+    case 2: return f(T{}, std::integral_constant<int, 2>{});    \
+    case 3: return f(T{}, std::integral_constant<int, 3>{});    \
+    case 4: return f(T{}, std::integral_constant<int, 4>{});    \
+    case 5: return f(T{}, std::integral_constant<int, 5>{});    \
+    case 6: return f(T{}, std::integral_constant<int, 6>{});    \
+    case 7: return f(T{}, std::integral_constant<int, 7>{});    \
+    default: return f(T{}, std::integral_constant<int, 8>{});   \
+  }
+  if (dtype == PC2D_DTYPE_F32) { PC2D_TAPS(float) }
+  if (dtype == PC2D_DTYPE_F16) { PC2D_TAPS(__half) }
+  PC2D_TAPS(__nv_bfloat16)
+#undef PC2D_TAPS
+}
+
+int check_conv(const char *what, int dtype, int wdtype, int batch, int channels, int length, int taps) {
+  if (!seq_dtype(dtype)) {
+    set_last_error("%s: unsupported dtype %d (float32, float16 and bfloat16)", what, dtype);
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if (wdtype != dtype && wdtype != PC2D_DTYPE_F32) {
+    set_last_error("%s: weights of dtype %d beside inputs of dtype %d (the inputs' type or float32)", what, wdtype,
+                   dtype);
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if (batch < 0 || channels < 0 || length < 0 || taps < 1) {
+    set_last_error("%s: invalid batch %d, channels %d, length %d or taps %d", what, batch, channels, length, taps);
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if (taps > kMaxTaps) {
+    set_last_error("%s: %d taps (at most %d)", what, taps, kMaxTaps);
+    return PC2D_ERR_UNSUPPORTED;
+  }
+  // the vectors of a row are counted in 32 bits, the warps of a launch too
+  if (length > 0x7ffffff0 - 16 || (int64_t)batch * channels > (int64_t)1 << 30 ||
+      (int64_t)batch * channels * (length / 256 + 2) > (int64_t)1 << 33) {
+    set_last_error("%s: problem too large", what);
+    return PC2D_ERR_UNSUPPORTED;
+  }
+  return PC2D_OK;
+}
+
+int check_aligned(const char *what, std::initializer_list<const void *> ptrs) {
+  for (const void *p : ptrs)
+    if (p && !aligned16(p)) {
+      set_last_error("%s: the activations and their gradients must be 16-byte aligned", what);
+      return PC2D_ERR_INVALID_ARGUMENT;
+    }
+  return PC2D_OK;
+}
+
+}  // namespace
+}  // namespace pc2d
+
+using namespace pc2d;
+
+extern "C" int pc2d_causal_conv_forward(int dtype, int wdtype, const void *input, const void *weight, const void *bias,
+                                        const void *initial_state, const int *lengths, int batch, int channels,
+                                        int length, int taps, int silu, void *output, void *final_state,
+                                        void *stream) {
+  NvtxRange range("pc2d_causal_conv_forward");
+  int st = check_conv("pc2d_causal_conv_forward", dtype, wdtype, batch, channels, length, taps);
+  if (st != PC2D_OK) return st;
+  if ((st = pending_device_error()) != PC2D_OK) return st;
+  ConvArgs a{};
+  a.rows = (int64_t)batch * channels;
+  if (a.rows == 0 || (length == 0 && (!final_state || taps == 1))) return PC2D_OK;
+  if (!weight || (length > 0 && (!input || !output))) {
+    set_last_error("pc2d_causal_conv_forward: null pointer (input, weight or output)");
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if ((st = check_aligned("pc2d_causal_conv_forward", {input, output})) != PC2D_OK) return st;
+  a.x = input; a.weight = weight; a.bias = bias; a.init = taps > 1 ? initial_state : nullptr;
+  a.lengths = lengths; a.wdtype = wdtype;
+  a.batch = batch; a.channels = channels; a.length = length; a.silu = silu != 0;
+  a.out = output; a.final_state = final_state;
+  conv_split(a, &a.nseg, &a.seg);
+  return by_type_and_taps(dtype, taps, [&](auto t, auto k) {
+    return launch_conv<decltype(t), decltype(k)::value>(kConvForward, a, reinterpret_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" size_t pc2d_causal_conv_backward_workspace_size(int batch, int channels, int length, int taps) {
+  if (check_conv("pc2d_causal_conv_backward_workspace_size", PC2D_DTYPE_F32, PC2D_DTYPE_F32, batch, channels, length,
+                 taps) != PC2D_OK)
+    return 0;
+  ConvArgs a{};
+  a.rows = (int64_t)batch * channels;
+  a.length = length;
+  int nseg, seg;
+  conv_split(a, &nseg, &seg);
+  return (size_t)a.rows * nseg * (taps + 1) * sizeof(float);
+}
+
+extern "C" int pc2d_causal_conv_backward(int dtype, int wdtype, const void *grad, const void *grad_final,
+                                         const void *input, const void *weight, const void *bias,
+                                         const void *initial_state, const int *lengths, int batch, int channels,
+                                         int length, int taps, int silu, void *inputgrad, void *weightgrad,
+                                         void *biasgrad, void *initialgrad, void *workspace, size_t workspace_bytes,
+                                         void *stream) {
+  NvtxRange range("pc2d_causal_conv_backward");
+  int st = check_conv("pc2d_causal_conv_backward", dtype, wdtype, batch, channels, length, taps);
+  if (st != PC2D_OK) return st;
+  if ((st = pending_device_error()) != PC2D_OK) return st;
+  if (channels == 0) return PC2D_OK;
+  ConvArgs a{};
+  a.rows = (int64_t)batch * channels;
+  if (!weight || (a.rows > 0 && length > 0 && (!grad || !input || !inputgrad))) {
+    set_last_error("pc2d_causal_conv_backward: null pointer (grad, input, weight or inputgrad)");
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if ((st = check_aligned("pc2d_causal_conv_backward", {grad, input, inputgrad})) != PC2D_OK) return st;
+  const size_t need = pc2d_causal_conv_backward_workspace_size(batch, channels, length, taps);
+  if (workspace_bytes < need || (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255)))) {
+    set_last_error("pc2d_causal_conv_backward: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", need,
+                   workspace_bytes);
+    return PC2D_ERR_WORKSPACE;
+  }
+  a.x = input; a.weight = weight; a.bias = bias; a.init = taps > 1 ? initial_state : nullptr;
+  a.lengths = lengths; a.wdtype = wdtype;
+  a.batch = batch; a.channels = channels; a.length = length; a.silu = silu != 0;
+  a.grad = grad; a.grad_final = taps > 1 ? grad_final : nullptr;
+  a.dx = inputgrad; a.dinit = taps > 1 ? initialgrad : nullptr;
+  a.part = static_cast<float *>(workspace);
+  conv_split(a, &a.nseg, &a.seg);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (a.rows > 0) {
+    st = by_type_and_taps(dtype, taps, [&](auto t, auto k) {
+      return launch_conv<decltype(t), decltype(k)::value>(kConvBackward, a, s);
+    });
+    if (st != PC2D_OK) return st;
+  }
+  if (!weightgrad && !biasgrad) return PC2D_OK;
+  conv_param_kernel<<<dim3((channels + 31) / 32, taps + 1), dim3(32, 8), 0, s>>>(a.part, batch * a.nseg, taps,
+                                                                               channels, wdtype, weightgrad, biasgrad);
+  PC2D_LAUNCH_CHECK("conv_param_kernel");
+  return PC2D_OK;
+}
+
+extern "C" int pc2d_causal_conv_step(int dtype, int wdtype, const void *input, void *state, const void *weight,
+                                     const void *bias, const int *slots, int batch, int places, int channels, int taps,
+                                     int silu, void *output, void *stream) {
+  NvtxRange range("pc2d_causal_conv_step");
+  int st = check_conv("pc2d_causal_conv_step", dtype, wdtype, batch, channels, 1, taps);
+  if (st != PC2D_OK) return st;
+  if (places < 0 || (!slots && batch > places && taps > 1)) {
+    set_last_error("pc2d_causal_conv_step: %d rows of a batch without slots, but %d states", batch, places);
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if ((st = pending_device_error()) != PC2D_OK) return st;
+  if (batch == 0 || channels == 0) return PC2D_OK;
+  if (!input || !weight || !output || (taps > 1 && !state && places > 0)) {
+    set_last_error("pc2d_causal_conv_step: null pointer (input, state, weight or output)");
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  ConvStepArgs a{};
+  a.x = input; a.weight = weight; a.bias = bias; a.slots = slots; a.state = state; a.out = output;
+  a.wdtype = wdtype; a.batch = batch; a.places = places; a.channels = channels; a.silu = silu != 0;
+  return by_type_and_taps(dtype, taps, [&](auto t, auto k) {
+    return launch_conv_step<decltype(t), decltype(k)::value>(a, reinterpret_cast<cudaStream_t>(stream));
+  });
+}

@@ -1,0 +1,178 @@
+// Dropout whose mask is never stored: both directions compute it again from a
+// counter-based generator, Philox4x32-10 (Salmon, Moraes, Dror and Shaw,
+// "Parallel random numbers: as easy as 1, 2, 3", 2011).
+//
+// Element i of the array takes 16 bits: the counter (i / 8, offset) under the
+// key `seed` gives four 32-bit words, which are eight halves, and element i
+// takes half i % 8 (the low half of word 0 first).  It is kept when its half
+// is at least thr = round(65536 p), and then multiplied by 65536 / (65536 -
+// thr), the inverse of the probability with which that happens, so that the
+// expectation is exact for the rounded p.  A dropped element is 0 whatever it
+// held (NaN too).  The mask depends on seed, offset and i alone: not on the
+// type, the launch or the device.
+//
+// The kernel streams: 4 bytes an element at 16 bits (6 with a residual).
+#include <math.h>
+
+#include <algorithm>
+
+#include "pc2d_seq.cuh"
+#include "pc2d_tc.cuh"
+
+namespace pc2d {
+namespace {
+
+constexpr int kDropThreads = 256;
+
+struct Words {
+  unsigned w[4];
+};
+
+__device__ __forceinline__ Words philox(uint64_t block, uint64_t offset, uint64_t seed) {
+  unsigned c0 = (unsigned)block, c1 = (unsigned)(block >> 32), c2 = (unsigned)offset, c3 = (unsigned)(offset >> 32);
+  unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t p = (uint64_t)0xD2511F53u * c0, q = (uint64_t)0xCD9E8D57u * c2;
+    c0 = (unsigned)(q >> 32) ^ c1 ^ k0;
+    c1 = (unsigned)q;
+    c2 = (unsigned)(p >> 32) ^ c3 ^ k1;
+    c3 = (unsigned)p;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return Words{{c0, c1, c2, c3}};
+}
+
+__device__ __forceinline__ double to_acc(double v) { return v; }
+template <typename T>
+__device__ __forceinline__ float to_acc(T v) { return to_f(v); }
+template <typename T, typename A>
+__device__ __forceinline__ T from_acc(A v) {
+  if constexpr (sizeof(T) == 8) return v;
+  else return from_f<T>(v);
+}
+
+template <typename T>
+struct Acc {
+  using type = float;
+};
+template <>
+struct Acc<double> {
+  using type = double;
+};
+
+template <typename T, bool kResidual>
+__global__ void __launch_bounds__(kDropThreads) dropout_kernel(const T *__restrict__ x, const T *__restrict__ res,
+                                                              const int64_t *__restrict__ key, unsigned thr,
+                                                              typename Acc<T>::type scale, int64_t n, bool vec,
+                                                              T *__restrict__ out) {
+  using A = typename Acc<T>::type;
+  const uint64_t seed = (uint64_t)key[0], offset = (uint64_t)key[1];
+  const int64_t stride = (int64_t)gridDim.x * kDropThreads;
+  const int64_t groups = (n + 7) / 8;
+  for (int64_t g = (int64_t)blockIdx.x * kDropThreads + threadIdx.x; g < groups; g += stride) {
+    Pack<T, 8> a, r, o;
+    const bool whole = vec && g * 8 + 8 <= n;
+    if (whole) {
+      a.load(x + g * 8);
+      if (kResidual) r.load(res + g * 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool in = g * 8 + i < n;
+        a.v[i] = in ? x[g * 8 + i] : T(0.f);
+        if (kResidual) r.v[i] = in ? res[g * 8 + i] : T(0.f);
+      }
+    }
+    const Words w = philox((uint64_t)g, offset, seed);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const unsigned half = i & 1 ? w.w[i / 2] >> 16 : w.w[i / 2] & 0xFFFFu;
+      A v = half >= thr ? to_acc(a.v[i]) * scale : A(0);
+      if (kResidual) v += to_acc(r.v[i]);
+      o.v[i] = from_acc<T>(v);
+    }
+    if (whole) {
+      o.store(out + g * 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (g * 8 + i < n) out[g * 8 + i] = o.v[i];
+    }
+  }
+}
+
+__global__ void dropout_next_key_kernel(int64_t *state, int64_t *key) {
+  key[0] = state[0];
+  key[1] = (int64_t)atomicAdd(reinterpret_cast<unsigned long long *>(state + 1), 1ull);
+}
+
+template <typename T>
+int launch_dropout(const void *x, const void *res, const int64_t *key, unsigned thr, double scale, int64_t n,
+                   void *out, cudaStream_t stream) {
+  const bool vec = aligned16(x) && aligned16(out) && (!res || aligned16(res));
+  const int64_t blocks = ((n + 7) / 8 + kDropThreads - 1) / kDropThreads;
+  const int grid = (int)std::min<int64_t>(blocks, (int64_t)device_sm_count() * 8);
+  using A = typename Acc<T>::type;
+  if (res)
+    dropout_kernel<T, true><<<grid, kDropThreads, 0, stream>>>((const T *)x, (const T *)res, key, thr, (A)scale, n,
+                                                               vec, (T *)out);
+  else
+    dropout_kernel<T, false><<<grid, kDropThreads, 0, stream>>>((const T *)x, nullptr, key, thr, (A)scale, n, vec,
+                                                                (T *)out);
+  PC2D_LAUNCH_CHECK("dropout_kernel");
+  return PC2D_OK;
+}
+
+}  // namespace
+}  // namespace pc2d
+
+using namespace pc2d;
+
+extern "C" int pc2d_dropout(int dtype, const void *input, const void *residual, const int64_t *key, double p,
+                            int64_t n, void *output, void *stream) {
+  NvtxRange range("pc2d_dropout");
+  if (!seq_dtype(dtype) && dtype != PC2D_DTYPE_F64) {
+    set_last_error("pc2d_dropout: unsupported dtype %d", dtype);
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if (!(p >= 0.0 && p <= 1.0)) {
+    set_last_error("pc2d_dropout: p must be in [0, 1], got %g", p);
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if (n < 0) {
+    set_last_error("pc2d_dropout: invalid element count %lld", (long long)n);
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  const int st = pending_device_error();
+  if (st != PC2D_OK) return st;
+  if (n == 0) return PC2D_OK;
+  if (!input || !key || !output) {
+    set_last_error("pc2d_dropout: null pointer (input, key or output)");
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  // round to even at a half, as Python's round() does
+  const unsigned thr = (unsigned)nearbyint(p * 65536.0);
+  const double scale = thr < 65536u ? 65536.0 / (65536.0 - thr) : 0.0;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case PC2D_DTYPE_F32: return launch_dropout<float>(input, residual, key, thr, scale, n, output, s);
+    case PC2D_DTYPE_F64: return launch_dropout<double>(input, residual, key, thr, scale, n, output, s);
+    case PC2D_DTYPE_F16: return launch_dropout<__half>(input, residual, key, thr, scale, n, output, s);
+    default: return launch_dropout<__nv_bfloat16>(input, residual, key, thr, scale, n, output, s);
+  }
+}
+
+extern "C" int pc2d_dropout_next_key(int64_t *state, int64_t *key, void *stream) {
+  NvtxRange range("pc2d_dropout_next_key");
+  if (!state || !key) {
+    set_last_error("pc2d_dropout_next_key: null pointer");
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  const int st = pending_device_error();
+  if (st != PC2D_OK) return st;
+  dropout_next_key_kernel<<<1, 1, 0, reinterpret_cast<cudaStream_t>(stream)>>>(state, key);
+  PC2D_LAUNCH_CHECK("dropout_next_key_kernel");
+  return PC2D_OK;
+}

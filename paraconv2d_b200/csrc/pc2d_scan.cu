@@ -1,0 +1,1087 @@
+// State space scan over [batch][channels][length], with N states per channel
+// and inputs B, C shared by the channels of a group:
+//
+//   D_t = softplus(delta_t + bias)         (or delta_t + bias)
+//   h_t[n] = exp(D_t A[n]) h_{t-1}[n] + D_t u_t B_t[n]
+//   y_t = sum_n C_t[n] h_t[n] + skip u_t           out_t = y_t silu(z_t)
+//
+// Backward, with dy = dout silu(z) and a_t = exp(D_t A):
+//
+//   dh_t = C_t dy_t + r_t       r_{t-1} = a_t dh_t  (r behind the last token: dfinal)
+//   dC_t[n] = sum_channels dy_t h_t[n]      dB_t[n] = sum_channels dh_t[n] D_t u_t
+//   through_t = sum_n dh_t[n] B_t[n]        m_t[n] = r_{t-1}[n] h_{t-1}[n]
+//   du_t = D_t through_t + skip dy_t        dD_t = u_t through_t + sum_n A[n] m_t[n]
+//   dA[n] = sum_t D_t m_t[n]     dskip = sum dy_t u_t     dz_t = dout_t y_t silu'(z_t)
+//   ddelta_t = dD_t softplus'(delta_t + bias)             dbias = sum ddelta_t
+//
+// P lanes share a channel and hold four of its states each (P the power of
+// two that covers N); a block of 128 threads has 128 / P channels of one
+// group and goes through the length in tiles.  Per tile the inputs come in by
+// vectors along the length, D_t, D_t u_t (and dy_t) go to shared memory as
+// 32-bit rows of the warp that uses them, B and C, which the whole block
+// reads, as [t][n] so that a lane takes its four states in one 16-byte read.
+// The recurrence stays in registers; sums over the states are made four (or
+// eight) tokens at a time, each exchange halving what a lane still holds.
+//
+// The bound is the arithmetic: an exp per channel, state and token (two in
+// the backward pass) at 16 a clock and SM, against 8 to 14 bytes of traffic
+// per channel and token.
+//
+// Few rows leave SMs empty.  Then the length is cut into segments that run at
+// the same time, after a first pass that gives each segment's end state from
+// zero and its sum of D_t: as the decay over a segment is exp(A sum D_t), a
+// segment gets its true state from those of the segments before it.  The
+// backward pass does the same with r, from the end.
+//
+// For the backward pass the forward one keeps the state at the start of each
+// of that pass's tiles; within a tile the states are computed again.
+#include <algorithm>
+#include <initializer_list>
+#include <type_traits>
+
+#include "pc2d_seq.cuh"
+#include "pc2d_tc.cuh"
+
+namespace pc2d {
+namespace {
+
+constexpr int kScanThreads = 128;
+constexpr int kS = 4;  // states per lane
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Tile lengths by the lanes per channel: shared memory and the elements a
+// thread loads per tile bound them.  A forward tile holds whole backward ones.
+template <int P>
+struct ScanTile {
+  static constexpr int kFwd = P == 1 ? 16 : P == 2 ? 32 : P <= 8 ? 64 : 32;
+  static constexpr int kBwd = P <= 2 ? 16 : P <= 8 ? 32 : 16;
+};
+inline int lanes_of(int states) {
+  int p = 1;
+  while (p * kS < states) p *= 2;
+  return p;
+}
+inline int bwd_tile_of(int states) {
+  const int p = lanes_of(states);
+  return p <= 2 ? 16 : p <= 8 ? 32 : 16;
+}
+
+struct ScanArgs {
+  const void *u, *delta, *z, *B, *C;
+  const float *A, *skip, *bias, *init;
+  const int *lengths;
+  int batch, channels, length, states, groups, per_group, softplus;
+  int nblk;            // blocks of channels per group
+  int nseg, seg_len;   // segments of the length, in tokens
+  void *out;
+  float *final_state;  // [batch][channels][states]
+  float *ckpt;         // [batch][tiles][channels][states], state at each backward tile's start
+  float *seg_state;    // [batch][nseg][channels][states]
+  float *seg_sum;      // [batch][nseg][channels]
+  // backward
+  const void *grad;
+  const float *grad_final;
+  void *du, *ddelta, *dz;
+  float *dinit;
+  float *part_bc;      // [batch][groups][nblk][2 states][length]: dB, then dC
+  float *part_par;     // [batch * nseg][channels * (states + 2)]: dA, dskip, dbias
+};
+
+__device__ __forceinline__ float exp2_f(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+__device__ __forceinline__ float softplus_f(float v) { return v > 20.f ? v : log1pf(expf(v)); }
+
+// Sums of v0..v3 over the P lanes of a channel.  P >= 4: lane p ends with
+// that of v[p % 4]; P = 2: with those of v[p] and v[p + 2]; P = 1: all four.
+template <int P>
+struct Sum4 {
+  static constexpr int kLeft = P >= 4 ? 1 : 4 / P;
+  float r[kLeft];
+  __device__ __forceinline__ Sum4(float v0, float v1, float v2, float v3, int p) {
+    if constexpr (P == 1) {
+      r[0] = v0;
+      r[1] = v1;
+      r[2] = v2;
+      r[3] = v3;
+    } else if constexpr (P == 2) {
+      const bool odd = p & 1;
+      r[0] = (odd ? v1 : v0) + __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 1);
+      r[1] = (odd ? v3 : v2) + __shfl_xor_sync(0xffffffffu, odd ? v2 : v3, 1);
+    } else {
+      const bool high = p & 2, odd = p & 1;
+      float k0 = (high ? v2 : v0) + __shfl_xor_sync(0xffffffffu, high ? v0 : v2, 2);
+      float k1 = (high ? v3 : v1) + __shfl_xor_sync(0xffffffffu, high ? v1 : v3, 2);
+      float s = (odd ? k1 : k0) + __shfl_xor_sync(0xffffffffu, odd ? k0 : k1, 1);
+#pragma unroll
+      for (int o = 4; o < P; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      r[0] = s;
+    }
+  }
+  // writes the four sums to dst[0..3], each by one lane
+  __device__ __forceinline__ void put(float *dst, int p) const {
+    if (P > 4 && p >= 4) return;
+#pragma unroll
+    for (int i = 0; i < kLeft; ++i) dst[p + i * P] = r[i];
+  }
+};
+
+// E elements of a row from t on, 0 at and behind `end` (nothing is read there).
+template <typename T, int E>
+__device__ __forceinline__ void load_row(Pack<T, E> &v, const T *row, int t, int end, bool vec) {
+  if (vec && t + E <= end) {
+    v.load(row + t);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v.v[i] = t + i < end ? row[t + i] : from_f<T>(0.f);
+  }
+}
+template <typename T, int E>
+__device__ __forceinline__ void store_row(const Pack<T, E> &v, T *row, int t, int end, bool vec) {
+  if (vec && t + E <= end) {
+    v.store(row + t);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (t + i < end) row[t + i] = v.v[i];
+  }
+}
+
+// A block's tile of B and C: loaded along the length, kept as [t][n].
+template <typename T, int P, int TT>
+struct TileBC {
+  static constexpr int NP = kS * P;
+  static constexpr int kPitch = NP + 4;
+  static constexpr int kEach = (NP * TT + kScanThreads - 1) / kScanThreads;
+  T b[kEach], c[kEach];
+  __device__ __forceinline__ void load(const T *B, const T *C, int states, int length, int t0, int end, bool with_c) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int e = i * kScanThreads + threadIdx.x, n = e / TT, t = t0 + e % TT;
+      const bool in = n < states && t < end && e < NP * TT;
+      b[i] = in ? B[(int64_t)n * length + t] : from_f<T>(0.f);
+      if (with_c) c[i] = in ? C[(int64_t)n * length + t] : from_f<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void put(float *sB, float *sC, bool with_c) const {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int e = i * kScanThreads + threadIdx.x, n = e / TT, t = e % TT;
+      if (e < NP * TT) {
+        sB[t * kPitch + n] = to_f(b[i]);
+        if (with_c) sC[t * kPitch + n] = to_f(c[i]);
+      }
+    }
+  }
+};
+
+// What a thread is: lane p of a channel, in a segment of the length.
+template <int P>
+struct ScanPlace {
+  int p, c, d, b, g, blk, seg, len;
+  bool valid;
+  int64_t row;   // batch row * channels + channel
+  __device__ __forceinline__ ScanPlace(const ScanArgs &a) {
+    p = threadIdx.x % P;
+    c = threadIdx.x / P;
+    int i = blockIdx.x;
+    seg = i % a.nseg;
+    i /= a.nseg;
+    blk = i % a.nblk;
+    i /= a.nblk;
+    g = i % a.groups;
+    b = i / a.groups;
+    const int in_group = blk * (kScanThreads / P) + c;
+    valid = in_group < a.per_group;
+    // a thread without a channel computes on its group's last one and writes nothing
+    d = g * a.per_group + (valid ? in_group : a.per_group - 1);
+    row = (int64_t)b * a.channels + d;
+    len = a.length;
+    if (a.lengths) len = min(max(a.lengths[b], 0), a.length);
+  }
+};
+
+template <int P>
+__device__ __forceinline__ void load_states(const float *src, int states, int p, float *h) {
+#pragma unroll
+  for (int s = 0; s < kS; ++s) h[s] = p * kS + s < states ? src[p * kS + s] : 0.f;
+}
+template <int P>
+__device__ __forceinline__ void store_states(float *dst, int states, int p, const float *h) {
+  if (states % kS == 0) {
+    // (rows of a multiple of four states in a 16-byte aligned array)
+    if (p * kS < states) *reinterpret_cast<float4 *>(dst + p * kS) = make_float4(h[0], h[1], h[2], h[3]);
+  } else {
+#pragma unroll
+    for (int s = 0; s < kS; ++s)
+      if (p * kS + s < states) dst[p * kS + s] = h[s];
+  }
+}
+
+// Forward pass; kStateOnly: the first pass over segments (end state from zero
+// and sum of D_t, no outputs).
+template <typename T, int P, bool kStateOnly>
+__global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(ScanArgs a) {
+  constexpr int CB = kScanThreads / P, TT = ScanTile<P>::kFwd, E = TT / P, TB = ScanTile<P>::kBwd;
+  constexpr int DP = TT + 4;
+  using BC = TileBC<T, P, TT>;
+  __shared__ __align__(16) float s_d[CB * DP], s_x[CB * DP], s_B[TT * BC::kPitch],
+      s_C[kStateOnly ? 4 : TT * BC::kPitch];
+  const ScanPlace<P> q(a);
+  const int p = q.p, N = a.states, L = a.length;
+  const T *u = static_cast<const T *>(a.u) + q.row * L, *dl = static_cast<const T *>(a.delta) + q.row * L;
+  const T *z = a.z ? static_cast<const T *>(a.z) + q.row * L : nullptr;
+  const int64_t bg = ((int64_t)q.b * a.groups + q.g) * N * L;
+  const T *B = static_cast<const T *>(a.B) + bg, *C = static_cast<const T *>(a.C) + bg;
+  T *out = static_cast<T *>(a.out) + q.row * L;
+  const bool vec = (L * (int64_t)sizeof(T)) % Pack<T, E>::kVec == 0;
+  const float bias = a.bias ? a.bias[q.d] : 0.f, skip = a.skip ? a.skip[q.d] : 0.f;
+  float A2[kS], h[kS];
+  load_states<P>(a.A + (int64_t)q.d * N, N, p, A2);
+#pragma unroll
+  for (int s = 0; s < kS; ++s) A2[s] *= kLog2e;
+  const int t_begin = q.seg * a.seg_len, t_stop = min(L, t_begin + a.seg_len), t_end = min(t_stop, q.len);
+#pragma unroll
+  for (int s = 0; s < kS; ++s) h[s] = 0.f;
+  if (!kStateOnly) {
+    if (a.init) load_states<P>(a.init + q.row * N, N, p, h);
+    for (int i = 0; i < q.seg; ++i) {
+      float e[kS];
+      const int64_t at = ((int64_t)q.b * a.nseg + i) * a.channels + q.d;
+      load_states<P>(a.seg_state + at * N, N, p, e);
+      const float sum = a.seg_sum[at];
+#pragma unroll
+      for (int s = 0; s < kS; ++s) h[s] = fmaf(exp2_f(sum * A2[s]), h[s], e[s]);
+    }
+  }
+  float total = 0.f;
+  float *row_d = s_d + q.c * DP, *row_x = s_x + q.c * DP;
+  Pack<T, E> nu, nd, nz;   // the next tile's inputs, on their way
+  BC nbc;
+  auto fetch = [&](int t0) {
+    load_row(nu, u, t0 + p * E, t_end, vec);
+    load_row(nd, dl, t0 + p * E, t_end, vec);
+    if (!kStateOnly && z) load_row(nz, z, t0 + p * E, t_end, vec);
+    nbc.load(B, C, N, L, t0, t_end, !kStateOnly);
+  };
+  if (t_begin < t_end) fetch(t_begin);
+  for (int t0 = t_begin; t0 < t_stop; t0 += TT) {
+    if (t0 >= t_end) {  // nothing but padding from here on
+      if (!kStateOnly && q.valid) {
+        Pack<T, E> o;
+#pragma unroll
+        for (int i = 0; i < E; ++i) o.v[i] = from_f<T>(0.f);
+        store_row(o, out, t0 + p * E, t_stop, vec);
+      }
+      continue;
+    }
+    const Pack<T, E> cu = nu, cz = nz;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      float v = nd.f(i) + bias;
+      if (a.softplus) v = softplus_f(v);
+      if (t0 + p * E + i >= t_end) v = 0.f;
+      row_d[p * E + i] = v;
+      row_x[p * E + i] = v * cu.f(i);
+      if (kStateOnly) total += v;
+    }
+    nbc.put(s_B, s_C, !kStateOnly);
+    __syncthreads();
+    if (t0 + TT < t_end) fetch(t0 + TT);
+    for (int t = 0; t < TT; t += 4) {
+      if (!kStateOnly && a.ckpt && t % TB == 0 && t0 + t < t_end && q.valid)
+        store_states<P>(a.ckpt + (((int64_t)q.b * ((L + TB - 1) / TB) + (t0 + t) / TB) * a.channels + q.d) * N, N, p, h);
+      const float4 d4 = *reinterpret_cast<const float4 *>(row_d + t);
+      const float4 x4 = *reinterpret_cast<const float4 *>(row_x + t);
+      const float dd[4] = {d4.x, d4.y, d4.z, d4.w}, xx[4] = {x4.x, x4.y, x4.z, x4.w};
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 b4 = *reinterpret_cast<const float4 *>(s_B + (t + j) * BC::kPitch + p * kS);
+        const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+        for (int s = 0; s < kS; ++s) h[s] = fmaf(exp2_f(dd[j] * A2[s]), h[s], xx[j] * bb[s]);
+        if (!kStateOnly) {
+          const float4 c4 = *reinterpret_cast<const float4 *>(s_C + (t + j) * BC::kPitch + p * kS);
+          y[j] = fmaf(h[0], c4.x, fmaf(h[1], c4.y, fmaf(h[2], c4.z, h[3] * c4.w)));
+        }
+      }
+      if (!kStateOnly) {
+        // y takes the place of D_t u_t: all lanes of the channel have read it
+        // (they are lanes of one warp, and the sums exchange among them)
+        const Sum4<P> sum(y[0], y[1], y[2], y[3], p);
+        __syncwarp();
+        sum.put(row_x + t, p);
+      }
+    }
+    if (!kStateOnly) {
+      __syncwarp();
+      if (q.valid) {
+        Pack<T, E> o;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          float v = fmaf(skip, cu.f(i), row_x[p * E + i]);
+          if (z) v *= cz.f(i) * sigmoid_f(cz.f(i));
+          if (t0 + p * E + i >= t_end) v = 0.f;
+          o.v[i] = from_f<T>(v);
+        }
+        store_row(o, out, t0 + p * E, t_stop, vec);
+      }
+    }
+    __syncthreads();
+  }
+  if (kStateOnly) {
+#pragma unroll
+    for (int o = 1; o < P; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (q.valid) {
+      const int64_t at = ((int64_t)q.b * a.nseg + q.seg) * a.channels + q.d;
+      store_states<P>(a.seg_state + at * N, N, p, h);
+      if (p == 0) a.seg_sum[at] = total;
+    }
+  } else if (a.final_state && q.seg == a.nseg - 1 && q.valid) {
+    store_states<P>(a.final_state + q.row * N, N, p, h);
+  }
+}
+
+// First pass of the backward over segments: r from zero behind the segment,
+// and the sum of D_t.
+template <typename T, int P>
+__global__ void __launch_bounds__(kScanThreads) scan_carry_kernel(ScanArgs a) {
+  constexpr int CB = kScanThreads / P, TT = ScanTile<P>::kBwd, E = TT >= P ? TT / P : 1;
+  constexpr int DP = TT + 4;
+  using BC = TileBC<T, P, TT>;
+  __shared__ __align__(16) float s_d[CB * DP], s_y[CB * DP], s_C[TT * BC::kPitch];
+  const ScanPlace<P> q(a);
+  const int p = q.p, N = a.states, L = a.length;
+  const T *dl = static_cast<const T *>(a.delta) + q.row * L, *grad = static_cast<const T *>(a.grad) + q.row * L;
+  const T *z = a.z ? static_cast<const T *>(a.z) + q.row * L : nullptr;
+  const T *C = static_cast<const T *>(a.C) + ((int64_t)q.b * a.groups + q.g) * N * L;
+  const bool vec = (L * (int64_t)sizeof(T)) % Pack<T, E>::kVec == 0;
+  const float bias = a.bias ? a.bias[q.d] : 0.f;
+  float A2[kS], r[kS];
+  load_states<P>(a.A + (int64_t)q.d * N, N, p, A2);
+#pragma unroll
+  for (int s = 0; s < kS; ++s) {
+    A2[s] *= kLog2e;
+    r[s] = 0.f;
+  }
+  const int t_begin = q.seg * a.seg_len, t_end = min(min(L, t_begin + a.seg_len), q.len);
+  float total = 0.f;
+  float *row_d = s_d + q.c * DP, *row_y = s_y + q.c * DP;
+  Pack<T, E> nd, ng, nz;
+  BC nbc;
+  auto fetch = [&](int t0) {
+    if (p * E < TT) {
+      load_row(nd, dl, t0 + p * E, t_end, vec);
+      load_row(ng, grad, t0 + p * E, t_end, vec);
+      if (z) load_row(nz, z, t0 + p * E, t_end, vec);
+    }
+    nbc.load(C, nullptr, N, L, t0, t_end, false);
+  };
+  const int last = t_begin + (t_end - t_begin - 1) / TT * TT;
+  if (t_begin < t_end) fetch(last);
+  for (int t0 = last; t0 >= t_begin && t_begin < t_end; t0 -= TT) {
+    if (p * E < TT) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        float v = nd.f(i) + bias;
+        if (a.softplus) v = softplus_f(v);
+        if (t0 + p * E + i >= t_end) v = 0.f;
+        row_d[p * E + i] = v;
+        total += v;
+        float dy = ng.f(i);
+        if (z) dy *= nz.f(i) * sigmoid_f(nz.f(i));
+        row_y[p * E + i] = dy;
+      }
+    }
+    nbc.put(s_C, nullptr, false);
+    __syncthreads();
+    if (t0 > t_begin) fetch(t0 - TT);
+    for (int t = TT - 4; t >= 0; t -= 4) {
+      const float4 d4 = *reinterpret_cast<const float4 *>(row_d + t);
+      const float4 y4 = *reinterpret_cast<const float4 *>(row_y + t);
+      const float dd[4] = {d4.x, d4.y, d4.z, d4.w}, yy[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll
+      for (int j = 3; j >= 0; --j) {
+        const float4 c4 = *reinterpret_cast<const float4 *>(s_C + (t + j) * BC::kPitch + p * kS);
+        const float cc[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+        for (int s = 0; s < kS; ++s) r[s] = exp2_f(dd[j] * A2[s]) * fmaf(cc[s], yy[j], r[s]);
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int o = 1; o < P; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (q.valid) {
+    const int64_t at = ((int64_t)q.b * a.nseg + q.seg) * a.channels + q.d;
+    store_states<P>(a.seg_state + at * N, N, p, r);
+    if (p == 0) a.seg_sum[at] = total;
+  }
+}
+
+constexpr int kSub = 8;  // tokens whose states and decays a lane holds at a time
+
+template <int P>
+struct BwdSmem {
+  static constexpr int CB = kScanThreads / P, TT = ScanTile<P>::kBwd, NP = kS * P;
+  static constexpr int DP = TT + 4, kPitch = NP + 4, kPart = 2 * NP + 1;
+  static constexpr int kRows = CB * DP;                          // D, D u, dy each
+  static constexpr int kFloats = 3 * kRows + 2 * TT * kPitch + (kScanThreads / 32) * TT * kPart;
+};
+
+// Sums of v[0..7] over the lanes of a warp that hold the same states of
+// different channels (lanes i, i + P, i + 2P ...): each step halves what a
+// lane holds.  Leaves kLeft values, the first of index `first`.
+template <int P>
+struct SumChannels {
+  static constexpr int kLevels = P >= 32 ? 0 : P == 16 ? 1 : P == 8 ? 2 : 3;
+  static constexpr int kLeft = 8 >> kLevels;
+  __device__ static __forceinline__ int first(int lane) {
+    int f = 0;
+    if (kLevels > 0 && (lane & P)) f += 4;
+    if (kLevels > 1 && (lane & (2 * P))) f += 2;
+    if (kLevels > 2 && (lane & (4 * P))) f += 1;
+    return f;
+  }
+  __device__ static __forceinline__ void sum(float *v, int lane) {
+    if constexpr (kLevels > 0) {
+      const bool hi = lane & P;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float keep = hi ? v[4 + i] : v[i], send = hi ? v[i] : v[4 + i];
+        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, P);
+      }
+    }
+    if constexpr (kLevels > 1) {
+      const bool hi = lane & (2 * P);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float keep = hi ? v[2 + i] : v[i], send = hi ? v[i] : v[2 + i];
+        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, 2 * P);
+      }
+    }
+    if constexpr (kLevels > 2) {
+      const bool hi = lane & (4 * P);
+      const float keep = hi ? v[1] : v[0], send = hi ? v[0] : v[1];
+      v[0] = keep + __shfl_xor_sync(0xffffffffu, send, 4 * P);
+#pragma unroll
+      for (int o = 8 * P; o < 32; o <<= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    }
+  }
+  // with P <= 2 several lanes end with the same sum: one of them writes it
+  __device__ static __forceinline__ bool writes(int lane) { return lane < 8 * P; }
+};
+
+template <typename T, int P>
+__global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs a) {
+  using S = BwdSmem<P>;
+  constexpr int TT = S::TT, E = TT >= P ? TT / P : 1, DP = S::DP, NP = S::NP;
+  using BC = TileBC<T, P, TT>;
+  extern __shared__ __align__(16) float smem[];
+  float *s_d = smem, *s_x = s_d + S::kRows, *s_y = s_x + S::kRows;
+  float *s_B = s_y + S::kRows, *s_C = s_B + TT * S::kPitch, *s_part = s_C + TT * S::kPitch;
+  const ScanPlace<P> q(a);
+  const int p = q.p, N = a.states, L = a.length, lane = threadIdx.x & 31;
+  const T *u = static_cast<const T *>(a.u) + q.row * L, *dl = static_cast<const T *>(a.delta) + q.row * L;
+  const T *grad = static_cast<const T *>(a.grad) + q.row * L;
+  const T *z = a.z ? static_cast<const T *>(a.z) + q.row * L : nullptr;
+  const int64_t bg = ((int64_t)q.b * a.groups + q.g) * N * L;
+  const T *B = static_cast<const T *>(a.B) + bg, *C = static_cast<const T *>(a.C) + bg;
+  T *du = static_cast<T *>(a.du) + q.row * L, *ddl = static_cast<T *>(a.ddelta) + q.row * L;
+  T *dz = a.z ? static_cast<T *>(a.dz) + q.row * L : nullptr;
+  float *part = a.part_bc + (((int64_t)q.b * a.groups + q.g) * a.nblk + q.blk) * 2 * N * L;
+  const bool vec = (L * (int64_t)sizeof(T)) % Pack<T, E>::kVec == 0;
+  const bool loads = p * E < TT;  // (more lanes than tokens of a tile)
+  const float bias = a.bias ? a.bias[q.d] : 0.f, skip = a.skip ? a.skip[q.d] : 0.f;
+  float A2[kS], r[kS], dA[kS], dskip = 0.f, dbias = 0.f;
+  load_states<P>(a.A + (int64_t)q.d * N, N, p, A2);
+#pragma unroll
+  for (int s = 0; s < kS; ++s) {
+    A2[s] *= kLog2e;
+    r[s] = dA[s] = 0.f;
+  }
+  if (a.grad_final) load_states<P>(a.grad_final + q.row * N, N, p, r);
+  for (int i = a.nseg - 1; i > q.seg; --i) {
+    float e[kS];
+    const int64_t at = ((int64_t)q.b * a.nseg + i) * a.channels + q.d;
+    load_states<P>(a.seg_state + at * N, N, p, e);
+    const float sum = a.seg_sum[at];
+#pragma unroll
+    for (int s = 0; s < kS; ++s) r[s] = fmaf(exp2_f(sum * A2[s]), r[s], e[s]);
+  }
+  const int t_begin = q.seg * a.seg_len, t_stop = min(L, t_begin + a.seg_len), t_end = min(t_stop, q.len);
+  float *row_d = s_d + q.c * DP, *row_x = s_x + q.c * DP, *row_y = s_y + q.c * DP;
+  float *my_part = s_part + (threadIdx.x / 32) * TT * S::kPart;
+  Pack<T, E> nu, nd, ng, nz;
+  BC nbc;
+  auto fetch = [&](int t0) {
+    if (loads) {
+      load_row(nu, u, t0 + p * E, t_end, vec);
+      load_row(nd, dl, t0 + p * E, t_end, vec);
+      load_row(ng, grad, t0 + p * E, t_end, vec);
+      if (z) load_row(nz, z, t0 + p * E, t_end, vec);
+    }
+    nbc.load(B, C, N, L, t0, t_end, true);
+  };
+  const int last_live = t_begin + (t_end - t_begin - 1) / TT * TT;
+  if (t_begin < t_end) fetch(last_live);
+  for (int t0 = t_begin + (t_stop - t_begin - 1) / TT * TT; t0 >= t_begin; t0 -= TT) {
+    if (t0 >= t_end) {  // padding: no gradient
+      if (q.valid && loads) {
+        Pack<T, E> o;
+#pragma unroll
+        for (int i = 0; i < E; ++i) o.v[i] = from_f<T>(0.f);
+        store_row(o, du, t0 + p * E, t_stop, vec);
+        store_row(o, ddl, t0 + p * E, t_stop, vec);
+        if (z) store_row(o, dz, t0 + p * E, t_stop, vec);
+      }
+      for (int e = threadIdx.x; e < 2 * N * TT; e += kScanThreads) {
+        const int n = e / TT, t = t0 + e % TT;
+        if (t < t_stop) part[(int64_t)n * L + t] = 0.f;
+      }
+      continue;
+    }
+    const Pack<T, E> cu = nu, cd = nd, cg = ng, cz = nz;
+    if (loads) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        float v = cd.f(i) + bias;
+        if (a.softplus) v = softplus_f(v);
+        if (t0 + p * E + i >= t_end) v = 0.f;
+        row_d[p * E + i] = v;
+        row_x[p * E + i] = v * cu.f(i);
+        float dy = cg.f(i);
+        if (z) dy *= cz.f(i) * sigmoid_f(cz.f(i));
+        // a thread without a channel adds nothing to the sums over channels
+        row_y[p * E + i] = q.valid ? dy : 0.f;
+      }
+    }
+    nbc.put(s_B, s_C, true);
+    __syncthreads();
+    if (t0 > t_begin) fetch(t0 - TT);
+    // the states at the start of each run of kSub tokens
+    float start[TT / kSub][kS];
+    load_states<P>(a.ckpt + (((int64_t)q.b * ((L + TT - 1) / TT) + t0 / TT) * a.channels + q.d) * N, N, p, start[0]);
+#pragma unroll
+    for (int k = 1; k < TT / kSub; ++k) {
+      float h[kS];
+#pragma unroll
+      for (int s = 0; s < kS; ++s) h[s] = start[k - 1][s];
+#pragma unroll
+      for (int j = 0; j < kSub; ++j) {
+        const int t = (k - 1) * kSub + j;
+        const float d = row_d[t], x = row_x[t];
+        const float4 b4 = *reinterpret_cast<const float4 *>(s_B + t * S::kPitch + p * kS);
+        const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+        for (int s = 0; s < kS; ++s) h[s] = fmaf(exp2_f(d * A2[s]), h[s], x * bb[s]);
+      }
+#pragma unroll
+      for (int s = 0; s < kS; ++s) start[k][s] = h[s];
+    }
+#pragma unroll
+    for (int k = TT / kSub - 1; k >= 0; --k) {
+      float h[kSub + 1][kS], dec[kSub][kS], y[kSub], s1[kSub], s2[kSub];
+#pragma unroll
+      for (int s = 0; s < kS; ++s) h[0][s] = start[k][s];
+#pragma unroll
+      for (int j = 0; j < kSub; ++j) {
+        const int t = k * kSub + j;
+        const float d = row_d[t], x = row_x[t];
+        const float4 b4 = *reinterpret_cast<const float4 *>(s_B + t * S::kPitch + p * kS);
+        const float4 c4 = *reinterpret_cast<const float4 *>(s_C + t * S::kPitch + p * kS);
+        const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+        for (int s = 0; s < kS; ++s) {
+          dec[j][s] = exp2_f(d * A2[s]);
+          h[j + 1][s] = fmaf(dec[j][s], h[j][s], x * bb[s]);
+        }
+        y[j] = fmaf(h[j + 1][0], c4.x, fmaf(h[j + 1][1], c4.y, fmaf(h[j + 1][2], c4.z, h[j + 1][3] * c4.w)));
+      }
+#pragma unroll
+      for (int j = kSub - 1; j >= 0; --j) {
+        const int t = k * kSub + j;
+        const float d = row_d[t], x = row_x[t], dy = row_y[t];
+        const float4 b4 = *reinterpret_cast<const float4 *>(s_B + t * S::kPitch + p * kS);
+        const float4 c4 = *reinterpret_cast<const float4 *>(s_C + t * S::kPitch + p * kS);
+        const float bb[4] = {b4.x, b4.y, b4.z, b4.w}, cc[4] = {c4.x, c4.y, c4.z, c4.w};
+        float v[8];
+        s1[j] = s2[j] = 0.f;
+#pragma unroll
+        for (int s = 0; s < kS; ++s) {
+          const float dh = fmaf(dy, cc[s], r[s]);
+          v[s] = q.valid ? dh * x : 0.f;
+          v[4 + s] = dy * h[j + 1][s];
+          s1[j] = fmaf(dh, bb[s], s1[j]);
+          r[s] = dec[j][s] * dh;
+          const float m = r[s] * h[j][s];
+          s2[j] = fmaf(m, A2[s], s2[j]);
+          dA[s] = fmaf(m, d, dA[s]);
+        }
+        SumChannels<P>::sum(v, lane);
+        if (SumChannels<P>::writes(lane)) {
+          const int f = SumChannels<P>::first(lane);
+#pragma unroll
+          for (int i = 0; i < SumChannels<P>::kLeft; ++i) {
+            const int idx = f + i;  // 0-3: dB of the lane's states, 4-7: dC
+            my_part[t * S::kPart + (idx / 4) * NP + p * kS + idx % 4] = v[i];
+          }
+        }
+      }
+      // the run's D, D u and dy have been read by all lanes: their places take
+      // the sums over the states
+#pragma unroll
+      for (int j = 0; j < kSub; j += 4) {
+        const Sum4<P> sy(y[j], y[j + 1], y[j + 2], y[j + 3], p);
+        const Sum4<P> sb(s1[j], s1[j + 1], s1[j + 2], s1[j + 3], p);
+        const Sum4<P> sm(s2[j], s2[j + 1], s2[j + 2], s2[j + 3], p);
+        __syncwarp();
+        sm.put(row_d + k * kSub + j, p);
+        sb.put(row_x + k * kSub + j, p);
+        sy.put(row_y + k * kSub + j, p);
+      }
+    }
+    __syncwarp();
+    if (q.valid && loads) {
+      Pack<T, E> ou, od, oz;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const bool live = t0 + p * E + i < t_end;
+        const float raw = cd.f(i) + bias, uu = cu.f(i), g = cg.f(i);
+        const float d = a.softplus ? softplus_f(raw) : raw;
+        float gate = 1.f, slope = 0.f;
+        if (z) {
+          const float zz = cz.f(i), e = sigmoid_f(zz);
+          gate = zz * e;
+          slope = e * fmaf(zz, 1.f - e, 1.f);
+        }
+        const float dy = g * gate, through = row_x[p * E + i];
+        float dd = fmaf(uu, through, row_d[p * E + i] * (1.f / kLog2e));
+        if (a.softplus && raw <= 20.f) dd *= sigmoid_f(raw);
+        if (!live) dd = 0.f;
+        ou.v[i] = from_f<T>(live ? fmaf(d, through, skip * dy) : 0.f);
+        od.v[i] = from_f<T>(dd);
+        if (z) oz.v[i] = from_f<T>(live ? g * slope * fmaf(skip, uu, row_y[p * E + i]) : 0.f);
+        dskip = fmaf(dy, uu, dskip);
+        dbias += dd;
+      }
+      store_row(ou, du, t0 + p * E, t_stop, vec);
+      store_row(od, ddl, t0 + p * E, t_stop, vec);
+      if (z) store_row(oz, dz, t0 + p * E, t_stop, vec);
+    }
+    __syncthreads();
+    // the warps' sums over their channels, added in order
+    for (int e = threadIdx.x; e < 2 * N * TT; e += kScanThreads) {
+      const int n = e / TT, t = e % TT;
+      if (t0 + t < t_stop) {
+        const float *src = s_part + t * S::kPart + (n < N ? n : NP + n - N);
+        float s = src[0];
+#pragma unroll
+        for (int w = 1; w < kScanThreads / 32; ++w) s += src[w * TT * S::kPart];
+        part[(int64_t)n * L + t0 + t] = s;
+      }
+    }
+    // (the next tile's first barrier comes before anything overwrites s_part)
+  }
+#pragma unroll
+  for (int o = 1; o < P; o <<= 1) {
+    dskip += __shfl_xor_sync(0xffffffffu, dskip, o);
+    dbias += __shfl_xor_sync(0xffffffffu, dbias, o);
+  }
+  if (q.valid) {
+    float *par = a.part_par + ((int64_t)q.b * a.nseg + q.seg) * a.channels * (N + 2);
+#pragma unroll
+    for (int s = 0; s < kS; ++s)
+      if (p * kS + s < N) par[(int64_t)q.d * N + p * kS + s] = dA[s];
+    if (p == 0) {
+      par[(int64_t)a.channels * N + q.d] = dskip;
+      par[(int64_t)a.channels * (N + 1) + q.d] = dbias;
+    }
+    if (a.dinit && q.seg == 0) store_states<P>(a.dinit + q.row * N, N, p, r);
+  }
+}
+
+// Adds up the blocks' shares of dB and dC (in 32 bits, over the blocks of a
+// group in order) and those of dA, dskip and dbias (in 64 bits, over the batch
+// and the segments in order).
+template <typename T>
+__global__ void __launch_bounds__(256) scan_params_kernel(ScanArgs a, T *dB, T *dC, float *dA, float *dskip,
+                                                         float *dbias, int64_t bc_blocks) {
+  const int N = a.states;
+  if (blockIdx.x < bc_blocks) {
+    const int64_t per = 2 * (int64_t)N * a.length, count = (int64_t)a.batch * a.groups * per;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= count) return;
+    const int64_t bg = i / per, e = i - bg * per, half = per / 2;
+    const float *src = a.part_bc + bg * a.nblk * per + e;
+    float s = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < a.nblk; ++k) s += src[k * per];
+    if (e < half) dB[bg * half + e] = from_f<T>(s);
+    else dC[bg * half + e - half] = from_f<T>(s);
+    return;
+  }
+  const int64_t count = (int64_t)a.channels * (N + 2), i = ((int64_t)blockIdx.x - bc_blocks) * 256 + threadIdx.x;
+  if (i >= count) return;
+  double s = 0.0;
+#pragma unroll 8
+  for (int k = 0; k < a.batch * a.nseg; ++k) s += a.part_par[k * count + i];
+  const int64_t dn = (int64_t)a.channels * N;
+  if (i < dn) dA[i] = (float)s;
+  else if (i < dn + a.channels) {
+    if (dskip) dskip[i - dn] = (float)s;
+  } else if (dbias) {
+    dbias[i - dn - a.channels] = (float)s;
+  }
+}
+
+struct ScanStepArgs {
+  const void *u, *delta, *z, *B, *C;
+  const float *A, *skip, *bias;
+  const int *slots;
+  float *state;
+  void *out;
+  int batch, places, channels, states, groups, per_group, softplus, nblk;
+};
+
+// One token: reads and writes each state once (8 bytes a state: what bounds it).
+template <typename T, int P>
+__global__ void __launch_bounds__(kScanThreads) scan_step_kernel(ScanStepArgs a) {
+  constexpr int CB = kScanThreads / P;
+  const int b = blockIdx.x / a.nblk, blk = blockIdx.x - b * a.nblk;
+  const int p = threadIdx.x % P, d = blk * CB + threadIdx.x / P, N = a.states;
+  const bool valid = d < a.channels;
+  bool bad;
+  const int place = step_place(a.slots, b, a.places, &bad);
+  const int64_t i = (int64_t)b * a.channels + (valid ? d : 0);
+  if (place < 0) {
+    if (valid && p == 0) static_cast<T *>(a.out)[i] = from_f<T>(bad ? __int_as_float(0x7fffffff) : 0.f);
+    return;
+  }
+  const int dd = valid ? d : 0, g = dd / a.per_group;
+  float *state = a.state + ((int64_t)place * a.channels + dd) * N;
+  alignas(16) float A2[kS], h[kS];
+  float y = 0.f;
+  const bool vec = N % kS == 0;
+  if (vec && p * kS < N) {
+    *reinterpret_cast<float4 *>(h) = *reinterpret_cast<const float4 *>(state + p * kS);
+    *reinterpret_cast<float4 *>(A2) = *reinterpret_cast<const float4 *>(a.A + (int64_t)dd * N + p * kS);
+  } else {
+    load_states<P>(state, N, p, h);
+    load_states<P>(a.A + (int64_t)dd * N, N, p, A2);
+  }
+  const float u = to_f(static_cast<const T *>(a.u)[i]);
+  float delta = to_f(static_cast<const T *>(a.delta)[i]) + (a.bias ? a.bias[dd] : 0.f);
+  if (a.softplus) delta = softplus_f(delta);
+  const T *B = static_cast<const T *>(a.B) + ((int64_t)b * a.groups + g) * N;
+  const T *C = static_cast<const T *>(a.C) + ((int64_t)b * a.groups + g) * N;
+#pragma unroll
+  for (int s = 0; s < kS; ++s) {
+    const int n = p * kS + s;
+    if (n < N) {
+      h[s] = fmaf(exp2_f(delta * (A2[s] * kLog2e)), h[s], delta * u * to_f(B[n]));
+      y = fmaf(h[s], to_f(C[n]), y);
+    }
+  }
+  if (valid) store_states<P>(state, N, p, h);
+#pragma unroll
+  for (int o = 1; o < P; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+  if (valid && p == 0) {
+    if (a.skip) y = fmaf(a.skip[dd], u, y);
+    if (a.z) {
+      const float z = to_f(static_cast<const T *>(a.z)[i]);
+      y *= z * sigmoid_f(z);
+    }
+    static_cast<T *>(a.out)[i] = from_f<T>(y);
+  }
+}
+
+// --------------------------------------------------------------------- host
+
+PerContext<uint64_t> g_scan_attr;
+
+template <typename F>
+int by_type_and_lanes(int dtype, int states, F &&f) {
+#define PC2D_LANES(T)                                            \
+  switch (lanes_of(states)) {                                    \
+    case 1: return f(T{}, std::integral_constant<int, 1>{});     \
+    case 2: return f(T{}, std::integral_constant<int, 2>{});     \
+    case 4: return f(T{}, std::integral_constant<int, 4>{});     \
+    case 8: return f(T{}, std::integral_constant<int, 8>{});     \
+    case 16: return f(T{}, std::integral_constant<int, 16>{});   \
+    default: return f(T{}, std::integral_constant<int, 32>{});   \
+  }
+  if (dtype == PC2D_DTYPE_F32) { PC2D_LANES(float) }
+  if (dtype == PC2D_DTYPE_F16) { PC2D_LANES(__half) }
+  PC2D_LANES(__nv_bfloat16)
+#undef PC2D_LANES
+}
+
+constexpr int kMaxStates = 128;
+
+int check_scan(const char *what, int dtype, int batch, int channels, int length, int states, int groups) {
+  if (!seq_dtype(dtype)) {
+    set_last_error("%s: unsupported dtype %d (float32, float16 and bfloat16)", what, dtype);
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if (batch < 0 || channels < 0 || length < 0 || states < 1 || groups < 1 || channels % groups != 0) {
+    set_last_error("%s: invalid batch %d, channels %d, length %d, states %d or groups %d (channels in equal groups)",
+                   what, batch, channels, length, states, groups);
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if (states > kMaxStates) {
+    set_last_error("%s: %d states per channel (at most %d)", what, states, kMaxStates);
+    return PC2D_ERR_UNSUPPORTED;
+  }
+  if (length > 0x7fffff00 || (int64_t)batch * channels > (int64_t)1 << 24) {
+    set_last_error("%s: problem too large", what);
+    return PC2D_ERR_UNSUPPORTED;
+  }
+  return PC2D_OK;
+}
+
+// Blocks and segments.  Segments cost the first pass over the inputs and its
+// exps again, so the length is cut only when the rows alone leave most of the
+// GPU idle, into as many as give four blocks per SM and at least two tiles of
+// the longer (forward) kind each.
+template <bool kBackward>
+void scan_split(ScanArgs *a) {
+  const int P = lanes_of(a->states), CB = kScanThreads / P;
+  a->per_group = a->channels / a->groups;
+  a->nblk = std::max(1, (a->per_group + CB - 1) / CB);
+  const int64_t blocks = (int64_t)a->batch * a->groups * a->nblk;
+  const int sms = device_sm_count();
+  constexpr int kStep = 64;  // a multiple of every tile
+  a->nseg = 1;
+  a->seg_len = std::max(kStep, (a->length + kStep - 1) / kStep * kStep);
+  if (blocks > 0 && blocks < sms + sms / 2) {
+    const int want = (int)std::min<int64_t>(64, (int64_t)sms * 4 / blocks);
+    const int len = std::max(2 * kStep, (int)((((int64_t)a->length + want - 1) / want + kStep - 1) / kStep * kStep));
+    const int n = std::max(1, (int)(((int64_t)a->length + len - 1) / len));
+    if (n > 2) {
+      a->nseg = n;
+      a->seg_len = len;
+    }
+  }
+}
+
+size_t scan_segment_bytes(const ScanArgs &a) {
+  if (a.nseg == 1) return 0;
+  return align_up((size_t)a.batch * a.nseg * a.channels * a.states * 4, 256) +
+         align_up((size_t)a.batch * a.nseg * a.channels * 4, 256);
+}
+size_t scan_part_bc_bytes(const ScanArgs &a) {
+  return align_up((size_t)a.batch * a.groups * a.nblk * 2 * a.states * a.length * 4, 256);
+}
+size_t scan_part_par_bytes(const ScanArgs &a) {
+  return align_up((size_t)a.batch * a.nseg * a.channels * (a.states + 2) * 4, 256);
+}
+char *take_segments(ScanArgs *a, char *ws) {
+  if (a->nseg == 1) return ws;
+  a->seg_state = reinterpret_cast<float *>(ws);
+  ws += align_up((size_t)a->batch * a->nseg * a->channels * a->states * 4, 256);
+  a->seg_sum = reinterpret_cast<float *>(ws);
+  return ws + align_up((size_t)a->batch * a->nseg * a->channels * 4, 256);
+}
+
+int check_ws(const char *what, const void *ws, size_t got, size_t need) {
+  if (got < need || (need > 0 && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255)))) {
+    set_last_error("%s: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", what, need, got);
+    return PC2D_ERR_WORKSPACE;
+  }
+  return PC2D_OK;
+}
+
+int check_aligned(const char *what, std::initializer_list<const void *> ptrs) {
+  for (const void *p : ptrs)
+    if (p && !aligned16(p)) {
+      set_last_error("%s: arrays must be 16-byte aligned", what);
+      return PC2D_ERR_INVALID_ARGUMENT;
+    }
+  return PC2D_OK;
+}
+
+ScanArgs scan_problem(int batch, int channels, int length, int states, int groups) {
+  ScanArgs a{};
+  a.batch = batch;
+  a.channels = channels;
+  a.length = length;
+  a.states = states;
+  a.groups = groups;
+  return a;
+}
+
+}  // namespace
+}  // namespace pc2d
+
+using namespace pc2d;
+
+extern "C" size_t pc2d_ssm_scan_checkpoint_size(int batch, int channels, int length, int states) {
+  if (check_scan("pc2d_ssm_scan_checkpoint_size", PC2D_DTYPE_F32, batch, channels, length, states, 1) != PC2D_OK)
+    return 0;
+  const int tile = bwd_tile_of(states);
+  return (size_t)batch * (((size_t)length + tile - 1) / tile) * channels * states * sizeof(float);
+}
+
+extern "C" size_t pc2d_ssm_scan_forward_workspace_size(int batch, int channels, int length, int states, int groups) {
+  if (check_scan("pc2d_ssm_scan_forward_workspace_size", PC2D_DTYPE_F32, batch, channels, length, states, groups) !=
+      PC2D_OK)
+    return 0;
+  ScanArgs a = scan_problem(batch, channels, length, states, groups);
+  scan_split<false>(&a);
+  return scan_segment_bytes(a);
+}
+
+extern "C" int pc2d_ssm_scan_forward(int dtype, const void *u, const void *delta, const float *A, const void *B,
+                                     const void *C, const float *skip, const void *z, const float *delta_bias,
+                                     const float *initial_state, const int *lengths, int delta_softplus, int batch,
+                                     int channels, int length, int states, int groups, void *output,
+                                     float *final_state, float *checkpoints, void *workspace, size_t workspace_bytes,
+                                     void *stream) {
+  NvtxRange range("pc2d_ssm_scan_forward");
+  int st = check_scan("pc2d_ssm_scan_forward", dtype, batch, channels, length, states, groups);
+  if (st != PC2D_OK) return st;
+  if ((st = pending_device_error()) != PC2D_OK) return st;
+  if (batch == 0 || channels == 0) return PC2D_OK;
+  if (!A || (length > 0 && (!u || !delta || !B || !C || !output))) {
+    set_last_error("pc2d_ssm_scan_forward: null pointer (u, delta, A, B, C or output)");
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if ((st = check_aligned("pc2d_ssm_scan_forward",
+                          {u, delta, z, output, initial_state, final_state, checkpoints, A})) != PC2D_OK)
+    return st;
+  ScanArgs a = scan_problem(batch, channels, length, states, groups);
+  scan_split<false>(&a);
+  if ((st = check_ws("pc2d_ssm_scan_forward", workspace, workspace_bytes, scan_segment_bytes(a))) != PC2D_OK) return st;
+  a.u = u; a.delta = delta; a.z = z; a.B = B; a.C = C;
+  a.A = A; a.skip = skip; a.bias = delta_bias; a.init = initial_state; a.lengths = lengths;
+  a.softplus = delta_softplus != 0;
+  a.out = output; a.final_state = final_state; a.ckpt = checkpoints;
+  take_segments(&a, static_cast<char *>(workspace));
+  const unsigned grid = (unsigned)((int64_t)batch * groups * a.nblk * a.nseg);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return by_type_and_lanes(dtype, states, [&](auto t, auto p) -> int {
+    using T = decltype(t);
+    constexpr int P = decltype(p)::value;
+    if (a.nseg > 1) {
+      scan_forward_kernel<T, P, true><<<grid, kScanThreads, 0, s>>>(a);
+      PC2D_LAUNCH_CHECK("scan_forward_kernel (segments)");
+    }
+    scan_forward_kernel<T, P, false><<<grid, kScanThreads, 0, s>>>(a);
+    PC2D_LAUNCH_CHECK("scan_forward_kernel");
+    return PC2D_OK;
+  });
+}
+
+extern "C" size_t pc2d_ssm_scan_backward_workspace_size(int batch, int channels, int length, int states, int groups) {
+  if (check_scan("pc2d_ssm_scan_backward_workspace_size", PC2D_DTYPE_F32, batch, channels, length, states, groups) !=
+      PC2D_OK)
+    return 0;
+  ScanArgs a = scan_problem(batch, channels, length, states, groups);
+  scan_split<true>(&a);
+  return scan_segment_bytes(a) + scan_part_bc_bytes(a) + scan_part_par_bytes(a);
+}
+
+extern "C" int pc2d_ssm_scan_backward(int dtype, const void *grad, const float *grad_final, const void *u,
+                                      const void *delta, const float *A, const void *B, const void *C,
+                                      const float *skip, const void *z, const float *delta_bias, const int *lengths,
+                                      const float *checkpoints, int delta_softplus, int batch, int channels,
+                                      int length, int states, int groups, void *ugrad, void *deltagrad, float *Agrad,
+                                      void *Bgrad, void *Cgrad, float *skipgrad, void *zgrad, float *biasgrad,
+                                      float *initialgrad, void *workspace, size_t workspace_bytes, void *stream) {
+  NvtxRange range("pc2d_ssm_scan_backward");
+  int st = check_scan("pc2d_ssm_scan_backward", dtype, batch, channels, length, states, groups);
+  if (st != PC2D_OK) return st;
+  if ((st = pending_device_error()) != PC2D_OK) return st;
+  if (channels == 0) return PC2D_OK;
+  const bool any = batch > 0 && length > 0;
+  if (!A || !Agrad || (any && (!grad || !u || !delta || !B || !C || !checkpoints || !ugrad || !deltagrad || !Bgrad ||
+                               !Cgrad || (z && !zgrad)))) {
+    set_last_error("pc2d_ssm_scan_backward: null pointer");
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if ((st = check_aligned("pc2d_ssm_scan_backward", {grad, u, delta, z, ugrad, deltagrad, zgrad, checkpoints,
+                                                     grad_final, initialgrad, A})) != PC2D_OK)
+    return st;
+  ScanArgs a = scan_problem(batch, channels, length, states, groups);
+  scan_split<true>(&a);
+  const size_t need = scan_segment_bytes(a) + scan_part_bc_bytes(a) + scan_part_par_bytes(a);
+  if ((st = check_ws("pc2d_ssm_scan_backward", workspace, workspace_bytes, need)) != PC2D_OK) return st;
+  a.u = u; a.delta = delta; a.z = z; a.B = B; a.C = C;
+  a.A = A; a.skip = skip; a.bias = delta_bias; a.lengths = lengths;
+  a.softplus = delta_softplus != 0;
+  a.ckpt = const_cast<float *>(checkpoints);
+  a.grad = grad; a.grad_final = grad_final;
+  a.du = ugrad; a.ddelta = deltagrad; a.dz = zgrad; a.dinit = initialgrad;
+  char *ws = take_segments(&a, static_cast<char *>(workspace));
+  a.part_bc = reinterpret_cast<float *>(ws);
+  a.part_par = reinterpret_cast<float *>(ws + scan_part_bc_bytes(a));
+  const unsigned grid = (unsigned)((int64_t)batch * groups * a.nblk * a.nseg);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return by_type_and_lanes(dtype, states, [&](auto t, auto p) -> int {
+    using T = decltype(t);
+    constexpr int P = decltype(p)::value;
+    if (grid > 0) {
+      constexpr int bytes = BwdSmem<P>::kFloats * 4;
+      // one bit per instance: 3 types x 6 lane counts
+      int bit = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 1 : 2;
+      for (int i = P; i > 1; i >>= 1) bit += 3;
+      const int attr = once_per_context(g_scan_attr, (uint64_t)1 << bit, []() -> int {
+        PC2D_CUDA_CHECK(cudaFuncSetAttribute(scan_backward_kernel<T, P>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             bytes));
+        return PC2D_OK;
+      });
+      if (attr != PC2D_OK) return attr;
+      if (a.nseg > 1) {
+        scan_carry_kernel<T, P><<<grid, kScanThreads, 0, s>>>(a);
+        PC2D_LAUNCH_CHECK("scan_carry_kernel");
+      }
+      scan_backward_kernel<T, P><<<grid, kScanThreads, bytes, s>>>(a);
+      PC2D_LAUNCH_CHECK("scan_backward_kernel");
+    }
+    const int64_t bc = ((int64_t)batch * groups * 2 * states * length + 255) / 256;
+    const int64_t par = ((int64_t)channels * (states + 2) + 255) / 256;
+    scan_params_kernel<T><<<(unsigned)(bc + par), 256, 0, s>>>(a, static_cast<T *>(Bgrad), static_cast<T *>(Cgrad),
+                                                               Agrad, skipgrad, biasgrad, bc);
+    PC2D_LAUNCH_CHECK("scan_params_kernel");
+    return PC2D_OK;
+  });
+}
+
+extern "C" int pc2d_ssm_scan_step(int dtype, const void *u, const void *delta, float *state, const float *A,
+                                  const void *B, const void *C, const float *skip, const void *z,
+                                  const float *delta_bias, const int *slots, int delta_softplus, int batch, int places,
+                                  int channels, int states, int groups, void *output, void *stream) {
+  NvtxRange range("pc2d_ssm_scan_step");
+  int st = check_scan("pc2d_ssm_scan_step", dtype, batch, channels, 1, states, groups);
+  if (st != PC2D_OK) return st;
+  if (places < 0 || (!slots && batch > places)) {
+    set_last_error("pc2d_ssm_scan_step: %d rows of a batch without slots, but %d states", batch, places);
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if ((st = pending_device_error()) != PC2D_OK) return st;
+  if (batch == 0 || channels == 0) return PC2D_OK;
+  if (!u || !delta || (!state && places > 0) || !A || !B || !C || !output) {
+    set_last_error("pc2d_ssm_scan_step: null pointer (u, delta, state, A, B, C or output)");
+    return PC2D_ERR_INVALID_ARGUMENT;
+  }
+  if ((st = check_aligned("pc2d_ssm_scan_step", {state, A})) != PC2D_OK) return st;
+  ScanStepArgs a{};
+  a.u = u; a.delta = delta; a.z = z; a.B = B; a.C = C; a.A = A; a.skip = skip; a.bias = delta_bias;
+  a.slots = slots; a.state = state; a.out = output;
+  a.batch = batch; a.places = places; a.channels = channels; a.states = states; a.groups = groups;
+  a.per_group = channels / groups;
+  a.softplus = delta_softplus != 0;
+  const int cb = kScanThreads / lanes_of(states);
+  a.nblk = (channels + cb - 1) / cb;
+  return by_type_and_lanes(dtype, states, [&](auto t, auto p) -> int {
+    scan_step_kernel<decltype(t), decltype(p)::value>
+        <<<(unsigned)((int64_t)a.nblk * batch), kScanThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+    PC2D_LAUNCH_CHECK("scan_step_kernel");
+    return PC2D_OK;
+  });
+}
