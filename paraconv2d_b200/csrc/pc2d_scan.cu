@@ -46,7 +46,8 @@ namespace pc2d {
 namespace {
 
 constexpr int kScanThreads = 128;
-constexpr int kS = 4;  // states per lane
+constexpr int kS = 4;    // states per lane
+constexpr int kSub = 8;  // tokens of an inner run
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Tile lengths by the lanes per channel: shared memory and the elements a
@@ -93,7 +94,101 @@ __device__ __forceinline__ float exp2_f(float v) {
   return r;
 }
 
-__device__ __forceinline__ float softplus_f(float v) { return v > 20.f ? v : log1pf(expf(v)); }
+// Two states at a time: the packed 32-bit instructions do twice the work of
+// the scalar ones per issue.
+struct F2 {
+  unsigned long long v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float a, float b) {
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  }
+  __device__ __forceinline__ float x() const {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+    return a;
+  }
+  __device__ __forceinline__ float y() const {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+    return b;
+  }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
+// exp2 of two arguments, the decays of two states.  The hardware exponential
+// is off by up to 2.4 units of 2^-24 and, on average over its table, low by
+// 0.3 to 0.8 (measured on [-2, 0]): a state that decays slowly adds the same
+// bias up over as many steps as it remembers.  So arguments below 1/8, where a
+// state remembers more than 11 steps, take 1 + x q(x) with the interpolation of
+// (2^x - 1)/x at the four Chebyshev nodes of [-1/8, 1/8] as q: one rounding
+// (0.5 units, no bias).  The other arguments, NaN and the infinities take the
+// hardware's.
+__device__ __forceinline__ F2 decay2(F2 x) {
+  const F2 one(1.f, 1.f);
+  F2 q = fma2(F2(0.009620536f, 0.009620536f), x, F2(0.055524945f, 0.055524945f));
+  q = fma2(q, x, F2(0.2402265f, 0.2402265f));
+  q = fma2(q, x, F2(0.6931471f, 0.6931471f));
+  q = fma2(q, x, one);
+  const float x0 = x.x(), x1 = x.y();
+  return F2(fabsf(x0) < 0.125f ? q.x() : exp2_f(x0), fabsf(x1) < 0.125f ? q.y() : exp2_f(x1));
+}
+constexpr int kH = kS / 2;  // pairs of states per lane
+// Two pairs from 16 aligned bytes of shared memory.
+__device__ __forceinline__ void load_pairs(const float *p, F2 *f) {
+  const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(p);
+  f[0].v = q.x;
+  f[1].v = q.y;
+}
+
+__device__ __forceinline__ void put_pairs(float *p, const F2 *f) {
+  *reinterpret_cast<ulonglong2 *>(p) = make_ulonglong2(f[0].v, f[1].v);
+}
+
+// softplus(v) = max(v, 0) + log(1 + e) with e = exp(-|v|), and its slope.
+// exp2 takes v log2(e) in two parts, so that e is off by 3 units of 2^-24
+// whatever v is; log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1/3, by the
+// interpolation of 2 atanh(s) / s at five Chebyshev nodes of s^2 in [0, 1/9]
+// (4e-9): it keeps its relative accuracy where e is small.
+__device__ __forceinline__ float exp_neg_abs(float v) {
+  const float a = -fabsf(v), hi = a * kLog2e;
+  const float lo = fmaf(a, 1.925963033e-8f, fmaf(a, kLog2e, -hi));
+  const float e = exp2_f(hi);
+  return hi < -126.f ? 0.f : fmaf(e, lo * 0.6931471806f, e);
+}
+__device__ __forceinline__ float softplus_f(float v) {
+  const float e = exp_neg_abs(v);
+  const float s = __fdividef(e, 2.f + e), w = s * s;
+  float q = fmaf(0.2815778f, w, 0.27965158f);
+  q = fmaf(q, w, 0.40024596f);
+  q = fmaf(q, w, 0.6666632f);
+  q = fmaf(q, w, 2.f);
+  return fmaf(q, s, fmaxf(v, 0.f));
+}
+// softplus'(v), the logistic function
+__device__ __forceinline__ float softplus_slope(float v) {
+  const float e = exp_neg_abs(v);
+  return __fdividef(v < 0.f ? e : 1.f, 1.f + e);
+}
+// Eight floats of a row, from a 16-byte boundary.
+__device__ __forceinline__ void load8f(const float *p, float *v) {
+  const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
 
 // Sums of v0..v3 over the P lanes of a channel.  P >= 4: lane p ends with
 // that of v[p % 4]; P = 2: with those of v[p] and v[p + 2]; P = 1: all four.
@@ -150,29 +245,41 @@ __device__ __forceinline__ void store_row(const Pack<T, E> &v, T *row, int t, in
   }
 }
 
-// A block's tile of B and C: loaded along the length, kept as [t][n].
+// A block's tile of B and C: loaded along the length by vectors, kept as
+// [t][n].  Rows are NP floats, and 4 more after every kVec of them, so that the
+// lanes of a warp, which store the same element of their vectors, meet
+// different banks.
 template <typename T, int P, int TT>
 struct TileBC {
-  static constexpr int NP = kS * P;
-  static constexpr int kPitch = NP + 4;
-  static constexpr int kEach = (NP * TT + kScanThreads - 1) / kScanThreads;
-  T b[kEach], c[kEach];
-  __device__ __forceinline__ void load(const T *B, const T *C, int states, int length, int t0, int end, bool with_c) {
+  static constexpr int NP = kS * P, kCount = NP * TT;
+  static constexpr int kEach = kCount / kScanThreads > 0 ? kCount / kScanThreads : 1;
+  static constexpr int kVec = kEach * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : kEach;
+  static constexpr int kNum = kEach / kVec;
+  static constexpr int kFloats = TT * NP + TT / kVec * 4;
+  __device__ static __forceinline__ int row(int t) { return t * NP + t / kVec * 4; }
+  // row(t + j) for t a multiple of 8 and a constant j < 8
+  __device__ static __forceinline__ int row8(int t, int j) { return t * NP + t / kVec * 4 + j * NP + j / kVec * 4; }
+  Pack<T, kVec> b[kNum], c[kNum];
+  __device__ __forceinline__ void load(const T *B, const T *C, int states, int length, int t0, int end, bool vec,
+                                       bool with_c) {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int e = i * kScanThreads + threadIdx.x, n = e / TT, t = t0 + e % TT;
-      const bool in = n < states && t < end && e < NP * TT;
-      b[i] = in ? B[(int64_t)n * length + t] : from_f<T>(0.f);
-      if (with_c) c[i] = in ? C[(int64_t)n * length + t] : from_f<T>(0.f);
+    for (int i = 0; i < kNum; ++i) {
+      const int e = (i * kScanThreads + threadIdx.x) * kVec, n = e / TT, t = t0 + e % TT;
+      const int stop = n < states && e < kCount ? end : t;  // nothing to read for missing states
+      load_row(b[i], B + (int64_t)n * length, t, stop, vec);
+      if (with_c) load_row(c[i], C + (int64_t)n * length, t, stop, vec);
     }
   }
   __device__ __forceinline__ void put(float *sB, float *sC, bool with_c) const {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int e = i * kScanThreads + threadIdx.x, n = e / TT, t = e % TT;
-      if (e < NP * TT) {
-        sB[t * kPitch + n] = to_f(b[i]);
-        if (with_c) sC[t * kPitch + n] = to_f(c[i]);
+    for (int i = 0; i < kNum; ++i) {
+      const int e = (i * kScanThreads + threadIdx.x) * kVec, n = e / TT, t = e % TT;
+      if (e < kCount) {
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) {
+          sB[row(t) + k * NP + n] = b[i].f(k);
+          if (with_c) sC[row(t) + k * NP + n] = c[i].f(k);
+        }
       }
     }
   }
@@ -224,12 +331,12 @@ __device__ __forceinline__ void store_states(float *dst, int states, int p, cons
 // Forward pass; kStateOnly: the first pass over segments (end state from zero
 // and sum of D_t, no outputs).
 template <typename T, int P, bool kStateOnly>
-__global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(kScanThreads, P <= 8 ? 4 : 2) scan_forward_kernel(ScanArgs a) {
   constexpr int CB = kScanThreads / P, TT = ScanTile<P>::kFwd, E = TT / P, TB = ScanTile<P>::kBwd;
   constexpr int DP = TT + 4;
   using BC = TileBC<T, P, TT>;
-  __shared__ __align__(16) float s_d[CB * DP], s_x[CB * DP], s_B[TT * BC::kPitch],
-      s_C[kStateOnly ? 4 : TT * BC::kPitch];
+  __shared__ __align__(16) float s_d[CB * DP], s_x[CB * DP], s_o[kStateOnly ? 4 : CB * DP], s_B[BC::kFloats],
+      s_C[kStateOnly ? 4 : BC::kFloats];
   const ScanPlace<P> q(a);
   const int p = q.p, N = a.states, L = a.length;
   const T *u = static_cast<const T *>(a.u) + q.row * L, *dl = static_cast<const T *>(a.delta) + q.row * L;
@@ -237,7 +344,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(ScanArgs a) 
   const int64_t bg = ((int64_t)q.b * a.groups + q.g) * N * L;
   const T *B = static_cast<const T *>(a.B) + bg, *C = static_cast<const T *>(a.C) + bg;
   T *out = static_cast<T *>(a.out) + q.row * L;
-  const bool vec = (L * (int64_t)sizeof(T)) % Pack<T, E>::kVec == 0;
+  const bool vec = (L * (int64_t)sizeof(T)) % 16 == 0;
   const float bias = a.bias ? a.bias[q.d] : 0.f, skip = a.skip ? a.skip[q.d] : 0.f;
   float A2[kS], h[kS];
   load_states<P>(a.A + (int64_t)q.d * N, N, p, A2);
@@ -258,15 +365,21 @@ __global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(ScanArgs a) 
     }
   }
   float total = 0.f;
-  float *row_d = s_d + q.c * DP, *row_x = s_x + q.c * DP;
+  float *row_d = s_d + q.c * DP, *row_x = s_x + q.c * DP, *row_o = s_o + (kStateOnly ? 0 : q.c * DP);
   Pack<T, E> nu, nd, nz;   // the next tile's inputs, on their way
   BC nbc;
   auto fetch = [&](int t0) {
     load_row(nu, u, t0 + p * E, t_end, vec);
     load_row(nd, dl, t0 + p * E, t_end, vec);
     if (!kStateOnly && z) load_row(nz, z, t0 + p * E, t_end, vec);
-    nbc.load(B, C, N, L, t0, t_end, !kStateOnly);
+    nbc.load(B, C, N, L, t0, t_end, vec, !kStateOnly);
   };
+  F2 A22[kH], h2[kH];
+#pragma unroll
+  for (int s = 0; s < kH; ++s) {
+    A22[s] = F2(A2[2 * s], A2[2 * s + 1]);
+    h2[s] = F2(h[2 * s], h[2 * s + 1]);
+  }
   if (t_begin < t_end) fetch(t_begin);
   for (int t0 = t_begin; t0 < t_stop; t0 += TT) {
     if (t0 >= t_end) {  // nothing but padding from here on
@@ -291,30 +404,36 @@ __global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(ScanArgs a) 
     nbc.put(s_B, s_C, !kStateOnly);
     __syncthreads();
     if (t0 + TT < t_end) fetch(t0 + TT);
-    for (int t = 0; t < TT; t += 4) {
-      if (!kStateOnly && a.ckpt && t % TB == 0 && t0 + t < t_end && q.valid)
-        store_states<P>(a.ckpt + (((int64_t)q.b * ((L + TB - 1) / TB) + (t0 + t) / TB) * a.channels + q.d) * N, N, p, h);
-      const float4 d4 = *reinterpret_cast<const float4 *>(row_d + t);
-      const float4 x4 = *reinterpret_cast<const float4 *>(row_x + t);
-      const float dd[4] = {d4.x, d4.y, d4.z, d4.w}, xx[4] = {x4.x, x4.y, x4.z, x4.w};
-      float y[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4 b4 = *reinterpret_cast<const float4 *>(s_B + (t + j) * BC::kPitch + p * kS);
-        const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-        for (int s = 0; s < kS; ++s) h[s] = fmaf(exp2_f(dd[j] * A2[s]), h[s], xx[j] * bb[s]);
-        if (!kStateOnly) {
-          const float4 c4 = *reinterpret_cast<const float4 *>(s_C + (t + j) * BC::kPitch + p * kS);
-          y[j] = fmaf(h[0], c4.x, fmaf(h[1], c4.y, fmaf(h[2], c4.z, h[3] * c4.w)));
-        }
+#pragma unroll 1
+    for (int tb = 0; tb < TT; tb += TB) {
+      if (!kStateOnly && a.ckpt && t0 + tb < t_end && q.valid) {
+        const float now[kS] = {h2[0].x(), h2[0].y(), h2[1].x(), h2[1].y()};
+        store_states<P>(a.ckpt + (((int64_t)q.b * ((L + TB - 1) / TB) + (t0 + tb) / TB) * a.channels + q.d) * N, N, p,
+                        now);
       }
-      if (!kStateOnly) {
-        // y takes the place of D_t u_t: all lanes of the channel have read it
-        // (they are lanes of one warp, and the sums exchange among them)
-        const Sum4<P> sum(y[0], y[1], y[2], y[3], p);
-        __syncwarp();
-        sum.put(row_x + t, p);
+#pragma unroll 1
+      for (int t = tb; t < tb + TB; t += kSub) {
+        float y[kSub], dd[kSub], xx[kSub];
+        load8f(row_d + t, dd);
+        load8f(row_x + t, xx);
+#pragma unroll
+        for (int j = 0; j < kSub; ++j) {
+          F2 b2[kH];
+          load_pairs(s_B + BC::row8(t, j) + p * kS, b2);
+          const F2 d2(dd[j], dd[j]), x2(xx[j], xx[j]);
+#pragma unroll
+          for (int s = 0; s < kH; ++s) h2[s] = fma2(decay2(mul2(d2, A22[s])), h2[s], mul2(x2, b2[s]));
+          if (!kStateOnly) {
+            F2 c2[kH];
+            load_pairs(s_C + BC::row8(t, j) + p * kS, c2);
+            const F2 y2 = fma2(h2[0], c2[0], mul2(h2[1], c2[1]));
+            y[j] = y2.x() + y2.y();
+          }
+        }
+        if (!kStateOnly) {
+#pragma unroll
+          for (int j = 0; j < kSub; j += 4) Sum4<P>(y[j], y[j + 1], y[j + 2], y[j + 3], p).put(row_o + t + j, p);
+        }
       }
     }
     if (!kStateOnly) {
@@ -323,7 +442,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(ScanArgs a) 
         Pack<T, E> o;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-          float v = fmaf(skip, cu.f(i), row_x[p * E + i]);
+          float v = fmaf(skip, cu.f(i), row_o[p * E + i]);
           if (z) v *= cz.f(i) * sigmoid_f(cz.f(i));
           if (t0 + p * E + i >= t_end) v = 0.f;
           o.v[i] = from_f<T>(v);
@@ -332,6 +451,11 @@ __global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(ScanArgs a) 
       }
     }
     __syncthreads();
+  }
+#pragma unroll
+  for (int s = 0; s < kH; ++s) {
+    h[2 * s] = h2[s].x();
+    h[2 * s + 1] = h2[s].y();
   }
   if (kStateOnly) {
 #pragma unroll
@@ -349,17 +473,17 @@ __global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(ScanArgs a) 
 // First pass of the backward over segments: r from zero behind the segment,
 // and the sum of D_t.
 template <typename T, int P>
-__global__ void __launch_bounds__(kScanThreads) scan_carry_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(kScanThreads, P <= 8 ? 4 : 2) scan_carry_kernel(ScanArgs a) {
   constexpr int CB = kScanThreads / P, TT = ScanTile<P>::kBwd, E = TT >= P ? TT / P : 1;
   constexpr int DP = TT + 4;
   using BC = TileBC<T, P, TT>;
-  __shared__ __align__(16) float s_d[CB * DP], s_y[CB * DP], s_C[TT * BC::kPitch];
+  __shared__ __align__(16) float s_d[CB * DP], s_y[CB * DP], s_C[BC::kFloats];
   const ScanPlace<P> q(a);
   const int p = q.p, N = a.states, L = a.length;
   const T *dl = static_cast<const T *>(a.delta) + q.row * L, *grad = static_cast<const T *>(a.grad) + q.row * L;
   const T *z = a.z ? static_cast<const T *>(a.z) + q.row * L : nullptr;
   const T *C = static_cast<const T *>(a.C) + ((int64_t)q.b * a.groups + q.g) * N * L;
-  const bool vec = (L * (int64_t)sizeof(T)) % Pack<T, E>::kVec == 0;
+  const bool vec = (L * (int64_t)sizeof(T)) % 16 == 0;
   const float bias = a.bias ? a.bias[q.d] : 0.f;
   float A2[kS], r[kS];
   load_states<P>(a.A + (int64_t)q.d * N, N, p, A2);
@@ -379,8 +503,14 @@ __global__ void __launch_bounds__(kScanThreads) scan_carry_kernel(ScanArgs a) {
       load_row(ng, grad, t0 + p * E, t_end, vec);
       if (z) load_row(nz, z, t0 + p * E, t_end, vec);
     }
-    nbc.load(C, nullptr, N, L, t0, t_end, false);
+    nbc.load(C, nullptr, N, L, t0, t_end, vec, false);
   };
+  F2 A22[kH], r2[kH];
+#pragma unroll
+  for (int s = 0; s < kH; ++s) {
+    A22[s] = F2(A2[2 * s], A2[2 * s + 1]);
+    r2[s] = F2(0.f, 0.f);
+  }
   const int last = t_begin + (t_end - t_begin - 1) / TT * TT;
   if (t_begin < t_end) fetch(last);
   for (int t0 = last; t0 >= t_begin && t_begin < t_end; t0 -= TT) {
@@ -400,16 +530,18 @@ __global__ void __launch_bounds__(kScanThreads) scan_carry_kernel(ScanArgs a) {
     nbc.put(s_C, nullptr, false);
     __syncthreads();
     if (t0 > t_begin) fetch(t0 - TT);
-    for (int t = TT - 4; t >= 0; t -= 4) {
-      const float4 d4 = *reinterpret_cast<const float4 *>(row_d + t);
-      const float4 y4 = *reinterpret_cast<const float4 *>(row_y + t);
-      const float dd[4] = {d4.x, d4.y, d4.z, d4.w}, yy[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll 1
+    for (int t = TT - kSub; t >= 0; t -= kSub) {
+      float dd[kSub], yy[kSub];
+      load8f(row_d + t, dd);
+      load8f(row_y + t, yy);
 #pragma unroll
-      for (int j = 3; j >= 0; --j) {
-        const float4 c4 = *reinterpret_cast<const float4 *>(s_C + (t + j) * BC::kPitch + p * kS);
-        const float cc[4] = {c4.x, c4.y, c4.z, c4.w};
+      for (int j = kSub - 1; j >= 0; --j) {
+        F2 c2[kH];
+        load_pairs(s_C + BC::row8(t, j) + p * kS, c2);
+        const F2 d2(dd[j], dd[j]), y2(yy[j], yy[j]);
 #pragma unroll
-        for (int s = 0; s < kS; ++s) r[s] = exp2_f(dd[j] * A2[s]) * fmaf(cc[s], yy[j], r[s]);
+        for (int s = 0; s < kH; ++s) r2[s] = mul2(decay2(mul2(d2, A22[s])), fma2(c2[s], y2, r2[s]));
       }
     }
     __syncthreads();
@@ -418,19 +550,24 @@ __global__ void __launch_bounds__(kScanThreads) scan_carry_kernel(ScanArgs a) {
   for (int o = 1; o < P; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (q.valid) {
     const int64_t at = ((int64_t)q.b * a.nseg + q.seg) * a.channels + q.d;
+#pragma unroll
+    for (int s = 0; s < kH; ++s) {
+      r[2 * s] = r2[s].x();
+      r[2 * s + 1] = r2[s].y();
+    }
     store_states<P>(a.seg_state + at * N, N, p, r);
     if (p == 0) a.seg_sum[at] = total;
   }
 }
 
-constexpr int kSub = 8;  // tokens whose states and decays a lane holds at a time
-
-template <int P>
+template <typename T, int P>
 struct BwdSmem {
   static constexpr int CB = kScanThreads / P, TT = ScanTile<P>::kBwd, NP = kS * P;
-  static constexpr int DP = TT + 4, kPitch = NP + 4, kPart = 2 * NP + 1;
-  static constexpr int kRows = CB * DP;                          // D, D u, dy each
-  static constexpr int kFloats = 3 * kRows + 2 * TT * kPitch + (kScanThreads / 32) * TT * kPart;
+  static constexpr int DP = TT + 4, kPart = 2 * NP + 1;
+  static constexpr int kRows = CB * DP;                          // D, D u, dy, and three sums over states
+  static constexpr int kStart = TT / kSub * kScanThreads * kS;   // states at the start of each run of kSub tokens
+  static constexpr int kBC = TileBC<T, P, TT>::kFloats;
+  static constexpr int kFloats = 6 * kRows + kStart + 2 * kBC + (kScanThreads / 32) * TT * kPart;
 };
 
 // Sums of v[0..7] over the lanes of a warp that hold the same states of
@@ -477,13 +614,13 @@ struct SumChannels {
 };
 
 template <typename T, int P>
-__global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs a) {
-  using S = BwdSmem<P>;
+__global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(ScanArgs a) {
+  using S = BwdSmem<T, P>;
   constexpr int TT = S::TT, E = TT >= P ? TT / P : 1, DP = S::DP, NP = S::NP;
   using BC = TileBC<T, P, TT>;
   extern __shared__ __align__(16) float smem[];
   float *s_d = smem, *s_x = s_d + S::kRows, *s_y = s_x + S::kRows;
-  float *s_B = s_y + S::kRows, *s_C = s_B + TT * S::kPitch, *s_part = s_C + TT * S::kPitch;
+  float *s_o = s_y + S::kRows, *s_start = s_o + 3 * S::kRows, *s_B = s_start + S::kStart, *s_C = s_B + S::kBC, *s_part = s_C + S::kBC;
   const ScanPlace<P> q(a);
   const int p = q.p, N = a.states, L = a.length, lane = threadIdx.x & 31;
   const T *u = static_cast<const T *>(a.u) + q.row * L, *dl = static_cast<const T *>(a.delta) + q.row * L;
@@ -494,15 +631,15 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs a)
   T *du = static_cast<T *>(a.du) + q.row * L, *ddl = static_cast<T *>(a.ddelta) + q.row * L;
   T *dz = a.z ? static_cast<T *>(a.dz) + q.row * L : nullptr;
   float *part = a.part_bc + (((int64_t)q.b * a.groups + q.g) * a.nblk + q.blk) * 2 * N * L;
-  const bool vec = (L * (int64_t)sizeof(T)) % Pack<T, E>::kVec == 0;
+  const bool vec = (L * (int64_t)sizeof(T)) % 16 == 0;
   const bool loads = p * E < TT;  // (more lanes than tokens of a tile)
   const float bias = a.bias ? a.bias[q.d] : 0.f, skip = a.skip ? a.skip[q.d] : 0.f;
-  float A2[kS], r[kS], dA[kS], dskip = 0.f, dbias = 0.f;
+  float A2[kS], r[kS], dskip = 0.f, dbias = 0.f;
   load_states<P>(a.A + (int64_t)q.d * N, N, p, A2);
 #pragma unroll
   for (int s = 0; s < kS; ++s) {
     A2[s] *= kLog2e;
-    r[s] = dA[s] = 0.f;
+    r[s] = 0.f;
   }
   if (a.grad_final) load_states<P>(a.grad_final + q.row * N, N, p, r);
   for (int i = a.nseg - 1; i > q.seg; --i) {
@@ -515,6 +652,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs a)
   }
   const int t_begin = q.seg * a.seg_len, t_stop = min(L, t_begin + a.seg_len), t_end = min(t_stop, q.len);
   float *row_d = s_d + q.c * DP, *row_x = s_x + q.c * DP, *row_y = s_y + q.c * DP;
+  float *row_sy = s_o + q.c * DP, *row_sb = row_sy + S::kRows, *row_sm = row_sb + S::kRows;
   float *my_part = s_part + (threadIdx.x / 32) * TT * S::kPart;
   Pack<T, E> nu, nd, ng, nz;
   BC nbc;
@@ -525,8 +663,15 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs a)
       load_row(ng, grad, t0 + p * E, t_end, vec);
       if (z) load_row(nz, z, t0 + p * E, t_end, vec);
     }
-    nbc.load(B, C, N, L, t0, t_end, true);
+    nbc.load(B, C, N, L, t0, t_end, vec, true);
   };
+  F2 A22[kH], r2[kH], dA2[kH];
+#pragma unroll
+  for (int s = 0; s < kH; ++s) {
+    A22[s] = F2(A2[2 * s], A2[2 * s + 1]);
+    r2[s] = F2(r[2 * s], r[2 * s + 1]);
+    dA2[s] = F2(0.f, 0.f);
+  }
   const int last_live = t_begin + (t_end - t_begin - 1) / TT * TT;
   if (t_begin < t_end) fetch(last_live);
   for (int t0 = t_begin + (t_stop - t_begin - 1) / TT * TT; t0 >= t_begin; t0 -= TT) {
@@ -553,10 +698,10 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs a)
         if (a.softplus) v = softplus_f(v);
         if (t0 + p * E + i >= t_end) v = 0.f;
         row_d[p * E + i] = v;
-        row_x[p * E + i] = v * cu.f(i);
         float dy = cg.f(i);
         if (z) dy *= cz.f(i) * sigmoid_f(cz.f(i));
         // a thread without a channel adds nothing to the sums over channels
+        row_x[p * E + i] = q.valid ? v * cu.f(i) : 0.f;
         row_y[p * E + i] = q.valid ? dy : 0.f;
       }
     }
@@ -564,64 +709,71 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs a)
     __syncthreads();
     if (t0 > t_begin) fetch(t0 - TT);
     // the states at the start of each run of kSub tokens
-    float start[TT / kSub][kS];
-    load_states<P>(a.ckpt + (((int64_t)q.b * ((L + TT - 1) / TT) + t0 / TT) * a.channels + q.d) * N, N, p, start[0]);
+    float *start = s_start + threadIdx.x * kS;
+    {
+      float h0[kS];
+      load_states<P>(a.ckpt + (((int64_t)q.b * ((L + TT - 1) / TT) + t0 / TT) * a.channels + q.d) * N, N, p, h0);
+      F2 h2[kH] = {F2(h0[0], h0[1]), F2(h0[2], h0[3])};
+      put_pairs(start, h2);
+#pragma unroll 1
+      for (int k = 1; k < TT / kSub; ++k) {
+        float dd[kSub], xx[kSub];
+        load8f(row_d + (k - 1) * kSub, dd);
+        load8f(row_x + (k - 1) * kSub, xx);
 #pragma unroll
-    for (int k = 1; k < TT / kSub; ++k) {
-      float h[kS];
+        for (int j = 0; j < kSub; ++j) {
+          F2 b2[kH];
+          load_pairs(s_B + BC::row8((k - 1) * kSub, j) + p * kS, b2);
+          const F2 d2(dd[j], dd[j]), x2(xx[j], xx[j]);
 #pragma unroll
-      for (int s = 0; s < kS; ++s) h[s] = start[k - 1][s];
-#pragma unroll
-      for (int j = 0; j < kSub; ++j) {
-        const int t = (k - 1) * kSub + j;
-        const float d = row_d[t], x = row_x[t];
-        const float4 b4 = *reinterpret_cast<const float4 *>(s_B + t * S::kPitch + p * kS);
-        const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-        for (int s = 0; s < kS; ++s) h[s] = fmaf(exp2_f(d * A2[s]), h[s], x * bb[s]);
-      }
-#pragma unroll
-      for (int s = 0; s < kS; ++s) start[k][s] = h[s];
-    }
-#pragma unroll
-    for (int k = TT / kSub - 1; k >= 0; --k) {
-      float h[kSub + 1][kS], dec[kSub][kS], y[kSub], s1[kSub], s2[kSub];
-#pragma unroll
-      for (int s = 0; s < kS; ++s) h[0][s] = start[k][s];
-#pragma unroll
-      for (int j = 0; j < kSub; ++j) {
-        const int t = k * kSub + j;
-        const float d = row_d[t], x = row_x[t];
-        const float4 b4 = *reinterpret_cast<const float4 *>(s_B + t * S::kPitch + p * kS);
-        const float4 c4 = *reinterpret_cast<const float4 *>(s_C + t * S::kPitch + p * kS);
-        const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-        for (int s = 0; s < kS; ++s) {
-          dec[j][s] = exp2_f(d * A2[s]);
-          h[j + 1][s] = fmaf(dec[j][s], h[j][s], x * bb[s]);
+          for (int s = 0; s < kH; ++s) h2[s] = fma2(decay2(mul2(d2, A22[s])), h2[s], mul2(x2, b2[s]));
         }
-        y[j] = fmaf(h[j + 1][0], c4.x, fmaf(h[j + 1][1], c4.y, fmaf(h[j + 1][2], c4.z, h[j + 1][3] * c4.w)));
+        put_pairs(start + k * kScanThreads * kS, h2);
+      }
+    }
+    F2 tile_dA[kH] = {F2(0.f, 0.f), F2(0.f, 0.f)};
+#pragma unroll 1
+    for (int k = TT / kSub - 1; k >= 0; --k) {
+      F2 h2[kSub + 1][kH], dec[kSub][kH];
+      float y[kSub], s1[kSub], s2[kSub], dd[kSub], xx[kSub], yy[kSub];
+      load8f(row_d + k * kSub, dd);
+      load8f(row_x + k * kSub, xx);
+      load8f(row_y + k * kSub, yy);
+      load_pairs(start + k * kScanThreads * kS, h2[0]);
+#pragma unroll
+      for (int j = 0; j < kSub; ++j) {
+        F2 b2[kH], c2[kH];
+        load_pairs(s_B + BC::row8(k * kSub, j) + p * kS, b2);
+        load_pairs(s_C + BC::row8(k * kSub, j) + p * kS, c2);
+        const F2 d2(dd[j], dd[j]), x2(xx[j], xx[j]);
+#pragma unroll
+        for (int s = 0; s < kH; ++s) {
+          dec[j][s] = decay2(mul2(d2, A22[s]));
+          h2[j + 1][s] = fma2(dec[j][s], h2[j][s], mul2(x2, b2[s]));
+        }
+        const F2 y2 = fma2(h2[j + 1][0], c2[0], mul2(h2[j + 1][1], c2[1]));
+        y[j] = y2.x() + y2.y();
       }
 #pragma unroll
       for (int j = kSub - 1; j >= 0; --j) {
         const int t = k * kSub + j;
-        const float d = row_d[t], x = row_x[t], dy = row_y[t];
-        const float4 b4 = *reinterpret_cast<const float4 *>(s_B + t * S::kPitch + p * kS);
-        const float4 c4 = *reinterpret_cast<const float4 *>(s_C + t * S::kPitch + p * kS);
-        const float bb[4] = {b4.x, b4.y, b4.z, b4.w}, cc[4] = {c4.x, c4.y, c4.z, c4.w};
-        float v[8];
-        s1[j] = s2[j] = 0.f;
+        F2 b2[kH], c2[kH], vb[kH], vc[kH], m2[kH], dh[kH];
+        load_pairs(s_B + BC::row8(k * kSub, j) + p * kS, b2);
+        load_pairs(s_C + BC::row8(k * kSub, j) + p * kS, c2);
+        const F2 d2(dd[j], dd[j]), x2(xx[j], xx[j]), dy2(yy[j], yy[j]);
 #pragma unroll
-        for (int s = 0; s < kS; ++s) {
-          const float dh = fmaf(dy, cc[s], r[s]);
-          v[s] = q.valid ? dh * x : 0.f;
-          v[4 + s] = dy * h[j + 1][s];
-          s1[j] = fmaf(dh, bb[s], s1[j]);
-          r[s] = dec[j][s] * dh;
-          const float m = r[s] * h[j][s];
-          s2[j] = fmaf(m, A2[s], s2[j]);
-          dA[s] = fmaf(m, d, dA[s]);
+        for (int s = 0; s < kH; ++s) {
+          dh[s] = fma2(dy2, c2[s], r2[s]);
+          vb[s] = mul2(dh[s], x2);
+          vc[s] = mul2(dy2, h2[j + 1][s]);
+          r2[s] = mul2(dec[j][s], dh[s]);
+          m2[s] = mul2(r2[s], h2[j][s]);
+          tile_dA[s] = fma2(m2[s], d2, tile_dA[s]);
         }
+        const F2 t1 = fma2(dh[0], b2[0], mul2(dh[1], b2[1])), t2 = fma2(m2[0], A22[0], mul2(m2[1], A22[1]));
+        s1[j] = t1.x() + t1.y();
+        s2[j] = t2.x() + t2.y();
+        float v[8] = {vb[0].x(), vb[0].y(), vb[1].x(), vb[1].y(), vc[0].x(), vc[0].y(), vc[1].x(), vc[1].y()};
         SumChannels<P>::sum(v, lane);
         if (SumChannels<P>::writes(lane)) {
           const int f = SumChannels<P>::first(lane);
@@ -632,19 +784,17 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs a)
           }
         }
       }
-      // the run's D, D u and dy have been read by all lanes: their places take
-      // the sums over the states
 #pragma unroll
       for (int j = 0; j < kSub; j += 4) {
-        const Sum4<P> sy(y[j], y[j + 1], y[j + 2], y[j + 3], p);
-        const Sum4<P> sb(s1[j], s1[j + 1], s1[j + 2], s1[j + 3], p);
-        const Sum4<P> sm(s2[j], s2[j + 1], s2[j + 2], s2[j + 3], p);
-        __syncwarp();
-        sm.put(row_d + k * kSub + j, p);
-        sb.put(row_x + k * kSub + j, p);
-        sy.put(row_y + k * kSub + j, p);
+        Sum4<P>(y[j], y[j + 1], y[j + 2], y[j + 3], p).put(row_sy + k * kSub + j, p);
+        Sum4<P>(s1[j], s1[j + 1], s1[j + 2], s1[j + 3], p).put(row_sb + k * kSub + j, p);
+        Sum4<P>(s2[j], s2[j + 1], s2[j + 2], s2[j + 3], p).put(row_sm + k * kSub + j, p);
       }
     }
+    // a tile's sum at a time: what a long sum of 32-bit numbers loses grows
+    // with the number of its terms
+#pragma unroll
+    for (int s = 0; s < kH; ++s) dA2[s] = add2(dA2[s], tile_dA[s]);
     __syncwarp();
     if (q.valid && loads) {
       Pack<T, E> ou, od, oz;
@@ -652,20 +802,20 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs a)
       for (int i = 0; i < E; ++i) {
         const bool live = t0 + p * E + i < t_end;
         const float raw = cd.f(i) + bias, uu = cu.f(i), g = cg.f(i);
-        const float d = a.softplus ? softplus_f(raw) : raw;
+        const float d = row_d[p * E + i];
         float gate = 1.f, slope = 0.f;
         if (z) {
           const float zz = cz.f(i), e = sigmoid_f(zz);
           gate = zz * e;
           slope = e * fmaf(zz, 1.f - e, 1.f);
         }
-        const float dy = g * gate, through = row_x[p * E + i];
-        float dd = fmaf(uu, through, row_d[p * E + i] * (1.f / kLog2e));
-        if (a.softplus && raw <= 20.f) dd *= sigmoid_f(raw);
+        const float dy = g * gate, through = row_sb[p * E + i];
+        float dd = fmaf(uu, through, row_sm[p * E + i] * (1.f / kLog2e));
+        if (a.softplus) dd *= softplus_slope(raw);
         if (!live) dd = 0.f;
         ou.v[i] = from_f<T>(live ? fmaf(d, through, skip * dy) : 0.f);
         od.v[i] = from_f<T>(dd);
-        if (z) oz.v[i] = from_f<T>(live ? g * slope * fmaf(skip, uu, row_y[p * E + i]) : 0.f);
+        if (z) oz.v[i] = from_f<T>(live ? g * slope * fmaf(skip, uu, row_sy[p * E + i]) : 0.f);
         dskip = fmaf(dy, uu, dskip);
         dbias += dd;
       }
@@ -693,6 +843,8 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs a)
     dbias += __shfl_xor_sync(0xffffffffu, dbias, o);
   }
   if (q.valid) {
+    const float dA[kS] = {dA2[0].x(), dA2[0].y(), dA2[1].x(), dA2[1].y()};
+    const float rr[kS] = {r2[0].x(), r2[0].y(), r2[1].x(), r2[1].y()};
     float *par = a.part_par + ((int64_t)q.b * a.nseg + q.seg) * a.channels * (N + 2);
 #pragma unroll
     for (int s = 0; s < kS; ++s)
@@ -701,7 +853,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs a)
       par[(int64_t)a.channels * N + q.d] = dskip;
       par[(int64_t)a.channels * (N + 1) + q.d] = dbias;
     }
-    if (a.dinit && q.seg == 0) store_states<P>(a.dinit + q.row * N, N, p, r);
+    if (a.dinit && q.seg == 0) store_states<P>(a.dinit + q.row * N, N, p, rr);
   }
 }
 
@@ -952,7 +1104,7 @@ extern "C" int pc2d_ssm_scan_forward(int dtype, const void *u, const void *delta
     return PC2D_ERR_INVALID_ARGUMENT;
   }
   if ((st = check_aligned("pc2d_ssm_scan_forward",
-                          {u, delta, z, output, initial_state, final_state, checkpoints, A})) != PC2D_OK)
+                          {u, delta, z, B, C, output, initial_state, final_state, checkpoints, A})) != PC2D_OK)
     return st;
   ScanArgs a = scan_problem(batch, channels, length, states, groups);
   scan_split<false>(&a);
@@ -1004,7 +1156,7 @@ extern "C" int pc2d_ssm_scan_backward(int dtype, const void *grad, const float *
     set_last_error("pc2d_ssm_scan_backward: null pointer");
     return PC2D_ERR_INVALID_ARGUMENT;
   }
-  if ((st = check_aligned("pc2d_ssm_scan_backward", {grad, u, delta, z, ugrad, deltagrad, zgrad, checkpoints,
+  if ((st = check_aligned("pc2d_ssm_scan_backward", {grad, u, delta, z, B, C, ugrad, deltagrad, zgrad, checkpoints,
                                                      grad_final, initialgrad, A})) != PC2D_OK)
     return st;
   ScanArgs a = scan_problem(batch, channels, length, states, groups);
@@ -1026,7 +1178,7 @@ extern "C" int pc2d_ssm_scan_backward(int dtype, const void *grad, const float *
     using T = decltype(t);
     constexpr int P = decltype(p)::value;
     if (grid > 0) {
-      constexpr int bytes = BwdSmem<P>::kFloats * 4;
+      constexpr int bytes = BwdSmem<T, P>::kFloats * 4;
       // one bit per instance: 3 types x 6 lane counts
       int bit = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 1 : 2;
       for (int i = P; i > 1; i >>= 1) bit += 3;
