@@ -45,18 +45,26 @@
 namespace pc2d {
 namespace {
 
-constexpr int kScanThreads = 128;
-constexpr int kS = 4;    // states per lane
-constexpr int kSub = 8;  // tokens of an inner run
+constexpr int kS = 4, kH = kS / 2;  // states per lane, and pairs of them (packed registers)
+constexpr int kRun = 8;             // tokens of an inner run
+constexpr int kThreads = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Tile lengths by the lanes per channel: shared memory and the elements a
-// thread loads per tile bound them.  A forward tile holds whole backward ones.
-template <int P>
-struct ScanTile {
-  static constexpr int kFwd = P == 1 ? 16 : P == 2 ? 32 : P <= 8 ? 64 : 32;
-  static constexpr int kBwd = P <= 2 ? 16 : P <= 8 ? 32 : 16;
+// How a block is laid out: P lanes per channel, and the tiles' lengths.  A
+// forward tile holds whole backward ones.  kMany: for grids that fill the GPU
+// several times, registers for four blocks per SM and a shorter tile; else for
+// two, which the compiler spends on overlapping more of a run (16384 tokens of
+// 2048 channels in 9 segments: 293 against 351 us; 4 x 2048 tokens of 2048
+// channels, 1.7 blocks per SM: 225 against 198 us).
+template <int P_, bool kMany_ = false>
+struct Layout {
+  static constexpr bool kMany = kMany_;
+  static constexpr int P = P_, NP = kS * P, CB = kThreads / P;
+  static constexpr int TF = P == 1 ? 16 : P == 2 || P >= 16 || kMany ? 32 : 64;
+  static constexpr int TB = P == 1 || P >= 16 ? 16 : 32;
+  static constexpr int kFwdBlocks = P >= 16 ? 2 : kMany ? 4 : 2;
 };
+constexpr int kBwdBlocks = 2;
 inline int lanes_of(int states) {
   int p = 1;
   while (p * kS < states) p *= 2;
@@ -64,7 +72,7 @@ inline int lanes_of(int states) {
 }
 inline int bwd_tile_of(int states) {
   const int p = lanes_of(states);
-  return p <= 2 ? 16 : p <= 8 ? 32 : 16;
+  return p == 1 || p >= 16 ? 16 : 32;
 }
 
 struct ScanArgs {
@@ -85,7 +93,9 @@ struct ScanArgs {
   void *du, *ddelta, *dz;
   float *dinit;
   float *part_bc;      // [batch][groups][nblk][2 states][length]: dB, then dC
-  float *part_par;     // [batch * nseg][channels * (states + 2)]: dA, dskip, dbias
+  float *part_par;     // [batch * nseg][par_stride]: dA, dskip, dbias
+  // rows of dA, dskip and dbias start on a 16-byte boundary
+  __host__ __device__ int64_t par_stride() const { return ((int64_t)channels * (states + 2) + 3) / 4 * 4; }
 };
 
 __device__ __forceinline__ float exp2_f(float v) {
@@ -129,33 +139,53 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   return r;
 }
 
-// exp2 of two arguments, the decays of two states.  The hardware exponential
-// is off by up to 2.4 units of 2^-24 and, on average over its table, low by
-// 0.3 to 0.8 (measured on [-2, 0]): a state that decays slowly adds the same
-// bias up over as many steps as it remembers.  So arguments below 1/8, where a
-// state remembers more than 11 steps, take 1 + x q(x) with the interpolation of
-// (2^x - 1)/x at the four Chebyshev nodes of [-1/8, 1/8] as q: one rounding
-// (0.5 units, no bias).  The other arguments, NaN and the infinities take the
-// hardware's.
-__device__ __forceinline__ F2 decay2(F2 x) {
-  const F2 one(1.f, 1.f);
-  F2 q = fma2(F2(0.009620536f, 0.009620536f), x, F2(0.055524945f, 0.055524945f));
-  q = fma2(q, x, F2(0.2402265f, 0.2402265f));
-  q = fma2(q, x, F2(0.6931471f, 0.6931471f));
-  q = fma2(q, x, one);
-  const float x0 = x.x(), x1 = x.y();
-  return F2(fabsf(x0) < 0.125f ? q.x() : exp2_f(x0), fabsf(x1) < 0.125f ? q.y() : exp2_f(x1));
+// Decays.  The hardware exponential is off by up to 2.4 units of 2^-24 and, on
+// average over its table, low by 0.1 to 0.8 of one (measured on [-2, 0]).  A
+// state that decays slowly would add that bias up over all the tokens it
+// remembers, a thousand or more.  So each tile of up to 32 tokens ends with a
+// correction: the product of the decays that were used is replaced by exp of
+// the tile's sum, for the state that entered the tile,
+//   h += h_entry (exp2(A2 sum d) - prod decays),
+// and the bias no longer grows beyond a tile.  exp2_tile, for that one value a
+// tile, takes 1 + x q(x) for |x| < 1/8 with the interpolation of (2^x - 1)/x at
+// the four Chebyshev nodes of [-1/8, 1/8] as q (no bias where many tiles are
+// remembered), else the hardware's.
+__device__ __forceinline__ F2 exp2_2(F2 x) { return F2(exp2_f(x.x()), exp2_f(x.y())); }
+__device__ __forceinline__ float exp2_tile(float x) {
+  float q = fmaf(0.009620536f, x, 0.055524945f);
+  q = fmaf(q, x, 0.2402265f);
+  q = fmaf(q, x, 0.6931471f);
+  return fabsf(x) < 0.125f ? fmaf(q, x, 1.f) : exp2_f(x);
 }
-constexpr int kH = kS / 2;  // pairs of states per lane
-// Two pairs from 16 aligned bytes of shared memory.
-__device__ __forceinline__ void load_pairs(const float *p, F2 *f) {
+// exp2(x) - prod; 0 for a growing state, whose product may have overflowed.
+__device__ __forceinline__ float tile_gap(float x, float prod) {
+  return x <= 0.f ? exp2_tile(x) - prod : 0.f;
+}
+__device__ __forceinline__ F2 tile_gap2(F2 x, F2 prod) {
+  return F2(tile_gap(x.x(), prod.x()), tile_gap(x.y(), prod.y()));
+}
+
+// Two pairs from, and to, 16 aligned bytes.
+__device__ __forceinline__ void load_pairs(const float *p, F2 (&f)[kH]) {
   const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(p);
   f[0].v = q.x;
   f[1].v = q.y;
 }
-
-__device__ __forceinline__ void put_pairs(float *p, const F2 *f) {
+__device__ __forceinline__ void put_pairs(float *p, const F2 (&f)[kH]) {
   *reinterpret_cast<ulonglong2 *>(p) = make_ulonglong2(f[0].v, f[1].v);
+}
+// sum of a[i] b[i] over a lane's states
+__device__ __forceinline__ float dot(const F2 (&a)[kH], const F2 (&b)[kH]) {
+  const F2 s = fma2(a[1], b[1], mul2(a[0], b[0]));
+  return s.x() + s.y();
+}
+template <int n>
+__device__ __forceinline__ void load_row_f(const float *p, float (&v)[n]) {
+#pragma unroll
+  for (int i = 0; i < n; i += 4) {
+    const float4 a = *reinterpret_cast<const float4 *>(p + i);
+    v[i] = a.x, v[i + 1] = a.y, v[i + 2] = a.z, v[i + 3] = a.w;
+  }
 }
 
 // softplus(v) = max(v, 0) + log(1 + e) with e = exp(-|v|), and its slope.
@@ -183,13 +213,6 @@ __device__ __forceinline__ float softplus_slope(float v) {
   const float e = exp_neg_abs(v);
   return __fdividef(v < 0.f ? e : 1.f, 1.f + e);
 }
-// Eight floats of a row, from a 16-byte boundary.
-__device__ __forceinline__ void load8f(const float *p, float *v) {
-  const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-  v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-
 // Sums of v0..v3 over the P lanes of a channel.  P >= 4: lane p ends with
 // that of v[p % 4]; P = 2: with those of v[p] and v[p + 2]; P = 1: all four.
 template <int P>
@@ -245,55 +268,110 @@ __device__ __forceinline__ void store_row(const Pack<T, E> &v, T *row, int t, in
   }
 }
 
-// A block's tile of B and C: loaded along the length by vectors, kept as
-// [t][n].  Rows are NP floats, and 4 more after every kVec of them, so that the
-// lanes of a warp, which store the same element of their vectors, meet
-// different banks.
-template <typename T, int P, int TT>
-struct TileBC {
-  static constexpr int NP = kS * P, kCount = NP * TT;
-  static constexpr int kEach = kCount / kScanThreads > 0 ? kCount / kScanThreads : 1;
-  static constexpr int kVec = kEach * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : kEach;
-  static constexpr int kNum = kEach / kVec;
-  static constexpr int kFloats = TT * NP + TT / kVec * 4;
-  __device__ static __forceinline__ int row(int t) { return t * NP + t / kVec * 4; }
-  // row(t + j) for t a multiple of 8 and a constant j < 8
-  __device__ static __forceinline__ int row8(int t, int j) { return t * NP + t / kVec * 4 + j * NP + j / kVec * 4; }
-  Pack<T, kVec> b[kNum], c[kNum];
-  __device__ __forceinline__ void load(const T *B, const T *C, int states, int length, int t0, int end, bool vec,
-                                       bool with_c) {
+// A lane's four values of B or C as they lie in shared memory.
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+  F2 f[kH];
+  __device__ __forceinline__ void unpack(F2 (&o)[kH]) const {
+    o[0] = f[0];
+    o[1] = f[1];
+  }
+};
+template <>
+struct Four<__half> {
+  __half2 h[kH];
+  __device__ __forceinline__ void unpack(F2 (&o)[kH]) const {
 #pragma unroll
-    for (int i = 0; i < kNum; ++i) {
-      const int e = (i * kScanThreads + threadIdx.x) * kVec, n = e / TT, t = t0 + e % TT;
-      const int stop = n < states && e < kCount ? end : t;  // nothing to read for missing states
-      load_row(b[i], B + (int64_t)n * length, t, stop, vec);
-      if (with_c) load_row(c[i], C + (int64_t)n * length, t, stop, vec);
+    for (int i = 0; i < kH; ++i) {
+      const float2 v = __half22float2(h[i]);
+      o[i] = F2(v.x, v.y);
     }
   }
-  __device__ __forceinline__ void put(float *sB, float *sC, bool with_c) const {
+};
+template <>
+struct Four<__nv_bfloat16> {
+  unsigned w[kH];
+  __device__ __forceinline__ void unpack(F2 (&o)[kH]) const {
+#pragma unroll
+    for (int i = 0; i < kH; ++i) o[i] = F2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+};
+
+// A block's tile of B and C, loaded along the length by vectors and kept in
+// their own type, a token a row: for each lane its four values of B, then of C,
+// which it takes in one read (two for float).  The rows of a vector's tokens
+// are followed by 16 bytes, so that the lanes of a warp, which store the same
+// element of their vectors, meet different banks.
+template <typename T, class G, int TT>
+struct TileBC {
+  static constexpr int NP = G::NP, kCount = NP * TT;
+  static constexpr int kEach = kCount / kThreads > 0 ? kCount / kThreads : 1;
+  static constexpr int kVec = kEach * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : kEach;
+  static constexpr int kNum = kEach / kVec;
+  static constexpr int kPad = 16 / (int)sizeof(T), kElems = TT * 2 * NP + TT / kVec * kPad;
+  static constexpr int kFloats = (kElems * (int)sizeof(T) + 3) / 4;
+  __device__ static __forceinline__ int row(int t) { return t * 2 * NP + t / kVec * kPad; }
+  // row(t + j) for t a multiple of n and a constant j < n
+  template <int n>
+  __device__ static __forceinline__ int row_in(int t, int j) {
+    return kVec < n ? row(t) + j * 2 * NP + j / kVec * kPad : row(t) + j * 2 * NP;
+  }
+  Pack<T, kVec> b[kNum], c[kNum];
+  __device__ __forceinline__ void load(const T *B, const T *C, int states, int length, int t0, int end, bool vec) {
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
-      const int e = (i * kScanThreads + threadIdx.x) * kVec, n = e / TT, t = e % TT;
+      const int e = (i * kThreads + threadIdx.x) * kVec, n = e / TT, t = t0 + e % TT;
+      const int stop = n < states && e < kCount ? end : t;  // nothing to read for missing states
+      load_row(b[i], B + (int64_t)n * length, t, stop, vec);
+      if (C) load_row(c[i], C + (int64_t)n * length, t, stop, vec);
+    }
+  }
+  __device__ __forceinline__ void put(T *tile, bool with_c) const {
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) {
+      const int e = (i * kThreads + threadIdx.x) * kVec, n = e / TT, t = e % TT;
       if (e < kCount) {
+        T *dst = tile + row(t) + n / kS * (2 * kS) + n % kS;
 #pragma unroll
         for (int k = 0; k < kVec; ++k) {
-          sB[row(t) + k * NP + n] = b[i].f(k);
-          if (with_c) sC[row(t) + k * NP + n] = c[i].f(k);
+          dst[k * 2 * NP] = b[i].v[k];
+          if (with_c) dst[k * 2 * NP + kS] = c[i].v[k];
         }
       }
     }
   }
+  struct alignas(16) Both {
+    Four<T> b, c;
+  };
+  // the first of a lane's two; both
+  __device__ static __forceinline__ Four<T> first(const T *tile, int at, int p) {
+    Four<T> r;
+    const T *src = tile + at + p * 2 * kS;
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(&r) = *reinterpret_cast<const uint4 *>(src);
+    else *reinterpret_cast<uint2 *>(&r) = *reinterpret_cast<const uint2 *>(src);
+    return r;
+  }
+  __device__ static __forceinline__ Both both(const T *tile, int at, int p) {
+    Both r;
+    const T *src = tile + at + p * 2 * kS;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(Both) / 16; ++i)
+      reinterpret_cast<uint4 *>(&r)[i] = reinterpret_cast<const uint4 *>(src)[i];
+    return r;
+  }
 };
 
 // What a thread is: lane p of a channel, in a segment of the length.
-template <int P>
+template <class G>
 struct ScanPlace {
   int p, c, d, b, g, blk, seg, len;
   bool valid;
   int64_t row;   // batch row * channels + channel
   __device__ __forceinline__ ScanPlace(const ScanArgs &a) {
-    p = threadIdx.x % P;
-    c = threadIdx.x / P;
+    p = threadIdx.x % G::P;
+    c = threadIdx.x / G::P;
     int i = blockIdx.x;
     seg = i % a.nseg;
     i /= a.nseg;
@@ -301,7 +379,7 @@ struct ScanPlace {
     i /= a.nblk;
     g = i % a.groups;
     b = i / a.groups;
-    const int in_group = blk * (kScanThreads / P) + c;
+    const int in_group = blk * G::CB + c;
     valid = in_group < a.per_group;
     // a thread without a channel computes on its group's last one and writes nothing
     d = g * a.per_group + (valid ? in_group : a.per_group - 1);
@@ -311,57 +389,67 @@ struct ScanPlace {
   }
 };
 
-template <int P>
-__device__ __forceinline__ void load_states(const float *src, int states, int p, float *h) {
+// A lane's states of a channel's row of them (0 for those beyond the last).
+__device__ __forceinline__ void load_states(const float *src, int states, int p, F2 (&h)[kH]) {
 #pragma unroll
-  for (int s = 0; s < kS; ++s) h[s] = p * kS + s < states ? src[p * kS + s] : 0.f;
+  for (int s = 0; s < kH; ++s) {
+    const int n = p * kS + 2 * s;
+    h[s] = F2(n < states ? src[n] : 0.f, n + 1 < states ? src[n + 1] : 0.f);
+  }
 }
-template <int P>
-__device__ __forceinline__ void store_states(float *dst, int states, int p, const float *h) {
+__device__ __forceinline__ void store_states(float *dst, int states, int p, const F2 (&h)[kH]) {
   if (states % kS == 0) {
     // (rows of a multiple of four states in a 16-byte aligned array)
-    if (p * kS < states) *reinterpret_cast<float4 *>(dst + p * kS) = make_float4(h[0], h[1], h[2], h[3]);
+    if (p * kS < states) put_pairs(dst + p * kS, h);
   } else {
 #pragma unroll
-    for (int s = 0; s < kS; ++s)
-      if (p * kS + s < states) dst[p * kS + s] = h[s];
+    for (int s = 0; s < kH; ++s) {
+      const int n = p * kS + 2 * s;
+      if (n < states) dst[n] = h[s].x();
+      if (n + 1 < states) dst[n + 1] = h[s].y();
+    }
   }
+}
+__device__ __forceinline__ void load_decay_rates(const ScanArgs &a, int d, int p, F2 (&A2)[kH]) {
+  load_states(a.A + (int64_t)d * a.states, a.states, p, A2);
+#pragma unroll
+  for (int s = 0; s < kH; ++s) A2[s] = mul2(A2[s], F2(kLog2e, kLog2e));
 }
 
 // Forward pass; kStateOnly: the first pass over segments (end state from zero
 // and sum of D_t, no outputs).
-template <typename T, int P, bool kStateOnly>
-__global__ void __launch_bounds__(kScanThreads, P <= 8 ? 4 : 2) scan_forward_kernel(ScanArgs a) {
-  constexpr int CB = kScanThreads / P, TT = ScanTile<P>::kFwd, E = TT / P, TB = ScanTile<P>::kBwd;
-  constexpr int DP = TT + 4;
-  using BC = TileBC<T, P, TT>;
-  __shared__ __align__(16) float s_d[CB * DP], s_x[CB * DP], s_o[kStateOnly ? 4 : CB * DP], s_B[BC::kFloats],
-      s_C[kStateOnly ? 4 : BC::kFloats];
-  const ScanPlace<P> q(a);
+template <typename T, class G, bool kStateOnly>
+__global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_forward_kernel(ScanArgs a) {
+  constexpr int P = G::P, TT = G::TF, TB = G::TB, E = TT / P, DP = TT + 4;
+  using BC = TileBC<T, G, TT>;
+  __shared__ __align__(16) float s_d[G::CB * DP], s_x[G::CB * DP], s_o[kStateOnly ? 4 : G::CB * DP];
+  __shared__ __align__(16) T s_bc[BC::kElems];
+  const ScanPlace<G> q(a);
   const int p = q.p, N = a.states, L = a.length;
   const T *u = static_cast<const T *>(a.u) + q.row * L, *dl = static_cast<const T *>(a.delta) + q.row * L;
   const T *z = a.z ? static_cast<const T *>(a.z) + q.row * L : nullptr;
   const int64_t bg = ((int64_t)q.b * a.groups + q.g) * N * L;
-  const T *B = static_cast<const T *>(a.B) + bg, *C = static_cast<const T *>(a.C) + bg;
+  const T *B = static_cast<const T *>(a.B) + bg, *C = kStateOnly ? nullptr : static_cast<const T *>(a.C) + bg;
   T *out = static_cast<T *>(a.out) + q.row * L;
   const bool vec = (L * (int64_t)sizeof(T)) % 16 == 0;
   const float bias = a.bias ? a.bias[q.d] : 0.f, skip = a.skip ? a.skip[q.d] : 0.f;
-  float A2[kS], h[kS];
-  load_states<P>(a.A + (int64_t)q.d * N, N, p, A2);
-#pragma unroll
-  for (int s = 0; s < kS; ++s) A2[s] *= kLog2e;
   const int t_begin = q.seg * a.seg_len, t_stop = min(L, t_begin + a.seg_len), t_end = min(t_stop, q.len);
+  F2 A2[kH], h[kH];
+  load_decay_rates(a, q.d, p, A2);
 #pragma unroll
-  for (int s = 0; s < kS; ++s) h[s] = 0.f;
+  for (int s = 0; s < kH; ++s) h[s] = F2(0.f, 0.f);
   if (!kStateOnly) {
-    if (a.init) load_states<P>(a.init + q.row * N, N, p, h);
+    if (a.init) load_states(a.init + q.row * N, N, p, h);
     for (int i = 0; i < q.seg; ++i) {
-      float e[kS];
+      F2 e[kH];
       const int64_t at = ((int64_t)q.b * a.nseg + i) * a.channels + q.d;
-      load_states<P>(a.seg_state + at * N, N, p, e);
+      load_states(a.seg_state + at * N, N, p, e);
       const float sum = a.seg_sum[at];
 #pragma unroll
-      for (int s = 0; s < kS; ++s) h[s] = fmaf(exp2_f(sum * A2[s]), h[s], e[s]);
+      for (int s = 0; s < kH; ++s) {
+        const F2 x = mul2(F2(sum, sum), A2[s]);
+        h[s] = fma2(F2(exp2_tile(x.x()), exp2_tile(x.y())), h[s], e[s]);
+      }
     }
   }
   float total = 0.f;
@@ -372,14 +460,8 @@ __global__ void __launch_bounds__(kScanThreads, P <= 8 ? 4 : 2) scan_forward_ker
     load_row(nu, u, t0 + p * E, t_end, vec);
     load_row(nd, dl, t0 + p * E, t_end, vec);
     if (!kStateOnly && z) load_row(nz, z, t0 + p * E, t_end, vec);
-    nbc.load(B, C, N, L, t0, t_end, vec, !kStateOnly);
+    nbc.load(B, C, N, L, t0, t_end, vec);
   };
-  F2 A22[kH], h2[kH];
-#pragma unroll
-  for (int s = 0; s < kH; ++s) {
-    A22[s] = F2(A2[2 * s], A2[2 * s + 1]);
-    h2[s] = F2(h[2 * s], h[2 * s + 1]);
-  }
   if (t_begin < t_end) fetch(t_begin);
   for (int t0 = t_begin; t0 < t_stop; t0 += TT) {
     if (t0 >= t_end) {  // nothing but padding from here on
@@ -399,42 +481,56 @@ __global__ void __launch_bounds__(kScanThreads, P <= 8 ? 4 : 2) scan_forward_ker
       if (t0 + p * E + i >= t_end) v = 0.f;
       row_d[p * E + i] = v;
       row_x[p * E + i] = v * cu.f(i);
-      if (kStateOnly) total += v;
     }
-    nbc.put(s_B, s_C, !kStateOnly);
+    nbc.put(s_bc, !kStateOnly);
     __syncthreads();
     if (t0 + TT < t_end) fetch(t0 + TT);
 #pragma unroll 1
     for (int tb = 0; tb < TT; tb += TB) {
-      if (!kStateOnly && a.ckpt && t0 + tb < t_end && q.valid) {
-        const float now[kS] = {h2[0].x(), h2[0].y(), h2[1].x(), h2[1].y()};
-        store_states<P>(a.ckpt + (((int64_t)q.b * ((L + TB - 1) / TB) + (t0 + tb) / TB) * a.channels + q.d) * N, N, p,
-                        now);
+      if (!kStateOnly && a.ckpt && t0 + tb < t_end && q.valid)
+        store_states(a.ckpt + (((int64_t)q.b * ((L + TB - 1) / TB) + (t0 + tb) / TB) * a.channels + q.d) * N, N, p, h);
+      F2 entry[kH], prod[kH];
+      float sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < kH; ++s) {
+        entry[s] = h[s];
+        prod[s] = F2(1.f, 1.f);
       }
 #pragma unroll 1
-      for (int t = tb; t < tb + TB; t += kSub) {
-        float y[kSub], dd[kSub], xx[kSub];
-        load8f(row_d + t, dd);
-        load8f(row_x + t, xx);
+      for (int t = tb; t < tb + TB; t += kRun) {
+        float y[kRun], dd[kRun], xx[kRun];
+        load_row_f(row_d + t, dd);
+        load_row_f(row_x + t, xx);
 #pragma unroll
-        for (int j = 0; j < kSub; ++j) {
-          F2 b2[kH];
-          load_pairs(s_B + BC::row8(t, j) + p * kS, b2);
+        for (int j = 0; j < kRun; ++j) {
+          F2 b[kH];
           const F2 d2(dd[j], dd[j]), x2(xx[j], xx[j]);
+          const int at = BC::template row_in<kRun>(t, j);
+          typename BC::Both bc;
+          if (kStateOnly) bc.b = BC::first(s_bc, at, p);
+          else bc = BC::both(s_bc, at, p);
+          bc.b.unpack(b);
+          sum += dd[j];
 #pragma unroll
-          for (int s = 0; s < kH; ++s) h2[s] = fma2(decay2(mul2(d2, A22[s])), h2[s], mul2(x2, b2[s]));
+          for (int s = 0; s < kH; ++s) {
+            const F2 dec = exp2_2(mul2(d2, A2[s]));
+            prod[s] = mul2(prod[s], dec);
+            h[s] = fma2(dec, h[s], mul2(x2, b[s]));
+          }
           if (!kStateOnly) {
-            F2 c2[kH];
-            load_pairs(s_C + BC::row8(t, j) + p * kS, c2);
-            const F2 y2 = fma2(h2[0], c2[0], mul2(h2[1], c2[1]));
-            y[j] = y2.x() + y2.y();
+            F2 c[kH];
+            bc.c.unpack(c);
+            y[j] = dot(h, c);
           }
         }
         if (!kStateOnly) {
 #pragma unroll
-          for (int j = 0; j < kSub; j += 4) Sum4<P>(y[j], y[j + 1], y[j + 2], y[j + 3], p).put(row_o + t + j, p);
+          for (int j = 0; j < kRun; j += 4) Sum4<P>(y[j], y[j + 1], y[j + 2], y[j + 3], p).put(row_o + t + j, p);
         }
       }
+#pragma unroll
+      for (int s = 0; s < kH; ++s) h[s] = fma2(entry[s], tile_gap2(mul2(F2(sum, sum), A2[s]), prod[s]), h[s]);
+      total += sum;
     }
     if (!kStateOnly) {
       __syncwarp();
@@ -452,65 +548,49 @@ __global__ void __launch_bounds__(kScanThreads, P <= 8 ? 4 : 2) scan_forward_ker
     }
     __syncthreads();
   }
-#pragma unroll
-  for (int s = 0; s < kH; ++s) {
-    h[2 * s] = h2[s].x();
-    h[2 * s + 1] = h2[s].y();
-  }
   if (kStateOnly) {
-#pragma unroll
-    for (int o = 1; o < P; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (q.valid) {
       const int64_t at = ((int64_t)q.b * a.nseg + q.seg) * a.channels + q.d;
-      store_states<P>(a.seg_state + at * N, N, p, h);
+      store_states(a.seg_state + at * N, N, p, h);
       if (p == 0) a.seg_sum[at] = total;
     }
   } else if (a.final_state && q.seg == a.nseg - 1 && q.valid) {
-    store_states<P>(a.final_state + q.row * N, N, p, h);
+    store_states(a.final_state + q.row * N, N, p, h);
   }
 }
 
 // First pass of the backward over segments: r from zero behind the segment,
 // and the sum of D_t.
-template <typename T, int P>
-__global__ void __launch_bounds__(kScanThreads, P <= 8 ? 4 : 2) scan_carry_kernel(ScanArgs a) {
-  constexpr int CB = kScanThreads / P, TT = ScanTile<P>::kBwd, E = TT >= P ? TT / P : 1;
-  constexpr int DP = TT + 4;
-  using BC = TileBC<T, P, TT>;
-  __shared__ __align__(16) float s_d[CB * DP], s_y[CB * DP], s_C[BC::kFloats];
-  const ScanPlace<P> q(a);
+template <typename T, class G>
+__global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_carry_kernel(ScanArgs a) {
+  constexpr int P = G::P, TT = G::TB, E = TT >= P ? TT / P : 1, DP = TT + 4;
+  using BC = TileBC<T, G, TT>;
+  __shared__ __align__(16) float s_d[G::CB * DP], s_y[G::CB * DP];
+  __shared__ __align__(16) T s_c[BC::kElems];
+  const ScanPlace<G> q(a);
   const int p = q.p, N = a.states, L = a.length;
   const T *dl = static_cast<const T *>(a.delta) + q.row * L, *grad = static_cast<const T *>(a.grad) + q.row * L;
   const T *z = a.z ? static_cast<const T *>(a.z) + q.row * L : nullptr;
   const T *C = static_cast<const T *>(a.C) + ((int64_t)q.b * a.groups + q.g) * N * L;
   const bool vec = (L * (int64_t)sizeof(T)) % 16 == 0;
   const float bias = a.bias ? a.bias[q.d] : 0.f;
-  float A2[kS], r[kS];
-  load_states<P>(a.A + (int64_t)q.d * N, N, p, A2);
+  F2 A2[kH], r[kH];
+  load_decay_rates(a, q.d, p, A2);
 #pragma unroll
-  for (int s = 0; s < kS; ++s) {
-    A2[s] *= kLog2e;
-    r[s] = 0.f;
-  }
+  for (int s = 0; s < kH; ++s) r[s] = F2(0.f, 0.f);
   const int t_begin = q.seg * a.seg_len, t_end = min(min(L, t_begin + a.seg_len), q.len);
   float total = 0.f;
   float *row_d = s_d + q.c * DP, *row_y = s_y + q.c * DP;
   Pack<T, E> nd, ng, nz;
-  BC nbc;
+  BC nc;
   auto fetch = [&](int t0) {
     if (p * E < TT) {
       load_row(nd, dl, t0 + p * E, t_end, vec);
       load_row(ng, grad, t0 + p * E, t_end, vec);
       if (z) load_row(nz, z, t0 + p * E, t_end, vec);
     }
-    nbc.load(C, nullptr, N, L, t0, t_end, vec, false);
+    nc.load(C, nullptr, N, L, t0, t_end, vec);
   };
-  F2 A22[kH], r2[kH];
-#pragma unroll
-  for (int s = 0; s < kH; ++s) {
-    A22[s] = F2(A2[2 * s], A2[2 * s + 1]);
-    r2[s] = F2(0.f, 0.f);
-  }
   const int last = t_begin + (t_end - t_begin - 1) / TT * TT;
   if (t_begin < t_end) fetch(last);
   for (int t0 = last; t0 >= t_begin && t_begin < t_end; t0 -= TT) {
@@ -521,53 +601,61 @@ __global__ void __launch_bounds__(kScanThreads, P <= 8 ? 4 : 2) scan_carry_kerne
         if (a.softplus) v = softplus_f(v);
         if (t0 + p * E + i >= t_end) v = 0.f;
         row_d[p * E + i] = v;
-        total += v;
         float dy = ng.f(i);
         if (z) dy *= nz.f(i) * sigmoid_f(nz.f(i));
         row_y[p * E + i] = dy;
       }
     }
-    nbc.put(s_C, nullptr, false);
+    nc.put(s_c, false);
     __syncthreads();
     if (t0 > t_begin) fetch(t0 - TT);
-#pragma unroll 1
-    for (int t = TT - kSub; t >= 0; t -= kSub) {
-      float dd[kSub], yy[kSub];
-      load8f(row_d + t, dd);
-      load8f(row_y + t, yy);
-#pragma unroll
-      for (int j = kSub - 1; j >= 0; --j) {
-        F2 c2[kH];
-        load_pairs(s_C + BC::row8(t, j) + p * kS, c2);
-        const F2 d2(dd[j], dd[j]), y2(yy[j], yy[j]);
-#pragma unroll
-        for (int s = 0; s < kH; ++s) r2[s] = mul2(decay2(mul2(d2, A22[s])), fma2(c2[s], y2, r2[s]));
-      }
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int o = 1; o < P; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (q.valid) {
-    const int64_t at = ((int64_t)q.b * a.nseg + q.seg) * a.channels + q.d;
+    F2 entry[kH], prod[kH];
+    float sum = 0.f;
 #pragma unroll
     for (int s = 0; s < kH; ++s) {
-      r[2 * s] = r2[s].x();
-      r[2 * s + 1] = r2[s].y();
+      entry[s] = r[s];
+      prod[s] = F2(1.f, 1.f);
     }
-    store_states<P>(a.seg_state + at * N, N, p, r);
+#pragma unroll 1
+    for (int t = TT - kRun; t >= 0; t -= kRun) {
+      float dd[kRun], yy[kRun];
+      load_row_f(row_d + t, dd);
+      load_row_f(row_y + t, yy);
+#pragma unroll
+      for (int j = kRun - 1; j >= 0; --j) {
+        F2 c[kH];
+        BC::first(s_c, BC::template row_in<kRun>(t, j), p).unpack(c);
+        const F2 d2(dd[j], dd[j]), y2(yy[j], yy[j]);
+        sum += dd[j];
+#pragma unroll
+        for (int s = 0; s < kH; ++s) {
+          const F2 dec = exp2_2(mul2(d2, A2[s]));
+          prod[s] = mul2(prod[s], dec);
+          r[s] = mul2(dec, fma2(c[s], y2, r[s]));
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kH; ++s) r[s] = fma2(entry[s], tile_gap2(mul2(F2(sum, sum), A2[s]), prod[s]), r[s]);
+    total += sum;
+    __syncthreads();
+  }
+  if (q.valid) {
+    const int64_t at = ((int64_t)q.b * a.nseg + q.seg) * a.channels + q.d;
+    store_states(a.seg_state + at * N, N, p, r);
     if (p == 0) a.seg_sum[at] = total;
   }
 }
 
-template <typename T, int P>
+constexpr int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
+
+template <typename T, class G>
 struct BwdSmem {
-  static constexpr int CB = kScanThreads / P, TT = ScanTile<P>::kBwd, NP = kS * P;
-  static constexpr int DP = TT + 4, kPart = 2 * NP + 1;
-  static constexpr int kRows = CB * DP;                          // D, D u, dy, and three sums over states
-  static constexpr int kStart = TT / kSub * kScanThreads * kS;   // states at the start of each run of kSub tokens
-  static constexpr int kBC = TileBC<T, P, TT>::kFloats;
-  static constexpr int kFloats = 6 * kRows + kStart + 2 * kBC + (kScanThreads / 32) * TT * kPart;
+  static constexpr int TT = G::TB, DP = TT + 4, kPart = 2 * G::NP + 1;
+  static constexpr int kRows = G::CB * DP;                     // D, D u, dy, and three sums over states
+  static constexpr int kStart = TT / kRun * kThreads * kS;     // states at the start of each run
+  static constexpr int kBC = (TileBC<T, G, TT>::kFloats + 3) / 4 * 4;
+  static constexpr int kFloats = 6 * kRows + kStart + kBC + (kThreads / 32) * TT * kPart;
 };
 
 // Sums of v[0..7] over the lanes of a warp that hold the same states of
@@ -575,53 +663,48 @@ struct BwdSmem {
 // lane holds.  Leaves kLeft values, the first of index `first`.
 template <int P>
 struct SumChannels {
-  static constexpr int kLevels = P >= 32 ? 0 : P == 16 ? 1 : P == 8 ? 2 : 3;
-  static constexpr int kLeft = 8 >> kLevels;
+  static constexpr int kValues = 2 * kS, kChannels = 32 / P;
+  static constexpr int kLevels = log2_of(kChannels < kValues ? kChannels : kValues);
+  static constexpr int kLeft = kValues >> kLevels;
   __device__ static __forceinline__ int first(int lane) {
     int f = 0;
-    if (kLevels > 0 && (lane & P)) f += 4;
-    if (kLevels > 1 && (lane & (2 * P))) f += 2;
-    if (kLevels > 2 && (lane & (4 * P))) f += 1;
+#pragma unroll
+    for (int i = 0; i < kLevels; ++i)
+      if (lane & (P << i)) f += kValues >> (i + 1);
     return f;
   }
-  __device__ static __forceinline__ void sum(float *v, int lane) {
-    if constexpr (kLevels > 0) {
-      const bool hi = lane & P;
+  __device__ static __forceinline__ void sum(float (&v)[kValues], int lane) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float keep = hi ? v[4 + i] : v[i], send = hi ? v[i] : v[4 + i];
-        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, P);
+    for (int i = 0; i < kLevels; ++i) {
+      const bool hi = lane & (P << i);
+      const int half = kValues >> (i + 1);
+#pragma unroll
+      for (int k = 0; k < half; ++k) {
+        const float keep = hi ? v[half + k] : v[k], send = hi ? v[k] : v[half + k];
+        v[k] = keep + __shfl_xor_sync(0xffffffffu, send, P << i);
       }
     }
-    if constexpr (kLevels > 1) {
-      const bool hi = lane & (2 * P);
+    if constexpr (kLeft == 1) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float keep = hi ? v[2 + i] : v[i], send = hi ? v[i] : v[2 + i];
-        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, 2 * P);
-      }
-    }
-    if constexpr (kLevels > 2) {
-      const bool hi = lane & (4 * P);
-      const float keep = hi ? v[1] : v[0], send = hi ? v[0] : v[1];
-      v[0] = keep + __shfl_xor_sync(0xffffffffu, send, 4 * P);
-#pragma unroll
-      for (int o = 8 * P; o < 32; o <<= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+      for (int o = P << kLevels; o < 32; o <<= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
     }
   }
-  // with P <= 2 several lanes end with the same sum: one of them writes it
-  __device__ static __forceinline__ bool writes(int lane) { return lane < 8 * P; }
+  // with more channels than values several lanes end with the same sum: one writes it
+  __device__ static __forceinline__ bool writes(int lane) { return lane < (P << kLevels); }
 };
 
-template <typename T, int P>
-__global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(ScanArgs a) {
-  using S = BwdSmem<T, P>;
-  constexpr int TT = S::TT, E = TT >= P ? TT / P : 1, DP = S::DP, NP = S::NP;
-  using BC = TileBC<T, P, TT>;
+template <typename T, class G>
+__global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(ScanArgs a) {
+  using M = BwdSmem<T, G>;
+  constexpr int P = G::P, NP = G::NP;
+  constexpr int TT = M::TT, E = TT >= P ? TT / P : 1, DP = M::DP;
+  using BC = TileBC<T, G, TT>;
   extern __shared__ __align__(16) float smem[];
-  float *s_d = smem, *s_x = s_d + S::kRows, *s_y = s_x + S::kRows;
-  float *s_o = s_y + S::kRows, *s_start = s_o + 3 * S::kRows, *s_B = s_start + S::kStart, *s_C = s_B + S::kBC, *s_part = s_C + S::kBC;
-  const ScanPlace<P> q(a);
+  float *s_d = smem, *s_x = s_d + M::kRows, *s_y = s_x + M::kRows;
+  float *s_o = s_y + M::kRows, *s_start = s_o + 3 * M::kRows;
+  T *s_bc = reinterpret_cast<T *>(s_start + M::kStart);
+  float *s_part = s_start + M::kStart + M::kBC;
+  const ScanPlace<G> q(a);
   const int p = q.p, N = a.states, L = a.length, lane = threadIdx.x & 31;
   const T *u = static_cast<const T *>(a.u) + q.row * L, *dl = static_cast<const T *>(a.delta) + q.row * L;
   const T *grad = static_cast<const T *>(a.grad) + q.row * L;
@@ -634,26 +717,27 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(ScanArgs
   const bool vec = (L * (int64_t)sizeof(T)) % 16 == 0;
   const bool loads = p * E < TT;  // (more lanes than tokens of a tile)
   const float bias = a.bias ? a.bias[q.d] : 0.f, skip = a.skip ? a.skip[q.d] : 0.f;
-  float A2[kS], r[kS], dskip = 0.f, dbias = 0.f;
-  load_states<P>(a.A + (int64_t)q.d * N, N, p, A2);
+  float dskip = 0.f, dbias = 0.f;
+  F2 A2[kH], r[kH], dA[kH];
+  load_decay_rates(a, q.d, p, A2);
 #pragma unroll
-  for (int s = 0; s < kS; ++s) {
-    A2[s] *= kLog2e;
-    r[s] = 0.f;
-  }
-  if (a.grad_final) load_states<P>(a.grad_final + q.row * N, N, p, r);
+  for (int s = 0; s < kH; ++s) r[s] = dA[s] = F2(0.f, 0.f);
+  if (a.grad_final) load_states(a.grad_final + q.row * N, N, p, r);
   for (int i = a.nseg - 1; i > q.seg; --i) {
-    float e[kS];
+    F2 e[kH];
     const int64_t at = ((int64_t)q.b * a.nseg + i) * a.channels + q.d;
-    load_states<P>(a.seg_state + at * N, N, p, e);
+    load_states(a.seg_state + at * N, N, p, e);
     const float sum = a.seg_sum[at];
 #pragma unroll
-    for (int s = 0; s < kS; ++s) r[s] = fmaf(exp2_f(sum * A2[s]), r[s], e[s]);
+    for (int s = 0; s < kH; ++s) {
+      const F2 x = mul2(F2(sum, sum), A2[s]);
+      r[s] = fma2(F2(exp2_tile(x.x()), exp2_tile(x.y())), r[s], e[s]);
+    }
   }
   const int t_begin = q.seg * a.seg_len, t_stop = min(L, t_begin + a.seg_len), t_end = min(t_stop, q.len);
   float *row_d = s_d + q.c * DP, *row_x = s_x + q.c * DP, *row_y = s_y + q.c * DP;
-  float *row_sy = s_o + q.c * DP, *row_sb = row_sy + S::kRows, *row_sm = row_sb + S::kRows;
-  float *my_part = s_part + (threadIdx.x / 32) * TT * S::kPart;
+  float *row_sy = s_o + q.c * DP, *row_sb = row_sy + M::kRows, *row_sm = row_sb + M::kRows;
+  float *my_part = s_part + (threadIdx.x / 32) * TT * M::kPart;
   Pack<T, E> nu, nd, ng, nz;
   BC nbc;
   auto fetch = [&](int t0) {
@@ -663,15 +747,8 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(ScanArgs
       load_row(ng, grad, t0 + p * E, t_end, vec);
       if (z) load_row(nz, z, t0 + p * E, t_end, vec);
     }
-    nbc.load(B, C, N, L, t0, t_end, vec, true);
+    nbc.load(B, C, N, L, t0, t_end, vec);
   };
-  F2 A22[kH], r2[kH], dA2[kH];
-#pragma unroll
-  for (int s = 0; s < kH; ++s) {
-    A22[s] = F2(A2[2 * s], A2[2 * s + 1]);
-    r2[s] = F2(r[2 * s], r[2 * s + 1]);
-    dA2[s] = F2(0.f, 0.f);
-  }
   const int last_live = t_begin + (t_end - t_begin - 1) / TT * TT;
   if (t_begin < t_end) fetch(last_live);
   for (int t0 = t_begin + (t_stop - t_begin - 1) / TT * TT; t0 >= t_begin; t0 -= TT) {
@@ -684,7 +761,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(ScanArgs
         store_row(o, ddl, t0 + p * E, t_stop, vec);
         if (z) store_row(o, dz, t0 + p * E, t_stop, vec);
       }
-      for (int e = threadIdx.x; e < 2 * N * TT; e += kScanThreads) {
+      for (int e = threadIdx.x; e < 2 * N * TT; e += kThreads) {
         const int n = e / TT, t = t0 + e % TT;
         if (t < t_stop) part[(int64_t)n * L + t] = 0.f;
       }
@@ -705,96 +782,107 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(ScanArgs
         row_y[p * E + i] = q.valid ? dy : 0.f;
       }
     }
-    nbc.put(s_B, s_C, true);
+    F2 h0[kH];
+    load_states(a.ckpt + (((int64_t)q.b * ((L + TT - 1) / TT) + t0 / TT) * a.channels + q.d) * N, N, p, h0);
+    nbc.put(s_bc, true);
     __syncthreads();
     if (t0 > t_begin) fetch(t0 - TT);
-    // the states at the start of each run of kSub tokens
+    // the states at the start of each run of kRun tokens
     float *start = s_start + threadIdx.x * kS;
-    {
-      float h0[kS];
-      load_states<P>(a.ckpt + (((int64_t)q.b * ((L + TT - 1) / TT) + t0 / TT) * a.channels + q.d) * N, N, p, h0);
-      F2 h2[kH] = {F2(h0[0], h0[1]), F2(h0[2], h0[3])};
-      put_pairs(start, h2);
+    put_pairs(start, h0);
 #pragma unroll 1
-      for (int k = 1; k < TT / kSub; ++k) {
-        float dd[kSub], xx[kSub];
-        load8f(row_d + (k - 1) * kSub, dd);
-        load8f(row_x + (k - 1) * kSub, xx);
+    for (int k = 1; k < TT / kRun; ++k) {
+      float dd[kRun], xx[kRun];
+      load_row_f(row_d + (k - 1) * kRun, dd);
+      load_row_f(row_x + (k - 1) * kRun, xx);
 #pragma unroll
-        for (int j = 0; j < kSub; ++j) {
-          F2 b2[kH];
-          load_pairs(s_B + BC::row8((k - 1) * kSub, j) + p * kS, b2);
-          const F2 d2(dd[j], dd[j]), x2(xx[j], xx[j]);
-#pragma unroll
-          for (int s = 0; s < kH; ++s) h2[s] = fma2(decay2(mul2(d2, A22[s])), h2[s], mul2(x2, b2[s]));
-        }
-        put_pairs(start + k * kScanThreads * kS, h2);
-      }
-    }
-    F2 tile_dA[kH] = {F2(0.f, 0.f), F2(0.f, 0.f)};
-#pragma unroll 1
-    for (int k = TT / kSub - 1; k >= 0; --k) {
-      F2 h2[kSub + 1][kH], dec[kSub][kH];
-      float y[kSub], s1[kSub], s2[kSub], dd[kSub], xx[kSub], yy[kSub];
-      load8f(row_d + k * kSub, dd);
-      load8f(row_x + k * kSub, xx);
-      load8f(row_y + k * kSub, yy);
-      load_pairs(start + k * kScanThreads * kS, h2[0]);
-#pragma unroll
-      for (int j = 0; j < kSub; ++j) {
-        F2 b2[kH], c2[kH];
-        load_pairs(s_B + BC::row8(k * kSub, j) + p * kS, b2);
-        load_pairs(s_C + BC::row8(k * kSub, j) + p * kS, c2);
+      for (int j = 0; j < kRun; ++j) {
+        F2 b[kH];
+        BC::first(s_bc, BC::template row_in<kRun>((k - 1) * kRun, j), p).unpack(b);
         const F2 d2(dd[j], dd[j]), x2(xx[j], xx[j]);
 #pragma unroll
+        for (int s = 0; s < kH; ++s) h0[s] = fma2(exp2_2(mul2(d2, A2[s])), h0[s], mul2(x2, b[s]));
+      }
+      put_pairs(start + k * kThreads * kS, h0);
+    }
+    F2 tile_dA[kH], entry[kH], prod[kH];
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < kH; ++s) {
+      tile_dA[s] = F2(0.f, 0.f);
+      entry[s] = r[s];
+      prod[s] = F2(1.f, 1.f);
+    }
+#pragma unroll 1
+    for (int k = TT / kRun - 1; k >= 0; --k) {
+      F2 h[kRun + 1][kH], dec[kRun][kH];
+      typename BC::Both bc[kRun];
+      float y[kRun], s1[kRun], s2[kRun], dd[kRun], xx[kRun], yy[kRun];
+      load_row_f(row_d + k * kRun, dd);
+      load_row_f(row_x + k * kRun, xx);
+      load_row_f(row_y + k * kRun, yy);
+      load_pairs(start + k * kThreads * kS, h[0]);
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        F2 b[kH], c[kH];
+        bc[j] = BC::both(s_bc, BC::template row_in<kRun>(k * kRun, j), p);
+        bc[j].b.unpack(b);
+        bc[j].c.unpack(c);
+        const F2 d2(dd[j], dd[j]), x2(xx[j], xx[j]);
+        sum += dd[j];
+#pragma unroll
         for (int s = 0; s < kH; ++s) {
-          dec[j][s] = decay2(mul2(d2, A22[s]));
-          h2[j + 1][s] = fma2(dec[j][s], h2[j][s], mul2(x2, b2[s]));
+          dec[j][s] = exp2_2(mul2(d2, A2[s]));
+          prod[s] = mul2(prod[s], dec[j][s]);
+          h[j + 1][s] = fma2(dec[j][s], h[j][s], mul2(x2, b[s]));
         }
-        const F2 y2 = fma2(h2[j + 1][0], c2[0], mul2(h2[j + 1][1], c2[1]));
-        y[j] = y2.x() + y2.y();
+        y[j] = dot(h[j + 1], c);
       }
 #pragma unroll
-      for (int j = kSub - 1; j >= 0; --j) {
-        const int t = k * kSub + j;
-        F2 b2[kH], c2[kH], vb[kH], vc[kH], m2[kH], dh[kH];
-        load_pairs(s_B + BC::row8(k * kSub, j) + p * kS, b2);
-        load_pairs(s_C + BC::row8(k * kSub, j) + p * kS, c2);
+      for (int j = kRun - 1; j >= 0; --j) {
+        F2 b[kH], c[kH], dh[kH], m[kH];
+        bc[j].b.unpack(b);
+        bc[j].c.unpack(c);
         const F2 d2(dd[j], dd[j]), x2(xx[j], xx[j]), dy2(yy[j], yy[j]);
+        float v[2 * kS];  // dB of the lane's states, then dC
 #pragma unroll
         for (int s = 0; s < kH; ++s) {
-          dh[s] = fma2(dy2, c2[s], r2[s]);
-          vb[s] = mul2(dh[s], x2);
-          vc[s] = mul2(dy2, h2[j + 1][s]);
-          r2[s] = mul2(dec[j][s], dh[s]);
-          m2[s] = mul2(r2[s], h2[j][s]);
-          tile_dA[s] = fma2(m2[s], d2, tile_dA[s]);
+          dh[s] = fma2(dy2, c[s], r[s]);
+          const F2 vb = mul2(dh[s], x2), vc = mul2(dy2, h[j + 1][s]);
+          v[2 * s] = vb.x();
+          v[2 * s + 1] = vb.y();
+          v[kS + 2 * s] = vc.x();
+          v[kS + 2 * s + 1] = vc.y();
+          r[s] = mul2(dec[j][s], dh[s]);
+          m[s] = mul2(r[s], h[j][s]);
+          tile_dA[s] = fma2(m[s], d2, tile_dA[s]);
         }
-        const F2 t1 = fma2(dh[0], b2[0], mul2(dh[1], b2[1])), t2 = fma2(m2[0], A22[0], mul2(m2[1], A22[1]));
-        s1[j] = t1.x() + t1.y();
-        s2[j] = t2.x() + t2.y();
-        float v[8] = {vb[0].x(), vb[0].y(), vb[1].x(), vb[1].y(), vc[0].x(), vc[0].y(), vc[1].x(), vc[1].y()};
+        s1[j] = dot(dh, b);
+        s2[j] = dot(m, A2);
         SumChannels<P>::sum(v, lane);
         if (SumChannels<P>::writes(lane)) {
           const int f = SumChannels<P>::first(lane);
 #pragma unroll
           for (int i = 0; i < SumChannels<P>::kLeft; ++i) {
-            const int idx = f + i;  // 0-3: dB of the lane's states, 4-7: dC
-            my_part[t * S::kPart + (idx / 4) * NP + p * kS + idx % 4] = v[i];
+            const int idx = f + i;
+            my_part[(k * kRun + j) * M::kPart + (idx / kS) * NP + p * kS + idx % kS] = v[i];
           }
         }
       }
 #pragma unroll
-      for (int j = 0; j < kSub; j += 4) {
-        Sum4<P>(y[j], y[j + 1], y[j + 2], y[j + 3], p).put(row_sy + k * kSub + j, p);
-        Sum4<P>(s1[j], s1[j + 1], s1[j + 2], s1[j + 3], p).put(row_sb + k * kSub + j, p);
-        Sum4<P>(s2[j], s2[j + 1], s2[j + 2], s2[j + 3], p).put(row_sm + k * kSub + j, p);
+      for (int j = 0; j < kRun; j += 4) {
+        Sum4<P>(y[j], y[j + 1], y[j + 2], y[j + 3], p).put(row_sy + k * kRun + j, p);
+        Sum4<P>(s1[j], s1[j + 1], s1[j + 2], s1[j + 3], p).put(row_sb + k * kRun + j, p);
+        Sum4<P>(s2[j], s2[j + 1], s2[j + 2], s2[j + 3], p).put(row_sm + k * kRun + j, p);
       }
     }
-    // a tile's sum at a time: what a long sum of 32-bit numbers loses grows
-    // with the number of its terms
+    // dA: a tile's sum at a time, as what a long sum of 32-bit numbers loses
+    // grows with the number of its terms
 #pragma unroll
-    for (int s = 0; s < kH; ++s) dA2[s] = add2(dA2[s], tile_dA[s]);
+    for (int s = 0; s < kH; ++s) {
+      dA[s] = add2(dA[s], tile_dA[s]);
+      r[s] = fma2(entry[s], tile_gap2(mul2(F2(sum, sum), A2[s]), prod[s]), r[s]);
+    }
     __syncwarp();
     if (q.valid && loads) {
       Pack<T, E> ou, od, oz;
@@ -825,14 +913,14 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(ScanArgs
     }
     __syncthreads();
     // the warps' sums over their channels, added in order
-    for (int e = threadIdx.x; e < 2 * N * TT; e += kScanThreads) {
+    for (int e = threadIdx.x; e < 2 * N * TT; e += kThreads) {
       const int n = e / TT, t = e % TT;
       if (t0 + t < t_stop) {
-        const float *src = s_part + t * S::kPart + (n < N ? n : NP + n - N);
-        float s = src[0];
+        const float *src = s_part + t * M::kPart + (n < N ? n : NP + n - N);
+        float v = src[0];
 #pragma unroll
-        for (int w = 1; w < kScanThreads / 32; ++w) s += src[w * TT * S::kPart];
-        part[(int64_t)n * L + t0 + t] = s;
+        for (int w = 1; w < kThreads / 32; ++w) v += src[w * TT * M::kPart];
+        part[(int64_t)n * L + t0 + t] = v;
       }
     }
     // (the next tile's first barrier comes before anything overwrites s_part)
@@ -843,17 +931,13 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(ScanArgs
     dbias += __shfl_xor_sync(0xffffffffu, dbias, o);
   }
   if (q.valid) {
-    const float dA[kS] = {dA2[0].x(), dA2[0].y(), dA2[1].x(), dA2[1].y()};
-    const float rr[kS] = {r2[0].x(), r2[0].y(), r2[1].x(), r2[1].y()};
-    float *par = a.part_par + ((int64_t)q.b * a.nseg + q.seg) * a.channels * (N + 2);
-#pragma unroll
-    for (int s = 0; s < kS; ++s)
-      if (p * kS + s < N) par[(int64_t)q.d * N + p * kS + s] = dA[s];
+    float *par = a.part_par + ((int64_t)q.b * a.nseg + q.seg) * a.par_stride();
+    store_states(par + (int64_t)q.d * N, N, p, dA);
     if (p == 0) {
       par[(int64_t)a.channels * N + q.d] = dskip;
       par[(int64_t)a.channels * (N + 1) + q.d] = dbias;
     }
-    if (a.dinit && q.seg == 0) store_states<P>(a.dinit + q.row * N, N, p, rr);
+    if (a.dinit && q.seg == 0) store_states(a.dinit + q.row * N, N, p, r);
   }
 }
 
@@ -881,7 +965,7 @@ __global__ void __launch_bounds__(256) scan_params_kernel(ScanArgs a, T *dB, T *
   if (i >= count) return;
   double s = 0.0;
 #pragma unroll 8
-  for (int k = 0; k < a.batch * a.nseg; ++k) s += a.part_par[k * count + i];
+  for (int k = 0; k < a.batch * a.nseg; ++k) s += a.part_par[k * a.par_stride() + i];
   const int64_t dn = (int64_t)a.channels * N;
   if (i < dn) dA[i] = (float)s;
   else if (i < dn + a.channels) {
@@ -901,9 +985,10 @@ struct ScanStepArgs {
 };
 
 // One token: reads and writes each state once (8 bytes a state: what bounds it).
+
 template <typename T, int P>
-__global__ void __launch_bounds__(kScanThreads) scan_step_kernel(ScanStepArgs a) {
-  constexpr int CB = kScanThreads / P;
+__global__ void __launch_bounds__(kThreads) scan_step_kernel(ScanStepArgs a) {
+  constexpr int CB = kThreads / P;
   const int b = blockIdx.x / a.nblk, blk = blockIdx.x - b * a.nblk;
   const int p = threadIdx.x % P, d = blk * CB + threadIdx.x / P, N = a.states;
   const bool valid = d < a.channels;
@@ -923,8 +1008,11 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(ScanStepArgs a)
     *reinterpret_cast<float4 *>(h) = *reinterpret_cast<const float4 *>(state + p * kS);
     *reinterpret_cast<float4 *>(A2) = *reinterpret_cast<const float4 *>(a.A + (int64_t)dd * N + p * kS);
   } else {
-    load_states<P>(state, N, p, h);
-    load_states<P>(a.A + (int64_t)dd * N, N, p, A2);
+#pragma unroll
+    for (int s = 0; s < kS; ++s) {
+      h[s] = p * kS + s < N ? state[p * kS + s] : 0.f;
+      A2[s] = p * kS + s < N ? a.A[(int64_t)dd * N + p * kS + s] : 0.f;
+    }
   }
   const float u = to_f(static_cast<const T *>(a.u)[i]);
   float delta = to_f(static_cast<const T *>(a.delta)[i]) + (a.bias ? a.bias[dd] : 0.f);
@@ -939,7 +1027,10 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(ScanStepArgs a)
       y = fmaf(h[s], to_f(C[n]), y);
     }
   }
-  if (valid) store_states<P>(state, N, p, h);
+  if (valid) {
+    const F2 pairs[kH] = {F2(h[0], h[1]), F2(h[2], h[3])};
+    store_states(state, N, p, pairs);
+  }
 #pragma unroll
   for (int o = 1; o < P; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
   if (valid && p == 0) {
@@ -956,21 +1047,22 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(ScanStepArgs a)
 
 PerContext<uint64_t> g_scan_attr;
 
+// f(T{}, Layout{}) for the call's type and states
 template <typename F>
-int by_type_and_lanes(int dtype, int states, F &&f) {
-#define PC2D_LANES(T)                                            \
-  switch (lanes_of(states)) {                                    \
-    case 1: return f(T{}, std::integral_constant<int, 1>{});     \
-    case 2: return f(T{}, std::integral_constant<int, 2>{});     \
-    case 4: return f(T{}, std::integral_constant<int, 4>{});     \
-    case 8: return f(T{}, std::integral_constant<int, 8>{});     \
-    case 16: return f(T{}, std::integral_constant<int, 16>{});   \
-    default: return f(T{}, std::integral_constant<int, 32>{});   \
+int by_type_and_layout(int dtype, int states, F &&f) {
+#define PC2D_LAYOUT(T)                          \
+  switch (lanes_of(states)) {                   \
+    case 1: return f(T{}, Layout<1>{});         \
+    case 2: return f(T{}, Layout<2>{});         \
+    case 4: return f(T{}, Layout<4>{});         \
+    case 8: return f(T{}, Layout<8>{});         \
+    case 16: return f(T{}, Layout<16>{});       \
+    default: return f(T{}, Layout<32>{});       \
   }
-  if (dtype == PC2D_DTYPE_F32) { PC2D_LANES(float) }
-  if (dtype == PC2D_DTYPE_F16) { PC2D_LANES(__half) }
-  PC2D_LANES(__nv_bfloat16)
-#undef PC2D_LANES
+  if (dtype == PC2D_DTYPE_F32) { PC2D_LAYOUT(float) }
+  if (dtype == PC2D_DTYPE_F16) { PC2D_LAYOUT(__half) }
+  PC2D_LAYOUT(__nv_bfloat16)
+#undef PC2D_LAYOUT
 }
 
 constexpr int kMaxStates = 128;
@@ -1002,7 +1094,7 @@ int check_scan(const char *what, int dtype, int batch, int channels, int length,
 // the longer (forward) kind each.
 template <bool kBackward>
 void scan_split(ScanArgs *a) {
-  const int P = lanes_of(a->states), CB = kScanThreads / P;
+  const int CB = kThreads / lanes_of(a->states);
   a->per_group = a->channels / a->groups;
   a->nblk = std::max(1, (a->per_group + CB - 1) / CB);
   const int64_t blocks = (int64_t)a->batch * a->groups * a->nblk;
@@ -1030,7 +1122,7 @@ size_t scan_part_bc_bytes(const ScanArgs &a) {
   return align_up((size_t)a.batch * a.groups * a.nblk * 2 * a.states * a.length * 4, 256);
 }
 size_t scan_part_par_bytes(const ScanArgs &a) {
-  return align_up((size_t)a.batch * a.nseg * a.channels * (a.states + 2) * 4, 256);
+  return align_up((size_t)a.batch * a.nseg * a.par_stride() * 4, 256);
 }
 char *take_segments(ScanArgs *a, char *ws) {
   if (a->nseg == 1) return ws;
@@ -1116,14 +1208,22 @@ extern "C" int pc2d_ssm_scan_forward(int dtype, const void *u, const void *delta
   take_segments(&a, static_cast<char *>(workspace));
   const unsigned grid = (unsigned)((int64_t)batch * groups * a.nblk * a.nseg);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return by_type_and_lanes(dtype, states, [&](auto t, auto p) -> int {
+  return by_type_and_layout(dtype, states, [&](auto t, auto layout) -> int {
     using T = decltype(t);
-    constexpr int P = decltype(p)::value;
+    using G = decltype(layout);
     if (a.nseg > 1) {
-      scan_forward_kernel<T, P, true><<<grid, kScanThreads, 0, s>>>(a);
+      scan_forward_kernel<T, G, true><<<grid, kThreads, 0, s>>>(a);
       PC2D_LAUNCH_CHECK("scan_forward_kernel (segments)");
     }
-    scan_forward_kernel<T, P, false><<<grid, kScanThreads, 0, s>>>(a);
+    // more blocks than two per SM: the layout for four
+    if (G::P == 4 || G::P == 8) {
+      if (grid > 2u * device_sm_count()) {
+        scan_forward_kernel<T, Layout<G::P, true>, false><<<grid, kThreads, 0, s>>>(a);
+        PC2D_LAUNCH_CHECK("scan_forward_kernel (many blocks)");
+        return PC2D_OK;
+      }
+    }
+    scan_forward_kernel<T, G, false><<<grid, kThreads, 0, s>>>(a);
     PC2D_LAUNCH_CHECK("scan_forward_kernel");
     return PC2D_OK;
   });
@@ -1174,25 +1274,25 @@ extern "C" int pc2d_ssm_scan_backward(int dtype, const void *grad, const float *
   a.part_par = reinterpret_cast<float *>(ws + scan_part_bc_bytes(a));
   const unsigned grid = (unsigned)((int64_t)batch * groups * a.nblk * a.nseg);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return by_type_and_lanes(dtype, states, [&](auto t, auto p) -> int {
+  return by_type_and_layout(dtype, states, [&](auto t, auto layout) -> int {
     using T = decltype(t);
-    constexpr int P = decltype(p)::value;
+    using G = decltype(layout);
     if (grid > 0) {
-      constexpr int bytes = BwdSmem<T, P>::kFloats * 4;
-      // one bit per instance: 3 types x 6 lane counts
+      constexpr int bytes = BwdSmem<T, G>::kFloats * 4;
+      // one bit per instance: 3 types x 6 layouts
       int bit = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 1 : 2;
-      for (int i = P; i > 1; i >>= 1) bit += 3;
+      bit += 3 * log2_of(G::P);
       const int attr = once_per_context(g_scan_attr, (uint64_t)1 << bit, []() -> int {
-        PC2D_CUDA_CHECK(cudaFuncSetAttribute(scan_backward_kernel<T, P>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        PC2D_CUDA_CHECK(cudaFuncSetAttribute(scan_backward_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              bytes));
         return PC2D_OK;
       });
       if (attr != PC2D_OK) return attr;
       if (a.nseg > 1) {
-        scan_carry_kernel<T, P><<<grid, kScanThreads, 0, s>>>(a);
+        scan_carry_kernel<T, G><<<grid, kThreads, 0, s>>>(a);
         PC2D_LAUNCH_CHECK("scan_carry_kernel");
       }
-      scan_backward_kernel<T, P><<<grid, kScanThreads, bytes, s>>>(a);
+      scan_backward_kernel<T, G><<<grid, kThreads, bytes, s>>>(a);
       PC2D_LAUNCH_CHECK("scan_backward_kernel");
     }
     const int64_t bc = ((int64_t)batch * groups * 2 * states * length + 255) / 256;
@@ -1228,11 +1328,11 @@ extern "C" int pc2d_ssm_scan_step(int dtype, const void *u, const void *delta, f
   a.batch = batch; a.places = places; a.channels = channels; a.states = states; a.groups = groups;
   a.per_group = channels / groups;
   a.softplus = delta_softplus != 0;
-  const int cb = kScanThreads / lanes_of(states);
+  const int cb = kThreads / lanes_of(states);
   a.nblk = (channels + cb - 1) / cb;
-  return by_type_and_lanes(dtype, states, [&](auto t, auto p) -> int {
-    scan_step_kernel<decltype(t), decltype(p)::value>
-        <<<(unsigned)((int64_t)a.nblk * batch), kScanThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+  return by_type_and_layout(dtype, states, [&](auto t, auto layout) -> int {
+    scan_step_kernel<decltype(t), decltype(layout)::P>
+        <<<(unsigned)((int64_t)a.nblk * batch), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
     PC2D_LAUNCH_CHECK("scan_step_kernel");
     return PC2D_OK;
   });
