@@ -942,30 +942,66 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
 }
 
 // Adds up the blocks' shares of dB and dC (in 32 bits, over the blocks of a
-// group in order) and those of dA, dskip and dbias (in 64 bits, over the batch
-// and the segments in order).
-template <typename T>
-__global__ void __launch_bounds__(256) scan_params_kernel(ScanArgs a, T *dB, T *dC, float *dA, float *dskip,
-                                                         float *dbias, int64_t bc_blocks) {
+// group) and those of dA, dskip and dbias (in 64 bits, over the batch and the
+// segments).  `ways` threads share a column (V neighbouring ones of dB and dC),
+// add every ways-th share and are then added in order: short chains of loads,
+// many of them at a time.  A block of the first kind stays within one batch
+// row and group (per_bg blocks each).
+constexpr int kParThreads = 256, kParWays = 8;
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kParThreads) scan_params_kernel(ScanArgs a, T *dB, T *dC, float *dA, float *dskip,
+                                                                 float *dbias, unsigned bc_blocks, unsigned per_bg,
+                                                                 int bc_ways) {
+  __shared__ __align__(16) double sums[kParThreads * V / 2 + kParThreads / 2];
   const int N = a.states;
   if (blockIdx.x < bc_blocks) {
-    const int64_t per = 2 * (int64_t)N * a.length, count = (int64_t)a.batch * a.groups * per;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= count) return;
-    const int64_t bg = i / per, e = i - bg * per, half = per / 2;
-    const float *src = a.part_bc + bg * a.nblk * per + e;
-    float s = 0.f;
+    const int ways = bc_ways, cols = kParThreads / ways;
+    const int way = threadIdx.x / cols, col = threadIdx.x - way * cols;
+    const int64_t half = (int64_t)N * a.length, per = 2 * half;
+    const int64_t bg = blockIdx.x / per_bg, e = ((int64_t)(blockIdx.x - bg * per_bg) * cols + col) * V;
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = 0.f;
+    if (e < per) {
+      const float *src = a.part_bc + bg * a.nblk * per + e;
 #pragma unroll 8
-    for (int k = 0; k < a.nblk; ++k) s += src[k * per];
-    if (e < half) dB[bg * half + e] = from_f<T>(s);
-    else dC[bg * half + e - half] = from_f<T>(s);
+      for (int k = way; k < a.nblk; k += ways) {
+        Pack<float, V> w;
+        w.load(src + k * per);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] += w.v[j];
+      }
+    }
+    float *mine = reinterpret_cast<float *>(sums) + threadIdx.x * V;
+    if (ways > 1) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) mine[j] = v[j];
+      __syncthreads();
+    }
+    if (way != 0 || e >= per) return;
+    for (int w = 1; w < ways; ++w)
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] += mine[w * cols * V + j];
+    Pack<T, V> o;
+#pragma unroll
+    for (int j = 0; j < V; ++j) o.v[j] = from_f<T>(v[j]);
+    o.store(e < half ? dB + bg * half + e : dC + bg * half + e - half);
     return;
   }
-  const int64_t count = (int64_t)a.channels * (N + 2), i = ((int64_t)blockIdx.x - bc_blocks) * 256 + threadIdx.x;
-  if (i >= count) return;
+  constexpr int cols = kParThreads / kParWays;
+  const int way = threadIdx.x / cols, col = threadIdx.x - way * cols;
+  const int64_t i = (int64_t)(blockIdx.x - bc_blocks) * cols + col;
+  const int64_t count = (int64_t)a.channels * (N + 2), stride = a.par_stride();
   double s = 0.0;
+  if (i < count) {
 #pragma unroll 8
-  for (int k = 0; k < a.batch * a.nseg; ++k) s += a.part_par[k * a.par_stride() + i];
+    for (int k = way; k < a.batch * a.nseg; k += kParWays) s += a.part_par[k * stride + i];
+  }
+  sums[threadIdx.x] = s;
+  __syncthreads();
+  if (way != 0 || i >= count) return;
+  for (int w = 1; w < kParWays; ++w) s += sums[w * cols + col];
   const int64_t dn = (int64_t)a.channels * N;
   if (i < dn) dA[i] = (float)s;
   else if (i < dn + a.channels) {
@@ -1295,10 +1331,18 @@ extern "C" int pc2d_ssm_scan_backward(int dtype, const void *grad, const float *
       scan_backward_kernel<T, G><<<grid, kThreads, bytes, s>>>(a);
       PC2D_LAUNCH_CHECK("scan_backward_kernel");
     }
-    const int64_t bc = ((int64_t)batch * groups * 2 * states * length + 255) / 256;
-    const int64_t par = ((int64_t)channels * (states + 2) + 255) / 256;
-    scan_params_kernel<T><<<(unsigned)(bc + par), 256, 0, s>>>(a, static_cast<T *>(Bgrad), static_cast<T *>(Cgrad),
-                                                               Agrad, skipgrad, biasgrad, bc);
+    const int ways = a.nblk >= 16 ? 8 : a.nblk >= 8 ? 4 : a.nblk >= 4 ? 2 : 1;
+    const int64_t half = (int64_t)states * length;
+    const bool four = half % 4 == 0;  // then every row of dB and dC starts on a vector of four
+    const unsigned per_bg = (unsigned)ceil_div(2 * half, (int64_t)kParThreads / ways * (four ? 4 : 1));
+    const unsigned bc = per_bg * (unsigned)(batch * groups);
+    const unsigned par = (unsigned)ceil_div((int64_t)channels * (states + 2), kParThreads / kParWays);
+    if (four)
+      scan_params_kernel<T, 4><<<bc + par, kParThreads, 0, s>>>(a, static_cast<T *>(Bgrad), static_cast<T *>(Cgrad),
+                                                               Agrad, skipgrad, biasgrad, bc, per_bg, ways);
+    else
+      scan_params_kernel<T, 1><<<bc + par, kParThreads, 0, s>>>(a, static_cast<T *>(Bgrad), static_cast<T *>(Cgrad),
+                                                               Agrad, skipgrad, biasgrad, bc, per_bg, ways);
     PC2D_LAUNCH_CHECK("scan_params_kernel");
     return PC2D_OK;
   });
