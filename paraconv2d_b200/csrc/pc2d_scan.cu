@@ -1292,7 +1292,7 @@ extern "C" int pc2d_ssm_scan_backward(int dtype, const void *grad, const float *
     set_last_error("pc2d_ssm_scan_backward: null pointer");
     return PC2D_ERR_INVALID_ARGUMENT;
   }
-  if ((st = check_aligned("pc2d_ssm_scan_backward", {grad, u, delta, z, B, C, ugrad, deltagrad, zgrad, checkpoints,
+  if ((st = check_aligned("pc2d_ssm_scan_backward", {grad, u, delta, z, B, C, ugrad, deltagrad, Bgrad, Cgrad, zgrad, checkpoints,
                                                      grad_final, initialgrad, A})) != PC2D_OK)
     return st;
   ScanArgs a = scan_problem(batch, channels, length, states, groups);
