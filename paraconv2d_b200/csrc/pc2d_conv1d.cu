@@ -57,26 +57,6 @@ __device__ __forceinline__ void store_param(void *p, int dtype, int64_t i, float
   else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// Eight elements t0 .. t0+7 of a row: zeros outside [0, n), the kept state's
-// values (init, K-1 of them, or zeros) before 0 if kState.
-template <typename T, int K, bool kState>
-__device__ __forceinline__ void load8(const T *row, int t0, int n, const T *init, float *v) {
-  if (t0 >= 0 && t0 + 8 <= n) {
-    Pack<T, 8> p;
-    p.load(row + t0);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = p.f(i);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int t = t0 + i;
-    v[i] = 0.f;
-    if (t >= 0 && t < n) v[i] = to_f(row[t]);
-    else if (kState && init && t < 0 && t >= -(K - 1)) v[i] = to_f(init[t + K - 1]);
-  }
-}
-
 // Element j (0 .. n+K-2) of a row's line.
 template <typename T, int K>
 __device__ __forceinline__ float line_at(const T *row, const T *init, int j) {
@@ -91,6 +71,7 @@ struct RowPlace {
   int64_t base;   // first element of the row in the array
   int e0;         // t of the first element of the row's vector 0: 0 or below
   int nvec;       // vectors that hold elements of the row
+  int lo, hi;     // vectors lo .. hi-1 lie within the row's tokens
 };
 
 __device__ __forceinline__ bool place_of(const ConvArgs &a, RowPlace *p) {
@@ -106,8 +87,82 @@ __device__ __forceinline__ bool place_of(const ConvArgs &a, RowPlace *p) {
   const int over = (int)(p->base & 7);
   p->e0 = -over;
   p->nvec = (int)(((int64_t)a.length + over + 7) >> 3);
+  p->lo = over ? 1 : 0;
+  p->hi = (p->n + over) >> 3;
   return true;
 }
+
+// The last inputs before a vector that its windows reach: 4 or 8 of them, so
+// that they are one aligned load.
+template <int K>
+constexpr int kBefore = K <= 5 ? 4 : 8;
+
+// A vector within the row's tokens: its eight elements behind those before it,
+// which for the row's first vector may be the kept state's or zeros.
+template <typename T, int K>
+struct Window {
+  Pack<T, 8> cur;
+  Pack<T, kBefore<K>> before;
+  __device__ __forceinline__ void load(const T *row, const T *init, int t0) {
+    cur.load(row + t0);
+    if (K == 1) return;
+    if (t0 >= kBefore<K>) {
+      before.load(row + t0 - kBefore<K>);
+    } else {
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k) {
+        const int t = t0 - (K - 1) + k;
+        T v = from_f<T>(0.f);
+        if (t >= 0) v = row[t];
+        else if (init) v = init[t + K - 1];
+        before.v[kBefore<K> - (K - 1) + k] = v;
+      }
+    }
+  }
+  // the 7 + K values of the line that the vector's windows cover
+  __device__ __forceinline__ void get(float (&x)[K + 7]) const {
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) x[k] = before.f(kBefore<K> - (K - 1) + k);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[K - 1 + i] = cur.f(i);
+  }
+};
+
+// The same for any vector of a row: zeros outside [0, n), the kept state's
+// values before 0.
+template <typename T, int K>
+__device__ __forceinline__ void load_window(const T *row, const T *init, int t0, int n, float (&x)[K + 7]) {
+#pragma unroll
+  for (int i = 0; i < K + 7; ++i) {
+    const int t = t0 + i - (K - 1);
+    x[i] = 0.f;
+    if (t >= 0 && t < n) x[i] = to_f(row[t]);
+    else if (init && t < 0 && t >= -(K - 1)) x[i] = to_f(init[t + K - 1]);
+  }
+}
+
+template <int K>
+__device__ __forceinline__ float filter(const float (&w)[K], float bias, const float (&x)[K + 7], int i) {
+  float s = bias;
+#pragma unroll
+  for (int k = 0; k < K; ++k) s = fmaf(w[k], x[i + k], s);
+  return s;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T *row, int t0, int length, const float (&y)[8]) {
+  Pack<T, 8> o;
+  o.set(y);
+  if (t0 >= 0 && t0 + 8 <= length) {
+    o.store(row + t0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (t0 + i >= 0 && t0 + i < length) row[t0 + i] = o.v[i];
+  }
+}
+
+constexpr int kConvUnroll = 2;  // vectors in flight per lane
 
 template <typename T, int K>
 __global__ void __launch_bounds__(kConvThreads) conv_forward_kernel(ConvArgs a) {
@@ -121,60 +176,76 @@ __global__ void __launch_bounds__(kConvThreads) conv_forward_kernel(ConvArgs a) 
 #pragma unroll
   for (int k = 0; k < K; ++k) w[k] = load_param(a.weight, a.wdtype, (int64_t)p.d * K + k);
   const float bias = a.bias ? load_param(a.bias, a.wdtype, p.d) : 0.f;
-  const int v1 = min(p.nvec, (p.seg + 1) * a.seg);
-  for (int v = p.seg * a.seg + lane; v < v1; v += 32) {
-    const int t0 = p.e0 + v * 8;
-    float x[16];
-    if (K > 1) load8<T, K, true>(row, t0 - 8, p.n, init, x);
-    load8<T, K, true>(row, t0, p.n, init, x + 8);
-    float y[8];
+  const int va = p.seg * a.seg, vb = min(p.nvec, va + a.seg);
+  const int lo = max(va, p.lo), hi = min(vb, p.hi);
+  // the vectors within the tokens
+  for (int v0 = lo + lane; v0 < hi; v0 += 32 * kConvUnroll) {
+    Window<T, K> win[kConvUnroll];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float s = bias;
+    for (int u = 0; u < kConvUnroll; ++u)
+      if (v0 + 32 * u < hi) win[u].load(row, init, p.e0 + (v0 + 32 * u) * 8);
 #pragma unroll
-      for (int k = 0; k < K; ++k) s = fmaf(w[k], x[8 + i - (K - 1) + k], s);
-      y[i] = a.silu ? s * sigmoid_f(s) : s;
-    }
-    if (t0 >= 0 && t0 + 8 <= p.n) {
+    for (int u = 0; u < kConvUnroll; ++u) {
+      if (v0 + 32 * u >= hi) break;
+      float x[K + 7], y[8];
+      win[u].get(x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[i] = filter<K>(w, bias, x, i);
+        if (a.silu) y[i] *= sigmoid_f(y[i]);
+      }
       Pack<T, 8> o;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o.v[i] = from_f<T>(y[i]);
-      o.store(out + t0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (t0 + i >= 0 && t0 + i < a.length) out[t0 + i] = t0 + i < p.n ? from_f<T>(y[i]) : from_f<T>(0.f);
+      o.set(y);
+      o.store(out + p.e0 + (v0 + 32 * u) * 8);
     }
   }
+  // those that reach beyond them: at most one before, and all behind
+  auto edge = [&](int v) {
+    const int t0 = p.e0 + v * 8;
+    float x[K + 7], y[8];
+    if (t0 < p.n) load_window<T, K>(row, init, t0, p.n, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[i] = 0.f;
+      if (t0 + i < p.n) {
+        y[i] = filter<K>(w, bias, x, i);
+        if (a.silu) y[i] *= sigmoid_f(y[i]);
+      }
+    }
+    store8(out, t0, a.length, y);
+  };
+  if (va < lo && lane == 0 && va < vb) edge(va);
+  for (int v = max(hi, lo) + lane; v < vb; v += 32) edge(v);
   if (a.final_state && p.seg == 0 && lane < K - 1)
     static_cast<T *>(a.final_state)[p.row * (K - 1) + lane] = from_f<T>(line_at<T, K>(row, init, p.n + lane));
 }
 
-// dpre of the eight elements from t0 on (zeros outside [0, n)) and the 16
-// values of the line that their windows cover.
+__device__ __forceinline__ float silu_slope(float v) {
+  const float e = sigmoid_f(v);
+  return e * fmaf(v, 1.f - e, 1.f);
+}
+
+// dpre of the eight elements from t0 on, of any vector (zeros outside [0, n)),
+// and the values that their windows cover.
 template <typename T, int K>
-__device__ __forceinline__ void dpre8(const ConvArgs &a, const T *row, const T *grad, const T *init, int t0, int n,
-                                      const float *w, float bias, float *x, float *dp) {
-  if (K > 1) load8<T, K, true>(row, t0 - 8, n, init, x);
-  load8<T, K, true>(row, t0, n, init, x + 8);
-  load8<T, K, false>(grad, t0, n, nullptr, dp);
-  if (!a.silu) return;
+__device__ __forceinline__ void dpre_any(const ConvArgs &a, const T *row, const T *grad, const T *init, int t0, int n,
+                                         const float (&w)[K], float bias, float (&x)[K + 7], float *dp) {
+  load_window<T, K>(row, init, t0, n, x);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float s = bias;
-#pragma unroll
-    for (int k = 0; k < K; ++k) s = fmaf(w[k], x[8 + i - (K - 1) + k], s);
-    const float e = sigmoid_f(s);
-    const float slope = e * fmaf(s, 1.f - e, 1.f);
-    // an element outside the row stays 0 whatever its window gives
-    dp[i] = t0 + i >= 0 && t0 + i < n ? dp[i] * slope : 0.f;
+    dp[i] = 0.f;
+    if (t0 + i >= 0 && t0 + i < n) {
+      dp[i] = to_f(grad[t0 + i]);
+      if (a.silu) dp[i] *= silu_slope(filter<K>(w, bias, x, i));
+    }
   }
 }
 
-// A warp goes through its run from the end to the beginning: the K-1 values of
-// dpre behind a lane's eight come from the next lane, and for lane 31 from
-// lane 0 of the 32 vectors done before (for the first ones from a computation
-// of the vector behind the run).
+// A warp goes through its run from the end to the beginning, 32 vectors at a
+// time: the K-1 values of dpre behind a lane's eight come from the next lane,
+// and for lane 31 from lane 0 of the 32 vectors done before (for the first ones
+// from a computation of the vector behind the run).  The inputs of 32 vectors
+// within the row's tokens are loaded while those before are computed.
 template <typename T, int K>
 __global__ void __launch_bounds__(kConvThreads) conv_backward_kernel(ConvArgs a) {
   RowPlace p;
@@ -193,24 +264,48 @@ __global__ void __launch_bounds__(kConvThreads) conv_backward_kernel(ConvArgs a)
   }
   const float bias = a.bias ? load_param(a.bias, a.wdtype, p.d) : 0.f;
   const int va = p.seg * a.seg, vb = min(p.nvec, va + a.seg);
-  float carry[K > 1 ? K - 1 : 1];  // dpre of the first elements of the vector behind
+  constexpr int B = K > 1 ? K - 1 : 1;
+  float carry[B];  // dpre of the first elements of the vector behind
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) carry[k] = 0.f;
+  for (int k = 0; k < B; ++k) carry[k] = 0.f;
   if (K > 1 && va < vb && vb < p.nvec) {
-    float x[16], dp[8];
-    dpre8<T, K>(a, row, grad, init, p.e0 + vb * 8, p.n, w, bias, x, dp);
+    float x[K + 7], dp[8];
+    dpre_any<T, K>(a, row, grad, init, p.e0 + vb * 8, p.n, w, bias, x, dp);
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) carry[k] = dp[k];
   }
-  for (int v0 = va + ((vb - va - 1) >> 5) * 32; v0 >= va && va < vb; v0 -= 32) {
-    const int v = v0 + lane;
-    const int t0 = p.e0 + v * 8;
-    float x[16], dp[8 + K];
+  Window<T, K> next_x;
+  Pack<T, 8> next_g;
+  auto inside = [&](int v0) { return v0 >= p.lo && v0 + 32 <= min(p.hi, vb); };
+  auto fetch = [&](int v0) {
+    const int t0 = p.e0 + (v0 + lane) * 8;
+    next_x.load(row, init, t0);
+    next_g.load(grad + t0);
+  };
+  const int top = va + ((vb - va - 1) >> 5) * 32;
+  if (va < vb && inside(top)) fetch(top);
+  for (int v0 = top; v0 >= va && va < vb; v0 -= 32) {
+    const int v = v0 + lane, t0 = p.e0 + v * 8;
+    const bool in = inside(v0);
+    float x[K + 7], dp[8 + B], g[8];
+    if (in) {
+      next_x.get(x);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+      for (int i = 0; i < 8; ++i) dp[i] = next_g.f(i);
+    }
+    if (v0 - 32 >= va && inside(v0 - 32)) fetch(v0 - 32);
+    if (in) {
+      if (a.silu) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dp[i] = 0.f;
-    if (v < vb) dpre8<T, K>(a, row, grad, init, t0, p.n, w, bias, x, dp);
+        for (int i = 0; i < 8; ++i) dp[i] *= silu_slope(filter<K>(w, bias, x, i));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < K + 7; ++i) x[i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dp[i] = 0.f;
+      if (v < vb && t0 < p.n) dpre_any<T, K>(a, row, grad, init, t0, p.n, w, bias, x, dp);
+    }
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
       // the last vector of the run may sit in any lane: lanes behind it hold
@@ -220,32 +315,33 @@ __global__ void __launch_bounds__(kConvThreads) conv_backward_kernel(ConvArgs a)
       dp[8 + k] = lane == 31 || v == vb - 1 ? carry[k] : next;
       carry[k] = first;
     }
-    if (v < vb) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      db += dp[i];
+#pragma unroll
+      for (int k = 0; k < K; ++k) dw[k] = fmaf(dp[i], x[i + k], dw[k]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      g[i] = w[K - 1] * dp[i];
+#pragma unroll
+      for (int k = 1; k < K; ++k) g[i] = fmaf(w[K - 1 - k], dp[i + k], g[i]);
+    }
+    if (K > 1 && dfinal && t0 + 8 + K - 1 > p.n) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        db += dp[i];
-#pragma unroll
-        for (int k = 0; k < K; ++k) dw[k] = fmaf(dp[i], x[8 + i - (K - 1) + k], dw[k]);
-      }
-      float g[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        g[i] = 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) g[i] = fmaf(w[K - 1 - k], dp[i + k], g[i]);
         const int j = t0 + i + (K - 1) - p.n;
-        if (K > 1 && dfinal && j >= 0 && t0 + i >= 0 && t0 + i < p.n) g[i] += to_f(dfinal[j]);
+        if (j >= 0 && t0 + i >= 0 && t0 + i < p.n) g[i] += to_f(dfinal[j]);
       }
-      if (t0 >= 0 && t0 + 8 <= a.length) {
-        Pack<T, 8> o;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o.v[i] = from_f<T>(t0 + i < p.n ? g[i] : 0.f);
-        o.store(dx + t0);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (t0 + i >= 0 && t0 + i < a.length) dx[t0 + i] = from_f<T>(t0 + i < p.n ? g[i] : 0.f);
-      }
+    }
+    if (in) {
+      Pack<T, 8> o;
+      o.set(g);
+      o.store(dx + t0);
+    } else if (v < vb) {
+      // (behind the last token dpre is 0, and so is g but for the K-1 elements
+      // before the first, which are not stored)
+      store8(dx, t0, a.length, g);
     }
   }
   // the warp's share of the parameter gradients, in a fixed order
@@ -266,8 +362,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_backward_kernel(ConvArgs a)
         float s = bias;
 #pragma unroll
         for (int k = 0; k < K; ++k) s = fmaf(w[k], line_at<T, K>(row, init, lane + k), s);
-        const float e = sigmoid_f(s);
-        dpj *= e * fmaf(s, 1.f - e, 1.f);
+        dpj *= silu_slope(s);
       }
     }
     float g = 0.f;
@@ -317,23 +412,29 @@ template <typename T, int K>
 __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(ConvStepArgs a) {
   const int nblk = (a.channels + kConvThreads - 1) / kConvThreads;
   const int b = blockIdx.x / nblk;
-  bool bad;
-  const int place = step_place(a.slots, b, a.places, &bad);
+  StepKind kind;
+  const int place = step_place(a.slots, b, a.places, &kind);
   const int d = (blockIdx.x - b * nblk) * kConvThreads + threadIdx.x;
-  if (d >= a.channels) return;
-  T *out = static_cast<T *>(a.out) + (int64_t)b * a.channels + d;
-  if (place < 0) {
-    *out = from_f<T>(bad ? __int_as_float(0x7fffffff) : 0.f);
-    return;
-  }
+  const bool valid = d < a.channels;
+  const int64_t at = (int64_t)b * a.channels + d;
   T *kept = static_cast<T *>(a.state) + ((int64_t)place * a.channels + d) * (K - 1);
   T line[K];
+  float s = 0.f;
+  if (valid && kind == kStepServed) {
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) line[k] = kept[k];
-  line[K - 1] = static_cast<const T *>(a.x)[(int64_t)b * a.channels + d];
-  float s = a.bias ? load_param(a.bias, a.wdtype, d) : 0.f;
+    for (int k = 0; k < K - 1; ++k) line[k] = kept[k];
+    line[K - 1] = static_cast<const T *>(a.x)[at];
+    if (a.bias) s = load_param(a.bias, a.wdtype, d);
 #pragma unroll
-  for (int k = 0; k < K; ++k) s = fmaf(load_param(a.weight, a.wdtype, (int64_t)d * K + k), to_f(line[k]), s);
+    for (int k = 0; k < K; ++k) s = fmaf(load_param(a.weight, a.wdtype, (int64_t)d * K + k), to_f(line[k]), s);
+  }
+  kind = step_served(a.slots, b, place, kind);
+  if (!valid) return;
+  T *out = static_cast<T *>(a.out) + at;
+  if (kind != kStepServed) {
+    *out = from_f<T>(step_nothing(kind));
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < K - 1; ++k) kept[k] = line[k + 1];
   *out = from_f<T>(a.silu ? s * sigmoid_f(s) : s);

@@ -1020,63 +1020,75 @@ struct ScanStepArgs {
   int batch, places, channels, states, groups, per_group, softplus, nblk;
 };
 
-// One token: reads and writes each state once (8 bytes a state: what bounds it).
+// One token: reads and writes each state once (8 bytes a state: what bounds
+// it).  All reads are on their way before the block learns whether it may write.
+constexpr int kStepThreads = 256;
 
 template <typename T, int P>
-__global__ void __launch_bounds__(kThreads) scan_step_kernel(ScanStepArgs a) {
-  constexpr int CB = kThreads / P;
+__global__ void __launch_bounds__(kStepThreads) scan_step_kernel(ScanStepArgs a) {
+  constexpr int CB = kStepThreads / P;
   const int b = blockIdx.x / a.nblk, blk = blockIdx.x - b * a.nblk;
   const int p = threadIdx.x % P, d = blk * CB + threadIdx.x / P, N = a.states;
   const bool valid = d < a.channels;
-  bool bad;
-  const int place = step_place(a.slots, b, a.places, &bad);
+  StepKind kind;
+  const int place = step_place(a.slots, b, a.places, &kind);
   const int64_t i = (int64_t)b * a.channels + (valid ? d : 0);
-  if (place < 0) {
-    if (valid && p == 0) static_cast<T *>(a.out)[i] = from_f<T>(bad ? __int_as_float(0x7fffffff) : 0.f);
-    return;
-  }
   const int dd = valid ? d : 0, g = dd / a.per_group;
   float *state = a.state + ((int64_t)place * a.channels + dd) * N;
-  alignas(16) float A2[kS], h[kS];
-  float y = 0.f;
-  const bool vec = N % kS == 0;
-  if (vec && p * kS < N) {
-    *reinterpret_cast<float4 *>(h) = *reinterpret_cast<const float4 *>(state + p * kS);
-    *reinterpret_cast<float4 *>(A2) = *reinterpret_cast<const float4 *>(a.A + (int64_t)dd * N + p * kS);
-  } else {
+  F2 A2[kH], h[kH];
+  float y = 0.f, u = 0.f, z = 0.f;
+  if (kind == kStepServed) {
+    const bool four = N % kS == 0;
+    float bb[kS], cc[kS];
+    const T *B = static_cast<const T *>(a.B) + ((int64_t)b * a.groups + g) * N + p * kS;
+    const T *C = static_cast<const T *>(a.C) + ((int64_t)b * a.groups + g) * N + p * kS;
+    if (four && p * kS < N) {
+      load_pairs(state + p * kS, h);
+      load_pairs(a.A + (int64_t)dd * N + p * kS, A2);
+      Pack<T, kS> vb, vc;
+      vb.load(B);
+      vc.load(C);
 #pragma unroll
-    for (int s = 0; s < kS; ++s) {
-      h[s] = p * kS + s < N ? state[p * kS + s] : 0.f;
-      A2[s] = p * kS + s < N ? a.A[(int64_t)dd * N + p * kS + s] : 0.f;
-    }
-  }
-  const float u = to_f(static_cast<const T *>(a.u)[i]);
-  float delta = to_f(static_cast<const T *>(a.delta)[i]) + (a.bias ? a.bias[dd] : 0.f);
-  if (a.softplus) delta = softplus_f(delta);
-  const T *B = static_cast<const T *>(a.B) + ((int64_t)b * a.groups + g) * N;
-  const T *C = static_cast<const T *>(a.C) + ((int64_t)b * a.groups + g) * N;
+      for (int s = 0; s < kS; ++s) {
+        bb[s] = vb.f(s);
+        cc[s] = vc.f(s);
+      }
+    } else {
+      load_states(state, N, p, h);
+      load_states(a.A + (int64_t)dd * N, N, p, A2);
 #pragma unroll
-  for (int s = 0; s < kS; ++s) {
-    const int n = p * kS + s;
-    if (n < N) {
-      h[s] = fmaf(exp2_f(delta * (A2[s] * kLog2e)), h[s], delta * u * to_f(B[n]));
-      y = fmaf(h[s], to_f(C[n]), y);
+      for (int s = 0; s < kS; ++s) {
+        const bool in = p * kS + s < N;
+        bb[s] = in ? to_f(B[s]) : 0.f;
+        cc[s] = in ? to_f(C[s]) : 0.f;
+      }
     }
-  }
-  if (valid) {
-    const F2 pairs[kH] = {F2(h[0], h[1]), F2(h[2], h[3])};
-    store_states(state, N, p, pairs);
+    u = to_f(static_cast<const T *>(a.u)[i]);
+    float delta = to_f(static_cast<const T *>(a.delta)[i]) + (a.bias ? a.bias[dd] : 0.f);
+    if (a.z) z = to_f(static_cast<const T *>(a.z)[i]);
+    if (a.softplus) delta = softplus_f(delta);
+    const F2 d2(delta * kLog2e, delta * kLog2e), x2(delta * u, delta * u);
+    F2 c2[kH];
+#pragma unroll
+    for (int s = 0; s < kH; ++s) {
+      const F2 x = mul2(d2, A2[s]);
+      h[s] = fma2(F2(exp2_tile(x.x()), exp2_tile(x.y())), h[s], mul2(x2, F2(bb[2 * s], bb[2 * s + 1])));
+      c2[s] = F2(cc[2 * s], cc[2 * s + 1]);
+    }
+    y = dot(h, c2);
   }
 #pragma unroll
   for (int o = 1; o < P; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-  if (valid && p == 0) {
+  kind = step_served(a.slots, b, place, kind);
+  if (!valid) return;
+  if (kind == kStepServed) {
+    store_states(state, N, p, h);
     if (a.skip) y = fmaf(a.skip[dd], u, y);
-    if (a.z) {
-      const float z = to_f(static_cast<const T *>(a.z)[i]);
-      y *= z * sigmoid_f(z);
-    }
-    static_cast<T *>(a.out)[i] = from_f<T>(y);
+    if (a.z) y *= z * sigmoid_f(z);
+  } else {
+    y = step_nothing(kind);
   }
+  if (p == 0) static_cast<T *>(a.out)[i] = from_f<T>(y);
 }
 
 // --------------------------------------------------------------------- host
@@ -1372,11 +1384,11 @@ extern "C" int pc2d_ssm_scan_step(int dtype, const void *u, const void *delta, f
   a.batch = batch; a.places = places; a.channels = channels; a.states = states; a.groups = groups;
   a.per_group = channels / groups;
   a.softplus = delta_softplus != 0;
-  const int cb = kThreads / lanes_of(states);
+  const int cb = kStepThreads / lanes_of(states);
   a.nblk = (channels + cb - 1) / cb;
   return by_type_and_layout(dtype, states, [&](auto t, auto layout) -> int {
     scan_step_kernel<decltype(t), decltype(layout)::P>
-        <<<(unsigned)((int64_t)a.nblk * batch), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+        <<<(unsigned)((int64_t)a.nblk * batch), kStepThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
     PC2D_LAUNCH_CHECK("scan_step_kernel");
     return PC2D_OK;
   });

@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "pc2d_common.cuh"
 
 namespace pc2d {
@@ -65,12 +67,32 @@ struct Pack {
     }
   }
   __device__ __forceinline__ float f(int i) const { return to_f(v[i]); }
+  // all N (even) at once: the 16-bit types round two per instruction
+  __device__ __forceinline__ void set(const float (&x)[N]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = x[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        if constexpr (std::is_same<T, __half>::value)
+          *reinterpret_cast<__half2 *>(v + i) = __floats2half2_rn(x[i], x[i + 1]);
+        else
+          *reinterpret_cast<__nv_bfloat162 *>(v + i) = __floats2bfloat162_rn(x[i], x[i + 1]);
+      }
+    }
+  }
 };
 
-// 1 / (1 + exp(-v)): 0 and 1 at the infinities.  __expf and __fdividef are off
-// by a few units of the last place, far below the bf16/fp16 rounding and of
-// the size of an fp32 sum's own roundings.
-__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+// 1 / (1 + exp(-v)): 0 and 1 at the infinities.  The two hardware functions and
+// the argument's rounding leave it off by 4 + |v| units of 2^-24 where v < 0, less
+// elsewhere.
+__device__ __forceinline__ float sigmoid_f(float v) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return r;
+}
 
 // Element types the sequence operators take.
 inline bool seq_dtype(int dtype) {
@@ -84,16 +106,25 @@ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 // padding (its output is 0).  A place outside the array, and one that an
 // earlier row has already, cannot be served: the output is NaN and no state
 // is touched, so that the mistake is seen and the result does not depend on
-// which of two blocks came first.  The whole block calls this.
-__device__ __forceinline__ int step_place(const int *slots, int b, int places, bool *bad) {
-  *bad = false;
-  if (!slots) return b;
-  const int place = slots[b];
-  if (place == -1) return -1;
-  int twice = place < 0 || place >= places;
+// which of two blocks came first.
+//
+// step_place gives a place that may be read (0 for rows that have none, where
+// the array has any); step_served, which the whole block calls after its reads
+// are on their way, says whether it may be written.
+enum StepKind { kStepServed, kStepPadding, kStepBad };
+__device__ __forceinline__ int step_place(const int *slots, int b, int places, StepKind *kind) {
+  const int place = slots ? slots[b] : b;
+  *kind = place == -1 ? kStepPadding : place < 0 || place >= places ? kStepBad : kStepServed;
+  return *kind == kStepServed ? place : 0;
+}
+__device__ __forceinline__ StepKind step_served(const int *slots, int b, int place, StepKind kind) {
+  if (!slots || kind != kStepServed) return kind;  // (the same in the whole block)
+  int twice = 0;
   for (int i = threadIdx.x; i < b; i += blockDim.x) twice |= slots[i] == place;
-  *bad = __syncthreads_or(twice) != 0;
-  return *bad ? -1 : place;
+  return __syncthreads_or(twice) ? kStepBad : kStepServed;
+}
+__device__ __forceinline__ float step_nothing(StepKind kind) {
+  return kind == kStepBad ? __int_as_float(0x7fffffff) : 0.f;
 }
 
 }  // namespace pc2d

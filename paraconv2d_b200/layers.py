@@ -36,11 +36,27 @@ from torch.autograd.function import once_differentiable
 from ._lib import load_op_library
 
 load_op_library()
-_ops = torch.ops.paraconv2d_b200
+
+
+class _ops:
+    """The C++ ops, their overloads looked up once."""
+
+    dropout = torch.ops.paraconv2d_b200.dropout.default
+    dropout_next_key = torch.ops.paraconv2d_b200.dropout_next_key.default
+    causal_conv_forward = torch.ops.paraconv2d_b200.causal_conv_forward.default
+    causal_conv_backward = torch.ops.paraconv2d_b200.causal_conv_backward.default
+    causal_conv_step = torch.ops.paraconv2d_b200.causal_conv_step.default
+    ssm_scan_forward = torch.ops.paraconv2d_b200.ssm_scan_forward.default
+    ssm_scan_backward = torch.ops.paraconv2d_b200.ssm_scan_backward.default
+    ssm_scan_step = torch.ops.paraconv2d_b200.ssm_scan_step.default
 
 
 def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _no_step_grad(what, *tensors):
