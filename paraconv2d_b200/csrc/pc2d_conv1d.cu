@@ -13,10 +13,10 @@
 //
 // All of it is a few operations per element: the kernels stream.  A warp takes
 // a run of one row, and a lane eight elements at a time, cut at the
-// 8-element boundaries of the whole array rather than of the row: every load
-// and store inside a row is then a 16-byte vector whatever the length is, and
-// only the (at most two) vectors that a row shares with its neighbours go
-// element by element.
+// 8-element boundaries of the whole array rather than of the row: every load is
+// then a 16-byte vector whatever the length is.  In the vectors that a row
+// shares with its neighbours, and behind its last token, the foreign elements
+// are replaced; only those vectors are stored element by element.
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>
@@ -27,7 +27,7 @@
 namespace pc2d {
 namespace {
 
-constexpr int kConvThreads = 256;
+constexpr int kConvThreads = 128;
 constexpr int kMaxTaps = 8;
 
 struct ConvArgs {
@@ -71,7 +71,6 @@ struct RowPlace {
   int64_t base;   // first element of the row in the array
   int e0;         // t of the first element of the row's vector 0: 0 or below
   int nvec;       // vectors that hold elements of the row
-  int lo, hi;     // vectors lo .. hi-1 lie within the row's tokens
 };
 
 __device__ __forceinline__ bool place_of(const ConvArgs &a, RowPlace *p) {
@@ -87,8 +86,6 @@ __device__ __forceinline__ bool place_of(const ConvArgs &a, RowPlace *p) {
   const int over = (int)(p->base & 7);
   p->e0 = -over;
   p->nvec = (int)(((int64_t)a.length + over + 7) >> 3);
-  p->lo = over ? 1 : 0;
-  p->hi = (p->n + over) >> 3;
   return true;
 }
 
@@ -97,49 +94,56 @@ __device__ __forceinline__ bool place_of(const ConvArgs &a, RowPlace *p) {
 template <int K>
 constexpr int kBefore = K <= 5 ? 4 : 8;
 
-// A vector within the row's tokens: its eight elements behind those before it,
-// which for the row's first vector may be the kept state's or zeros.
+// One vector of the array, and what its windows need of the one before.
 template <typename T, int K>
 struct Window {
   Pack<T, 8> cur;
   Pack<T, kBefore<K>> before;
-  __device__ __forceinline__ void load(const T *row, const T *init, int t0) {
-    cur.load(row + t0);
-    if (K == 1) return;
-    if (t0 >= kBefore<K>) {
-      before.load(row + t0 - kBefore<K>);
-    } else {
-#pragma unroll
-      for (int k = 0; k < K - 1; ++k) {
-        const int t = t0 - (K - 1) + k;
-        T v = from_f<T>(0.f);
-        if (t >= 0) v = row[t];
-        else if (init) v = init[t + K - 1];
-        before.v[kBefore<K> - (K - 1) + k] = v;
-      }
+  // `at`: the vector's first element in the array of `total`.  kInside: the
+  // vector lies within the array.
+  template <bool kInside>
+  __device__ __forceinline__ void load(const T *array, int64_t at, int64_t total) {
+    load8<kInside>(cur, array, at, total);
+    // (before the array's first vector there is nothing: any values do, as they
+    // are replaced)
+    if (K > 1) {
+      if (kInside) before.load(array + (at > 0 ? at - kBefore<K> : at));
+      else if (at > 0) before.load(array + at - kBefore<K>);
     }
   }
-  // the 7 + K values of the line that the vector's windows cover
-  __device__ __forceinline__ void get(float (&x)[K + 7]) const {
+  template <bool kInside>
+  __device__ static __forceinline__ void load8(Pack<T, 8> &v, const T *array, int64_t at, int64_t total) {
+    if (kInside || at + 8 <= total) {
+      v.load(array + at);
+    } else {  // the array's last elements
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (at + i < total) v.v[i] = array[at + i];
+    }
+  }
+  // The 7 + K values of the row's line that the windows of its elements t0 ..
+  // t0+7 cover: zeros behind the n tokens, the kept state's (or zeros) before.
+  // kInside: no element lies behind them.
+  template <bool kInside>
+  __device__ __forceinline__ void get(float (&x)[K + 7], int t0, int n, const T *init) const {
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) x[k] = before.f(kBefore<K> - (K - 1) + k);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[K - 1 + i] = cur.f(i);
+    if (t0 < K - 1) {  // (the first one or two vectors of a row)
+#pragma unroll
+      for (int i = 0; i < K + 6; ++i) {
+        const int t = t0 + i - (K - 1);
+        if (t < 0) x[i] = init && t >= -(K - 1) ? to_f(init[t + K - 1]) : 0.f;
+      }
+    }
+    if (!kInside && t0 + 8 > n) {
+#pragma unroll
+      for (int i = 0; i < K + 7; ++i)
+        if (t0 + i - (K - 1) >= n) x[i] = 0.f;
+    }
   }
 };
-
-// The same for any vector of a row: zeros outside [0, n), the kept state's
-// values before 0.
-template <typename T, int K>
-__device__ __forceinline__ void load_window(const T *row, const T *init, int t0, int n, float (&x)[K + 7]) {
-#pragma unroll
-  for (int i = 0; i < K + 7; ++i) {
-    const int t = t0 + i - (K - 1);
-    x[i] = 0.f;
-    if (t >= 0 && t < n) x[i] = to_f(row[t]);
-    else if (init && t < 0 && t >= -(K - 1)) x[i] = to_f(init[t + K - 1]);
-  }
-}
 
 template <int K>
 __device__ __forceinline__ float filter(const float (&w)[K], float bias, const float (&x)[K + 7], int i) {
@@ -162,62 +166,68 @@ __device__ __forceinline__ void store8(T *row, int t0, int length, const float (
   }
 }
 
-constexpr int kConvUnroll = 2;  // vectors in flight per lane
+// Two vectors in flight per lane, and as many blocks per SM as hold them without
+// spilling (4 x 4096 x 2048 bf16 with 4 taps: 33 us, 4.1 TB/s, against 38 with
+// the compiler's choice of registers and 36 with four vectors).
+constexpr int kConvUnroll = 2;
+template <typename T, int K>
+constexpr int kConvFwdBlocks = sizeof(T) == 2 && K <= 5 ? 8 : 5;
 
 template <typename T, int K>
-__global__ void __launch_bounds__(kConvThreads) conv_forward_kernel(ConvArgs a) {
+__global__ void __launch_bounds__(kConvThreads, kConvFwdBlocks<T, K>) conv_forward_kernel(ConvArgs a) {
+  constexpr int U = kConvUnroll;
   RowPlace p;
   if (!place_of(a, &p)) return;
   const int lane = threadIdx.x & 31;
-  const T *row = static_cast<const T *>(a.x) + p.base;
+  const T *array = static_cast<const T *>(a.x), *row = array + p.base;
   T *out = static_cast<T *>(a.out) + p.base;
   const T *init = a.init ? static_cast<const T *>(a.init) + p.row * (K - 1) : nullptr;
+  const int64_t total = a.rows * a.length;
+  float last = 0.f;
+  const bool ends = a.final_state && p.seg == 0 && lane < K - 1;
+  if (ends) last = line_at<T, K>(row, init, p.n + lane);
   float w[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) w[k] = load_param(a.weight, a.wdtype, (int64_t)p.d * K + k);
   const float bias = a.bias ? load_param(a.bias, a.wdtype, p.d) : 0.f;
-  const int va = p.seg * a.seg, vb = min(p.nvec, va + a.seg);
-  const int lo = max(va, p.lo), hi = min(vb, p.hi);
-  // the vectors within the tokens
-  for (int v0 = lo + lane; v0 < hi; v0 += 32 * kConvUnroll) {
-    Window<T, K> win[kConvUnroll];
+  const int vb = min(p.nvec, (p.seg + 1) * a.seg);
+  // U vectors per lane; kInside: all of them, in all lanes, within the tokens
+  auto vectors = [&](int v0, auto inside) {
+    constexpr bool kInside = decltype(inside)::value;
+    Window<T, K> win[U];
 #pragma unroll
-    for (int u = 0; u < kConvUnroll; ++u)
-      if (v0 + 32 * u < hi) win[u].load(row, init, p.e0 + (v0 + 32 * u) * 8);
+    for (int u = 0; u < U; ++u) {
+      const int v = v0 + lane + 32 * u, t0 = p.e0 + v * 8;
+      if (kInside || (v < vb && t0 < p.n)) win[u].template load<kInside>(array, p.base + t0, total);
+    }
 #pragma unroll
-    for (int u = 0; u < kConvUnroll; ++u) {
-      if (v0 + 32 * u >= hi) break;
+    for (int u = 0; u < U; ++u) {
+      const int v = v0 + lane + 32 * u, t0 = p.e0 + v * 8;
+      if (!kInside && v >= vb) break;
       float x[K + 7], y[8];
-      win[u].get(x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        y[i] = filter<K>(w, bias, x, i);
-        if (a.silu) y[i] *= sigmoid_f(y[i]);
-      }
-      Pack<T, 8> o;
-      o.set(y);
-      o.store(out + p.e0 + (v0 + 32 * u) * 8);
-    }
-  }
-  // those that reach beyond them: at most one before, and all behind
-  auto edge = [&](int v) {
-    const int t0 = p.e0 + v * 8;
-    float x[K + 7], y[8];
-    if (t0 < p.n) load_window<T, K>(row, init, t0, p.n, x);
+      for (int i = 0; i < 8; ++i) y[i] = 0.f;
+      if (kInside || t0 < p.n) {
+        win[u].template get<kInside>(x, t0, p.n, init);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      y[i] = 0.f;
-      if (t0 + i < p.n) {
-        y[i] = filter<K>(w, bias, x, i);
-        if (a.silu) y[i] *= sigmoid_f(y[i]);
+        for (int i = 0; i < 8; ++i) {
+          y[i] = filter<K>(w, bias, x, i);
+          if (a.silu) y[i] *= sigmoid_f(y[i]);
+        }
+        if (!kInside && t0 + 8 > p.n) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (t0 + i >= p.n) y[i] = 0.f;
+        }
       }
+      store8(out, t0, a.length, y);
     }
-    store8(out, t0, a.length, y);
   };
-  if (va < lo && lane == 0 && va < vb) edge(va);
-  for (int v = max(hi, lo) + lane; v < vb; v += 32) edge(v);
-  if (a.final_state && p.seg == 0 && lane < K - 1)
-    static_cast<T *>(a.final_state)[p.row * (K - 1) + lane] = from_f<T>(line_at<T, K>(row, init, p.n + lane));
+  for (int v0 = p.seg * a.seg; v0 < vb; v0 += 32 * U) {
+    if (v0 + 32 * U <= vb && p.e0 + (v0 + 32 * U) * 8 <= p.n) vectors(v0, std::true_type{});
+    else vectors(v0, std::false_type{});
+  }
+  if (ends) static_cast<T *>(a.final_state)[p.row * (K - 1) + lane] = from_f<T>(last);
 }
 
 __device__ __forceinline__ float silu_slope(float v) {
@@ -225,37 +235,62 @@ __device__ __forceinline__ float silu_slope(float v) {
   return e * fmaf(v, 1.f - e, 1.f);
 }
 
-// dpre of the eight elements from t0 on, of any vector (zeros outside [0, n)),
-// and the values that their windows cover.
+// A vector's inputs of the backward pass.
 template <typename T, int K>
-__device__ __forceinline__ void dpre_any(const ConvArgs &a, const T *row, const T *grad, const T *init, int t0, int n,
-                                         const float (&w)[K], float bias, float (&x)[K + 7], float *dp) {
-  load_window<T, K>(row, init, t0, n, x);
+struct BackWindow {
+  Window<T, K> x;
+  Pack<T, 8> g;
+  template <bool kInside>
+  __device__ __forceinline__ void load(const ConvArgs &a, int64_t at, int64_t total) {
+    x.template load<kInside>(static_cast<const T *>(a.x), at, total);
+    Window<T, K>::template load8<kInside>(g, static_cast<const T *>(a.grad), at, total);
+  }
+  // the values that its windows cover, and dpre (zeros outside [0, n))
+  __device__ __forceinline__ void get(const ConvArgs &a, int t0, int n, const T *init, const float (&w)[K], float bias,
+                                      float (&v)[K + 7], float *dp) const {
+    x.template get<false>(v, t0, n, init);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    dp[i] = 0.f;
-    if (t0 + i >= 0 && t0 + i < n) {
-      dp[i] = to_f(grad[t0 + i]);
-      if (a.silu) dp[i] *= silu_slope(filter<K>(w, bias, x, i));
+    for (int i = 0; i < 8; ++i) dp[i] = g.f(i);
+    if (a.silu) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dp[i] *= silu_slope(filter<K>(w, bias, v, i));
+    }
+    if (t0 < 0 || t0 + 8 > n) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (t0 + i < 0 || t0 + i >= n) dp[i] = 0.f;
     }
   }
-}
+};
+
+// Blocks per SM, by the registers that they leave (4 x 4096 x 2048 bf16 with 4
+// taps: 67 us, 3.0 TB/s, with 7; 72 with 6, 73 with 8).
+template <typename T, int K>
+constexpr int kConvBackBlocks = K <= 4 ? (sizeof(T) == 2 ? 7 : 6) : 4;
 
 // A warp goes through its run from the end to the beginning, 32 vectors at a
 // time: the K-1 values of dpre behind a lane's eight come from the next lane,
 // and for lane 31 from lane 0 of the 32 vectors done before (for the first ones
 // from a computation of the vector behind the run).  The inputs of 32 vectors
-// within the row's tokens are loaded while those before are computed.
+// are loaded while those before are computed.
 template <typename T, int K>
-__global__ void __launch_bounds__(kConvThreads) conv_backward_kernel(ConvArgs a) {
+__global__ void __launch_bounds__(kConvThreads, kConvBackBlocks<T, K>) conv_backward_kernel(ConvArgs a) {
   RowPlace p;
   if (!place_of(a, &p)) return;
   const int lane = threadIdx.x & 31;
-  const T *row = static_cast<const T *>(a.x) + p.base;
-  const T *grad = static_cast<const T *>(a.grad) + p.base;
   const T *init = a.init ? static_cast<const T *>(a.init) + p.row * (K - 1) : nullptr;
   const T *dfinal = a.grad_final ? static_cast<const T *>(a.grad_final) + p.row * (K - 1) : nullptr;
   T *dx = static_cast<T *>(a.dx) + p.base;
+  const int64_t total = a.rows * a.length;
+  const int va = p.seg * a.seg, vb = min(p.nvec, va + a.seg);
+  const int top = va + ((vb - va - 1) >> 5) * 32;
+  BackWindow<T, K> next;
+  auto fetch = [&](int v0) {
+    const int t0 = p.e0 + (v0 + lane) * 8;
+    if (v0 + 32 <= vb && p.e0 + (v0 + 32) * 8 <= p.n) next.template load<true>(a, p.base + t0, total);
+    else if (v0 + lane < vb && t0 < p.n) next.template load<false>(a, p.base + t0, total);
+  };
+  if (va < vb) fetch(top);
   float w[K], dw[K], db = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -263,56 +298,37 @@ __global__ void __launch_bounds__(kConvThreads) conv_backward_kernel(ConvArgs a)
     dw[k] = 0.f;
   }
   const float bias = a.bias ? load_param(a.bias, a.wdtype, p.d) : 0.f;
-  const int va = p.seg * a.seg, vb = min(p.nvec, va + a.seg);
   constexpr int B = K > 1 ? K - 1 : 1;
   float carry[B];  // dpre of the first elements of the vector behind
 #pragma unroll
   for (int k = 0; k < B; ++k) carry[k] = 0.f;
-  if (K > 1 && va < vb && vb < p.nvec) {
+  if (K > 1 && va < vb && vb < p.nvec && p.e0 + vb * 8 < p.n) {
+    BackWindow<T, K> behind;
     float x[K + 7], dp[8];
-    dpre_any<T, K>(a, row, grad, init, p.e0 + vb * 8, p.n, w, bias, x, dp);
+    behind.template load<false>(a, p.base + p.e0 + vb * 8, total);
+    behind.get(a, p.e0 + vb * 8, p.n, init, w, bias, x, dp);
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) carry[k] = dp[k];
   }
-  Window<T, K> next_x;
-  Pack<T, 8> next_g;
-  auto inside = [&](int v0) { return v0 >= p.lo && v0 + 32 <= min(p.hi, vb); };
-  auto fetch = [&](int v0) {
-    const int t0 = p.e0 + (v0 + lane) * 8;
-    next_x.load(row, init, t0);
-    next_g.load(grad + t0);
-  };
-  const int top = va + ((vb - va - 1) >> 5) * 32;
-  if (va < vb && inside(top)) fetch(top);
   for (int v0 = top; v0 >= va && va < vb; v0 -= 32) {
     const int v = v0 + lane, t0 = p.e0 + v * 8;
-    const bool in = inside(v0);
     float x[K + 7], dp[8 + B], g[8];
-    if (in) {
-      next_x.get(x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) dp[i] = next_g.f(i);
-    }
-    if (v0 - 32 >= va && inside(v0 - 32)) fetch(v0 - 32);
-    if (in) {
-      if (a.silu) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dp[i] *= silu_slope(filter<K>(w, bias, x, i));
-      }
+    if (v < vb && t0 < p.n) {
+      next.get(a, t0, p.n, init, w, bias, x, dp);
     } else {
 #pragma unroll
       for (int i = 0; i < K + 7; ++i) x[i] = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) dp[i] = 0.f;
-      if (v < vb && t0 < p.n) dpre_any<T, K>(a, row, grad, init, t0, p.n, w, bias, x, dp);
     }
+    if (v0 > va) fetch(v0 - 32);
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
       // the last vector of the run may sit in any lane: lanes behind it hold
       // zeros, so it takes the carry itself
-      const float next = __shfl_down_sync(0xffffffffu, dp[k], 1);
+      const float behind = __shfl_down_sync(0xffffffffu, dp[k], 1);
       const float first = __shfl_sync(0xffffffffu, dp[k], 0);
-      dp[8 + k] = lane == 31 || v == vb - 1 ? carry[k] : next;
+      dp[8 + k] = lane == 31 || v == vb - 1 ? carry[k] : behind;
       carry[k] = first;
     }
 #pragma unroll
@@ -334,30 +350,26 @@ __global__ void __launch_bounds__(kConvThreads) conv_backward_kernel(ConvArgs a)
         if (j >= 0 && t0 + i >= 0 && t0 + i < p.n) g[i] += to_f(dfinal[j]);
       }
     }
-    if (in) {
-      Pack<T, 8> o;
-      o.set(g);
-      o.store(dx + t0);
-    } else if (v < vb) {
-      // (behind the last token dpre is 0, and so is g but for the K-1 elements
-      // before the first, which are not stored)
-      store8(dx, t0, a.length, g);
-    }
+    // (behind the last token dpre is 0, and so is g)
+    if (v < vb) store8(dx, t0, a.length, g);
   }
   // the warp's share of the parameter gradients, in a fixed order
+  float mine = 0.f;
 #pragma unroll
   for (int k = 0; k <= K; ++k) {
     float s = k < K ? dw[k < K ? k : 0] : db;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const int64_t b = p.row / a.channels;
-    if (lane == 0) a.part[((b * a.nseg + p.seg) * (K + 1) + k) * a.channels + p.d] = s;
+    if (lane == k) mine = s;
   }
+  const int64_t b = p.row / a.channels;
+  if (lane <= K) a.part[((b * a.nseg + p.seg) * (K + 1) + lane) * a.channels + p.d] = mine;
   if (K > 1 && a.dinit && p.seg == 0) {
     // dline[s], s < K-1: lane j computes dpre[j] from its own window
+    const T *row = static_cast<const T *>(a.x) + p.base;
     float dpj = 0.f;
     if (lane < K - 1 && lane < p.n) {
-      dpj = to_f(grad[lane]);
+      dpj = to_f(static_cast<const T *>(a.grad)[p.base + lane]);
       if (a.silu) {
         float s = bias;
 #pragma unroll
@@ -414,6 +426,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(ConvStepArgs a)
   const int b = blockIdx.x / nblk;
   StepKind kind;
   const int place = step_place(a.slots, b, a.places, &kind);
+  const int twice = step_twice(a.slots, b, place, kind);
   const int d = (blockIdx.x - b * nblk) * kConvThreads + threadIdx.x;
   const bool valid = d < a.channels;
   const int64_t at = (int64_t)b * a.channels + d;
@@ -428,7 +441,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(ConvStepArgs a)
 #pragma unroll
     for (int k = 0; k < K; ++k) s = fmaf(load_param(a.weight, a.wdtype, (int64_t)d * K + k), to_f(line[k]), s);
   }
-  kind = step_served(a.slots, b, place, kind);
+  kind = step_served(twice, kind);
   if (!valid) return;
   T *out = static_cast<T *>(a.out) + at;
   if (kind != kStepServed) {
@@ -443,12 +456,16 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(ConvStepArgs a)
 enum ConvWhat { kConvForward, kConvBackward };
 
 // Vectors per warp: long runs amortise a warp's set-up (parameters, the vector
-// behind the run), short ones fill the GPU when there are few rows.
+// behind the run), short ones fill the GPU when there are few rows.  Runs of a
+// row are equally long, in whole groups of 32 vectors.
 void conv_split(const ConvArgs &a, int *nseg, int *seg) {
-  const int nvec = (int)(((int64_t)a.length + 7 + 7) >> 3);
-  int iters = 8;
-  while (iters > 1 && a.rows * ((nvec + 32 * iters - 1) / (32 * iters)) < (int64_t)device_sm_count() * 32) iters /= 2;
-  *seg = 32 * iters;
+  // (a row that starts off a vector boundary reaches into one vector more)
+  const int nvec = a.length % 8 == 0 ? a.length / 8 : (int)(((int64_t)a.length + 14) >> 3);
+  const int groups = std::max(1, (nvec + 31) / 32);
+  int most = 8;
+  while (most > 1 && a.rows * ((groups + most - 1) / most) < (int64_t)device_sm_count() * 32) most /= 2;
+  const int runs = (groups + most - 1) / most;
+  *seg = 32 * ((groups + runs - 1) / runs);
   *nseg = std::max(1, (nvec + *seg - 1) / *seg);
 }
 

@@ -1032,6 +1032,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(ScanStepArgs a)
   const bool valid = d < a.channels;
   StepKind kind;
   const int place = step_place(a.slots, b, a.places, &kind);
+  const int twice = step_twice(a.slots, b, place, kind);
   const int64_t i = (int64_t)b * a.channels + (valid ? d : 0);
   const int dd = valid ? d : 0, g = dd / a.per_group;
   float *state = a.state + ((int64_t)place * a.channels + dd) * N;
@@ -1079,7 +1080,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(ScanStepArgs a)
   }
 #pragma unroll
   for (int o = 1; o < P; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-  kind = step_served(a.slots, b, place, kind);
+  kind = step_served(twice, kind);
   if (!valid) return;
   if (kind == kStepServed) {
     store_states(state, N, p, h);

@@ -108,20 +108,24 @@ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 // is touched, so that the mistake is seen and the result does not depend on
 // which of two blocks came first.
 //
-// step_place gives a place that may be read (0 for rows that have none, where
-// the array has any); step_served, which the whole block calls after its reads
-// are on their way, says whether it may be written.
+// step_place gives a place that may be read (0 for rows that have none);
+// step_twice, whether this thread's share of the earlier rows has it too; and
+// step_served, which the whole block calls after its reads are on their way,
+// whether it may be written.
 enum StepKind { kStepServed, kStepPadding, kStepBad };
 __device__ __forceinline__ int step_place(const int *slots, int b, int places, StepKind *kind) {
   const int place = slots ? slots[b] : b;
   *kind = place == -1 ? kStepPadding : place < 0 || place >= places ? kStepBad : kStepServed;
   return *kind == kStepServed ? place : 0;
 }
-__device__ __forceinline__ StepKind step_served(const int *slots, int b, int place, StepKind kind) {
-  if (!slots || kind != kStepServed) return kind;  // (the same in the whole block)
+__device__ __forceinline__ int step_twice(const int *slots, int b, int place, StepKind kind) {
   int twice = 0;
-  for (int i = threadIdx.x; i < b; i += blockDim.x) twice |= slots[i] == place;
-  return __syncthreads_or(twice) ? kStepBad : kStepServed;
+  if (slots && kind == kStepServed)
+    for (int i = threadIdx.x; i < b; i += blockDim.x) twice |= slots[i] == place;
+  return twice;
+}
+__device__ __forceinline__ StepKind step_served(int twice, StepKind kind) {
+  return __syncthreads_or(twice) ? kStepBad : kind;
 }
 __device__ __forceinline__ float step_nothing(StepKind kind) {
   return kind == kStepBad ? __int_as_float(0x7fffffff) : 0.f;
