@@ -157,6 +157,14 @@ __device__ __forceinline__ float exp2_tile(float x) {
   q = fmaf(q, x, 0.6931471f);
   return fabsf(x) < 0.125f ? fmaf(q, x, 1.f) : exp2_f(x);
 }
+// The same for two values.
+__device__ __forceinline__ F2 exp2_tile2(F2 x) {
+  F2 q = fma2(F2(0.009620536f, 0.009620536f), x, F2(0.055524945f, 0.055524945f));
+  q = fma2(q, x, F2(0.2402265f, 0.2402265f));
+  q = fma2(q, x, F2(0.6931471f, 0.6931471f));
+  q = fma2(q, x, F2(1.f, 1.f));
+  return F2(fabsf(x.x()) < 0.125f ? q.x() : exp2_f(x.x()), fabsf(x.y()) < 0.125f ? q.y() : exp2_f(x.y()));
+}
 // exp2(x) - prod; 0 for a growing state, whose product may have overflowed.
 __device__ __forceinline__ float tile_gap(float x, float prod) {
   return x <= 0.f ? exp2_tile(x) - prod : 0.f;
@@ -447,8 +455,7 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_forward_kernel(S
       const float sum = a.seg_sum[at];
 #pragma unroll
       for (int s = 0; s < kH; ++s) {
-        const F2 x = mul2(F2(sum, sum), A2[s]);
-        h[s] = fma2(F2(exp2_tile(x.x()), exp2_tile(x.y())), h[s], e[s]);
+        h[s] = fma2(exp2_tile2(mul2(F2(sum, sum), A2[s])), h[s], e[s]);
       }
     }
   }
@@ -730,8 +737,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
     const float sum = a.seg_sum[at];
 #pragma unroll
     for (int s = 0; s < kH; ++s) {
-      const F2 x = mul2(F2(sum, sum), A2[s]);
-      r[s] = fma2(F2(exp2_tile(x.x()), exp2_tile(x.y())), r[s], e[s]);
+      r[s] = fma2(exp2_tile2(mul2(F2(sum, sum), A2[s])), r[s], e[s]);
     }
   }
   const int t_begin = q.seg * a.seg_len, t_stop = min(L, t_begin + a.seg_len), t_end = min(t_stop, q.len);
@@ -1021,12 +1027,19 @@ struct ScanStepArgs {
 };
 
 // One token: reads and writes each state once (8 bytes a state: what bounds
-// it).  All reads are on their way before the block learns whether it may write.
-constexpr int kStepThreads = 256;
+// it).  A lane has eight states, so that what a channel needs once (softplus,
+// the gate) is not computed by more lanes than need be.  All reads are on their
+// way before the block learns whether it may write.
+constexpr int kStepThreads = 64, kStepQuads = 2;
+inline int step_lanes_of(int states) {
+  int p = 1;
+  while (p * kStepQuads * kS < states) p *= 2;
+  return p;
+}
 
 template <typename T, int P>
 __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(ScanStepArgs a) {
-  constexpr int CB = kStepThreads / P;
+  constexpr int CB = kStepThreads / P, Q = kStepQuads;
   const int b = blockIdx.x / a.nblk, blk = blockIdx.x - b * a.nblk;
   const int p = threadIdx.x % P, d = blk * CB + threadIdx.x / P, N = a.states;
   const bool valid = d < a.channels;
@@ -1034,34 +1047,31 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(ScanStepArgs a)
   const int place = step_place(a.slots, b, a.places, &kind);
   const int twice = step_twice(a.slots, b, place, kind);
   const int64_t i = (int64_t)b * a.channels + (valid ? d : 0);
-  const int dd = valid ? d : 0, g = dd / a.per_group;
+  const int dd = valid ? d : 0, g = a.groups == 1 ? 0 : dd / a.per_group;
   float *state = a.state + ((int64_t)place * a.channels + dd) * N;
-  F2 A2[kH], h[kH];
+  F2 h[Q][kH];
   float y = 0.f, u = 0.f, z = 0.f;
   if (kind == kStepServed) {
-    const bool four = N % kS == 0;
-    float bb[kS], cc[kS];
-    const T *B = static_cast<const T *>(a.B) + ((int64_t)b * a.groups + g) * N + p * kS;
-    const T *C = static_cast<const T *>(a.C) + ((int64_t)b * a.groups + g) * N + p * kS;
-    if (four && p * kS < N) {
-      load_pairs(state + p * kS, h);
-      load_pairs(a.A + (int64_t)dd * N + p * kS, A2);
-      Pack<T, kS> vb, vc;
-      vb.load(B);
-      vc.load(C);
+    F2 A2[Q][kH];
+    Pack<T, kS> vb[Q], vc[Q];
+    const T *B = static_cast<const T *>(a.B) + ((int64_t)b * a.groups + g) * N;
+    const T *C = static_cast<const T *>(a.C) + ((int64_t)b * a.groups + g) * N;
 #pragma unroll
-      for (int s = 0; s < kS; ++s) {
-        bb[s] = vb.f(s);
-        cc[s] = vc.f(s);
-      }
-    } else {
-      load_states(state, N, p, h);
-      load_states(a.A + (int64_t)dd * N, N, p, A2);
+    for (int k = 0; k < Q; ++k) {
+      const int n = (p * Q + k) * kS;
+      if (N % kS == 0 && n < N) {
+        load_pairs(state + n, h[k]);
+        load_pairs(a.A + (int64_t)dd * N + n, A2[k]);
+        vb[k].load(B + n);
+        vc[k].load(C + n);
+      } else {
+        load_states(state, N, p * Q + k, h[k]);
+        load_states(a.A + (int64_t)dd * N, N, p * Q + k, A2[k]);
 #pragma unroll
-      for (int s = 0; s < kS; ++s) {
-        const bool in = p * kS + s < N;
-        bb[s] = in ? to_f(B[s]) : 0.f;
-        cc[s] = in ? to_f(C[s]) : 0.f;
+        for (int s = 0; s < kS; ++s) {
+          vb[k].v[s] = n + s < N ? B[n + s] : from_f<T>(0.f);
+          vc[k].v[s] = n + s < N ? C[n + s] : from_f<T>(0.f);
+        }
       }
     }
     u = to_f(static_cast<const T *>(a.u)[i]);
@@ -1069,21 +1079,25 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(ScanStepArgs a)
     if (a.z) z = to_f(static_cast<const T *>(a.z)[i]);
     if (a.softplus) delta = softplus_f(delta);
     const F2 d2(delta * kLog2e, delta * kLog2e), x2(delta * u, delta * u);
-    F2 c2[kH];
 #pragma unroll
-    for (int s = 0; s < kH; ++s) {
-      const F2 x = mul2(d2, A2[s]);
-      h[s] = fma2(F2(exp2_tile(x.x()), exp2_tile(x.y())), h[s], mul2(x2, F2(bb[2 * s], bb[2 * s + 1])));
-      c2[s] = F2(cc[2 * s], cc[2 * s + 1]);
+    for (int k = 0; k < Q; ++k) {
+      F2 c2[kH];
+#pragma unroll
+      for (int s = 0; s < kH; ++s) {
+        h[k][s] = fma2(exp2_tile2(mul2(d2, A2[k][s])), h[k][s],
+                       mul2(x2, F2(vb[k].f(2 * s), vb[k].f(2 * s + 1))));
+        c2[s] = F2(vc[k].f(2 * s), vc[k].f(2 * s + 1));
+      }
+      y += dot(h[k], c2);
     }
-    y = dot(h, c2);
   }
 #pragma unroll
   for (int o = 1; o < P; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
   kind = step_served(twice, kind);
   if (!valid) return;
   if (kind == kStepServed) {
-    store_states(state, N, p, h);
+#pragma unroll
+    for (int k = 0; k < Q; ++k) store_states(state, N, p * Q + k, h[k]);
     if (a.skip) y = fmaf(a.skip[dd], u, y);
     if (a.z) y *= z * sigmoid_f(z);
   } else {
@@ -1385,9 +1399,10 @@ extern "C" int pc2d_ssm_scan_step(int dtype, const void *u, const void *delta, f
   a.batch = batch; a.places = places; a.channels = channels; a.states = states; a.groups = groups;
   a.per_group = channels / groups;
   a.softplus = delta_softplus != 0;
-  const int cb = kStepThreads / lanes_of(states);
+  const int cb = kStepThreads / step_lanes_of(states);
   a.nblk = (channels + cb - 1) / cb;
-  return by_type_and_layout(dtype, states, [&](auto t, auto layout) -> int {
+  // (as many lanes as a layout for that many states' quads has)
+  return by_type_and_layout(dtype, step_lanes_of(states) * kS, [&](auto t, auto layout) -> int {
     scan_step_kernel<decltype(t), decltype(layout)::P>
         <<<(unsigned)((int64_t)a.nblk * batch), kStepThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
     PC2D_LAUNCH_CHECK("scan_step_kernel");
