@@ -207,20 +207,22 @@ __device__ __forceinline__ float exp_neg_abs(float v) {
   const float e = exp2_f(hi);
   return hi < -126.f ? 0.f : fmaf(e, lo * 0.6931471806f, e);
 }
-__device__ __forceinline__ float softplus_f(float v) {
+// softplus and its slope, the logistic function, from one exponential
+__device__ __forceinline__ float softplus_f(float v, float *slope) {
   const float e = exp_neg_abs(v);
   const float s = __fdividef(e, 2.f + e), w = s * s;
   float q = fmaf(0.2815778f, w, 0.27965158f);
   q = fmaf(q, w, 0.40024596f);
   q = fmaf(q, w, 0.6666632f);
   q = fmaf(q, w, 2.f);
+  *slope = __fdividef(v < 0.f ? e : 1.f, 1.f + e);
   return fmaf(q, s, fmaxf(v, 0.f));
 }
-// softplus'(v), the logistic function
-__device__ __forceinline__ float softplus_slope(float v) {
-  const float e = exp_neg_abs(v);
-  return __fdividef(v < 0.f ? e : 1.f, 1.f + e);
+__device__ __forceinline__ float softplus_f(float v) {
+  float unused;
+  return softplus_f(v, &unused);
 }
+
 // Sums of v0..v3 over the P lanes of a channel.  P >= 4: lane p ends with
 // that of v[p % 4]; P = 2: with those of v[p] and v[p + 2]; P = 1: all four.
 template <int P>
@@ -399,6 +401,13 @@ struct ScanPlace {
 
 // A lane's states of a channel's row of them (0 for those beyond the last).
 __device__ __forceinline__ void load_states(const float *src, int states, int p, F2 (&h)[kH]) {
+  if (states % kS == 0 && p * kS < states) {
+    // (rows of a multiple of four states in a 16-byte aligned array)
+    const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(src + p * kS);
+    h[0].v = q.x;
+    h[1].v = q.y;
+    return;
+  }
 #pragma unroll
   for (int s = 0; s < kH; ++s) {
     const int n = p * kS + 2 * s;
@@ -407,7 +416,6 @@ __device__ __forceinline__ void load_states(const float *src, int states, int p,
 }
 __device__ __forceinline__ void store_states(float *dst, int states, int p, const F2 (&h)[kH]) {
   if (states % kS == 0) {
-    // (rows of a multiple of four states in a 16-byte aligned array)
     if (p * kS < states) put_pairs(dst + p * kS, h);
   } else {
 #pragma unroll
@@ -658,11 +666,12 @@ constexpr int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
 
 template <typename T, class G>
 struct BwdSmem {
-  static constexpr int TT = G::TB, DP = TT + 4, kPart = 2 * G::NP + 1;
-  static constexpr int kRows = G::CB * DP;                     // D, D u, dy, and three sums over states
+  static constexpr int TT = G::TB, DP = TT + 4, kPart = 2 * G::NP + 4;
+  // D, D u, dy, the slopes of softplus and of the gate, and three sums over states
+  static constexpr int kRows = G::CB * DP;
   static constexpr int kStart = TT / kRun * kThreads * kS;     // states at the start of each run
   static constexpr int kBC = (TileBC<T, G, TT>::kFloats + 3) / 4 * 4;
-  static constexpr int kFloats = 6 * kRows + kStart + kBC + (kThreads / 32) * TT * kPart;
+  static constexpr int kFloats = 8 * kRows + kStart + kBC + (kThreads / 32) * TT * kPart;
 };
 
 // Sums of v[0..7] over the lanes of a warp that hold the same states of
@@ -708,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
   using BC = TileBC<T, G, TT>;
   extern __shared__ __align__(16) float smem[];
   float *s_d = smem, *s_x = s_d + M::kRows, *s_y = s_x + M::kRows;
-  float *s_o = s_y + M::kRows, *s_start = s_o + 3 * M::kRows;
+  float *s_o = s_y + M::kRows, *s_start = s_o + 5 * M::kRows;
   T *s_bc = reinterpret_cast<T *>(s_start + M::kStart);
   float *s_part = s_start + M::kStart + M::kBC;
   const ScanPlace<G> q(a);
@@ -743,10 +752,13 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
   const int t_begin = q.seg * a.seg_len, t_stop = min(L, t_begin + a.seg_len), t_end = min(t_stop, q.len);
   float *row_d = s_d + q.c * DP, *row_x = s_x + q.c * DP, *row_y = s_y + q.c * DP;
   float *row_sy = s_o + q.c * DP, *row_sb = row_sy + M::kRows, *row_sm = row_sb + M::kRows;
+  float *row_ds = row_sm + M::kRows, *row_gs = row_ds + M::kRows;
   float *my_part = s_part + (threadIdx.x / 32) * TT * M::kPart;
   Pack<T, E> nu, nd, ng, nz;
+  F2 nh[kH];
   BC nbc;
   auto fetch = [&](int t0) {
+    load_states(a.ckpt + (((int64_t)q.b * ((L + TT - 1) / TT) + t0 / TT) * a.channels + q.d) * N, N, p, nh);
     if (loads) {
       load_row(nu, u, t0 + p * E, t_end, vec);
       load_row(nd, dl, t0 + p * E, t_end, vec);
@@ -773,23 +785,27 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
       }
       continue;
     }
-    const Pack<T, E> cu = nu, cd = nd, cg = ng, cz = nz;
+    const Pack<T, E> cu = nu;
+    F2 h0[kH] = {nh[0], nh[1]};
     if (loads) {
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        float v = cd.f(i) + bias;
-        if (a.softplus) v = softplus_f(v);
-        if (t0 + p * E + i >= t_end) v = 0.f;
+        const bool live = t0 + p * E + i < t_end;
+        float v = nd.f(i) + bias, slope = 1.f, dy = ng.f(i);
+        if (a.softplus) v = softplus_f(v, &slope);
+        if (z) {
+          const float zz = nz.f(i), e = sigmoid_f(zz);
+          row_gs[p * E + i] = dy * (e * fmaf(zz, 1.f - e, 1.f));
+          dy *= zz * e;
+        }
+        if (!live) v = slope = 0.f;
         row_d[p * E + i] = v;
-        float dy = cg.f(i);
-        if (z) dy *= cz.f(i) * sigmoid_f(cz.f(i));
+        row_ds[p * E + i] = slope;
         // a thread without a channel adds nothing to the sums over channels
         row_x[p * E + i] = q.valid ? v * cu.f(i) : 0.f;
         row_y[p * E + i] = q.valid ? dy : 0.f;
       }
     }
-    F2 h0[kH];
-    load_states(a.ckpt + (((int64_t)q.b * ((L + TT - 1) / TT) + t0 / TT) * a.channels + q.d) * N, N, p, h0);
     nbc.put(s_bc, true);
     __syncthreads();
     if (t0 > t_begin) fetch(t0 - TT);
@@ -894,22 +910,12 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
       Pack<T, E> ou, od, oz;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const bool live = t0 + p * E + i < t_end;
-        const float raw = cd.f(i) + bias, uu = cu.f(i), g = cg.f(i);
-        const float d = row_d[p * E + i];
-        float gate = 1.f, slope = 0.f;
-        if (z) {
-          const float zz = cz.f(i), e = sigmoid_f(zz);
-          gate = zz * e;
-          slope = e * fmaf(zz, 1.f - e, 1.f);
-        }
-        const float dy = g * gate, through = row_sb[p * E + i];
-        float dd = fmaf(uu, through, row_sm[p * E + i] * (1.f / kLog2e));
-        if (a.softplus) dd *= softplus_slope(raw);
-        if (!live) dd = 0.f;
-        ou.v[i] = from_f<T>(live ? fmaf(d, through, skip * dy) : 0.f);
+        // (behind the last token D, the slopes and dy are 0)
+        const float uu = cu.f(i), dy = row_y[p * E + i], through = row_sb[p * E + i];
+        const float dd = fmaf(uu, through, row_sm[p * E + i] * (1.f / kLog2e)) * row_ds[p * E + i];
+        ou.v[i] = from_f<T>(fmaf(row_d[p * E + i], through, skip * dy));
         od.v[i] = from_f<T>(dd);
-        if (z) oz.v[i] = from_f<T>(live ? g * slope * fmaf(skip, uu, row_sy[p * E + i]) : 0.f);
+        if (z) oz.v[i] = from_f<T>(row_gs[p * E + i] * fmaf(skip, uu, row_sy[p * E + i]));
         dskip = fmaf(dy, uu, dskip);
         dbias += dd;
       }
@@ -918,16 +924,25 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
       if (z) store_row(oz, dz, t0 + p * E, t_stop, vec);
     }
     __syncthreads();
-    // the warps' sums over their channels, added in order
-    for (int e = threadIdx.x; e < 2 * N * TT; e += kThreads) {
-      const int n = e / TT, t = e % TT;
-      if (t0 + t < t_stop) {
-        const float *src = s_part + t * M::kPart + (n < N ? n : NP + n - N);
-        float v = src[0];
+    // the warps' sums over their channels, added in order, four states at a time
+    for (int e = threadIdx.x; e < 2 * P * TT; e += kThreads) {
+      const int n = e / TT * kS, t = e % TT;  // n: 0 .. 2 NP, dB's states and dC's
+      const float *src = s_part + t * M::kPart + n;
+      F2 v[kH];
+      load_pairs(src, v);
 #pragma unroll
-        for (int w = 1; w < kThreads / 32; ++w) v += src[w * TT * M::kPart];
-        part[(int64_t)n * L + t0 + t] = v;
+      for (int w = 1; w < kThreads / 32; ++w) {
+        F2 o[kH];
+        load_pairs(src + w * TT * M::kPart, o);
+        v[0] = add2(v[0], o[0]);
+        v[1] = add2(v[1], o[1]);
       }
+      const float f[kS] = {v[0].x(), v[0].y(), v[1].x(), v[1].y()};
+      const int first = n < NP ? n : n - NP;  // state
+      float *dst = part + ((int64_t)(n < NP ? 0 : N) + first) * L + t0 + t;
+#pragma unroll
+      for (int s = 0; s < kS; ++s)
+        if (first + s < N && t0 + t < t_stop) dst[(int64_t)s * L] = f[s];
     }
     // (the next tile's first barrier comes before anything overwrites s_part)
   }
