@@ -6,10 +6,16 @@
 // starts off a 16-byte boundary is copied), work runs on torch's current
 // stream of the tensors' device, scratch comes from torch's caching allocator.
 // A state that a step moves on in place is never copied: it has to be
-// contiguous.  The autograd functions are in layers.py.
+// contiguous.
+//
+// The gradients are registered here as well (Autograd key): a training step of
+// a small layer is bound by the host, and going through Python functions took
+// it about twice as long.  The backward passes are differentiable once.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <climits>
@@ -319,6 +325,197 @@ Tensor ssm_scan_step_cuda(const Tensor &u_, const Tensor &delta_, Tensor state, 
   return out;
 }
 
+// ------------------------------------------------------------------ autograd
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool needs_grad(std::initializer_list<const Tensor *> tensors, std::initializer_list<const OptTensor *> optional) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor *t : tensors)
+    if (t->requires_grad()) return true;
+  for (const OptTensor *t : optional)
+    if (t->has_value() && (*t)->defined() && (*t)->requires_grad()) return true;
+  return false;
+}
+
+void check_cuda(const Tensor &t, const char *what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(t.is_cuda(), "paraconv2d_b200.", what, ": CUDA tensors only, got one on ", t.device());
+}
+
+OptTensor optional_of(const Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+// Runs a backward pass without recording it; where the caller asked for a graph
+// of it (create_graph), the gradients raise when they are differentiated.
+template <typename F>
+variable_list once(const char *what, F &&run) {
+  variable_list grads;
+  {
+    at::AutoGradMode off(false);
+    grads = run();
+  }
+  if (at::GradMode::is_enabled()) {
+    variable_list defined;
+    for (const Tensor &t : grads)
+      if (t.defined()) defined.push_back(t);
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        std::string("paraconv2d_b200.") + what + " is differentiable once only", (int)defined.size());
+    // (a gradient that needs none would not lead to the error)
+    for (Tensor &t : defined) t = t.detach().requires_grad_(true);
+    defined = (*error)(std::move(defined));
+    size_t k = 0;
+    for (Tensor &t : grads)
+      if (t.defined()) t = defined[k++];
+  }
+  return grads;
+}
+
+struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &input, const Tensor &key, double p,
+                        const OptTensor &residual) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({key});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["input"] = input.requires_grad();
+    ctx->saved_data["residual"] = residual.has_value() && residual->defined() && residual->requires_grad();
+    return dropout_cuda(input, key, p, residual);
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+    const Tensor key = ctx->get_saved_variables()[0];
+    // (linear: its gradient is the same operation, which may be differentiated again)
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow("paraconv2d_b200::dropout", "")
+                               .typed<Tensor(const Tensor &, const Tensor &, double, const OptTensor &)>();
+    Tensor dx;
+    if (ctx->saved_data["input"].toBool()) dx = op.call(grads[0], key, ctx->saved_data["p"].toDouble(), OptTensor());
+    return {dx, Tensor(), Tensor(), ctx->saved_data["residual"].toBool() ? grads[0] : Tensor()};
+  }
+};
+
+Tensor dropout_autograd(const Tensor &input, const Tensor &key, double p, const OptTensor &residual) {
+  check_cuda(input, "dropout");
+  if (needs_grad({&input}, {&residual})) return DropoutFunction::apply(input, key, p, residual);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return dropout_cuda(input, key, p, residual);
+}
+
+struct ConvFunction : torch::autograd::Function<ConvFunction> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &input, const Tensor &weight, const OptTensor &bias,
+                               const OptTensor &initial, const OptTensor &lengths, bool silu, bool final_state) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor x = dense(input);
+    auto outs = causal_conv_forward_cuda(x, weight, bias, initial, lengths, silu, final_state);
+    ctx->save_for_backward({x, weight, bias.value_or(Tensor()), initial.value_or(Tensor()), lengths.value_or(Tensor())});
+    ctx->saved_data["silu"] = silu;
+    ctx->set_materialize_grads(false);
+    return outs;
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+    return once("causal_conv", [&]() -> variable_list {
+      const auto saved = ctx->get_saved_variables();
+      const c10::cuda::CUDAGuard guard(saved[0].device());
+      const Tensor grad = grads[0].defined() ? grads[0] : at::zeros_like(saved[0]);
+      const auto g = causal_conv_backward_cuda(grad, grads.size() > 1 ? optional_of(grads[1]) : OptTensor(), saved[0],
+                                               saved[1], optional_of(saved[2]), optional_of(saved[3]),
+                                               optional_of(saved[4]), ctx->saved_data["silu"].toBool());
+      return {g[0], g[1], saved[2].defined() ? g[2] : Tensor(), saved[3].defined() ? g[3] : Tensor(),
+              Tensor(), Tensor(), Tensor()};
+    });
+  }
+};
+
+std::vector<Tensor> causal_conv_forward_autograd(const Tensor &input, const Tensor &weight, const OptTensor &bias,
+                                                 const OptTensor &initial, const OptTensor &lengths, bool silu,
+                                                 bool final_state) {
+  check_cuda(input, "causal_conv");
+  if (needs_grad({&input, &weight}, {&bias, &initial}))
+    return ConvFunction::apply(input, weight, bias, initial, lengths, silu, final_state);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return causal_conv_forward_cuda(input, weight, bias, initial, lengths, silu, final_state);
+}
+
+struct ScanFunction : torch::autograd::Function<ScanFunction> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &u_, const Tensor &delta_, const Tensor &A_,
+                               const Tensor &B_, const Tensor &C_, const OptTensor &D, const OptTensor &z_,
+                               const OptTensor &delta_bias, const OptTensor &initial, const OptTensor &lengths,
+                               bool delta_softplus, bool final_state) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor u = dense(u_), delta = dense(delta_), A = dense(A_), B = dense(B_), C = dense(C_);
+    const Tensor z = z_.has_value() && z_->defined() ? dense(*z_) : Tensor();
+    auto outs = ssm_scan_forward_cuda(u, delta, A, B, C, D, optional_of(z), delta_bias, initial, lengths,
+                                      delta_softplus, final_state, true);
+    ctx->save_for_backward({u, delta, A, B, C, D.value_or(Tensor()), z, delta_bias.value_or(Tensor()),
+                            lengths.value_or(Tensor()), outs[2]});
+    ctx->saved_data["softplus"] = delta_softplus;
+    ctx->saved_data["initial"] = initial.has_value() && initial->defined() && initial->requires_grad();
+    ctx->set_materialize_grads(false);
+    outs.pop_back();
+    if (!final_state) outs.pop_back();
+    return outs;
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+    return once("ssm_scan", [&]() -> variable_list {
+      const auto s = ctx->get_saved_variables();
+      const c10::cuda::CUDAGuard guard(s[0].device());
+      const Tensor grad = grads[0].defined() ? grads[0] : at::zeros_like(s[0]);
+      const bool initial = ctx->saved_data["initial"].toBool();
+      const auto g = ssm_scan_backward_cuda(grad, grads.size() > 1 ? optional_of(grads[1]) : OptTensor(), s[0], s[1],
+                                            s[2], s[3], s[4], optional_of(s[5]), optional_of(s[6]), optional_of(s[7]),
+                                            optional_of(s[8]), s[9], ctx->saved_data["softplus"].toBool(), initial);
+      return {g[0], g[1], g[2], g[3], g[4], s[5].defined() ? g[5] : Tensor(), s[6].defined() ? g[6] : Tensor(),
+              s[7].defined() ? g[7] : Tensor(), initial ? g[8] : Tensor(), Tensor(), Tensor(), Tensor()};
+    });
+  }
+};
+
+// With gradients the checkpoints are the graph's own: the third result is empty.
+std::vector<Tensor> ssm_scan_forward_autograd(const Tensor &u, const Tensor &delta, const Tensor &A, const Tensor &B,
+                                              const Tensor &C, const OptTensor &D, const OptTensor &z,
+                                              const OptTensor &delta_bias, const OptTensor &initial,
+                                              const OptTensor &lengths, bool delta_softplus, bool final_state,
+                                              bool checkpoints) {
+  check_cuda(u, "ssm_scan");
+  if (needs_grad({&u, &delta, &A, &B, &C}, {&D, &z, &delta_bias, &initial})) {
+    auto outs = ScanFunction::apply(u, delta, A, B, C, D, z, delta_bias, initial, lengths, delta_softplus, final_state);
+    while (outs.size() < 3) outs.push_back(at::empty({0}, A.options()));
+    return outs;
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return ssm_scan_forward_cuda(u, delta, A, B, C, D, z, delta_bias, initial, lengths, delta_softplus, final_state,
+                               checkpoints);
+}
+
+// A step changes its state in place: there is no gradient, and what autograd
+// has saved of the state is no longer what it was.
+void no_step_grad(const char *what, bool needs) {
+  TORCH_CHECK(!needs, "paraconv2d_b200.", what, " moves its state on in place and has no backward pass: call it under "
+              "torch.no_grad(), or use the operator over whole sequences");
+}
+void changed(const Tensor &state) {
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+}
+
+Tensor causal_conv_step_autograd(const Tensor &input, Tensor state, const Tensor &weight, const OptTensor &bias,
+                                 const OptTensor &slots, bool silu) {
+  no_step_grad("causal_conv_step", needs_grad({&input, &state, &weight}, {&bias}));
+  check_cuda(input, "causal_conv_step");
+  at::AutoDispatchBelowADInplaceOrView below;
+  Tensor out = causal_conv_step_cuda(input, state, weight, bias, slots, silu);
+  changed(state);
+  return out;
+}
+
+Tensor ssm_scan_step_autograd(const Tensor &u, const Tensor &delta, Tensor state, const Tensor &A, const Tensor &B,
+                              const Tensor &C, const OptTensor &D, const OptTensor &z, const OptTensor &delta_bias,
+                              const OptTensor &slots, bool delta_softplus) {
+  no_step_grad("ssm_scan_step", needs_grad({&u, &delta, &state, &A, &B, &C}, {&D, &z, &delta_bias}));
+  check_cuda(u, "ssm_scan_step");
+  at::AutoDispatchBelowADInplaceOrView below;
+  Tensor out = ssm_scan_step_cuda(u, delta, state, A, B, C, D, z, delta_bias, slots, delta_softplus);
+  changed(state);
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(paraconv2d_b200, m) {
@@ -355,4 +552,12 @@ TORCH_LIBRARY_IMPL(paraconv2d_b200, CUDA, m) {
   m.impl("ssm_scan_forward", ssm_scan_forward_cuda);
   m.impl("ssm_scan_backward", ssm_scan_backward_cuda);
   m.impl("ssm_scan_step", ssm_scan_step_cuda);
+}
+
+TORCH_LIBRARY_IMPL(paraconv2d_b200, Autograd, m) {
+  m.impl("dropout", dropout_autograd);
+  m.impl("causal_conv_forward", causal_conv_forward_autograd);
+  m.impl("causal_conv_step", causal_conv_step_autograd);
+  m.impl("ssm_scan_forward", ssm_scan_forward_autograd);
+  m.impl("ssm_scan_step", ssm_scan_step_autograd);
 }

@@ -17,10 +17,11 @@ convolution layer is one with ``x.flatten(2)``, and goes back with
 
 CUDA tensors only (float32, float16 and bfloat16; dropout float64 too), on the
 current stream of the tensors' device; sums and states in 32 bits.  Results
-and gradients are deterministic.  The backward passes are not differentiable
-again.  They can be captured into CUDA graphs; as for every backward pass,
-leaves that still belong to an eager autograd graph made on another stream
-must be released (or their graph run on the capturing stream) before that.
+and gradients are deterministic.  Dropout is differentiable any number of
+times, the convolution and the scan once.  All of it, backward passes too, can
+be captured into CUDA graphs; as for every backward pass, leaves that still
+belong to an eager autograd graph made on another stream must be released (or
+their graph run on the capturing stream) before that.
 """
 from __future__ import annotations
 
@@ -30,8 +31,6 @@ from typing import Optional
 import torch
 import torch.nn as nn
 from torch import Tensor
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from ._lib import load_op_library
 
@@ -44,25 +43,9 @@ class _ops:
     dropout = torch.ops.paraconv2d_b200.dropout.default
     dropout_next_key = torch.ops.paraconv2d_b200.dropout_next_key.default
     causal_conv_forward = torch.ops.paraconv2d_b200.causal_conv_forward.default
-    causal_conv_backward = torch.ops.paraconv2d_b200.causal_conv_backward.default
     causal_conv_step = torch.ops.paraconv2d_b200.causal_conv_step.default
     ssm_scan_forward = torch.ops.paraconv2d_b200.ssm_scan_forward.default
-    ssm_scan_backward = torch.ops.paraconv2d_b200.ssm_scan_backward.default
     ssm_scan_step = torch.ops.paraconv2d_b200.ssm_scan_step.default
-
-
-def _needs_grad(*tensors) -> bool:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
-
-
-def _no_step_grad(what, *tensors):
-    if _needs_grad(*tensors):
-        raise RuntimeError(f"{what} moves its state on in place and has no backward pass: call it under "
-                           "torch.no_grad(), or use the function over whole sequences")
 
 
 def _silu(activation) -> bool:
@@ -72,21 +55,6 @@ def _silu(activation) -> bool:
 
 
 # -------------------------------------------------------------------- dropout
-
-class _Dropout(Function):
-    @staticmethod
-    def forward(ctx, x, key, p, residual):
-        ctx.save_for_backward(key)
-        ctx.p = p
-        return _ops.dropout(x, key, p, residual)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        key, = ctx.saved_tensors
-        dx = _ops.dropout(grad, key, ctx.p, None) if ctx.needs_input_grad[0] else None
-        return dx, None, None, grad if ctx.needs_input_grad[3] else None
-
 
 def dropout(x: Tensor, p: float, key: Tensor, residual: Optional[Tensor] = None) -> Tensor:
     """``x`` with each element dropped with probability ``p`` and the others
@@ -99,9 +67,6 @@ def dropout(x: Tensor, p: float, key: Tensor, residual: Optional[Tensor] = None)
     multiple of 2^-16, and the scale is the inverse of the rounded
     probability.  A dropped element is 0, whatever it held.
     """
-    p = float(p)
-    if _needs_grad(x, residual):
-        return _Dropout.apply(x, key, p, residual)
     return _ops.dropout(x, key, p, residual)
 
 
@@ -131,26 +96,6 @@ class Dropout(nn.Module):
 
 # --------------------------------------------------------- causal convolution
 
-class _CausalConv(Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, initial_state, lengths, silu, final_state):
-        x = x.contiguous()
-        ctx.save_for_backward(x, weight, bias, initial_state, lengths)
-        ctx.silu = silu
-        ctx.set_materialize_grads(False)
-        outs = _ops.causal_conv_forward(x, weight, bias, initial_state, lengths, silu, final_state)
-        return tuple(outs)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad, grad_final=None):
-        x, weight, bias, initial_state, lengths = ctx.saved_tensors
-        if grad is None:
-            grad = torch.zeros_like(x)
-        dx, dw, db, di = _ops.causal_conv_backward(grad, grad_final, x, weight, bias, initial_state, lengths, ctx.silu)
-        return (dx, dw, db if bias is not None else None, di if initial_state is not None else None, None, None, None)
-
-
 def causal_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None,
                 initial_state: Optional[Tensor] = None, lengths: Optional[Tensor] = None,
                 return_final_state: bool = False):
@@ -166,11 +111,8 @@ def causal_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activa
     (output, the last taps-1 inputs of each row).  1 to 8 taps; weight and bias
     of x's type or float32.
     """
-    silu = _silu(activation)
-    if _needs_grad(x, weight, bias, initial_state):
-        outs = _CausalConv.apply(x, weight, bias, initial_state, lengths, silu, bool(return_final_state))
-    else:
-        outs = _ops.causal_conv_forward(x, weight, bias, initial_state, lengths, silu, bool(return_final_state))
+    outs = _ops.causal_conv_forward(x, weight, bias, initial_state, lengths, _silu(activation),
+                                    bool(return_final_state))
     return (outs[0], outs[1]) if return_final_state else outs[0]
 
 
@@ -183,7 +125,6 @@ def causal_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Te
     without a request: its output is 0 and no state changes.  A slot outside
     the states, or one that an earlier row has too, makes the row NaN and
     changes no state."""
-    _no_step_grad("causal_conv_step", x, state, weight, bias)
     return _ops.causal_conv_step(x, state, weight, bias, slots, _silu(activation))
 
 
@@ -220,31 +161,6 @@ class CausalConv(nn.Module):
 
 # ----------------------------------------------------------- state space scan
 
-class _SSMScan(Function):
-    @staticmethod
-    def forward(ctx, u, delta, A, B, C, D, z, delta_bias, initial_state, lengths, delta_softplus, final_state):
-        u, delta, A, B, C = (t.contiguous() for t in (u, delta, A, B, C))
-        z = z.contiguous() if z is not None else None
-        out, last, kept = _ops.ssm_scan_forward(u, delta, A, B, C, D, z, delta_bias, initial_state, lengths,
-                                                delta_softplus, final_state, True)
-        ctx.save_for_backward(u, delta, A, B, C, D, z, delta_bias, lengths, kept)
-        ctx.delta_softplus = delta_softplus
-        ctx.set_materialize_grads(False)
-        return (out, last) if final_state else (out,)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad, grad_final=None):
-        u, delta, A, B, C, D, z, delta_bias, lengths, kept = ctx.saved_tensors
-        if grad is None:
-            grad = torch.zeros_like(u)
-        need = ctx.needs_input_grad[8]
-        du, dd, dA, dB, dC, dD, dz, dbias, dinit = _ops.ssm_scan_backward(
-            grad, grad_final, u, delta, A, B, C, D, z, delta_bias, lengths, kept, ctx.delta_softplus, need)
-        return (du, dd, dA, dB, dC, dD if D is not None else None, dz if z is not None else None,
-                dbias if delta_bias is not None else None, dinit if need else None, None, None, None)
-
-
 def ssm_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor] = None,
              z: Optional[Tensor] = None, delta_bias: Optional[Tensor] = None, delta_softplus: bool = False,
              initial_state: Optional[Tensor] = None, lengths: Optional[Tensor] = None,
@@ -266,11 +182,8 @@ def ssm_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optio
     the backward pass the forward one keeps the states of every 16th or 32nd
     token in float32.
     """
-    args = (u, delta, A, B, C, D, z, delta_bias, initial_state)
-    if _needs_grad(*args):
-        outs = _SSMScan.apply(*args, lengths, bool(delta_softplus), bool(return_final_state))
-    else:
-        outs = _ops.ssm_scan_forward(*args, lengths, bool(delta_softplus), bool(return_final_state), False)
+    outs = _ops.ssm_scan_forward(u, delta, A, B, C, D, z, delta_bias, initial_state, lengths, bool(delta_softplus),
+                                 bool(return_final_state), False)
     return (outs[0], outs[1]) if return_final_state else outs[0]
 
 
@@ -281,7 +194,6 @@ def ssm_scan_step(u: Tensor, delta: Tensor, state: Tensor, A: Tensor, B: Tensor,
     [batch, channels], ``B``, ``C`` [batch, groups, states]; ``state`` float32
     [places, channels, states] is moved on in place, with ``slots`` as for
     :func:`causal_conv_step`."""
-    _no_step_grad("ssm_scan_step", u, delta, state, A, B, C, D, z, delta_bias)
     return _ops.ssm_scan_step(u, delta, state, A, B, C, D, z, delta_bias, slots, bool(delta_softplus))
 
 
