@@ -525,7 +525,7 @@ int check_conv(const char *what, int dtype, int wdtype, int batch, int channels,
     return PC2D_ERR_UNSUPPORTED;
   }
   // the vectors of a row are counted in 32 bits, the warps of a launch too
-  if (length > 0x7ffffff0 - 16 || (int64_t)batch * channels > (int64_t)1 << 30 ||
+  if (length > 1 << 30 || (int64_t)batch * channels > (int64_t)1 << 30 ||
       (int64_t)batch * channels * (length / 256 + 2) > (int64_t)1 << 33) {
     set_last_error("%s: problem too large", what);
     return PC2D_ERR_UNSUPPORTED;

@@ -165,12 +165,14 @@ __device__ __forceinline__ F2 exp2_tile2(F2 x) {
   q = fma2(q, x, F2(1.f, 1.f));
   return F2(fabsf(x.x()) < 0.125f ? q.x() : exp2_f(x.x()), fabsf(x.y()) < 0.125f ? q.y() : exp2_f(x.y()));
 }
-// exp2(x) - prod; 0 for a growing state, whose product may have overflowed.
-__device__ __forceinline__ float tile_gap(float x, float prod) {
-  return x <= 0.f ? exp2_tile(x) - prod : 0.f;
+// h corrected for the tile: x = A2 sum d, prod = the decays' product.  Not for a
+// growing state, whose product may have overflowed, nor for an infinite one.
+__device__ __forceinline__ float correct_tile(float h, float entry, float x, float prod) {
+  const bool apply = x <= 0.f && fabsf(entry) < __int_as_float(0x7f800000);
+  return apply ? fmaf(entry, exp2_tile(x) - prod, h) : h;
 }
-__device__ __forceinline__ F2 tile_gap2(F2 x, F2 prod) {
-  return F2(tile_gap(x.x(), prod.x()), tile_gap(x.y(), prod.y()));
+__device__ __forceinline__ F2 correct_tile2(F2 h, F2 entry, F2 x, F2 prod) {
+  return F2(correct_tile(h.x(), entry.x(), x.x(), prod.x()), correct_tile(h.y(), entry.y(), x.y(), prod.y()));
 }
 
 // Two pairs from, and to, 16 aligned bytes.
@@ -544,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_forward_kernel(S
         }
       }
 #pragma unroll
-      for (int s = 0; s < kH; ++s) h[s] = fma2(entry[s], tile_gap2(mul2(F2(sum, sum), A2[s]), prod[s]), h[s]);
+      for (int s = 0; s < kH; ++s) h[s] = correct_tile2(h[s], entry[s], mul2(F2(sum, sum), A2[s]), prod[s]);
       total += sum;
     }
     if (!kStateOnly) {
@@ -651,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_carry_kernel(Sca
       }
     }
 #pragma unroll
-    for (int s = 0; s < kH; ++s) r[s] = fma2(entry[s], tile_gap2(mul2(F2(sum, sum), A2[s]), prod[s]), r[s]);
+    for (int s = 0; s < kH; ++s) r[s] = correct_tile2(r[s], entry[s], mul2(F2(sum, sum), A2[s]), prod[s]);
     total += sum;
     __syncthreads();
   }
@@ -903,7 +905,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
 #pragma unroll
     for (int s = 0; s < kH; ++s) {
       dA[s] = add2(dA[s], tile_dA[s]);
-      r[s] = fma2(entry[s], tile_gap2(mul2(F2(sum, sum), A2[s]), prod[s]), r[s]);
+      r[s] = correct_tile2(r[s], entry[s], mul2(F2(sum, sum), A2[s]), prod[s]);
     }
     __syncwarp();
     if (q.valid && loads) {
@@ -1159,7 +1161,7 @@ int check_scan(const char *what, int dtype, int batch, int channels, int length,
     set_last_error("%s: %d states per channel (at most %d)", what, states, kMaxStates);
     return PC2D_ERR_UNSUPPORTED;
   }
-  if (length > 0x7fffff00 || (int64_t)batch * channels > (int64_t)1 << 24) {
+  if (length > 1 << 30 || (int64_t)batch * channels > (int64_t)1 << 24) {
     set_last_error("%s: problem too large", what);
     return PC2D_ERR_UNSUPPORTED;
   }
@@ -1327,7 +1329,13 @@ extern "C" int pc2d_ssm_scan_backward(int dtype, const void *grad, const float *
   int st = check_scan("pc2d_ssm_scan_backward", dtype, batch, channels, length, states, groups);
   if (st != PC2D_OK) return st;
   if ((st = pending_device_error()) != PC2D_OK) return st;
-  if (channels == 0) return PC2D_OK;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (channels == 0) {  // B and C reach nothing
+    const size_t bytes = (size_t)batch * groups * states * length * seq_dtype_size(dtype);
+    if (bytes && Bgrad) PC2D_CUDA_CHECK(cudaMemsetAsync(Bgrad, 0, bytes, s));
+    if (bytes && Cgrad) PC2D_CUDA_CHECK(cudaMemsetAsync(Cgrad, 0, bytes, s));
+    return PC2D_OK;
+  }
   const bool any = batch > 0 && length > 0;
   if (!A || !Agrad || (any && (!grad || !u || !delta || !B || !C || !checkpoints || !ugrad || !deltagrad || !Bgrad ||
                                !Cgrad || (z && !zgrad)))) {
@@ -1351,7 +1359,6 @@ extern "C" int pc2d_ssm_scan_backward(int dtype, const void *grad, const float *
   a.part_bc = reinterpret_cast<float *>(ws);
   a.part_par = reinterpret_cast<float *>(ws + scan_part_bc_bytes(a));
   const unsigned grid = (unsigned)((int64_t)batch * groups * a.nblk * a.nseg);
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return by_type_and_layout(dtype, states, [&](auto t, auto layout) -> int {
     using T = decltype(t);
     using G = decltype(layout);

@@ -302,6 +302,32 @@ def test_conv_step_places():
     assert torch.equal(state[rest], before[rest])
 
 
+def test_conv_infinite_and_nan_tokens_stay_in_their_windows():
+    x = torch.zeros(2, 2, 40, device=DEV)
+    x[0, 0, 10], x[0, 1, 39], x[1, 0, 0] = math.inf, math.nan, math.nan
+    w = torch.ones(2, 4, device=DEV)
+    out = pc.causal_conv(x, w).cpu()
+    want = torch.zeros(2, 2, 40)
+    want[0, 0, 10:14], want[0, 1, 39], want[1, 0, :4] = math.inf, math.nan, math.nan
+    assert torch.equal(torch.nan_to_num(out, nan=7.0, posinf=8.0), torch.nan_to_num(want, nan=7.0, posinf=8.0))
+
+
+def test_conv_beyond_32_bit_offsets():
+    """Rows whose elements lie beyond 2^31 of the array, forwards and backwards."""
+    L = (1 << 30) - 3
+    x = torch.zeros(1, 3, L, dtype=torch.float16, device=DEV)
+    x[0, 2, -5:] = 1.0
+    x.requires_grad_()
+    w = torch.tensor([[1.0, 2.0]], device=DEV).expand(3, 2).contiguous().half().requires_grad_()
+    out = pc.causal_conv(x, w)
+    assert out[0, 2, -7:].tolist() == [0, 0, 2, 3, 3, 3, 3] and not out[0, :2].any()
+    grad = torch.zeros_like(x)
+    grad[0, 2, -1] = 1.0
+    dx, dw = torch.autograd.grad(out, [x, w], grad)
+    assert dx[0, 2, -3:].tolist() == [0, 1, 2] and not dx[0, :2].any()
+    assert dw.tolist() == [[0, 0], [0, 0], [1, 1]]
+
+
 def test_conv_refuses():
     x, w = torch.zeros(2, 3, 5, device=DEV), torch.zeros(3, 4, device=DEV)
     state = torch.zeros(2, 3, 3, device=DEV)
@@ -437,6 +463,32 @@ def test_scan_empty():
     out = pc.ssm_scan(u, u, A, z(0, 1, 4, 5, device=DEV), z(0, 1, 4, 5, device=DEV))
     dA, = torch.autograd.grad(out.sum(), A)
     assert out.shape == (0, 6, 5) and torch.equal(dA, torch.zeros_like(A))
+
+
+def test_scan_without_channels():
+    z = lambda *s: torch.zeros(*s, device=DEV, requires_grad=True)  # noqa: E731
+    B, C = z(2, 1, 4, 9), z(2, 1, 4, 9)
+    out, final = pc.ssm_scan(z(2, 0, 9), z(2, 0, 9), z(0, 4), B, C, return_final_state=True)
+    assert out.shape == (2, 0, 9) and final.shape == (2, 0, 4)
+    dB, dC = torch.autograd.grad(out.sum(), [B, C])
+    assert not dB.any() and not dC.any()
+
+
+@pytest.mark.parametrize("L", [5, 40, 700])
+def test_scan_infinite_states(L):
+    """A state that is infinite stays so, decaying, growing or kept; the other
+    states of its channel and the other channels are what they are without."""
+    c, _, _, _ = scan_case(L, 1, 40, L, 4, 1, torch.float32)
+    c["A"][1, 2], c["A"][2, 2] = 0.01, 0.0
+    t = {k: dev(a) for k, a in c.items()}
+    want_out, want = scan_call(t, True, None, return_final_state=True)
+    for ch in range(3):
+        t["init"][0, ch, 2] = -math.inf
+    out, final = scan_call(t, True, None, return_final_state=True)
+    far = torch.zeros(40, 4, dtype=torch.bool)
+    far[:3, 2] = True
+    assert (final[0].cpu()[far] == -math.inf).all() and torch.equal(final[0].cpu()[~far], want[0].cpu()[~far])
+    assert torch.equal(out[0, 3:], want_out[0, 3:]) and not torch.isfinite(out[0, :3]).any()
 
 
 def test_scan_strided_inputs_and_partial_gradients():
@@ -620,7 +672,7 @@ def test_block_over_a_paraconv_map():
     want = s + torch.where(keep, y * ref.keep_scale(0.25), 0.0)
     (want * go.cpu().double()).sum().backward()
     # (each value passes at most 42 steps and two sums of 8 in fp32: 1e-4 of the largest)
-    assert float((out.detach().cpu().double() - want).abs().max()) <= 1e-4 * float(want.abs().max())
+    assert float((out.detach().cpu().double() - want.detach()).abs().max()) <= 1e-4 * float(want.detach().abs().max())
     for got, ref_ in [(seq.grad, s.grad)] + [(q.grad, p[n].grad) for n, q in block.named_parameters()]:
         assert float((got.cpu().double() - ref_).abs().max()) <= 2e-4 * float(ref_.abs().max())
 
