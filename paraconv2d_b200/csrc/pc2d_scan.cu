@@ -56,9 +56,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 // two, which the compiler spends on overlapping more of a run (16384 tokens of
 // 2048 channels in 9 segments: 293 against 351 us; 4 x 2048 tokens of 2048
 // channels, 1.7 blocks per SM: 225 against 198 us).
-template <int P_, bool kMany_ = false>
+// kWhole: every row of the arrays starts on a 16-byte boundary.
+template <int P_, bool kWhole_, bool kMany_ = false>
 struct Layout {
-  static constexpr bool kMany = kMany_;
+  static constexpr bool kWhole = kWhole_, kMany = kMany_;
   static constexpr int P = P_, NP = kS * P, CB = kThreads / P;
   static constexpr int TF = P == 1 ? 16 : P == 2 || P >= 16 || kMany ? 32 : 64;
   static constexpr int TB = P == 1 || P >= 16 ? 16 : 32;
@@ -259,24 +260,94 @@ struct Sum4 {
   }
 };
 
-// E elements of a row from t on, 0 at and behind `end` (nothing is read there).
-template <typename T, int E>
-__device__ __forceinline__ void load_row(Pack<T, E> &v, const T *row, int t, int end, bool vec) {
-  if (vec && t + E <= end) {
-    v.load(row + t);
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; ++i) v.v[i] = t + i < end ? row[t + i] : from_f<T>(0.f);
+// An array of `total` elements whose rows are read along their length.
+template <typename T>
+struct Rows {
+  const T *array;
+  int64_t total;
+};
+
+// E elements of a row, on their way: load() only issues the reads, get() gives
+// the elements (0 at and behind `end`, where nothing is read).  Where rows may
+// start anywhere, the aligned vectors that hold the elements are read and
+// shifted by the elements before them when they are wanted; reads of single
+// elements, which are packed as they arrive, would wait for each other and for
+// memory (4 x 2048 x 2047 bf16 forwards: 317 us, as against 181 for 2048).
+template <typename T, int E, bool kWhole>
+struct RowLoad {
+  static constexpr int V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
+  static constexpr bool kShift = !kWhole && V > 1;
+  static constexpr int NV = E / V + (kShift ? 1 : 0), kPer = kShift ? V * (int)sizeof(T) / 4 : 1;
+  Pack<T, V> q[NV];
+
+  // whether the vectors can be read whole (kShift: one more than the elements fill)
+  __device__ static __forceinline__ bool vectors(const Rows<T> &r, int64_t row, int t, int end) {
+    return kWhole ? t + E <= end : kShift && t < end && row + t + E + V <= r.total;
   }
-}
-template <typename T, int E>
-__device__ __forceinline__ void store_row(const Pack<T, E> &v, T *row, int t, int end, bool vec) {
-  if (vec && t + E <= end) {
-    v.store(row + t);
+  __device__ __forceinline__ void load(const Rows<T> &r, int64_t row, int t, int end) {
+    const int64_t at = row + t;
+    if (vectors(r, row, t, end)) {
+      const T *p = r.array + (kShift ? at & ~(int64_t)(V - 1) : at);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) q[i].load(p + i * V);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) q[i / V].v[i % V] = t + i < end ? r.array[at + i] : from_f<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void get(const Rows<T> &r, int64_t row, int t, int end, Pack<T, E> &v) const {
+    if constexpr (!kShift) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) v.v[i] = q[i / V].v[i % V];
+    } else {
+      // (without vectors the elements lie unshifted)
+      const int m = vectors(r, row, t, end) ? (int)((row + t) & (V - 1)) : 0;
+      unsigned w[NV * kPer];
+#pragma unroll
+      for (int i = 0; i < NV * kPer; ++i) w[i] = reinterpret_cast<const unsigned *>(q[i / kPer].v)[i % kPer];
+#pragma unroll
+      for (int e = V / 2; e * (int)sizeof(T) >= 4; e /= 2) {
+        const int step = e * (int)sizeof(T) / 4;
+#pragma unroll
+        for (int i = 0; i + step < NV * kPer; ++i) w[i] = m & e ? w[i + step] : w[i];
+      }
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i + 1 < NV * kPer; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (m & 1) * 16);
+      }
+#pragma unroll
+      for (int i = 0; i < E * (int)sizeof(T) / 4; ++i) reinterpret_cast<unsigned *>(v.v)[i] = w[i];
+      if (t + E > end) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if (t + i >= end) v.v[i] = from_f<T>(0.f);
+      }
+    }
+  }
+};
+
+template <bool kWhole, typename T, int E>
+__device__ __forceinline__ void store_row(const Pack<T, E> &v, T *array, int64_t row, int t, int end) {
+  T *dst = array + row + t;
+  if (kWhole && t + E <= end) {
+    v.store(dst);
+  } else if (!kWhole && sizeof(T) == 2 && E >= 2 && t + E <= end) {
+    // two elements a store, from an even one on
+    const int odd = (int)((row + t) & 1);
+    const unsigned *w = reinterpret_cast<const unsigned *>(v.v);
+    if (odd) {
+      dst[0] = v.v[0];
+#pragma unroll
+      for (int i = 0; i + 1 < E / 2; ++i) reinterpret_cast<unsigned *>(dst + 1)[i] = __funnelshift_r(w[i], w[i + 1], 16);
+      dst[E - 1] = v.v[E - 1];
+    } else {
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) reinterpret_cast<unsigned *>(dst)[i] = w[i];
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < E; ++i)
-      if (t + i < end) row[t + i] = v.v[i];
+      if (t + i < end) dst[i] = v.v[i];
   }
 }
 
@@ -330,26 +401,35 @@ struct TileBC {
   __device__ static __forceinline__ int row_in(int t, int j) {
     return kVec < n ? row(t) + j * 2 * NP + j / kVec * kPad : row(t) + j * 2 * NP;
   }
-  Pack<T, kVec> b[kNum], c[kNum];
-  __device__ __forceinline__ void load(const T *B, const T *C, int states, int length, int t0, int end, bool vec) {
+  using Load = RowLoad<T, kVec, G::kWhole>;
+  Load b[kNum], c[kNum];
+  // at: where the group's first state's row begins
+  __device__ __forceinline__ void load(const Rows<T> &B, const Rows<T> *C, int64_t at, int states, int length, int t0,
+                                       int end) {
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
       const int e = (i * kThreads + threadIdx.x) * kVec, n = e / TT, t = t0 + e % TT;
       const int stop = n < states && e < kCount ? end : t;  // nothing to read for missing states
-      load_row(b[i], B + (int64_t)n * length, t, stop, vec);
-      if (C) load_row(c[i], C + (int64_t)n * length, t, stop, vec);
+      b[i].load(B, at + (int64_t)n * length, t, stop);
+      if (C) c[i].load(*C, at + (int64_t)n * length, t, stop);
     }
   }
-  __device__ __forceinline__ void put(T *tile, bool with_c) const {
+  // (with the arguments of the load)
+  __device__ __forceinline__ void put(T *tile, const Rows<T> &B, const Rows<T> *C, int64_t at, int states, int length,
+                                      int t0, int end) const {
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
       const int e = (i * kThreads + threadIdx.x) * kVec, n = e / TT, t = e % TT;
       if (e < kCount) {
+        const int stop = n < states ? end : t0 + t;
         T *dst = tile + row(t) + n / kS * (2 * kS) + n % kS;
+        Pack<T, kVec> vb, vc;
+        b[i].get(B, at + (int64_t)n * length, t0 + t, stop, vb);
+        if (C) c[i].get(*C, at + (int64_t)n * length, t0 + t, stop, vc);
 #pragma unroll
         for (int k = 0; k < kVec; ++k) {
-          dst[k * 2 * NP] = b[i].v[k];
-          if (with_c) dst[k * 2 * NP + kS] = c[i].v[k];
+          dst[k * 2 * NP] = vb.v[k];
+          if (C) dst[k * 2 * NP + kS] = vc.v[k];
         }
       }
     }
@@ -444,12 +524,13 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_forward_kernel(S
   __shared__ __align__(16) T s_bc[BC::kElems];
   const ScanPlace<G> q(a);
   const int p = q.p, N = a.states, L = a.length;
-  const T *u = static_cast<const T *>(a.u) + q.row * L, *dl = static_cast<const T *>(a.delta) + q.row * L;
-  const T *z = a.z ? static_cast<const T *>(a.z) + q.row * L : nullptr;
+  const int64_t row = q.row * L, all = (int64_t)a.batch * a.channels * L, all_bc = (int64_t)a.batch * a.groups * N * L;
+  const Rows<T> u{static_cast<const T *>(a.u), all}, dl{static_cast<const T *>(a.delta), all};
+  const Rows<T> zr{static_cast<const T *>(a.z), all};
   const int64_t bg = ((int64_t)q.b * a.groups + q.g) * N * L;
-  const T *B = static_cast<const T *>(a.B) + bg, *C = kStateOnly ? nullptr : static_cast<const T *>(a.C) + bg;
-  T *out = static_cast<T *>(a.out) + q.row * L;
-  const bool vec = (L * (int64_t)sizeof(T)) % 16 == 0;
+  const Rows<T> B{static_cast<const T *>(a.B), all_bc}, C{static_cast<const T *>(a.C), all_bc};
+  const bool z = a.z != nullptr;
+  T *out = static_cast<T *>(a.out);
   const float bias = a.bias ? a.bias[q.d] : 0.f, skip = a.skip ? a.skip[q.d] : 0.f;
   const int t_begin = q.seg * a.seg_len, t_stop = min(L, t_begin + a.seg_len), t_end = min(t_stop, q.len);
   F2 A2[kH], h[kH];
@@ -471,13 +552,13 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_forward_kernel(S
   }
   float total = 0.f;
   float *row_d = s_d + q.c * DP, *row_x = s_x + q.c * DP, *row_o = s_o + (kStateOnly ? 0 : q.c * DP);
-  Pack<T, E> nu, nd, nz;   // the next tile's inputs, on their way
+  RowLoad<T, E, G::kWhole> nu, nd, nz;   // the next tile's inputs, on their way
   BC nbc;
   auto fetch = [&](int t0) {
-    load_row(nu, u, t0 + p * E, t_end, vec);
-    load_row(nd, dl, t0 + p * E, t_end, vec);
-    if (!kStateOnly && z) load_row(nz, z, t0 + p * E, t_end, vec);
-    nbc.load(B, C, N, L, t0, t_end, vec);
+    nu.load(u, row, t0 + p * E, t_end);
+    nd.load(dl, row, t0 + p * E, t_end);
+    if (!kStateOnly && z) nz.load(zr, row, t0 + p * E, t_end);
+    nbc.load(B, kStateOnly ? nullptr : &C, bg, N, L, t0, t_end);
   };
   if (t_begin < t_end) fetch(t_begin);
   for (int t0 = t_begin; t0 < t_stop; t0 += TT) {
@@ -486,20 +567,23 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_forward_kernel(S
         Pack<T, E> o;
 #pragma unroll
         for (int i = 0; i < E; ++i) o.v[i] = from_f<T>(0.f);
-        store_row(o, out, t0 + p * E, t_stop, vec);
+        store_row<G::kWhole>(o, out, row, t0 + p * E, t_stop);
       }
       continue;
     }
-    const Pack<T, E> cu = nu, cz = nz;
+    Pack<T, E> cu, cd, cz;
+    nu.get(u, row, t0 + p * E, t_end, cu);
+    nd.get(dl, row, t0 + p * E, t_end, cd);
+    if (!kStateOnly && z) nz.get(zr, row, t0 + p * E, t_end, cz);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      float v = nd.f(i) + bias;
+      float v = cd.f(i) + bias;
       if (a.softplus) v = softplus_f(v);
       if (t0 + p * E + i >= t_end) v = 0.f;
       row_d[p * E + i] = v;
       row_x[p * E + i] = v * cu.f(i);
     }
-    nbc.put(s_bc, !kStateOnly);
+    nbc.put(s_bc, B, kStateOnly ? nullptr : &C, bg, N, L, t0, t_end);
     __syncthreads();
     if (t0 + TT < t_end) fetch(t0 + TT);
 #pragma unroll 1
@@ -560,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_forward_kernel(S
           if (t0 + p * E + i >= t_end) v = 0.f;
           o.v[i] = from_f<T>(v);
         }
-        store_row(o, out, t0 + p * E, t_stop, vec);
+        store_row<G::kWhole>(o, out, row, t0 + p * E, t_stop);
       }
     }
     __syncthreads();
@@ -586,10 +670,11 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_carry_kernel(Sca
   __shared__ __align__(16) T s_c[BC::kElems];
   const ScanPlace<G> q(a);
   const int p = q.p, N = a.states, L = a.length;
-  const T *dl = static_cast<const T *>(a.delta) + q.row * L, *grad = static_cast<const T *>(a.grad) + q.row * L;
-  const T *z = a.z ? static_cast<const T *>(a.z) + q.row * L : nullptr;
-  const T *C = static_cast<const T *>(a.C) + ((int64_t)q.b * a.groups + q.g) * N * L;
-  const bool vec = (L * (int64_t)sizeof(T)) % 16 == 0;
+  const int64_t row = q.row * L, all = (int64_t)a.batch * a.channels * L, all_bc = (int64_t)a.batch * a.groups * N * L;
+  const Rows<T> dl{static_cast<const T *>(a.delta), all}, grad{static_cast<const T *>(a.grad), all};
+  const Rows<T> zr{static_cast<const T *>(a.z), all}, C{static_cast<const T *>(a.C), all_bc};
+  const int64_t bg = ((int64_t)q.b * a.groups + q.g) * N * L;
+  const bool z = a.z != nullptr;
   const float bias = a.bias ? a.bias[q.d] : 0.f;
   F2 A2[kH], r[kH];
   load_decay_rates(a, q.d, p, A2);
@@ -598,32 +683,36 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_carry_kernel(Sca
   const int t_begin = q.seg * a.seg_len, t_end = min(min(L, t_begin + a.seg_len), q.len);
   float total = 0.f;
   float *row_d = s_d + q.c * DP, *row_y = s_y + q.c * DP;
-  Pack<T, E> nd, ng, nz;
+  RowLoad<T, E, G::kWhole> nd, ng, nz;
   BC nc;
   auto fetch = [&](int t0) {
     if (p * E < TT) {
-      load_row(nd, dl, t0 + p * E, t_end, vec);
-      load_row(ng, grad, t0 + p * E, t_end, vec);
-      if (z) load_row(nz, z, t0 + p * E, t_end, vec);
+      nd.load(dl, row, t0 + p * E, t_end);
+      ng.load(grad, row, t0 + p * E, t_end);
+      if (z) nz.load(zr, row, t0 + p * E, t_end);
     }
-    nc.load(C, nullptr, N, L, t0, t_end, vec);
+    nc.load(C, nullptr, bg, N, L, t0, t_end);
   };
   const int last = t_begin + (t_end - t_begin - 1) / TT * TT;
   if (t_begin < t_end) fetch(last);
   for (int t0 = last; t0 >= t_begin && t_begin < t_end; t0 -= TT) {
     if (p * E < TT) {
+      Pack<T, E> cd, cg, cz;
+      nd.get(dl, row, t0 + p * E, t_end, cd);
+      ng.get(grad, row, t0 + p * E, t_end, cg);
+      if (z) nz.get(zr, row, t0 + p * E, t_end, cz);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        float v = nd.f(i) + bias;
+        float v = cd.f(i) + bias;
         if (a.softplus) v = softplus_f(v);
         if (t0 + p * E + i >= t_end) v = 0.f;
         row_d[p * E + i] = v;
-        float dy = ng.f(i);
-        if (z) dy *= nz.f(i) * sigmoid_f(nz.f(i));
+        float dy = cg.f(i);
+        if (z) dy *= cz.f(i) * sigmoid_f(cz.f(i));
         row_y[p * E + i] = dy;
       }
     }
-    nc.put(s_c, false);
+    nc.put(s_c, C, nullptr, bg, N, L, t0, t_end);
     __syncthreads();
     if (t0 > t_begin) fetch(t0 - TT);
     F2 entry[kH], prod[kH];
@@ -724,15 +813,14 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
   float *s_part = s_start + M::kStart + M::kBC;
   const ScanPlace<G> q(a);
   const int p = q.p, N = a.states, L = a.length, lane = threadIdx.x & 31;
-  const T *u = static_cast<const T *>(a.u) + q.row * L, *dl = static_cast<const T *>(a.delta) + q.row * L;
-  const T *grad = static_cast<const T *>(a.grad) + q.row * L;
-  const T *z = a.z ? static_cast<const T *>(a.z) + q.row * L : nullptr;
+  const int64_t row = q.row * L, all = (int64_t)a.batch * a.channels * L, all_bc = (int64_t)a.batch * a.groups * N * L;
+  const Rows<T> u{static_cast<const T *>(a.u), all}, dl{static_cast<const T *>(a.delta), all};
+  const Rows<T> grad{static_cast<const T *>(a.grad), all}, zr{static_cast<const T *>(a.z), all};
   const int64_t bg = ((int64_t)q.b * a.groups + q.g) * N * L;
-  const T *B = static_cast<const T *>(a.B) + bg, *C = static_cast<const T *>(a.C) + bg;
-  T *du = static_cast<T *>(a.du) + q.row * L, *ddl = static_cast<T *>(a.ddelta) + q.row * L;
-  T *dz = a.z ? static_cast<T *>(a.dz) + q.row * L : nullptr;
+  const Rows<T> B{static_cast<const T *>(a.B), all_bc}, C{static_cast<const T *>(a.C), all_bc};
+  const bool z = a.z != nullptr;
+  T *du = static_cast<T *>(a.du), *ddl = static_cast<T *>(a.ddelta), *dz = static_cast<T *>(a.dz);
   float *part = a.part_bc + (((int64_t)q.b * a.groups + q.g) * a.nblk + q.blk) * 2 * N * L;
-  const bool vec = (L * (int64_t)sizeof(T)) % 16 == 0;
   const bool loads = p * E < TT;  // (more lanes than tokens of a tile)
   const float bias = a.bias ? a.bias[q.d] : 0.f, skip = a.skip ? a.skip[q.d] : 0.f;
   float dskip = 0.f, dbias = 0.f;
@@ -756,18 +844,18 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
   float *row_sy = s_o + q.c * DP, *row_sb = row_sy + M::kRows, *row_sm = row_sb + M::kRows;
   float *row_ds = row_sm + M::kRows, *row_gs = row_ds + M::kRows;
   float *my_part = s_part + (threadIdx.x / 32) * TT * M::kPart;
-  Pack<T, E> nu, nd, ng, nz;
+  RowLoad<T, E, G::kWhole> nu, nd, ng, nz;
   F2 nh[kH];
   BC nbc;
   auto fetch = [&](int t0) {
     load_states(a.ckpt + (((int64_t)q.b * ((L + TT - 1) / TT) + t0 / TT) * a.channels + q.d) * N, N, p, nh);
     if (loads) {
-      load_row(nu, u, t0 + p * E, t_end, vec);
-      load_row(nd, dl, t0 + p * E, t_end, vec);
-      load_row(ng, grad, t0 + p * E, t_end, vec);
-      if (z) load_row(nz, z, t0 + p * E, t_end, vec);
+      nu.load(u, row, t0 + p * E, t_end);
+      nd.load(dl, row, t0 + p * E, t_end);
+      ng.load(grad, row, t0 + p * E, t_end);
+      if (z) nz.load(zr, row, t0 + p * E, t_end);
     }
-    nbc.load(B, C, N, L, t0, t_end, vec);
+    nbc.load(B, &C, bg, N, L, t0, t_end);
   };
   const int last_live = t_begin + (t_end - t_begin - 1) / TT * TT;
   if (t_begin < t_end) fetch(last_live);
@@ -777,9 +865,9 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
         Pack<T, E> o;
 #pragma unroll
         for (int i = 0; i < E; ++i) o.v[i] = from_f<T>(0.f);
-        store_row(o, du, t0 + p * E, t_stop, vec);
-        store_row(o, ddl, t0 + p * E, t_stop, vec);
-        if (z) store_row(o, dz, t0 + p * E, t_stop, vec);
+        store_row<G::kWhole>(o, du, row, t0 + p * E, t_stop);
+        store_row<G::kWhole>(o, ddl, row, t0 + p * E, t_stop);
+        if (z) store_row<G::kWhole>(o, dz, row, t0 + p * E, t_stop);
       }
       for (int e = threadIdx.x; e < 2 * N * TT; e += kThreads) {
         const int n = e / TT, t = t0 + e % TT;
@@ -787,16 +875,21 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
       }
       continue;
     }
-    const Pack<T, E> cu = nu;
+    Pack<T, E> cu;
     F2 h0[kH] = {nh[0], nh[1]};
     if (loads) {
+      Pack<T, E> cd, cg, cz;
+      nu.get(u, row, t0 + p * E, t_end, cu);
+      nd.get(dl, row, t0 + p * E, t_end, cd);
+      ng.get(grad, row, t0 + p * E, t_end, cg);
+      if (z) nz.get(zr, row, t0 + p * E, t_end, cz);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const bool live = t0 + p * E + i < t_end;
-        float v = nd.f(i) + bias, slope = 1.f, dy = ng.f(i);
+        float v = cd.f(i) + bias, slope = 1.f, dy = cg.f(i);
         if (a.softplus) v = softplus_f(v, &slope);
         if (z) {
-          const float zz = nz.f(i), e = sigmoid_f(zz);
+          const float zz = cz.f(i), e = sigmoid_f(zz);
           row_gs[p * E + i] = dy * (e * fmaf(zz, 1.f - e, 1.f));
           dy *= zz * e;
         }
@@ -808,7 +901,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
         row_y[p * E + i] = q.valid ? dy : 0.f;
       }
     }
-    nbc.put(s_bc, true);
+    nbc.put(s_bc, B, &C, bg, N, L, t0, t_end);
     __syncthreads();
     if (t0 > t_begin) fetch(t0 - TT);
     // the states at the start of each run of kRun tokens
@@ -921,9 +1014,9 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
         dskip = fmaf(dy, uu, dskip);
         dbias += dd;
       }
-      store_row(ou, du, t0 + p * E, t_stop, vec);
-      store_row(od, ddl, t0 + p * E, t_stop, vec);
-      if (z) store_row(oz, dz, t0 + p * E, t_stop, vec);
+      store_row<G::kWhole>(ou, du, row, t0 + p * E, t_stop);
+      store_row<G::kWhole>(od, ddl, row, t0 + p * E, t_stop);
+      if (z) store_row<G::kWhole>(oz, dz, row, t0 + p * E, t_stop);
     }
     __syncthreads();
     // the warps' sums over their channels, added in order, four states at a time
@@ -1127,22 +1220,27 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(ScanStepArgs a)
 
 PerContext<uint64_t> g_scan_attr;
 
-// f(T{}, Layout{}) for the call's type and states
-template <typename F>
-int by_type_and_layout(int dtype, int states, F &&f) {
-#define PC2D_LAYOUT(T)                          \
-  switch (lanes_of(states)) {                   \
-    case 1: return f(T{}, Layout<1>{});         \
-    case 2: return f(T{}, Layout<2>{});         \
-    case 4: return f(T{}, Layout<4>{});         \
-    case 8: return f(T{}, Layout<8>{});         \
-    case 16: return f(T{}, Layout<16>{});       \
-    default: return f(T{}, Layout<32>{});       \
+// f(T{}, Layout{}) for the call's type, states and length
+template <bool kWhole, typename F>
+int by_type_and_states(int dtype, int states, F &&f) {
+#define PC2D_LAYOUT(T)                             \
+  switch (lanes_of(states)) {                      \
+    case 1: return f(T{}, Layout<1, kWhole>{});    \
+    case 2: return f(T{}, Layout<2, kWhole>{});    \
+    case 4: return f(T{}, Layout<4, kWhole>{});    \
+    case 8: return f(T{}, Layout<8, kWhole>{});    \
+    case 16: return f(T{}, Layout<16, kWhole>{});  \
+    default: return f(T{}, Layout<32, kWhole>{});  \
   }
   if (dtype == PC2D_DTYPE_F32) { PC2D_LAYOUT(float) }
   if (dtype == PC2D_DTYPE_F16) { PC2D_LAYOUT(__half) }
   PC2D_LAYOUT(__nv_bfloat16)
 #undef PC2D_LAYOUT
+}
+template <typename F>
+int by_type_and_layout(int dtype, int states, int length, F &&f) {
+  if (length * (int64_t)seq_dtype_size(dtype) % 16 == 0) return by_type_and_states<true>(dtype, states, f);
+  return by_type_and_states<false>(dtype, states, f);
 }
 
 constexpr int kMaxStates = 128;
@@ -1288,7 +1386,7 @@ extern "C" int pc2d_ssm_scan_forward(int dtype, const void *u, const void *delta
   take_segments(&a, static_cast<char *>(workspace));
   const unsigned grid = (unsigned)((int64_t)batch * groups * a.nblk * a.nseg);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return by_type_and_layout(dtype, states, [&](auto t, auto layout) -> int {
+  return by_type_and_layout(dtype, states, length, [&](auto t, auto layout) -> int {
     using T = decltype(t);
     using G = decltype(layout);
     if (a.nseg > 1) {
@@ -1296,9 +1394,9 @@ extern "C" int pc2d_ssm_scan_forward(int dtype, const void *u, const void *delta
       PC2D_LAUNCH_CHECK("scan_forward_kernel (segments)");
     }
     // more blocks than two per SM: the layout for four
-    if (G::P == 4 || G::P == 8) {
+    if constexpr (G::kWhole && (G::P == 4 || G::P == 8)) {
       if (grid > 2u * device_sm_count()) {
-        scan_forward_kernel<T, Layout<G::P, true>, false><<<grid, kThreads, 0, s>>>(a);
+        scan_forward_kernel<T, Layout<G::P, G::kWhole, true>, false><<<grid, kThreads, 0, s>>>(a);
         PC2D_LAUNCH_CHECK("scan_forward_kernel (many blocks)");
         return PC2D_OK;
       }
@@ -1359,14 +1457,14 @@ extern "C" int pc2d_ssm_scan_backward(int dtype, const void *grad, const float *
   a.part_bc = reinterpret_cast<float *>(ws);
   a.part_par = reinterpret_cast<float *>(ws + scan_part_bc_bytes(a));
   const unsigned grid = (unsigned)((int64_t)batch * groups * a.nblk * a.nseg);
-  return by_type_and_layout(dtype, states, [&](auto t, auto layout) -> int {
+  return by_type_and_layout(dtype, states, length, [&](auto t, auto layout) -> int {
     using T = decltype(t);
     using G = decltype(layout);
     if (grid > 0) {
       constexpr int bytes = BwdSmem<T, G>::kFloats * 4;
-      // one bit per instance: 3 types x 6 layouts
+      // one bit per instance: 3 types x 6 lane counts x 2
       int bit = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 1 : 2;
-      bit += 3 * log2_of(G::P);
+      bit += 3 * log2_of(G::P) + (G::kWhole ? 0 : 18);
       const int attr = once_per_context(g_scan_attr, (uint64_t)1 << bit, []() -> int {
         PC2D_CUDA_CHECK(cudaFuncSetAttribute(scan_backward_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              bytes));
@@ -1424,7 +1522,7 @@ extern "C" int pc2d_ssm_scan_step(int dtype, const void *u, const void *delta, f
   const int cb = kStepThreads / step_lanes_of(states);
   a.nblk = (channels + cb - 1) / cb;
   // (as many lanes as a layout for that many states' quads has)
-  return by_type_and_layout(dtype, step_lanes_of(states) * kS, [&](auto t, auto layout) -> int {
+  return by_type_and_states<true>(dtype, step_lanes_of(states) * kS, [&](auto t, auto layout) -> int {
     scan_step_kernel<decltype(t), decltype(layout)::P>
         <<<(unsigned)((int64_t)a.nblk * batch), kStepThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
     PC2D_LAUNCH_CHECK("scan_step_kernel");
