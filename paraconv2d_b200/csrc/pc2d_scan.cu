@@ -1268,8 +1268,9 @@ int check_scan(const char *what, int dtype, int batch, int channels, int length,
 
 // Blocks and segments.  Segments cost the first pass over the inputs and its
 // exps again, so the length is cut only when the rows alone leave most of the
-// GPU idle, into as many as give four blocks per SM and at least two tiles of
-// the longer (forward) kind each.
+// GPU idle, into as many as give each SM the blocks that it holds at a time
+// (four forwards, two backwards) and at least two tiles of the longer (forward)
+// kind each.
 template <bool kBackward>
 void scan_split(ScanArgs *a) {
   const int CB = kThreads / lanes_of(a->states);
@@ -1281,7 +1282,7 @@ void scan_split(ScanArgs *a) {
   a->nseg = 1;
   a->seg_len = std::max(kStep, (a->length + kStep - 1) / kStep * kStep);
   if (blocks > 0 && blocks < sms + sms / 2) {
-    const int want = (int)std::min<int64_t>(64, (int64_t)sms * 4 / blocks);
+    const int want = (int)std::min<int64_t>(64, (int64_t)sms * (kBackward ? kBwdBlocks : 4) / blocks);
     const int len = std::max(2 * kStep, (int)((((int64_t)a->length + want - 1) / want + kStep - 1) / kStep * kStep));
     const int n = std::max(1, (int)(((int64_t)a->length + len - 1) / len));
     if (n > 2) {
@@ -1393,8 +1394,9 @@ extern "C" int pc2d_ssm_scan_forward(int dtype, const void *u, const void *delta
       scan_forward_kernel<T, G, true><<<grid, kThreads, 0, s>>>(a);
       PC2D_LAUNCH_CHECK("scan_forward_kernel (segments)");
     }
-    // more blocks than two per SM: the layout for four
-    if constexpr (G::kWhole && (G::P == 4 || G::P == 8)) {
+    // more blocks than two per SM: the layout for four (the rule goes by the grid; rows of a ragged batch that end
+    // early may leave less, and then it costs up to a tenth)
+    if constexpr (G::P == 4 || G::P == 8) {
       if (grid > 2u * device_sm_count()) {
         scan_forward_kernel<T, Layout<G::P, G::kWhole, true>, false><<<grid, kThreads, 0, s>>>(a);
         PC2D_LAUNCH_CHECK("scan_forward_kernel (many blocks)");
