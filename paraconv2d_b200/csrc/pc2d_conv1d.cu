@@ -153,11 +153,11 @@ __device__ __forceinline__ float filter(const float (&w)[K], float bias, const f
   return s;
 }
 
-template <typename T>
+template <bool kInside, typename T>
 __device__ __forceinline__ void store8(T *row, int t0, int length, const float (&y)[8]) {
   Pack<T, 8> o;
   o.set(y);
-  if (t0 >= 0 && t0 + 8 <= length) {
+  if (t0 >= 0 && (kInside || t0 + 8 <= length)) {
     o.store(row + t0);
   } else {
 #pragma unroll
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kConvThreads, kConvFwdBlocks<T, K>) conv_forwa
             if (t0 + i >= p.n) y[i] = 0.f;
         }
       }
-      store8(out, t0, a.length, y);
+      store8<kInside>(out, t0, a.length, y);
     }
   };
   for (int v0 = p.seg * a.seg; v0 < vb; v0 += 32 * U) {
@@ -246,25 +246,26 @@ struct BackWindow {
     Window<T, K>::template load8<kInside>(g, static_cast<const T *>(a.grad), at, total);
   }
   // the values that its windows cover, and dpre (zeros outside [0, n))
+  template <bool kInside>
   __device__ __forceinline__ void get(const ConvArgs &a, int t0, int n, const T *init, const float (&w)[K], float bias,
                                       float (&v)[K + 7], float *dp) const {
-    x.template get<false>(v, t0, n, init);
+    x.template get<kInside>(v, t0, n, init);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dp[i] = g.f(i);
     if (a.silu) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) dp[i] *= silu_slope(filter<K>(w, bias, v, i));
     }
-    if (t0 < 0 || t0 + 8 > n) {
+    if (t0 < 0 || (!kInside && t0 + 8 > n)) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (t0 + i < 0 || t0 + i >= n) dp[i] = 0.f;
+        if (t0 + i < 0 || (!kInside && t0 + i >= n)) dp[i] = 0.f;
     }
   }
 };
 
 // Blocks per SM, by the registers that they leave (4 x 4096 x 2048 bf16 with 4
-// taps: 67 us, 3.0 TB/s, with 7; 72 with 6, 73 with 8).
+// taps: 64 us, 3.1 TB/s, with 7; 69 with 6, 76 with 8).
 template <typename T, int K>
 constexpr int kConvBackBlocks = K <= 4 ? (sizeof(T) == 2 ? 7 : 6) : 4;
 
@@ -285,9 +286,11 @@ __global__ void __launch_bounds__(kConvThreads, kConvBackBlocks<T, K>) conv_back
   const int va = p.seg * a.seg, vb = min(p.nvec, va + a.seg);
   const int top = va + ((vb - va - 1) >> 5) * 32;
   BackWindow<T, K> next;
+  // 32 vectors from v0 on: all of them within the row's tokens
+  auto inside = [&](int v0) { return v0 + 32 <= vb && p.e0 + (v0 + 32) * 8 <= p.n; };
   auto fetch = [&](int v0) {
     const int t0 = p.e0 + (v0 + lane) * 8;
-    if (v0 + 32 <= vb && p.e0 + (v0 + 32) * 8 <= p.n) next.template load<true>(a, p.base + t0, total);
+    if (inside(v0)) next.template load<true>(a, p.base + t0, total);
     else if (v0 + lane < vb && t0 < p.n) next.template load<false>(a, p.base + t0, total);
   };
   if (va < vb) fetch(top);
@@ -306,15 +309,16 @@ __global__ void __launch_bounds__(kConvThreads, kConvBackBlocks<T, K>) conv_back
     BackWindow<T, K> behind;
     float x[K + 7], dp[8];
     behind.template load<false>(a, p.base + p.e0 + vb * 8, total);
-    behind.get(a, p.e0 + vb * 8, p.n, init, w, bias, x, dp);
+    behind.template get<false>(a, p.e0 + vb * 8, p.n, init, w, bias, x, dp);
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) carry[k] = dp[k];
   }
-  for (int v0 = top; v0 >= va && va < vb; v0 -= 32) {
+  auto vectors = [&](int v0, auto all) {
+    constexpr bool kInside = decltype(all)::value;
     const int v = v0 + lane, t0 = p.e0 + v * 8;
     float x[K + 7], dp[8 + B], g[8];
-    if (v < vb && t0 < p.n) {
-      next.get(a, t0, p.n, init, w, bias, x, dp);
+    if (kInside || (v < vb && t0 < p.n)) {
+      next.template get<kInside>(a, t0, p.n, init, w, bias, x, dp);
     } else {
 #pragma unroll
       for (int i = 0; i < K + 7; ++i) x[i] = 0.f;
@@ -328,7 +332,7 @@ __global__ void __launch_bounds__(kConvThreads, kConvBackBlocks<T, K>) conv_back
       // zeros, so it takes the carry itself
       const float behind = __shfl_down_sync(0xffffffffu, dp[k], 1);
       const float first = __shfl_sync(0xffffffffu, dp[k], 0);
-      dp[8 + k] = lane == 31 || v == vb - 1 ? carry[k] : behind;
+      dp[8 + k] = lane == 31 || (!kInside && v == vb - 1) ? carry[k] : behind;
       carry[k] = first;
     }
 #pragma unroll
@@ -351,7 +355,11 @@ __global__ void __launch_bounds__(kConvThreads, kConvBackBlocks<T, K>) conv_back
       }
     }
     // (behind the last token dpre is 0, and so is g)
-    if (v < vb) store8(dx, t0, a.length, g);
+    if (kInside || v < vb) store8<kInside>(dx, t0, a.length, g);
+  };
+  for (int v0 = top; v0 >= va && va < vb; v0 -= 32) {
+    if (inside(v0)) vectors(v0, std::true_type{});
+    else vectors(v0, std::false_type{});
   }
   // the warp's share of the parameter gradients, in a fixed order
   float mine = 0.f;

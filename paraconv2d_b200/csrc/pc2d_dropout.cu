@@ -23,7 +23,7 @@ namespace pc2d {
 namespace {
 
 // Two vectors in flight per thread and 16 blocks per SM: 66 us (6.1 TB/s) for
-// 2^26 bf16 elements with a residual and 53 us (5.1 TB/s) without; one vector
+// 2^26 bf16 elements with a residual and 52 us (5.2 TB/s) without; one vector
 // 71 and 57, four 74 and 55, 8 blocks per SM 70 and 54 us.  With 4 rounds of the
 // generator instead of 10 it would be 63 and 47: its 20 wide products and 20
 // exclusive-ors for eight elements, with five operations an element, come near
@@ -69,12 +69,15 @@ struct Acc<double> {
 };
 
 template <typename T, bool kResidual>
-__device__ __forceinline__ T drop_one(T x, T res, const Words &w, int i, unsigned thr, typename Acc<T>::type scale) {
+__device__ __forceinline__ typename Acc<T>::type drop_one(T x, T res, const Words &w, int i, unsigned thr,
+                                                          typename Acc<T>::type scale) {
   using A = typename Acc<T>::type;
-  const unsigned half = i & 1 ? w.w[i / 2] >> 16 : w.w[i / 2] & 0xFFFFu;
-  A v = half >= thr ? to_acc(x) * scale : A(0);
+  // the half in the upper bits against the limit in the upper bits: what lies
+  // below an upper half does not change the comparison
+  const unsigned half = i & 1 ? w.w[i / 2] : w.w[i / 2] << 16;
+  A v = half >= thr << 16 ? to_acc(x) * scale : A(0);
   if (kResidual) v += to_acc(res);
-  return from_acc<T>(v);
+  return v;
 }
 
 template <typename T, bool kResidual>
@@ -101,8 +104,15 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const T *__restri
       if (g < whole) {
         const Words w = philox((uint64_t)g, offset, seed);
         Pack<T, 8> o;
+        if constexpr (sizeof(T) == 2) {
+          float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o.v[i] = drop_one<T, kResidual>(a[k].v[i], r[k].v[i], w, i, thr, scale);
+          for (int i = 0; i < 8; ++i) v[i] = drop_one<T, kResidual>(a[k].v[i], r[k].v[i], w, i, thr, scale);
+          o.set(v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o.v[i] = drop_one<T, kResidual>(a[k].v[i], r[k].v[i], w, i, thr, scale);
+        }
         o.store(out + g * 8);
       }
     }
@@ -112,7 +122,7 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const T *__restri
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int64_t e = g * 8 + i;
-      if (e < n) out[e] = drop_one<T, kResidual>(x[e], kResidual ? res[e] : x[e], w, i, thr, scale);
+      if (e < n) out[e] = from_acc<T>(drop_one<T, kResidual>(x[e], kResidual ? res[e] : x[e], w, i, thr, scale));
     }
   }
 }
@@ -168,8 +178,14 @@ extern "C" int pc2d_dropout(int dtype, const void *input, const void *residual, 
   }
   // round to even at a half, as Python's round() does
   const unsigned thr = (unsigned)nearbyint(p * 65536.0);
-  const double scale = thr < 65536u ? 65536.0 / (65536.0 - thr) : 0.0;
+  const double scale = 65536.0 / (65536.0 - thr);  // (not used where every element is dropped)
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (thr == 65536u) {  // every element is dropped (the kernel's limits are below that)
+    const size_t bytes = (size_t)n * (dtype == PC2D_DTYPE_F64 ? 8 : seq_dtype_size(dtype));
+    if (residual) PC2D_CUDA_CHECK(cudaMemcpyAsync(output, residual, bytes, cudaMemcpyDeviceToDevice, s));
+    else PC2D_CUDA_CHECK(cudaMemsetAsync(output, 0, bytes, s));
+    return PC2D_OK;
+  }
   switch (dtype) {
     case PC2D_DTYPE_F32: return launch_dropout<float>(input, residual, key, thr, scale, n, output, s);
     case PC2D_DTYPE_F64: return launch_dropout<double>(input, residual, key, thr, scale, n, output, s);
