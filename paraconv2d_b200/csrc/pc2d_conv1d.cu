@@ -644,7 +644,7 @@ extern "C" int pc2d_causal_conv_step(int dtype, int wdtype, const void *input, v
   NvtxRange range("pc2d_causal_conv_step");
   int st = check_conv("pc2d_causal_conv_step", dtype, wdtype, batch, channels, 1, taps);
   if (st != PC2D_OK) return st;
-  if (places < 0 || (!slots && batch > places && taps > 1)) {
+  if (places < 0 || (!slots && batch > places)) {
     set_last_error("pc2d_causal_conv_step: %d rows of a batch without slots, but %d states", batch, places);
     return PC2D_ERR_INVALID_ARGUMENT;
   }

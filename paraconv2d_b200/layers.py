@@ -76,7 +76,10 @@ class Dropout(nn.Module):
     on the GPU in the buffer ``state`` and counted there: a call that a CUDA
     graph replays drops other elements each time, and a checkpoint goes on
     where it was saved.  Ranks of a data-parallel job need seeds of their own,
-    and so have layers whose masks should not be the same."""
+    and so have layers whose masks should not be the same; a wrapper that
+    broadcasts buffers would give all ranks the same seed.  Where activations
+    are computed again in the backward pass, a second call would drop other
+    elements: take a key before, and call :func:`dropout` with it."""
 
     def __init__(self, p: float = 0.5, seed: int = 0, device=None):
         super().__init__()

@@ -199,6 +199,8 @@ def test_step_refuses_more_rows_than_states():
     assert lib.pc2d_ssm_scan_step(0, one, one, one, one, one, one, None, None, None, None, 1, 3, 2, 4, 16, 1, one,
                                   None) == INVALID
     assert lib.pc2d_causal_conv_step(0, 0, one, one, one, None, None, 3, 2, 4, 4, 1, one, None) == INVALID
+    # (one tap keeps nothing, but a row still needs its place)
+    assert lib.pc2d_causal_conv_step(0, 0, one, None, one, None, None, 3, 2, 4, 1, 1, one, None) == INVALID
 
 
 def test_scan_backward_refuses_a_short_workspace():
