@@ -167,8 +167,8 @@ __device__ __forceinline__ void store8(T *row, int t0, int length, const float (
 }
 
 // Two vectors in flight per lane, and as many blocks per SM as hold them without
-// spilling (4 x 4096 x 2048 bf16 with 4 taps: 33 us, 4.1 TB/s, against 38 with
-// the compiler's choice of registers and 36 with four vectors).
+// spilling (4 x 4096 x 2048 bf16 with 4 taps: 32.8 us, 4.1 TB/s, against 33.2
+// with the compiler's choice of registers and 37.3 with four vectors).
 constexpr int kConvUnroll = 2;
 template <typename T, int K>
 constexpr int kConvFwdBlocks = sizeof(T) == 2 && K <= 5 ? 8 : 5;

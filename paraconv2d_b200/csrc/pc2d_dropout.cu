@@ -24,8 +24,8 @@ namespace {
 
 // Two vectors in flight per thread and 16 blocks per SM: 66 us (6.1 TB/s) for
 // 2^26 bf16 elements with a residual and 52 us (5.2 TB/s) without; one vector
-// 71 and 57, four 74 and 55, 8 blocks per SM 70 and 54 us.  With 4 rounds of the
-// generator instead of 10 it would be 63 and 47: its 20 wide products and 20
+// 65 and 55, four 77 and 54, 8 blocks per SM 69 and 53 us.  With 4 rounds of the
+// generator instead of 10 it would be 63 and 42: its 20 wide products and 20
 // exclusive-ors for eight elements, with five operations an element, come near
 // the time of the traffic.
 constexpr int kDropThreads = 256, kDropUnroll = 2, kDropBlocks = 16;
