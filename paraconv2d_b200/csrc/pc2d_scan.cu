@@ -1518,7 +1518,7 @@ extern "C" int pc2d_ssm_scan_step(int dtype, const void *u, const void *delta, f
     set_last_error("pc2d_ssm_scan_step: null pointer (u, delta, state, A, B, C or output)");
     return PC2D_ERR_INVALID_ARGUMENT;
   }
-  if ((st = check_aligned("pc2d_ssm_scan_step", {state, A})) != PC2D_OK) return st;
+  if ((st = check_aligned("pc2d_ssm_scan_step", {state, A, B, C})) != PC2D_OK) return st;
   ScanStepArgs a{};
   a.u = u; a.delta = delta; a.z = z; a.B = B; a.C = C; a.A = A; a.skip = skip; a.bias = delta_bias;
   a.slots = slots; a.state = state; a.out = output;
