@@ -217,8 +217,9 @@ int pc2d_param_step(int dtype, void *pars, const void *grad, void *momentum_buf,
  * Sequence operators, beside the convolution and over the maps it writes: an
  * [N][C][H][W] map is [batch][channels][length] with length = H*W.  They have
  * no counterpart in the reference.  All arrays are contiguous; activations,
- * states, checkpoints and their gradients are 16-byte aligned; no output may
- * overlap an input.  float32, float16 and bfloat16 (dropout float64 too); sums
+ * states, checkpoints and their gradients are 16-byte aligned, all others
+ * aligned to their elements (what is off the boundary that a call needs is
+ * refused); no output may overlap an input.  float32, float16 and bfloat16 (dropout float64 too); sums
  * and states are held in 32 bits and rounded once to the outputs' type.  The
  * results do not depend on the order in which blocks run.  With `lengths`
  * (int32 on the device, one per batch row, taken as 0 .. length), the

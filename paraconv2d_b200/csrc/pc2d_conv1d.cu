@@ -570,7 +570,11 @@ extern "C" int pc2d_causal_conv_forward(int dtype, int wdtype, const void *input
     set_last_error("pc2d_causal_conv_forward: null pointer (input, weight or output)");
     return PC2D_ERR_INVALID_ARGUMENT;
   }
-  if ((st = check_aligned("pc2d_causal_conv_forward", {input, output})) != PC2D_OK) return st;
+  if ((st = check_aligned("pc2d_causal_conv_forward", {input, output})) != PC2D_OK ||
+      (st = check_elements("pc2d_causal_conv_forward", seq_dtype_size(dtype), {initial_state, final_state})) != PC2D_OK ||
+      (st = check_elements("pc2d_causal_conv_forward", seq_dtype_size(wdtype), {weight, bias})) != PC2D_OK ||
+      (st = check_elements("pc2d_causal_conv_forward", 4, {lengths})) != PC2D_OK)
+    return st;
   a.x = input; a.weight = weight; a.bias = bias; a.init = taps > 1 ? initial_state : nullptr;
   a.lengths = lengths; a.wdtype = wdtype;
   a.batch = batch; a.channels = channels; a.length = length; a.silu = silu != 0;
@@ -610,7 +614,13 @@ extern "C" int pc2d_causal_conv_backward(int dtype, int wdtype, const void *grad
     set_last_error("pc2d_causal_conv_backward: null pointer (grad, input, weight or inputgrad)");
     return PC2D_ERR_INVALID_ARGUMENT;
   }
-  if ((st = check_aligned("pc2d_causal_conv_backward", {grad, input, inputgrad})) != PC2D_OK) return st;
+  if ((st = check_aligned("pc2d_causal_conv_backward", {grad, input, inputgrad})) != PC2D_OK ||
+      (st = check_elements("pc2d_causal_conv_backward", seq_dtype_size(dtype),
+                           {grad_final, initial_state, initialgrad})) != PC2D_OK ||
+      (st = check_elements("pc2d_causal_conv_backward", seq_dtype_size(wdtype),
+                           {weight, bias, weightgrad, biasgrad})) != PC2D_OK ||
+      (st = check_elements("pc2d_causal_conv_backward", 4, {lengths})) != PC2D_OK)
+    return st;
   const size_t need = pc2d_causal_conv_backward_workspace_size(batch, channels, length, taps);
   if (workspace_bytes < need || (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255)))) {
     set_last_error("pc2d_causal_conv_backward: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", need,
@@ -654,6 +664,10 @@ extern "C" int pc2d_causal_conv_step(int dtype, int wdtype, const void *input, v
     set_last_error("pc2d_causal_conv_step: null pointer (input, state, weight or output)");
     return PC2D_ERR_INVALID_ARGUMENT;
   }
+  if ((st = check_elements("pc2d_causal_conv_step", seq_dtype_size(dtype), {input, state, output})) != PC2D_OK ||
+      (st = check_elements("pc2d_causal_conv_step", seq_dtype_size(wdtype), {weight, bias})) != PC2D_OK ||
+      (st = check_elements("pc2d_causal_conv_step", 4, {slots})) != PC2D_OK)
+    return st;
   ConvStepArgs a{};
   a.x = input; a.weight = weight; a.bias = bias; a.slots = slots; a.state = state; a.out = output;
   a.wdtype = wdtype; a.batch = batch; a.places = places; a.channels = channels; a.silu = silu != 0;

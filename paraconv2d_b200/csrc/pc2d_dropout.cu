@@ -169,19 +169,23 @@ extern "C" int pc2d_dropout(int dtype, const void *input, const void *residual, 
     set_last_error("pc2d_dropout: invalid element count %lld", (long long)n);
     return PC2D_ERR_INVALID_ARGUMENT;
   }
-  const int st = pending_device_error();
+  int st = pending_device_error();
   if (st != PC2D_OK) return st;
   if (n == 0) return PC2D_OK;
   if (!input || !key || !output) {
     set_last_error("pc2d_dropout: null pointer (input, key or output)");
     return PC2D_ERR_INVALID_ARGUMENT;
   }
+  const size_t size = dtype == PC2D_DTYPE_F64 ? 8 : seq_dtype_size(dtype);
+  if ((st = check_elements("pc2d_dropout", size, {input, residual, output})) != PC2D_OK ||
+      (st = check_elements("pc2d_dropout", 8, {key})) != PC2D_OK)
+    return st;
   // round to even at a half, as Python's round() does
   const unsigned thr = (unsigned)nearbyint(p * 65536.0);
   const double scale = 65536.0 / (65536.0 - thr);  // (not used where every element is dropped)
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (thr == 65536u) {  // every element is dropped (the kernel's limits are below that)
-    const size_t bytes = (size_t)n * (dtype == PC2D_DTYPE_F64 ? 8 : seq_dtype_size(dtype));
+    const size_t bytes = (size_t)n * size;
     if (residual) PC2D_CUDA_CHECK(cudaMemcpyAsync(output, residual, bytes, cudaMemcpyDeviceToDevice, s));
     else PC2D_CUDA_CHECK(cudaMemsetAsync(output, 0, bytes, s));
     return PC2D_OK;
@@ -200,8 +204,8 @@ extern "C" int pc2d_dropout_next_key(int64_t *state, int64_t *key, void *stream)
     set_last_error("pc2d_dropout_next_key: null pointer");
     return PC2D_ERR_INVALID_ARGUMENT;
   }
-  const int st = pending_device_error();
-  if (st != PC2D_OK) return st;
+  int st = check_elements("pc2d_dropout_next_key", 8, {state, key});
+  if (st != PC2D_OK || (st = pending_device_error()) != PC2D_OK) return st;
   dropout_next_key_kernel<<<1, 1, 0, reinterpret_cast<cudaStream_t>(stream)>>>(state, key);
   PC2D_LAUNCH_CHECK("dropout_next_key_kernel");
   return PC2D_OK;

@@ -1378,7 +1378,8 @@ extern "C" int pc2d_ssm_scan_forward(int dtype, const void *u, const void *delta
     return PC2D_ERR_INVALID_ARGUMENT;
   }
   if ((st = check_aligned("pc2d_ssm_scan_forward",
-                          {u, delta, z, B, C, output, initial_state, final_state, checkpoints, A})) != PC2D_OK)
+                          {u, delta, z, B, C, output, initial_state, final_state, checkpoints, A})) != PC2D_OK ||
+      (st = check_elements("pc2d_ssm_scan_forward", 4, {skip, delta_bias, lengths})) != PC2D_OK)
     return st;
   ScanArgs a = scan_problem(batch, channels, length, states, groups);
   scan_split<false>(&a);
@@ -1447,7 +1448,9 @@ extern "C" int pc2d_ssm_scan_backward(int dtype, const void *grad, const float *
     return PC2D_ERR_INVALID_ARGUMENT;
   }
   if ((st = check_aligned("pc2d_ssm_scan_backward", {grad, u, delta, z, B, C, ugrad, deltagrad, Bgrad, Cgrad, zgrad, checkpoints,
-                                                     grad_final, initialgrad, A})) != PC2D_OK)
+                                                     grad_final, initialgrad, A})) != PC2D_OK ||
+      (st = check_elements("pc2d_ssm_scan_backward", 4,
+                           {skip, delta_bias, lengths, Agrad, skipgrad, biasgrad})) != PC2D_OK)
     return st;
   ScanArgs a = scan_problem(batch, channels, length, states, groups);
   scan_split<true>(&a);
@@ -1518,7 +1521,10 @@ extern "C" int pc2d_ssm_scan_step(int dtype, const void *u, const void *delta, f
     set_last_error("pc2d_ssm_scan_step: null pointer (u, delta, state, A, B, C or output)");
     return PC2D_ERR_INVALID_ARGUMENT;
   }
-  if ((st = check_aligned("pc2d_ssm_scan_step", {state, A, B, C})) != PC2D_OK) return st;
+  if ((st = check_aligned("pc2d_ssm_scan_step", {state, A, B, C})) != PC2D_OK ||
+      (st = check_elements("pc2d_ssm_scan_step", seq_dtype_size(dtype), {u, delta, z, output})) != PC2D_OK ||
+      (st = check_elements("pc2d_ssm_scan_step", 4, {skip, delta_bias, slots})) != PC2D_OK)
+    return st;
   ScanStepArgs a{};
   a.u = u; a.delta = delta; a.z = z; a.B = B; a.C = C; a.A = A; a.skip = skip; a.bias = delta_bias;
   a.slots = slots; a.state = state; a.out = output;

@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <initializer_list>
 #include <type_traits>
 
 #include "pc2d_common.cuh"
@@ -100,6 +101,16 @@ inline bool seq_dtype(int dtype) {
 }
 inline size_t seq_dtype_size(int dtype) { return dtype == PC2D_DTYPE_F32 ? 4 : 2; }
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Arrays that are read element by element: each on a boundary of its elements,
+// off which any access faults.
+inline int check_elements(const char *what, size_t bytes, std::initializer_list<const void *> ptrs) {
+  for (const void *p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) {
+      set_last_error("%s: an array of %zu-byte elements is not aligned to them", what, bytes);
+      return PC2D_ERR_INVALID_ARGUMENT;
+    }
+  return PC2D_OK;
+}
 
 // Where a single-token step finds the state of batch row b: slots[b] of the
 // `places` rows of the state array, or row b without slots.  -1: the row is
