@@ -73,6 +73,17 @@ struct Call {
     TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, what, ": ", name,
                 " is updated in place and must start on a 16-byte boundary");
   }
+  // What a step reads may not lie within the state that it moves on: one row's
+  // place may be written before another row has read its input.
+  void apart(const Tensor &state, std::initializer_list<const Tensor *> inputs) const {
+    const auto first = reinterpret_cast<uintptr_t>(state.data_ptr()), last = first + state.nbytes();
+    for (const Tensor *t : inputs) {
+      if (!t->defined()) continue;
+      const auto at = reinterpret_cast<uintptr_t>(t->data_ptr());
+      TORCH_CHECK(at >= last || at + t->nbytes() <= first || !t->numel() || !state.numel(), what,
+                  ": an input shares memory with the state, which is updated in place");
+    }
+  }
 };
 
 template <typename T = void>
@@ -198,6 +209,7 @@ Tensor causal_conv_step_cuda(const Tensor &input_, Tensor state, const Tensor &w
   const Tensor weight = call.need(weight_, "weight", weight_.scalar_type(), weight_.sizes());
   const Tensor bias = call.maybe(bias_, "bias", weight_.scalar_type(), {channels});
   const Tensor slots = call.maybe(slots_, "slots", at::kInt, {batch});
+  call.apart(state, {&input, &weight, &bias, &slots});
   Tensor out = at::empty({batch, channels}, input.options());
   check_status(pc2d_causal_conv_step(dt, wdt, ptr(input), ptr(state), ptr(weight), ptr(bias), ptr<int>(slots), batch,
                                      places, channels, taps, silu, ptr(out), stream_now()),
@@ -317,6 +329,7 @@ Tensor ssm_scan_step_cuda(const Tensor &u_, const Tensor &delta_, Tensor state, 
   const Tensor skip = call.maybe(D_, "D", at::kFloat, {channels}), z = call.maybe(z_, "z", type, u.sizes());
   const Tensor bias = call.maybe(bias_, "delta_bias", at::kFloat, {channels});
   const Tensor slots = call.maybe(slots_, "slots", at::kInt, {batch});
+  call.apart(state, {&u, &delta, &A, &B, &C, &skip, &z, &bias, &slots});
   Tensor out = at::empty({batch, channels}, u.options());
   check_status(pc2d_ssm_scan_step(dt, ptr(u), ptr(delta), ptr<float>(state), ptr<float>(A), ptr(B), ptr(C),
                                   ptr<float>(skip), ptr(z), ptr<float>(bias), ptr<int>(slots), delta_softplus, batch,

@@ -127,7 +127,7 @@ def causal_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Te
     [batch], on the GPU), or place b without slots.  A slot of -1 marks a row
     without a request: its output is 0 and no state changes.  A slot outside
     the states, or one that an earlier row has too, makes the row NaN and
-    changes no state."""
+    changes no state.  Inputs that share memory with ``state`` are refused."""
     return _ops.causal_conv_step(x, state, weight, bias, slots, _silu(activation))
 
 

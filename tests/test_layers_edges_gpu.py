@@ -1,0 +1,53 @@
+"""The layers beside ParaConv2d on the GPU where a call or a value leaves the
+ordinary.  Tolerances as in test_layers_gpu.py, unless said at the test.
+"""
+import math
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+import layers_ref as ref
+import paraconv2d_b200 as pc
+from test_layers_gpu import DEV, SCAN_GRADS, check, conv_case, dev, gen, scan_call, scan_case
+
+pytestmark = pytest.mark.gpu
+
+
+# --------------------------------------------------------------------- steps
+
+def test_steps_refuse_inputs_within_their_state():
+    """A view of the state as a token: other rows' places would be written
+    while it is read.  Neighbours of the state in one allocation are fine, and
+    so are views that have to be copied first."""
+    w = torch.randn(16, 2, device=DEV)
+    pool = torch.randn(6, 16, 1, device=DEV)
+    slots = torch.tensor([2, 3], dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError, match="shares memory with the state"):
+        pc.causal_conv_step(pool[:2, :, 0], pool, w, slots=slots)
+    with pytest.raises(RuntimeError, match="shares memory with the state"):
+        pc.causal_conv_step(torch.zeros(2, 16, device=DEV), pool, w, bias=pool[5, :, 0], slots=slots)
+    before = pool.clone()
+    got = pc.causal_conv_step(pool[:2, :, 0], pool[2:4], w)
+    assert torch.equal(got, pc.causal_conv_step(before[:2, :, 0], before[2:4].clone(), w))
+    u, B = torch.randn(2, 16, device=DEV), torch.randn(2, 1, 16, device=DEV)
+    A = -torch.rand(16, 16, device=DEV)
+    pool = torch.randn(6, 16, 16, device=DEV)
+    names = dict(u=u, delta=u.abs(), A=A, B=B, C=B, D=u[0].clone(), z=u.clone(), delta_bias=u[1].clone())
+
+    def step(state, **kw):
+        t = {**names, **kw}
+        return pc.ssm_scan_step(t["u"], t["delta"], state, t["A"], t["B"], t["C"], D=t["D"], z=t["z"],
+                                delta_bias=t["delta_bias"], slots=slots)
+
+    step(pool)
+    within = dict(u=pool[0, :2], delta=pool[5, 14:], A=pool[1], B=pool[0, :2].view(2, 1, 16), C=pool[5, 14:].view(2, 1, 16),
+                  D=pool[0, 0], z=pool[0, :2], delta_bias=pool[5, 15])
+    for k, v in within.items():
+        with pytest.raises(RuntimeError, match="shares memory with the state"):
+            step(pool, **{k: v})
+    # a strided view is copied before anything is written
+    views, whole = pool.clone(), pool.clone()
+    got = step(views, u=views[:2, :, 3])
+    assert torch.equal(got, step(whole, u=pool[:2, :, 3].contiguous())) and torch.equal(views, whole)
+
