@@ -16,6 +16,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <climits>
@@ -352,6 +353,16 @@ bool needs_grad(std::initializer_list<const Tensor *> tensors, std::initializer_
   return false;
 }
 
+// A derivative that comes with an input (forward mode) would be lost without a
+// word in the kernels' outputs.
+void no_forward_mode(const char *what, std::initializer_list<const Tensor *> tensors,
+                     std::initializer_list<const OptTensor *> optional) {
+  bool any = false;
+  for (const Tensor *t : tensors) any = any || torch::autograd::isFwGradDefined(*t);
+  for (const OptTensor *t : optional) any = any || torch::autograd::isFwGradDefined(*t);
+  TORCH_CHECK_NOT_IMPLEMENTED(!any, "paraconv2d_b200.", what, ": forward-mode derivatives are not implemented");
+}
+
 void check_cuda(const Tensor &t, const char *what) {
   TORCH_CHECK_NOT_IMPLEMENTED(t.is_cuda(), "paraconv2d_b200.", what, ": CUDA tensors only, got one on ", t.device());
 }
@@ -406,6 +417,7 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
 };
 
 Tensor dropout_autograd(const Tensor &input, const Tensor &key, double p, const OptTensor &residual) {
+  no_forward_mode("dropout", {&input}, {&residual});
   check_cuda(input, "dropout");
   if (needs_grad({&input}, {&residual})) return DropoutFunction::apply(input, key, p, residual);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -440,6 +452,7 @@ struct ConvFunction : torch::autograd::Function<ConvFunction> {
 std::vector<Tensor> causal_conv_forward_autograd(const Tensor &input, const Tensor &weight, const OptTensor &bias,
                                                  const OptTensor &initial, const OptTensor &lengths, bool silu,
                                                  bool final_state) {
+  no_forward_mode("causal_conv", {&input, &weight}, {&bias, &initial});
   check_cuda(input, "causal_conv");
   if (needs_grad({&input, &weight}, {&bias, &initial}))
     return ConvFunction::apply(input, weight, bias, initial, lengths, silu, final_state);
@@ -487,6 +500,7 @@ std::vector<Tensor> ssm_scan_forward_autograd(const Tensor &u, const Tensor &del
                                               const OptTensor &delta_bias, const OptTensor &initial,
                                               const OptTensor &lengths, bool delta_softplus, bool final_state,
                                               bool checkpoints) {
+  no_forward_mode("ssm_scan", {&u, &delta, &A, &B, &C}, {&D, &z, &delta_bias, &initial});
   check_cuda(u, "ssm_scan");
   if (needs_grad({&u, &delta, &A, &B, &C}, {&D, &z, &delta_bias, &initial})) {
     auto outs = ScanFunction::apply(u, delta, A, B, C, D, z, delta_bias, initial, lengths, delta_softplus, final_state);
@@ -510,6 +524,7 @@ void changed(const Tensor &state) {
 
 Tensor causal_conv_step_autograd(const Tensor &input, Tensor state, const Tensor &weight, const OptTensor &bias,
                                  const OptTensor &slots, bool silu) {
+  no_forward_mode("causal_conv_step", {&input, &state, &weight}, {&bias});
   no_step_grad("causal_conv_step", needs_grad({&input, &state, &weight}, {&bias}));
   check_cuda(input, "causal_conv_step");
   at::AutoDispatchBelowADInplaceOrView below;
@@ -521,6 +536,7 @@ Tensor causal_conv_step_autograd(const Tensor &input, Tensor state, const Tensor
 Tensor ssm_scan_step_autograd(const Tensor &u, const Tensor &delta, Tensor state, const Tensor &A, const Tensor &B,
                               const Tensor &C, const OptTensor &D, const OptTensor &z, const OptTensor &delta_bias,
                               const OptTensor &slots, bool delta_softplus) {
+  no_forward_mode("ssm_scan_step", {&u, &delta, &state, &A, &B, &C}, {&D, &z, &delta_bias});
   no_step_grad("ssm_scan_step", needs_grad({&u, &delta, &state, &A, &B, &C}, {&D, &z, &delta_bias}));
   check_cuda(u, "ssm_scan_step");
   at::AutoDispatchBelowADInplaceOrView below;

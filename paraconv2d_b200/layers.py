@@ -18,10 +18,11 @@ convolution layer is one with ``x.flatten(2)``, and goes back with
 CUDA tensors only (float32, float16 and bfloat16; dropout float64 too), on the
 current stream of the tensors' device; sums and states in 32 bits.  Results
 and gradients are deterministic.  Dropout is differentiable any number of
-times, the convolution and the scan once.  All of it, backward passes too, can
-be captured into CUDA graphs; as for every backward pass, leaves that still
-belong to an eager autograd graph made on another stream must be released (or
-their graph run on the capturing stream) before that.
+times, the convolution and the scan once; forward-mode derivatives are
+refused.  All of it, backward passes too, can be captured into CUDA graphs; as
+for every backward pass, leaves that still belong to an eager autograd graph
+made on another stream must be released (or their graph run on the capturing
+stream) before that.
 """
 from __future__ import annotations
 

@@ -1,7 +1,10 @@
 """Calls of the layers beside ParaConv2d that have to be refused before
 anything is launched, or that a tracer makes: without a GPU."""
 import pytest
+import torch
+import torch.autograd.forward_ad as fwd
 
+import paraconv2d_b200 as pc
 from paraconv2d_b200 import _lib
 
 lib = _lib.cabi()
@@ -70,3 +73,46 @@ def test_wider_elements_off_their_boundary_are_refused():
         assert lib.pc2d_dropout(dtype, ONE, None, ONE + 4, 0.5, 8, ONE, None) == INVALID
     assert lib.pc2d_dropout_next_key(ONE + 4, ONE, None) == INVALID
     assert lib.pc2d_dropout_next_key(ONE, ONE + 4, None) == INVALID
+
+
+def _fw_calls():
+    """Each entry point with each of its tensors that can carry a derivative."""
+    r = lambda *s: torch.randn(*s)  # noqa: E731
+    key = torch.tensor([1, 2])
+    x, w, one = r(2, 6, 8), r(6, 4), r(2, 6)
+    yield "dropout", lambda t: pc.dropout(t["x"], 0.5, key, residual=t["residual"]), dict(x=x, residual=r(2, 6, 8))
+    yield "causal_conv", lambda t: pc.causal_conv(t["x"], t["w"], t["b"], None, t["init"]), dict(x=x, w=w, b=r(6), init=r(2, 6, 3))
+    yield "causal_conv_step", lambda t: pc.causal_conv_step(t["x"], t["state"], t["w"], t["b"]), dict(
+        x=one, state=r(2, 6, 3), w=w, b=r(6))
+    scan = dict(u=x, delta=x, A=r(6, 4), B=r(2, 1, 4, 8), C=r(2, 1, 4, 8), D=r(6), z=x, bias=r(6), init=r(2, 6, 4))
+    yield "ssm_scan", lambda t: pc.ssm_scan(t["u"], t["delta"], t["A"], t["B"], t["C"], t["D"], t["z"], t["bias"], True,
+                                            t["init"]), scan
+    step = dict(u=one, delta=one, state=r(2, 6, 4), A=r(6, 4), B=r(2, 1, 4), C=r(2, 1, 4), D=r(6), z=one, bias=r(6))
+    yield "ssm_scan_step", lambda t: pc.ssm_scan_step(t["u"], t["delta"], t["state"], t["A"], t["B"], t["C"], t["D"],
+                                                      t["z"], t["bias"]), step
+
+
+FW = {name: (call, tensors) for name, call, tensors in _fw_calls()}
+
+
+@pytest.mark.parametrize("name", list(FW))
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(name, grad):
+    """With a tangent in any input: an error that says so, not an output
+    without a derivative.  (Before the refusal of tensors on the CPU.)"""
+    call, tensors = FW[name]
+    for k, v in tensors.items():
+        with fwd.dual_level():
+            dual = fwd.make_dual(v.clone().requires_grad_() if grad and "step" not in name else v, torch.ones_like(v))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call({**tensors, k: dual})
+        with pytest.raises(NotImplementedError, match="CUDA tensors only|CPU"):
+            call(tensors)
+
+
+@pytest.mark.parametrize("name", ["dropout", "causal_conv", "ssm_scan"])
+def test_jvp_is_refused(name):
+    call, tensors = FW[name]
+    k = next(iter(tensors))
+    with pytest.raises((NotImplementedError, RuntimeError), match="forward-mode|functorch"):
+        torch.func.jvp(lambda v: call({**tensors, k: v}), (tensors[k],), (torch.ones_like(tensors[k]),))

@@ -51,3 +51,30 @@ def test_steps_refuse_inputs_within_their_state():
     got = step(views, u=views[:2, :, 3])
     assert torch.equal(got, step(whole, u=pool[:2, :, 3].contiguous())) and torch.equal(views, whole)
 
+
+# ------------------------------------------------------------------ autograd
+
+def test_forward_mode_is_refused():
+    """An input with a tangent: no derivative rather than one of zero."""
+    c, _, _, _ = scan_case(1, 2, 6, 8, 4, 1, torch.float32)
+    t = {k: dev(a) for k, a in c.items()}
+    key = torch.tensor([1, 2], device=DEV)
+    one = {k: (v[..., 0].contiguous() if k in ("u", "delta", "z", "B", "C") else v) for k, v in t.items()}
+    w = torch.randn(6, 4, device=DEV)
+    with fwd.dual_level():
+        dual = {k: fwd.make_dual(v, torch.ones_like(v)) for k, v in t.items()}
+        for k in dual:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                scan_call({**t, k: dual[k]}, True, None)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            pc.dropout(dual["u"], 0.5, key)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            pc.dropout(t["u"], 0.5, key, residual=dual["u"])
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            pc.causal_conv(t["u"], fwd.make_dual(w, w))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            pc.causal_conv_step(fwd.make_dual(one["u"], one["u"]), torch.zeros(2, 6, 3, device=DEV), w)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            pc.ssm_scan_step(one["u"], one["delta"], fwd.make_dual(t["init"].clone(), t["init"]), one["A"], one["B"], one["C"])
+    assert torch.equal(scan_call(t, True, None), scan_call(t, True, None))
+
