@@ -102,6 +102,13 @@ Tensor workspace(size_t bytes, const Tensor &like) {
   return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 
+// What a call changes in place, autograd must know to be no longer what it may
+// have saved.  (Here, and not in an Autograd kernel, which inference mode and
+// redispatched calls pass by.)
+void changed(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // ------------------------------------------------------------------- dropout
 
 Tensor dropout_cuda(const Tensor &input_, const Tensor &key_, double p, const OptTensor &residual_) {
@@ -123,6 +130,7 @@ Tensor dropout_next_key_cuda(Tensor state) {
   call.in_place(state, "state", at::kLong, {2});
   Tensor key = at::empty({2}, state.options());
   check_status(pc2d_dropout_next_key(ptr<int64_t>(state), ptr<int64_t>(key), stream_now()), call.what);
+  changed(state);
   return key;
 }
 
@@ -215,6 +223,7 @@ Tensor causal_conv_step_cuda(const Tensor &input_, Tensor state, const Tensor &w
   check_status(pc2d_causal_conv_step(dt, wdt, ptr(input), ptr(state), ptr(weight), ptr(bias), ptr<int>(slots), batch,
                                      places, channels, taps, silu, ptr(out), stream_now()),
                call.what);
+  changed(state);
   return out;
 }
 
@@ -336,6 +345,7 @@ Tensor ssm_scan_step_cuda(const Tensor &u_, const Tensor &delta_, Tensor state, 
                                   ptr<float>(skip), ptr(z), ptr<float>(bias), ptr<int>(slots), delta_softplus, batch,
                                   places, channels, states, groups, ptr(out), stream_now()),
                call.what);
+  changed(state);
   return out;
 }
 
@@ -512,14 +522,10 @@ std::vector<Tensor> ssm_scan_forward_autograd(const Tensor &u, const Tensor &del
                                checkpoints);
 }
 
-// A step changes its state in place: there is no gradient, and what autograd
-// has saved of the state is no longer what it was.
+// A step changes its state in place: there is no gradient.
 void no_step_grad(const char *what, bool needs) {
   TORCH_CHECK(!needs, "paraconv2d_b200.", what, " moves its state on in place and has no backward pass: call it under "
               "torch.no_grad(), or use the operator over whole sequences");
-}
-void changed(const Tensor &state) {
-  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
 }
 
 Tensor causal_conv_step_autograd(const Tensor &input, Tensor state, const Tensor &weight, const OptTensor &bias,
@@ -528,9 +534,7 @@ Tensor causal_conv_step_autograd(const Tensor &input, Tensor state, const Tensor
   no_step_grad("causal_conv_step", needs_grad({&input, &state, &weight}, {&bias}));
   check_cuda(input, "causal_conv_step");
   at::AutoDispatchBelowADInplaceOrView below;
-  Tensor out = causal_conv_step_cuda(input, state, weight, bias, slots, silu);
-  changed(state);
-  return out;
+  return causal_conv_step_cuda(input, state, weight, bias, slots, silu);
 }
 
 Tensor ssm_scan_step_autograd(const Tensor &u, const Tensor &delta, Tensor state, const Tensor &A, const Tensor &B,
@@ -540,9 +544,7 @@ Tensor ssm_scan_step_autograd(const Tensor &u, const Tensor &delta, Tensor state
   no_step_grad("ssm_scan_step", needs_grad({&u, &delta, &state, &A, &B, &C}, {&D, &z, &delta_bias}));
   check_cuda(u, "ssm_scan_step");
   at::AutoDispatchBelowADInplaceOrView below;
-  Tensor out = ssm_scan_step_cuda(u, delta, state, A, B, C, D, z, delta_bias, slots, delta_softplus);
-  changed(state);
-  return out;
+  return ssm_scan_step_cuda(u, delta, state, A, B, C, D, z, delta_bias, slots, delta_softplus);
 }
 
 }  // namespace

@@ -78,3 +78,31 @@ def test_forward_mode_is_refused():
             pc.ssm_scan_step(one["u"], one["delta"], fwd.make_dual(t["init"].clone(), t["init"]), one["A"], one["B"], one["C"])
     assert torch.equal(scan_call(t, True, None), scan_call(t, True, None))
 
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_what_autograd_saved_and_a_call_changed_is_noticed(mode):
+    """A key that is counted on, and kept inputs that a step moves on, between
+    a call that saved them and its backward pass."""
+    x = torch.randn(2, 6, 9, device=DEV, requires_grad=True)
+    w = torch.randn(6, 4, device=DEV)
+    state = torch.tensor([5, 0], device=DEV)
+    out = pc.dropout(x, 0.5, state)
+    with mode():
+        torch.ops.paraconv2d_b200.dropout_next_key(state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    kept = torch.randn(2, 6, 3, device=DEV)
+    out = pc.causal_conv(x, w, initial_state=kept)
+    with mode():
+        pc.causal_conv_step(x.detach()[..., 0], kept, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    h = torch.randn(2, 6, 4, device=DEV)
+    before = h._version
+    with mode():
+        pc.ssm_scan_step(x.detach()[..., 0], x.detach()[..., 0], h, -torch.ones(6, 4, device=DEV),
+                         torch.ones(2, 1, 4, device=DEV), torch.ones(2, 1, 4, device=DEV))
+    assert h._version > before
+    with torch.inference_mode():  # (an inference tensor has no version to count)
+        pc.causal_conv_step(x.detach()[..., 0], torch.zeros(2, 6, 3, device=DEV), w)
+
