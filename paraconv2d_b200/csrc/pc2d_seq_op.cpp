@@ -10,13 +10,14 @@
 //
 // The gradients are registered here as well (Autograd key): a training step of
 // a small layer is bound by the host, and going through Python functions took
-// it about twice as long.  The backward passes are differentiable once.
+// it about twice as long.  The backward passes are differentiable once.  The
+// Autograd kernels go on through the dispatcher (0.3 us a call), as whatever
+// stands in between has to see the calls.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <climits>
@@ -200,7 +201,7 @@ std::vector<Tensor> causal_conv_backward_cuda(const Tensor &grad_, const OptTens
   return {dx, dw, db, di};
 }
 
-Tensor causal_conv_step_cuda(const Tensor &input_, Tensor state, const Tensor &weight_, const OptTensor &bias_,
+Tensor causal_conv_step_cuda(const Tensor &input_, const Tensor &state, const Tensor &weight_, const OptTensor &bias_,
                              const OptTensor &slots_, bool silu) {
   const Call call{"paraconv2d_b200.causal_conv_step", input_.device()};
   const c10::cuda::CUDAGuard guard(input_.device());
@@ -315,7 +316,7 @@ std::vector<Tensor> ssm_scan_backward_cuda(const Tensor &grad_, const OptTensor 
   return {du, dd, dA, dB, dC, given(dskip), given(dz), given(dbias), given(dinit)};
 }
 
-Tensor ssm_scan_step_cuda(const Tensor &u_, const Tensor &delta_, Tensor state, const Tensor &A_, const Tensor &B_,
+Tensor ssm_scan_step_cuda(const Tensor &u_, const Tensor &delta_, const Tensor &state, const Tensor &A_, const Tensor &B_,
                           const Tensor &C_, const OptTensor &D_, const OptTensor &z_, const OptTensor &bias_,
                           const OptTensor &slots_, bool delta_softplus) {
   const Call call{"paraconv2d_b200.ssm_scan_step", u_.device()};
@@ -364,18 +365,35 @@ bool needs_grad(std::initializer_list<const Tensor *> tensors, std::initializer_
 }
 
 // A derivative that comes with an input (forward mode) would be lost without a
-// word in the kernels' outputs.
+// word in the kernels' outputs.  (What autograd has nothing to say about has
+// none: steps, which the host bounds, mostly end there.)
+bool has_tangent(const Tensor &t) {
+  return t.defined() && t.unsafeGetTensorImpl()->autograd_meta() && t._fw_grad(0).defined();
+}
 void no_forward_mode(const char *what, std::initializer_list<const Tensor *> tensors,
                      std::initializer_list<const OptTensor *> optional) {
   bool any = false;
-  for (const Tensor *t : tensors) any = any || torch::autograd::isFwGradDefined(*t);
-  for (const OptTensor *t : optional) any = any || torch::autograd::isFwGradDefined(*t);
+  for (const Tensor *t : tensors) any = any || has_tangent(*t);
+  for (const OptTensor *t : optional) any = any || (t->has_value() && has_tangent(**t));
   TORCH_CHECK_NOT_IMPLEMENTED(!any, "paraconv2d_b200.", what, ": forward-mode derivatives are not implemented");
 }
 
 void check_cuda(const Tensor &t, const char *what) {
   TORCH_CHECK_NOT_IMPLEMENTED(t.is_cuda(), "paraconv2d_b200.", what, ": CUDA tensors only, got one on ", t.device());
 }
+
+// The op's kernel below Autograd, through the dispatcher: modes and tracers that
+// stand in between (fake tensors among them) see the call.  Signature: that of
+// the CUDA function.
+template <typename Signature>
+auto below_autograd(const char *name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
+}
+#define PC2D_BELOW(op)                                                                                 \
+  ([]() -> const auto & {                                                                              \
+    static const auto handle = below_autograd<decltype(op##_cuda)>("paraconv2d_b200::" #op);          \
+    return handle;                                                                                     \
+  }())
 
 OptTensor optional_of(const Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
@@ -386,6 +404,7 @@ variable_list once(const char *what, F &&run) {
   variable_list grads;
   {
     at::AutoGradMode off(false);
+    at::AutoDispatchBelowADInplaceOrView below;
     grads = run();
   }
   if (at::GradMode::is_enabled()) {
@@ -412,16 +431,15 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
     ctx->saved_data["p"] = p;
     ctx->saved_data["input"] = input.requires_grad();
     ctx->saved_data["residual"] = residual.has_value() && residual->defined() && residual->requires_grad();
-    return dropout_cuda(input, key, p, residual);
+    return PC2D_BELOW(dropout).call(input, key, p, residual);
   }
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
     const Tensor key = ctx->get_saved_variables()[0];
     // (linear: its gradient is the same operation, which may be differentiated again)
-    static const auto op = c10::Dispatcher::singleton()
-                               .findSchemaOrThrow("paraconv2d_b200::dropout", "")
-                               .typed<Tensor(const Tensor &, const Tensor &, double, const OptTensor &)>();
+    // (through Autograd again)
     Tensor dx;
-    if (ctx->saved_data["input"].toBool()) dx = op.call(grads[0], key, ctx->saved_data["p"].toDouble(), OptTensor());
+    if (ctx->saved_data["input"].toBool())
+      dx = PC2D_BELOW(dropout).call(grads[0], key, ctx->saved_data["p"].toDouble(), OptTensor());
     return {dx, Tensor(), Tensor(), ctx->saved_data["residual"].toBool() ? grads[0] : Tensor()};
   }
 };
@@ -431,15 +449,15 @@ Tensor dropout_autograd(const Tensor &input, const Tensor &key, double p, const 
   check_cuda(input, "dropout");
   if (needs_grad({&input}, {&residual})) return DropoutFunction::apply(input, key, p, residual);
   at::AutoDispatchBelowADInplaceOrView below;
-  return dropout_cuda(input, key, p, residual);
+  return PC2D_BELOW(dropout).call(input, key, p, residual);
 }
 
 struct ConvFunction : torch::autograd::Function<ConvFunction> {
   static variable_list forward(AutogradContext *ctx, const Tensor &input, const Tensor &weight, const OptTensor &bias,
                                const OptTensor &initial, const OptTensor &lengths, bool silu, bool final_state) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor x = dense(input);
-    auto outs = causal_conv_forward_cuda(x, weight, bias, initial, lengths, silu, final_state);
+    const Tensor x = input.contiguous();
+    auto outs = PC2D_BELOW(causal_conv_forward).call(x, weight, bias, initial, lengths, silu, final_state);
     ctx->save_for_backward({x, weight, bias.value_or(Tensor()), initial.value_or(Tensor()), lengths.value_or(Tensor())});
     ctx->saved_data["silu"] = silu;
     ctx->set_materialize_grads(false);
@@ -448,11 +466,11 @@ struct ConvFunction : torch::autograd::Function<ConvFunction> {
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
     return once("causal_conv", [&]() -> variable_list {
       const auto saved = ctx->get_saved_variables();
-      const c10::cuda::CUDAGuard guard(saved[0].device());
       const Tensor grad = grads[0].defined() ? grads[0] : at::zeros_like(saved[0]);
-      const auto g = causal_conv_backward_cuda(grad, grads.size() > 1 ? optional_of(grads[1]) : OptTensor(), saved[0],
-                                               saved[1], optional_of(saved[2]), optional_of(saved[3]),
-                                               optional_of(saved[4]), ctx->saved_data["silu"].toBool());
+      const auto g = PC2D_BELOW(causal_conv_backward)
+                         .call(grad, grads.size() > 1 ? optional_of(grads[1]) : OptTensor(), saved[0], saved[1],
+                               optional_of(saved[2]), optional_of(saved[3]), optional_of(saved[4]),
+                               ctx->saved_data["silu"].toBool());
       return {g[0], g[1], saved[2].defined() ? g[2] : Tensor(), saved[3].defined() ? g[3] : Tensor(),
               Tensor(), Tensor(), Tensor()};
     });
@@ -467,7 +485,7 @@ std::vector<Tensor> causal_conv_forward_autograd(const Tensor &input, const Tens
   if (needs_grad({&input, &weight}, {&bias, &initial}))
     return ConvFunction::apply(input, weight, bias, initial, lengths, silu, final_state);
   at::AutoDispatchBelowADInplaceOrView below;
-  return causal_conv_forward_cuda(input, weight, bias, initial, lengths, silu, final_state);
+  return PC2D_BELOW(causal_conv_forward).call(input, weight, bias, initial, lengths, silu, final_state);
 }
 
 struct ScanFunction : torch::autograd::Function<ScanFunction> {
@@ -476,10 +494,11 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
                                const OptTensor &delta_bias, const OptTensor &initial, const OptTensor &lengths,
                                bool delta_softplus, bool final_state) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor u = dense(u_), delta = dense(delta_), A = dense(A_), B = dense(B_), C = dense(C_);
-    const Tensor z = z_.has_value() && z_->defined() ? dense(*z_) : Tensor();
-    auto outs = ssm_scan_forward_cuda(u, delta, A, B, C, D, optional_of(z), delta_bias, initial, lengths,
-                                      delta_softplus, final_state, true);
+    const Tensor u = u_.contiguous(), delta = delta_.contiguous(), A = A_.contiguous(), B = B_.contiguous(),
+                 C = C_.contiguous();
+    const Tensor z = z_.has_value() && z_->defined() ? z_->contiguous() : Tensor();
+    auto outs = PC2D_BELOW(ssm_scan_forward).call(u, delta, A, B, C, D, optional_of(z), delta_bias, initial, lengths,
+                                                  delta_softplus, final_state, true);
     ctx->save_for_backward({u, delta, A, B, C, D.value_or(Tensor()), z, delta_bias.value_or(Tensor()),
                             lengths.value_or(Tensor()), outs[2]});
     ctx->saved_data["softplus"] = delta_softplus;
@@ -492,12 +511,12 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
     return once("ssm_scan", [&]() -> variable_list {
       const auto s = ctx->get_saved_variables();
-      const c10::cuda::CUDAGuard guard(s[0].device());
       const Tensor grad = grads[0].defined() ? grads[0] : at::zeros_like(s[0]);
       const bool initial = ctx->saved_data["initial"].toBool();
-      const auto g = ssm_scan_backward_cuda(grad, grads.size() > 1 ? optional_of(grads[1]) : OptTensor(), s[0], s[1],
-                                            s[2], s[3], s[4], optional_of(s[5]), optional_of(s[6]), optional_of(s[7]),
-                                            optional_of(s[8]), s[9], ctx->saved_data["softplus"].toBool(), initial);
+      const auto g = PC2D_BELOW(ssm_scan_backward)
+                         .call(grad, grads.size() > 1 ? optional_of(grads[1]) : OptTensor(), s[0], s[1], s[2], s[3],
+                               s[4], optional_of(s[5]), optional_of(s[6]), optional_of(s[7]), optional_of(s[8]), s[9],
+                               ctx->saved_data["softplus"].toBool(), initial);
       return {g[0], g[1], g[2], g[3], g[4], s[5].defined() ? g[5] : Tensor(), s[6].defined() ? g[6] : Tensor(),
               s[7].defined() ? g[7] : Tensor(), initial ? g[8] : Tensor(), Tensor(), Tensor(), Tensor()};
     });
@@ -518,8 +537,8 @@ std::vector<Tensor> ssm_scan_forward_autograd(const Tensor &u, const Tensor &del
     return outs;
   }
   at::AutoDispatchBelowADInplaceOrView below;
-  return ssm_scan_forward_cuda(u, delta, A, B, C, D, z, delta_bias, initial, lengths, delta_softplus, final_state,
-                               checkpoints);
+  return PC2D_BELOW(ssm_scan_forward).call(u, delta, A, B, C, D, z, delta_bias, initial, lengths, delta_softplus,
+                                           final_state, checkpoints);
 }
 
 // A step changes its state in place: there is no gradient.
@@ -528,23 +547,23 @@ void no_step_grad(const char *what, bool needs) {
               "torch.no_grad(), or use the operator over whole sequences");
 }
 
-Tensor causal_conv_step_autograd(const Tensor &input, Tensor state, const Tensor &weight, const OptTensor &bias,
+Tensor causal_conv_step_autograd(const Tensor &input, const Tensor &state, const Tensor &weight, const OptTensor &bias,
                                  const OptTensor &slots, bool silu) {
   no_forward_mode("causal_conv_step", {&input, &state, &weight}, {&bias});
   no_step_grad("causal_conv_step", needs_grad({&input, &state, &weight}, {&bias}));
   check_cuda(input, "causal_conv_step");
   at::AutoDispatchBelowADInplaceOrView below;
-  return causal_conv_step_cuda(input, state, weight, bias, slots, silu);
+  return PC2D_BELOW(causal_conv_step).call(input, state, weight, bias, slots, silu);
 }
 
-Tensor ssm_scan_step_autograd(const Tensor &u, const Tensor &delta, Tensor state, const Tensor &A, const Tensor &B,
+Tensor ssm_scan_step_autograd(const Tensor &u, const Tensor &delta, const Tensor &state, const Tensor &A, const Tensor &B,
                               const Tensor &C, const OptTensor &D, const OptTensor &z, const OptTensor &delta_bias,
                               const OptTensor &slots, bool delta_softplus) {
   no_forward_mode("ssm_scan_step", {&u, &delta, &state, &A, &B, &C}, {&D, &z, &delta_bias});
   no_step_grad("ssm_scan_step", needs_grad({&u, &delta, &state, &A, &B, &C}, {&D, &z, &delta_bias}));
   check_cuda(u, "ssm_scan_step");
   at::AutoDispatchBelowADInplaceOrView below;
-  return ssm_scan_step_cuda(u, delta, state, A, B, C, D, z, delta_bias, slots, delta_softplus);
+  return PC2D_BELOW(ssm_scan_step).call(u, delta, state, A, B, C, D, z, delta_bias, slots, delta_softplus);
 }
 
 }  // namespace

@@ -3,6 +3,7 @@ anything is launched, or that a tracer makes: without a GPU."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
+from torch._subclasses.fake_tensor import FakeTensorMode, UnsupportedOperatorException
 
 import paraconv2d_b200 as pc
 from paraconv2d_b200 import _lib
@@ -116,3 +117,21 @@ def test_jvp_is_refused(name):
     k = next(iter(tensors))
     with pytest.raises((NotImplementedError, RuntimeError), match="forward-mode|functorch"):
         torch.func.jvp(lambda v: call({**tensors, k: v}), (tensors[k],), (torch.ones_like(tensors[k]),))
+
+
+@pytest.mark.parametrize("name", list(FW))
+@pytest.mark.parametrize("grad", [False, True])
+def test_fake_tensors_are_refused_as_a_tracer_expects(name, grad, recwarn):
+    """Tensors without data (a tracer's) on a GPU that need not be there: no
+    kernel's host code runs on them, and the error is the tracer's own."""
+    call, tensors = FW[name]
+    key = {"key": torch.zeros(2, dtype=torch.int64)}
+    with FakeTensorMode():
+        t = {k: torch.empty(v.shape, device="cuda", dtype=v.dtype) for k, v in {**tensors, **key}.items()}
+        if grad and "step" not in name:
+            t[next(iter(tensors))].requires_grad_()
+        if name == "dropout":
+            call = lambda t: pc.dropout(t["x"], 0.5, t["key"], residual=t["residual"])  # noqa: E731
+        with pytest.raises(UnsupportedOperatorException):
+            call(t)
+    assert not [w for w in recwarn if "data pointer" in str(w.message)]

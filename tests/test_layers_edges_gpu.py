@@ -106,3 +106,28 @@ def test_what_autograd_saved_and_a_call_changed_is_noticed(mode):
     with torch.inference_mode():  # (an inference tensor has no version to count)
         pc.causal_conv_step(x.detach()[..., 0], torch.zeros(2, 6, 3, device=DEV), w)
 
+
+def test_dispatch_modes_see_the_calls():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Log(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(func.name())
+            return func(*args, **(kwargs or {}))
+
+    c, go, _, _ = scan_case(1, 2, 6, 8, 4, 1, torch.float32)
+    t = {k: dev(a).requires_grad_() for k, a in c.items()}
+    w = torch.randn(6, 4, device=DEV, requires_grad=True)
+    with Log() as log:
+        y = pc.dropout(scan_call({**t, "u": pc.causal_conv(t["u"], w)}, True, None), 0.5, torch.tensor([1, 2], device=DEV))
+        torch.autograd.grad(y, [t["u"], w], dev(go))
+        with torch.no_grad():
+            pc.causal_conv_step(t["u"][..., 0], torch.zeros(2, 6, 3, device=DEV), w)
+    own = [n.split("::")[1] for n in log.names if n.startswith("paraconv2d_b200")]
+    assert own == ["causal_conv_forward", "ssm_scan_forward", "dropout", "dropout", "ssm_scan_backward",
+                   "causal_conv_backward", "causal_conv_step"]
+
