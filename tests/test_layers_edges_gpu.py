@@ -131,3 +131,74 @@ def test_dispatch_modes_see_the_calls():
     assert own == ["causal_conv_forward", "ssm_scan_forward", "dropout", "dropout", "ssm_scan_backward",
                    "causal_conv_backward", "causal_conv_step"]
 
+
+# ---------------------------------------------- infinities in the convolution
+
+def finite_part(t):
+    """What a finite value can contain."""
+    return torch.where(torch.isfinite(t), t, 0.0)
+
+
+def same_or_both_not_finite(got, value, mag, units, what):
+    """Finite where the formula's value is, and then within the tolerance."""
+    g = got.detach().cpu()
+    ok = torch.isfinite(value)
+    assert torch.equal(torch.isfinite(g), ok), (what, g, value)
+    check(torch.where(ok, g, 0.0), torch.where(ok, value, 0.0), torch.where(ok, mag, 0.0), units, what)
+
+
+@pytest.mark.parametrize("L", [5, 8, 13, 16, 21, 300, 523])
+@pytest.mark.parametrize("K", [2, 4, 8])
+def test_conv_weight_gradients_leave_out_what_taps_do_not_meet(L, K):
+    """A row's last tokens meet its last taps only, the kept inputs its first:
+    an infinity there makes those taps' gradients infinite and no others."""
+    c, go, gf, _ = conv_case(L + K, 2, 5, L, K, torch.float32, bias=False)
+    for b in range(2):
+        c["x"][b, 0, -1] = math.inf
+        c["x"][b, 1, -min(2, L)] = math.nan
+        c["init"][b, 2, 0] = -math.inf
+        c["init"][b, 3, -1] = math.inf
+    v, _ = ref.conv(c["x"], c["w"], None, False, c["init"], None, go, gf)
+    _, m = ref.conv(finite_part(c["x"]), c["w"], None, False, finite_part(c["init"]), None, go, gf)
+    assert torch.isfinite(v["dw"]).any() and not torch.isfinite(v["dw"]).all()
+    x, w, init = (dev(c[k]).requires_grad_() for k in ("x", "w", "init"))
+    out, final = pc.causal_conv(x, w, initial_state=init, return_final_state=True)
+    got = torch.autograd.grad([out, final], [x, w, init], [dev(go), dev(gf)])
+    for g, n in zip(got, ("dx", "dw", "dinit")):
+        same_or_both_not_finite(g, v[n], m[n], 160, n)
+    # the same rows within a padded batch
+    pad = torch.full((2, 5, L + 11), math.nan, device=DEV)
+    pad[..., :L] = x.detach()
+    pad.requires_grad_()
+    lens = torch.full((2,), L, dtype=torch.int32, device=DEV)
+    out, final = pc.causal_conv(pad, w, initial_state=init, lengths=lens, return_final_state=True)
+    pgo = torch.full((2, 5, L + 11), math.nan, device=DEV)
+    pgo[..., :L] = dev(go)
+    got = torch.autograd.grad([out, final], [pad, w, init], [pgo, dev(gf)])
+    assert not got[0][..., L:].any() and not out[..., L:].any()
+    for g, n in zip((got[0][..., :L], *got[1:]), ("dx", "dw", "dinit")):
+        same_or_both_not_finite(g, v[n], m[n], 160, n)
+
+
+@pytest.mark.parametrize("n", [1, 2, 13, 16, 290])
+@pytest.mark.parametrize("K", [1, 2, 4, 8])
+def test_conv_infinite_weights_reach_their_windows_only(n, K):
+    """An infinite weight: the gradient of an input that its tap does not meet
+    stays finite, and behind a row's tokens everything stays 0."""
+    L = n + 13
+    c, go, _, _ = conv_case(n + K, 2, 4, n, K, torch.float32, bias=False)
+    c["w"][0, 0], c["w"][1, -1], c["w"][2, K // 2] = math.inf, -math.inf, math.nan
+    go[:, :, n // 2] = 0.0
+    v, _ = ref.conv(c["x"], c["w"], None, False, c["init"], None, go, torch.zeros(2, 4, K - 1))
+    _, m = ref.conv(c["x"], finite_part(c["w"]), None, False, c["init"], None, go, torch.zeros(2, 4, K - 1))
+    x, pgo = (torch.full((2, 4, L), math.nan, device=DEV) for _ in range(2))
+    x[..., :n], pgo[..., :n] = dev(c["x"]), dev(go)
+    x.requires_grad_()
+    init = dev(c["init"]).requires_grad_()
+    out = pc.causal_conv(x, dev(c["w"]), initial_state=init, lengths=torch.full((2,), n, dtype=torch.int32, device=DEV))
+    dx, di = torch.autograd.grad(out, [x, init], pgo)
+    assert not out[..., n:].any() and not dx[..., n:].any()
+    same_or_both_not_finite(out[..., :n], v["out"], m["out"], 40, "out")
+    same_or_both_not_finite(dx[..., :n], v["dx"], m["dx"], 64, "dx")
+    same_or_both_not_finite(di, v["dinit"], m["dinit"], 64, "dinit")
+
