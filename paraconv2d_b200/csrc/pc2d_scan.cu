@@ -517,6 +517,73 @@ __device__ __forceinline__ void load_decay_rates(const ScanArgs &a, int d, int p
   for (int s = 0; s < kH; ++s) A2[s] = mul2(A2[s], F2(kLog2e, kLog2e));
 }
 
+// A segment's state after it: `own`, from zero, and the state h that entered it,
+// decayed by exp2(x).  The decay may leave 32 bits where the product does not,
+// so it goes in two halves then; 0 stays 0, and an infinite state infinite (as
+// it would token by token), whatever the decay.
+__device__ __forceinline__ float join_segment(float x, float h, float own) {
+  if (h == 0.f) return own;
+  if (fabsf(h) == __int_as_float(0x7f800000)) return h + own;
+  if (fabsf(x) <= 126.f) return fmaf(exp2_tile(x), h, own);
+  const float half = exp2_f(0.5f * x);
+  return fmaf(half, half * h, own);
+}
+// Takes the states h of a lane through the segments from `i` on, up to `stop` or
+// down to it; state and sum: those of the row's segment 0.  (Not inlined: called
+// once, it would only take registers from the kernels' loops.)
+struct LaneStates {
+  F2 h[kH];
+};
+__device__ __noinline__ LaneStates join_segments(const float *state, const float *sum, int64_t channels, int N, int p,
+                                                 F2 A0, F2 A1, int i, int stop, LaneStates in) {
+  const F2 A2[kH] = {A0, A1};
+  const int step = i < stop ? 1 : -1;
+  F2 h[kH] = {in.h[0], in.h[1]};
+  float largest = 0.f;
+  auto load = [&](int k, F2 (&own)[kH], F2 (&x)[kH]) {
+    load_states(state + k * channels * N, N, p, own);
+    const float d = sum[k * channels];
+#pragma unroll
+    for (int s = 0; s < kH; ++s) x[s] = mul2(F2(d, d), A2[s]);
+  };
+#pragma unroll 8
+  for (int k = i; k != stop; k += step) {
+    F2 own[kH], x[kH];
+    load(k, own, x);
+#pragma unroll
+    for (int s = 0; s < kH; ++s) {
+      largest = fmaxf(largest, fmaxf(fabsf(h[s].x()), fabsf(h[s].y())));
+      h[s] = fma2(exp2_tile2(x[s]), h[s], own[s]);
+    }
+  }
+  // An infinity or NaN may come of a decay alone (and stays).  A decay that
+  // underflows loses less than 2^-86 of what is at most 2^40.
+  const float sum_of = fabsf(h[0].x()) + fabsf(h[0].y()) + fabsf(h[1].x()) + fabsf(h[1].y());
+  if (!(sum_of < __int_as_float(0x7f800000)) || largest > 0x1p40f) {
+    h[0] = in.h[0];
+    h[1] = in.h[1];
+#pragma unroll 1
+    for (int k = i; k != stop; k += step) {
+      F2 own[kH], x[kH];
+      load(k, own, x);
+#pragma unroll
+      for (int s = 0; s < kH; ++s)
+        h[s] = F2(join_segment(x[s].x(), h[s].x(), own[s].x()), join_segment(x[s].y(), h[s].y(), own[s].y()));
+    }
+  }
+  return LaneStates{{h[0], h[1]}};
+}
+template <class G>
+__device__ __forceinline__ void enter_segment(const ScanArgs &a, const ScanPlace<G> &q, const F2 (&A2)[kH], int from,
+                                              F2 (&h)[kH]) {
+  if (from == q.seg) return;
+  const int64_t at = (int64_t)q.b * a.nseg * a.channels + q.d;
+  const LaneStates r = join_segments(a.seg_state + at * a.states, a.seg_sum + at, a.channels, a.states, q.p, A2[0],
+                                     A2[1], from, q.seg, LaneStates{{h[0], h[1]}});
+  h[0] = r.h[0];
+  h[1] = r.h[1];
+}
+
 // Forward pass; kStateOnly: the first pass over segments (end state from zero
 // and sum of D_t, no outputs).
 template <typename T, class G, bool kStateOnly>
@@ -542,16 +609,7 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_forward_kernel(S
   for (int s = 0; s < kH; ++s) h[s] = F2(0.f, 0.f);
   if (!kStateOnly) {
     if (a.init) load_states(a.init + q.row * N, N, p, h);
-    for (int i = 0; i < q.seg; ++i) {
-      F2 e[kH];
-      const int64_t at = ((int64_t)q.b * a.nseg + i) * a.channels + q.d;
-      load_states(a.seg_state + at * N, N, p, e);
-      const float sum = a.seg_sum[at];
-#pragma unroll
-      for (int s = 0; s < kH; ++s) {
-        h[s] = fma2(exp2_tile2(mul2(F2(sum, sum), A2[s])), h[s], e[s]);
-      }
-    }
+    enter_segment(a, q, A2, 0, h);
   }
   float total = 0.f;
   float *row_d = s_d + q.c * DP, *row_x = s_x + q.c * DP, *row_o = s_o + (kStateOnly ? 0 : q.c * DP);
@@ -832,16 +890,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
 #pragma unroll
   for (int s = 0; s < kH; ++s) r[s] = dA[s] = F2(0.f, 0.f);
   if (a.grad_final) load_states(a.grad_final + q.row * N, N, p, r);
-  for (int i = a.nseg - 1; i > q.seg; --i) {
-    F2 e[kH];
-    const int64_t at = ((int64_t)q.b * a.nseg + i) * a.channels + q.d;
-    load_states(a.seg_state + at * N, N, p, e);
-    const float sum = a.seg_sum[at];
-#pragma unroll
-    for (int s = 0; s < kH; ++s) {
-      r[s] = fma2(exp2_tile2(mul2(F2(sum, sum), A2[s])), r[s], e[s]);
-    }
-  }
+  enter_segment(a, q, A2, a.nseg - 1, r);
   const int t_begin = q.seg * a.seg_len, t_stop = min(L, t_begin + a.seg_len), t_end = min(t_stop, q.len);
   float *row_d = s_d + q.c * DP, *row_x = s_x + q.c * DP, *row_y = s_y + q.c * DP;
   float *row_sy = s_o + q.c * DP, *row_sb = row_sy + M::kRows, *row_sm = row_sb + M::kRows;

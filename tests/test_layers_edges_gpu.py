@@ -202,3 +202,70 @@ def test_conv_infinite_weights_reach_their_windows_only(n, K):
     same_or_both_not_finite(dx[..., :n], v["dx"], m["dx"], 64, "dx")
     same_or_both_not_finite(di, v["dinit"], m["dinit"], 64, "dinit")
 
+
+# ------------------------------------------- the scan's states, beyond bounds
+
+def test_scan_segments_keep_infinite_states_that_decay_fast():
+    """700 tokens of one row are cut into segments, over each of which these
+    states decay by more than 32 bits hold: an infinite one stays infinite."""
+    c, _, _, _ = scan_case(1, 1, 40, 700, 4, 1, torch.float32)
+    c["A"][:3, 2] = -100.0
+    t = {k: dev(a) for k, a in c.items()}
+    _, want = scan_call(t, True, None, return_final_state=True)
+    t["init"][0, :3, 2] = -math.inf
+    _, final = scan_call(t, True, None, return_final_state=True)
+    far = torch.zeros(40, 4, dtype=torch.bool)
+    far[:3, 2] = True
+    assert (final[0].cpu()[far] == -math.inf).all() and torch.equal(final[0].cpu()[~far], want[0].cpu()[~far])
+    # backwards: an infinite gradient of the final state reaches the first one
+    t["init"] = dev(c["init"]).requires_grad_()
+    gf = torch.zeros(1, 40, 4, device=DEV)
+    gf[0, :3, 2] = math.inf
+    _, final = scan_call(t, True, None, return_final_state=True)
+    di, = torch.autograd.grad(final, t["init"], gf)
+    assert (di[0].cpu()[far] == math.inf).all() and not di[0].cpu()[~far].any()
+
+
+def test_scan_segments_of_growing_states_that_are_zero_or_small():
+    """Growth over a segment that overflows 32 bits by itself, of states that
+    are still 0, or small enough to stay within them."""
+    c, go, _, _ = scan_case(2, 1, 40, 700, 4, 1, torch.float32, gate=False, carried=False)
+    c["delta"][:] = -2.3  # d = 0.095
+    c["bias"][:] = 0.0
+    c["A"][:] = 20.0
+    c["u"][..., :-5] = 0.0   # the states stay 0 up to the last tokens,
+    go[..., 5:] = 0.0        # their gradients from the first ones on
+    v, m = ref.scan(**{k: c[k] for k in ("u", "delta", "A", "B", "C", "D", "z", "bias")}, softplus=True,
+                    grad=torch.zeros_like(go), grad_final=None)
+    t = {k: dev(a) for k, a in c.items()}
+    units = 704 * (8 + 4 * float(v["weight"])) + 64
+    out, final = scan_call(t, True, None, return_final_state=True)
+    check(out, v["out"], m["out"], units, "out")
+    check(final, v["final"], m["final"], units, "final")
+    c["u"] = ref.rand(gen(3), 1, 40, 700)
+    c["u"][..., 5:] = 0.0
+    c["A"][:] = torch.where(torch.arange(40)[:, None] < 20, 20.0, -20.0)
+    t = {k: dev(a) for k, a in c.items()}
+    leaves = {k: t[k].requires_grad_() for k in ("u", "B")}
+    out = scan_call(t, True, None)
+    du, dB = torch.autograd.grad(out, list(leaves.values()), dev(go))
+    assert torch.isfinite(du).all() and not du[..., 5:].any()
+    assert torch.isfinite(dB).all()
+
+
+@pytest.mark.parametrize("A,init", [(8.0, 1e-30), (-8.0, 1e30)])
+def test_scan_segment_factor_out_of_range_beside_a_state_that_is_not(A, init):
+    """exp of 128 tokens' sum overflows (underflows); times the state that it
+    meets, it does not.  The rest of the row changes nothing (d = 0)."""
+    c, _, _, _ = scan_case(4, 1, 40, 300, 4, 1, torch.float32, gate=False)
+    c["bias"][:] = 0.0
+    c["delta"][..., :128] = -2.3
+    c["delta"][..., 128:] = -200.0
+    c["u"][:] = 0.0
+    c["A"][:], c["init"][:] = A, init
+    v, m = ref.scan(**{k: c[k] for k in ("u", "delta", "A", "B", "C", "D", "z", "bias")}, softplus=True, init=c["init"])
+    t = {k: dev(a) for k, a in c.items()}
+    _, final = scan_call(t, True, None, return_final_state=True)
+    # (the exponent, 102, is off by its d's 4 roundings and its sum's 128 at most: 132 * 102 of them)
+    check(final, v["final"], m["final"], 132 * 102 + 304 * 12, "final")
+
