@@ -38,6 +38,8 @@
 //
 // For the backward pass the forward one keeps the state at the start of each
 // of that pass's tiles; within a tile the states are computed again.
+#include <float.h>
+
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>
@@ -511,10 +513,16 @@ __device__ __forceinline__ void store_states(float *dst, int states, int p, cons
     }
   }
 }
-__device__ __forceinline__ void load_decay_rates(const ScanArgs &a, int d, int p, F2 (&A2)[kH]) {
-  load_states(a.A + (int64_t)d * a.states, a.states, p, A2);
+// A log2(e); the lowest (largest) number for an infinite one, so that a step of
+// d = 0, and the places of a tile that have no token, change nothing.
+__device__ __forceinline__ float decay_rate(float A) {
+  const float x = A * kLog2e;
+  return x < -FLT_MAX ? -FLT_MAX : x > FLT_MAX ? FLT_MAX : x;
+}
+__device__ __forceinline__ void load_decay_rates(const float *A, int states, int p, F2 (&A2)[kH]) {
+  load_states(A, states, p, A2);
 #pragma unroll
-  for (int s = 0; s < kH; ++s) A2[s] = mul2(A2[s], F2(kLog2e, kLog2e));
+  for (int s = 0; s < kH; ++s) A2[s] = F2(decay_rate(A2[s].x()), decay_rate(A2[s].y()));
 }
 
 // A segment's state after it: `own`, from zero, and the state h that entered it,
@@ -604,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_forward_kernel(S
   const float bias = a.bias ? a.bias[q.d] : 0.f, skip = a.skip ? a.skip[q.d] : 0.f;
   const int t_begin = q.seg * a.seg_len, t_stop = min(L, t_begin + a.seg_len), t_end = min(t_stop, q.len);
   F2 A2[kH], h[kH];
-  load_decay_rates(a, q.d, p, A2);
+  load_decay_rates(a.A + (int64_t)q.d * N, N, p, A2);
 #pragma unroll
   for (int s = 0; s < kH; ++s) h[s] = F2(0.f, 0.f);
   if (!kStateOnly) {
@@ -738,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_carry_kernel(Sca
   const bool z = a.z != nullptr;
   const float bias = a.bias ? a.bias[q.d] : 0.f;
   F2 A2[kH], r[kH];
-  load_decay_rates(a, q.d, p, A2);
+  load_decay_rates(a.A + (int64_t)q.d * N, N, p, A2);
 #pragma unroll
   for (int s = 0; s < kH; ++s) r[s] = F2(0.f, 0.f);
   const int t_begin = q.seg * a.seg_len, t_end = min(min(L, t_begin + a.seg_len), q.len);
@@ -886,7 +894,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
   const float bias = a.bias ? a.bias[q.d] : 0.f, skip = a.skip ? a.skip[q.d] : 0.f;
   float dskip = 0.f, dbias = 0.f;
   F2 A2[kH], r[kH], dA[kH];
-  load_decay_rates(a, q.d, p, A2);
+  load_decay_rates(a.A + (int64_t)q.d * N, N, p, A2);
 #pragma unroll
   for (int s = 0; s < kH; ++s) r[s] = dA[s] = F2(0.f, 0.f);
   if (a.grad_final) load_states(a.grad_final + q.row * N, N, p, r);
@@ -1241,15 +1249,19 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(ScanStepArgs a)
     if (a.z) z = to_f(static_cast<const T *>(a.z)[i]);
     if (a.softplus) delta = softplus_f(delta);
     const F2 d2(delta * kLog2e, delta * kLog2e), x2(delta * u, delta * u);
+    if (delta != 0.f) {  // (a step of 0 changes nothing, also where A is infinite)
+#pragma unroll
+      for (int k = 0; k < Q; ++k)
+#pragma unroll
+        for (int s = 0; s < kH; ++s)
+          h[k][s] = fma2(exp2_tile2(mul2(d2, A2[k][s])), h[k][s],
+                         mul2(x2, F2(vb[k].f(2 * s), vb[k].f(2 * s + 1))));
+    }
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
       F2 c2[kH];
 #pragma unroll
-      for (int s = 0; s < kH; ++s) {
-        h[k][s] = fma2(exp2_tile2(mul2(d2, A2[k][s])), h[k][s],
-                       mul2(x2, F2(vb[k].f(2 * s), vb[k].f(2 * s + 1))));
-        c2[s] = F2(vc[k].f(2 * s), vc[k].f(2 * s + 1));
-      }
+      for (int s = 0; s < kH; ++s) c2[s] = F2(vc[k].f(2 * s), vc[k].f(2 * s + 1));
       y += dot(h[k], c2);
     }
   }

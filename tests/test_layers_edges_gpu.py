@@ -269,3 +269,36 @@ def test_scan_segment_factor_out_of_range_beside_a_state_that_is_not(A, init):
     # (the exponent, 102, is off by its d's 4 roundings and its sum's 128 at most: 132 * 102 of them)
     check(final, v["final"], m["final"], 132 * 102 + 304 * 12, "final")
 
+
+@pytest.mark.parametrize("L,lengths", [(5, None), (37, None), (64, None), (45, [45, 7, 0]), (700, None)])
+@pytest.mark.parametrize("N", [3, 16])
+def test_scan_infinite_decay_rates(L, lengths, N):
+    """A = -inf forgets at every token, and only at tokens: what a lowest
+    finite rate gives, bit for bit, gradients too."""
+    nb = 1 if lengths is None else len(lengths)
+    c, go, gf, lens = scan_case(L + N, nb, 10, L, N, 1, torch.float32, lengths=lengths)
+    results = []
+    for low in (-math.inf, -1e38):
+        t = {k: dev(a) for k, a in c.items()}
+        t["A"][::2, 1] = low
+        leaves = [t[k].requires_grad_() for k in t]
+        out, final = scan_call(t, True, dev(lens), return_final_state=True)
+        results.append([out, final, *torch.autograd.grad([out, final], leaves, [dev(go), dev(gf)])])
+    for a, b in zip(*results):
+        assert torch.isfinite(b).all() and torch.equal(a, b)
+
+
+def test_scan_step_infinite_decay_rates():
+    c, _, _, _ = scan_case(2, 2, 10, 1, 16, 1, torch.float32)
+    c["delta"][0] = -200.0  # d = 0: nothing is forgotten
+    results = []
+    for low in (-math.inf, -1e38):
+        t = {k: dev(a[..., 0].contiguous() if k in ("u", "delta", "z", "B", "C") else a) for k, a in c.items()}
+        t["A"][:, 1] = low
+        state = t["init"].clone()
+        out = pc.ssm_scan_step(t["u"], t["delta"], state, t["A"], t["B"], t["C"], D=t["D"], z=t["z"],
+                               delta_bias=t["bias"], delta_softplus=True)
+        results.append((out, state))
+    assert torch.isfinite(results[0][1]).all()
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+
