@@ -54,6 +54,7 @@ constexpr int kS = 4, kH = kS / 2;  // states per lane, and pairs of them (packe
 constexpr int kRun = 8;             // tokens of an inner run
 constexpr int kThreads = 128;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInf = __builtin_huge_valf();
 
 // How a block is laid out: P lanes per channel, and the tiles' lengths.  A
 // forward tile holds whole backward ones.  kMany: for grids that fill the GPU
@@ -174,7 +175,7 @@ __device__ __forceinline__ F2 exp2_tile2(F2 x) {
 // h corrected for the tile: x = A2 sum d, prod = the decays' product.  Not for a
 // growing state, whose product may have overflowed, nor for an infinite one.
 __device__ __forceinline__ float correct_tile(float h, float entry, float x, float prod) {
-  const bool apply = x <= 0.f && fabsf(entry) < __int_as_float(0x7f800000);
+  const bool apply = x <= 0.f && fabsf(entry) < kInf;
   return apply ? fmaf(entry, exp2_tile(x) - prod, h) : h;
 }
 __device__ __forceinline__ F2 correct_tile2(F2 h, F2 entry, F2 x, F2 prod) {
@@ -531,7 +532,7 @@ __device__ __forceinline__ void load_decay_rates(const float *A, int states, int
 // it would token by token), whatever the decay.
 __device__ __forceinline__ float join_segment(float x, float h, float own) {
   if (h == 0.f) return own;
-  if (fabsf(h) == __int_as_float(0x7f800000)) return h + own;
+  if (fabsf(h) == kInf) return h + own;
   if (fabsf(x) <= 126.f) return fmaf(exp2_tile(x), h, own);
   const float half = exp2_f(0.5f * x);
   return fmaf(half, half * h, own);
@@ -567,7 +568,7 @@ __device__ __noinline__ LaneStates join_segments(const float *state, const float
   // An infinity or NaN may come of a decay alone (and stays).  A decay that
   // underflows loses less than 2^-86 of what is at most 2^40.
   const float sum_of = fabsf(h[0].x()) + fabsf(h[0].y()) + fabsf(h[1].x()) + fabsf(h[1].y());
-  if (!(sum_of < __int_as_float(0x7f800000)) || largest > 0x1p40f) {
+  if (!(sum_of < kInf) || largest > 0x1p40f) {
     h[0] = in.h[0];
     h[1] = in.h[1];
 #pragma unroll 1
@@ -869,8 +870,117 @@ struct SumChannels {
   __device__ static __forceinline__ bool writes(int lane) { return lane < (P << kLevels); }
 };
 
+// The gradients behind the last token, in its tile: 0.
 template <typename T, class G>
-__global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(ScanArgs a) {
+__device__ __noinline__ void clear_rest(const ScanArgs &a) {
+  constexpr int TT = G::TB;
+  const ScanPlace<G> q(a);
+  const int t_begin = q.seg * a.seg_len, t_stop = min(a.length, t_begin + a.seg_len);
+  const int to = min(t_stop, t_begin + (q.len - t_begin + TT - 1) / TT * TT), N = a.states, L = a.length;
+  if (q.valid) {
+    for (int t = q.len + q.p; t < to; t += G::P) {
+      const int64_t at = q.row * L + t;
+      static_cast<T *>(a.du)[at] = static_cast<T *>(a.ddelta)[at] = from_f<T>(0.f);
+      if (a.z) static_cast<T *>(a.dz)[at] = from_f<T>(0.f);
+    }
+  }
+  float *part = a.part_bc + (((int64_t)q.b * a.groups + q.g) * a.nblk + q.blk) * 2 * N * L;
+  for (int n = threadIdx.x; n < 2 * N; n += kThreads)
+    for (int t = q.len; t < to; ++t) part[(int64_t)n * L + t] = 0.f;
+}
+
+// A warp's shares of dA and dbias (with the channel's first lane) once more, a
+// token at a time, for rows where the products of the last tile's places
+// without a token were NaN.  (Conditions in the loops cost the backward pass of
+// 4 x 2048 x 2048 bf16 up to a tenth.)
+struct RateShares {
+  F2 dA[kH];
+  float dbias;
+};
+template <typename T, class G>
+__device__ __noinline__ RateShares rate_shares(const ScanArgs &a) {
+  constexpr int P = G::P, TT = G::TB;
+  const ScanPlace<G> q(a);
+  const int N = a.states, L = a.length, t_begin = q.seg * a.seg_len, t_end = min(min(L, t_begin + a.seg_len), q.len);
+  const int64_t row = q.row * L, bg = ((int64_t)q.b * a.groups + q.g) * N * L;
+  const float bias = a.bias ? a.bias[q.d] : 0.f;
+  F2 A2[kH], r[kH] = {F2(0.f, 0.f), F2(0.f, 0.f)};
+  load_decay_rates(a.A + (int64_t)q.d * N, N, q.p, A2);
+  if (a.grad_final) load_states(a.grad_final + q.row * N, N, q.p, r);
+  enter_segment(a, q, A2, a.nseg - 1, r);
+  RateShares sums{{F2(0.f, 0.f), F2(0.f, 0.f)}, 0.f};
+  auto at = [&](const void *array, int64_t i) { return to_f(static_cast<const T *>(array)[i]); };
+  auto states_of = [&](const void *array, int t, F2 (&v)[kH]) {
+    float f[kS];
+#pragma unroll
+    for (int s = 0; s < kS; ++s) f[s] = q.p * kS + s < N ? at(array, bg + (int64_t)(q.p * kS + s) * L + t) : 0.f;
+    v[0] = F2(f[0], f[1]);
+    v[1] = F2(f[2], f[3]);
+  };
+  auto step = [&](int t, float *slope) {
+    const float d = at(a.delta, row + t) + bias;
+    *slope = 1.f;
+    return a.softplus ? softplus_f(d, slope) : d;
+  };
+#pragma unroll 1
+  for (int t0 = t_begin + (t_end - t_begin - 1) / TT * TT; t0 >= t_begin; t0 -= TT) {
+    const int n = min(TT, t_end - t0);
+    F2 before[TT][kH], b[kH], c[kH], h[kH];
+    float slope;
+    load_states(a.ckpt + (((int64_t)q.b * ((L + TT - 1) / TT) + t0 / TT) * a.channels + q.d) * N, N, q.p, h);
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const float d = step(t0 + j, &slope), x = d * at(a.u, row + t0 + j);
+      states_of(a.B, t0 + j, b);
+#pragma unroll
+      for (int s = 0; s < kH; ++s) {
+        before[j][s] = h[s];
+        h[s] = fma2(exp2_2(mul2(F2(d, d), A2[s])), h[s], mul2(F2(x, x), b[s]));
+      }
+    }
+    F2 tile_dA[kH] = {F2(0.f, 0.f), F2(0.f, 0.f)}, prod[kH] = {F2(1.f, 1.f), F2(1.f, 1.f)}, dh[kH], m[kH];
+    const F2 entry[kH] = {r[0], r[1]};
+    float sum = 0.f;
+#pragma unroll 1
+    for (int j = n - 1; j >= 0; --j) {
+      const float d = step(t0 + j, &slope);
+      float dy = at(a.grad, row + t0 + j);
+      if (a.z) {
+        const float z = at(a.z, row + t0 + j);
+        dy *= z * sigmoid_f(z);
+      }
+      states_of(a.B, t0 + j, b);
+      states_of(a.C, t0 + j, c);
+      sum += d;
+#pragma unroll
+      for (int s = 0; s < kH; ++s) {
+        const F2 dec = exp2_2(mul2(F2(d, d), A2[s]));
+        dh[s] = fma2(F2(dy, dy), c[s], r[s]);
+        r[s] = mul2(dec, dh[s]);
+        m[s] = mul2(r[s], before[j][s]);
+        prod[s] = mul2(prod[s], dec);
+        tile_dA[s] = fma2(m[s], F2(d, d), tile_dA[s]);
+      }
+      float through = dot(dh, b), moved = dot(m, A2);
+#pragma unroll
+      for (int o = 1; o < P; o <<= 1) {
+        through += __shfl_xor_sync(0xffffffffu, through, o);
+        moved += __shfl_xor_sync(0xffffffffu, moved, o);
+      }
+      if (q.p == 0) sums.dbias += fmaf(at(a.u, row + t0 + j), through, moved * (1.f / kLog2e)) * slope;
+    }
+#pragma unroll
+    for (int s = 0; s < kH; ++s) {
+      sums.dA[s] = add2(sums.dA[s], tile_dA[s]);
+      r[s] = correct_tile2(r[s], entry[s], mul2(F2(sum, sum), A2[s]), prod[s]);
+    }
+  }
+  return sums;
+}
+
+template <typename T, class G>
+__global__ void __launch_bounds__(kThreads, kBwdBlocks)
+    scan_backward_kernel(const __grid_constant__ ScanArgs a) {
   using M = BwdSmem<T, G>;
   constexpr int P = G::P, NP = G::NP;
   constexpr int TT = M::TT, E = TT >= P ? TT / P : 1, DP = M::DP;
@@ -894,11 +1004,14 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
   const float bias = a.bias ? a.bias[q.d] : 0.f, skip = a.skip ? a.skip[q.d] : 0.f;
   float dskip = 0.f, dbias = 0.f;
   F2 A2[kH], r[kH], dA[kH];
-  load_decay_rates(a.A + (int64_t)q.d * N, N, p, A2);
+  // a thread without a channel has states of 0 that stay 0: nothing of the
+  // channel whose inputs it reads reaches the sums over channels
+  const int own = q.valid ? N : 0;
+  load_decay_rates(a.A + (int64_t)q.d * N, own, p, A2);
 #pragma unroll
   for (int s = 0; s < kH; ++s) r[s] = dA[s] = F2(0.f, 0.f);
-  if (a.grad_final) load_states(a.grad_final + q.row * N, N, p, r);
-  enter_segment(a, q, A2, a.nseg - 1, r);
+  if (a.grad_final) load_states(a.grad_final + q.row * N, own, p, r);
+  if (q.valid) enter_segment(a, q, A2, a.nseg - 1, r);
   const int t_begin = q.seg * a.seg_len, t_stop = min(L, t_begin + a.seg_len), t_end = min(t_stop, q.len);
   float *row_d = s_d + q.c * DP, *row_x = s_x + q.c * DP, *row_y = s_y + q.c * DP;
   float *row_sy = s_o + q.c * DP, *row_sb = row_sy + M::kRows, *row_sm = row_sb + M::kRows;
@@ -908,7 +1021,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
   F2 nh[kH];
   BC nbc;
   auto fetch = [&](int t0) {
-    load_states(a.ckpt + (((int64_t)q.b * ((L + TT - 1) / TT) + t0 / TT) * a.channels + q.d) * N, N, p, nh);
+    load_states(a.ckpt + (((int64_t)q.b * ((L + TT - 1) / TT) + t0 / TT) * a.channels + q.d) * N, own, p, nh);
     if (loads) {
       nu.load(u, row, t0 + p * E, t_end);
       nd.load(dl, row, t0 + p * E, t_end);
@@ -1100,6 +1213,18 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) scan_backward_kernel(Sca
         if (first + s < N && t0 + t < t_stop) dst[(int64_t)s * L] = f[s];
     }
     // (the next tile's first barrier comes before anything overwrites s_part)
+  }
+  if (t_begin < t_end && (t_end - t_begin) % TT != 0) {
+    // The last tile went over places without a token.  D, dy and the inputs are
+    // 0 there, but the state, r or skip may be infinite: then the products NaN.
+    const float size = fabsf(dA[0].x()) + fabsf(dA[0].y()) + fabsf(dA[1].x()) + fabsf(dA[1].y()) + fabsf(dbias);
+    if (__syncthreads_or(!(size < kInf && fabsf(skip) < kInf))) {
+      const RateShares again = rate_shares<T, G>(a);
+      dA[0] = again.dA[0];
+      dA[1] = again.dA[1];
+      dbias = again.dbias;
+      clear_rest<T, G>(a);
+    }
   }
 #pragma unroll
   for (int o = 1; o < P; o <<= 1) {

@@ -302,3 +302,53 @@ def test_scan_step_infinite_decay_rates():
     assert torch.isfinite(results[0][1]).all()
     assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
 
+
+@pytest.mark.parametrize("L,n", [(13, 13), (40, 13), (32, 32), (700, 655)])
+@pytest.mark.parametrize("N,channel", [(4, 0), (16, 0), (16, 9)])
+def test_scan_state_that_overflows_at_the_last_token(L, n, N, channel):
+    """The last token makes a state infinite: its own output and dC are so,
+    and nothing else; not the gradients behind it, nor the sums that pass
+    over the rest of its tile, nor those over lanes without a channel."""
+    c, go, _, _ = scan_case(L + N, 1, 10, n, N, 1, torch.float32, gate=False)
+    c["u"][0, channel, -1] = 1e38
+    c["B"][0, 0, 2, -1] = 1e5
+    go[0, :, -1] *= 1e-12
+    v, m = ref.scan(**{k: c[k] for k in ("u", "delta", "A", "B", "C", "D", "z", "bias")}, softplus=True,
+                    init=c["init"], grad=go)
+    t = {k: dev(a) for k, a in c.items()}
+    pgo = torch.full((1, 10, L), math.nan, device=DEV)
+    pgo[..., :n] = dev(go)
+    for k in ("u", "delta", "B", "C"):
+        t[k] = torch.nn.functional.pad(t[k], (0, L - n), value=math.nan)
+    leaves = {k: a.requires_grad_() for k, a in t.items() if a is not None}
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    out, final = scan_call(t, True, lens, return_final_state=True)
+    assert torch.isinf(final[0, channel, 2]) and torch.isfinite(final).sum() == 10 * N - 1
+    assert not torch.isfinite(out[0, channel, n - 1]) and torch.isfinite(out).sum() == 10 * L - 1
+    grads = dict(zip(leaves, torch.autograd.grad(out, list(leaves.values()), pgo)))
+    units = 2 * ((n + 4) * (8 + 4 * float(v["weight"])) + 64)
+    assert torch.isinf(grads["C"][0, 0, 2, n - 1])
+    grads["C"][0, 0, 2, n - 1] = 0.0
+    v["dC"][0, 0, 2, n - 1] = 0.0
+    for k, gr in grads.items():
+        if k in ("u", "delta", "B", "C"):
+            assert not gr[..., n:].any(), k
+            gr = gr[..., :n]
+        check(gr, v[SCAN_GRADS[k]], m[SCAN_GRADS[k]], units, SCAN_GRADS[k])
+
+
+@pytest.mark.parametrize("L,n", [(40, 13), (700, 655), (64, 33)])
+@pytest.mark.parametrize("N", [4, 16, 40])
+def test_scan_infinite_skip_and_final_gradient_leave_padding_at_0(L, n, N):
+    c, go, gf, lens = scan_case(L + N, 1, 10, L, N, 1, torch.float32, lengths=[n])
+    c["D"][0], gf[0, 1, 0] = math.inf, -math.inf
+    t = {k: dev(a).requires_grad_() for k, a in c.items()}
+    out, final = scan_call(t, True, dev(lens), return_final_state=True)
+    grads = dict(zip(t, torch.autograd.grad([out, final], list(t.values()), [dev(go), dev(gf)])))
+    for k in ("u", "delta", "z", "B", "C"):
+        assert not grads[k][..., n:].any(), k
+    for k in ("u", "delta", "z"):
+        assert torch.isfinite(grads[k][0, 2:]).all(), k
+    assert torch.isfinite(grads["A"][2:]).all() and torch.isfinite(grads["bias"][2:]).all()
+    assert torch.isinf(grads["u"][0, 0, :n]).all() and torch.isinf(grads["init"][0, 1, 0])
+
