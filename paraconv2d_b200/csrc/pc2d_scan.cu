@@ -173,10 +173,10 @@ __device__ __forceinline__ F2 exp2_tile2(F2 x) {
   return F2(fabsf(x.x()) < 0.125f ? q.x() : exp2_f(x.x()), fabsf(x.y()) < 0.125f ? q.y() : exp2_f(x.y()));
 }
 // h corrected for the tile: x = A2 sum d, prod = the decays' product.  Not for a
-// growing state, whose product may have overflowed, nor for an infinite one.
+// growing state, nor an infinite one, nor where the product overflowed.
 __device__ __forceinline__ float correct_tile(float h, float entry, float x, float prod) {
-  const bool apply = x <= 0.f && fabsf(entry) < kInf;
-  return apply ? fmaf(entry, exp2_tile(x) - prod, h) : h;
+  const float by = entry * (exp2_tile(x) - prod);
+  return x <= 0.f && fabsf(by) < kInf ? h + by : h;
 }
 __device__ __forceinline__ F2 correct_tile2(F2 h, F2 entry, F2 x, F2 prod) {
   return F2(correct_tile(h.x(), entry.x(), x.x(), prod.x()), correct_tile(h.y(), entry.y(), x.y(), prod.y()));

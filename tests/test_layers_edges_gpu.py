@@ -352,3 +352,21 @@ def test_scan_infinite_skip_and_final_gradient_leave_padding_at_0(L, n, N):
     assert torch.isfinite(grads["A"][2:]).all() and torch.isfinite(grads["bias"][2:]).all()
     assert torch.isinf(grads["u"][0, 0, :n]).all() and torch.isinf(grads["init"][0, 1, 0])
 
+
+def test_scan_states_that_grow_and_decay_within_a_tile():
+    """Growth over a few tokens whose product overflows 32 bits, taken back
+    within the same 16 tokens: zero states stay 0 and small ones come back."""
+    c, go, _, _ = scan_case(6, 1, 8, 20, 4, 1, torch.float32, gate=False, bias=False)
+    c["A"][:] = -1.0
+    c["delta"][:] = 0.1
+    c["delta"][..., 0:2], c["delta"][..., 2:4] = -70.0, 75.0
+    c["u"][..., :4] = 0.0
+    c["init"][:, ::2], c["init"][:, 1::2] = 0.0, 1e-30
+    v, m = ref.scan(**{k: c[k] for k in ("u", "delta", "A", "B", "C", "D", "z", "bias")}, init=c["init"])
+    t = {k: dev(a) for k, a in c.items()}
+    out, final = scan_call(t, False, None, return_final_state=True)
+    # (decays of exponents up to 75: each off by 75 roundings more than the general bound has)
+    units = 24 * (8 + 4 * float(v["weight"]) + 75) + 64
+    check(out, v["out"], m["out"], units, "out")
+    check(final, v["final"], m["final"], units, "final")
+
