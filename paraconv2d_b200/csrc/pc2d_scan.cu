@@ -832,7 +832,8 @@ struct BwdSmem {
   static constexpr int kRows = G::CB * DP;
   static constexpr int kStart = TT / kRun * kThreads * kS;     // states at the start of each run
   static constexpr int kBC = (TileBC<T, G, TT>::kFloats + 3) / 4 * 4;
-  static constexpr int kFloats = 8 * kRows + kStart + kBC + (kThreads / 32) * TT * kPart;
+  static constexpr int kSums = 8 * kRows + kStart + kBC + (kThreads / 32) * TT * kPart;  // dskip, dbias of each thread
+  static constexpr int kFloats = kSums + 4 * kThreads;
 };
 
 // Sums of v[0..7] over the lanes of a warp that hold the same states of
@@ -895,7 +896,7 @@ __device__ __noinline__ void clear_rest(const ScanArgs &a) {
 // 4 x 2048 x 2048 bf16 up to a tenth.)
 struct RateShares {
   F2 dA[kH];
-  float dbias;
+  double dbias;
 };
 template <typename T, class G>
 __device__ __noinline__ RateShares rate_shares(const ScanArgs &a) {
@@ -908,7 +909,7 @@ __device__ __noinline__ RateShares rate_shares(const ScanArgs &a) {
   load_decay_rates(a.A + (int64_t)q.d * N, N, q.p, A2);
   if (a.grad_final) load_states(a.grad_final + q.row * N, N, q.p, r);
   enter_segment(a, q, A2, a.nseg - 1, r);
-  RateShares sums{{F2(0.f, 0.f), F2(0.f, 0.f)}, 0.f};
+  RateShares sums{{F2(0.f, 0.f), F2(0.f, 0.f)}, 0.0};
   auto at = [&](const void *array, int64_t i) { return to_f(static_cast<const T *>(array)[i]); };
   auto states_of = [&](const void *array, int t, F2 (&v)[kH]) {
     float f[kS];
@@ -1002,7 +1003,10 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks)
   float *part = a.part_bc + (((int64_t)q.b * a.groups + q.g) * a.nblk + q.blk) * 2 * N * L;
   const bool loads = p * E < TT;  // (more lanes than tokens of a tile)
   const float bias = a.bias ? a.bias[q.d] : 0.f, skip = a.skip ? a.skip[q.d] : 0.f;
-  float dskip = 0.f, dbias = 0.f;
+  // dskip and dbias: a tile's sum in 32 bits, the row's in 64 (kept where it
+  // takes no registers from the loops)
+  double2 *sums = reinterpret_cast<double2 *>(smem + M::kSums) + threadIdx.x;
+  *sums = make_double2(0.0, 0.0);
   F2 A2[kH], r[kH], dA[kH];
   // a thread without a channel has states of 0 that stay 0: nothing of the
   // channel whose inputs it reads reaches the sums over channels
@@ -1176,6 +1180,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks)
     __syncwarp();
     if (q.valid && loads) {
       Pack<T, E> ou, od, oz;
+      float tile_skip = 0.f, tile_bias = 0.f;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         // (behind the last token D, the slopes and dy are 0)
@@ -1184,9 +1189,10 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks)
         ou.v[i] = from_f<T>(fmaf(row_d[p * E + i], through, skip * dy));
         od.v[i] = from_f<T>(dd);
         if (z) oz.v[i] = from_f<T>(row_gs[p * E + i] * fmaf(skip, uu, row_sy[p * E + i]));
-        dskip = fmaf(dy, uu, dskip);
-        dbias += dd;
+        tile_skip = fmaf(dy, uu, tile_skip);
+        tile_bias += dd;
       }
+      *sums = make_double2(sums->x + tile_skip, sums->y + tile_bias);
       store_row<G::kWhole>(ou, du, row, t0 + p * E, t_stop);
       store_row<G::kWhole>(od, ddl, row, t0 + p * E, t_stop);
       if (z) store_row<G::kWhole>(oz, dz, row, t0 + p * E, t_stop);
@@ -1214,6 +1220,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks)
     }
     // (the next tile's first barrier comes before anything overwrites s_part)
   }
+  float dskip = (float)sums->x, dbias = (float)sums->y;
   if (t_begin < t_end && (t_end - t_begin) % TT != 0) {
     // The last tile went over places without a token.  D, dy and the inputs are
     // 0 there, but the state, r or skip may be infinite: then the products NaN.
@@ -1222,7 +1229,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks)
       const RateShares again = rate_shares<T, G>(a);
       dA[0] = again.dA[0];
       dA[1] = again.dA[1];
-      dbias = again.dbias;
+      dbias = (float)again.dbias;
       clear_rest<T, G>(a);
     }
   }

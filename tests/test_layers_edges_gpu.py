@@ -370,3 +370,26 @@ def test_scan_states_that_grow_and_decay_within_a_tile():
     check(out, v["out"], m["out"], units, "out")
     check(final, v["final"], m["final"], units, "final")
 
+
+@pytest.mark.parametrize("N", [1, 16])
+def test_scan_long_sums_of_parameter_gradients(N):
+    """dD of rows that are not cut (256 groups of a channel each): 65536 terms
+    of one sign, the same in 32 bits here and in 64 there.  A lane adds at most
+    16 terms of a tile in 32 bits, the tiles in 64, and at most 4 lanes are
+    joined: 16 + 2 + 2 roundings of the sum.  One running sum in 32 bits would
+    be off by about 256, as its roundings add up like a random walk."""
+    ch, L = 256, 65536
+    g = torch.Generator(device=DEV).manual_seed(1)
+    u = torch.rand(1, ch, L, generator=g, device=DEV) + 0.5
+    go = torch.rand(1, ch, L, generator=g, device=DEV) + 0.5
+    D = torch.ones(ch, device=DEV, requires_grad=True)
+    B = torch.zeros(1, ch, N, L, device=DEV)
+    delta = torch.ones(1, ch, L, device=DEV)
+    bias = torch.zeros(ch, device=DEV, requires_grad=True)
+    out = pc.ssm_scan(u, delta, -torch.ones(ch, N, device=DEV), B, B + 1.0, D=D, delta_bias=bias,
+                      initial_state=torch.zeros(1, ch, N, device=DEV))
+    dD, db = torch.autograd.grad(out, [D, bias], go)
+    exact = (go.double() * u.double()).sum((0, 2)).cpu()
+    check(dD, exact, exact.abs(), 20, "dD")
+    assert not db.any()  # (B and the states are 0)
+
