@@ -150,13 +150,16 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 // average over its table, low by 0.1 to 0.8 of one (measured on [-2, 0]).  A
 // state that decays slowly would add that bias up over all the tokens it
 // remembers, a thousand or more.  So each tile of up to 32 tokens ends with a
-// correction: the product of the decays that were used is replaced by exp of
-// the tile's sum, for the state that entered the tile,
-//   h += h_entry (exp2(A2 sum d) - prod decays),
-// and the bias no longer grows beyond a tile.  exp2_tile, for that one value a
-// tile, takes 1 + x q(x) for |x| < 1/8 with the interpolation of (2^x - 1)/x at
-// the four Chebyshev nodes of [-1/8, 1/8] as q (no bias where many tiles are
-// remembered), else the hardware's.
+// correction: what is left of the state that entered the tile, by the decays
+// that were used, is replaced by exp of the tile's sum,
+//   h += h_entry exp2(A2 sum d) - left,       left = h_entry a_1 a_2 ...
+// and the bias no longer grows beyond a tile.  (The decays' product by itself,
+// from 1 on, would not do: of (1 - a)(1 - b) the small a b is rounded off, always
+// to the same side; a state's own digits round to both.  With the product,
+// states that remember 20000 tokens were off by 1600 units.)  exp2_tile, for
+// that one value a tile, takes 1 + x q(x) for |x| < 1/8 with the interpolation
+// of (2^x - 1)/x at the four Chebyshev nodes of [-1/8, 1/8] as q (no bias where
+// many tiles are remembered), else the hardware's.
 __device__ __forceinline__ F2 exp2_2(F2 x) { return F2(exp2_f(x.x()), exp2_f(x.y())); }
 __device__ __forceinline__ float exp2_tile(float x) {
   float q = fmaf(0.009620536f, x, 0.055524945f);
@@ -172,14 +175,14 @@ __device__ __forceinline__ F2 exp2_tile2(F2 x) {
   q = fma2(q, x, F2(1.f, 1.f));
   return F2(fabsf(x.x()) < 0.125f ? q.x() : exp2_f(x.x()), fabsf(x.y()) < 0.125f ? q.y() : exp2_f(x.y()));
 }
-// h corrected for the tile: x = A2 sum d, prod = the decays' product.  Not for a
-// growing state, nor an infinite one, nor where the product overflowed.
-__device__ __forceinline__ float correct_tile(float h, float entry, float x, float prod) {
-  const float by = entry * (exp2_tile(x) - prod);
+// h corrected for the tile: x = A2 sum d.  Not for a growing state, nor an
+// infinite one, nor where the decays overflowed.
+__device__ __forceinline__ float correct_tile(float h, float entry, float x, float left) {
+  const float by = fmaf(entry, exp2_tile(x), -left);
   return x <= 0.f && fabsf(by) < kInf ? h + by : h;
 }
-__device__ __forceinline__ F2 correct_tile2(F2 h, F2 entry, F2 x, F2 prod) {
-  return F2(correct_tile(h.x(), entry.x(), x.x(), prod.x()), correct_tile(h.y(), entry.y(), x.y(), prod.y()));
+__device__ __forceinline__ F2 correct_tile2(F2 h, F2 entry, F2 x, F2 left) {
+  return F2(correct_tile(h.x(), entry.x(), x.x(), left.x()), correct_tile(h.y(), entry.y(), x.y(), left.y()));
 }
 
 // Two pairs from, and to, 16 aligned bytes.
@@ -660,12 +663,11 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_forward_kernel(S
     for (int tb = 0; tb < TT; tb += TB) {
       if (!kStateOnly && a.ckpt && t0 + tb < t_end && q.valid)
         store_states(a.ckpt + (((int64_t)q.b * ((L + TB - 1) / TB) + (t0 + tb) / TB) * a.channels + q.d) * N, N, p, h);
-      F2 entry[kH], prod[kH];
+      F2 entry[kH], left[kH];
       float sum = 0.f;
 #pragma unroll
       for (int s = 0; s < kH; ++s) {
-        entry[s] = h[s];
-        prod[s] = F2(1.f, 1.f);
+        entry[s] = left[s] = h[s];
       }
 #pragma unroll 1
       for (int t = tb; t < tb + TB; t += kRun) {
@@ -685,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_forward_kernel(S
 #pragma unroll
           for (int s = 0; s < kH; ++s) {
             const F2 dec = exp2_2(mul2(d2, A2[s]));
-            prod[s] = mul2(prod[s], dec);
+            left[s] = mul2(left[s], dec);
             h[s] = fma2(dec, h[s], mul2(x2, b[s]));
           }
           if (!kStateOnly) {
@@ -700,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_forward_kernel(S
         }
       }
 #pragma unroll
-      for (int s = 0; s < kH; ++s) h[s] = correct_tile2(h[s], entry[s], mul2(F2(sum, sum), A2[s]), prod[s]);
+      for (int s = 0; s < kH; ++s) h[s] = correct_tile2(h[s], entry[s], mul2(F2(sum, sum), A2[s]), left[s]);
       total += sum;
     }
     if (!kStateOnly) {
@@ -785,12 +787,11 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_carry_kernel(Sca
     nc.put(s_c, C, nullptr, bg, N, L, t0, t_end);
     __syncthreads();
     if (t0 > t_begin) fetch(t0 - TT);
-    F2 entry[kH], prod[kH];
+    F2 entry[kH], left[kH];
     float sum = 0.f;
 #pragma unroll
     for (int s = 0; s < kH; ++s) {
-      entry[s] = r[s];
-      prod[s] = F2(1.f, 1.f);
+      entry[s] = left[s] = r[s];
     }
 #pragma unroll 1
     for (int t = TT - kRun; t >= 0; t -= kRun) {
@@ -806,13 +807,13 @@ __global__ void __launch_bounds__(kThreads, G::kFwdBlocks) scan_carry_kernel(Sca
 #pragma unroll
         for (int s = 0; s < kH; ++s) {
           const F2 dec = exp2_2(mul2(d2, A2[s]));
-          prod[s] = mul2(prod[s], dec);
+          left[s] = mul2(left[s], dec);
           r[s] = mul2(dec, fma2(c[s], y2, r[s]));
         }
       }
     }
 #pragma unroll
-    for (int s = 0; s < kH; ++s) r[s] = correct_tile2(r[s], entry[s], mul2(F2(sum, sum), A2[s]), prod[s]);
+    for (int s = 0; s < kH; ++s) r[s] = correct_tile2(r[s], entry[s], mul2(F2(sum, sum), A2[s]), left[s]);
     total += sum;
     __syncthreads();
   }
@@ -939,7 +940,7 @@ __device__ __noinline__ RateShares rate_shares(const ScanArgs &a) {
         h[s] = fma2(exp2_2(mul2(F2(d, d), A2[s])), h[s], mul2(F2(x, x), b[s]));
       }
     }
-    F2 tile_dA[kH] = {F2(0.f, 0.f), F2(0.f, 0.f)}, prod[kH] = {F2(1.f, 1.f), F2(1.f, 1.f)}, dh[kH], m[kH];
+    F2 tile_dA[kH] = {F2(0.f, 0.f), F2(0.f, 0.f)}, left[kH] = {r[0], r[1]}, dh[kH], m[kH];
     const F2 entry[kH] = {r[0], r[1]};
     float sum = 0.f;
 #pragma unroll 1
@@ -959,7 +960,7 @@ __device__ __noinline__ RateShares rate_shares(const ScanArgs &a) {
         dh[s] = fma2(F2(dy, dy), c[s], r[s]);
         r[s] = mul2(dec, dh[s]);
         m[s] = mul2(r[s], before[j][s]);
-        prod[s] = mul2(prod[s], dec);
+        left[s] = mul2(left[s], dec);
         tile_dA[s] = fma2(m[s], F2(d, d), tile_dA[s]);
       }
       float through = dot(dh, b), moved = dot(m, A2);
@@ -973,7 +974,7 @@ __device__ __noinline__ RateShares rate_shares(const ScanArgs &a) {
 #pragma unroll
     for (int s = 0; s < kH; ++s) {
       sums.dA[s] = add2(sums.dA[s], tile_dA[s]);
-      r[s] = correct_tile2(r[s], entry[s], mul2(F2(sum, sum), A2[s]), prod[s]);
+      r[s] = correct_tile2(r[s], entry[s], mul2(F2(sum, sum), A2[s]), left[s]);
     }
   }
   return sums;
@@ -1099,13 +1100,12 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks)
       }
       put_pairs(start + k * kThreads * kS, h0);
     }
-    F2 tile_dA[kH], entry[kH], prod[kH];
+    F2 tile_dA[kH], entry[kH], left[kH];
     float sum = 0.f;
 #pragma unroll
     for (int s = 0; s < kH; ++s) {
       tile_dA[s] = F2(0.f, 0.f);
-      entry[s] = r[s];
-      prod[s] = F2(1.f, 1.f);
+      entry[s] = left[s] = r[s];
     }
 #pragma unroll 1
     for (int k = TT / kRun - 1; k >= 0; --k) {
@@ -1127,7 +1127,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks)
 #pragma unroll
         for (int s = 0; s < kH; ++s) {
           dec[j][s] = exp2_2(mul2(d2, A2[s]));
-          prod[s] = mul2(prod[s], dec[j][s]);
+          left[s] = mul2(left[s], dec[j][s]);
           h[j + 1][s] = fma2(dec[j][s], h[j][s], mul2(x2, b[s]));
         }
         y[j] = dot(h[j + 1], c);
@@ -1175,7 +1175,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks)
 #pragma unroll
     for (int s = 0; s < kH; ++s) {
       dA[s] = add2(dA[s], tile_dA[s]);
-      r[s] = correct_tile2(r[s], entry[s], mul2(F2(sum, sum), A2[s]), prod[s]);
+      r[s] = correct_tile2(r[s], entry[s], mul2(F2(sum, sum), A2[s]), left[s]);
     }
     __syncwarp();
     if (q.valid && loads) {
