@@ -273,13 +273,16 @@ int pc2d_causal_conv_step(int dtype, int wdtype, const void *input, void *state,
  *   d_t = delta_t + delta_bias[c]        (softplus of it with delta_softplus)
  *   h_t[n] = exp(d_t A[c][n]) h_{t-1}[n] + d_t u_t B_t[n]
  *   output_t = (sum_n C_t[n] h_t[n] + skip[c] u_t) * (z_t sigmoid(z_t) with z)
- * from h = initial_state (NULL: 0); final_state = h after the last token.
+ * from h = initial_state (NULL: 0); final_state = h after the last token.  Up to
+ * 2^24 rows (batch * channels; of the step too) and 2^30 tokens.
  * u, delta, z and output [batch][channels][length]; A [channels][states],
  * skip and delta_bias [channels] (NULL: 0), states [batch][channels][states]:
  * float32.  `checkpoints` (NULL: none) receives the states that the backward
  * pass starts its tiles from, pc2d_ssm_scan_checkpoint_size() bytes.  The
  * backward pass gives the gradients of all inputs (skipgrad, biasgrad,
- * initialgrad and grad_final may be NULL; zgrad goes with z).
+ * initialgrad and grad_final may be NULL; zgrad goes with z).  Its workspace is
+ * about states^2 / 64 bytes per channel and token (blocks have fewer channels
+ * the more states these have, and each has shares of Bgrad and Cgrad of its own).
  * pc2d_ssm_scan_step takes one token per row (u, delta, z [batch][channels],
  * B, C [batch][groups][states]) and moves its state [places][channels][states]
  * on in place; slots as for pc2d_causal_conv_step. */

@@ -26,9 +26,9 @@
 // The bound is the arithmetic: an exp per channel, state and token (two in
 // the backward pass) at 16 a clock and SM, against 8 to 14 bytes of traffic
 // per channel and token.  4 x 2048 x 2048 bf16 with 16 states and a gate take
-// 190 us forwards and 498 backwards: 256 blocks are 7 warps per SM, whose
+// 185 us forwards and 495 backwards: 256 blocks are 7 warps per SM, whose
 // issue slots are half used and no pipe is full; with 14 warps (one row of
-// 16384 tokens in segments) 65 % are used.
+// 16384 tokens in segments) 64 % are used.
 //
 // Few rows leave SMs empty.  Then the length is cut into segments that run at
 // the same time, after a first pass that gives each segment's end state from
@@ -60,8 +60,8 @@ constexpr float kInf = __builtin_huge_valf();
 // forward tile holds whole backward ones.  kMany: for grids that fill the GPU
 // several times, registers for four blocks per SM and a shorter tile; else for
 // two, which the compiler spends on overlapping more of a run (16384 tokens of
-// 2048 channels in 9 segments: 284 against 338 us; 4 x 2048 tokens of 2048
-// channels, 1.7 blocks per SM: 212 against 190 us).
+// 2048 channels in 9 segments: 287 against 330 us; 4 x 2048 tokens of 2048
+// channels, 1.7 blocks per SM: 209 against 184 us).
 // kWhole: every row of the arrays starts on a 16-byte boundary.
 template <int P_, bool kWhole_, bool kMany_ = false>
 struct Layout {
@@ -1466,7 +1466,8 @@ int check_scan(const char *what, int dtype, int batch, int channels, int length,
 // exps again, so the length is cut only when the rows alone leave most of the
 // GPU idle, into as many as give each SM the blocks that it holds at a time
 // (four forwards, two backwards) and at least two tiles of the longer (forward)
-// kind each.
+// kind each.  Two segments are not made (2 x 2048 x 2048 bf16, 128 blocks
+// backwards: 358 us as it is, 326 with two).
 template <bool kBackward>
 void scan_split(ScanArgs *a) {
   const int CB = kThreads / lanes_of(a->states);
@@ -1593,7 +1594,7 @@ extern "C" int pc2d_ssm_scan_forward(int dtype, const void *u, const void *delta
     }
     // more blocks than two per SM: the layout for four (the rule goes by the grid; rows of a ragged batch that end
     // early may leave less, and then it costs up to a tenth: 7 x 1002 channels of 24 states over up to 777 tokens,
-    // fp16, 93 against 86 us)
+    // fp16, 91 against 84 us; with all 777 in every row 131 against 157)
     if constexpr (G::P == 4 || G::P == 8) {
       if (grid > 2u * device_sm_count()) {
         scan_forward_kernel<T, Layout<G::P, G::kWhole, true>, false><<<grid, kThreads, 0, s>>>(a);

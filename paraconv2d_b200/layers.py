@@ -74,8 +74,8 @@ def dropout(x: Tensor, p: float, key: Tensor, residual: Optional[Tensor] = None)
 class Dropout(nn.Module):
     """:func:`dropout` in training, the identity (plus the residual) in
     evaluation.  Every call in training uses the next offset of ``seed``, kept
-    on the GPU in the buffer ``state`` and counted there: a call that a CUDA
-    graph replays drops other elements each time, and a checkpoint goes on
+    on the GPU in the buffer ``state`` and counted there (by a small launch of
+    its own): a call that a CUDA graph replays drops other elements each time, and a checkpoint goes on
     where it was saved.  Ranks of a data-parallel job need seeds of their own,
     and so have layers whose masks should not be the same; a wrapper that
     broadcasts buffers would give all ranks the same seed.  Where activations
@@ -179,12 +179,15 @@ def ssm_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optio
     ``B`` and ``C``: [batch, groups, states, length], each group for
     channels/groups neighbouring channels; all of one type.  ``A`` [channels,
     states], ``D`` and ``delta_bias`` [channels] (None: 0) and the states
-    [batch, channels, states] are float32.  1 to 128 states.
+    [batch, channels, states] are float32.  1 to 128 states; up to 2^24 rows
+    (batch times channels) and 2^30 tokens.  A of -inf forgets at every token.
 
     ``initial_state`` (None: 0), ``lengths`` and ``return_final_state`` as for
     :func:`causal_conv`.  Gradients reach every tensor but ``lengths``.  For
     the backward pass the forward one keeps the states of every 16th or 32nd
-    token in float32.
+    token in float32: 2 bytes per channel and token with 16 states, 32 with
+    128.  The backward pass itself takes scratch of about states^2 / 64 bytes
+    per channel and token: 4 with 16 states, but 64 with 64 and 256 with 128.
     """
     outs = _ops.ssm_scan_forward(u, delta, A, B, C, D, z, delta_bias, initial_state, lengths, bool(delta_softplus),
                                  bool(return_final_state), False)
@@ -205,7 +208,9 @@ class SSMScan(nn.Module):
     """:func:`ssm_scan` with softplus and its parameters: ``A_log`` [channels,
     states] (A = -exp(A_log), decays of 1 to ``states`` at first), ``D`` and
     ``delta_bias`` [channels] (steps from 0.001 to 0.1 at first).  delta, B and
-    C come with each call: projections of the input make them."""
+    C come with each call: projections of the input make them.  Every call
+    makes A from A_log, by two small launches before its own; a loop over
+    tokens may make A once and call :func:`ssm_scan_step` with it."""
 
     def __init__(self, channels: int, states: int = 16, device=None):
         super().__init__()
