@@ -148,7 +148,7 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 
 // Decays.  The hardware exponential is off by up to 2.4 units of 2^-24 and, on
 // average over its table, low by 0.1 to 0.8 of one (measured on [-2, 0]).  A
-// state that decays slowly would add that bias up over all the tokens it
+// state that decays (or grows) slowly would add that bias up over all the tokens it
 // remembers, a thousand or more.  So each tile of up to 32 tokens ends with a
 // correction: what is left of the state that entered the tile, by the decays
 // that were used, is replaced by exp of the tile's sum,
@@ -175,11 +175,11 @@ __device__ __forceinline__ F2 exp2_tile2(F2 x) {
   q = fma2(q, x, F2(1.f, 1.f));
   return F2(fabsf(x.x()) < 0.125f ? q.x() : exp2_f(x.x()), fabsf(x.y()) < 0.125f ? q.y() : exp2_f(x.y()));
 }
-// h corrected for the tile: x = A2 sum d.  Not for a growing state, nor an
-// infinite one, nor where the decays overflowed.
+// h corrected for the tile: x = A2 sum d.  Not for an infinite state, nor where
+// the decays overflowed.
 __device__ __forceinline__ float correct_tile(float h, float entry, float x, float left) {
   const float by = fmaf(entry, exp2_tile(x), -left);
-  return x <= 0.f && fabsf(by) < kInf ? h + by : h;
+  return fabsf(by) < kInf ? h + by : h;
 }
 __device__ __forceinline__ F2 correct_tile2(F2 h, F2 entry, F2 x, F2 left) {
   return F2(correct_tile(h.x(), entry.x(), x.x(), left.x()), correct_tile(h.y(), entry.y(), x.y(), left.y()));

@@ -119,3 +119,12 @@ def test_scan_slow_decays_are_not_biased(G, N, rate):
     exact = torch.exp(A.double() * total[:, -1:])
     mean = float(((first[0].double() - exact) / exact).mean()) / U32
     assert abs(mean) <= 32, f"gradients off by {mean:.3g} units on average"
+
+
+@pytest.mark.parametrize("G", [1, 256], ids=["in segments", "uncut"])
+@pytest.mark.parametrize("N", [4, 16])
+@pytest.mark.parametrize("rate", [2e-4, 5e-5, 1e-5])
+def test_scan_slow_growth_is_not_biased(G, N, rate):
+    """The same with A > 0: states that grow by up to e^5 over the row, whose
+    tokens all stay remembered.  The bounds are those of slow decays."""
+    test_scan_slow_decays_are_not_biased(G, N, -rate)
