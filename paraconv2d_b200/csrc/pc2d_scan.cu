@@ -26,7 +26,7 @@
 // The bound is the arithmetic: an exp per channel, state and token (two in
 // the backward pass) at 16 a clock and SM, against 8 to 14 bytes of traffic
 // per channel and token.  4 x 2048 x 2048 bf16 with 16 states and a gate take
-// 185 us forwards and 495 backwards: 256 blocks are 7 warps per SM, whose
+// 181 us forwards and 494 backwards: 256 blocks are 7 warps per SM, whose
 // issue slots are half used and no pipe is full; with 14 warps (one row of
 // 16384 tokens in segments) 64 % are used.
 //
