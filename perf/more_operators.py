@@ -425,7 +425,10 @@ def _encode(x, low, signed):
     normal = size >= least
     shifted = torch.where(normal, size, size + least).view(torch.int32)
     code = ((shifted + down) >> 20) - wide + torch.where(normal, 8, 0)
-    code = torch.where(wide == 255 << 3, 0, code.clamp(max=8 * top + 7))
+    code = code.clamp(max=8 * top + 7)
+    if not signed:  # a second moment that is not zero stays so: the step is divided by its root
+        code = torch.where((size > 0) & (code == 0), 1, code)
+    code = torch.where(wide == 255 << 3, 0, code)
     if signed:
         code = code | torch.where(x < 0, 128, 0)
     return code.to(torch.uint8), scale.to(torch.uint8)
@@ -670,7 +673,8 @@ def _exact_adamw(s):
                    for p in (0, 2)]
             chance = [(torch.from_numpy(x.reshape(-1)[:n].astype(np.float64)).cuda() + 0.5) / 256 for x in low]
             m = torch.sign(m) * _held(m.abs(), chance[0], 15)
-            v = _held(v, chance[1], 31)
+            held = _held(v, chance[1], 31)
+            v = torch.where((held == 0) & (v > 0), _held(v, 1.0, 31), held)
         shape = (n,) if bits8 else param.shape
         ms.append(m.view(shape))
         vs.append(v.view(shape))
