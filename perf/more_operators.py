@@ -411,21 +411,20 @@ def _bits8(n, seed, step, index):
 def _encode(x, low, signed):
     """The values x as 8-bit floats with 3 bits of mantissa, under the
     exponent of the smallest normal number of each block of 256: the one that
-    brings the block's largest into the topmost of 15 (beside a sign) or 31
-    binades.  Rounded up with the probability of what is cut off, by the
+    brings the block's largest, rounded up to a code, into the topmost of 15
+    (beside a sign) or 31 binades.  Rounded up with the probability of what is cut off, by the
     8-bit numbers `low`."""
     n, top = x.numel(), 15 if signed else 31
     size = x.abs()
     blocks = torch.nn.functional.pad(size, (0, -n % BLOCK)).view(-1, BLOCK)
-    most = blocks.amax(1).view(torch.int32) >> 23
-    scale = torch.where(most == 255, 255, (most - (top - 1)).clamp(min=1))
+    most = blocks.amax(1).view(torch.int32)
+    scale = torch.where(most >> 23 == 255, 255, ((most + 0xFFFFF >> 23) - (top - 1)).clamp(min=1))
     least = (scale << 23).view(torch.float32).repeat_interleave(BLOCK)[:n]
     wide = scale.repeat_interleave(BLOCK)[:n] << 3
     down = low * 4096 + 2048
     normal = size >= least
     shifted = torch.where(normal, size, size + least).view(torch.int32)
     code = ((shifted + down) >> 20) - wide + torch.where(normal, 8, 0)
-    code = code.clamp(max=8 * top + 7)
     if not signed:  # a second moment that is not zero stays so: the step is divided by its root
         code = torch.where((size > 0) & (code == 0), 1, code)
     code = torch.where(wide == 255 << 3, 0, code)
@@ -622,12 +621,12 @@ def _held(x, chance, top):
     binade; of the lowest binade's under that) below it, or above it with the
     chance's probability."""
     blocks = torch.nn.functional.pad(x, (0, -x.numel() % BLOCK)).view(-1, BLOCK)
-    most = torch.floor(torch.log2(blocks.amax(1).clamp(min=2.0 ** -126)))
+    # (above 15/8 of its binade, a block's largest may be rounded up into the next one)
+    most = torch.floor(torch.log2((blocks.amax(1) * (16 / 15)).clamp(min=2.0 ** -126)))
     lowest = (most - (top - 1)).clamp(min=-126).repeat_interleave(BLOCK)[:x.numel()]
     binade = torch.maximum(torch.floor(torch.log2(x.clamp(min=1e-300))), lowest)
     step = torch.exp2(binade - 3)
-    largest = torch.exp2(lowest + (top - 1)) * 15 / 8
-    return torch.minimum(torch.floor(x / step + chance) * step, largest)
+    return torch.floor(x / step + chance) * step
 
 
 def _exact_adamw(s):
