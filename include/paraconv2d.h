@@ -305,6 +305,48 @@ int pc2d_ssm_scan_step(int dtype, const void *u, const void *delta, float *state
                        int delta_softplus, int batch, int places, int channels, int states, int groups, void *output,
                        void *stream);
 
+/* ---------------------------------------------------------------------------
+ * AdamW over many tensors of one or several types, with the moments in 32 or
+ * in 8 bits (state_bits).  At step t = ++*step (int64 on the device), for each
+ * element w of tensor i with gradient g = grad * *grad_scale (NULL: 1):
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   w = (1 - lr rate weight_decay decay) w - lr rate m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps)
+ * in 32 bits; rate is rate_first for the first `split` elements and rate_rest
+ * behind them.  *lr_device (NULL: lr) lets a captured call follow a schedule.
+ * dtype F32, F16 or BF16; gradients of the same type or F32.  With `master`
+ * (16-bit parameters only) w is held there in float32, and the parameter is
+ * its rounding.  Written arrays may not overlap any other.
+ * 32 bits: exp_avg (m) and exp_avg_sq (v) are float32 [n].  8 bits: they are
+ * codes [n], and scales [ceil(n/256)][2] holds the exponent byte E of each
+ * moment for every 256 elements; zeros are zero moments.  A code's size c (m:
+ * the low 7 bits, the sign above them) stands for c/8 s below 8 and for
+ * 2^((c >> 3) - 1) (1 + (c & 7)/8) s from there on, s = 2^(E - 127); E = 255
+ * (a value of the block was not finite): NaN.  E brings the block's largest
+ * value, rounded up to a code, into the topmost binade, and values are rounded up with the
+ * probability of what is cut off: size/step + (r + 1/2)/256, rounded down,
+ * where r is byte j of the first (m) or of the last (v) two words that
+ * Philox4x32-10 gives for the counter (element/8, i, t low, t high) under the
+ * key `seed`, j = element % 8; a v that is not zero gets code 1 at least.  Per call: two launches, and more beyond 320 tensors
+ * or for more types.  workspace: pc2d_adamw_workspace_size() bytes.
+ * pc2d_adamw_state_values writes the values of 8-bit moments (exp_avg,
+ * exp_avg_sq, scales and n of each tensor) as F32 or BF16, both exact. */
+typedef struct {
+  int dtype, grad_dtype;
+  void *param;
+  const void *grad;
+  void *exp_avg, *exp_avg_sq;
+  float *master;         /* NULL: none */
+  unsigned char *scales; /* 8 bits only */
+  int64_t n, split;
+  double rate_first, rate_rest, decay;
+} pc2d_adamw_tensor;
+size_t pc2d_adamw_workspace_size(void);
+int pc2d_adamw_step(int state_bits, const pc2d_adamw_tensor *tensors, int count, int64_t *step, const float *lr_device,
+                    double lr, double beta1, double beta2, double eps, double weight_decay, const float *grad_scale,
+                    int64_t seed, void *workspace, size_t workspace_bytes, void *stream);
+int pc2d_adamw_state_values(int dtype, const pc2d_adamw_tensor *tensors, int count, void *const *exp_avgs,
+                            void *const *exp_avg_sqs, void *stream);
+
 /* Human-readable name of a pc2d_status. */
 const char *pc2d_status_string(int status);
 

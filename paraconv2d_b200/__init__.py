@@ -29,7 +29,9 @@ from .layers import (  # noqa: F401
     ssm_scan,
     ssm_scan_step,
 )
+from .optim import ParaboloidAdamW, ParaboloidSGD, adamw_new_state, adamw_state_values, adamw_step  # noqa: F401
 
 __all__ = ["ParaConv2d", "ParaConv2dFunction", "spotlightinit", "pnnconvert", "ptparaconv2d", "cabi", "set_algo",
            "CausalConv", "Dropout", "SSMScan", "causal_conv", "causal_conv_step", "dropout", "ssm_scan", "ssm_scan_step",
+           "ParaboloidAdamW", "ParaboloidSGD", "adamw_new_state", "adamw_state_values", "adamw_step",
            "load_op_library", "PC2D_ALGO_AUTO", "PC2D_ALGO_SIMT", "PC2D_ALGO_TC"]

@@ -32,6 +32,18 @@ PC2D_ALGO_AUTO = 0
 PC2D_ALGO_SIMT = 1
 PC2D_ALGO_TC = 2
 
+
+
+class AdamWTensor(ctypes.Structure):
+    """pc2d_adamw_tensor of include/paraconv2d.h"""
+
+    _fields_ = [("dtype", ctypes.c_int), ("grad_dtype", ctypes.c_int), ("param", ctypes.c_void_p),
+                ("grad", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p), ("exp_avg_sq", ctypes.c_void_p),
+                ("master", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("n", ctypes.c_int64),
+                ("split", ctypes.c_int64), ("rate_first", ctypes.c_double), ("rate_rest", ctypes.c_double),
+                ("decay", ctypes.c_double)]
+
+
 _lock = threading.Lock()
 _op_loaded = False
 _cabi = None
@@ -101,6 +113,10 @@ def cabi() -> ctypes.CDLL:
             "pc2d_ssm_scan_backward_workspace_size": ([I] * 5, S),
             "pc2d_ssm_scan_backward": ([I] + [P] * 12 + [I] * 6 + [P] * 10 + [S, P], I),
             "pc2d_ssm_scan_step": ([I] + [P] * 10 + [I] * 6 + [P] * 2, I),
+            "pc2d_adamw_workspace_size": ([], S),
+            "pc2d_adamw_step": ([I, ctypes.POINTER(AdamWTensor), I, P, P] + [D] * 5 + [P, L, P, S, P], I),
+            "pc2d_adamw_state_values": ([I, ctypes.POINTER(AdamWTensor), I, ctypes.POINTER(P), ctypes.POINTER(P), P],
+                                        I),
             "pc2d_status_string": ([I], ctypes.c_char_p),
             "pc2d_last_error": ([], ctypes.c_char_p),
             "pc2d_device_status": ([], I),

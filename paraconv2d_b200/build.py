@@ -5,7 +5,8 @@
 * ``libptparaconv2d.so`` -- the ``torch.ops.ptparaconv2d`` registration
   (g++ against the installed torch, links libpc2d_sm100.so).
 
-Both are rebuilt only when a source or header is newer than the library.
+Both are rebuilt only when a source or header is newer than the library (an
+object only when its own source or a header is newer).
 Usage: ``python paraconv2d_b200/build.py [--force] [--verbose]`` (run as a file: importing
 the package loads the libraries this builds).
 """
@@ -65,8 +66,12 @@ def build_kernel_lib(force=False, verbose=False, ptxas_verbose=False):
     os.makedirs(BUILD, exist_ok=True)
     extra = ["-Xptxas", "-v"] if ptxas_verbose else []
 
+    newest = _newest(headers() + [__file__])
+
     def compile_one(src):
         obj = os.path.join(BUILD, os.path.basename(src) + ".o")
+        if not (force or ptxas_verbose) and os.path.exists(obj) and os.path.getmtime(obj) >= max(newest, os.path.getmtime(src)):
+            return obj
         _run([NVCC, *ARCH_FLAGS, *NVCC_FLAGS, *extra, "-c", src, "-o", obj], verbose or ptxas_verbose)
         return obj
 
@@ -79,9 +84,9 @@ def build_kernel_lib(force=False, verbose=False, ptxas_verbose=False):
 
 
 def build_op_lib(force=False, verbose=False):
-    srcs = [os.path.join(CSRC, "pc2d_op.cpp"), os.path.join(CSRC, "pc2d_seq_op.cpp")]
-    if (not force and os.path.exists(OP_LIB)
-            and os.path.getmtime(OP_LIB) >= _newest([*srcs, os.path.join(INCLUDE, "paraconv2d.h"), KERNEL_LIB, __file__])):
+    srcs = [os.path.join(CSRC, n) for n in ("pc2d_op.cpp", "pc2d_seq_op.cpp", "pc2d_train_op.cpp")]
+    deps = [os.path.join(CSRC, "pc2d_op_common.h"), os.path.join(INCLUDE, "paraconv2d.h"), KERNEL_LIB, __file__]
+    if not force and os.path.exists(OP_LIB) and os.path.getmtime(OP_LIB) >= _newest(srcs + deps):
         return OP_LIB
     import sysconfig
 
@@ -91,11 +96,20 @@ def build_op_lib(force=False, verbose=False):
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     cxx = shutil.which("g++") or "c++"
     tmp = OP_LIB + f".tmp{os.getpid()}"
-    _run([cxx, "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-          "-isystem", os.path.join(tdir, "include"),
-          "-isystem", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
-          "-isystem", sysconfig.get_path("include"), "-I" + os.path.join(CUDA_HOME, "include"), "-I" + INCLUDE,
-          *srcs, "-o", tmp,
+    os.makedirs(BUILD, exist_ok=True)
+
+    def compile_one(src):
+        obj = os.path.join(BUILD, os.path.basename(src) + ".o")
+        _run([cxx, "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+              "-isystem", os.path.join(tdir, "include"),
+              "-isystem", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
+              "-isystem", sysconfig.get_path("include"), "-I" + os.path.join(CUDA_HOME, "include"), "-I" + INCLUDE,
+              "-c", src, "-o", obj], verbose)
+        return obj
+
+    with cf.ThreadPoolExecutor(max_workers=len(srcs)) as ex:
+        objs = list(ex.map(compile_one, srcs))
+    _run([cxx, "-shared", *objs, "-o", tmp,
           "-L" + PKG, "-l:libpc2d_sm100.so", "-Wl,-rpath,$ORIGIN",
           "-L" + os.path.join(tdir, "lib"), "-Wl,-rpath," + os.path.join(tdir, "lib"),
           "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_cuda",

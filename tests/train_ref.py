@@ -1,0 +1,102 @@
+"""The operators of a training step from their definitions, in 64 bits on the
+CPU, each value beside its magnitude: the sum of the absolute values of the
+terms that make it up."""
+import numpy as np
+import torch
+
+from layers_ref import philox
+
+BLOCK = 256
+
+
+# ---------------------------------------------------------------------- AdamW
+
+def adamw_decode(codes, scale, signed):
+    """Values of codes [n] under the exponent bytes scale [blocks]."""
+    c = codes.long()
+    size = c & 127 if signed else c
+    least = torch.exp2(scale.double() - 127).repeat_interleave(BLOCK)[:c.numel()]
+    x = torch.where(size < 8, size.double() / 8, torch.exp2((size >> 3).double() - 1) * (1 + (size & 7).double() / 8))
+    x = torch.where(scale.repeat_interleave(BLOCK)[:c.numel()] == 255, float("nan"), x * least)
+    return torch.where(c > 127, -x, x) if signed else x
+
+
+def adamw_encode(x, low, signed):
+    """Codes and exponent bytes of the 32-bit values x (held in 64 bits), with
+    the 8-bit random numbers `low`: multiples of a step, by definition."""
+    n, top = x.numel(), 15 if signed else 31
+    x, low = x.double(), torch.as_tensor(np.asarray(low), dtype=torch.float64)
+    codes, scales = torch.zeros(n, dtype=torch.uint8), []
+    for at in range(0, n, BLOCK):
+        part, r = x[at:at + BLOCK], low[at:at + BLOCK]
+        size = part.abs()
+        most = float(size.max())
+        if not np.isfinite(most):
+            scales.append(255)
+            code = torch.zeros(part.numel(), dtype=torch.long)
+        else:
+            binade = -126 if most < 2.0 ** -126 else int(np.floor(np.log2(most)))
+            binade += most > 15 / 8 * 2.0 ** binade and most >= 2.0 ** -126  # may be rounded up into the next one
+            lowest = max(binade - (top - 1), -126)
+            scales.append(lowest + 127)
+            _, e = torch.frexp(size)  # size = mantissa in [1/2, 1) times 2^e
+            e = torch.where(size < 2.0 ** lowest, lowest, e.long() - 1)
+            parts = size * torch.exp2(3 - e.double())
+            if bool((size < 2.0 ** lowest).any()):  # added to the smallest normal number in 32 bits
+                small = ((size + 2.0 ** lowest).float().double() - 2.0 ** lowest) * 2.0 ** (3 - lowest)
+                parts = torch.where(size < 2.0 ** lowest, small, parts)
+            eighths = torch.floor(parts + (r + 0.5) / 256).long()
+            code = (e - lowest) * 8 + eighths
+            if not signed:
+                code = torch.where((size > 0) & (code == 0), 1, code)
+        if signed:
+            code = code + 128 * (part < 0).long()
+        codes[at:at + BLOCK] = code.to(torch.uint8)
+    return codes, torch.tensor(scales, dtype=torch.uint8)
+
+
+def adamw_random(n, seed, t, index):
+    """The bytes for the first and the second moments of n elements."""
+    seed, t = seed & (2 ** 64 - 1), t & (2 ** 64 - 1)
+    rows = [[], []]
+    for group in range((n + 7) // 8):
+        words = philox((group, index, t & 0xFFFFFFFF, t >> 32), (seed & 0xFFFFFFFF, seed >> 32))
+        for k in range(2):
+            rows[k] += [w >> s & 255 for w in words[2 * k:2 * k + 2] for s in (0, 8, 16, 24)]
+    return [r[:n] for r in rows]
+
+
+def adamw(c, t, lr, betas, eps, weight_decay, factors=None, grad_scale=None, seed=0):
+    """Values and magnitudes after step t, a dict for each tensor; moments in
+    8 bits as the codes of the 32-bit moments."""
+    b1, b2 = betas
+    outs = []
+    for i, p in enumerate(c["params"]):
+        n = p.numel()
+        split, first, rest, decay = (factors[i] if factors else None) or (n, 1.0, 1.0, 1.0)
+        rate = torch.where(torch.arange(n) < split, first, rest).double() * lr
+        g = c["grads"][i].float()
+        if grad_scale is not None:
+            g = g * torch.tensor(grad_scale)
+        m, v = c["m"][i], c["v"][i]
+        if c["scales"] is not None:
+            m, v = (adamw_decode(x, c["scales"][i][:, k], k == 0) for k, x in enumerate((m, v)))
+        w = (c["masters"][i] if c["masters"] else p).double()
+        g64, m0, v0 = g.double(), m.double(), v.double()
+        m1, v1 = b1 * m0 + (1 - b1) * g64, b2 * v0 + (1 - b2) * g64 * g64
+        o = dict(m=m1, v=v1, m_size=(b1 * m0).abs() + ((1 - b1) * g64).abs(), v_size=v1)
+        kept = w * (1 - rate * weight_decay * decay)
+        root = (v1 / (1 - b2 ** t)).sqrt() + eps
+        o["param"] = kept - rate * m1 / (1 - b1 ** t) / root
+        o["param_size"] = kept.abs() + rate.abs() * o["m_size"] / (1 - b1 ** t) / root
+        if c["scales"] is not None:
+            # the moments of 32 bits, product by product
+            f = np.float32
+            m32 = m.float() * float(f(b1)) + g * float(f(1 - b1))
+            v32 = v.float() * float(f(b2)) + (g * float(f(1 - b2))) * g
+            low = adamw_random(n, seed, t, i) if n else ([], [])
+            o["m_code"], sm = adamw_encode(m32, low[0], True)
+            o["v_code"], sv = adamw_encode(v32, low[1], False)
+            o["scales"] = torch.stack([sm, sv], 1)
+        outs.append(o)
+    return outs
