@@ -306,6 +306,30 @@ int pc2d_ssm_scan_step(int dtype, const void *u, const void *delta, float *state
                        void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Group norm over [batch][channels][length] maps, or with channels_last over
+ * [batch][length][channels], with an optional SiLU:
+ *   xhat = (x - mean) / sqrt(variance + eps), over the channels/groups channels
+ *   of a group and all tokens of a batch row (population variance);
+ *   pre = xhat weight[c] + bias[c];  output = pre, or pre sigmoid(pre) with silu.
+ * float32, float16 and bfloat16; weight and bias [channels] (NULL: 1 and 0) of
+ * the input's type or float32 (wdtype).  lengths as for the sequence operators
+ * (NULL: all tokens).  stats [batch][groups][2] (NULL: not kept) receives the
+ * mean and 1/sqrt(variance + eps), which the backward pass takes; weightgrad
+ * and biasgrad may be NULL.  Arrays need their elements' alignment (16 bytes
+ * are faster); no output may overlap an input.  Up to 8192 channels a group,
+ * 2^24 batch * groups and 2^30 positions. */
+size_t pc2d_group_norm_workspace_size(int dtype, int channels_last, int batch, int channels, int length, int groups,
+                                      int backward);
+int pc2d_group_norm_forward(int dtype, int wdtype, int channels_last, const void *input, const void *weight,
+                            const void *bias, const int *lengths, int batch, int channels, int length, int groups,
+                            double eps, int silu, void *output, float *stats, void *workspace, size_t workspace_bytes,
+                            void *stream);
+int pc2d_group_norm_backward(int dtype, int wdtype, int channels_last, const void *grad, const void *input,
+                             const void *weight, const void *bias, const int *lengths, const float *stats, int batch,
+                             int channels, int length, int groups, int silu, void *inputgrad, void *weightgrad,
+                             void *biasgrad, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------
  * AdamW over many tensors of one or several types, with the moments in 32 or
  * in 8 bits (state_bits).  At step t = ++*step (int64 on the device), for each
  * element w of tensor i with gradient g = grad * *grad_scale (NULL: 1):

@@ -22,16 +22,18 @@ from .ptparaconv2d import ParaConv2d, ParaConv2dFunction, pnnconvert, spotlighti
 from .layers import (  # noqa: F401
     CausalConv,
     Dropout,
+    GroupNorm,
     SSMScan,
     causal_conv,
     causal_conv_step,
     dropout,
+    group_norm,
     ssm_scan,
     ssm_scan_step,
 )
 from .optim import ParaboloidAdamW, ParaboloidSGD, adamw_new_state, adamw_state_values, adamw_step  # noqa: F401
 
 __all__ = ["ParaConv2d", "ParaConv2dFunction", "spotlightinit", "pnnconvert", "ptparaconv2d", "cabi", "set_algo",
-           "CausalConv", "Dropout", "SSMScan", "causal_conv", "causal_conv_step", "dropout", "ssm_scan", "ssm_scan_step",
+           "CausalConv", "Dropout", "SSMScan", "causal_conv", "causal_conv_step", "dropout", "GroupNorm", "group_norm", "ssm_scan", "ssm_scan_step",
            "ParaboloidAdamW", "ParaboloidSGD", "adamw_new_state", "adamw_state_values", "adamw_step",
            "load_op_library", "PC2D_ALGO_AUTO", "PC2D_ALGO_SIMT", "PC2D_ALGO_TC"]

@@ -113,6 +113,9 @@ def cabi() -> ctypes.CDLL:
             "pc2d_ssm_scan_backward_workspace_size": ([I] * 5, S),
             "pc2d_ssm_scan_backward": ([I] + [P] * 12 + [I] * 6 + [P] * 10 + [S, P], I),
             "pc2d_ssm_scan_step": ([I] + [P] * 10 + [I] * 6 + [P] * 2, I),
+            "pc2d_group_norm_workspace_size": ([I] * 7, S),
+            "pc2d_group_norm_forward": ([I] * 3 + [P] * 4 + [I] * 4 + [D, I, P, P, P, S, P], I),
+            "pc2d_group_norm_backward": ([I] * 3 + [P] * 6 + [I] * 5 + [P] * 4 + [S, P], I),
             "pc2d_adamw_workspace_size": ([], S),
             "pc2d_adamw_step": ([I, ctypes.POINTER(AdamWTensor), I, P, P] + [D] * 5 + [P, L, P, S, P], I),
             "pc2d_adamw_state_values": ([I, ctypes.POINTER(AdamWTensor), I, ctypes.POINTER(P), ctypes.POINTER(P), P],

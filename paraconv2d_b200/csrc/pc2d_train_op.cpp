@@ -1,6 +1,6 @@
-// torch.ops.paraconv2d_b200: the AdamW step over many tensors, on top of the C
-// ABI of libpc2d_sm100.so.  Argument checks, streams and scratch as for the
-// sequence operators.
+// torch.ops.paraconv2d_b200: group norm and the AdamW step over many tensors,
+// on top of the C ABI of libpc2d_sm100.so.  Argument checks, streams, scratch
+// and gradients as for the sequence operators.
 #include <algorithm>
 
 #include "pc2d_op_common.h"
@@ -39,6 +39,8 @@ struct Ranges {
     }
   }
 };
+
+// --------------------------------------------------------------------- AdamW
 
 void adamw_step_cuda(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs, at::TensorList exp_avg_sqs,
                      at::TensorList masters, at::TensorList scales, const Tensor &step, const OptTensor &lr_tensor,
@@ -174,6 +176,130 @@ std::vector<Tensor> adamw_state_values_cuda(at::TensorList exp_avgs, at::TensorL
   return outs;
 }
 
+// ---------------------------------------------------------------- group norm
+
+// Channels last: the order in which the dimension 1 is the innermost one.
+Tensor last_view(const Tensor &t) { return t.movedim(1, -1); }
+
+struct NormCall {
+  Call call;
+  int dt, wdt, last, batch, channels, length, groups;
+  Tensor input, weight, bias, lengths;
+};
+
+// A tensor in the order of dimensions of the call, its view in memory's order.
+Tensor in_order(const NormCall &c, const Tensor &t) { return c.last ? last_view(t).contiguous() : t.contiguous(); }
+
+NormCall norm_call(const char *what, const Tensor &input, const OptTensor &weight, const OptTensor &bias,
+                   const OptTensor &lengths, int64_t groups) {
+  NormCall c{{what, input.device()}};
+  c.dt = seq_dtype_code(input, what);
+  TORCH_CHECK(input.dim() >= 2, what, ": input must be [batch, channels, ...], got ", input.sizes());
+  c.batch = as_int(input.size(0), what, "batch");
+  c.channels = as_int(input.size(1), what, "channels");
+  int64_t length = 1;
+  for (int64_t d = 2; d < input.dim(); ++d) length *= input.size(d);
+  c.length = as_int(length, what, "the number of positions");
+  c.groups = as_int(groups, what, "groups");
+  c.last = input.dim() > 2 && !input.is_contiguous() && last_view(input).is_contiguous();
+  const auto wtype = weight.has_value() && weight->defined() ? weight->scalar_type()
+                     : bias.has_value() && bias->defined()   ? bias->scalar_type()
+                                                             : input.scalar_type();
+  TORCH_CHECK(wtype == input.scalar_type() || wtype == at::kFloat, what,
+              ": weight and bias must be of the input's type or float32, got ", wtype);
+  c.wdt = wtype == at::kFloat ? PC2D_DTYPE_F32 : c.dt;
+  c.input = in_order(c, input);
+  c.weight = c.call.maybe(weight, "weight", wtype, {c.channels});
+  c.bias = c.call.maybe(bias, "bias", wtype, {c.channels});
+  TORCH_CHECK(!(lengths.has_value() && lengths->defined()) || input.dim() == 3, what,
+              ": lengths go with [batch, channels, length] only, got ", input.sizes());
+  c.lengths = c.call.maybe(lengths, "lengths", at::kInt, {c.batch});
+  return c;
+}
+
+// A result in the order of dimensions of the input.
+Tensor norm_result(const NormCall &c, const Tensor &input) {
+  const Tensor t = at::empty(c.input.sizes(), c.input.options());
+  return c.last ? t.movedim(-1, 1) : t.view(input.sizes());
+}
+
+std::vector<Tensor> group_norm_forward_cuda(const Tensor &input, const OptTensor &weight, const OptTensor &bias,
+                                            const OptTensor &lengths, int64_t groups, double eps, bool silu,
+                                            bool keep_stats) {
+  const c10::cuda::CUDAGuard guard(input.device());
+  const NormCall c = norm_call("paraconv2d_b200.group_norm_forward", input, weight, bias, lengths, groups);
+  Tensor out = norm_result(c, input);
+  Tensor stats = at::empty(keep_stats ? at::IntArrayRef({c.batch, c.groups, 2}) : at::IntArrayRef({0}),
+                           input.options().dtype(at::kFloat));
+  const size_t bytes = pc2d_group_norm_workspace_size(c.dt, c.last, c.batch, c.channels, c.length, c.groups, 0);
+  const Tensor ws = workspace(bytes, input);
+  check_status(pc2d_group_norm_forward(c.dt, c.wdt, c.last, ptr(c.input), ptr(c.weight), ptr(c.bias),
+                                       ptr<int>(c.lengths), c.batch, c.channels, c.length, c.groups, eps, silu, ptr(out),
+                                       keep_stats ? ptr<float>(stats) : nullptr, ptr(ws), bytes, stream_now()),
+               c.call.what);
+  return {out, stats};
+}
+
+std::vector<Tensor> group_norm_backward_cuda(const Tensor &grad_, const Tensor &input, const OptTensor &weight,
+                                             const OptTensor &bias, const OptTensor &lengths, const Tensor &stats_,
+                                             int64_t groups, bool silu) {
+  const c10::cuda::CUDAGuard guard(input.device());
+  const NormCall c = norm_call("paraconv2d_b200.group_norm_backward", input, weight, bias, lengths, groups);
+  TORCH_CHECK(grad_.device() == input.device() && grad_.scalar_type() == input.scalar_type() &&
+                  grad_.sizes() == input.sizes(),
+              c.call.what, ": grad must be like the input");
+  const Tensor grad = in_order(c, grad_);
+  const Tensor stats = c.call.need(stats_, "stats", at::kFloat, {c.batch, c.groups, 2});
+  Tensor dx = norm_result(c, input);
+  auto like = [&](const Tensor &t) { return at::empty(t.defined() ? t.sizes() : at::IntArrayRef({0}),
+                                                      t.defined() ? t.options() : input.options()); };
+  Tensor dw = like(c.weight), db = like(c.bias);
+  const size_t bytes = pc2d_group_norm_workspace_size(c.dt, c.last, c.batch, c.channels, c.length, c.groups, 1);
+  const Tensor ws = workspace(bytes, input);
+  check_status(pc2d_group_norm_backward(c.dt, c.wdt, c.last, ptr(grad), ptr(c.input), ptr(c.weight), ptr(c.bias),
+                                        ptr<int>(c.lengths), ptr<float>(stats), c.batch, c.channels, c.length, c.groups,
+                                        silu, ptr(dx), c.weight.defined() ? ptr(dw) : nullptr,
+                                        c.bias.defined() ? ptr(db) : nullptr, ptr(ws), bytes, stream_now()),
+               c.call.what);
+  return {dx, dw, db};
+}
+
+struct NormFunction : torch::autograd::Function<NormFunction> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &input, const OptTensor &weight, const OptTensor &bias,
+                        const OptTensor &lengths, int64_t groups, double eps, bool silu) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto outs = PC2D_BELOW(group_norm_forward).call(input, weight, bias, lengths, groups, eps, silu, true);
+    ctx->save_for_backward({input, weight.value_or(Tensor()), bias.value_or(Tensor()), lengths.value_or(Tensor()),
+                            outs[1]});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["silu"] = silu;
+    return outs[0];
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+    return once("group_norm", [&]() -> variable_list {
+      const auto s = ctx->get_saved_variables();
+      const auto g = PC2D_BELOW(group_norm_backward)
+                         .call(grads[0], s[0], optional_of(s[1]), optional_of(s[2]), optional_of(s[3]), s[4],
+                               ctx->saved_data["groups"].toInt(), ctx->saved_data["silu"].toBool());
+      return {g[0], s[1].defined() ? g[1] : Tensor(), s[2].defined() ? g[2] : Tensor(), Tensor(), Tensor(), Tensor(),
+              Tensor()};
+    });
+  }
+};
+
+// With gradients the statistics are the graph's own: the second result is empty.
+std::vector<Tensor> group_norm_forward_autograd(const Tensor &input, const OptTensor &weight, const OptTensor &bias,
+                                                const OptTensor &lengths, int64_t groups, double eps, bool silu,
+                                                bool keep_stats) {
+  no_forward_mode("group_norm", {&input}, {&weight, &bias});
+  check_cuda(input, "group_norm");
+  if (needs_grad({&input}, {&weight, &bias}))
+    return {NormFunction::apply(input, weight, bias, lengths, groups, eps, silu),
+            at::empty({0}, input.options().dtype(at::kFloat))};
+  at::AutoDispatchBelowADInplaceOrView below;
+  return PC2D_BELOW(group_norm_forward).call(input, weight, bias, lengths, groups, eps, silu, keep_stats);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(paraconv2d_b200, m) {
@@ -181,10 +307,22 @@ TORCH_LIBRARY_FRAGMENT(paraconv2d_b200, m) {
       "adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avgs, Tensor(c!)[] exp_avg_sqs, "
       "Tensor(d!)[] masters, Tensor(e!)[] scales, Tensor(f!) step, Tensor? lr_tensor, float lr, float beta1, "
       "float beta2, float eps, float weight_decay, Tensor? grad_scale, int[] splits, float[] factors, int seed) -> ()");
+  m.def(
+      "group_norm_forward(Tensor input, Tensor? weight, Tensor? bias, Tensor? lengths, int groups, float eps, bool "
+      "silu, bool keep_stats) -> Tensor[]");
+  m.def(
+      "group_norm_backward(Tensor grad, Tensor input, Tensor? weight, Tensor? bias, Tensor? lengths, Tensor stats, "
+      "int groups, bool silu) -> Tensor[]");
   m.def("adamw_state_values(Tensor[] exp_avgs, Tensor[] exp_avg_sqs, Tensor[] scales, ScalarType dtype) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(paraconv2d_b200, CUDA, m) {
   m.impl("adamw_step", adamw_step_cuda);
   m.impl("adamw_state_values", adamw_state_values_cuda);
+  m.impl("group_norm_forward", group_norm_forward_cuda);
+  m.impl("group_norm_backward", group_norm_backward_cuda);
+}
+
+TORCH_LIBRARY_IMPL(paraconv2d_b200, Autograd, m) {
+  m.impl("group_norm_forward", group_norm_forward_autograd);
 }

@@ -47,6 +47,7 @@ class _ops:
     causal_conv_step = torch.ops.paraconv2d_b200.causal_conv_step.default
     ssm_scan_forward = torch.ops.paraconv2d_b200.ssm_scan_forward.default
     ssm_scan_step = torch.ops.paraconv2d_b200.ssm_scan_step.default
+    group_norm_forward = torch.ops.paraconv2d_b200.group_norm_forward.default
 
 
 def _silu(activation) -> bool:
@@ -242,3 +243,43 @@ class SSMScan(nn.Module):
 
     def extra_repr(self) -> str:
         return f"channels={self.channels}, states={self.states}"
+
+
+# ----------------------------------------------------------------- group norm
+
+def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
+               eps: float = 1e-5, activation: Optional[str] = None, lengths: Optional[Tensor] = None) -> Tensor:
+    """``x`` [batch, channels, ...] less its mean and divided by its deviation
+    over each of ``groups`` equal groups of neighbouring channels and all
+    positions of a batch row, times ``weight`` plus ``bias`` [channels] (None:
+    1 and 0; x's type or float32), through ``activation`` (None or 'silu').
+
+    ``x`` is taken as it lies, contiguous or channels last (the memory format,
+    or any [batch, channels, length] view of [batch, length, channels]), and
+    the result lies likewise; in another order it is copied.  ``lengths``
+    (int32 [batch], on the GPU; for [batch, channels, length] only): the
+    tokens of each row; what lies behind them is not read and counts nothing,
+    and outputs and gradients there are 0.  Up to 8192 channels a group.
+    """
+    return _ops.group_norm_forward(x, weight, bias, lengths, groups, eps, _silu(activation), False)[0]
+
+
+class GroupNorm(nn.Module):
+    """:func:`group_norm` with its ``weight`` and ``bias`` [channels]."""
+
+    def __init__(self, groups: int, channels: int, eps: float = 1e-5, affine: bool = True,
+                 activation: Optional[str] = None, device=None, dtype=None):
+        super().__init__()
+        if groups < 1 or channels % groups:
+            raise ValueError(f"channels ({channels}) must be a multiple of groups ({groups})")
+        _silu(activation)
+        self.groups, self.channels, self.eps, self.activation = groups, channels, eps, activation
+        kw = dict(device=device, dtype=dtype)
+        self.weight = nn.Parameter(torch.ones(channels, **kw)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(channels, **kw)) if affine else None
+
+    def forward(self, x, lengths=None):
+        return group_norm(x, self.groups, self.weight, self.bias, self.eps, self.activation, lengths)
+
+    def extra_repr(self) -> str:
+        return f"groups={self.groups}, channels={self.channels}, eps={self.eps}, activation={self.activation}"

@@ -100,3 +100,62 @@ def adamw(c, t, lr, betas, eps, weight_decay, factors=None, grad_scale=None, see
             o["scales"] = torch.stack([sm, sv], 1)
         outs.append(o)
     return outs
+
+
+# ----------------------------------------------------------------- group norm
+
+def norm(x, groups, w=None, b=None, eps=1e-5, silu=False, lengths=None, grad=None):
+    """Values of out and (with grad) dx, dw, db, and what each is made of:
+    sizes of the terms that may cancel."""
+    f64 = lambda t: None if t is None else t.detach().cpu().double()  # noqa: E731
+    x, w, b, grad = f64(x), f64(w), f64(b), f64(grad)
+    B, C = x.shape[:2]
+    shape = x.shape
+    x = x.reshape(B, C, -1)
+    L, cg = x.shape[2], C // groups
+    w = torch.ones(C, dtype=torch.float64) if w is None else w
+    b = torch.zeros(C, dtype=torch.float64) if b is None else b
+    v = {"out": torch.zeros(B, C, L, dtype=torch.float64)}
+    m = {"out": torch.zeros(B, C, L, dtype=torch.float64)}
+    if grad is not None:
+        grad = grad.reshape(B, C, -1)
+        for d in (v, m):
+            d.update(dx=torch.zeros(B, C, L, dtype=torch.float64), dw=torch.zeros(C, dtype=torch.float64),
+                     db=torch.zeros(C, dtype=torch.float64))
+    for i in range(B):
+        n = L if lengths is None else min(max(int(lengths[i]), 0), L)
+        if n == 0:
+            continue
+        for g in range(groups):
+            c = slice(g * cg, (g + 1) * cg)
+            p = x[i, c, :n]
+            mean = p.mean()
+            rstd = 1 / ((p - mean).square().mean() + eps).sqrt()
+            xhat = (p - mean) * rstd
+            wc, bc = w[c, None], b[c, None]
+            pre = xhat * wc + bc
+            sig = torch.sigmoid(pre)
+            act = sig if silu else torch.ones_like(pre)
+            slope = sig * (1 + pre * (1 - sig)) if silu else torch.ones_like(pre)
+            # x itself is exact, its mean off by a rounding of the values' size: xhat by that times rstd
+            off = xhat.abs() + rstd * p.abs().mean()
+            v["out"][i, c, :n] = pre * act
+            m["out"][i, c, :n] = (off * wc.abs() + bc.abs()) * ((1 + pre.abs()) if silu else 1)
+            if grad is None:
+                continue
+            d = grad[i, c, :n]
+            h = d * slope
+            hsize = d.abs() * (1.1 + (off * wc.abs() + bc.abs() if silu else 0))  # (the slope is at most 1.1, its own at most 1/2)
+            hw, hx = (h * wc).mean(), (h * wc * xhat).mean()
+            v["dx"][i, c, :n] = rstd * (h * wc - hw - xhat * hx)
+            top = hsize * wc.abs()
+            m["dx"][i, c, :n] = rstd * (top + top.mean() + off * (top * off).mean())
+            v["dw"][c] += (h * xhat).sum(1)
+            m["dw"][c] += (hsize * off).sum(1)
+            v["db"][c] += h.sum(1)
+            m["db"][c] += hsize.sum(1)
+    for d in (v, m):
+        for k in ("out", "dx"):
+            if k in d:
+                d[k] = d[k].view(shape)
+    return v, m
