@@ -236,7 +236,8 @@ def _own(s):
         outs = {"out": out[0], "state": out[1]} if _keeps(case) else {"out": out}
         grads = [s.get("grad"), s.get("grad_state")][:len(outs)]
     if case["train"]:
-        got = torch.autograd.grad(list(outs.values()), [s[n] for n in s["wanted"]], grads)
+        given = [(o, g) for o, g in zip(outs.values(), grads) if g is not None]
+        got = torch.autograd.grad([o for o, _ in given], [s[n] for n in s["wanted"]], [g for _, g in given])
         outs.update({"grad_" + n: v for n, v in zip(s["wanted"], got)})
     return outs
 
