@@ -330,6 +330,41 @@ int pc2d_group_norm_backward(int dtype, int wdtype, int channels_last, const voi
                              void *biasgrad, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Linear attention with a decay for each head.  Per batch row and head:
+ *   S_t = exp(g_t) S_(t-1) + k_t v_t^T  (dk x dv);  output_t = scale S_t^T q_t
+ * q, k [batch][groups][dk][length], each group for heads/groups neighbouring
+ * heads; v and output [batch][heads][dv][length]; log_decay g (float32, at
+ * most 0 in use; -inf forgets) [heads], or with decay_per_token
+ * [batch][heads][length].  States [batch][heads][dk][dv] are float32;
+ * initial_state (NULL: 0), lengths and final_state (NULL: not wanted) as for
+ * the sequence operators.  1 to 128 for dk and dv, up to 2^30 tokens and 2^20
+ * rows times heads.  `states` (NULL: none), ..._states_size() bytes, receives
+ * what the backward pass starts its chunks from: 4 dk dv bytes for every 64
+ * tokens of a head (every 32 in float32 and float16).  The backward pass gives all gradients
+ * (grad_final and initialgrad may be NULL), decaygrad in the decays' shape.
+ * Arrays need their elements' alignment (16 bytes and lengths that are
+ * multiples of 8 are faster).  pc2d_linear_attention_step takes one token per
+ * row (q, k [batch][groups][dk], v [batch][heads][dv], log_decay [heads] or
+ * with decay_per_row [batch][heads]) and moves its state [places][heads][dk]
+ * [dv] (16-byte aligned) on in place; slots as for pc2d_causal_conv_step. */
+size_t pc2d_linear_attention_states_size(int dtype, int batch, int heads, int length, int dk, int dv);
+size_t pc2d_linear_attention_workspace_size(int dtype, int batch, int heads, int groups, int length, int dk, int dv,
+                                            int backward);
+int pc2d_linear_attention_forward(int dtype, const void *q, const void *k, const void *v, const float *log_decay,
+                                  int decay_per_token, const float *initial_state, const int *lengths, int batch,
+                                  int heads, int groups, int length, int dk, int dv, double scale, void *output,
+                                  float *final_state, float *states, void *workspace, size_t workspace_bytes,
+                                  void *stream);
+int pc2d_linear_attention_backward(int dtype, const void *grad, const float *grad_final, const void *q, const void *k,
+                                   const void *v, const float *log_decay, int decay_per_token, const float *states,
+                                   const int *lengths, int batch, int heads, int groups, int length, int dk, int dv,
+                                   double scale, void *qgrad, void *kgrad, void *vgrad, float *decaygrad,
+                                   float *initialgrad, void *workspace, size_t workspace_bytes, void *stream);
+int pc2d_linear_attention_step(int dtype, const void *q, const void *k, const void *v, const float *log_decay,
+                               int decay_per_row, float *state, const int *slots, int batch, int places, int heads,
+                               int groups, int dk, int dv, double scale, void *output, void *stream);
+
+/* ---------------------------------------------------------------------------
  * AdamW over many tensors of one or several types, with the moments in 32 or
  * in 8 bits (state_bits).  At step t = ++*step (int64 on the device), for each
  * element w of tensor i with gradient g = grad * *grad_scale (NULL: 1):

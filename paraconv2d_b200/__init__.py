@@ -23,17 +23,21 @@ from .layers import (  # noqa: F401
     CausalConv,
     Dropout,
     GroupNorm,
+    LinearAttention,
     SSMScan,
     causal_conv,
     causal_conv_step,
     dropout,
     group_norm,
+    linear_attention,
+    linear_attention_step,
     ssm_scan,
     ssm_scan_step,
 )
 from .optim import ParaboloidAdamW, ParaboloidSGD, adamw_new_state, adamw_state_values, adamw_step  # noqa: F401
 
 __all__ = ["ParaConv2d", "ParaConv2dFunction", "spotlightinit", "pnnconvert", "ptparaconv2d", "cabi", "set_algo",
-           "CausalConv", "Dropout", "SSMScan", "causal_conv", "causal_conv_step", "dropout", "GroupNorm", "group_norm", "ssm_scan", "ssm_scan_step",
+           "CausalConv", "Dropout", "SSMScan", "causal_conv", "causal_conv_step", "dropout", "GroupNorm", "group_norm",
+           "LinearAttention", "linear_attention", "linear_attention_step", "ssm_scan", "ssm_scan_step",
            "ParaboloidAdamW", "ParaboloidSGD", "adamw_new_state", "adamw_state_values", "adamw_step",
            "load_op_library", "PC2D_ALGO_AUTO", "PC2D_ALGO_SIMT", "PC2D_ALGO_TC"]

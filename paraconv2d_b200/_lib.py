@@ -116,6 +116,11 @@ def cabi() -> ctypes.CDLL:
             "pc2d_group_norm_workspace_size": ([I] * 7, S),
             "pc2d_group_norm_forward": ([I] * 3 + [P] * 4 + [I] * 4 + [D, I, P, P, P, S, P], I),
             "pc2d_group_norm_backward": ([I] * 3 + [P] * 6 + [I] * 5 + [P] * 4 + [S, P], I),
+            "pc2d_linear_attention_states_size": ([I] * 6, S),
+            "pc2d_linear_attention_workspace_size": ([I] * 8, S),
+            "pc2d_linear_attention_forward": ([I] + [P] * 4 + [I, P, P] + [I] * 6 + [D] + [P] * 4 + [S, P], I),
+            "pc2d_linear_attention_backward": ([I] + [P] * 6 + [I, P, P] + [I] * 6 + [D] + [P] * 6 + [S, P], I),
+            "pc2d_linear_attention_step": ([I] + [P] * 4 + [I, P, P] + [I] * 6 + [D, P, P], I),
             "pc2d_adamw_workspace_size": ([], S),
             "pc2d_adamw_step": ([I, ctypes.POINTER(AdamWTensor), I, P, P] + [D] * 5 + [P, L, P, S, P], I),
             "pc2d_adamw_state_values": ([I, ctypes.POINTER(AdamWTensor), I, ctypes.POINTER(P), ctypes.POINTER(P), P],

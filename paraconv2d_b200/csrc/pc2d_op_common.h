@@ -147,6 +147,12 @@ auto below_autograd(const char *name) {
     return handle;                                                                                     \
   }())
 
+// A step changes its state in place: there is no gradient.
+inline void no_step_grad(const char *what, bool needs) {
+  TORCH_CHECK(!needs, "paraconv2d_b200.", what, " moves its state on in place and has no backward pass: call it under "
+              "torch.no_grad(), or use the operator over whole sequences");
+}
+
 inline OptTensor optional_of(const Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
 // Runs a backward pass without recording it; where the caller asked for a graph

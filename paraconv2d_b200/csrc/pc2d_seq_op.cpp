@@ -379,12 +379,6 @@ std::vector<Tensor> ssm_scan_forward_autograd(const Tensor &u, const Tensor &del
                                            final_state, checkpoints);
 }
 
-// A step changes its state in place: there is no gradient.
-void no_step_grad(const char *what, bool needs) {
-  TORCH_CHECK(!needs, "paraconv2d_b200.", what, " moves its state on in place and has no backward pass: call it under "
-              "torch.no_grad(), or use the operator over whole sequences");
-}
-
 Tensor causal_conv_step_autograd(const Tensor &input, const Tensor &state, const Tensor &weight, const OptTensor &bias,
                                  const OptTensor &slots, bool silu) {
   no_forward_mode("causal_conv_step", {&input, &state, &weight}, {&bias});

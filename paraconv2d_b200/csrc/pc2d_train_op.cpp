@@ -1,5 +1,5 @@
-// torch.ops.paraconv2d_b200: group norm and the AdamW step over many tensors,
-// on top of the C ABI of libpc2d_sm100.so.  Argument checks, streams, scratch
+// torch.ops.paraconv2d_b200: group norm, linear attention and the AdamW step
+// over many tensors, on top of the C ABI of libpc2d_sm100.so.  Argument checks, streams, scratch
 // and gradients as for the sequence operators.
 #include <algorithm>
 
@@ -300,6 +300,173 @@ std::vector<Tensor> group_norm_forward_autograd(const Tensor &input, const OptTe
   return PC2D_BELOW(group_norm_forward).call(input, weight, bias, lengths, groups, eps, silu, keep_stats);
 }
 
+// ---------------------------------------------------------- linear attention
+
+struct AttentionCall {
+  Call call;
+  int dt, batch, heads, groups, length, dk, dv;
+  bool per_token;
+  Tensor q, k, v, decay, lengths;
+};
+
+AttentionCall attention_call(const char *what, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &decay,
+                             const OptTensor &lengths) {
+  AttentionCall c{{what, v.device()}};
+  const auto type = v.scalar_type();
+  c.dt = seq_dtype_code(v, what);
+  TORCH_CHECK(v.dim() == 4, what, ": v must be [batch, heads, values, length], got ", v.sizes());
+  TORCH_CHECK(q.dim() == 4, what, ": q must be [batch, groups, keys, length], got ", q.sizes());
+  c.batch = as_int(v.size(0), what, "batch");
+  c.heads = as_int(v.size(1), what, "heads");
+  c.dv = as_int(v.size(2), what, "values");
+  c.length = as_int(v.size(3), what, "length");
+  c.groups = as_int(q.size(1), what, "groups");
+  c.dk = as_int(q.size(2), what, "keys");
+  c.q = c.call.need(q, "q", type, {c.batch, c.groups, c.dk, c.length});
+  c.k = c.call.need(k, "k", type, {c.batch, c.groups, c.dk, c.length});
+  c.v = dense(v);
+  c.per_token = decay.dim() != 1;
+  c.decay = c.per_token ? c.call.need(decay, "log_decay", at::kFloat, {c.batch, c.heads, c.length})
+                        : c.call.need(decay, "log_decay", at::kFloat, {c.heads});
+  c.lengths = c.call.maybe(lengths, "lengths", at::kInt, {c.batch});
+  return c;
+}
+
+std::vector<Tensor> linear_attention_forward_cuda(const Tensor &q, const Tensor &k, const Tensor &v,
+                                                  const Tensor &log_decay, const OptTensor &initial_,
+                                                  const OptTensor &lengths, double scale, bool final_state,
+                                                  bool keep_states) {
+  const c10::cuda::CUDAGuard guard(v.device());
+  const AttentionCall c = attention_call("paraconv2d_b200.linear_attention_forward", q, k, v, log_decay, lengths);
+  const Tensor initial = c.call.maybe(initial_, "initial_state", at::kFloat, {c.batch, c.heads, c.dk, c.dv});
+  Tensor out = at::empty(c.v.sizes(), c.v.options());
+  const auto fopts = c.decay.options();
+  Tensor last = at::empty(final_state ? at::IntArrayRef({c.batch, c.heads, c.dk, c.dv}) : at::IntArrayRef({0}), fopts);
+  const size_t size =
+      keep_states ? pc2d_linear_attention_states_size(c.dt, c.batch, c.heads, c.length, c.dk, c.dv) : 0;
+  Tensor states = at::empty({(int64_t)(size / 4)}, fopts);
+  const size_t bytes =
+      pc2d_linear_attention_workspace_size(c.dt, c.batch, c.heads, c.groups, c.length, c.dk, c.dv, 0);
+  const Tensor ws = workspace(bytes, c.v);
+  check_status(pc2d_linear_attention_forward(c.dt, ptr(c.q), ptr(c.k), ptr(c.v), ptr<float>(c.decay), c.per_token,
+                                             ptr<float>(initial), ptr<int>(c.lengths), c.batch, c.heads, c.groups,
+                                             c.length, c.dk, c.dv, scale, ptr(out),
+                                             final_state ? ptr<float>(last) : nullptr,
+                                             size ? ptr<float>(states) : nullptr, ptr(ws), bytes, stream_now()),
+               c.call.what);
+  return {out, last, states};
+}
+
+std::vector<Tensor> linear_attention_backward_cuda(const Tensor &grad_, const OptTensor &grad_final_, const Tensor &q,
+                                                   const Tensor &k, const Tensor &v, const Tensor &log_decay,
+                                                   const Tensor &states_, const OptTensor &lengths, double scale,
+                                                   bool initial_grad) {
+  const c10::cuda::CUDAGuard guard(v.device());
+  const AttentionCall c = attention_call("paraconv2d_b200.linear_attention_backward", q, k, v, log_decay, lengths);
+  const Tensor grad = c.call.need(grad_, "grad", v.scalar_type(), v.sizes());
+  const Tensor grad_final = c.call.maybe(grad_final_, "grad_final", at::kFloat, {c.batch, c.heads, c.dk, c.dv});
+  const int64_t kept =
+      (int64_t)(pc2d_linear_attention_states_size(c.dt, c.batch, c.heads, c.length, c.dk, c.dv) / 4);
+  const Tensor states = c.call.need(states_, "states", at::kFloat, {kept});
+  auto like = [](const Tensor &t) { return at::empty(t.sizes(), t.options()); };
+  Tensor dq = like(c.q), dk = like(c.k), dv = like(c.v), dg = like(c.decay);
+  Tensor dinit = initial_grad ? at::empty({c.batch, c.heads, c.dk, c.dv}, c.decay.options()) : Tensor();
+  const size_t bytes =
+      pc2d_linear_attention_workspace_size(c.dt, c.batch, c.heads, c.groups, c.length, c.dk, c.dv, 1);
+  const Tensor ws = workspace(bytes, c.v);
+  check_status(pc2d_linear_attention_backward(c.dt, ptr(grad), ptr<float>(grad_final), ptr(c.q), ptr(c.k), ptr(c.v),
+                                              ptr<float>(c.decay), c.per_token, ptr<float>(states),
+                                              ptr<int>(c.lengths), c.batch, c.heads, c.groups, c.length, c.dk, c.dv,
+                                              scale, ptr(dq), ptr(dk), ptr(dv), ptr<float>(dg), ptr<float>(dinit),
+                                              ptr(ws), bytes, stream_now()),
+               c.call.what);
+  return {dq, dk, dv, dg, dinit.defined() ? dinit : at::empty({0}, c.decay.options())};
+}
+
+Tensor linear_attention_step_cuda(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &log_decay,
+                                  const Tensor &state, const OptTensor &slots_, double scale) {
+  const Call call{"paraconv2d_b200.linear_attention_step", v_.device()};
+  const c10::cuda::CUDAGuard guard(v_.device());
+  const auto type = v_.scalar_type();
+  const int dt = seq_dtype_code(v_, call.what);
+  TORCH_CHECK(v_.dim() == 3, call.what, ": v must be [batch, heads, values], got ", v_.sizes());
+  TORCH_CHECK(q_.dim() == 3, call.what, ": q must be [batch, groups, keys], got ", q_.sizes());
+  const int batch = as_int(v_.size(0), call.what, "batch"), heads = as_int(v_.size(1), call.what, "heads");
+  const int dv = as_int(v_.size(2), call.what, "values"), groups = as_int(q_.size(1), call.what, "groups");
+  const int dk = as_int(q_.size(2), call.what, "keys");
+  TORCH_CHECK(state.dim() == 4, call.what, ": state must be [places, ", heads, ", ", dk, ", ", dv, "], got ",
+              state.sizes());
+  const int places = as_int(state.size(0), call.what, "places");
+  call.in_place(state, "state", at::kFloat, {places, heads, dk, dv});
+  const Tensor q = call.need(q_, "q", type, {batch, groups, dk}), k = call.need(k_, "k", type, {batch, groups, dk});
+  const Tensor v = dense(v_);
+  const bool per_row = log_decay.dim() != 1;
+  const Tensor decay = per_row ? call.need(log_decay, "log_decay", at::kFloat, {batch, heads})
+                               : call.need(log_decay, "log_decay", at::kFloat, {heads});
+  const Tensor slots = call.maybe(slots_, "slots", at::kInt, {batch});
+  call.apart(state, {&q, &k, &v, &decay, &slots});
+  Tensor out = at::empty({batch, heads, dv}, v.options());
+  check_status(pc2d_linear_attention_step(dt, ptr(q), ptr(k), ptr(v), ptr<float>(decay), per_row, ptr<float>(state),
+                                          ptr<int>(slots), batch, places, heads, groups, dk, dv, scale, ptr(out),
+                                          stream_now()),
+               call.what);
+  changed(state);
+  return out;
+}
+
+struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &q_, const Tensor &k_, const Tensor &v_,
+                               const Tensor &log_decay, const OptTensor &initial, const OptTensor &lengths, double scale,
+                               bool final_state) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor q = q_.contiguous(), k = k_.contiguous(), v = v_.contiguous(), g = log_decay.contiguous();
+    auto outs = PC2D_BELOW(linear_attention_forward).call(q, k, v, g, initial, lengths, scale, final_state, true);
+    ctx->save_for_backward({q, k, v, g, outs[2], lengths.value_or(Tensor())});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["initial"] = initial.has_value() && initial->defined() && initial->requires_grad();
+    ctx->set_materialize_grads(false);
+    outs.pop_back();
+    if (!final_state) outs.pop_back();
+    return outs;
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+    return once("linear_attention", [&]() -> variable_list {
+      const auto s = ctx->get_saved_variables();
+      const Tensor grad = grads[0].defined() ? grads[0] : at::zeros_like(s[2]);
+      const bool initial = ctx->saved_data["initial"].toBool();
+      const auto g = PC2D_BELOW(linear_attention_backward)
+                         .call(grad, grads.size() > 1 ? optional_of(grads[1]) : OptTensor(), s[0], s[1], s[2], s[3],
+                               s[4], optional_of(s[5]), ctx->saved_data["scale"].toDouble(), initial);
+      return {g[0], g[1], g[2], g[3], initial ? g[4] : Tensor(), Tensor(), Tensor(), Tensor()};
+    });
+  }
+};
+
+// With gradients the states are the graph's own: the third result is empty.
+std::vector<Tensor> linear_attention_forward_autograd(const Tensor &q, const Tensor &k, const Tensor &v,
+                                                      const Tensor &log_decay, const OptTensor &initial,
+                                                      const OptTensor &lengths, double scale, bool final_state,
+                                                      bool keep_states) {
+  no_forward_mode("linear_attention", {&q, &k, &v, &log_decay}, {&initial});
+  check_cuda(v, "linear_attention");
+  if (needs_grad({&q, &k, &v, &log_decay}, {&initial})) {
+    auto outs = AttentionFunction::apply(q, k, v, log_decay, initial, lengths, scale, final_state);
+    while (outs.size() < 3) outs.push_back(at::empty({0}, log_decay.options()));
+    return outs;
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return PC2D_BELOW(linear_attention_forward).call(q, k, v, log_decay, initial, lengths, scale, final_state, keep_states);
+}
+
+Tensor linear_attention_step_autograd(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
+                                      const Tensor &state, const OptTensor &slots, double scale) {
+  no_forward_mode("linear_attention_step", {&q, &k, &v, &log_decay, &state}, {});
+  no_step_grad("linear_attention_step", needs_grad({&q, &k, &v, &log_decay, &state}, {}));
+  check_cuda(v, "linear_attention_step");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return PC2D_BELOW(linear_attention_step).call(q, k, v, log_decay, state, slots, scale);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(paraconv2d_b200, m) {
@@ -313,6 +480,15 @@ TORCH_LIBRARY_FRAGMENT(paraconv2d_b200, m) {
   m.def(
       "group_norm_backward(Tensor grad, Tensor input, Tensor? weight, Tensor? bias, Tensor? lengths, Tensor stats, "
       "int groups, bool silu) -> Tensor[]");
+  m.def(
+      "linear_attention_forward(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? initial_state, Tensor? lengths, "
+      "float scale, bool final_state, bool keep_states) -> Tensor[]");
+  m.def(
+      "linear_attention_backward(Tensor grad, Tensor? grad_final, Tensor q, Tensor k, Tensor v, Tensor log_decay, "
+      "Tensor states, Tensor? lengths, float scale, bool initial_grad) -> Tensor[]");
+  m.def(
+      "linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor(a!) state, Tensor? slots, float "
+      "scale) -> Tensor");
   m.def("adamw_state_values(Tensor[] exp_avgs, Tensor[] exp_avg_sqs, Tensor[] scales, ScalarType dtype) -> Tensor[]");
 }
 
@@ -321,8 +497,13 @@ TORCH_LIBRARY_IMPL(paraconv2d_b200, CUDA, m) {
   m.impl("adamw_state_values", adamw_state_values_cuda);
   m.impl("group_norm_forward", group_norm_forward_cuda);
   m.impl("group_norm_backward", group_norm_backward_cuda);
+  m.impl("linear_attention_forward", linear_attention_forward_cuda);
+  m.impl("linear_attention_backward", linear_attention_backward_cuda);
+  m.impl("linear_attention_step", linear_attention_step_cuda);
 }
 
 TORCH_LIBRARY_IMPL(paraconv2d_b200, Autograd, m) {
   m.impl("group_norm_forward", group_norm_forward_autograd);
+  m.impl("linear_attention_forward", linear_attention_forward_autograd);
+  m.impl("linear_attention_step", linear_attention_step_autograd);
 }

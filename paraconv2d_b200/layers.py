@@ -47,6 +47,8 @@ class _ops:
     causal_conv_step = torch.ops.paraconv2d_b200.causal_conv_step.default
     ssm_scan_forward = torch.ops.paraconv2d_b200.ssm_scan_forward.default
     ssm_scan_step = torch.ops.paraconv2d_b200.ssm_scan_step.default
+    linear_attention_forward = torch.ops.paraconv2d_b200.linear_attention_forward.default
+    linear_attention_step = torch.ops.paraconv2d_b200.linear_attention_step.default
     group_norm_forward = torch.ops.paraconv2d_b200.group_norm_forward.default
 
 
@@ -243,6 +245,79 @@ class SSMScan(nn.Module):
 
     def extra_repr(self) -> str:
         return f"channels={self.channels}, states={self.states}"
+
+
+# ----------------------------------------------------------- linear attention
+
+def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, scale: Optional[float] = None,
+                     initial_state: Optional[Tensor] = None, lengths: Optional[Tensor] = None,
+                     return_final_state: bool = False):
+    """The recurrence, for each head::
+
+        S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T        (keys x values)
+        out_t = scale S_t^T q_t
+
+    ``q`` and ``k``: [batch, groups, keys, length], each group for
+    heads/groups neighbouring heads; ``v`` and the result: [batch, heads,
+    values, length]; of one type.  ``log_decay``: float32, [heads] or [batch,
+    heads, length], at most 0 in use (-inf forgets all before a token).
+    ``scale``: keys^-0.5 if None.  States [batch, heads, keys, values] are
+    float32.  1 to 128 keys and values; up to 2^20 heads of rows and 2^30
+    tokens.
+
+    ``initial_state`` (None: 0), ``lengths`` and ``return_final_state`` as for
+    :func:`causal_conv`.  Gradients reach every tensor but ``lengths``.  For
+    the backward pass the forward one keeps the states of every 64th token
+    (every 32nd in float32 and float16), keys*values/16 bytes (/8) per head and
+    token, and the backward pass takes as much again.
+    """
+    scale = q.shape[-2] ** -0.5 if scale is None else float(scale)
+    outs = _ops.linear_attention_forward(q, k, v, log_decay, initial_state, lengths, scale, bool(return_final_state),
+                                         False)
+    return (outs[0], outs[1]) if return_final_state else outs[0]
+
+
+def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor,
+                          scale: Optional[float] = None, slots: Optional[Tensor] = None) -> Tensor:
+    """:func:`linear_attention` of one token for each row: ``q``, ``k`` [batch,
+    groups, keys], ``v`` [batch, heads, values], ``log_decay`` [heads] or
+    [batch, heads]; ``state`` float32 [places, heads, keys, values] is moved on
+    in place, with ``slots`` as for :func:`causal_conv_step`."""
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    return _ops.linear_attention_step(q, k, v, log_decay, state, slots, scale)
+
+
+class LinearAttention(nn.Module):
+    """:func:`linear_attention` with a decay for each head as its parameter
+    ``rate`` [heads] (log_decay = -exp(rate)): memories of 32 to 4096 tokens
+    over the heads at first.  q, k and v come with each call: projections of
+    the input make them.  Where decays come with the tokens too, call the
+    function."""
+
+    def __init__(self, heads: int, keys: int, values: int, scale: Optional[float] = None, device=None):
+        super().__init__()
+        if heads < 1 or not 1 <= keys <= 128 or not 1 <= values <= 128:
+            raise ValueError(f"heads must be positive, keys and values 1 to 128, got {heads}, {keys} and {values}")
+        self.heads, self.keys, self.values, self.scale = heads, keys, values, scale
+        spread = torch.linspace(5, 12, heads, device=device, dtype=torch.float32)
+        self.rate = nn.Parameter(torch.log(-torch.log1p(-torch.exp2(-spread))))
+
+    def new_state(self, places: int) -> Tensor:
+        """Zero states for ``places`` requests."""
+        return torch.zeros(places, self.heads, self.keys, self.values, device=self.rate.device)
+
+    def _log_decay(self):
+        return -torch.exp(self.rate.float())  # float32 also in a module that was moved to a 16-bit type
+
+    def forward(self, q, k, v, initial_state=None, lengths=None, return_final_state=False):
+        return linear_attention(q, k, v, self._log_decay(), self.scale, initial_state, lengths, return_final_state)
+
+    @torch.no_grad()
+    def step(self, q, k, v, state, slots=None):
+        return linear_attention_step(q, k, v, self._log_decay(), state, self.scale, slots)
+
+    def extra_repr(self) -> str:
+        return f"heads={self.heads}, keys={self.keys}, values={self.values}"
 
 
 # ----------------------------------------------------------------- group norm

@@ -159,3 +159,56 @@ def norm(x, groups, w=None, b=None, eps=1e-5, silu=False, lengths=None, grad=Non
             if k in d:
                 d[k] = d[k].view(shape)
     return v, m
+
+
+# ----------------------------------------------------------- linear attention
+
+def attention(q, k, v, g, scale=None, init=None, lengths=None, grad=None, grad_final=None, chunk=64):
+    """One token at a time: values and magnitudes of out, final and (with
+    grad) dq, dk, dv, dg (for each token) and dinit."""
+    f64 = lambda t: None if t is None else t.detach().cpu().double()  # noqa: E731
+    q, k, v, g, init, grad, grad_final = (f64(t) for t in (q, k, v, g, init, grad, grad_final))
+    B, H, dv, L = v.shape
+    G, dk = q.shape[1:3]
+    scale = dk ** -0.5 if scale is None else scale
+    if g.dim() == 1:
+        g = g[:, None].expand(B, H, L)
+    owner = torch.arange(H) // (H // G)
+    z = lambda *s: torch.zeros(*s, dtype=torch.float64)  # noqa: E731
+    vals = {"out": z(B, H, dv, L), "final": z(B, H, dk, dv)}
+    mags = {"out": z(B, H, dv, L), "final": z(B, H, dk, dv)}
+    if grad is not None:
+        for d in (vals, mags):
+            d.update(dq=z(B, G, dk, L), dk=z(B, G, dk, L), dv=z(B, H, dv, L), dg=z(B, H, L), dinit=z(B, H, dk, dv))
+    for b in range(B):
+        n = L if lengths is None else min(max(int(lengths[b]), 0), L)
+        for absolute, d in ((False, vals), (True, mags)):
+            f = torch.abs if absolute else (lambda t: t)
+            Q, K = f(q[b, owner]), f(k[b, owner])
+            V = f(v[b])
+            S = f(init[b]) if init is not None else z(H, dk, dv)
+            states = [S]
+            for t in range(n):
+                S = torch.exp(g[b, :, t])[:, None, None] * S + K[:, :, t, None] * V[:, None, :, t]
+                states.append(S)
+                d["out"][b, :, :, t] = f(torch.tensor(scale, dtype=torch.float64)) * torch.einsum("hk,hkv->hv", Q[:, :, t], S)
+            d["final"][b] = S
+            if grad is None:
+                continue
+            s_ = abs(scale) if absolute else scale
+            R = f(grad_final[b]) if grad_final is not None else z(H, dk, dv)
+            O = f(grad[b])
+            for t in reversed(range(n)):
+                D = R + s_ * Q[:, :, t, None] * O[:, None, :, t]
+                a = torch.exp(g[b, :, t])[:, None, None]
+                dq = s_ * torch.einsum("hkv,hv->hk", states[t + 1], O[:, :, t])
+                d["dq"][b, :, :, t].index_add_(0, owner, dq)
+                d["dk"][b, :, :, t].index_add_(0, owner, torch.einsum("hkv,hv->hk", D, V[:, :, t]))
+                d["dv"][b, :, :, t] = torch.einsum("hkv,hk->hv", D, K[:, :, t])
+                d["dg"][b, :, t] += (a * states[t] * D).sum((1, 2))
+                if absolute:  # pairs on one side of a token of the chunk are added and taken away again
+                    c = t // chunk * chunk
+                    d["dg"][b, :, c:min(c + chunk, n)] += (Q[:, :, t] * dq).sum(1)[:, None]
+                R = a * D
+            d["dinit"][b] = R
+    return vals, mags
