@@ -343,7 +343,7 @@ int pc2d_group_norm_backward(int dtype, int wdtype, int channels_last, const voi
  * tokens of a head (every 32 in float32 and float16).  The backward pass gives all gradients
  * (grad_final and initialgrad may be NULL), decaygrad in the decays' shape.
  * Arrays need their elements' alignment (16 bytes and lengths that are
- * multiples of 8 are faster).  pc2d_linear_attention_step takes one token per
+ * multiples of 8 are faster), `states` 16 bytes.  pc2d_linear_attention_step takes one token per
  * row (q, k [batch][groups][dk], v [batch][heads][dv], log_decay [heads] or
  * with decay_per_row [batch][heads]) and moves its state [places][heads][dk]
  * [dv] (16-byte aligned) on in place; slots as for pc2d_causal_conv_step. */

@@ -67,28 +67,27 @@ struct Items {
 
 static_assert(sizeof(Items<kMany>) <= 32000 && sizeof(Items<kFew>) <= 4000, "a launch's parameters");
 
-// What every element needs of the step, made by one thread.
+// What every element needs of the step, made by one thread.  (In 32 bits: the
+// GPU's 64-bit arithmetic is so slow that its latency showed in every block.)
 struct Coef {
-  double lr, lr1;  // lr, lr / (1 - beta1^t)
-  float root;      // 1 / sqrt(1 - beta2^t)
+  float lr, lr1, root;  // lr, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
   int pad;
   int64_t t;
 };
 
 struct Betas {
-  float b1, c1, b2, c2, eps;
-  double wd;
+  float b1, c1, b2, c2, eps, wd;
   uint64_t seed;
 };
 
-__global__ void adamw_coef_kernel(int64_t *step, const float *lr_device, double lr, double beta1, double beta2,
-                                  Coef *coef) {
+// log1, log2: logarithms of the betas (1 - beta^t by expm1, which keeps its digits where it is small)
+__global__ void adamw_coef_kernel(int64_t *step, const float *lr_device, float lr, float log1, float log2, Coef *coef) {
   const int64_t t = *step + 1;
   *step = t;
   if (lr_device) lr = *lr_device;
   coef->lr = lr;
-  coef->lr1 = lr / (1.0 - pow(beta1, (double)t));
-  coef->root = (float)rsqrt(1.0 - pow(beta2, (double)t));
+  coef->lr1 = lr / -expm1f((float)t * log1);
+  coef->root = rsqrtf(-expm1f((float)t * log2));
   coef->t = t;
 }
 
@@ -196,12 +195,12 @@ __device__ __forceinline__ void put(const float (&x)[N], T *p, bool whole, int l
 }
 
 __device__ __forceinline__ Rates rates_of(const Item &it, const Coef *coef, const float *grad_scale, const Betas &b) {
-  const double lr = coef->lr, lr1 = coef->lr1;
+  const float lr = coef->lr, lr1 = coef->lr1;
   Rates r;
-  r.keep_first = (float)(1.0 - lr * it.rate_first * b.wd * it.decay);
-  r.keep_rest = (float)(1.0 - lr * it.rate_rest * b.wd * it.decay);
-  r.lr_first = (float)(lr1 * it.rate_first);
-  r.lr_rest = (float)(lr1 * it.rate_rest);
+  r.keep_first = 1.f - lr * it.rate_first * b.wd * it.decay;
+  r.keep_rest = 1.f - lr * it.rate_rest * b.wd * it.decay;
+  r.lr_first = lr1 * it.rate_first;
+  r.lr_rest = lr1 * it.rate_rest;
   r.root = coef->root;
   r.scale = grad_scale ? *grad_scale : 1.f;
   r.split = it.split;
@@ -483,9 +482,9 @@ extern "C" int pc2d_adamw_step(int state_bits, const pc2d_adamw_tensor *tensors,
     return st;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   Coef *coef = static_cast<Coef *>(workspace);
-  adamw_coef_kernel<<<1, 1, 0, s>>>(step, lr_device, lr, beta1, beta2, coef);
+  adamw_coef_kernel<<<1, 1, 0, s>>>(step, lr_device, (float)lr, (float)log(beta1), (float)log(beta2), coef);
   PC2D_LAUNCH_CHECK("adamw_coef_kernel");
-  const Betas b{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, weight_decay,
+  const Betas b{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)weight_decay,
                 (uint64_t)seed};
   const int F = PC2D_DTYPE_F32, H = PC2D_DTYPE_F16, B = PC2D_DTYPE_BF16;
   if ((st = launch_group<float, float>(state_bits, tensors, count, F, F, coef, grad_scale, b, s)) != PC2D_OK ||

@@ -10,10 +10,11 @@
 //   o_t = scale (exp(b_t) S^T q_t + sum_(s <= t) exp(b_t - b_s) (q_t k_s) v_s)
 //   S' = exp(b_C) S + sum_s exp(b_C - b_s) k_s v_s^T
 //
-// which are matrix products.  The b are summed in 64 bits and kept as pairs of
-// 32-bit numbers, so that a difference b_t - b_s is off by a rounding of itself
-// and not of the b, which may be far larger.  A decay to nothing (g = -inf)
-// counts as -kNothing, whose exponential is 0 too.
+// which are matrix products.  The b are kept as pairs of 32-bit numbers, so that
+// a difference b_t - b_s is off by a rounding of itself and not of the b, which
+// may be far larger.  (In 64 bits, which are slow on this GPU, the chain of sums
+// and an exponential took longer than a chunk's products.)  A decay to nothing
+// (g = -inf) counts as -kNothing, whose exponential is 0 too.
 //
 // Gradients, with D_t that of S_t and do_t that of o_t:
 //
@@ -39,7 +40,7 @@ namespace pc2d {
 namespace {
 
 constexpr int kMaxDim = 128;
-constexpr double kNothing = 1e5;  // in powers of two: exp2(-1e5) is 0 in 32 bits
+constexpr float kNothing = 1e5f;  // in powers of two: exp2(-1e5) is 0 in 32 bits
 
 // How many planes the operands of a type have: its inputs; scores and states
 // that meet inputs in the outputs; the decayed values in the state's update,
@@ -50,15 +51,15 @@ template <typename T>
 struct Planes;
 template <>
 struct Planes<__nv_bfloat16> {
-  static constexpr int in = 1, out = 1, update = 3, back = 2, chunk = 64, stages = 2;
+  static constexpr int in = 1, out = 1, update = 3, back = 3, chunk = 64;
 };
 template <>
 struct Planes<__half> {
-  static constexpr int in = 2, out = 2, update = 3, back = 2, chunk = 32, stages = 1;
+  static constexpr int in = 2, out = 2, update = 3, back = 3, chunk = 32;
 };
 template <>
 struct Planes<float> {
-  static constexpr int in = 3, out = 3, update = 3, back = 3, chunk = 32, stages = 1;
+  static constexpr int in = 3, out = 3, update = 3, back = 3, chunk = 32;
 };
 
 struct Args {
@@ -72,7 +73,7 @@ struct Args {
   float *states;        // [batch][heads][chunks][dk][dv]: S before each chunk
   float *dstates;       // likewise: D behind each chunk
   float *starts;        // [batch][heads][segments][dk][dv]: of segments, then their starts
-  double *decays;       // [batch][heads][segments]: log2 of a segment's decay
+  float2 *decays;       // [batch][heads][segments]: log2 of a segment's decay, as a pair
   void *dq, *dk_, *dv_;
   float *dq_heads, *dk_heads;  // [batch][heads][dk][length] where heads share queries and keys
   float *dg;            // [batch][heads][length]
@@ -117,17 +118,19 @@ __device__ __forceinline__ uint32_t pair(float lo, float hi) {
 __device__ __forceinline__ float2 unpair(uint32_t p) {
   return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
 }
-// Two numbers as N planes.  Values that are not finite stay in the first one.
+// Two numbers as N planes: upper halves, of 8 bits of mantissa, and the rests'
+// in turn; the last one is rounded.  (The rest of an infinity is NaN.)
 template <int N>
 __device__ __forceinline__ void split(float x, float y, uint32_t (&p)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    p[i] = pair(x, y);
-    if (i + 1 < N) {
-      const float2 r = unpair(p[i]);
-      // (an infinity's rest would be NaN)
-      x = fabsf(r.x) <= 3.4e38f ? x - r.x : 0.f;
-      y = fabsf(r.y) <= 3.4e38f ? y - r.y : 0.f;
+    if (i + 1 == N) {
+      p[i] = pair(x, y);
+    } else {
+      const uint32_t u = __float_as_uint(x), v = __float_as_uint(y);
+      p[i] = __byte_perm(u, v, 0x7632);
+      x -= __uint_as_float(u & 0xffff0000u);
+      y -= __uint_as_float(v & 0xffff0000u);
     }
   }
 }
@@ -261,14 +264,43 @@ __device__ __forceinline__ void fill(const Tile &t, const T *src, int rows, int 
   }
 }
 
+// A number as the sum of two, the second below half a unit of the first.
+__device__ __forceinline__ float2 two_sum(float a, float b) {
+  const float s = a + b, t = s - a;
+  return make_float2(s, (a - (s - t)) + (b - t));
+}
+__device__ __forceinline__ float2 two_sum(float2 a, float2 b) {
+  const float2 s = two_sum(a.x, b.x);
+  const float low = s.y + (a.y + b.y), hi = s.x + low;
+  return make_float2(hi, low - (hi - s.x));
+}
+// 2^x of a pair, off by little more than half a unit: 2^n (1 + y + y^2 q(y)),
+// y = ln 2 (x - n) at most 0.35, by the exponential's series, its last two sums
+// with their roundings.  A state passes through this factor at every chunk.
+__device__ __forceinline__ float exp2_pair(float2 x) {
+  const float n = rintf(x.x), f = x.x - n;
+  constexpr float ln2 = 0.693147182464599609f, ln2_low = -1.904654323148236e-9f;
+  const float y = f * ln2, y_low = fmaf(f, ln2, -y) + fmaf(f, ln2_low, x.y * ln2);
+  float q = 2.48015873e-5f;  // 1/8!
+  q = fmaf(q, y, 1.98412698e-4f);
+  q = fmaf(q, y, 1.38888889e-3f);
+  q = fmaf(q, y, 8.33333333e-3f);
+  q = fmaf(q, y, 4.16666667e-2f);
+  q = fmaf(q, y, 1.66666667e-1f);
+  q = fmaf(q, y, 0.5f);
+  const float2 s = two_sum(y, fmaf(y * y, q, y_low));
+  const float2 r = two_sum(1.f, s.x);
+  return ldexpf(r.x + (r.y + s.y), (int)fminf(fmaxf(n, -1000.f), 1000.f));
+}
+
 // What a chunk's decays come to, in powers of two.
 template <int C>
 struct Decays {
-  float hi[C], lo[C];  // b_t as a pair
-  float begin[C];      // exp2(b_t)
-  float end[C];        // exp2(b_C - b_t)
+  float hi[C], lo[C];         // b_t as a pair
+  alignas(8) float begin[C];  // exp2(b_t)
+  alignas(8) float end[C];    // exp2(b_C - b_t)
   float whole;         // exp2(b_C)
-  double sum;          // b_C
+  float2 sum;          // b_C
   // log2 of exp(b_t - b_s)
   __device__ __forceinline__ float between(int t, int s) const { return (hi[t] - hi[s]) + (lo[t] - lo[s]); }
 };
@@ -286,31 +318,36 @@ struct DecayLoad {
   }
   __device__ __forceinline__ void finish(Decays<C> &d) const {
     const int lane = threadIdx.x & 31;
-    double b[C / 32], sum = 0.0;
+    constexpr float log2e = 1.44269502162933349609f, log2e_low = 1.925963033500811e-8f;
+    float2 b[C / 32], upto;
 #pragma unroll
     for (int i = 0; i < C / 32; ++i) {
-      const double x = (double)v[i] * 1.4426950408889634074;
-      sum += x < -kNothing ? -kNothing : x;  // (a NaN stays one)
-      b[i] = sum;
+      const float x = v[i] * log2e;
+      // (a NaN stays one)
+      const float2 at = x < -kNothing ? make_float2(-kNothing, 0.f)
+                                      : make_float2(x, fmaf(v[i], log2e_low, fmaf(v[i], log2e, -x)));
+      b[i] = upto = i ? two_sum(upto, at) : at;
     }
-    double upto = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const double x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
+      const float2 x = make_float2(__shfl_up_sync(0xffffffffu, upto.x, o), __shfl_up_sync(0xffffffffu, upto.y, o));
+      if (lane >= o) upto = two_sum(x, upto);
     }
-    const double whole = __shfl_sync(0xffffffffu, upto, 31);
+    const float2 whole =
+        make_float2(__shfl_sync(0xffffffffu, upto.x, 31), __shfl_sync(0xffffffffu, upto.y, 31));
+    float2 before = make_float2(__shfl_up_sync(0xffffffffu, upto.x, 1), __shfl_up_sync(0xffffffffu, upto.y, 1));
+    if (lane == 0) before = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < C / 32; ++i) {
       const int t = lane * (C / 32) + i;
-      const double at = upto - sum + b[i];
-      d.hi[t] = (float)at;
-      d.lo[t] = (float)(at - d.hi[t]);
-      d.begin[t] = exp2_fast((float)at);
-      d.end[t] = exp2_fast((float)(whole - at));
+      const float2 at = two_sum(before, b[i]);
+      d.hi[t] = at.x;
+      d.lo[t] = at.y;
+      d.begin[t] = exp2_pair(at);
+      d.end[t] = exp2_pair(two_sum(whole, make_float2(-at.x, -at.y)));
     }
     if (lane == 0) {
-      d.whole = exp2_fast((float)whole);
+      d.whole = exp2_pair(whole);
       d.sum = whole;
     }
   }
@@ -336,10 +373,14 @@ enum Mode { kOutput, kForwardState, kBackwardState };
 // the state that a segment adds.  kBackwardState: D, from the last chunk to
 // the first, from queries and the outputs' gradients in the places of keys and
 // values; with `dstates` those behind each chunk, else what a segment adds.
+// The chain of dependent steps that a chunk takes is long, so what counts is
+// the warps that an SM has to change between: the outputs go by 32 tokens at a
+// time, tiles have no second buffer, and registers are held to four blocks an SM
+// (six for up to 64 keys).
 template <typename T, int DK, Mode kMode>
-__global__ void __launch_bounds__(128) linattn_kernel(const Args a) {
+__global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) linattn_kernel(const Args a) {
   using Pl = Planes<T>;
-  constexpr int C = Pl::chunk, N = Pl::in, kStages = Pl::stages;
+  constexpr int C = Pl::chunk, N = Pl::in;
   constexpr bool kOut = kMode == kOutput, kBack = kMode == kBackwardState;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Decays<C> decays[2];
@@ -363,17 +404,15 @@ __global__ void __launch_bounds__(128) linattn_kernel(const Args a) {
   const int used = min(last, (len + C - 1) / C);  // chunks with tokens
 
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
-  const int row_bytes = 2 * C, kb = dk16 * row_bytes, vb = a.slab * row_bytes, stage = N * ((kOut ? 2 : 1) * kb + vb);
-  auto tile_k = [&](int s) { return Tile{base + s * stage, row_bytes, kb}; };
-  auto tile_v = [&](int s) { return Tile{base + s * stage + N * kb, row_bytes, vb}; };
-  auto tile_q = [&](int s) { return Tile{base + s * stage + N * (kb + vb), row_bytes, kb}; };
-  const Tile scores{base + kStages * stage, row_bytes, C * row_bytes};
-  auto bring = [&](int c, int s) {
+  const int row_bytes = 2 * C, kb = dk16 * row_bytes, vb = a.slab * row_bytes;
+  const Tile tk{base, row_bytes, kb}, tv{base + N * kb, row_bytes, vb}, tq{base + N * (kb + vb), row_bytes, kb},
+      scores{base + N * (2 * kb + vb), row_bytes, C * row_bytes};
+  auto bring = [&](int c) {
     const int64_t t0 = (int64_t)c * C;
     const int n = min(C, (int)(len - t0));
-    fill<T, C>(tile_k(s), k, a.dk, dk16, L, t0, n, a.vec);
-    fill<T, C>(tile_v(s), v, rows, rows16, L, t0, n, a.vec);
-    if (kOut) fill<T, C>(tile_q(s), q, a.dk, dk16, L, t0, n, a.vec);
+    fill<T, C>(tk, k, a.dk, dk16, L, t0, n, a.vec);
+    fill<T, C>(tv, v, rows, rows16, L, t0, n, a.vec);
+    if (kOut) fill<T, C>(tq, q, a.dk, dk16, L, t0, n, a.vec);
   };
 
   // S^T of this warp's 16 values: tile j holds keys 8j .. 8j+7
@@ -405,71 +444,37 @@ __global__ void __launch_bounds__(128) linattn_kernel(const Args a) {
   const int count = max(0, used - first);
   auto chunk_at = [&](int i) { return kBack ? first + count - 1 - i : first + i; };
   DecayLoad<C> ahead;
-  double total = 0.0;
+  float2 total = make_float2(0.f, 0.f);
   if (count) {
     const int c = chunk_at(0);
-    bring(c, 0);
+    bring(c);
     if (warp == 0) {
       ahead.load(a, b, h, (int64_t)c * C, min(C, len - c * C));
       ahead.finish(decays[0]);
     }
   }
   for (int i = 0; i < count; ++i) {
-    const int c = chunk_at(i), s = kStages == 2 ? i & 1 : 0;
+    const int c = chunk_at(i);
     const int64_t t0 = (int64_t)c * C;
     const int n = min(C, (int)(len - t0));
     copies_done();
     __syncthreads();
     const Decays<C> &d = decays[i & 1];
-    if (i + 1 < count) {
-      if (kStages == 2) bring(chunk_at(i + 1), s ^ 1);
-      if (warp == 0) ahead.load(a, b, h, (int64_t)chunk_at(i + 1) * C, min(C, len - chunk_at(i + 1) * C));
-    }
-    if (kOut && a.states)
+    if (warp == 0 && i + 1 < count)
+      ahead.load(a, b, h, (int64_t)chunk_at(i + 1) * C, min(C, len - chunk_at(i + 1) * C));
+    if (float *keep = kOut ? a.states : kBack ? a.dstates : nullptr)
       each_state([&](float &x, int key, int value) {
-        a.states[(head * a.chunks + c) * state_size + (int64_t)key * a.dv + value] = x;
+        keep[(head * a.chunks + c) * state_size + (int64_t)key * a.dv + value] = x;
       });
-    if (kBack && a.dstates)
-      each_state([&](float &x, int key, int value) {
-        a.dstates[(head * a.chunks + c) * state_size + (int64_t)key * a.dv + value] = x;
-      });
-    const Tile tk = tile_k(s), tv = tile_v(s);
-    float o[C / 8][4];
     if (kOut) {
-      const Tile tq = tile_q(s);
-      // what the state before the chunk gives
-#pragma unroll
-      for (int j = 0; j < C / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < DK / 16; ++kk) {
-        if (kk * 16 >= dk16) break;
-        uint32_t A[Pl::out][4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t p[Pl::out];
-          split<Pl::out>(S[2 * kk + (e >> 1)][2 * (e & 1)], S[2 * kk + (e >> 1)][2 * (e & 1) + 1], p);
-#pragma unroll
-          for (int z = 0; z < Pl::out; ++z) A[z][e] = p[z];
-        }
-#pragma unroll
-        for (int j = 0; j < C / 16; ++j) {
-          uint32_t B[N][4];
-          load_b<true>(B, tq, kk * 16, j * 16);
-          product(o[2 * j], o[2 * j + 1], A, B);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < C / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] *= a.scale * d.begin[8 * j + 2 * gc + (e & 1)];
       // the scores, a 16x16 block at a time
       for (int blk = warp; blk < (C / 16) * (C / 16 + 1) / 2; blk += blockDim.x >> 5) {
         int row, col;
         block_of<C>(blk, row, col);
         float x[2][4] = {};
-        for (int kk = 0; kk < dk16; kk += 16) {
+#pragma unroll
+        for (int kk = 0; kk < DK; kk += 16) {
+          if (kk >= dk16) break;
           uint32_t A[N][4], B[N][4];
           load_a<true>(A, tq, row * 16, kk);
           load_b<true>(B, tk, kk, col * 16);
@@ -490,8 +495,73 @@ __global__ void __launch_bounds__(128) linattn_kernel(const Args a) {
           }
       }
       __syncthreads();
+      if (warp * 16 < rows) {
+#pragma unroll
+        for (int part = 0; part < C / 32; ++part) {
+          // what the state before the chunk gives 32 tokens
+          float o[4][4] = {};
+#pragma unroll
+          for (int kk = 0; kk < DK / 16; ++kk) {
+            if (kk * 16 >= dk16) break;
+            uint32_t A[Pl::out][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t p[Pl::out];
+              split<Pl::out>(S[2 * kk + (e >> 1)][2 * (e & 1)], S[2 * kk + (e >> 1)][2 * (e & 1) + 1], p);
+#pragma unroll
+              for (int z = 0; z < Pl::out; ++z) A[z][e] = p[z];
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t B[N][4];
+              load_b<true>(B, tq, kk * 16, part * 32 + j * 16);
+              product(o[2 * j], o[2 * j + 1], A, B);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][e] *= a.scale * d.begin[part * 32 + 8 * j + 2 * gc + (e & 1)];
+          // and what the chunk's values give
+#pragma unroll
+          for (int ss = 0; ss < 2 * part + 2; ++ss) {
+            uint32_t V[N][4];
+            load_a<false>(V, tv, warp * 16, ss * 16);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int at = 2 * part + j;
+              if (at < ss) continue;
+              if (at == ss && any_not_finite(V[0])) {
+                border<N, Pl::out, true>(o[2 * j], o[2 * j + 1], tv, warp * 16, scores, at * 16);
+                continue;
+              }
+              uint32_t B[Pl::out][4];
+              load_b<false>(B, scores, ss * 16, at * 16);
+              product(o[2 * j], o[2 * j + 1], V, B);
+            }
+          }
+#pragma unroll
+          for (int r8 = 0; r8 < 2; ++r8) {
+            const int r = warp * 16 + gr + r8 * 8;
+            if (r >= rows) continue;
+            T *out = (T *)a.out + values + r * L + t0 + part * 32 + 2 * gc;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int left = n - (part * 32 + 8 * j + 2 * gc);
+              if (a.vec && left > 1) {
+                Pack<T, 2> p;
+                p.set({o[j][2 * r8], o[j][2 * r8 + 1]});
+                p.store(out + 8 * j);
+              } else {
+                if (left > 0) out[8 * j] = from_f<T>(o[j][2 * r8]);
+                if (left > 1) out[8 * j + 1] = from_f<T>(o[j][2 * r8 + 1]);
+              }
+            }
+          }
+        }
+      }
     }
-    // the values' part of the outputs, and the state behind the chunk
+    // the state behind the chunk
     const float whole = d.whole;
 #pragma unroll
     for (int j = 0; j < DK / 8; ++j)
@@ -500,23 +570,8 @@ __global__ void __launch_bounds__(128) linattn_kernel(const Args a) {
     if (warp * 16 < rows) {
 #pragma unroll
       for (int ss = 0; ss < C / 16; ++ss) {
-        uint32_t V[N][4];
+        uint32_t V[N][4], W[Pl::update][4];
         load_a<false>(V, tv, warp * 16, ss * 16);
-        if (kOut) {
-          const bool strange = any_not_finite(V[0]);
-#pragma unroll
-          for (int j = 0; j < C / 16; ++j) {
-            if (j < ss) continue;
-            if (j == ss && strange) {
-              border<N, Pl::out, true>(o[2 * j], o[2 * j + 1], tv, warp * 16, scores, j * 16);
-              continue;
-            }
-            uint32_t B[Pl::out][4];
-            load_b<false>(B, scores, ss * 16, j * 16);
-            product(o[2 * j], o[2 * j + 1], V, B);
-          }
-        }
-        uint32_t W[Pl::update][4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int t = ss * 16 + (e >> 1) * 8 + 2 * gc;
@@ -527,9 +582,9 @@ __global__ void __launch_bounds__(128) linattn_kernel(const Args a) {
             x += r.x;
             y += r.y;
           }
-          const float w0 = kBack ? d.begin[t] * a.scale : d.end[t], w1 = kBack ? d.begin[t + 1] * a.scale : d.end[t + 1];
+          const float2 w = *reinterpret_cast<const float2 *>((kBack ? d.begin : d.end) + t);
           uint32_t p[Pl::update];
-          split<Pl::update>(x * w0, y * w1, p);
+          split<Pl::update>(x * (kBack ? w.x * a.scale : w.x), y * (kBack ? w.y * a.scale : w.y), p);
 #pragma unroll
           for (int z = 0; z < Pl::update; ++z) W[z][e] = p[z];
         }
@@ -542,31 +597,13 @@ __global__ void __launch_bounds__(128) linattn_kernel(const Args a) {
         }
       }
     }
-    if (kOut) {
-#pragma unroll
-      for (int j = 0; j < C / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const int r = warp * 16 + gr + (e >> 1) * 8, t = 8 * j + 2 * gc;
-          if (r >= rows) continue;
-          T *out = (T *)a.out + values + r * L + t0 + t;
-          if (a.vec && t + 1 < n) {
-            Pack<T, 2> p;
-            p.set({o[j][e], o[j][e + 1]});
-            p.store(out);
-          } else {
-            if (t < n) out[0] = from_f<T>(o[j][e]);
-            if (t + 1 < n) out[1] = from_f<T>(o[j][e + 1]);
-          }
-        }
-    }
     if (warp == 0) {
-      total += d.sum;
+      total = two_sum(total, d.sum);
       if (i + 1 < count) ahead.finish(decays[(i + 1) & 1]);
     }
-    if (kStages == 1 && i + 1 < count) {
+    if (i + 1 < count) {
       __syncthreads();
-      bring(chunk_at(i + 1), 0);
+      bring(chunk_at(i + 1));
     }
   }
   if (kOut) {  // zeros behind the last token
@@ -593,12 +630,21 @@ __global__ void __launch_bounds__(256) linattn_carry_kernel(const Args a, bool b
   if (i >= size || head >= (int64_t)a.batch * a.heads) return;
   const float *from = back ? a.last_grad : a.initial;
   float s = from ? from[head * size + i] : 0.f;
-  for (int j = 0; j < a.segments; ++j) {
-    const int seg = back ? a.segments - 1 - j : j;
-    float *at = a.starts + (head * a.segments + seg) * size + i;
-    const float added = *at;
-    *at = s;
-    s = exp2f((float)a.decays[head * a.segments + seg]) * s + added;
+  for (int j = 0; j < a.segments; j += 8) {  // eight reads in flight
+    float added[8], decay[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (j + k < a.segments) {
+        const int64_t seg = head * a.segments + (back ? a.segments - 1 - j - k : j + k);
+        added[k] = a.starts[seg * size + i];
+        decay[k] = exp2_pair(a.decays[seg]);
+      }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (j + k < a.segments) {
+        a.starts[(head * a.segments + (back ? a.segments - 1 - j - k : j + k)) * size + i] = s;
+        s = fmaf(decay[k], s, added[k]);
+      }
   }
   if (a.final_state) a.final_state[head * size + i] = s;
 }
@@ -620,15 +666,16 @@ __device__ __forceinline__ float column_sum(float v) {  // over the eight rows o
 // and the decays' from the pairs W_ts = P_ts (do_t v_s), s < t, the parts that
 // S and D have in q dq and k dk, and exp(b_C) <S, D>; none of these cancel
 // but the W of pairs on one side of a token, which are the same numbers.
-// Each warp has 16 of the dk or dv rows of a gradient.
+// A warp takes 16 of the dk or dv rows of a gradient and 32 tokens at a time.
 template <typename T>
-__global__ void __launch_bounds__(256) linattn_backward_kernel(const Args a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_kernel(const Args a) {
   using Pl = Planes<T>;
   constexpr int C = Pl::chunk, N = Pl::in, X = Pl::back, B16 = C / 16, kBlocks = B16 * (B16 + 1) / 2;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Decays<C> d;
   __shared__ float row_sums[kBlocks][16], col_sums[kBlocks][16], old_part[8][C], new_part[8][C], across_part[8];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, gc = lane & 3, warps = blockDim.x >> 5;
+  constexpr int warps = 8;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, gc = lane & 3;
   int64_t unit = blockIdx.x;
   const int c = unit % a.chunks;
   const int64_t head = unit / a.chunks;
@@ -663,23 +710,60 @@ __global__ void __launch_bounds__(256) linattn_backward_kernel(const Args a) {
 
   const int64_t state_size = (int64_t)a.dk * a.dv;
   const float *S = a.states + (head * a.chunks + c) * state_size, *D = a.dstates + (head * a.chunks + c) * state_size;
-  auto bring_state = [&](const float *from) {
-    for (int i = threadIdx.x; i < dk16 * (dv64 / 2); i += blockDim.x) {
-      const int row = i / (dv64 / 2), col = i % (dv64 / 2) * 2;
-      const float x = row < a.dk && col < a.dv ? from[(int64_t)row * a.dv + col] : 0.f;
-      const float y = row < a.dk && col + 1 < a.dv ? from[(int64_t)row * a.dv + col + 1] : 0.f;
-      uint32_t p[X];
-      split<X>(x, y, p);
+  // Brings a state into `ts`, four values of a key to a thread and eight of these in flight; also the sum of its
+  // products with another one's values (or 0).
+  const int quads = dv64 / 4;
+  auto bring_state = [&](const float *from, const float *other) {
+    float sum = 0.f;
+    const bool wide = a.dv % 4 == 0;
+    constexpr int U = 4;
+    for (int i0 = threadIdx.x; i0 < dk16 * quads; i0 += 256 * U) {
+      float x[U][4] = {}, y[U][4] = {};
 #pragma unroll
-      for (int z = 0; z < X; ++z)
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(ts.piece(row, col / 8, z) + (col & 7) * 2), "r"(p[z]) : "memory");
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * 256, row = i / quads, col = i % quads * 4;
+        if (row < a.dk && col < a.dv) {
+          const int64_t at = (int64_t)row * a.dv + col;
+          if (wide) {
+            *reinterpret_cast<float4 *>(x[u]) = *reinterpret_cast<const float4 *>(from + at);
+            if (other) *reinterpret_cast<float4 *>(y[u]) = *reinterpret_cast<const float4 *>(other + at);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col + e < a.dv) {
+                x[u][e] = from[at + e];
+                if (other) y[u][e] = other[at + e];
+              }
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * 256, row = i / quads, col = i % quads * 4;
+        if (row >= dk16) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = fmaf(x[u][e], y[u][e], sum);
+        uint32_t p[X], q[X];
+        split<X>(x[u][0], x[u][1], p);
+        split<X>(x[u][2], x[u][3], q);
+#pragma unroll
+        for (int z = 0; z < X; ++z)
+          asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(ts.piece(row, col / 8, z) + (col & 7) * 2), "r"(p[z]), "r"(q[z])
+                       : "memory");
+      }
     }
+    return sum;
   };
   fill<T, C>(tq, (const T *)a.q + shared_at, a.dk, dk16, L, t0, n, a.vec);
   fill<T, C>(tk, (const T *)a.k + shared_at, a.dk, dk16, L, t0, n, a.vec);
   fill<T, C>(tv, (const T *)a.v + values_at, a.dv, dv16, L, t0, n, a.vec);
   fill<T, C>(to, (const T *)a.grad + values_at, a.dv, dv16, L, t0, n, a.vec);
-  bring_state(S);
+  {
+    float x = bring_state(S, D);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    if (lane == 0) across_part[warp] = x;
+  }
   if (warp == 0) {
     DecayLoad<C> g;
     g.load(a, b, h, t0, n);
@@ -692,12 +776,14 @@ __global__ void __launch_bounds__(256) linattn_backward_kernel(const Args a) {
     int row, col;
     block_of<C>(blk, row, col);
     float x[2][4] = {}, y[2][4] = {};
+#pragma unroll 4
     for (int kk = 0; kk < dk16; kk += 16) {
       uint32_t A[N][4], B[N][4];
       load_a<true>(A, tq, row * 16, kk);
       load_b<true>(B, tk, kk, col * 16);
       product(x[0], x[1], A, B);
     }
+#pragma unroll 4
     for (int kk = 0; kk < dv16; kk += 16) {
       uint32_t A[N][4], B[N][4];
       load_a<true>(A, to, row * 16, kk);
@@ -744,29 +830,48 @@ __global__ void __launch_bounds__(256) linattn_backward_kernel(const Args a) {
       }
   }
 
-  float acc[C / 8][4];
+  // A piece of a gradient: 16 of its rows (of keys or values) and 32 tokens.
+  constexpr int kParts = C / 32;
+  const int key_tiles = dk16 / 16, value_tiles = dv16 / 16;
+  float acc[4][4];
   auto zero = [&]() {
 #pragma unroll
-    for (int j = 0; j < C / 8; ++j)
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
   };
-  // scales the columns by their tokens' factors, and sums acc * x over the warp's rows of x for each token
-  auto share_of = [&](const float *factor, float scale, const Tile &x, float *part) {
+  // acc += A[rows m ..][k] B[k][tokens], k over `depth`; A of X planes, transposed or not
+  auto times = [&](auto trans, int m, const Tile &B_, int depth, int part) {
+#pragma unroll 2
+    for (int kk = 0; kk < depth; kk += 16) {
+      uint32_t A[X][4];
+      load_a<decltype(trans)::value>(A, ts, m, kk);
 #pragma unroll
-    for (int j = 0; j < C / 8; ++j) {
-      float s[2] = {};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc[j][e] *= scale * factor[8 * j + 2 * gc + (e & 1)];
+      for (int j = 0; j < 2; ++j) {
+        uint32_t B[N][4];
+        load_b<true>(B, B_, kk, part * 32 + j * 16);
+        product(acc[2 * j], acc[2 * j + 1], A, B);
       }
+    }
+  };
+  auto factors = [&](const float *factor, float scale, int part) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] *= scale * factor[part * 32 + 8 * j + 2 * gc + (e & 1)];
+  };
+  // the sums of acc times x's rows, for each token
+  auto share_of = [&](const Tile &x, int m, int part, float *sums) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float s[2] = {};
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float f0 = 0.f, f1 = 0.f;
 #pragma unroll
         for (int z = N - 1; z >= 0; --z) {
           uint32_t w;
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(x.piece(warp * 16 + gr + r * 8, j, z) + 4 * gc));
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(x.piece(m + gr + r * 8, part * 4 + j, z) + 4 * gc));
           const float2 v = unpair(w);
           f0 += v.x;
           f1 += v.y;
@@ -777,148 +882,110 @@ __global__ void __launch_bounds__(256) linattn_backward_kernel(const Args a) {
       s[0] = column_sum(s[0]);
       s[1] = column_sum(s[1]);
       if (gr == 0) {
-        part[8 * j + 2 * gc] = s[0];
-        part[8 * j + 2 * gc + 1] = s[1];
+        sums[part * 32 + 8 * j + 2 * gc] = s[0];
+        sums[part * 32 + 8 * j + 2 * gc + 1] = s[1];
       }
     }
   };
-  auto each = [&](int limit, auto &&f) {  // f(row, token, value) for the gradient's rows
-#pragma unroll
-    for (int j = 0; j < C / 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = warp * 16 + gr + (e >> 1) * 8, t = 8 * j + 2 * gc + (e & 1);
-        if (row < limit && t < kept) f(row, t, t < n ? acc[j][e] : 0.f);
-      }
-  };
-  // the states' part of dq
-  const bool has_k = warp * 16 < a.dk, has_v = warp * 16 < a.dv;
-  zero();
-  if (has_k) {
-    for (int kk = 0; kk < dv16; kk += 16) {
-      uint32_t A[X][4];
-      load_a<false>(A, ts, warp * 16, kk);
-#pragma unroll
-      for (int j = 0; j < B16; ++j) {
-        uint32_t B[N][4];
-        load_b<true>(B, to, kk, j * 16);
-        product(acc[2 * j], acc[2 * j + 1], A, B);
-      }
-    }
-    share_of(d.begin, a.scale, tq, old_part[warp]);
-  }
-  __syncthreads();  // the scores are there, S is done with
-  if (has_k) {
+  // acc += x[rows m ..][tokens up to (or from) each one on] times the scores between them
+  auto within = [&](auto up_to, const Tile &x, int m, const Tile &scores, int part) {
+    constexpr bool kUpTo = decltype(up_to)::value;
 #pragma unroll
     for (int s = 0; s < B16; ++s) {
+      if (kUpTo ? s > 2 * part + 1 : s < 2 * part) continue;
       uint32_t A[N][4];
-      load_a<false>(A, tk, warp * 16, s * 16);
-      const bool strange = any_not_finite(A[0]);
+      load_a<false>(A, x, m, s * 16);
 #pragma unroll
-      for (int j = 0; j < B16; ++j) {
-        if (j < s) continue;
-        if (j == s && strange) {
-          border<N, Pl::out, true>(acc[2 * j], acc[2 * j + 1], tk, warp * 16, te, j * 16);
+      for (int j = 0; j < 2; ++j) {
+        const int at = 2 * part + j;
+        if (kUpTo ? s > at : s < at) continue;
+        if (at == s && any_not_finite(A[0])) {
+          border<N, Pl::out, kUpTo>(acc[2 * j], acc[2 * j + 1], x, m, scores, at * 16);
           continue;
         }
         uint32_t B[Pl::out][4];
-        load_b<false>(B, te, s * 16, j * 16);
+        load_b<!kUpTo>(B, scores, s * 16, at * 16);
         product(acc[2 * j], acc[2 * j + 1], A, B);
       }
     }
-    each(a.dk, [&](int row, int t, float x) { put_shared((T *)a.dq, a.dq_heads, row, t, x); });
-  }
-  bring_state(D);
-  {
-    float x = 0.f;
-    for (int64_t i = threadIdx.x; i < state_size; i += blockDim.x) x = fmaf(S[i], D[i], x);
+  };
+  const std::true_type yes;
+  const std::false_type no;
+  // f(row, token, value, next token's value) for a piece's pairs of tokens
+  auto each = [&](int m, int limit, int part, auto &&f) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    if (lane == 0) across_part[warp] = x;
+    for (int r = 0; r < 2; ++r) {
+      const int row = m + gr + r * 8;
+      if (row >= limit) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = part * 32 + 8 * j + 2 * gc;
+        f(row, t, t < n ? acc[j][2 * r] : 0.f, t + 1 < n ? acc[j][2 * r + 1] : 0.f);
+      }
+    }
+  };
+  auto put = [&](auto *out, int t, float x, float y) {
+    using O = std::remove_pointer_t<decltype(out)>;
+    if (a.vec && t + 1 < kept) {
+      Pack<O, 2> p;
+      p.set({x, y});
+      p.store(out + t);
+    } else {
+      if (t < kept) out[t] = from_f<O>(x);
+      if (t + 1 < kept) out[t + 1] = from_f<O>(y);
+    }
+  };
+  auto put_keys = [&](void *out, float *heads, int row, int t, float x, float y) {
+    if (heads) put(heads + (head * a.dk + row) * L + t0, t, x, y);
+    else put((T *)out + shared_at + row * L + t0, t, x, y);
+  };
+  // (the first pieces' states are multiplied before the barrier, while other warps still make scores)
+  for (int it = warp; it < key_tiles * kParts; it += warps) {
+    const int m = it / kParts * 16, part = it % kParts;
+    zero();
+    times(no, m, to, dv16, part);
+    factors(d.begin, a.scale, part);
+    share_of(tq, m, part, old_part[m / 16]);
+    if (it == warp) __syncthreads();  // the scores are there
+    within(yes, tk, m, te, part);
+    each(m, a.dk, part, [&](int row, int t, float x, float y) { put_keys(a.dq, a.dq_heads, row, t, x, y); });
   }
+  if (warp >= key_tiles * kParts) __syncthreads();
+  __syncthreads();  // S is done with
+  bring_state(D, nullptr);
   __syncthreads();
-  if (has_k) {
+  for (int it = warp; it < (key_tiles + value_tiles) * kParts; it += warps) {
+    const int tile = it / kParts, part = it % kParts;
     zero();
-    for (int kk = 0; kk < dv16; kk += 16) {
-      uint32_t A[X][4];
-      load_a<false>(A, ts, warp * 16, kk);
-#pragma unroll
-      for (int j = 0; j < B16; ++j) {
-        uint32_t B[N][4];
-        load_b<true>(B, tv, kk, j * 16);
-        product(acc[2 * j], acc[2 * j + 1], A, B);
-      }
+    if (tile < key_tiles) {
+      const int m = tile * 16;
+      times(no, m, tv, dv16, part);
+      factors(d.end, 1.f, part);
+      share_of(tk, m, part, new_part[tile]);
+      within(no, tq, m, te, part);
+      each(m, a.dk, part, [&](int row, int t, float x, float y) { put_keys(a.dk_, a.dk_heads, row, t, x, y); });
+    } else {
+      const int m = (tile - key_tiles) * 16;
+      times(yes, m, tk, dk16, part);
+      factors(d.end, 1.f, part);
+      within(no, to, m, tp, part);
+      each(m, a.dv, part, [&](int row, int t, float x, float y) { put((T *)a.dv_ + values_at + row * L + t0, t, x, y); });
     }
-    share_of(d.end, 1.f, tk, new_part[warp]);
-#pragma unroll
-    for (int t = 0; t < B16; ++t) {
-      uint32_t A[N][4];
-      load_a<false>(A, tq, warp * 16, t * 16);
-      const bool strange = any_not_finite(A[0]);
-#pragma unroll
-      for (int j = 0; j < B16; ++j) {
-        if (j > t) continue;
-        if (j == t && strange) {
-          border<N, Pl::out, false>(acc[2 * j], acc[2 * j + 1], tq, warp * 16, te, j * 16);
-          continue;
-        }
-        uint32_t B[Pl::out][4];
-        load_b<true>(B, te, t * 16, j * 16);
-        product(acc[2 * j], acc[2 * j + 1], A, B);
-      }
-    }
-    each(a.dk, [&](int row, int t, float x) { put_shared((T *)a.dk_, a.dk_heads, row, t, x); });
-  }
-  if (has_v) {
-    zero();
-    for (int kk = 0; kk < dk16; kk += 16) {
-      uint32_t A[X][4];
-      load_a<true>(A, ts, warp * 16, kk);
-#pragma unroll
-      for (int j = 0; j < B16; ++j) {
-        uint32_t B[N][4];
-        load_b<true>(B, tk, kk, j * 16);
-        product(acc[2 * j], acc[2 * j + 1], A, B);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < C / 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[j][e] *= d.end[8 * j + 2 * gc + (e & 1)];
-#pragma unroll
-    for (int t = 0; t < B16; ++t) {
-      uint32_t A[N][4];
-      load_a<false>(A, to, warp * 16, t * 16);
-      const bool strange = any_not_finite(A[0]);
-#pragma unroll
-      for (int j = 0; j < B16; ++j) {
-        if (j > t) continue;
-        if (j == t && strange) {
-          border<N, Pl::out, false>(acc[2 * j], acc[2 * j + 1], to, warp * 16, tp, j * 16);
-          continue;
-        }
-        uint32_t B[Pl::out][4];
-        load_b<true>(B, tp, t * 16, j * 16);
-        product(acc[2 * j], acc[2 * j + 1], A, B);
-      }
-    }
-    each(a.dv, [&](int row, int t, float x) { ((T *)a.dv_)[values_at + row * L + t0 + t] = from_f<T>(x); });
   }
   __syncthreads();
   if (warp == 0) {
     // dg_t = sum_(u >= t) (late_u) + sum_(u < t) new_u + across, with late = row sums - column sums + old
     constexpr int M = C / 32;
-    double late[M], fresh[M], late_sum = 0.0, fresh_sum = 0.0;
-    const int key_warps = (a.dk + 15) / 16;
+    float late[M], fresh[M], late_sum = 0.f, fresh_sum = 0.f;
 #pragma unroll
     for (int i = 0; i < M; ++i) {
       const int t = lane * M + i, tb = t / 16;
-      double x = 0.0, y = 0.0;
+      float x = 0.f, y = 0.f;
       for (int o = 0; o < B16; ++o) {
         if (o <= tb) x += row_sums[tb * (tb + 1) / 2 + o][t % 16];
         if (o >= tb) x -= col_sums[o * (o + 1) / 2 + tb][t % 16];
       }
-      for (int w = 0; w < key_warps; ++w) {
+      for (int w = 0; w < key_tiles; ++w) {
         x += old_part[w][t];
         y += new_part[w][t];
       }
@@ -929,27 +996,27 @@ __global__ void __launch_bounds__(256) linattn_backward_kernel(const Args a) {
     }
     // sums from this lane's tokens on, and up to them (neither as a difference, that what is not finite stays on
     // its side)
-    double from = late_sum, before = fresh_sum;
+    float from = late_sum, before = fresh_sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const double x = __shfl_down_sync(0xffffffffu, from, o), y = __shfl_up_sync(0xffffffffu, before, o);
+      const float x = __shfl_down_sync(0xffffffffu, from, o), y = __shfl_up_sync(0xffffffffu, before, o);
       if (lane + o < 32) from += x;
       if (lane >= o) before += y;
     }
     from = __shfl_down_sync(0xffffffffu, from, 1);  // behind this lane's
     before = __shfl_up_sync(0xffffffffu, before, 1);
-    if (lane == 31) from = 0.0;
-    if (lane == 0) before = 0.0;
-    double across = 0.0;
+    if (lane == 31) from = 0.f;
+    if (lane == 0) before = 0.f;
+    float across = 0.f;
     for (int w = 0; w < warps; ++w) across += across_part[w];
     across *= d.whole;
 #pragma unroll
     for (int i = 0; i < M; ++i) {
       const int t = lane * M + i;
-      double x = from + before + across;
+      float x = from + before + across;
 #pragma unroll
       for (int j = 0; j < M; ++j) x += j < i ? fresh[j] : late[j];
-      if (t < kept) dg[t] = t < n ? (float)x : 0.f;
+      if (t < kept) dg[t] = t < n ? x : 0.f;
     }
   }
 }
@@ -1070,7 +1137,7 @@ Plan make_plan(int dtype, int batch, int heads, int length, int dv) {
   p.slabs = (tiles + 3) / 4;
   p.slab = 16 * ((tiles + p.slabs - 1) / p.slabs);
   p.chunks = ceil_div(length, chunk_of(dtype));
-  const int64_t units = (int64_t)batch * heads * p.slabs, wanted = (int64_t)device_sm_count() * 2;
+  const int64_t units = (int64_t)batch * heads * p.slabs, wanted = (int64_t)device_sm_count() * 4;
   p.segments = 1;
   if (units * 2 <= wanted && p.chunks >= 8)
     p.segments = (int)std::min<int64_t>(wanted / units, p.chunks / 4);
@@ -1089,7 +1156,7 @@ template <typename T>
 size_t forward_smem(const Args &a, bool out) {
   using Pl = Planes<T>;
   const int dk16 = (a.dk + 15) & ~15, bytes = 2 * Pl::chunk;
-  return (size_t)Pl::stages * Pl::in * ((out ? 2 : 1) * dk16 + a.slab) * bytes + (out ? (size_t)Pl::out * Pl::chunk * bytes : 0);
+  return (size_t)Pl::in * ((out ? 2 : 1) * dk16 + a.slab) * bytes + (out ? (size_t)Pl::out * Pl::chunk * bytes : 0);
 }
 template <typename T>
 size_t backward_smem(const Args &a) {
@@ -1155,8 +1222,8 @@ int run_backward(Args a, void *dq, void *dk, cudaStream_t stream) {
   auto *kernel = linattn_backward_kernel<T>;
   static PerContext<uint64_t> allowed;
   if ((st = allow_smem(kernel, allowed)) != PC2D_OK) return st;
-  kernel<<<(unsigned)((int64_t)a.batch * a.heads * a.chunks), std::max(a.dk, a.dv) <= 64 ? 128 : 256,
-           backward_smem<T>(a), stream>>>(a);
+  kernel<<<(unsigned)((int64_t)a.batch * a.heads * a.chunks), 256, backward_smem<T>(a),
+           stream>>>(a);
   PC2D_LAUNCH_CHECK("linattn_backward_kernel");
   if (a.dq_heads) {
     const int64_t size = (int64_t)a.dk * a.length, count = size * a.batch * a.groups;
@@ -1184,6 +1251,12 @@ int check_linattn(const char *what, int dtype, int batch, int heads, int groups,
     return PC2D_ERR_UNSUPPORTED;
   }
   return PC2D_OK;
+}
+
+int check_states(const char *what, const float *states) {
+  if (aligned16(states)) return PC2D_OK;
+  set_last_error("%s: the kept states must be on a 16-byte boundary", what);
+  return PC2D_ERR_INVALID_ARGUMENT;
 }
 
 int need_workspace(const char *what, const void *workspace, size_t bytes, size_t need) {
@@ -1252,7 +1325,8 @@ extern "C" int pc2d_linear_attention_forward(int dtype, const void *q, const voi
     set_last_error("%s: null pointer (q, k, v, log_decay or output)", what);
     return PC2D_ERR_INVALID_ARGUMENT;
   }
-  if ((st = check_elements(what, size, {q, k, v, output})) != PC2D_OK) return st;
+  if ((st = check_elements(what, size, {q, k, v, output})) != PC2D_OK || (st = check_states(what, states)) != PC2D_OK)
+    return st;
   Plan p = make_plan(dtype, batch, heads, length, dv);
   sizes_of(p, batch, heads, dk, dv);
   if ((st = need_workspace(what, workspace, workspace_bytes, p.starts + p.decays)) != PC2D_OK) return st;
@@ -1270,7 +1344,7 @@ extern "C" int pc2d_linear_attention_forward(int dtype, const void *q, const voi
   a.final_state = final_state;
   a.states = states;
   a.starts = static_cast<float *>(workspace);
-  a.decays = reinterpret_cast<double *>(static_cast<char *>(workspace) + p.starts);
+  a.decays = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + p.starts);
   a.batch = batch;
   a.heads = heads;
   a.groups = groups;
@@ -1319,7 +1393,9 @@ extern "C" int pc2d_linear_attention_backward(int dtype, const void *grad, const
     set_last_error("%s: null pointer", what);
     return PC2D_ERR_INVALID_ARGUMENT;
   }
-  if ((st = check_elements(what, size, {grad, q, k, v, qgrad, kgrad, vgrad})) != PC2D_OK) return st;
+  if ((st = check_elements(what, size, {grad, q, k, v, qgrad, kgrad, vgrad})) != PC2D_OK ||
+      (st = check_states(what, states)) != PC2D_OK)
+    return st;
   if ((st = need_workspace(what, workspace, workspace_bytes,
                            pc2d_linear_attention_workspace_size(dtype, batch, heads, groups, length, dk, dv, 1))) != PC2D_OK)
     return st;
@@ -1333,7 +1409,7 @@ extern "C" int pc2d_linear_attention_backward(int dtype, const void *grad, const
   };
   Args a{};
   a.starts = reinterpret_cast<float *>(take(p.starts));
-  a.decays = reinterpret_cast<double *>(take(p.decays));
+  a.decays = reinterpret_cast<float2 *>(take(p.decays));
   a.dstates =
       reinterpret_cast<float *>(take(pc2d_linear_attention_states_size(dtype, batch, heads, length, dk, dv)));
   float *per_token = reinterpret_cast<float *>(take((size_t)batch * heads * length * 4));
@@ -1369,7 +1445,8 @@ extern "C" int pc2d_linear_attention_backward(int dtype, const void *grad, const
   a.segments = p.segments;
   a.per_segment = p.per_segment;
   a.scale = (float)scale;
-  a.vec = length % 8 == 0 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(grad);
+  a.vec = length % 8 == 0 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(grad) && aligned16(qgrad) &&
+          aligned16(kgrad) && aligned16(vgrad);
   switch (dtype) {
     case PC2D_DTYPE_F32: st = run_backward<float>(a, qgrad, kgrad, s); break;
     case PC2D_DTYPE_F16: st = run_backward<__half>(a, qgrad, kgrad, s); break;
