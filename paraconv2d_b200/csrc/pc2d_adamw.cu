@@ -121,6 +121,10 @@ __device__ __forceinline__ float weight(float w, float m, float v, bool first, c
 
 // ------------------------------------------------------------- 8-bit moments
 
+// 2^e, for e from -127 to 127
+__device__ __forceinline__ constexpr unsigned exp2_bits(int e) { return e < -126 ? 1u << 22 : (unsigned)(e + 127) << 23; }
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float(exp2_bits(e)); }
+
 template <bool kSigned>
 struct Code {
   static constexpr int kTop = kSigned ? 15 : 31;  // binades of normal numbers
@@ -129,22 +133,22 @@ struct Code {
     // (above 15/8 of its binade it may be rounded up into the next one)
     return most >= 0x7f800000u ? 255u : (unsigned)max((int)((most + 0xFFFFFu) >> 23) - (kTop - 1), 1);
   }
-  static __device__ __forceinline__ float decode(unsigned code, unsigned E) {
-    const unsigned c = kSigned ? code & 127u : code, least = E << 23;
-    // below 8: c eighths of the smallest normal number, as (1 + c/8) of it less itself
-    float x = __uint_as_float((c < 8 ? c << 20 : (c - 8) << 20) + least);
-    if (c < 8) x -= __uint_as_float(least);
-    if (E == 255) x = __uint_as_float(0x7fffffffu);
-    return kSigned && (code & 128u) ? -x : x;
+  // A code at bit 20 has the fields of a 32-bit float, small codes those of its
+  // subnormal numbers: two exact products with powers of two (one would
+  // overflow) bring the smallest normal number, 2^-126, to 2^(E - 127).
+  static __device__ __forceinline__ float up(unsigned E) {
+    return E == 255 ? __uint_as_float(0x7fffffffu) : exp2i((int)E - 127);
   }
-  // `low`: the 8 random bits
-  static __device__ __forceinline__ unsigned encode(float x, unsigned E, unsigned low) {
-    const float least = __uint_as_float(E << 23), size = fabsf(x);
-    const bool normal = size >= least;
-    // below the smallest normal number, adding it makes the steps those of its own binade
-    const unsigned bits = __float_as_uint(normal ? size : __fadd_rn(size, least));
-    const int c = (int)((bits + (low << 12) + 2048u) >> 20) - (int)(E << 3) + (normal ? 8 : 0);
-    const unsigned code = E == 255 ? 0u : (unsigned)(kSigned || size == 0.f ? c : max(c, 1));
+  static __device__ __forceinline__ float decode(unsigned code, float up) {
+    const unsigned bits = kSigned ? (code & 127u) << 20 | (code & 128u) << 24 : code << 20;
+    return __uint_as_float(bits) * exp2i(126) * up;
+  }
+  // And back, with the rounding of the second product at the subnormal numbers'
+  // step.  `low`: the 8 random bits, at bit 12.
+  static __device__ __forceinline__ unsigned encode(float x, float down, unsigned low) {
+    const unsigned bits = __float_as_uint(fabsf(x) * down * exp2i(-126));
+    unsigned code = (bits + low + 2048u) >> 20;
+    if (!kSigned && x > 0.f) code = max(code, 1u);
     return kSigned && x < 0.f ? code | 128u : code;
   }
 };
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
 
 // Moments in 8 bits: a warp takes a block of 256 at a time, eight a lane.
 template <typename P, typename G, int N>
-__global__ void __launch_bounds__(kThreads) adamw8_kernel(const __grid_constant__ Items<N> a, const Coef *coef,
+__global__ void __launch_bounds__(kThreads, 3) adamw8_kernel(const __grid_constant__ Items<N> a, const Coef *coef,
                                                           const float *grad_scale, const Betas b) {
   constexpr int V = 8;
   const int k = find_item(a, blockIdx.x);
@@ -287,7 +291,7 @@ __global__ void __launch_bounds__(kThreads) adamw8_kernel(const __grid_constant_
     if (it.master) fetch(w, it.master + e, whole, left);
     else fetch(p, param + e, whole, left);
     unsigned char *scale = it.scales + block / kBlock * 2;
-    const unsigned em = scale[0], ev = scale[1];
+    const float em = Code<true>::up(scale[0]), ev = Code<false>::up(scale[1]);
     const Bytes16 low = random16((uint64_t)(e / V), (unsigned)it.index, t, b.seed);
     float m[V], v[V], x[V];
     unsigned most_m = 0, most_v = 0;
@@ -306,11 +310,20 @@ __global__ void __launch_bounds__(kThreads) adamw8_kernel(const __grid_constant_
     put<P, V>(x, param + e, whole, left);
     const unsigned nm = Code<true>::scale(__reduce_max_sync(0xffffffffu, most_m));
     const unsigned nv = Code<false>::scale(__reduce_max_sync(0xffffffffu, most_v));
+    // (values that are not finite have code 0: their exponent says what they are)
+    const float dm = nm == 255 ? 0.f : exp2i(127 - (int)nm), dv = nv == 255 ? 0.f : exp2i(127 - (int)nv);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      mc.v[i] = (unsigned char)Code<true>::encode(m[i], nm, (low.w[i / 4] >> (8 * (i % 4))) & 255u);
-      vc.v[i] = (unsigned char)Code<false>::encode(v[i], nv, (low.w[2 + i / 4] >> (8 * (i % 4))) & 255u);
+      const unsigned rm = low.w[i / 4], rv = low.w[2 + i / 4], mask = 255u << 12;
+      mc.v[i] = (unsigned char)Code<true>::encode(m[i], dm, (i % 4 < 2 ? rm << (12 - 8 * (i % 4)) : rm >> (8 * (i % 4) - 12)) & mask);
+      vc.v[i] = (unsigned char)Code<false>::encode(v[i], dv, (i % 4 < 2 ? rv << (12 - 8 * (i % 4)) : rv >> (8 * (i % 4) - 12)) & mask);
     }
+    if (nm == 255)
+#pragma unroll
+      for (int i = 0; i < V; ++i) mc.v[i] = 0;
+    if (nv == 255)
+#pragma unroll
+      for (int i = 0; i < V; ++i) vc.v[i] = 0;
     if (whole) {
       mc.store(ms + e);
       vc.store(vs + e);
@@ -345,7 +358,7 @@ __global__ void __launch_bounds__(kThreads) adamw_values_kernel(const __grid_con
     Pack<unsigned char, V> mc, vc;
     fetch(mc, ms + e, whole, left);
     fetch(vc, vs + e, whole, left);
-    const unsigned em = it.scales[e / kBlock * 2], ev = it.scales[e / kBlock * 2 + 1];
+    const float em = Code<true>::up(it.scales[e / kBlock * 2]), ev = Code<false>::up(it.scales[e / kBlock * 2 + 1]);
     float m[V], v[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {

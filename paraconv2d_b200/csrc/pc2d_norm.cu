@@ -130,21 +130,62 @@ __device__ __forceinline__ void join(const float *v, int entries, At &&at, Count
   m2 = warp_sum(q);
 }
 
-__device__ __forceinline__ float silu_slope(float pre, float s) { return s * (1.f + pre * (1.f - s)); }
+// Pairs of numbers, one instruction for two.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 sigmoid2(float2 v) {  // as sigmoid_f
+  float2 e = mul2(v, both(-1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(e.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(e.y));
+  e = add2(e, both(1.f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(e.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(e.y));
+  return e;
+}
+// The SiLU's slope at `pre`, whose sigmoid is s.
+__device__ __forceinline__ float2 silu_slope(float2 pre, float2 s) {
+  return mul2(s, fma2(pre, fma2(s, both(-1.f), both(1.f)), both(1.f)));
+}
 
 template <typename T, int V>
 struct Norm {
   using Vec = Pack<T, V>;
+  static constexpr int P = (V + 1) / 2;  // pairs of a vector (of one element: half of one)
 
-  // N vectors in flight
+  // vectors in flight
   static constexpr int kFlight = 4;
 
-  static __device__ __forceinline__ void write(T *p, const float (&v)[V]) {
+  static __device__ __forceinline__ float2 get(const Vec &v, int i) {
+    if constexpr (V == 1) {
+      return make_float2(v.f(0), 0.f);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const unsigned w = reinterpret_cast<const unsigned *>(v.v)[i];
+      return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    } else if constexpr (std::is_same<T, __half>::value) {
+      return __half22float2(reinterpret_cast<const __half2 *>(v.v)[i]);
+    } else {
+      return make_float2(v.v[2 * i], v.v[2 * i + 1]);
+    }
+  }
+  static __device__ __forceinline__ void write(T *p, const float2 (&v)[P]) {
     Vec o;
-    if constexpr (V > 1) o.set(v);
-    else o.v[0] = from_f<T>(v[0]);
+    if constexpr (V > 1) {
+      float x[V];
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        x[2 * i] = v[i].x;
+        x[2 * i + 1] = v[i].y;
+      }
+      o.set(x);
+    } else {
+      o.v[0] = from_f<T>(v[0].x);
+    }
     o.store(p);
   }
+  // number i of a vector's pairs
+  static __device__ __forceinline__ float &at(float2 (&v)[P], int i) { return i & 1 ? v[i >> 1].y : v[i >> 1].x; }
 
   // ------------------------------------------------------------ channels last
   // Threads: `cols` vectors of channels by `rows` tokens; a slab of more
@@ -166,7 +207,7 @@ struct Norm {
 
   // Tokens behind the row's last: zeros.
   static __device__ void clear_last(const NormArgs &a, const Place &p, const Last &l) {
-    const float zero[V] = {};
+    const float2 zero[P] = {};
     const int behind = a.P - p.len, first = p.len + (int)((int64_t)behind * p.rank / a.split),
               last = p.len + (int)((int64_t)behind * (p.rank + 1) / a.split);
     for (int64_t i = threadIdx.x; i < (int64_t)(last - first) * l.sv; i += kThreads)
@@ -186,44 +227,41 @@ struct Norm {
         const int col = c0 + tx;
         if (ty < l.rows && col < l.sv) {
           const T *at = x + l.base + col * V;
-          float k[V], s[V] = {}, q[V] = {};
+          float2 k[P] = {}, s[P] = {}, q[P] = {};
           const int first = l.r0 + ty;
+          auto one = [&](const Vec &v) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+              const float2 d = add2(get(v, i), k[i]);
+              s[i] = add2(s[i], d);
+              q[i] = fma2(d, d, q[i]);
+            }
+          };
           if (first < l.r1) {
             Vec v;
             v.load(at + (int64_t)first * a.C);
 #pragma unroll
-            for (int i = 0; i < V; ++i) k[i] = v.f(i);
+            for (int i = 0; i < P; ++i) k[i] = mul2(get(v, i), both(-1.f));
             int r = first + l.rows;
             for (; r + (kFlight - 1) * l.rows < l.r1; r += kFlight * l.rows) {
               Vec u[kFlight];
 #pragma unroll
               for (int j = 0; j < kFlight; ++j) u[j].load(at + (int64_t)(r + j * l.rows) * a.C);
 #pragma unroll
-              for (int j = 0; j < kFlight; ++j)
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                  const float d = u[j].f(i) - k[i];
-                  s[i] += d;
-                  q[i] = fmaf(d, d, q[i]);
-                }
+              for (int j = 0; j < kFlight; ++j) one(u[j]);
             }
             for (; r < l.r1; r += l.rows) {
               v.load(at + (int64_t)r * a.C);
-#pragma unroll
-              for (int i = 0; i < V; ++i) {
-                const float d = v.f(i) - k[i];
-                s[i] += d;
-                q[i] = fmaf(d, d, q[i]);
-              }
+              one(v);
             }
           }
           const float n = l.count(ty), inv = n > 0.f ? 1.f / n : 0.f;
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const float m = s[i] * inv;
+            const float m = Norm::at(s, i) * inv;
             float *e = red + 2 * ((size_t)ty * l.sc + col * V + i);
-            e[0] = n > 0.f ? k[i] + m : 0.f;
-            e[1] = q[i] - s[i] * m;
+            e[0] = n > 0.f ? m - Norm::at(k, i) : 0.f;
+            e[1] = Norm::at(q, i) - Norm::at(s, i) * m;
           }
         }
       }
@@ -248,21 +286,21 @@ struct Norm {
     for (int c0 = 0; c0 < l.sv; c0 += l.cols) {
       const int col = c0 + tx;
       if (ty < l.rows && col < l.sv) {
-        float mean[V], scale[V], shift[V];
+        float2 mean[P] = {}, scale[P] = {}, shift[P] = {};  // (the mean's negative)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const int c = col * V + i, g = c / a.cg, ch = p.slab * a.slab_channels + c;
-          mean[i] = stat[2 * g];
-          scale[i] = stat[2 * g + 1] * load_w<T>(a.w, ch, a.wf32, 1.f);
-          shift[i] = load_w<T>(a.b, ch, a.wf32, 0.f);
+          Norm::at(mean, i) = -stat[2 * g];
+          Norm::at(scale, i) = stat[2 * g + 1] * load_w<T>(a.w, ch, a.wf32, 1.f);
+          Norm::at(shift, i) = load_w<T>(a.b, ch, a.wf32, 0.f);
         }
         const int64_t at = l.base + col * V;
         auto one = [&](const Vec &v, int64_t e) {
-          float y[V];
+          float2 y[P];
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float pre = fmaf(v.f(i) - mean[i], scale[i], shift[i]);
-            y[i] = a.silu ? pre * sigmoid_f(pre) : pre;
+          for (int i = 0; i < P; ++i) {
+            const float2 pre = fma2(add2(get(v, i), mean[i]), scale[i], shift[i]);
+            y[i] = a.silu ? mul2(pre, sigmoid2(pre)) : pre;
           }
           write((T *)a.out + e, y);
         };
@@ -314,25 +352,23 @@ struct Norm {
     float *mine = red + (size_t)2 * l.rows * l.sc;     // [sc][2]: sums of h and of h xhat
     float *chan = mine + 2 * l.sc, *sums = chan + 2 * l.sc;  // [sc][2]; [groups][2]: means of h w and of h w xhat
     const float *stats = a.stats + 2 * ((size_t)p.n * a.G + p.slab * a.slab_channels / a.cg);
-    float mean[V], rstd[V], w[V], b[V];
+    float2 mean[P] = {}, rstd[P] = {}, w[P] = {}, b[P] = {};  // (the mean's negative)
     auto channel = [&](int col) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int c = col * V + i, g = c / a.cg, ch = p.slab * a.slab_channels + c;
-        mean[i] = stats[2 * g];
-        rstd[i] = stats[2 * g + 1];
-        w[i] = load_w<T>(a.w, ch, a.wf32, 1.f);
-        b[i] = load_w<T>(a.b, ch, a.wf32, 0.f);
+        Norm::at(mean, i) = -stats[2 * g];
+        Norm::at(rstd, i) = stats[2 * g + 1];
+        Norm::at(w, i) = load_w<T>(a.w, ch, a.wf32, 1.f);
+        Norm::at(b, i) = load_w<T>(a.b, ch, a.wf32, 0.f);
       }
     };
-    auto slope = [&](const Vec &vx, const Vec &vd, int i, float &xhat) {
-      xhat = (vx.f(i) - mean[i]) * rstd[i];
-      float h = vd.f(i);
-      if (a.silu) {
-        const float pre = fmaf(xhat, w[i], b[i]);
-        h *= silu_slope(pre, sigmoid_f(pre));
-      }
-      return h;
+    auto slope = [&](const Vec &vx, const Vec &vd, int i, float2 &xhat) {
+      xhat = mul2(add2(get(vx, i), mean[i]), rstd[i]);
+      const float2 h = get(vd, i);
+      if (!a.silu) return h;
+      const float2 pre = fma2(xhat, w[i], b[i]);
+      return mul2(h, silu_slope(pre, sigmoid2(pre)));
     };
     if (a.phase != kApply) {
       for (int c0 = 0; c0 < l.sv; c0 += l.cols) {
@@ -340,14 +376,14 @@ struct Norm {
         if (ty < l.rows && col < l.sv) {
           channel(col);
           const int64_t at = l.base + col * V;
-          float s[V] = {}, q[V] = {};
+          float2 s[P] = {}, q[P] = {};
           auto one = [&](const Vec &vx, const Vec &vd) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              float xhat;
-              const float h = slope(vx, vd, i, xhat);
-              s[i] += h;
-              q[i] = fmaf(h, xhat, q[i]);
+            for (int i = 0; i < P; ++i) {
+              float2 xhat;
+              const float2 h = slope(vx, vd, i, xhat);
+              s[i] = add2(s[i], h);
+              q[i] = fma2(h, xhat, q[i]);
             }
           };
           int r = l.r0 + ty;
@@ -370,8 +406,8 @@ struct Norm {
 #pragma unroll
           for (int i = 0; i < V; ++i) {
             float *e = red + 2 * ((size_t)ty * l.sc + col * V + i);
-            e[0] = s[i];
-            e[1] = q[i];
+            e[0] = Norm::at(s, i);
+            e[1] = Norm::at(q, i);
           }
         }
       }
@@ -388,20 +424,20 @@ struct Norm {
       const int col = c0 + tx;
       if (ty < l.rows && col < l.sv) {
         channel(col);
-        float hw[V], hx[V];
+        float2 hw[P] = {}, hx[P] = {};  // (their negatives)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          hw[i] = sums[2 * ((col * V + i) / a.cg)];
-          hx[i] = sums[2 * ((col * V + i) / a.cg) + 1];
+          Norm::at(hw, i) = -sums[2 * ((col * V + i) / a.cg)];
+          Norm::at(hx, i) = -sums[2 * ((col * V + i) / a.cg) + 1];
         }
         const int64_t at = l.base + col * V;
         auto one = [&](const Vec &vx, const Vec &vd, int64_t e) {
-          float o[V];
+          float2 o[P];
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            float xhat;
-            const float h = slope(vx, vd, i, xhat);
-            o[i] = rstd[i] * (h * w[i] - hw[i] - xhat * hx[i]);
+          for (int i = 0; i < P; ++i) {
+            float2 xhat;
+            const float2 h = slope(vx, vd, i, xhat);
+            o[i] = mul2(rstd[i], fma2(xhat, hx[i], fma2(h, w[i], hw[i])));
           }
           write((T *)a.out + e, o);
         };
@@ -492,7 +528,7 @@ struct Norm {
 
   static __device__ void clear_first(const NormArgs &a, const Place &p, const First &f) {
     if (p.len == a.P) return;
-    const float zero[V] = {};
+    const float2 zero[P] = {};
     pieces(a, f, a.P, [&](int, int row, int t0, int t1) {
       T *out = (T *)a.out + f.base + (int64_t)row * a.P;
       // (a vector that the row's last token is in has been written)
@@ -507,43 +543,39 @@ struct Norm {
     const T *x = (const T *)a.x;
     float *red = smem, *mine = red + 3 * kThreads, *all = mine + 3, *stat = all + 3 * a.split;
     if (a.phase != kApply) {
-      float k = 0.f, s = 0.f, q = 0.f;
+      float k = 0.f;
+      float2 s2 = {}, q2 = {};
       int n = 0;
       pieces(a, f, p.len, [&](int, int row, int t0, int t1) {
         const T *at = x + f.base + (int64_t)row * a.P;
-        auto one = [&](const Vec &v, int t) {
+        // a vector of `left` tokens, all of them or (at a row's last) some
+        auto one = [&](const Vec &v, int left) {
+          left = min(left, V);
           if (n == 0) k = v.f(0);
+          n += left;
 #pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (t + i < t1) {
-              const float d = v.f(i) - k;
-              s += d;
-              q = fmaf(d, d, q);
-              ++n;
-            }
+          for (int i = 0; i < P; ++i) {
+            float2 d = add2(get(v, i), both(-k));
+            if (left < V || V == 1) d = make_float2(2 * i < left ? d.x : 0.f, 2 * i + 1 < left ? d.y : 0.f);
+            s2 = add2(s2, d);
+            q2 = fma2(d, d, q2);
+          }
         };
         int t = t0 + f.lane * V;
         for (; t + ((kFlight - 1) * f.lanes + 1) * V <= t1; t += kFlight * f.lanes * V) {
           Vec u[kFlight];
 #pragma unroll
           for (int j = 0; j < kFlight; ++j) u[j].load(at + t + j * f.lanes * V);
-          if (n == 0) k = u[0].f(0);
 #pragma unroll
-          for (int j = 0; j < kFlight; ++j)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const float d = u[j].f(i) - k;
-              s += d;
-              q = fmaf(d, d, q);
-            }
-          n += kFlight * V;
+          for (int j = 0; j < kFlight; ++j) one(u[j], V);
         }
         for (; t < t1; t += f.lanes * V) {
           Vec v;
           v.load(at + t);
-          one(v, t);
+          one(v, t1 - t);
         }
       });
+      const float s = s2.x + s2.y, q = q2.x + q2.y;
       const float m = n ? s / n : 0.f;
       float *e = red + 3 * threadIdx.x;
       e[0] = (float)n;
@@ -569,13 +601,14 @@ struct Norm {
     pieces(a, f, p.len, [&](int, int row, int t0, int t1) {
       const int64_t at = f.base + (int64_t)row * a.P;
       const int ch = p.slab * a.cg + row;
-      const float scale = rstd * load_w<T>(a.w, ch, a.wf32, 1.f), shift = load_w<T>(a.b, ch, a.wf32, 0.f);
+      const float2 scale = both(rstd * load_w<T>(a.w, ch, a.wf32, 1.f)), shift = both(load_w<T>(a.b, ch, a.wf32, 0.f));
       auto one = [&](const Vec &v, int t) {
-        float y[V];
+        float2 y[P];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float pre = fmaf(v.f(i) - mean, scale, shift);
-          y[i] = t + i < t1 ? a.silu ? pre * sigmoid_f(pre) : pre : 0.f;
+        for (int i = 0; i < P; ++i) {
+          const float2 pre = fma2(add2(get(v, i), both(-mean)), scale, shift);
+          y[i] = a.silu ? mul2(pre, sigmoid2(pre)) : pre;
+          if (t + V > t1) y[i] = make_float2(t + 2 * i < t1 ? y[i].x : 0.f, t + 2 * i + 1 < t1 ? y[i].y : 0.f);
         }
         write((T *)a.out + at + t, y);
       };
@@ -607,13 +640,17 @@ struct Norm {
     const float *stats = a.stats + 2 * ((size_t)p.n * a.G + p.slab);
     const float mean = stats[0], rstd = stats[1];
     float w = 0.f, b = 0.f;
-    auto slope = [&](float vx, float vd, float &xhat) {
-      xhat = (vx - mean) * rstd;
-      if (a.silu) {
-        const float pre = fmaf(xhat, w, b);
-        vd *= silu_slope(pre, sigmoid_f(pre));
-      }
-      return vd;
+    auto slope = [&](const Vec &vx, const Vec &vd, int i, float2 &xhat) {
+      xhat = mul2(add2(get(vx, i), both(-mean)), both(rstd));
+      const float2 h = get(vd, i);
+      if (!a.silu) return h;
+      const float2 pre = fma2(xhat, both(w), both(b));
+      return mul2(h, silu_slope(pre, sigmoid2(pre)));
+    };
+    // pair i of a vector that has `left` tokens, with zeros behind them
+    auto held = [&](float2 v, int i, int left) {
+      left = min(left, V);
+      return left == V && V > 1 ? v : make_float2(2 * i < left ? v.x : 0.f, 2 * i + 1 < left ? v.y : 0.f);
     };
     auto channel = [&](int row) {
       w = load_w<T>(a.w, p.slab * a.cg + row, a.wf32, 1.f);
@@ -643,21 +680,21 @@ struct Norm {
       // (all lanes of a warp go through the same number of pieces)
       for (int i0 = f.begin; i0 < f.end; i0 += f.takers) {
         const int i = i0 + f.who;
-        float s = 0.f, q = 0.f;
+        float2 s2 = {}, q2 = {};
         if (i < f.end) {
           const int row = i / a.segs, t0 = (i - row * a.segs) * a.seg * V, t1 = min(t0 + a.seg * V, p.len);
           channel(row);
           vectors(f.base + (int64_t)row * a.P, t0, t1, [&](const Vec &u, const Vec &d, int t) {
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-              if (t + j < t1) {
-                float xhat;
-                const float h = slope(u.f(j), d.f(j), xhat);
-                s += h;
-                q = fmaf(h, xhat, q);
-              }
+            for (int j = 0; j < P; ++j) {
+              float2 xhat;
+              const float2 h = held(slope(u, d, j, xhat), j, t1 - t);
+              s2 = add2(s2, h);
+              q2 = add2(q2, held(mul2(h, xhat), j, t1 - t));
+            }
           });
         }
+        float s = s2.x + s2.y, q = q2.x + q2.y;
         for (int o = f.lanes >> 1; o; o >>= 1) {
           s += __shfl_xor_sync(0xffffffffu, s, o);
           q += __shfl_xor_sync(0xffffffffu, q, o);
@@ -683,12 +720,12 @@ struct Norm {
       channel(row);
       const int64_t at = f.base + (int64_t)row * a.P;
       vectors(at, t0, t1, [&](const Vec &u, const Vec &d, int t) {
-        float o[V];
+        float2 o[P];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float xhat;
-          const float h = slope(u.f(j), d.f(j), xhat);
-          o[j] = t + j < t1 ? rstd * (h * w - hw - xhat * hx) : 0.f;
+        for (int j = 0; j < P; ++j) {
+          float2 xhat;
+          const float2 h = slope(u, d, j, xhat);
+          o[j] = held(mul2(both(rstd), fma2(xhat, both(-hx), fma2(h, both(w), both(-hw)))), j, t1 - t);
         }
         write((T *)a.out + at + t, o);
       });
@@ -698,7 +735,7 @@ struct Norm {
 };
 
 template <typename T, int V, bool kLast, bool kBackward>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) norm_kernel(const NormArgs a) {
   extern __shared__ float smem[];
   if constexpr (kLast && kBackward) Norm<T, V>::backward_last(a, smem);
   else if constexpr (kLast) Norm<T, V>::forward_last(a, smem);
