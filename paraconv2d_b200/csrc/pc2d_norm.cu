@@ -10,9 +10,10 @@
 //
 // A slab, all that shares statistics (and, channels last, the neighbouring
 // groups that fill a few sectors of a token), is one cluster of 1 to 8 thread
-// blocks' work: they read it, exchange their partial sums through distributed
-// shared memory, and read it again, from the L2 cache, which holds the slabs of
-// all clusters at work.  Where there are too few slabs for the GPU, two launches
+// blocks' work.  They bring it into shared memory by asynchronous copies, all
+// under way at once, sum, exchange their sums through distributed shared memory,
+// and go over it again there; what does not fit is read again, from the L2
+// cache as a rule.  Each thread reads only what it has copied.  Where there are too few slabs for the GPU, two launches
 // share the same code and exchange the partial sums in device memory instead.
 //
 // Variance: each thread sums x - K and its square, K its own first value (of
@@ -38,6 +39,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxSplit = 64;         // blocks of a slab that exchange through device memory
 constexpr int kMaxChannels = 8192;    // of a slab: its sums are in shared memory
+constexpr int kCacheBytes = 64 * 1024;  // of a slab's share that a block keeps, x and dy together
 
 enum Phase { kFused, kSums, kApply };
 
@@ -51,8 +53,11 @@ struct NormArgs {
   int batch, C, P, G, cg;
   int slab_channels;    // channels of a slab: cg, or a multiple of it
   int slabs;            // slabs of a batch row
-  int split;            // blocks of a slab
+  int split, split_log;  // blocks of a slab, a power of two
+  int cols_log;         // channels last: 2^cols_log threads for the vectors of a slab's token
   int seg, segs;        // channels first: vectors and number of the pieces of a row
+  int red;              // channels last: numbers of the block's partial sums
+  int cache;            // vectors of an array that a thread keeps in shared memory
   int wf32;             // weight and bias in float32, else in x's type
   int silu;
   Phase phase;
@@ -71,15 +76,25 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// (Integer divisions are chains of tens of dependent instructions, which is what
+// a small block's time would go to: powers of two where that can be arranged,
+// and numbers that the host has divided.)
+
+// Where part i of 2^log equal parts of n begins.
+__device__ __forceinline__ int part_of(int n, int i, int log) {
+  const int each = n >> log;
+  return i * each + min(i, n - (each << log));
+}
+
 struct Place {
   int rank, n, slab, len;  // block of its slab; batch row; slab of the row; tokens of the row
 };
 __device__ __forceinline__ Place place_of(const NormArgs &a) {
   Place p;
-  p.rank = blockIdx.x % a.split;
-  const int unit = blockIdx.x / a.split;
-  p.n = unit / a.slabs;
-  p.slab = unit % a.slabs;
+  p.rank = blockIdx.x & (a.split - 1);
+  const int unit = blockIdx.x >> a.split_log;
+  p.n = a.slabs == 1 ? unit : unit / a.slabs;
+  p.slab = unit - p.n * a.slabs;
   p.len = a.lengths ? min(max(a.lengths[p.n], 0), a.P) : a.P;
   return p;
 }
@@ -89,8 +104,8 @@ __device__ __forceinline__ Place place_of(const NormArgs &a) {
 // all of its blocks.  False: this block is done.
 template <typename Take>
 __device__ __forceinline__ bool exchange(const NormArgs &a, const float *mine, int count, Take &&take) {
-  const int rank = blockIdx.x % a.split;
-  float *global = a.part + (size_t)(blockIdx.x / a.split) * a.split * count;
+  const int rank = blockIdx.x & (a.split - 1);
+  float *global = a.part + (size_t)(blockIdx.x - rank) * count;
   __syncthreads();
   if (a.phase == kSums) {
     for (int i = threadIdx.x; i < count; i += kThreads) global[(size_t)rank * count + i] = mine[i];
@@ -104,30 +119,46 @@ __device__ __forceinline__ bool exchange(const NormArgs &a, const float *mine, i
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     take([&](int r, int i) { return cluster.map_shared_rank(mine, r)[i]; });
-    cluster.sync();  // nobody leaves while its numbers are read
+    cluster.barrier_arrive();  // (and leave() at the end)
   }
   __syncthreads();
   return true;
 }
+// Nobody leaves while others may still read its numbers.
+__device__ __forceinline__ void leave(const NormArgs &a) {
+  if (a.phase == kFused && a.split > 1) cg::this_cluster().barrier_wait();
+}
 
-// (count, mean, M2) of `entries` entries by one warp, the mean and the M2 of
-// entry i at v[at(i)] and v[at(i) + 1] and its count n(i).
+// (count, mean, M2) of rows x cols entries by one warp, the mean and the M2 of
+// entry (r, c) at v[at(r, c)] and v[at(r, c) + 1] and its count n(r).
 template <typename At, typename Count>
-__device__ __forceinline__ void join(const float *v, int entries, At &&at, Count &&n, float &total, float &mean,
+__device__ __forceinline__ void join(const float *v, int rows, int cols, At &&at, Count &&n, float &total, float &mean,
                                      float &m2) {
-  const int lane = threadIdx.x & 31;
+  // lanes: 2^k columns by 32 / 2^k rows (no division, whose chain would be longer than all of this)
+  const int lane = threadIdx.x & 31, shift = cols >= 32 ? 5 : 31 - __clz(cols);
+  auto each = [&](auto &&f) {
+    for (int r = lane >> shift; r < rows; r += 32 >> shift) {
+      const float k = n(r);
+      for (int c = lane & ((1 << shift) - 1); c < cols; c += 1 << shift) f(at(r, c), k);
+    }
+  };
   float c = 0.f, s = 0.f, q = 0.f;
-  for (int i = lane; i < entries; i += 32) {
-    c += n(i);
-    s += n(i) * v[at(i)];
-  }
+  each([&](int i, float k) {
+    c += k;
+    s += k * v[i];
+  });
   total = warp_sum(c);
   mean = total > 0.f ? warp_sum(s) / total : 0.f;
-  for (int i = lane; i < entries; i += 32) {
-    const float d = v[at(i)] - mean;
-    q += n(i) > 0.f ? v[at(i) + 1] + n(i) * d * d : 0.f;
-  }
-  m2 = warp_sum(q);
+  // (the differences from it, whose sum corrects its rounding)
+  s = 0.f;
+  each([&](int i, float k) {
+    const float d = k > 0.f ? v[i] - mean : 0.f;
+    s = fmaf(k, d, s);
+    q += k > 0.f ? v[i + 1] + k * d * d : 0.f;
+  });
+  s = total > 0.f ? warp_sum(s) / total : 0.f;
+  m2 = warp_sum(q) - total * s * s;
+  mean += s;
 }
 
 // Pairs of numbers, one instruction for two.
@@ -152,11 +183,117 @@ __device__ __forceinline__ float2 silu_slope(float2 pre, float2 s) {
 template <typename T, int V>
 struct Norm {
   using Vec = Pack<T, V>;
+  static_assert(kThreads == 256, "Last");
   static constexpr int P = (V + 1) / 2;  // pairs of a vector (of one element: half of one)
 
-  // vectors in flight
-  static constexpr int kFlight = 4;
+  struct Two {
+    Vec x, d;
+  };
 
+  // vectors in flight
+  static constexpr int kFlight = 2;
+
+  // The weights of channels ch .. ch+V-1, or `none`.
+  static __device__ __forceinline__ void weights(float2 (&v)[P], const void *p, int ch, bool f32, float none) {
+    if (!p) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) at(v, i) = none;
+    } else if (f32) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) at(v, i) = static_cast<const float *>(p)[ch + i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) at(v, i) = to_f(static_cast<const T *>(p)[ch + i]);
+    }
+  }
+  // f(i, group of channel c + i) for the V channels from c on of a slab
+  template <typename F>
+  static __device__ __forceinline__ void with_groups(int c, int cg, F &&f) {
+    int g = c / cg, left = cg - (c - g * cg);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      f(i, g);
+      if (--left == 0) left = cg, ++g;
+    }
+  }
+
+  static constexpr bool kKeeps = V * sizeof(T) == 16;
+  // Vector `slot` of this thread, from `p`: copied ahead, and taken from the copy where there is one.
+  static __device__ __forceinline__ void ahead(const NormArgs &a, unsigned char *kept, int slot, const T *p) {
+    if constexpr (kKeeps) {
+      const unsigned to = (unsigned)__cvta_generic_to_shared(kept + ((size_t)slot * kThreads + threadIdx.x) * 16);
+      if (slot < a.cache) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p) : "memory");
+    }
+  }
+  static __device__ __forceinline__ void arrived() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+  static __device__ __forceinline__ Vec copied(const unsigned char *kept, int slot) {
+    Vec v;
+    *reinterpret_cast<uint4 *>(v.v) =
+        *reinterpret_cast<const uint4 *>(kept + ((size_t)slot * kThreads + threadIdx.x) * 16);
+    return v;
+  }
+  // use(vector i, i) for the thread's n vectors from `p` on, `stride` apart, the first one's slot given.
+  template <int U, typename Use>
+  static __device__ __forceinline__ void each(const NormArgs &a, const unsigned char *kept, int slot, const T *p,
+                                              int64_t stride, int n, Use &&use) {
+    int i = 0;
+    if constexpr (kKeeps) {
+      const int here = min(n, a.cache - slot);
+      if (here > 0) {
+        batches<1>(here, [&](int j) { return copied(kept, slot + j); }, use);
+        i = here;
+      }
+    }
+    batches<U>(
+        n - i,
+        [&](int j) {
+          Vec v;
+          v.load(p + (i + j) * stride);
+          return v;
+        },
+        [&](const Vec &v, int j) { use(v, i + j); });
+  }
+  template <int U, typename Use>
+  static __device__ __forceinline__ void each_two(const NormArgs &a, const unsigned char *kept, int slot, const T *p,
+                                                  const T *d, int64_t stride, int n, Use &&use) {
+    int i = 0;
+    if constexpr (kKeeps) {
+      const int here = min(n, a.cache - slot);
+      if (here > 0) {
+        batches<1>(here, [&](int j) { return Two{copied(kept, slot + j), copied(kept, a.cache + slot + j)}; }, use);
+        i = here;
+      }
+    }
+    batches<U>(
+        n - i,
+        [&](int j) {
+          Two v;
+          v.x.load(p + (i + j) * stride);
+          v.d.load(d + (i + j) * stride);
+          return v;
+        },
+        [&](const Two &v, int j) { use(v, i + j); });
+  }
+  // Calls f with SiLU as a constant.
+  template <typename F>
+  static __device__ __forceinline__ void by_silu(const NormArgs &a, F &&f) {
+    if (a.silu) f(std::true_type());
+    else f(std::false_type());
+  }
+
+  // use(get(i), i) for i < count, U of them in flight
+  template <int U, typename Get, typename Use>
+  static __device__ __forceinline__ void batches(int count, Get &&get, Use &&use) {
+    int i = 0;
+    if constexpr (U > 1) for (; i + U <= count; i += U) {
+      decltype(get(0)) u[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) u[j] = get(i + j);
+#pragma unroll
+      for (int j = 0; j < U; ++j) use(u[j], i + j);
+    }
+    for (; i < count; ++i) use(get(i), i);
+  }
   static __device__ __forceinline__ float2 get(const Vec &v, int i) {
     if constexpr (V == 1) {
       return make_float2(v.f(0), 0.f);
@@ -188,279 +325,322 @@ struct Norm {
   static __device__ __forceinline__ float &at(float2 (&v)[P], int i) { return i & 1 ? v[i >> 1].y : v[i >> 1].x; }
 
   // ------------------------------------------------------------ channels last
-  // Threads: `cols` vectors of channels by `rows` tokens; a slab of more
-  // vectors than threads is gone through by columns of `cols`.
+  // Threads: `cols` vectors of channels (a power of two: some lanes may have
+  // none) by `rows` tokens; a slab of more vectors than threads is gone through
+  // by columns of `cols`.
   struct Last {
-    int sc, sv, cols, rows, r0, r1;
+    int sc, sv, cols, rows, r0, r1, each, more;  // `each` tokens a thread, and one more for the first `more` rows
     int64_t base;  // of the slab's first channel at token 0
+    int tx, ty, log;
     __device__ Last(const NormArgs &a, const Place &p) {
       sc = min(a.slab_channels, a.C - p.slab * a.slab_channels);
       sv = sc / V;
-      cols = min(sv, kThreads);
-      rows = kThreads / cols;
-      r0 = (int)((int64_t)p.len * p.rank / a.split);
-      r1 = (int)((int64_t)p.len * (p.rank + 1) / a.split);
+      log = a.cols_log;
+      cols = 1 << log;
+      rows = kThreads >> log;
+      ty = threadIdx.x >> log;
+      tx = threadIdx.x & (cols - 1);
+      r0 = part_of(p.len, p.rank, a.split_log);
+      r1 = part_of(p.len, p.rank + 1, a.split_log);
+      each = (r1 - r0) >> (8 - log);  // (2^8 threads)
+      more = (r1 - r0) & (rows - 1);
       base = (int64_t)p.n * a.P * a.C + (int64_t)p.slab * a.slab_channels;
     }
-    __device__ float count(int ty) const { return (float)((r1 - r0 - ty + rows - 1) / rows); }
+    // Where a warp has whole rows of a slab, their sums are joined by shuffles: one row of sums for a warp.
+    __device__ bool folds() const { return log <= 5; }
+    __device__ int sum_rows() const { return folds() ? kWarps : rows; }
+    __device__ int sum_row(int ty) const { return folds() ? threadIdx.x >> 5 : ty; }
+    __device__ bool sums_here() const { return !folds() || (int)(threadIdx.x & 31) < cols; }
+    __device__ int warp_count(int warp) const {  // tokens of a warp's rows
+      const int per = 32 >> log, first = warp * per;
+      return per * each + min(max(more - first, 0), per);
+    }
+    __device__ int slots() const { return each + (more > 0); }
+    __device__ int count(int ty) const { return each + (ty < more); }
   };
 
   // Tokens behind the row's last: zeros.
   static __device__ void clear_last(const NormArgs &a, const Place &p, const Last &l) {
+    if (p.len == a.P) return;
     const float2 zero[P] = {};
-    const int behind = a.P - p.len, first = p.len + (int)((int64_t)behind * p.rank / a.split),
-              last = p.len + (int)((int64_t)behind * (p.rank + 1) / a.split);
+    const int behind = a.P - p.len, first = p.len + part_of(behind, p.rank, a.split_log),
+              last = p.len + part_of(behind, p.rank + 1, a.split_log);
     for (int64_t i = threadIdx.x; i < (int64_t)(last - first) * l.sv; i += kThreads)
       write((T *)a.out + l.base + (first + i / l.sv) * a.C + i % l.sv * V, zero);
   }
 
-  static __device__ void forward_last(const NormArgs &a, float *smem) {
+  static __device__ void forward_last(const NormArgs &a, unsigned char *kept) {
     const Place p = place_of(a);
     const Last l(a, p);
     const T *x = (const T *)a.x;
-    const int groups = l.sc / a.cg, tx = threadIdx.x % l.cols, ty = threadIdx.x / l.cols;
-    float *red = smem;                                    // [rows][sc][2]
-    float *mine = red + (size_t)2 * l.rows * l.sc;        // [groups][3]
-    float *all = mine + 3 * groups, *stat = all + (size_t)a.split * 3 * groups;  // [split][groups][3], [groups][2]
+    const int groups = l.sc / a.cg, tx = l.tx, ty = l.ty;
+    float *red = reinterpret_cast<float *>(kept + (size_t)a.cache * kThreads * 16);  // [rows][sc][2]
+    float *mine = red + a.red;                                                        // [groups][3]
+    float *all = mine + 3 * groups, *stat = all + 3 * kWarps;  // the block's parts [8][3]; [groups][2]
+    // f(column, its first slot, this thread's tokens) for the thread's columns
+    auto columns = [&](auto &&f) {
+      int slot = 0;
+      for (int c0 = 0; c0 < l.sv; c0 += l.cols, slot += l.slots()) f(c0 + tx, slot, c0 + tx < l.sv ? l.count(ty) : 0);
+    };
+    const int64_t stride = (int64_t)l.rows * a.C;
+    auto place = [&](int col) { return l.base + col * V + (int64_t)(l.r0 + ty) * a.C; };
     if (a.phase != kApply) {
-      for (int c0 = 0; c0 < l.sv; c0 += l.cols) {
-        const int col = c0 + tx;
-        if (ty < l.rows && col < l.sv) {
-          const T *at = x + l.base + col * V;
-          float2 k[P] = {}, s[P] = {}, q[P] = {};
-          const int first = l.r0 + ty;
-          auto one = [&](const Vec &v) {
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-              const float2 d = add2(get(v, i), k[i]);
-              s[i] = add2(s[i], d);
-              q[i] = fma2(d, d, q[i]);
-            }
-          };
-          if (first < l.r1) {
-            Vec v;
-            v.load(at + (int64_t)first * a.C);
+      if (a.cache) {
+        columns([&](int col, int slot, int n) {
+          const T *at = x + place(col);
+          for (int i = 0; i < min(n, a.cache - slot); ++i) ahead(a, kept, slot + i, at + i * stride);
+        });
+        arrived();
+      }
+      columns([&](int col, int slot, int n) {
+        float2 k[P] = {}, s[P] = {}, q[P] = {};
+        each<kFlight>(a, kept, slot, x + place(col), stride, n, [&](const Vec &v, int j) {
+          if (j == 0)
 #pragma unroll
             for (int i = 0; i < P; ++i) k[i] = mul2(get(v, i), both(-1.f));
-            int r = first + l.rows;
-            for (; r + (kFlight - 1) * l.rows < l.r1; r += kFlight * l.rows) {
-              Vec u[kFlight];
 #pragma unroll
-              for (int j = 0; j < kFlight; ++j) u[j].load(at + (int64_t)(r + j * l.rows) * a.C);
-#pragma unroll
-              for (int j = 0; j < kFlight; ++j) one(u[j]);
-            }
-            for (; r < l.r1; r += l.rows) {
-              v.load(at + (int64_t)r * a.C);
-              one(v);
-            }
+          for (int i = 0; i < P; ++i) {
+            const float2 d = add2(get(v, i), k[i]);
+            s[i] = add2(s[i], d);
+            q[i] = fma2(d, d, q[i]);
           }
-          const float n = l.count(ty), inv = n > 0.f ? 1.f / n : 0.f;
+        });
+        const float inv = n > 0 ? 1.f / n : 0.f;
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float m = Norm::at(s, i) * inv;
-            float *e = red + 2 * ((size_t)ty * l.sc + col * V + i);
-            e[0] = n > 0.f ? m - Norm::at(k, i) : 0.f;
-            e[1] = Norm::at(q, i) - Norm::at(s, i) * m;
+        for (int i = 0; i < P; ++i) {  // s: the mean, q: M2
+          const float2 m = mul2(s[i], both(inv));
+          q[i] = fma2(s[i], mul2(m, both(-1.f)), q[i]);
+          s[i] = n > 0 ? fma2(k[i], both(-1.f), m) : both(0.f);
+        }
+        if (l.folds()) {
+          float count = n;
+          for (int o = l.cols; o < 32; o <<= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, count, o), sum = count + other;
+            const float share = sum > 0.f ? other / sum : 0.f;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+              const float2 m = make_float2(__shfl_xor_sync(0xffffffffu, s[i].x, o), __shfl_xor_sync(0xffffffffu, s[i].y, o));
+              const float2 v = make_float2(__shfl_xor_sync(0xffffffffu, q[i].x, o), __shfl_xor_sync(0xffffffffu, q[i].y, o));
+              const float2 d = fma2(s[i], both(-1.f), m);
+              s[i] = fma2(d, both(share), s[i]);
+              q[i] = add2(add2(q[i], v), mul2(mul2(d, d), both(count * share)));
+            }
+            count = sum;
           }
         }
-      }
+        if (l.sums_here() && col < l.sv)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            float *e = red + 2 * ((size_t)l.sum_row(ty) * l.sc + col * V + i);
+            e[0] = Norm::at(s, i);
+            e[1] = Norm::at(q, i);
+          }
+      });
       __syncthreads();
-      for (int g = threadIdx.x >> 5; g < groups; g += kWarps) {
+      // few groups of many sums: several warps share one's rows
+      const int warp = threadIdx.x >> 5, share = l.sum_rows() * a.cg > 2048 && groups < kWarps ? kWarps / groups : 1;
+      for (int i = warp; i < groups * share; i += kWarps) {
+        const int g = share == 1 ? i : i / share, part = i - g * share, r0 = share == 1 ? 0 : l.sum_rows() * part / share,
+                  r1 = share == 1 ? l.sum_rows() : l.sum_rows() * (part + 1) / share;
         float n, mean, m2;
-        join(red, l.rows * a.cg, [&](int i) { return 2 * ((i / a.cg) * l.sc + g * a.cg + i % a.cg); },
-             [&](int i) { return l.count(i / a.cg); }, n, mean, m2);
+        join(red, r1 - r0, a.cg, [&](int r, int c) { return 2 * ((r0 + r) * l.sc + g * a.cg + c); },
+             [&](int r) { return (float)(l.folds() ? l.warp_count(r0 + r) : l.count(r0 + r)); }, n, mean, m2);
         if ((threadIdx.x & 31) == 0) {
-          mine[3 * g] = n;
-          mine[3 * g + 1] = mean;
-          mine[3 * g + 2] = m2;
+          float *out = share == 1 ? mine + 3 * g : all + 3 * i;
+          out[0] = n;
+          out[1] = mean;
+          out[2] = m2;
+        }
+      }
+      if (share > 1) {
+        __syncthreads();
+        if (warp < groups) {
+          float n, mean, m2;
+          join(all + 3 * warp * share, share, 1, [](int r, int) { return 3 * r + 1; },
+               [&](int r) { return all[3 * (warp * share + r)]; }, n, mean, m2);
+          if ((threadIdx.x & 31) == 0) {
+            mine[3 * warp] = n;
+            mine[3 * warp + 1] = mean;
+            mine[3 * warp + 2] = m2;
+          }
         }
       }
     }
-    if (!exchange(a, mine, 3 * groups, [&](auto &&number) {
-          for (int i = threadIdx.x; i < a.split * 3 * groups; i += kThreads)
-            all[i] = number(i / (3 * groups), i % (3 * groups));
-        }))
-      return;
-    finish_stats(a, p, all, stat, groups, p.slab * a.slab_channels / a.cg);
-    for (int c0 = 0; c0 < l.sv; c0 += l.cols) {
-      const int col = c0 + tx;
-      if (ty < l.rows && col < l.sv) {
-        float2 mean[P] = {}, scale[P] = {}, shift[P] = {};  // (the mean's negative)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int c = col * V + i, g = c / a.cg, ch = p.slab * a.slab_channels + c;
-          Norm::at(mean, i) = -stat[2 * g];
-          Norm::at(scale, i) = stat[2 * g + 1] * load_w<T>(a.w, ch, a.wf32, 1.f);
-          Norm::at(shift, i) = load_w<T>(a.b, ch, a.wf32, 0.f);
-        }
-        const int64_t at = l.base + col * V;
-        auto one = [&](const Vec &v, int64_t e) {
+    const int first = p.slab * (a.slab_channels / a.cg);
+    if (!exchange(a, mine, 3 * groups, [&](auto &&number) { finish_stats(a, p, number, stat, groups, first); })) return;
+    columns([&](int col, int slot, int n) {
+      if (!n) return;
+      float2 mean[P] = {}, scale[P] = {}, shift[P] = {};  // (the mean's negative)
+      const int ch = p.slab * a.slab_channels + col * V;
+      weights(scale, a.w, ch, a.wf32, 1.f);
+      weights(shift, a.b, ch, a.wf32, 0.f);
+      with_groups(col * V, a.cg, [&](int i, int g) {
+        Norm::at(mean, i) = -stat[2 * g];
+        Norm::at(scale, i) *= stat[2 * g + 1];
+      });
+      T *out = (T *)a.out + place(col);
+      by_silu(a, [&](auto silu) {
+        each<kFlight>(a, kept, slot, x + place(col), stride, n, [&](const Vec &v, int j) {
           float2 y[P];
 #pragma unroll
           for (int i = 0; i < P; ++i) {
             const float2 pre = fma2(add2(get(v, i), mean[i]), scale[i], shift[i]);
-            y[i] = a.silu ? mul2(pre, sigmoid2(pre)) : pre;
+            y[i] = decltype(silu)::value ? mul2(pre, sigmoid2(pre)) : pre;
           }
-          write((T *)a.out + e, y);
-        };
-        int r = l.r0 + ty;
-        for (; r + (kFlight - 1) * l.rows < l.r1; r += kFlight * l.rows) {
-          Vec u[kFlight];
-#pragma unroll
-          for (int j = 0; j < kFlight; ++j) u[j].load(x + at + (int64_t)(r + j * l.rows) * a.C);
-#pragma unroll
-          for (int j = 0; j < kFlight; ++j) one(u[j], at + (int64_t)(r + j * l.rows) * a.C);
-        }
-        for (; r < l.r1; r += l.rows) {
-          Vec v;
-          v.load(x + at + (int64_t)r * a.C);
-          one(v, at + (int64_t)r * a.C);
-        }
-      }
-    }
+          write(out + j * stride, y);
+        });
+      });
+    });
     clear_last(a, p, l);
+    leave(a);
   }
 
-  // Joins the blocks' (count, mean, M2) of each group to (mean, rstd).
-  static __device__ void finish_stats(const NormArgs &a, const Place &p, const float *all, float *stat, int groups,
-                                      int first) {
-    for (int g = threadIdx.x >> 5; g < groups; g += kWarps) {
-      float n, mean, m2;
-      join(all, a.split, [&](int i) { return 3 * (i * groups + g) + 1; }, [&](int i) { return all[3 * (i * groups + g)]; },
-           n, mean, m2);
-      const float rstd = n > 0.f ? 1.f / sqrtf(m2 / n + a.eps) : 0.f;
-      if ((threadIdx.x & 31) == 0) {
-        stat[2 * g] = mean;
-        stat[2 * g + 1] = rstd;
-        if (p.rank == 0 && a.stats) {
-          float *s = a.stats + 2 * ((size_t)p.n * a.G + first + g);
-          s[0] = mean;
-          s[1] = rstd;
-        }
+  // Joins the blocks' (count, mean, M2) of each group to (mean, rstd); a thread a group.
+  template <typename Number>
+  static __device__ __forceinline__ void finish_stats(const NormArgs &a, const Place &p, Number &&number, float *stat,
+                                                      int groups, int first) {
+    for (int g = threadIdx.x; g < groups; g += kThreads) {
+      float n = 0.f, s = 0.f, m2 = 0.f, off = 0.f;
+#pragma unroll 4
+      for (int r = 0; r < a.split; ++r) {
+        n += number(r, 3 * g);
+        s += number(r, 3 * g) * number(r, 3 * g + 1);
+        m2 += number(r, 3 * g + 2);
+      }
+      const float inv = n > 0.f ? 1.f / n : 0.f;
+      float mean = s * inv;
+#pragma unroll 4
+      for (int r = 0; r < a.split; ++r) {  // (as in join)
+        const float k = number(r, 3 * g), d = k > 0.f ? number(r, 3 * g + 1) - mean : 0.f;
+        off = fmaf(k, d, off);
+        m2 += k * d * d;
+      }
+      off *= inv;
+      m2 -= n * off * off;
+      mean += off;
+      const float rstd = n > 0.f ? 1.f / sqrtf((m2 < 0.f ? 0.f : m2) * inv + a.eps) : 0.f;
+      stat[2 * g] = mean;
+      stat[2 * g + 1] = rstd;
+      if (p.rank == 0 && a.stats) {
+        float *out = a.stats + 2 * ((size_t)p.n * a.G + first + g);
+        out[0] = mean;
+        out[1] = rstd;
       }
     }
-    __syncthreads();
   }
 
-  static __device__ void backward_last(const NormArgs &a, float *smem) {
+  static __device__ void backward_last(const NormArgs &a, unsigned char *kept) {
     const Place p = place_of(a);
     const Last l(a, p);
     const T *x = (const T *)a.x, *dy = (const T *)a.dy;
-    const int groups = l.sc / a.cg, tx = threadIdx.x % l.cols, ty = threadIdx.x / l.cols;
-    float *red = smem;                                 // [rows][sc][2]
-    float *mine = red + (size_t)2 * l.rows * l.sc;     // [sc][2]: sums of h and of h xhat
+    const int groups = l.sc / a.cg, tx = l.tx, ty = l.ty;
+    unsigned char *kept_d = kept + (size_t)a.cache * kThreads * 16;
+    float *red = reinterpret_cast<float *>(kept_d + (size_t)a.cache * kThreads * 16);  // [rows][sc][2]
+    float *mine = red + a.red;                                                          // [sc][2]: sums of h and of h xhat
     float *chan = mine + 2 * l.sc, *sums = chan + 2 * l.sc;  // [sc][2]; [groups][2]: means of h w and of h w xhat
     const float *stats = a.stats + 2 * ((size_t)p.n * a.G + p.slab * a.slab_channels / a.cg);
+    auto columns = [&](auto &&f) {
+      int slot = 0;
+      for (int c0 = 0; c0 < l.sv; c0 += l.cols, slot += l.slots()) f(c0 + tx, slot, c0 + tx < l.sv ? l.count(ty) : 0);
+    };
+    const int64_t stride = (int64_t)l.rows * a.C;
+    auto place = [&](int col) { return l.base + col * V + (int64_t)(l.r0 + ty) * a.C; };
     float2 mean[P] = {}, rstd[P] = {}, w[P] = {}, b[P] = {};  // (the mean's negative)
     auto channel = [&](int col) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int c = col * V + i, g = c / a.cg, ch = p.slab * a.slab_channels + c;
+      const int ch = p.slab * a.slab_channels + col * V;
+      weights(w, a.w, ch, a.wf32, 1.f);
+      weights(b, a.b, ch, a.wf32, 0.f);
+      with_groups(col * V, a.cg, [&](int i, int g) {
         Norm::at(mean, i) = -stats[2 * g];
         Norm::at(rstd, i) = stats[2 * g + 1];
-        Norm::at(w, i) = load_w<T>(a.w, ch, a.wf32, 1.f);
-        Norm::at(b, i) = load_w<T>(a.b, ch, a.wf32, 0.f);
-      }
+      });
     };
-    auto slope = [&](const Vec &vx, const Vec &vd, int i, float2 &xhat) {
-      xhat = mul2(add2(get(vx, i), mean[i]), rstd[i]);
-      const float2 h = get(vd, i);
-      if (!a.silu) return h;
+    auto slope = [&](auto silu, const Two &v, int i, float2 &xhat) {
+      xhat = mul2(add2(get(v.x, i), mean[i]), rstd[i]);
+      const float2 h = get(v.d, i);
+      if constexpr (!decltype(silu)::value) return h;
       const float2 pre = fma2(xhat, w[i], b[i]);
       return mul2(h, silu_slope(pre, sigmoid2(pre)));
     };
     if (a.phase != kApply) {
-      for (int c0 = 0; c0 < l.sv; c0 += l.cols) {
-        const int col = c0 + tx;
-        if (ty < l.rows && col < l.sv) {
-          channel(col);
-          const int64_t at = l.base + col * V;
-          float2 s[P] = {}, q[P] = {};
-          auto one = [&](const Vec &vx, const Vec &vd) {
+      if (a.cache)
+        columns([&](int col, int slot, int n) {
+          const int64_t at = place(col);
+          for (int i = 0; i < min(n, a.cache - slot); ++i) {
+            ahead(a, kept, slot + i, x + at + i * stride);
+            ahead(a, kept_d, slot + i, dy + at + i * stride);
+          }
+        });
+      columns([&](int col, int slot, int n) {
+        if (n) channel(col);
+        if (slot == 0) arrived();
+        float2 s[P] = {}, q[P] = {};
+        by_silu(a, [&](auto silu) {
+          each_two<2>(a, kept, slot, x + place(col), dy + place(col), stride, n, [&](const Two &v, int) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
               float2 xhat;
-              const float2 h = slope(vx, vd, i, xhat);
+              const float2 h = slope(silu, v, i, xhat);
               s[i] = add2(s[i], h);
               q[i] = fma2(h, xhat, q[i]);
             }
-          };
-          int r = l.r0 + ty;
-          for (; r + l.rows < l.r1; r += 2 * l.rows) {
-            Vec u[2], d[2];
+          });
+        });
+        if (l.folds())
+          for (int o = l.cols; o < 32; o <<= 1)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              u[j].load(x + at + (int64_t)(r + j * l.rows) * a.C);
-              d[j].load(dy + at + (int64_t)(r + j * l.rows) * a.C);
+            for (int i = 0; i < P; ++i) {
+              s[i] = add2(s[i], make_float2(__shfl_xor_sync(0xffffffffu, s[i].x, o), __shfl_xor_sync(0xffffffffu, s[i].y, o)));
+              q[i] = add2(q[i], make_float2(__shfl_xor_sync(0xffffffffu, q[i].x, o), __shfl_xor_sync(0xffffffffu, q[i].y, o)));
             }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) one(u[j], d[j]);
-          }
-          for (; r < l.r1; r += l.rows) {
-            Vec u, d;
-            u.load(x + at + (int64_t)r * a.C);
-            d.load(dy + at + (int64_t)r * a.C);
-            one(u, d);
-          }
+        if (l.sums_here() && col < l.sv)
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            float *e = red + 2 * ((size_t)ty * l.sc + col * V + i);
+            float *e = red + 2 * ((size_t)l.sum_row(ty) * l.sc + col * V + i);
             e[0] = Norm::at(s, i);
             e[1] = Norm::at(q, i);
           }
-        }
-      }
+      });
       __syncthreads();
-      for (int i = threadIdx.x; i < 2 * l.sc; i += kThreads) {
+      // a number's rows over up to 32 lanes
+      int lanes = 1;
+      const int rows = l.sum_rows();
+      while (lanes < 32 && lanes * 2 <= rows && lanes * 4 * l.sc <= kThreads) lanes *= 2;
+      for (int i0 = 0; i0 < 2 * l.sc; i0 += kThreads / lanes) {
+        const int i = i0 + threadIdx.x / lanes;
         float s = 0.f;
-        for (int r = 0; r < l.rows; ++r) s += red[(size_t)2 * r * l.sc + i];
-        mine[i] = s;
+        if (i < 2 * l.sc)
+          for (int r = threadIdx.x % lanes; r < rows; r += lanes) s += red[(size_t)2 * r * l.sc + i];
+        for (int o = lanes >> 1; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (i < 2 * l.sc && threadIdx.x % lanes == 0) mine[i] = s;
       }
     }
     if (!exchange(a, mine, 2 * l.sc, [&](auto &&number) { join_sums(a, chan, l.sc, number); })) return;
     finish_sums(a, p, sums, chan, l.sc, groups, p.slab * a.slab_channels);
-    for (int c0 = 0; c0 < l.sv; c0 += l.cols) {
-      const int col = c0 + tx;
-      if (ty < l.rows && col < l.sv) {
-        channel(col);
-        float2 hw[P] = {}, hx[P] = {};  // (their negatives)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          Norm::at(hw, i) = -sums[2 * ((col * V + i) / a.cg)];
-          Norm::at(hx, i) = -sums[2 * ((col * V + i) / a.cg) + 1];
-        }
-        const int64_t at = l.base + col * V;
-        auto one = [&](const Vec &vx, const Vec &vd, int64_t e) {
+    columns([&](int col, int slot, int n) {
+      if (!n) return;
+      channel(col);
+      float2 hw[P] = {}, hx[P] = {};  // (their negatives)
+      with_groups(col * V, a.cg, [&](int i, int g) {
+        Norm::at(hw, i) = -sums[2 * g];
+        Norm::at(hx, i) = -sums[2 * g + 1];
+      });
+      T *out = (T *)a.out + place(col);
+      by_silu(a, [&](auto silu) {
+        each_two<2>(a, kept, slot, x + place(col), dy + place(col), stride, n, [&](const Two &v, int j) {
           float2 o[P];
 #pragma unroll
           for (int i = 0; i < P; ++i) {
             float2 xhat;
-            const float2 h = slope(vx, vd, i, xhat);
+            const float2 h = slope(silu, v, i, xhat);
             o[i] = mul2(rstd[i], fma2(xhat, hx[i], fma2(h, w[i], hw[i])));
           }
-          write((T *)a.out + e, o);
-        };
-        int r = l.r0 + ty;
-        for (; r + l.rows < l.r1; r += 2 * l.rows) {
-          Vec u[2], d[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            u[j].load(x + at + (int64_t)(r + j * l.rows) * a.C);
-            d[j].load(dy + at + (int64_t)(r + j * l.rows) * a.C);
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) one(u[j], d[j], at + (int64_t)(r + j * l.rows) * a.C);
-        }
-        for (; r < l.r1; r += l.rows) {
-          Vec u, d;
-          u.load(x + at + (int64_t)r * a.C);
-          d.load(dy + at + (int64_t)r * a.C);
-          one(u, d, at + (int64_t)r * a.C);
-        }
-      }
-    }
+          write(out + j * stride, o);
+        });
+      });
+    });
     clear_last(a, p, l);
+    leave(a);
   }
 
   // Joins the blocks' sums of a slab's channels.
@@ -509,50 +689,62 @@ struct Norm {
       lane = threadIdx.x % lanes;
       who = threadIdx.x / lanes;
       takers = kThreads / lanes;
-      const int64_t pieces = (int64_t)a.cg * a.segs;
-      begin = (int)(pieces * p.rank / a.split);
-      end = (int)(pieces * (p.rank + 1) / a.split);
+      begin = part_of(a.cg * a.segs, p.rank, a.split_log);
+      end = part_of(a.cg * a.segs, p.rank + 1, a.split_log);
       base = ((int64_t)p.n * a.C + (int64_t)p.slab * a.cg) * a.P;
     }
   };
 
-  // Calls body(row, first token, last token) for this thread's pieces, the
-  // tokens cut at `len`.
+  // Calls body(row, first token, end, first slot, vectors) for this thread's
+  // pieces, the tokens cut at `len`: the thread's own are every f.lanes-th vector
+  // from the first token on.
   template <typename Body>
   static __device__ __forceinline__ void pieces(const NormArgs &a, const First &f, int len, Body &&body) {
+    int slot = 0;
     for (int i = f.begin + f.who; i < f.end; i += f.takers) {
-      const int row = i / a.segs, t0 = (i - row * a.segs) * a.seg * V;
-      body(i, row, t0, min(t0 + a.seg * V, len));
+      const int row = i / a.segs, t0 = (i - row * a.segs) * a.seg * V, t1 = min(t0 + a.seg * V, len);
+      const int left = t1 - t0 - f.lane * V, n = left > 0 ? (left - 1) / (f.lanes * V) + 1 : 0;
+      body(row, t0 + f.lane * V, t1, slot, n);
+      slot += n;
     }
   }
 
   static __device__ void clear_first(const NormArgs &a, const Place &p, const First &f) {
     if (p.len == a.P) return;
     const float2 zero[P] = {};
-    pieces(a, f, a.P, [&](int, int row, int t0, int t1) {
+    pieces(a, f, a.P, [&](int row, int t, int t1, int, int) {
       T *out = (T *)a.out + f.base + (int64_t)row * a.P;
       // (a vector that the row's last token is in has been written)
-      for (int t = t0 + f.lane * V; t < t1; t += f.lanes * V)
+      for (; t < t1; t += f.lanes * V)
         if (t >= p.len) write(out + t, zero);
     });
   }
 
-  static __device__ void forward_first(const NormArgs &a, float *smem) {
+  static __device__ void forward_first(const NormArgs &a, unsigned char *kept) {
     const Place p = place_of(a);
     const First f(a, p);
     const T *x = (const T *)a.x;
-    float *red = smem, *mine = red + 3 * kThreads, *all = mine + 3, *stat = all + 3 * a.split;
+    float *red = reinterpret_cast<float *>(kept + (size_t)a.cache * kThreads * 16);
+    float *mine = red + 3 * kThreads, *stat = mine + 3;
+    const int step = f.lanes * V;
     if (a.phase != kApply) {
+      if (a.cache) {
+        pieces(a, f, p.len, [&](int row, int t0, int, int slot, int n) {
+          const T *at = x + f.base + (int64_t)row * a.P + t0;
+          for (int i = 0; i < n && slot + i < a.cache; ++i) ahead(a, kept, slot + i, at + i * step);
+        });
+        arrived();
+      }
       float k = 0.f;
       float2 s2 = {}, q2 = {};
-      int n = 0;
-      pieces(a, f, p.len, [&](int, int row, int t0, int t1) {
-        const T *at = x + f.base + (int64_t)row * a.P;
-        // a vector of `left` tokens, all of them or (at a row's last) some
-        auto one = [&](const Vec &v, int left) {
-          left = min(left, V);
-          if (n == 0) k = v.f(0);
-          n += left;
+      int count = 0;
+      pieces(a, f, p.len, [&](int row, int t0, int t1, int slot, int n) {
+        const T *at = x + f.base + (int64_t)row * a.P + t0;
+        each<kFlight>(a, kept, slot, at, step, n, [&](const Vec &v, int j) {
+          // all of a vector's tokens, or (at a row's last) some
+          const int left = min(t1 - t0 - j * step, V);
+          if (count == 0) k = v.f(0);
+          count += left;
 #pragma unroll
           for (int i = 0; i < P; ++i) {
             float2 d = add2(get(v, i), both(-k));
@@ -560,31 +752,17 @@ struct Norm {
             s2 = add2(s2, d);
             q2 = fma2(d, d, q2);
           }
-        };
-        int t = t0 + f.lane * V;
-        for (; t + ((kFlight - 1) * f.lanes + 1) * V <= t1; t += kFlight * f.lanes * V) {
-          Vec u[kFlight];
-#pragma unroll
-          for (int j = 0; j < kFlight; ++j) u[j].load(at + t + j * f.lanes * V);
-#pragma unroll
-          for (int j = 0; j < kFlight; ++j) one(u[j], V);
-        }
-        for (; t < t1; t += f.lanes * V) {
-          Vec v;
-          v.load(at + t);
-          one(v, t1 - t);
-        }
+        });
       });
-      const float s = s2.x + s2.y, q = q2.x + q2.y;
-      const float m = n ? s / n : 0.f;
+      const float s = s2.x + s2.y, q = q2.x + q2.y, m = count ? s / count : 0.f;
       float *e = red + 3 * threadIdx.x;
-      e[0] = (float)n;
-      e[1] = n ? k + m : 0.f;
+      e[0] = (float)count;
+      e[1] = count ? k + m : 0.f;
       e[2] = q - s * m;
       __syncthreads();
       if (threadIdx.x < 32) {
         float total, mean, m2;
-        join(red, kThreads, [](int i) { return 3 * i + 1; }, [&](int i) { return red[3 * i]; }, total, mean, m2);
+        join(red, kThreads, 1, [](int r, int) { return 3 * r + 1; }, [&](int r) { return red[3 * r]; }, total, mean, m2);
         if (threadIdx.x == 0) {
           mine[0] = total;
           mine[1] = mean;
@@ -592,59 +770,50 @@ struct Norm {
         }
       }
     }
-    if (!exchange(a, mine, 3, [&](auto &&number) {
-          for (int i = threadIdx.x; i < a.split * 3; i += kThreads) all[i] = number(i / 3, i % 3);
-        }))
-      return;
-    finish_stats(a, p, all, stat, 1, p.slab);
-    const float mean = stat[0], rstd = stat[1];
-    pieces(a, f, p.len, [&](int, int row, int t0, int t1) {
-      const int64_t at = f.base + (int64_t)row * a.P;
+    if (!exchange(a, mine, 3, [&](auto &&number) { finish_stats(a, p, number, stat, 1, p.slab); })) return;
+    const float2 mean = both(-stat[0]);
+    const float rstd = stat[1];
+    pieces(a, f, p.len, [&](int row, int t0, int t1, int slot, int n) {
+      const int64_t at = f.base + (int64_t)row * a.P + t0;
       const int ch = p.slab * a.cg + row;
       const float2 scale = both(rstd * load_w<T>(a.w, ch, a.wf32, 1.f)), shift = both(load_w<T>(a.b, ch, a.wf32, 0.f));
-      auto one = [&](const Vec &v, int t) {
-        float2 y[P];
+      by_silu(a, [&](auto silu) {
+        each<kFlight>(a, kept, slot, x + at, step, n, [&](const Vec &v, int j) {
+          const int left = t1 - t0 - j * step;
+          float2 y[P];
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-          const float2 pre = fma2(add2(get(v, i), both(-mean)), scale, shift);
-          y[i] = a.silu ? mul2(pre, sigmoid2(pre)) : pre;
-          if (t + V > t1) y[i] = make_float2(t + 2 * i < t1 ? y[i].x : 0.f, t + 2 * i + 1 < t1 ? y[i].y : 0.f);
-        }
-        write((T *)a.out + at + t, y);
-      };
-      int t = t0 + f.lane * V;
-      for (; t + ((kFlight - 1) * f.lanes + 1) * V <= t1; t += kFlight * f.lanes * V) {
-        Vec u[kFlight];
-#pragma unroll
-        for (int j = 0; j < kFlight; ++j) u[j].load(x + at + t + j * f.lanes * V);
-#pragma unroll
-        for (int j = 0; j < kFlight; ++j) one(u[j], t + j * f.lanes * V);
-      }
-      for (; t < t1; t += f.lanes * V) {
-        Vec v;
-        v.load(x + at + t);
-        one(v, t);
-      }
+          for (int i = 0; i < P; ++i) {
+            const float2 pre = fma2(add2(get(v, i), mean), scale, shift);
+            y[i] = decltype(silu)::value ? mul2(pre, sigmoid2(pre)) : pre;
+            if (left < V) y[i] = make_float2(2 * i < left ? y[i].x : 0.f, 2 * i + 1 < left ? y[i].y : 0.f);
+          }
+          write((T *)a.out + at + j * step, y);
+        });
+      });
     });
     clear_first(a, p, f);
+    leave(a);
   }
 
-  static __device__ void backward_first(const NormArgs &a, float *smem) {
+  static __device__ void backward_first(const NormArgs &a, unsigned char *kept) {
     const Place p = place_of(a);
     const First f(a, p);
     const T *x = (const T *)a.x, *dy = (const T *)a.dy;
+    unsigned char *kept_d = kept + (size_t)a.cache * kThreads * 16;
     const int most = (int)(((int64_t)a.cg * a.segs + a.split - 1) / a.split) + 1;  // pieces of a block
-    float *red = smem;                                   // [pieces][2]
-    float *mine = red + (size_t)2 * most;                // [cg][2]
+    float *red = reinterpret_cast<float *>(kept_d + (size_t)a.cache * kThreads * 16);  // [pieces][2]
+    float *mine = red + (size_t)2 * most;                                               // [cg][2]
     float *chan = mine + 2 * a.cg, *sums = chan + 2 * a.cg;
     const float *stats = a.stats + 2 * ((size_t)p.n * a.G + p.slab);
-    const float mean = stats[0], rstd = stats[1];
-    float w = 0.f, b = 0.f;
-    auto slope = [&](const Vec &vx, const Vec &vd, int i, float2 &xhat) {
-      xhat = mul2(add2(get(vx, i), both(-mean)), both(rstd));
-      const float2 h = get(vd, i);
-      if (!a.silu) return h;
-      const float2 pre = fma2(xhat, both(w), both(b));
+    const float2 mean = both(-stats[0]), rstd = both(stats[1]);
+    const int step = f.lanes * V;
+    constexpr bool kReuse = kKeeps && sizeof(T) == 4;
+    float2 w = {}, b = {};
+    auto slope = [&](auto silu, const Two &v, int i, float2 &xhat) {
+      xhat = mul2(add2(get(v.x, i), mean), rstd);
+      const float2 h = get(v.d, i);
+      if constexpr (!decltype(silu)::value) return h;
+      const float2 pre = fma2(xhat, w, b);
       return mul2(h, silu_slope(pre, sigmoid2(pre)));
     };
     // pair i of a vector that has `left` tokens, with zeros behind them
@@ -653,46 +822,46 @@ struct Norm {
       return left == V && V > 1 ? v : make_float2(2 * i < left ? v.x : 0.f, 2 * i + 1 < left ? v.y : 0.f);
     };
     auto channel = [&](int row) {
-      w = load_w<T>(a.w, p.slab * a.cg + row, a.wf32, 1.f);
-      b = load_w<T>(a.b, p.slab * a.cg + row, a.wf32, 0.f);
-    };
-    // body(x, dy, token) for this thread's vectors of a piece, two in flight
-    auto vectors = [&](int64_t at, int t0, int t1, auto &&body) {
-      int t = t0 + f.lane * V;
-      for (; t + f.lanes * V < t1; t += 2 * f.lanes * V) {
-        Vec u[2], d[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          u[j].load(x + at + t + j * f.lanes * V);
-          d[j].load(dy + at + t + j * f.lanes * V);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) body(u[j], d[j], t + j * f.lanes * V);
-      }
-      if (t < t1) {
-        Vec u, d;
-        u.load(x + at + t);
-        d.load(dy + at + t);
-        body(u, d, t);
-      }
+      w = both(load_w<T>(a.w, p.slab * a.cg + row, a.wf32, 1.f));
+      b = both(load_w<T>(a.b, p.slab * a.cg + row, a.wf32, 0.f));
     };
     if (a.phase != kApply) {
+      if (a.cache) {
+        pieces(a, f, p.len, [&](int row, int t0, int, int slot, int n) {
+          const int64_t at = f.base + (int64_t)row * a.P + t0;
+          for (int i = 0; i < n && slot + i < a.cache; ++i) {
+            ahead(a, kept, slot + i, x + at + i * step);
+            ahead(a, kept_d, slot + i, dy + at + i * step);
+          }
+        });
+        arrived();
+      }
       // (all lanes of a warp go through the same number of pieces)
+      int slot = 0;
       for (int i0 = f.begin; i0 < f.end; i0 += f.takers) {
         const int i = i0 + f.who;
         float2 s2 = {}, q2 = {};
         if (i < f.end) {
-          const int row = i / a.segs, t0 = (i - row * a.segs) * a.seg * V, t1 = min(t0 + a.seg * V, p.len);
+          const int row = i / a.segs, start = (i - row * a.segs) * a.seg * V, t1 = min(start + a.seg * V, p.len);
+          const int t0 = start + f.lane * V, n = t1 > t0 ? (t1 - t0 - 1) / step + 1 : 0;
           channel(row);
-          vectors(f.base + (int64_t)row * a.P, t0, t1, [&](const Vec &u, const Vec &d, int t) {
+          const int64_t at = f.base + (int64_t)row * a.P + t0;
+          by_silu(a, [&](auto silu) {
+            each_two<2>(a, kept, slot, x + at, dy + at, step, n, [&](const Two &v, int j) {
+              float2 h[P];
 #pragma unroll
-            for (int j = 0; j < P; ++j) {
-              float2 xhat;
-              const float2 h = held(slope(u, d, j, xhat), j, t1 - t);
-              s2 = add2(s2, h);
-              q2 = add2(q2, held(mul2(h, xhat), j, t1 - t));
-            }
+              for (int e = 0; e < P; ++e) {
+                float2 xhat;
+                h[e] = held(slope(silu, v, e, xhat), e, t1 - t0 - j * step);
+                s2 = add2(s2, h[e]);
+                q2 = add2(q2, held(mul2(h[e], xhat), e, t1 - t0 - j * step));
+              }
+              // (in 32 bits, what the second pass needs of dy is kept in its place)
+              if (kReuse && slot + j < a.cache)
+                write(reinterpret_cast<T *>(kept_d + ((size_t)(slot + j) * kThreads + threadIdx.x) * 16), h);
+            });
           });
+          slot += n;
         }
         float s = s2.x + s2.y, q = q2.x + q2.y;
         for (int o = f.lanes >> 1; o; o >>= 1) {
@@ -715,28 +884,35 @@ struct Norm {
     }
     if (!exchange(a, mine, 2 * a.cg, [&](auto &&number) { join_sums(a, chan, a.cg, number); })) return;
     finish_sums(a, p, sums, chan, a.cg, 1, p.slab * a.cg);
-    const float hw = sums[0], hx = sums[1];
-    pieces(a, f, p.len, [&](int, int row, int t0, int t1) {
+    const float2 hw = both(-sums[0]), hx = both(-sums[1]);
+    pieces(a, f, p.len, [&](int row, int t0, int t1, int slot, int n) {
       channel(row);
-      const int64_t at = f.base + (int64_t)row * a.P;
-      vectors(at, t0, t1, [&](const Vec &u, const Vec &d, int t) {
-        float2 o[P];
+      const int64_t at = f.base + (int64_t)row * a.P + t0;
+      auto last_pass = [&](auto silu, int slot, int64_t at, int t0, int n) {
+        each_two<2>(a, kept, slot, x + at, dy + at, step, n, [&](const Two &v, int j) {
+          float2 o[P];
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
-          float2 xhat;
-          const float2 h = slope(u, d, j, xhat);
-          o[j] = held(mul2(both(rstd), fma2(xhat, both(-hx), fma2(h, both(w), both(-hw)))), j, t1 - t);
-        }
-        write((T *)a.out + at + t, o);
-      });
+          for (int e = 0; e < P; ++e) {
+            float2 xhat;
+            const float2 h = slope(silu, v, e, xhat);
+            o[e] = held(mul2(rstd, fma2(xhat, hx, fma2(h, w, hw))), e, t1 - t0 - j * step);
+          }
+          write((T *)a.out + at + j * step, o);
+        });
+      };
+      const int here = kReuse ? min(n, max(0, a.cache - slot)) : 0;  // dy's places hold h
+      if (here) last_pass(std::false_type(), slot, at, t0, here);
+      if (here < n)
+        by_silu(a, [&](auto silu) { last_pass(silu, slot + here, at + here * step, t0 + here * step, n - here); });
     });
     clear_first(a, p, f);
+    leave(a);
   }
 };
 
 template <typename T, int V, bool kLast, bool kBackward>
 __global__ void __launch_bounds__(kThreads, 3) norm_kernel(const NormArgs a) {
-  extern __shared__ float smem[];
+  extern __shared__ __align__(16) unsigned char smem[];
   if constexpr (kLast && kBackward) Norm<T, V>::backward_last(a, smem);
   else if constexpr (kLast) Norm<T, V>::forward_last(a, smem);
   else if constexpr (kBackward) Norm<T, V>::backward_first(a, smem);
@@ -764,7 +940,7 @@ __global__ void __launch_bounds__(kThreads) norm_weight_kernel(const float *chan
 
 // The launch of a problem: how its slabs are cut and shared.
 struct Plan {
-  int V, slab_channels, slabs, split, seg, segs;
+  int V, slab_channels, slabs, split, seg, segs, cache, red, cols_log;
   bool fused;
   size_t numbers;  // of a block's part
   size_t smem, part_bytes;
@@ -780,8 +956,9 @@ Plan make_plan(int size, bool last, bool backward, int batch, int C, int P, int 
     p.V = v;
     p.slab_channels = cg;
     if (!last) break;
-    // whole groups, whole vectors and 128 bytes of a token (the L2 cache's line) where the channels allow it
-    while (p.slab_channels < C && (p.slab_channels % v || p.slab_channels * size < 128)) p.slab_channels += cg;
+    // whole groups, whole vectors and 64 bytes of a token where the channels allow it (with 128 a block's share of
+    // 16 maps of 512x64x64 bf16 has no room in shared memory)
+    while (p.slab_channels < C && (p.slab_channels % v || p.slab_channels * size < 64)) p.slab_channels += cg;
     if (p.slab_channels <= kMaxChannels) break;
   }
   p.slabs = ceil_div(C, p.slab_channels);
@@ -811,10 +988,29 @@ Plan make_plan(int size, bool last, bool backward, int batch, int C, int P, int 
   const int sc = p.slab_channels, groups = sc / cg;
   p.numbers = backward ? 2 * (size_t)sc : 3 * (size_t)groups;
   size_t red;
-  if (last) red = 2 * (size_t)std::max(kThreads * p.V, sc);
+  if (last) {
+    // (as Last::sum_rows(): a row of sums for a warp, or for each row of threads)
+    while (p.cols_log < 8 && 1 << p.cols_log < sc / p.V) ++p.cols_log;
+    red = 2 * (size_t)sc * (p.cols_log <= 5 ? kWarps : kThreads >> p.cols_log);
+    p.red = (int)red;
+  }
   else if (backward) red = 2 * ((size_t)ceil_div((int64_t)cg * p.segs, p.split) + 1);
   else red = 3 * kThreads;
-  p.smem = 4 * (red + p.numbers * (backward ? 2 : 1 + p.split) + 2 * (size_t)groups);
+  // what a block keeps: as many of its vectors as there is room for
+  const int arrays = backward ? 2 : 1;
+  const size_t sums = 4 * (red + p.numbers * (backward ? 2 : 1) + 2 * (size_t)groups + 3 * kWarps);
+  const size_t space = std::min<size_t>(kCacheBytes, 224 * 1024 - sums);
+  const int room = (int)(space / (kThreads * 16 * arrays));
+  int64_t need;
+  if (last) {
+    need = (int64_t)ceil_div(ceil_div(P, p.split), kThreads >> p.cols_log) * ceil_div(sc / p.V, 1 << p.cols_log);
+  } else {
+    int lanes = 32;
+    while (lanes > 1 && lanes / 2 >= p.seg) lanes >>= 1;
+    need = (int64_t)ceil_div(ceil_div((int64_t)cg * p.segs, p.split), kThreads / lanes) * ceil_div(p.seg, lanes);
+  }
+  p.cache = p.fused && p.V == widest ? (int)std::min<int64_t>(need, room) : 0;
+  p.smem = (size_t)p.cache * arrays * kThreads * 16 + sums;
   p.part_bytes = p.fused ? 0 : (size_t)units * p.split * p.numbers * 4;
   return p;
 }
@@ -944,7 +1140,11 @@ extern "C" int pc2d_group_norm_forward(int dtype, int wdtype, int channels_last,
   a.slab_channels = p.slab_channels;
   a.slabs = p.slabs;
   a.split = p.split;
+  a.split_log = 31 - __builtin_clz(p.split);
+  a.cols_log = p.cols_log;
   a.seg = p.seg;
+  a.cache = p.cache;
+  a.red = p.red;
   a.segs = p.segs;
   a.wf32 = wdtype == PC2D_DTYPE_F32;
   a.silu = silu;
@@ -1008,7 +1208,11 @@ extern "C" int pc2d_group_norm_backward(int dtype, int wdtype, int channels_last
   a.slab_channels = p.slab_channels;
   a.slabs = p.slabs;
   a.split = p.split;
+  a.split_log = 31 - __builtin_clz(p.split);
+  a.cols_log = p.cols_log;
   a.seg = p.seg;
+  a.cache = p.cache;
+  a.red = p.red;
   a.segs = p.segs;
   a.wf32 = wdtype == PC2D_DTYPE_F32;
   a.silu = silu;
