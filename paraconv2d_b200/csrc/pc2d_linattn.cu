@@ -135,31 +135,39 @@ __device__ __forceinline__ void split(float x, float y, uint32_t (&p)[N]) {
   }
 }
 
-// A matrix in shared memory: rows of `bytes` bytes of 16-bit numbers, their
-// 16-byte pieces exchanged within the row so that the eight rows of an
-// ldmatrix are in different banks.  Planes follow one another.
+// A matrix in shared memory: rows of RB bytes (0: of `bytes`, 128 or 256) of
+// 16-bit numbers, their 16-byte pieces exchanged within the row so that the eight
+// rows of an ldmatrix are in different banks.  Planes follow one another.
+template <int RB>
 struct Tile {
   uint32_t at;
-  int bytes, plane;
+  int plane, bytes;
+  __device__ __forceinline__ Tile(uint32_t at, int plane, int bytes = RB) : at(at), plane(plane), bytes(bytes) {}
+  __device__ __forceinline__ int row_bytes() const { return RB ? RB : bytes; }
+  static __device__ __forceinline__ int turn(int row) { return RB == 64 ? row >> 1 & 3 : row & 7; }
   __device__ __forceinline__ uint32_t piece(int row, int col8, int p = 0) const {
-    const int turn = bytes == 64 ? row >> 1 & 3 : row & 7;
-    return at + p * plane + row * bytes + ((col8 ^ turn) << 4);
+    return at + p * plane + row * row_bytes() + ((col8 ^ turn(row)) << 4);
+  }
+  // The address that this lane gives an ldmatrix of the 16x16 numbers at (row, col), both multiples of 16: of its
+  // four 8x8 parts, the second one to the right (kRight) or below.
+  template <bool kRight>
+  __device__ __forceinline__ uint32_t part(int row, int col, int p) const {
+    const int lane = threadIdx.x & 31, w = lane & 7, i = lane >> 3, down = kRight ? i >> 1 : i & 1, right = kRight ? i & 1 : i >> 1;
+    return at + (down * 8 + w) * row_bytes() + p * plane + row * row_bytes() + ((col >> 3 ^ (right ^ turn(w))) << 4);
   }
 };
 // The 16x16 operand A (rows m, columns k) of a product, stored [m][k] or (trans) [k][m].
-template <bool kTrans>
-__device__ __forceinline__ void load_a(uint32_t (&r)[4], const Tile &t, int m, int k, int p) {
-  const int lane = threadIdx.x & 31, i = lane >> 3, w = lane & 7;
-  if (kTrans) ldsm_t(r, t.piece(k + (i >> 1) * 8 + w, m / 8 + (i & 1), p));
-  else ldsm(r, t.piece(m + (i & 1) * 8 + w, k / 8 + (i >> 1), p));
+template <bool kTrans, int RB>
+__device__ __forceinline__ void load_a(uint32_t (&r)[4], const Tile<RB> &t, int m, int k, int p) {
+  if (kTrans) ldsm_t(r, t.template part<true>(k, m, p));
+  else ldsm(r, t.template part<false>(m, k, p));
 }
 // The 16x16 operand B (rows k, columns n), stored [n][k] or (trans) [k][n]:
 // r[0], r[1] are the first 8 columns', r[2], r[3] the others'.
-template <bool kTrans>
-__device__ __forceinline__ void load_b(uint32_t (&r)[4], const Tile &t, int k, int n, int p) {
-  const int lane = threadIdx.x & 31, i = lane >> 3, w = lane & 7;
-  if (kTrans) ldsm_t(r, t.piece(k + (i & 1) * 8 + w, n / 8 + (i >> 1), p));
-  else ldsm(r, t.piece(n + (i >> 1) * 8 + w, k / 8 + (i & 1), p));
+template <bool kTrans, int RB>
+__device__ __forceinline__ void load_b(uint32_t (&r)[4], const Tile<RB> &t, int k, int n, int p) {
+  if (kTrans) ldsm_t(r, t.template part<false>(k, n, p));
+  else ldsm(r, t.template part<true>(n, k, p));
 }
 // c0 and c1 += A times the two halves of B, for the planes' products that are
 // not below the last plane of the finer operand (all of them for two planes,
@@ -177,13 +185,13 @@ __device__ __forceinline__ void product(float (&c0)[4], float (&c1)[4], const ui
         mma(c1, a[i], b[j][2], b[j][3]);
       }
 }
-template <bool kTrans, int N>
-__device__ __forceinline__ void load_a(uint32_t (&r)[N][4], const Tile &t, int m, int k) {
+template <bool kTrans, int N, int RB>
+__device__ __forceinline__ void load_a(uint32_t (&r)[N][4], const Tile<RB> &t, int m, int k) {
 #pragma unroll
   for (int p = 0; p < N; ++p) load_a<kTrans>(r[p], t, m, k, p);
 }
-template <bool kTrans, int N>
-__device__ __forceinline__ void load_b(uint32_t (&r)[N][4], const Tile &t, int k, int n) {
+template <bool kTrans, int N, int RB>
+__device__ __forceinline__ void load_b(uint32_t (&r)[N][4], const Tile<RB> &t, int k, int n) {
 #pragma unroll
   for (int p = 0; p < N; ++p) load_b<kTrans>(r[p], t, k, n, p);
 }
@@ -200,8 +208,8 @@ __device__ __forceinline__ bool any_not_finite(const uint32_t (&a)[4]) {
   for (int i = 0; i < 4; ++i) x = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&a[i]), zero, x);
   return __any_sync(0xffffffffu, *reinterpret_cast<const uint32_t *>(&x) != 0u);
 }
-template <int N>
-__device__ __forceinline__ float number(const Tile &t, int row, int col) {
+template <int N, int RB>
+__device__ __forceinline__ float number(const Tile<RB> &t, int row, int col) {
   float x = 0.f;
 #pragma unroll
   for (int p = N - 1; p >= 0; --p) {
@@ -213,19 +221,23 @@ __device__ __forceinline__ float number(const Tile &t, int row, int col) {
 }
 // c0, c1 += x[rows m ..][tokens at ..] times the border's scores: of a token
 // and those up to it (kUpTo), or of a token and those from it on.
-template <int N, int M, bool kUpTo>
-__device__ __noinline__ void border(float (&c0)[4], float (&c1)[4], const Tile &x, int m, const Tile &scores, int at) {
+// (Inline and not unrolled: a call would keep c0 and c1 in memory.)
+template <int N, int M, bool kUpTo, int RB>
+__device__ __forceinline__ void border(float (&c0)[4], float (&c1)[4], const Tile<RB> &x, int m, const Tile<RB> &scores,
+                                       int at) {
   const int lane = threadIdx.x & 31, gr = lane >> 2, gc = lane & 3;
+#pragma unroll 1
   for (int e = 0; e < 8; ++e) {
     const int row = m + gr + (e >> 1 & 1) * 8, mine = (e >> 2) * 8 + 2 * gc + (e & 1);
     float s = 0.f;
+#pragma unroll 1
     for (int i = kUpTo ? 0 : mine; i < (kUpTo ? mine + 1 : 16); ++i)
       s += number<N>(x, row, at + i) *
            (kUpTo ? number<M>(scores, at + mine, at + i) : number<M>(scores, at + i, at + mine));
 #pragma unroll
     for (int f = 0; f < 4; ++f) {  // (no register is indexed by a variable)
-      if (e == f) c0[f] += s;
-      if (e == f + 4) c1[f] += s;
+      c0[f] += e == f ? s : 0.f;
+      c1[f] += e == f + 4 ? s : 0.f;
     }
   }
 }
@@ -236,7 +248,7 @@ __device__ __noinline__ void border(float (&c0)[4], float (&c1)[4], const Tile &
 // zeros elsewhere.  bfloat16 on a vector's boundary comes by asynchronous
 // copies.
 template <typename T, int C>
-__device__ __forceinline__ void fill(const Tile &t, const T *src, int rows, int rows16, int64_t length, int64_t t0, int n,
+__device__ __forceinline__ void fill(const Tile<2 * C> &t, const T *src, int rows, int rows16, int64_t length, int64_t t0, int n,
                                      bool vec) {
   constexpr int N = Planes<T>::in;
   for (int i = threadIdx.x; i < rows16 * (C / 8); i += blockDim.x) {
@@ -296,13 +308,13 @@ __device__ __forceinline__ float exp2_pair(float2 x) {
 // What a chunk's decays come to, in powers of two.
 template <int C>
 struct Decays {
-  float hi[C], lo[C];         // b_t as a pair
+  float2 at[C];               // b_t as a pair
   alignas(8) float begin[C];  // exp2(b_t)
   alignas(8) float end[C];    // exp2(b_C - b_t)
   float whole;         // exp2(b_C)
   float2 sum;          // b_C
   // log2 of exp(b_t - b_s)
-  __device__ __forceinline__ float between(int t, int s) const { return (hi[t] - hi[s]) + (lo[t] - lo[s]); }
+  static __device__ __forceinline__ float between(float2 t, float2 s) { return (t.x - s.x) + (t.y - s.y); }
 };
 // A warp's share of the decays of tokens t0 .. t0+n-1, loaded ahead.
 template <int C>
@@ -341,8 +353,7 @@ struct DecayLoad {
     for (int i = 0; i < C / 32; ++i) {
       const int t = lane * (C / 32) + i;
       const float2 at = two_sum(before, b[i]);
-      d.hi[t] = at.x;
-      d.lo[t] = at.y;
+      d.at[t] = at;
       d.begin[t] = exp2_pair(at);
       d.end[t] = exp2_pair(two_sum(whole, make_float2(-at.x, -at.y)));
     }
@@ -404,9 +415,10 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
   const int used = min(last, (len + C - 1) / C);  // chunks with tokens
 
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
-  const int row_bytes = 2 * C, kb = dk16 * row_bytes, vb = a.slab * row_bytes;
-  const Tile tk{base, row_bytes, kb}, tv{base + N * kb, row_bytes, vb}, tq{base + N * (kb + vb), row_bytes, kb},
-      scores{base + N * (2 * kb + vb), row_bytes, C * row_bytes};
+  constexpr int kRow = 2 * C;
+  const int kb = dk16 * kRow, vb = a.slab * kRow;
+  const Tile<kRow> tk(base, kb), tv(base + N * kb, vb), tq(base + N * (kb + vb), kb),
+      scores(base + N * (2 * kb + vb), C * kRow);
   auto bring = [&](int c) {
     const int64_t t0 = (int64_t)c * C;
     const int n = min(C, (int)(len - t0));
@@ -485,8 +497,8 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
 #pragma unroll
           for (int e = 0; e < 4; e += 2) {
             const int t = row * 16 + gr + (e >> 1) * 8, u = col * 16 + j * 8 + 2 * gc;
-            const float x0 = u <= t ? x[j][e] * a.scale * exp2_fast(d.between(t, u)) : 0.f;
-            const float x1 = u + 1 <= t ? x[j][e + 1] * a.scale * exp2_fast(d.between(t, u + 1)) : 0.f;
+            const float x0 = u <= t ? x[j][e] * a.scale * exp2_fast(d.between(d.at[t], d.at[u])) : 0.f;
+            const float x1 = u + 1 <= t ? x[j][e + 1] * a.scale * exp2_fast(d.between(d.at[t], d.at[u + 1])) : 0.f;
             uint32_t p[Pl::out];
             split<Pl::out>(x0, x1, p);
 #pragma unroll
@@ -701,12 +713,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
     return;
   }
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
-  const int row_bytes = 2 * C, kb = dk16 * row_bytes, vb = dv16 * row_bytes;
-  const Tile tq{base, row_bytes, kb}, tk{base + N * kb, row_bytes, kb}, tv{base + 2 * N * kb, row_bytes, vb},
-      to{base + 2 * N * kb + N * vb, row_bytes, vb};
+  constexpr int kRow = 2 * C;
+  const int kb = dk16 * kRow, vb = dv16 * kRow;
+  const Tile<kRow> tq(base, kb), tk(base + N * kb, kb), tv(base + 2 * N * kb, vb), to(base + 2 * N * kb + N * vb, vb);
   const uint32_t behind = base + 2 * N * (kb + vb);
-  const Tile tp{behind, row_bytes, C * row_bytes}, te{behind + Pl::out * C * row_bytes, row_bytes, C * row_bytes};
-  const Tile ts{behind + 2 * Pl::out * C * row_bytes, 2 * dv64, dk16 * 2 * dv64};  // S, then D, [dk][dv]
+  const Tile<kRow> tp(behind, C * kRow), te(behind + Pl::out * C * kRow, C * kRow);
+  const Tile<0> ts(behind + 2 * Pl::out * C * kRow, dk16 * 2 * dv64, 2 * dv64);  // S, then D, [dk][dv]
 
   const int64_t state_size = (int64_t)a.dk * a.dv;
   const float *S = a.states + (head * a.chunks + c) * state_size, *D = a.dstates + (head * a.chunks + c) * state_size;
@@ -799,7 +811,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
         float p[2], q[2];
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
-          const float z = u + f <= t ? a.scale * exp2_fast(d.between(t, u + f)) : 0.f;
+          const float z = u + f <= t ? a.scale * exp2_fast(d.between(d.at[t], d.at[u + f])) : 0.f;
           p[f] = u + f <= t ? x[j][e + f] * z : 0.f;
           q[f] = u + f <= t ? y[j][e + f] * z : 0.f;
           const float w = u + f < t ? p[f] * y[j][e + f] : 0.f;
@@ -841,7 +853,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
   };
   // acc += A[rows m ..][k] B[k][tokens], k over `depth`; A of X planes, transposed or not
-  auto times = [&](auto trans, int m, const Tile &B_, int depth, int part) {
+  auto times = [&](auto trans, int m, const Tile<kRow> &B_, int depth, int part) {
 #pragma unroll 2
     for (int kk = 0; kk < depth; kk += 16) {
       uint32_t A[X][4];
@@ -861,7 +873,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
       for (int e = 0; e < 4; ++e) acc[j][e] *= scale * factor[part * 32 + 8 * j + 2 * gc + (e & 1)];
   };
   // the sums of acc times x's rows, for each token
-  auto share_of = [&](const Tile &x, int m, int part, float *sums) {
+  auto share_of = [&](const Tile<kRow> &x, int m, int part, float *sums) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float s[2] = {};
@@ -888,7 +900,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
     }
   };
   // acc += x[rows m ..][tokens up to (or from) each one on] times the scores between them
-  auto within = [&](auto up_to, const Tile &x, int m, const Tile &scores, int part) {
+  auto within = [&](auto up_to, const Tile<kRow> &x, int m, const Tile<kRow> &scores, int part) {
     constexpr bool kUpTo = decltype(up_to)::value;
 #pragma unroll
     for (int s = 0; s < B16; ++s) {
