@@ -73,7 +73,7 @@ struct Args {
   float *states;        // [batch][heads][chunks][dk][dv]: S before each chunk
   float *dstates;       // likewise: D behind each chunk
   float *starts;        // [batch][heads][segments][dk][dv]: of segments, then their starts
-  float2 *decays;       // [batch][heads][segments]: log2 of a segment's decay, as a pair
+  float *decays;        // [batch][heads][segments]: a segment's decay
   void *dq, *dk_, *dv_;
   float *dq_heads, *dk_heads;  // [batch][heads][dk][length] where heads share queries and keys
   float *dg;            // [batch][heads][length]
@@ -386,15 +386,15 @@ enum Mode { kOutput, kForwardState, kBackwardState };
 // values; with `dstates` those behind each chunk, else what a segment adds.
 // The chain of dependent steps that a chunk takes is long, so what counts is
 // the warps that an SM has to change between: the outputs go by 32 tokens at a
-// time, tiles have no second buffer, and registers are held to four blocks an SM
-// (six for up to 64 keys).
+// time, their tiles have no second buffer, and registers are held to four blocks
+// an SM (five for up to 64 keys).
 template <typename T, int DK, Mode kMode>
 __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) linattn_kernel(const Args a) {
   using Pl = Planes<T>;
   constexpr int C = Pl::chunk, N = Pl::in;
   constexpr bool kOut = kMode == kOutput, kBack = kMode == kBackwardState;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ Decays<C> decays[2];
+  __shared__ Decays<C> decays[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, gc = lane & 3;
   int unit = blockIdx.x;
   const int slab = unit % a.slabs;
@@ -417,14 +417,21 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
   constexpr int kRow = 2 * C;
   const int kb = dk16 * kRow, vb = a.slab * kRow;
-  const Tile<kRow> tk(base, kb), tv(base + N * kb, vb), tq(base + N * (kb + vb), kb),
-      scores(base + N * (2 * kb + vb), C * kRow);
-  auto bring = [&](int c) {
+  // keys and values; behind them queries and scores, or (where the copies are asynchronous) the next chunk's
+  constexpr bool kAhead = !kOut && N == 1;
+  const int stage = N * (kb + vb);
+  const Tile<kRow> tq(base + stage, kb), scores(base + stage + N * kb, C * kRow);
+  auto tile_k = [&](int s) { return Tile<kRow>(base + s * stage, kb); };
+  auto tile_v = [&](int s) { return Tile<kRow>(base + s * stage + N * kb, vb); };
+  auto bring = [&](int c, int s) {
     const int64_t t0 = (int64_t)c * C;
     const int n = min(C, (int)(len - t0));
-    fill<T, C>(tk, k, a.dk, dk16, L, t0, n, a.vec);
-    fill<T, C>(tv, v, rows, rows16, L, t0, n, a.vec);
-    if (kOut) fill<T, C>(tq, q, a.dk, dk16, L, t0, n, a.vec);
+    fill<T, C>(tile_k(s), k, a.dk, dk16, L, t0, n, a.vec);
+    fill<T, C>(tile_v(s), v, rows, rows16, L, t0, n, a.vec);
+  };
+  auto bring_queries = [&](int c) {
+    const int64_t t0 = (int64_t)c * C;
+    fill<T, C>(tq, q, a.dk, dk16, L, t0, min(C, (int)(len - t0)), a.vec);
   };
 
   // S^T of this warp's 16 values: tile j holds keys 8j .. 8j+7
@@ -455,25 +462,34 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
   // chunks in the order of the pass
   const int count = max(0, used - first);
   auto chunk_at = [&](int i) { return kBack ? first + count - 1 - i : first + i; };
+  // The decays of as many chunks as there are warps are made at once, a warp each: one warp's chain of sums and
+  // exponentials for every chunk is what the others would wait for.
+  const int warps = blockDim.x >> 5;
   DecayLoad<C> ahead;
+  auto load_decays = [&](int i) {
+    if (i + warp < count) ahead.load(a, b, h, (int64_t)chunk_at(i + warp) * C, min(C, len - chunk_at(i + warp) * C));
+  };
   float2 total = make_float2(0.f, 0.f);
   if (count) {
-    const int c = chunk_at(0);
-    bring(c);
-    if (warp == 0) {
-      ahead.load(a, b, h, (int64_t)c * C, min(C, len - c * C));
-      ahead.finish(decays[0]);
-    }
+    bring(chunk_at(0), 0);
+    if (kOut) bring_queries(chunk_at(0));
+    load_decays(0);
   }
-  for (int i = 0; i < count; ++i) {
+  for (int i = 0, turn = 0; i < count; ++i, turn = turn + 1 == warps ? 0 : turn + 1) {
     const int c = chunk_at(i);
     const int64_t t0 = (int64_t)c * C;
     const int n = min(C, (int)(len - t0));
+    if (turn == 0) {
+      if (i) __syncthreads();
+      if (i + warp < count) ahead.finish(decays[warp]);
+      load_decays(i + warps);
+    }
     copies_done();
     __syncthreads();
-    const Decays<C> &d = decays[i & 1];
-    if (warp == 0 && i + 1 < count)
-      ahead.load(a, b, h, (int64_t)chunk_at(i + 1) * C, min(C, len - chunk_at(i + 1) * C));
+    const Decays<C> &d = decays[turn];
+    const int s = kAhead ? i & 1 : 0;
+    const Tile<kRow> tk = tile_k(s), tv = tile_v(s);
+    if (kAhead && i + 1 < count) bring(chunk_at(i + 1), s ^ 1);
     if (float *keep = kOut ? a.states : kBack ? a.dstates : nullptr)
       each_state([&](float &x, int key, int value) {
         keep[(head * a.chunks + c) * state_size + (int64_t)key * a.dv + value] = x;
@@ -573,6 +589,10 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
         }
       }
     }
+    if (kOut && i + 1 < count) {  // the queries are done with
+      __syncthreads();
+      bring_queries(chunk_at(i + 1));
+    }
     // the state behind the chunk
     const float whole = d.whole;
 #pragma unroll
@@ -609,13 +629,10 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
         }
       }
     }
-    if (warp == 0) {
-      total = two_sum(total, d.sum);
-      if (i + 1 < count) ahead.finish(decays[(i + 1) & 1]);
-    }
-    if (i + 1 < count) {
+    total = two_sum(total, d.sum);
+    if (!kAhead && i + 1 < count) {
       __syncthreads();
-      bring(chunk_at(i + 1));
+      bring(chunk_at(i + 1), 0);
     }
   }
   if (kOut) {  // zeros behind the last token
@@ -628,7 +645,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
     each_state([&](float &s, int key, int value) {
       a.starts[(head * a.segments + seg) * state_size + (int64_t)key * a.dv + value] = s;
     });
-    if (slab == 0 && threadIdx.x == 0) a.decays[head * a.segments + seg] = total;
+    if (slab == 0 && threadIdx.x == 0) a.decays[head * a.segments + seg] = exp2_pair(total);
   } else if (alone && a.final_state) {
     each_state([&](float &s, int key, int value) { a.final_state[head * state_size + (int64_t)key * a.dv + value] = s; });
   }
@@ -649,7 +666,7 @@ __global__ void __launch_bounds__(256) linattn_carry_kernel(const Args a, bool b
       if (j + k < a.segments) {
         const int64_t seg = head * a.segments + (back ? a.segments - 1 - j - k : j + k);
         added[k] = a.starts[seg * size + i];
-        decay[k] = exp2_pair(a.decays[seg]);
+        decay[k] = a.decays[seg];
       }
 #pragma unroll
     for (int k = 0; k < 8; ++k)
@@ -852,11 +869,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
   };
-  // acc += A[rows m ..][k] B[k][tokens], k over `depth`; A of X planes, transposed or not
-  auto times = [&](auto trans, int m, const Tile<kRow> &B_, int depth, int part) {
+  // acc += A[rows m ..][k] B[k][tokens], k over `depth`; A the state's first planes, transposed or not
+  auto times = [&](auto trans, auto planes, int m, const Tile<kRow> &B_, int depth, int part) {
 #pragma unroll 2
     for (int kk = 0; kk < depth; kk += 16) {
-      uint32_t A[X][4];
+      uint32_t A[decltype(planes)::value][4];
       load_a<decltype(trans)::value>(A, ts, m, kk);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -921,6 +938,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
       }
     }
   };
+  // (dv goes into no decay's gradient: one plane more than its scores have is enough)
+  const std::integral_constant<int, X> all_planes;
+  const std::integral_constant<int, (X < Pl::out + 1 ? X : Pl::out + 1)> some_planes;
   const std::true_type yes;
   const std::false_type no;
   // f(row, token, value, next token's value) for a piece's pairs of tokens
@@ -955,7 +975,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
   for (int it = warp; it < key_tiles * kParts; it += warps) {
     const int m = it / kParts * 16, part = it % kParts;
     zero();
-    times(no, m, to, dv16, part);
+    times(no, all_planes, m, to, dv16, part);
     factors(d.begin, a.scale, part);
     share_of(tq, m, part, old_part[m / 16]);
     if (it == warp) __syncthreads();  // the scores are there
@@ -971,14 +991,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
     zero();
     if (tile < key_tiles) {
       const int m = tile * 16;
-      times(no, m, tv, dv16, part);
+      times(no, all_planes, m, tv, dv16, part);
       factors(d.end, 1.f, part);
       share_of(tk, m, part, new_part[tile]);
       within(no, tq, m, te, part);
       each(m, a.dk, part, [&](int row, int t, float x, float y) { put_keys(a.dk_, a.dk_heads, row, t, x, y); });
     } else {
       const int m = (tile - key_tiles) * 16;
-      times(yes, m, tk, dk16, part);
+      times(yes, some_planes, m, tk, dk16, part);
       factors(d.end, 1.f, part);
       within(no, to, m, tp, part);
       each(m, a.dv, part, [&](int row, int t, float x, float y) { put((T *)a.dv_ + values_at + row * L + t0, t, x, y); });
@@ -1160,7 +1180,7 @@ Plan make_plan(int dtype, int batch, int heads, int length, int dv) {
 void sizes_of(Plan &p, int batch, int heads, int dk, int dv) {
   if (p.segments > 1) {
     p.starts = align_up((size_t)batch * heads * p.segments * dk * dv * 4, 256);
-    p.decays = align_up((size_t)batch * heads * p.segments * 8, 256);
+    p.decays = align_up((size_t)batch * heads * p.segments * 4, 256);
   }
 }
 
@@ -1168,7 +1188,8 @@ template <typename T>
 size_t forward_smem(const Args &a, bool out) {
   using Pl = Planes<T>;
   const int dk16 = (a.dk + 15) & ~15, bytes = 2 * Pl::chunk;
-  return (size_t)Pl::in * ((out ? 2 : 1) * dk16 + a.slab) * bytes + (out ? (size_t)Pl::out * Pl::chunk * bytes : 0);
+  const size_t stage = (size_t)Pl::in * (dk16 + a.slab) * bytes;
+  return out ? stage + (size_t)(Pl::in * dk16 + Pl::out * Pl::chunk) * bytes : Pl::in == 1 ? 2 * stage : stage;
 }
 template <typename T>
 size_t backward_smem(const Args &a) {
@@ -1356,7 +1377,7 @@ extern "C" int pc2d_linear_attention_forward(int dtype, const void *q, const voi
   a.final_state = final_state;
   a.states = states;
   a.starts = static_cast<float *>(workspace);
-  a.decays = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + p.starts);
+  a.decays = reinterpret_cast<float *>(static_cast<char *>(workspace) + p.starts);
   a.batch = batch;
   a.heads = heads;
   a.groups = groups;
@@ -1421,7 +1442,7 @@ extern "C" int pc2d_linear_attention_backward(int dtype, const void *grad, const
   };
   Args a{};
   a.starts = reinterpret_cast<float *>(take(p.starts));
-  a.decays = reinterpret_cast<float2 *>(take(p.decays));
+  a.decays = reinterpret_cast<float *>(take(p.decays));
   a.dstates =
       reinterpret_cast<float *>(take(pc2d_linear_attention_states_size(dtype, batch, heads, length, dk, dv)));
   float *per_token = reinterpret_cast<float *>(take((size_t)batch * heads * length * 4));
