@@ -97,7 +97,7 @@ __device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t at) {
                : "r"(at));
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -171,19 +171,32 @@ __device__ __forceinline__ void load_b(uint32_t (&r)[4], const Tile<RB> &t, int 
 }
 // c0 and c1 += A times the two halves of B, for the planes' products that are
 // not below the last plane of the finer operand (all of them for two planes,
-// whose last product would be the largest one left out).
-template <int NA, int NB>
-__device__ __forceinline__ void product(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4],
-                                        const uint32_t (&b)[NB][4]) {
+// whose last product would be the largest one left out).  The matrix unit cuts
+// its sums off instead of rounding them, by about half a unit each time and all
+// to one side, so that long chains of sums drift: with kApart all but the
+// largest of the products have sums of their own, l0 and l1, which are small.
+template <bool kApart, int NA, int NB>
+__device__ __forceinline__ void product(float (&c0)[4], float (&c1)[4], float (&l0)[4], float (&l1)[4],
+                                        const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][4]) {
   constexpr int most = NA == 2 && NB == 2 ? 3 : NA > NB ? NA : NB;
+  // (small ones first)
 #pragma unroll
-  for (int i = 0; i < NA; ++i)
+  for (int sum = most - 1; sum >= 0; --sum)
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
-      if (i + j < most) {
-        mma(c0, a[i], b[j][0], b[j][1]);
-        mma(c1, a[i], b[j][2], b[j][3]);
-      }
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        if (i + j == sum) {
+          mma(kApart && sum ? l0 : c0, a[i], b[j][0], b[j][1]);
+          mma(kApart && sum ? l1 : c1, a[i], b[j][2], b[j][3]);
+        }
+}
+template <int M>
+__device__ __forceinline__ void join(float (&c)[M][4], const float (&l)[M][4]) {
+#pragma unroll
+  for (int j = 0; j < M; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[j][e] += l[j][e];
 }
 template <bool kTrans, int N, int RB>
 __device__ __forceinline__ void load_a(uint32_t (&r)[N][4], const Tile<RB> &t, int m, int k) {
@@ -392,6 +405,7 @@ template <typename T, int DK, Mode kMode>
 __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) linattn_kernel(const Args a) {
   using Pl = Planes<T>;
   constexpr int C = Pl::chunk, N = Pl::in;
+  constexpr bool kApart = N > 1;
   constexpr bool kOut = kMode == kOutput, kBack = kMode == kBackwardState;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Decays<C> decays[4];
@@ -499,15 +513,16 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
       for (int blk = warp; blk < (C / 16) * (C / 16 + 1) / 2; blk += blockDim.x >> 5) {
         int row, col;
         block_of<C>(blk, row, col);
-        float x[2][4] = {};
+        float x[2][4] = {}, xl[2][4] = {};
 #pragma unroll
         for (int kk = 0; kk < DK; kk += 16) {
           if (kk >= dk16) break;
           uint32_t A[N][4], B[N][4];
           load_a<true>(A, tq, row * 16, kk);
           load_b<true>(B, tk, kk, col * 16);
-          product(x[0], x[1], A, B);
+          product<kApart>(x[0], x[1], xl[0], xl[1], A, B);
         }
+        if (kApart) join(x, xl);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -527,7 +542,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
 #pragma unroll
         for (int part = 0; part < C / 32; ++part) {
           // what the state before the chunk gives 32 tokens
-          float o[4][4] = {};
+          float o[4][4] = {}, ol[4][4] = {};
 #pragma unroll
           for (int kk = 0; kk < DK / 16; ++kk) {
             if (kk * 16 >= dk16) break;
@@ -543,9 +558,10 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
             for (int j = 0; j < 2; ++j) {
               uint32_t B[N][4];
               load_b<true>(B, tq, kk * 16, part * 32 + j * 16);
-              product(o[2 * j], o[2 * j + 1], A, B);
+              product<kApart>(o[2 * j], o[2 * j + 1], ol[2 * j], ol[2 * j + 1], A, B);
             }
           }
+          if (kApart) join(o, ol);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -565,7 +581,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
               }
               uint32_t B[Pl::out][4];
               load_b<false>(B, scores, ss * 16, at * 16);
-              product(o[2 * j], o[2 * j + 1], V, B);
+              product<false>(o[2 * j], o[2 * j + 1], o[2 * j], o[2 * j + 1], V, B);
             }
           }
 #pragma unroll
@@ -595,10 +611,6 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
     }
     // the state behind the chunk
     const float whole = d.whole;
-#pragma unroll
-    for (int j = 0; j < DK / 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) S[j][e] *= whole;
     if (warp * 16 < rows) {
 #pragma unroll
       for (int ss = 0; ss < C / 16; ++ss) {
@@ -625,7 +637,14 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
           if (j * 16 >= dk16) break;
           uint32_t B[N][4];
           load_b<false>(B, tk, ss * 16, j * 16);
-          product(S[2 * j], S[2 * j + 1], W, B);
+          // (added in 32 bits, which rounds: a state is a sum over thousands of tokens)
+          float u[2][4] = {};
+          product<false>(u[0], u[1], u[0], u[1], W, B);
+#pragma unroll
+          for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              S[2 * j + z][e] = ss == 0 ? fmaf(whole, S[2 * j + z][e], u[z][e]) : S[2 * j + z][e] + u[z][e];
         }
       }
     }
@@ -700,6 +719,7 @@ template <typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_kernel(const Args a) {
   using Pl = Planes<T>;
   constexpr int C = Pl::chunk, N = Pl::in, X = Pl::back, B16 = C / 16, kBlocks = B16 * (B16 + 1) / 2;
+  constexpr bool kApart = N > 1;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Decays<C> d;
   __shared__ float row_sums[kBlocks][16], col_sums[kBlocks][16], old_part[8][C], new_part[8][C], across_part[8];
@@ -804,20 +824,24 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
   for (int blk = warp; blk < kBlocks; blk += warps) {
     int row, col;
     block_of<C>(blk, row, col);
-    float x[2][4] = {}, y[2][4] = {};
+    float x[2][4] = {}, y[2][4] = {}, xl[2][4] = {}, yl[2][4] = {};
 #pragma unroll 4
     for (int kk = 0; kk < dk16; kk += 16) {
       uint32_t A[N][4], B[N][4];
       load_a<true>(A, tq, row * 16, kk);
       load_b<true>(B, tk, kk, col * 16);
-      product(x[0], x[1], A, B);
+      product<kApart>(x[0], x[1], xl[0], xl[1], A, B);
     }
 #pragma unroll 4
     for (int kk = 0; kk < dv16; kk += 16) {
       uint32_t A[N][4], B[N][4];
       load_a<true>(A, to, row * 16, kk);
       load_b<true>(B, tv, kk, col * 16);
-      product(y[0], y[1], A, B);
+      product<kApart>(y[0], y[1], yl[0], yl[1], A, B);
+    }
+    if (kApart) {
+      join(x, xl);
+      join(y, yl);
     }
     float rs[2] = {}, cs[2][2] = {};
 #pragma unroll
@@ -871,6 +895,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
   };
   // acc += A[rows m ..][k] B[k][tokens], k over `depth`; A the state's first planes, transposed or not
   auto times = [&](auto trans, auto planes, int m, const Tile<kRow> &B_, int depth, int part) {
+    float low[4][4] = {};
 #pragma unroll 2
     for (int kk = 0; kk < depth; kk += 16) {
       uint32_t A[decltype(planes)::value][4];
@@ -879,9 +904,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
       for (int j = 0; j < 2; ++j) {
         uint32_t B[N][4];
         load_b<true>(B, B_, kk, part * 32 + j * 16);
-        product(acc[2 * j], acc[2 * j + 1], A, B);
+        product<kApart>(acc[2 * j], acc[2 * j + 1], low[2 * j], low[2 * j + 1], A, B);
       }
     }
+    if (kApart) join(acc, low);
   };
   auto factors = [&](const float *factor, float scale, int part) {
 #pragma unroll
@@ -934,7 +960,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
         }
         uint32_t B[Pl::out][4];
         load_b<!kUpTo>(B, scores, s * 16, at * 16);
-        product(acc[2 * j], acc[2 * j + 1], A, B);
+        product<false>(acc[2 * j], acc[2 * j + 1], acc[2 * j], acc[2 * j + 1], A, B);
       }
     }
   };

@@ -630,10 +630,10 @@ struct Norm {
         each_two<2>(a, kept, slot, x + place(col), dy + place(col), stride, n, [&](const Two &v, int j) {
           float2 o[P];
 #pragma unroll
-          for (int i = 0; i < P; ++i) {
+          for (int i = 0; i < P; ++i) {  // (h w rounded as in its mean: a group of one value has no gradient)
             float2 xhat;
             const float2 h = slope(silu, v, i, xhat);
-            o[i] = mul2(rstd[i], fma2(xhat, hx[i], fma2(h, w[i], hw[i])));
+            o[i] = mul2(rstd[i], fma2(xhat, hx[i], add2(mul2(h, w[i]), hw[i])));
           }
           write(out + j * stride, o);
         });
@@ -895,7 +895,7 @@ struct Norm {
           for (int e = 0; e < P; ++e) {
             float2 xhat;
             const float2 h = slope(silu, v, e, xhat);
-            o[e] = held(mul2(rstd, fma2(xhat, hx, fma2(h, w, hw))), e, t1 - t0 - j * step);
+            o[e] = held(mul2(rstd, fma2(xhat, hx, add2(mul2(h, w), hw))), e, t1 - t0 - j * step);
           }
           write((T *)a.out + at + j * step, o);
         });
