@@ -264,6 +264,15 @@ template <typename T, int C>
 __device__ __forceinline__ void fill(const Tile<2 * C> &t, const T *src, int rows, int rows16, int64_t length, int64_t t0, int n,
                                      bool vec) {
   constexpr int N = Planes<T>::in;
+  if (N == 1 && vec && n == C) {  // whole chunks: few instructions a copy
+    const int c8 = threadIdx.x % (C / 8), step = blockDim.x / (C / 8);
+    const T *from = src + (threadIdx.x / (C / 8)) * length + t0 + c8 * 8;
+    int row = threadIdx.x / (C / 8);
+    for (; row < rows; row += step, from += step * length) copy16(t.piece(row, c8), from);
+    for (; row < rows16; row += step)
+      asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(t.piece(row, c8)), "r"(0) : "memory");
+    return;
+  }
   for (int i = threadIdx.x; i < rows16 * (C / 8); i += blockDim.x) {
     const int row = i / (C / 8), c8 = i % (C / 8), left = row < rows ? n - c8 * 8 : 0;
     const T *from = src + row * length + t0 + c8 * 8;
@@ -589,17 +598,19 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
             const int r = warp * 16 + gr + r8 * 8;
             if (r >= rows) continue;
             T *out = (T *)a.out + values + r * L + t0 + part * 32 + 2 * gc;
+            if (a.vec && n == C) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int left = n - (part * 32 + 8 * j + 2 * gc);
-              if (a.vec && left > 1) {
+              for (int j = 0; j < 4; ++j) {
                 Pack<T, 2> p;
                 p.set({o[j][2 * r8], o[j][2 * r8 + 1]});
                 p.store(out + 8 * j);
-              } else {
-                if (left > 0) out[8 * j] = from_f<T>(o[j][2 * r8]);
-                if (left > 1) out[8 * j + 1] = from_f<T>(o[j][2 * r8 + 1]);
               }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (part * 32 + 8 * j + 2 * gc + e < n) out[8 * j + e] = from_f<T>(o[j][2 * r8 + e]);
             }
           }
         }
@@ -643,8 +654,13 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
 #pragma unroll
           for (int z = 0; z < 2; ++z)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              S[2 * j + z][e] = ss == 0 ? fmaf(whole, S[2 * j + z][e], u[z][e]) : S[2 * j + z][e] + u[z][e];
+            for (int e = 0; e < 4; e += 2) {
+              float *x = &S[2 * j + z][e];
+              const float2 had = make_float2(x[0], x[1]), more = make_float2(u[z][e], u[z][e + 1]);
+              const float2 now = ss == 0 ? __ffma2_rn(make_float2(whole, whole), had, more) : __fadd2_rn(had, more);
+              x[0] = now.x;
+              x[1] = now.y;
+            }
         }
       }
     }
@@ -969,33 +985,35 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
   const std::integral_constant<int, (X < Pl::out + 1 ? X : Pl::out + 1)> some_planes;
   const std::true_type yes;
   const std::false_type no;
-  // f(row, token, value, next token's value) for a piece's pairs of tokens
-  auto each = [&](int m, int limit, int part, auto &&f) {
+  // Writes a piece to rows m .. of `out` (its row 0 at the chunk's first token).
+  auto put = [&](auto *out, int m, int limit, int part) {
+    using O = std::remove_pointer_t<decltype(out)>;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int row = m + gr + r * 8;
+      const int row = m + gr + r * 8, t = part * 32 + 2 * gc;
       if (row >= limit) continue;
+      O *at = out + row * L + t;
+      if (a.vec && n == C) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = part * 32 + 8 * j + 2 * gc;
-        f(row, t, t < n ? acc[j][2 * r] : 0.f, t + 1 < n ? acc[j][2 * r + 1] : 0.f);
+        for (int j = 0; j < 4; ++j) {
+          Pack<O, 2> p;
+          p.set({acc[j][2 * r], acc[j][2 * r + 1]});
+          p.store(at + 8 * j);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int u = t + 8 * j + e;
+            if (u < kept) at[8 * j + e] = from_f<O>(u < n ? acc[j][2 * r + e] : 0.f);
+          }
       }
     }
   };
-  auto put = [&](auto *out, int t, float x, float y) {
-    using O = std::remove_pointer_t<decltype(out)>;
-    if (a.vec && t + 1 < kept) {
-      Pack<O, 2> p;
-      p.set({x, y});
-      p.store(out + t);
-    } else {
-      if (t < kept) out[t] = from_f<O>(x);
-      if (t + 1 < kept) out[t + 1] = from_f<O>(y);
-    }
-  };
-  auto put_keys = [&](void *out, float *heads, int row, int t, float x, float y) {
-    if (heads) put(heads + (head * a.dk + row) * L + t0, t, x, y);
-    else put((T *)out + shared_at + row * L + t0, t, x, y);
+  auto put_keys = [&](void *out, float *heads, int m, int part) {
+    if (heads) put(heads + head * a.dk * L + t0, m, a.dk, part);
+    else put((T *)out + shared_at + t0, m, a.dk, part);
   };
   // (the first pieces' states are multiplied before the barrier, while other warps still make scores)
   for (int it = warp; it < key_tiles * kParts; it += warps) {
@@ -1006,7 +1024,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
     share_of(tq, m, part, old_part[m / 16]);
     if (it == warp) __syncthreads();  // the scores are there
     within(yes, tk, m, te, part);
-    each(m, a.dk, part, [&](int row, int t, float x, float y) { put_keys(a.dq, a.dq_heads, row, t, x, y); });
+    put_keys(a.dq, a.dq_heads, m, part);
   }
   if (warp >= key_tiles * kParts) __syncthreads();
   __syncthreads();  // S is done with
@@ -1021,13 +1039,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
       factors(d.end, 1.f, part);
       share_of(tk, m, part, new_part[tile]);
       within(no, tq, m, te, part);
-      each(m, a.dk, part, [&](int row, int t, float x, float y) { put_keys(a.dk_, a.dk_heads, row, t, x, y); });
+      put_keys(a.dk_, a.dk_heads, m, part);
     } else {
       const int m = (tile - key_tiles) * 16;
       times(yes, some_planes, m, tk, dk16, part);
       factors(d.end, 1.f, part);
       within(no, to, m, tp, part);
-      each(m, a.dv, part, [&](int row, int t, float x, float y) { put((T *)a.dv_ + values_at + row * L + t0, t, x, y); });
+      put((T *)a.dv_ + values_at + t0, m, a.dv, part);
     }
   }
   __syncthreads();
