@@ -143,6 +143,19 @@ void adamw_step_cuda(at::TensorList params, at::TensorList grads, at::TensorList
     for (const Tensor &t : list) changed(t);
 }
 
+// (The parameters need gradients; the step is not differentiated.)
+void adamw_step_autograd(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs,
+                         at::TensorList exp_avg_sqs, at::TensorList masters, at::TensorList scales, const Tensor &step,
+                         const OptTensor &lr_tensor, double lr, double beta1, double beta2, double eps,
+                         double weight_decay, const OptTensor &grad_scale, at::IntArrayRef splits,
+                         at::ArrayRef<double> factors, int64_t seed) {
+  check_cuda(step, "adamw_step");
+  at::AutoDispatchBelowADInplaceOrView below;
+  PC2D_BELOW(adamw_step)
+      .call(params, grads, exp_avgs, exp_avg_sqs, masters, scales, step, lr_tensor, lr, beta1, beta2, eps, weight_decay,
+            grad_scale, splits, factors, seed);
+}
+
 std::vector<Tensor> adamw_state_values_cuda(at::TensorList exp_avgs, at::TensorList exp_avg_sqs, at::TensorList scales,
                                             at::ScalarType dtype) {
   const size_t count = exp_avgs.size();
@@ -503,6 +516,7 @@ TORCH_LIBRARY_IMPL(paraconv2d_b200, CUDA, m) {
 }
 
 TORCH_LIBRARY_IMPL(paraconv2d_b200, Autograd, m) {
+  m.impl("adamw_step", adamw_step_autograd);
   m.impl("group_norm_forward", group_norm_forward_autograd);
   m.impl("linear_attention_forward", linear_attention_forward_autograd);
   m.impl("linear_attention_step", linear_attention_step_autograd);

@@ -113,7 +113,6 @@ class ParaboloidSGD(Optimizer):
 
 # ---------------------------------------------------------------------- AdamW
 
-@torch.no_grad()
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
                exp_avg_sqs: Sequence[Tensor], step: Tensor, *, lr: Union[float, Tensor],
                betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
@@ -148,7 +147,6 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
 
     No tensor that is written may share memory with another one of the call.
     """
-    params = list(params)
     if not params:
         return
     rate, rate_tensor = (0.0, lr) if isinstance(lr, Tensor) else (float(lr), None)
@@ -156,16 +154,15 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
         none = step.new_empty(0, dtype=torch.float32) if any(m is None for m in masters) else None
         masters = [none if m is None else m for m in masters]
     splits, rates = [], []
-    if factors is not None and any(f is not None for f in factors):
+    if factors is not None:
+        if len(factors) != len(params):
+            raise ValueError(f"factors must be as many as params ({len(params)}), got {len(factors)}")
         for p, f in zip(params, factors):
             split, first, rest, decay = (p.numel(), 1.0, 1.0, 1.0) if f is None else f
-            splits.append(int(split))
-            rates += [float(first), float(rest), float(decay)]
-        if len(splits) != len(params) or len(factors) != len(params):
-            raise ValueError(f"factors must be as many as params ({len(params)}), got {len(factors)}")
-    _adamw_step(params, list(grads), list(exp_avgs), list(exp_avg_sqs), masters or [], list(scales or []), step,
-                rate_tensor, rate, float(betas[0]), float(betas[1]), float(eps), float(weight_decay), grad_scale,
-                splits, rates, int(seed))
+            splits.append(split)
+            rates += (first, rest, decay)
+    _adamw_step(params, grads, exp_avgs, exp_avg_sqs, masters or [], scales or [], step, rate_tensor, rate, betas[0],
+                betas[1], eps, weight_decay, grad_scale, splits, rates, seed)
 
 
 def adamw_new_state(param: Tensor, bits: int = 32):
