@@ -5,7 +5,9 @@ Drop-in for GeoND-tech/ParaConv2d: ``torch.ops.ptparaconv2d.forward/backward``
 ``ptparaconv2d`` module mirror (``ParaConv2d``, ``ParaConv2dFunction``,
 ``spotlightinit``, ``pnnconvert``).  The kernels live in ``libpc2d_sm100.so``
 behind the C ABI of ``include/paraconv2d.h``.  ``layers`` has the layers
-beside ParaConv2d: dropout, a short causal convolution and a state space scan.
+beside ParaConv2d: dropout, group norm, a short causal convolution, a state
+space scan and linear attention.  ``optim`` has the optimizers that honour
+ParaConv2d's tags, SGD and AdamW.
 
 Importing this package loads the op library; a missing library raises.
 """

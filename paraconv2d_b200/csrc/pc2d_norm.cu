@@ -165,6 +165,10 @@ __device__ __forceinline__ void join(const float *v, int rows, int cols, At &&at
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+// A product that no sum takes in (the intrinsics' products may become part of a fused one).
+__device__ __forceinline__ float2 mul2_rounded(float2 a, float2 b) {
+  return make_float2(__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y));
+}
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 sigmoid2(float2 v) {  // as sigmoid_f
   float2 e = mul2(v, both(-1.4426950408889634f));
@@ -633,7 +637,7 @@ struct Norm {
           for (int i = 0; i < P; ++i) {  // (h w rounded as in its mean: a group of one value has no gradient)
             float2 xhat;
             const float2 h = slope(silu, v, i, xhat);
-            o[i] = mul2(rstd[i], fma2(xhat, hx[i], add2(mul2(h, w[i]), hw[i])));
+            o[i] = mul2(rstd[i], fma2(xhat, hx[i], add2(mul2_rounded(h, w[i]), hw[i])));
           }
           write(out + j * stride, o);
         });
@@ -664,8 +668,8 @@ struct Norm {
       for (int i = threadIdx.x & 31; i < a.cg; i += 32) {
         const int c = g * a.cg + i;
         const float w = load_w<T>(a.w, first + c, a.wf32, 1.f);
-        s += w * chan[2 * c];
-        q += w * chan[2 * c + 1];
+        s += __fmul_rn(w, chan[2 * c]);
+        q += __fmul_rn(w, chan[2 * c + 1]);
       }
       s = warp_sum(s);
       q = warp_sum(q);
@@ -895,7 +899,7 @@ struct Norm {
           for (int e = 0; e < P; ++e) {
             float2 xhat;
             const float2 h = slope(silu, v, e, xhat);
-            o[e] = held(mul2(rstd, fma2(xhat, hx, add2(mul2(h, w), hw))), e, t1 - t0 - j * step);
+            o[e] = held(mul2(rstd, fma2(xhat, hx, add2(mul2_rounded(h, w), hw))), e, t1 - t0 - j * step);
           }
           write((T *)a.out + at + j * step, o);
         });

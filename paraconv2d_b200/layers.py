@@ -1,5 +1,5 @@
-"""Layers beside ParaConv2d: dropout, a short causal convolution and a state
-space scan, each as a function and as a module.
+"""Layers beside ParaConv2d: dropout, a short causal convolution, a state
+space scan, linear attention and group norm, each as a function and as a module.
 
 They take [batch, channels, length] tensors: the map [N, C, H, W] of a
 convolution layer is one with ``x.flatten(2)``, and goes back with
@@ -14,15 +14,20 @@ convolution layer is one with ``x.flatten(2)``, and goes back with
 * :func:`ssm_scan` / :class:`SSMScan`: a diagonal linear recurrence whose decay
   and inputs depend on the token; :func:`ssm_scan_step` for one token of each
   request.
+* :func:`linear_attention` / :class:`LinearAttention`: a matrix state for each
+  head, with a decay; :func:`linear_attention_step` for one token of each
+  request.
+* :func:`group_norm` / :class:`GroupNorm`: over groups of channels, with an
+  optional SiLU, in both orders of dimensions.
 
 CUDA tensors only (float32, float16 and bfloat16; dropout float64 too), on the
 current stream of the tensors' device; sums and states in 32 bits.  Results
 and gradients are deterministic.  Dropout is differentiable any number of
-times, the convolution and the scan once; forward-mode derivatives are
-refused.  All of it, backward passes too, can be captured into CUDA graphs; as
-for every backward pass, leaves that still belong to an eager autograd graph
-made on another stream must be released (or their graph run on the capturing
-stream) before that.
+times, the others once; forward-mode derivatives are refused.  All of it,
+backward passes too, can be captured into CUDA graphs; as for every backward
+pass, leaves that still belong to an eager autograd graph made on another
+stream must be released (or their graph run on the capturing stream) before
+that.
 """
 from __future__ import annotations
 

@@ -194,8 +194,8 @@ class ParaboloidAdamW(Optimizer):
     ``p_lr_factor`` multiply the learning rate of the two halves of a layer's
     ``pars``, ``wd_factor`` its weight decay.
 
-    ``state_bits``: 32, or 8 for moments of two bytes and a 64th in all per
-    element.  ``masters``: keep float32 copies of 16-bit parameters.  ``seed``:
+    ``state_bits``: 32, or 8 for moments of two bytes and a 128th per element
+    instead of eight.  ``masters``: keep float32 copies of 16-bit parameters.  ``seed``:
     of the stochastic rounding of 8-bit moments; ranks that hold the same
     parameters need the same one.  ``lr`` may be a float32 tensor on the GPU.
     Steps are counted on the GPU, for all parameters that have had the same

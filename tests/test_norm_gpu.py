@@ -121,6 +121,20 @@ def test_large_means_and_outliers(last):
     close(pc.group_norm(xd, 2), v["out"], m["out"], "out")
 
 
+@pytest.mark.parametrize("last", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape,lengths", [((5, 32, 1), None), ((3, 6, 1), None), ((2, 7, 9), [1, 0]), ((2, 8, 8), [1, 1])])
+def test_groups_of_one_value_have_no_gradient(shape, lengths, dtype, last):
+    """Their result is the bias whatever they hold."""
+    g = gen(20)
+    x, w, b, d = (torch.randn(s, generator=g).to(dtype).to(DEV) for s in (shape, shape[1], shape[1], shape))
+    if last:
+        x, d = (t.movedim(1, -1).contiguous().movedim(-1, 1) for t in (x, d))
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    out, grads = run(x, shape[1], w, b, True, lengths=n, grad=d)
+    assert not grads[0].any() and not grads[1].any()
+
+
 def test_constant_input():
     x = torch.full((2, 8, 30), 7.25, device=DEV)
     b = torch.arange(8, device=DEV, dtype=F32)
