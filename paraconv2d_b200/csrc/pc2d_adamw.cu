@@ -212,6 +212,9 @@ __device__ __forceinline__ Rates rates_of(const Item &it, const Coef *coef, cons
 }
 
 // Moments in 32 bits: V elements a thread and vector, two vectors in flight.
+// Memory bounds it: 92 million bfloat16 parameters with masters, 28 bytes each,
+// take 395 us, 6.5 TB/s.  Small sets are bound by the two launches: 225,000
+// float32 parameters in four tensors 8.5 us on the GPU, 20 with the host's share.
 template <typename P, typename G, int N>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Items<N> a, const Coef *coef,
                                                          const float *grad_scale, const Betas b) {
@@ -262,7 +265,12 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
   }
 }
 
-// Moments in 8 bits: a warp takes a block of 256 at a time, eight a lane.
+// Moments in 8 bits: a warp takes a block of 256 at a time, eight a lane (the
+// generator's 16 bytes are for eight elements; the largest values meet in one
+// instruction a warp).  Instructions bound it, not memory: 46 million bfloat16
+// parameters, 10 bytes each, take 184 us, 2.5 TB/s.  Codes by comparisons and
+// shifts instead of products took 242, two blocks an SM instead of three
+// included.
 template <typename P, typename G, int N>
 __global__ void __launch_bounds__(kThreads, 3) adamw8_kernel(const __grid_constant__ Items<N> a, const Coef *coef,
                                                           const float *grad_scale, const Betas b) {
@@ -342,7 +350,8 @@ __global__ void __launch_bounds__(kThreads, 3) adamw8_kernel(const __grid_consta
   }
 }
 
-// 8-bit moments read out: m into `param`, v into `master` of an item.
+// 8-bit moments read out: m into `param`, v into `master` of an item.  Memory
+// bounds it: 46 million to bfloat16 in 42 us, 6.6 TB/s.
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) adamw_values_kernel(const __grid_constant__ Items<N> a) {
   constexpr int V = 8;

@@ -29,6 +29,18 @@
 // three), and the products of planes that matter: mma.sync with operands that
 // stay in registers from one product to the next.  (bfloat16 planes and not
 // float16 ones for float16 inputs too: states and scores outgrow its range.)
+// The state, which is scaled at every chunk and multiplied as an operand of the
+// next product, never leaves a warp's registers that way; in tensor memory
+// (tcgen05) it would be read, scaled, split and written again for each.
+//
+// Measured (one B200).  4 rows of 32 heads of 64 at 2048 tokens, bfloat16, a
+// training step: 438 us, of these outputs 89, states of the segments 37,
+// gradients' states 38 + 45, gradients 232.  16 heads of 128 at 16384 tokens:
+// 300 us, states of the segments 100 (tensor pipe half busy: it multiplies
+// three planes), outputs 205.  Everywhere the steps from one product to the
+// next (loads from shared memory, splits, exponentials) leave the tensor pipe
+// idle; what helped was more warps for an SM, fewer instructions between
+// products (no calls, fixed strides) and no 64-bit arithmetic.
 #include <math.h>
 
 #include <algorithm>
@@ -1128,7 +1140,8 @@ __global__ void __launch_bounds__(256) linattn_decay_kernel(const float *dg, int
 // -------------------------------------------------------------- single tokens
 
 // One token of a row and head: the state is read and written once, V values of
-// a key to a thread, the keys over the threads that are left.
+// a key to a thread, the keys over the threads that are left.  Memory bounds it:
+// 64 rows of 32 heads of 128x128 (268 MB) take 51 us, 5.2 TB/s.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) linattn_step_kernel(const T *q, const T *k, const T *v, const float *g,
                                                            int64_t g_batch, int64_t g_head, float *state,

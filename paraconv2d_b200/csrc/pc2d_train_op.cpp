@@ -191,17 +191,24 @@ std::vector<Tensor> adamw_state_values_cuda(at::TensorList exp_avgs, at::TensorL
 
 // ---------------------------------------------------------------- group norm
 
-// Channels last: the order in which the dimension 1 is the innermost one.
-Tensor last_view(const Tensor &t) { return t.movedim(1, -1); }
-
 struct NormCall {
   Call call;
   int dt, wdt, last, batch, channels, length, groups;
   Tensor input, weight, bias, lengths;
 };
 
-// A tensor in the order of dimensions of the call, its view in memory's order.
-Tensor in_order(const NormCall &c, const Tensor &t) { return c.last ? last_view(t).contiguous() : t.contiguous(); }
+// Channels last: the order in which dimension 1 is the innermost one.
+bool is_last(const Tensor &t) {
+  if (t.dim() < 3) return false;
+  int64_t stride = t.size(1);
+  if (t.size(1) > 1 && t.stride(1) != 1) return false;
+  for (int64_t d = t.dim() - 1; d != 1; d = d == 2 ? 0 : d - 1) {
+    if (t.size(d) > 1 && t.stride(d) != stride) return false;
+    stride *= t.size(d);
+    if (d == 0) break;
+  }
+  return true;
+}
 
 NormCall norm_call(const char *what, const Tensor &input, const OptTensor &weight, const OptTensor &bias,
                    const OptTensor &lengths, int64_t groups) {
@@ -214,14 +221,14 @@ NormCall norm_call(const char *what, const Tensor &input, const OptTensor &weigh
   for (int64_t d = 2; d < input.dim(); ++d) length *= input.size(d);
   c.length = as_int(length, what, "the number of positions");
   c.groups = as_int(groups, what, "groups");
-  c.last = input.dim() > 2 && !input.is_contiguous() && last_view(input).is_contiguous();
+  c.last = !input.is_contiguous() && is_last(input);
   const auto wtype = weight.has_value() && weight->defined() ? weight->scalar_type()
                      : bias.has_value() && bias->defined()   ? bias->scalar_type()
                                                              : input.scalar_type();
   TORCH_CHECK(wtype == input.scalar_type() || wtype == at::kFloat, what,
               ": weight and bias must be of the input's type or float32, got ", wtype);
   c.wdt = wtype == at::kFloat ? PC2D_DTYPE_F32 : c.dt;
-  c.input = in_order(c, input);
+  c.input = c.last ? input : input.contiguous();
   c.weight = c.call.maybe(weight, "weight", wtype, {c.channels});
   c.bias = c.call.maybe(bias, "bias", wtype, {c.channels});
   TORCH_CHECK(!(lengths.has_value() && lengths->defined()) || input.dim() == 3, what,
@@ -231,17 +238,14 @@ NormCall norm_call(const char *what, const Tensor &input, const OptTensor &weigh
 }
 
 // A result in the order of dimensions of the input.
-Tensor norm_result(const NormCall &c, const Tensor &input) {
-  const Tensor t = at::empty(c.input.sizes(), c.input.options());
-  return c.last ? t.movedim(-1, 1) : t.view(input.sizes());
-}
+Tensor norm_result(const NormCall &c) { return at::empty_strided(c.input.sizes(), c.input.strides(), c.input.options()); }
 
 std::vector<Tensor> group_norm_forward_cuda(const Tensor &input, const OptTensor &weight, const OptTensor &bias,
                                             const OptTensor &lengths, int64_t groups, double eps, bool silu,
                                             bool keep_stats) {
   const c10::cuda::CUDAGuard guard(input.device());
   const NormCall c = norm_call("paraconv2d_b200.group_norm_forward", input, weight, bias, lengths, groups);
-  Tensor out = norm_result(c, input);
+  Tensor out = norm_result(c);
   Tensor stats = at::empty(keep_stats ? at::IntArrayRef({c.batch, c.groups, 2}) : at::IntArrayRef({0}),
                            input.options().dtype(at::kFloat));
   const size_t bytes = pc2d_group_norm_workspace_size(c.dt, c.last, c.batch, c.channels, c.length, c.groups, 0);
@@ -261,9 +265,9 @@ std::vector<Tensor> group_norm_backward_cuda(const Tensor &grad_, const Tensor &
   TORCH_CHECK(grad_.device() == input.device() && grad_.scalar_type() == input.scalar_type() &&
                   grad_.sizes() == input.sizes(),
               c.call.what, ": grad must be like the input");
-  const Tensor grad = in_order(c, grad_);
+  const Tensor grad = same_layout(c.input, grad_) ? grad_ : norm_result(c).copy_(grad_);
   const Tensor stats = c.call.need(stats_, "stats", at::kFloat, {c.batch, c.groups, 2});
-  Tensor dx = norm_result(c, input);
+  Tensor dx = norm_result(c);
   auto like = [&](const Tensor &t) { return at::empty(t.defined() ? t.sizes() : at::IntArrayRef({0}),
                                                       t.defined() ? t.options() : input.options()); };
   Tensor dw = like(c.weight), db = like(c.bias);
