@@ -204,6 +204,10 @@ struct Norm {
 
   // vectors in flight
   static constexpr int kFlight = 2;
+  // pairs of vectors in the backward pass, where half of a large slab has no room in shared memory: four take the
+  // registers of two blocks an SM, which 16-bit types gain from (16x512x64x64 bfloat16, both passes: 148 to 139 us)
+  // and float32 loses by (64x128x56x56: 118 to 127 us)
+  static constexpr int kFlightTwo = sizeof(T) == 2 ? 4 : 2;
 
   // The weights of channels ch .. ch+V-1, or `none`.
   static __device__ __forceinline__ void weights(float2 (&v)[P], const void *p, int ch, bool f32, float none) {
@@ -588,7 +592,7 @@ struct Norm {
         if (slot == 0) arrived();
         float2 s[P] = {}, q[P] = {};
         by_silu(a, [&](auto silu) {
-          each_two<2>(a, kept, slot, x + place(col), dy + place(col), stride, n, [&](const Two &v, int) {
+          each_two<kFlightTwo>(a, kept, slot, x + place(col), dy + place(col), stride, n, [&](const Two &v, int) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
               float2 xhat;
@@ -639,7 +643,7 @@ struct Norm {
       });
       T *out = (T *)a.out + place(col);
       by_silu(a, [&](auto silu) {
-        each_two<2>(a, kept, slot, x + place(col), dy + place(col), stride, n, [&](const Two &v, int j) {
+        each_two<kFlightTwo>(a, kept, slot, x + place(col), dy + place(col), stride, n, [&](const Two &v, int j) {
           float2 o[P];
 #pragma unroll
           for (int i = 0; i < P; ++i) {  // (h w rounded as in its mean: a group of one value has no gradient)
@@ -859,7 +863,7 @@ struct Norm {
           channel(row);
           const int64_t at = f.base + (int64_t)row * a.P + t0;
           by_silu(a, [&](auto silu) {
-            each_two<2>(a, kept, slot, x + at, dy + at, step, n, [&](const Two &v, int j) {
+            each_two<kFlightTwo>(a, kept, slot, x + at, dy + at, step, n, [&](const Two &v, int j) {
               float2 h[P];
 #pragma unroll
               for (int e = 0; e < P; ++e) {
@@ -901,7 +905,7 @@ struct Norm {
       channel(row);
       const int64_t at = f.base + (int64_t)row * a.P + t0;
       auto last_pass = [&](auto silu, int slot, int64_t at, int t0, int n) {
-        each_two<2>(a, kept, slot, x + at, dy + at, step, n, [&](const Two &v, int j) {
+        each_two<kFlightTwo>(a, kept, slot, x + at, dy + at, step, n, [&](const Two &v, int j) {
           float2 o[P];
 #pragma unroll
           for (int e = 0; e < P; ++e) {
@@ -923,7 +927,7 @@ struct Norm {
 };
 
 template <typename T, int V, bool kLast, bool kBackward>
-__global__ void __launch_bounds__(kThreads, 3) norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kThreads, kBackward && sizeof(T) == 2 ? 2 : 3) norm_kernel(const NormArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   if constexpr (kLast && kBackward) Norm<T, V>::backward_last(a, smem);
   else if constexpr (kLast) Norm<T, V>::forward_last(a, smem);
