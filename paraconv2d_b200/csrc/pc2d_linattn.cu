@@ -410,7 +410,7 @@ __device__ __forceinline__ int tokens_of(const Args &a, int b) {
   return a.lengths ? min(max(a.lengths[b], 0), a.length) : a.length;
 }
 
-enum Mode { kOutput, kForwardState, kBackwardState };
+enum Mode { kOutput, kOutputOnly, kForwardState, kBackwardState };
 
 // One slab of up to 64 values of one head: 16 of them a warp, with their
 // transposed state in registers.  kOutput: the outputs of a segment of chunks
@@ -418,6 +418,7 @@ enum Mode { kOutput, kForwardState, kBackwardState };
 // the state that a segment adds.  kBackwardState: D, from the last chunk to
 // the first, from queries and the outputs' gradients in the places of keys and
 // values; with `dstates` those behind each chunk, else what a segment adds.
+// kOutputOnly: outputs whose states nobody sees.
 // The chain of dependent steps that a chunk takes is long, so what counts is
 // the warps that an SM has to change between: the outputs go by 32 tokens at a
 // time, their tiles have no second buffer, and registers are held to four blocks
@@ -427,7 +428,9 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
   using Pl = Planes<T>;
   constexpr int C = Pl::chunk, N = Pl::in;
   constexpr bool kApart = N > 1;
-  constexpr bool kOut = kMode == kOutput, kBack = kMode == kBackwardState;
+  constexpr bool kOut = kMode == kOutput || kMode == kOutputOnly, kBack = kMode == kBackwardState;
+  // (two planes, 2^-16, for states that go into nothing but the outputs)
+  constexpr int kUpdate = kMode == kOutputOnly && Pl::out == 1 ? 2 : Pl::update;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Decays<C> decays[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, gc = lane & 3;
@@ -637,7 +640,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
     if (warp * 16 < rows) {
 #pragma unroll
       for (int ss = 0; ss < C / 16; ++ss) {
-        uint32_t V[N][4], W[Pl::update][4];
+        uint32_t V[N][4], W[kUpdate][4];
         load_a<false>(V, tv, warp * 16, ss * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -650,10 +653,10 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
             y += r.y;
           }
           const float2 w = *reinterpret_cast<const float2 *>((kBack ? d.begin : d.end) + t);
-          uint32_t p[Pl::update];
-          split<Pl::update>(x * (kBack ? w.x * a.scale : w.x), y * (kBack ? w.y * a.scale : w.y), p);
+          uint32_t p[kUpdate];
+          split<kUpdate>(x * (kBack ? w.x * a.scale : w.x), y * (kBack ? w.y * a.scale : w.y), p);
 #pragma unroll
-          for (int z = 0; z < Pl::update; ++z) W[z][e] = p[z];
+          for (int z = 0; z < kUpdate; ++z) W[z][e] = p[z];
         }
 #pragma unroll
         for (int j = 0; j < DK / 16; ++j) {
@@ -1220,16 +1223,22 @@ int chunk_of(int dtype) {
 
 // Slabs of up to 64 values, of equal numbers of 16; and, where heads and slabs
 // leave the GPU without work, the sequence in segments (each at least 4 chunks).
-Plan make_plan(int dtype, int batch, int heads, int length, int dv) {
+Plan make_plan(int dtype, int batch, int heads, int length, int dk, int dv) {
   Plan p{};
   const int tiles = (dv + 15) / 16;
   p.slabs = (tiles + 3) / 4;
   p.slab = 16 * ((tiles + p.slabs - 1) / p.slabs);
   p.chunks = ceil_div(length, chunk_of(dtype));
-  const int64_t units = (int64_t)batch * heads * p.slabs, wanted = (int64_t)device_sm_count() * 4;
-  p.segments = 1;
-  if (units * 2 <= wanted && p.chunks >= 8)
-    p.segments = (int)std::min<int64_t>(wanted / units, p.chunks / 4);
+  const int64_t units = (int64_t)batch * heads * p.slabs;
+  auto segments = [&](int blocks) {  // for so many blocks an SM
+    const int64_t wanted = (int64_t)device_sm_count() * blocks;
+    return units * 2 <= wanted && p.chunks >= 8 ? (int)std::min<int64_t>(wanted / units, p.chunks / 4) : 1;
+  };
+  p.segments = segments(4);
+  // Five fit with up to 64 keys: taken where their segments are shorter by as much as they share the SM more (70 heads
+  // of 48x80 at 777 tokens: 5 segments of 5 chunks 70 us, 4 of up to 7 84; 128 heads of 64 at 2048 tokens, where they
+  // would be 5 of up to 7 chunks for 4 of 8: 449 us for 438).
+  if (dk <= 64 && ceil_div(p.chunks, segments(5)) * 5 <= ceil_div(p.chunks, p.segments) * 4) p.segments = segments(5);
   p.per_segment = ceil_div(p.chunks, p.segments);
   p.segments = std::max(1, ceil_div(p.chunks, std::max(1, p.per_segment)));
   return p;
@@ -1271,7 +1280,7 @@ int launch_pass(const Args &a, cudaStream_t stream) {
   const int st = allow_smem(kernel, allowed);
   if (st != PC2D_OK) return st;
   const int64_t grid = (int64_t)a.batch * a.heads * a.slabs * a.segments;
-  kernel<<<(unsigned)grid, a.slab * 2, forward_smem<T>(a, kMode == kOutput), stream>>>(a);
+  kernel<<<(unsigned)grid, a.slab * 2, forward_smem<T>(a, kMode == kOutput || kMode == kOutputOnly), stream>>>(a);
   PC2D_LAUNCH_CHECK("linattn_kernel");
   return PC2D_OK;
 }
@@ -1296,6 +1305,8 @@ int run_forward(const Args &a, cudaStream_t stream) {
   if (a.segments > 1 && ((st = launch_passes<T, kForwardState>(a, stream)) != PC2D_OK ||
                          (st = launch_carry(a, false, stream)) != PC2D_OK))
     return st;
+  // (of several segments the final state comes from the first pass)
+  if (Planes<T>::out == 1 && a.segments > 1 && !a.states) return launch_passes<T, kOutputOnly>(a, stream);
   return launch_passes<T, kOutput>(a, stream);
 }
 
@@ -1371,7 +1382,7 @@ extern "C" size_t pc2d_linear_attention_workspace_size(int dtype, int batch, int
                                                        int dv, int backward) {
   if (check_linattn("pc2d_linear_attention_workspace_size", dtype, batch, heads, groups, length, dk, dv) != PC2D_OK)
     return 0;
-  Plan p = make_plan(dtype, batch, heads, length, dv);
+  Plan p = make_plan(dtype, batch, heads, length, dk, dv);
   sizes_of(p, batch, heads, dk, dv);
   size_t bytes = p.starts + p.decays;
   if (backward) {
@@ -1417,7 +1428,7 @@ extern "C" int pc2d_linear_attention_forward(int dtype, const void *q, const voi
   }
   if ((st = check_elements(what, size, {q, k, v, output})) != PC2D_OK || (st = check_states(what, states)) != PC2D_OK)
     return st;
-  Plan p = make_plan(dtype, batch, heads, length, dv);
+  Plan p = make_plan(dtype, batch, heads, length, dk, dv);
   sizes_of(p, batch, heads, dk, dv);
   if ((st = need_workspace(what, workspace, workspace_bytes, p.starts + p.decays)) != PC2D_OK) return st;
   Args a{};
@@ -1489,7 +1500,7 @@ extern "C" int pc2d_linear_attention_backward(int dtype, const void *grad, const
   if ((st = need_workspace(what, workspace, workspace_bytes,
                            pc2d_linear_attention_workspace_size(dtype, batch, heads, groups, length, dk, dv, 1))) != PC2D_OK)
     return st;
-  Plan p = make_plan(dtype, batch, heads, length, dv);
+  Plan p = make_plan(dtype, batch, heads, length, dk, dv);
   sizes_of(p, batch, heads, dk, dv);
   char *at = static_cast<char *>(workspace);
   auto take = [&](size_t bytes) {
