@@ -36,8 +36,8 @@
 // Measured (one B200).  4 rows of 32 heads of 64 at 2048 tokens, bfloat16, a
 // training step: 438 us, of these outputs 89, states of the segments 37,
 // gradients' states 38 + 45, gradients 232.  16 heads of 128 at 16384 tokens:
-// 300 us, states of the segments 100 (tensor pipe half busy: it multiplies
-// three planes), outputs 205.  Everywhere the steps from one product to the
+// 283 us, states of the segments 100 (tensor pipe half busy: it multiplies
+// three planes), outputs 187.  Everywhere the steps from one product to the
 // next (loads from shared memory, splits, exponentials) leave the tensor pipe
 // idle; what helped was more warps for an SM, fewer instructions between
 // products (no calls, fixed strides) and no 64-bit arithmetic.
