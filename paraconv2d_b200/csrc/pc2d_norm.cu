@@ -57,6 +57,7 @@ struct NormArgs {
   void *out;            // y, or dx
   float *stats;         // [batch][groups][2]: mean and rstd
   float *part;          // kSums, kApply: [slab][split][numbers of a block]
+  int numbers;          // of a block of a whole slab: what the blocks' parts lie apart (the last slab may have fewer)
   float *chan;          // backward: [batch][channels][2], sums of h and of h xhat
   int batch, C, P, G, cg;
   int slab_channels;    // channels of a slab: cg, or a multiple of it
@@ -113,14 +114,14 @@ __device__ __forceinline__ Place place_of(const NormArgs &a) {
 template <typename Take>
 __device__ __forceinline__ bool exchange(const NormArgs &a, const float *mine, int count, Take &&take) {
   const int rank = blockIdx.x & (a.split - 1);
-  float *global = a.part + (size_t)(blockIdx.x - rank) * count;
+  float *global = a.part + (size_t)(blockIdx.x - rank) * a.numbers;
   __syncthreads();
   if (a.phase == kSums) {
-    for (int i = threadIdx.x; i < count; i += kThreads) global[(size_t)rank * count + i] = mine[i];
+    for (int i = threadIdx.x; i < count; i += kThreads) global[(size_t)rank * a.numbers + i] = mine[i];
     return false;
   }
   if (a.phase == kApply) {
-    take([&](int r, int i) { return global[(size_t)r * count + i]; });
+    take([&](int r, int i) { return global[(size_t)r * a.numbers + i]; });
   } else if (a.split == 1) {
     take([&](int, int i) { return mine[i]; });
   } else {
@@ -1164,6 +1165,7 @@ extern "C" int pc2d_group_norm_forward(int dtype, int wdtype, int channels_last,
   a.cache = p.cache;
   a.red = p.red;
   a.segs = p.segs;
+  a.numbers = (int)p.numbers;
   a.wf32 = wdtype == PC2D_DTYPE_F32;
   a.silu = silu;
   a.eps = (float)eps;
@@ -1232,6 +1234,7 @@ extern "C" int pc2d_group_norm_backward(int dtype, int wdtype, int channels_last
   a.cache = p.cache;
   a.red = p.red;
   a.segs = p.segs;
+  a.numbers = (int)p.numbers;
   a.wf32 = wdtype == PC2D_DTYPE_F32;
   a.silu = silu;
   if (!weightgrad && !biasgrad) a.chan = nullptr;
