@@ -410,7 +410,7 @@ __device__ __forceinline__ int tokens_of(const Args &a, int b) {
   return a.lengths ? min(max(a.lengths[b], 0), a.length) : a.length;
 }
 
-enum Mode { kOutput, kOutputOnly, kForwardState, kBackwardState };
+enum Mode { kOutput, kForwardState, kBackwardState };
 
 // One slab of up to 64 values of one head: 16 of them a warp, with their
 // transposed state in registers.  kOutput: the outputs of a segment of chunks
@@ -418,7 +418,6 @@ enum Mode { kOutput, kOutputOnly, kForwardState, kBackwardState };
 // the state that a segment adds.  kBackwardState: D, from the last chunk to
 // the first, from queries and the outputs' gradients in the places of keys and
 // values; with `dstates` those behind each chunk, else what a segment adds.
-// kOutputOnly: outputs whose states nobody sees.
 // The chain of dependent steps that a chunk takes is long, so what counts is
 // the warps that an SM has to change between: the outputs go by 32 tokens at a
 // time, their tiles have no second buffer, and registers are held to four blocks
@@ -428,9 +427,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
   using Pl = Planes<T>;
   constexpr int C = Pl::chunk, N = Pl::in;
   constexpr bool kApart = N > 1;
-  constexpr bool kOut = kMode == kOutput || kMode == kOutputOnly, kBack = kMode == kBackwardState;
-  // (two planes, 2^-16, for states that go into nothing but the outputs)
-  constexpr int kUpdate = kMode == kOutputOnly && Pl::out == 1 ? 2 : Pl::update;
+  constexpr bool kOut = kMode == kOutput, kBack = kMode == kBackwardState;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Decays<C> decays[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, gc = lane & 3;
@@ -640,7 +637,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
     if (warp * 16 < rows) {
 #pragma unroll
       for (int ss = 0; ss < C / 16; ++ss) {
-        uint32_t V[N][4], W[kUpdate][4];
+        uint32_t V[N][4], W[Pl::update][4];
         load_a<false>(V, tv, warp * 16, ss * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -653,10 +650,10 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
             y += r.y;
           }
           const float2 w = *reinterpret_cast<const float2 *>((kBack ? d.begin : d.end) + t);
-          uint32_t p[kUpdate];
-          split<kUpdate>(x * (kBack ? w.x * a.scale : w.x), y * (kBack ? w.y * a.scale : w.y), p);
+          uint32_t p[Pl::update];
+          split<Pl::update>(x * (kBack ? w.x * a.scale : w.x), y * (kBack ? w.y * a.scale : w.y), p);
 #pragma unroll
-          for (int z = 0; z < kUpdate; ++z) W[z][e] = p[z];
+          for (int z = 0; z < Pl::update; ++z) W[z][e] = p[z];
         }
 #pragma unroll
         for (int j = 0; j < DK / 16; ++j) {
@@ -1280,7 +1277,7 @@ int launch_pass(const Args &a, cudaStream_t stream) {
   const int st = allow_smem(kernel, allowed);
   if (st != PC2D_OK) return st;
   const int64_t grid = (int64_t)a.batch * a.heads * a.slabs * a.segments;
-  kernel<<<(unsigned)grid, a.slab * 2, forward_smem<T>(a, kMode == kOutput || kMode == kOutputOnly), stream>>>(a);
+  kernel<<<(unsigned)grid, a.slab * 2, forward_smem<T>(a, kMode == kOutput), stream>>>(a);
   PC2D_LAUNCH_CHECK("linattn_kernel");
   return PC2D_OK;
 }
@@ -1306,7 +1303,6 @@ int run_forward(const Args &a, cudaStream_t stream) {
                          (st = launch_carry(a, false, stream)) != PC2D_OK))
     return st;
   // (of several segments the final state comes from the first pass)
-  if (Planes<T>::out == 1 && a.segments > 1 && !a.states) return launch_passes<T, kOutputOnly>(a, stream);
   return launch_passes<T, kOutput>(a, stream);
 }
 
