@@ -58,12 +58,15 @@ constexpr float kNothing = 1e5f;  // in powers of two: exp2(-1e5) is 0 in 32 bit
 // that meet inputs in the outputs; the decayed values in the state's update,
 // whose result is a state of 32 bits; states in the backward pass, whose
 // products make the decays' gradients of 32 bits.  With bfloat16 a score or
-// state is rounded to a plane as the outputs are rounded in the end.
+// state is off by 2^-15 of itself at most, so that outputs are rounded once, to
+// their type, as far as that shows (errors in norm 1.67e-3, which the rounding
+// alone has too; with one plane, 2^-8, 2.35e-3, and a training step of 4 rows of
+// 32 heads of 64 at 2048 tokens 448 us instead of 468).
 template <typename T>
 struct Planes;
 template <>
 struct Planes<__nv_bfloat16> {
-  static constexpr int in = 1, out = 1, update = 3, back = 3, chunk = 64;
+  static constexpr int in = 1, out = 2, update = 3, back = 3, chunk = 64;
 };
 template <>
 struct Planes<__half> {
@@ -221,6 +224,37 @@ __device__ __forceinline__ void load_b(uint32_t (&r)[N][4], const Tile<RB> &t, i
   for (int p = 0; p < N; ++p) load_b<kTrans>(r[p], t, k, n, p);
 }
 
+// A chunk's scores: the 16x16 blocks on and below the diagonal, in P planes.  Of 64 tokens, rows of 1 to 4 blocks,
+// two planes lie in 80 rows of 128 bytes instead of 128 (with these a fourth block of an SM would not fit for 128 keys:
+// 16384 tokens of 16 heads of 128 432 us instead of 337): a plane's rows of one and of three blocks side by side, its
+// four-block rows below them, and at last the two-block rows of both planes side by side.
+template <int C, int P>
+struct Scores {
+  static constexpr bool kPacked = C == 64 && P == 2;
+  static constexpr int kBytes = kPacked ? 80 * 128 : P * C * 2 * C;
+  Tile<2 * C> t;
+  __device__ __forceinline__ explicit Scores(uint32_t at) : t(at, C * 2 * C) {}
+  // where the block (row, col) of plane p is: a block of `t`, in its plane 0 if packed
+  static __device__ __forceinline__ void place(int row, int col, int p, int &r, int &c) {
+    r = !kPacked ? row : row == 1 ? 4 : 2 * p + (row == 3);
+    c = !kPacked ? col : row == 1 ? 2 * p + col : col + (row == 2);
+  }
+  __device__ __forceinline__ uint32_t piece(int row, int col8, int p) const {
+    int r, c;
+    place(row >> 4, col8 >> 1, p, r, c);
+    return t.piece(r * 16 + (row & 15), c * 2 + (col8 & 1), kPacked ? 0 : p);
+  }
+  // the operand B of tokens s as its rows k and tokens `at` as its columns n, both as blocks
+  __device__ __forceinline__ void load(uint32_t (&b)[P][4], int s, int at) const {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      int r, c;
+      place(at, s, p, r, c);
+      load_b<false>(b[p], t, c * 16, r * 16, kPacked ? 0 : p);
+    }
+  }
+};
+
 // Scores beyond the causal border are zeros that a product multiplies, which an
 // infinity or NaN on the other side would turn into NaN for tokens that it does
 // not reach.  Only the 16x16 blocks on the border hold such zeros: where A has
@@ -233,8 +267,8 @@ __device__ __forceinline__ bool any_not_finite(const uint32_t (&a)[4]) {
   for (int i = 0; i < 4; ++i) x = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&a[i]), zero, x);
   return __any_sync(0xffffffffu, *reinterpret_cast<const uint32_t *>(&x) != 0u);
 }
-template <int N, int RB>
-__device__ __forceinline__ float number(const Tile<RB> &t, int row, int col) {
+template <int N, typename Matrix>
+__device__ __forceinline__ float number(const Matrix &t, int row, int col) {
   float x = 0.f;
 #pragma unroll
   for (int p = N - 1; p >= 0; --p) {
@@ -247,8 +281,8 @@ __device__ __forceinline__ float number(const Tile<RB> &t, int row, int col) {
 // c0, c1 += x[rows m ..][tokens at ..] times the border's scores: of a token
 // and those up to it (kUpTo), or of a token and those from it on.
 // (Inline and not unrolled: a call would keep c0 and c1 in memory.)
-template <int N, int M, bool kUpTo, int RB>
-__device__ __forceinline__ void border(float (&c0)[4], float (&c1)[4], const Tile<RB> &x, int m, const Tile<RB> &scores,
+template <int N, int M, bool kUpTo, int RB, typename Matrix>
+__device__ __forceinline__ void border(float (&c0)[4], float (&c1)[4], const Tile<RB> &x, int m, const Matrix &scores,
                                        int at) {
   const int lane = threadIdx.x & 31, gr = lane >> 2, gc = lane & 3;
 #pragma unroll 1
@@ -455,7 +489,8 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
   // keys and values; behind them queries and scores, or (where the copies are asynchronous) the next chunk's
   constexpr bool kAhead = !kOut && N == 1;
   const int stage = N * (kb + vb);
-  const Tile<kRow> tq(base + stage, kb), scores(base + stage + N * kb, C * kRow);
+  const Tile<kRow> tq(base + stage, kb);
+  const Scores<C, Pl::out> scores(base + stage + N * kb);
   auto tile_k = [&](int s) { return Tile<kRow>(base + s * stage, kb); };
   auto tile_v = [&](int s) { return Tile<kRow>(base + s * stage + N * kb, vb); };
   auto bring = [&](int c, int s) {
@@ -554,8 +589,14 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
             uint32_t p[Pl::out];
             split<Pl::out>(x0, x1, p);
 #pragma unroll
-            for (int z = 0; z < Pl::out; ++z)
-              asm volatile("st.shared.b32 [%0], %1;" ::"r"(scores.piece(t, u / 8, z) + (u & 7) * 2), "r"(p[z]) : "memory");
+            for (int z = 0; z < Pl::out; ++z) {
+              int br, bc;
+              scores.place(row, col, z, br, bc);
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(scores.t.piece(br * 16 + gr + (e >> 1) * 8, bc * 2 + j,
+                                                                          scores.kPacked ? 0 : z) + gc * 4),
+                           "r"(p[z])
+                           : "memory");
+            }
           }
       }
       __syncthreads();
@@ -601,7 +642,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (DK == 64 ? 5 : 4) : 2) 
                 continue;
               }
               uint32_t B[Pl::out][4];
-              load_b<false>(B, scores, ss * 16, at * 16);
+              scores.load(B, ss, at);
               product<false>(o[2 * j], o[2 * j + 1], o[2 * j], o[2 * j + 1], V, B);
             }
           }
@@ -921,12 +962,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
   };
-  // acc += A[rows m ..][k] B[k][tokens], k over `depth`; A the state's first planes, transposed or not
-  auto times = [&](auto trans, auto planes, int m, const Tile<kRow> &B_, int depth, int part) {
+  // acc += A[rows m ..][k] B[k][tokens], k over `depth`; A the state, transposed or not
+  auto times = [&](auto trans, int m, const Tile<kRow> &B_, int depth, int part) {
     float low[4][4] = {};
 #pragma unroll 2
     for (int kk = 0; kk < depth; kk += 16) {
-      uint32_t A[decltype(planes)::value][4];
+      uint32_t A[X][4];
       load_a<decltype(trans)::value>(A, ts, m, kk);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -992,9 +1033,6 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
       }
     }
   };
-  // (dv goes into no decay's gradient: one plane more than its scores have is enough)
-  const std::integral_constant<int, X> all_planes;
-  const std::integral_constant<int, (X < Pl::out + 1 ? X : Pl::out + 1)> some_planes;
   const std::true_type yes;
   const std::false_type no;
   // Writes a piece to rows m .. of `out` (its row 0 at the chunk's first token).
@@ -1031,7 +1069,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
   for (int it = warp; it < key_tiles * kParts; it += warps) {
     const int m = it / kParts * 16, part = it % kParts;
     zero();
-    times(no, all_planes, m, to, dv16, part);
+    times(no, m, to, dv16, part);
     factors(d.begin, a.scale, part);
     share_of(tq, m, part, old_part[m / 16]);
     if (it == warp) __syncthreads();  // the scores are there
@@ -1047,14 +1085,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
     zero();
     if (tile < key_tiles) {
       const int m = tile * 16;
-      times(no, all_planes, m, tv, dv16, part);
+      times(no, m, tv, dv16, part);
       factors(d.end, 1.f, part);
       share_of(tk, m, part, new_part[tile]);
       within(no, tq, m, te, part);
       put_keys(a.dk_, a.dk_heads, m, part);
     } else {
       const int m = (tile - key_tiles) * 16;
-      times(yes, some_planes, m, tk, dk16, part);
+      times(yes, m, tk, dk16, part);
       factors(d.end, 1.f, part);
       within(no, to, m, tp, part);
       put((T *)a.dv_ + values_at + t0, m, a.dv, part);
@@ -1252,7 +1290,7 @@ size_t forward_smem(const Args &a, bool out) {
   using Pl = Planes<T>;
   const int dk16 = (a.dk + 15) & ~15, bytes = 2 * Pl::chunk;
   const size_t stage = (size_t)Pl::in * (dk16 + a.slab) * bytes;
-  return out ? stage + (size_t)(Pl::in * dk16 + Pl::out * Pl::chunk) * bytes : Pl::in == 1 ? 2 * stage : stage;
+  return out ? stage + (size_t)Pl::in * dk16 * bytes + Scores<Pl::chunk, Pl::out>::kBytes : Pl::in == 1 ? 2 * stage : stage;
 }
 template <typename T>
 size_t backward_smem(const Args &a) {
