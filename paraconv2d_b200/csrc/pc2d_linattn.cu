@@ -780,9 +780,13 @@ __device__ __forceinline__ float column_sum(float v) {  // over the eight rows o
 //   dq_t = sum_s E_ts k_s + scale exp(b_t) S do_t
 //   dk_s = sum_t E_ts q_t + exp(b_C - b_s) D v_s
 //   dv_s = sum_t P_ts do_t + exp(b_C - b_s) D^T k_s
-// and the decays' from the pairs W_ts = P_ts (do_t v_s), s < t, the parts that
-// S and D have in q dq and k dk, and exp(b_C) <S, D>; none of these cancel
-// but the W of pairs on one side of a token, which are the same numbers.
+// and the decays', dg_t, from the pairs W_us = P_us (do_u v_s), s < t <= u, the
+// parts that S has in q dq from t on and D in k dk before t, and exp(b_C) <S, D>.
+// The pairs of a 16x16 block on the diagonal are summed for each t: along its
+// rows before t, then down its columns from t on.  Of the other blocks t has
+// whole ones, rows from t on and columns before t.  So each sum has only what
+// belongs to it: nothing is added and taken away again, and what is not finite
+// stays on its side.
 // A warp takes 16 of the dk or dv rows of a gradient and 32 tokens at a time.
 template <typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_kernel(const Args a) {
@@ -791,7 +795,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
   constexpr bool kApart = N > 1;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Decays<C> d;
-  __shared__ float row_sums[kBlocks][16], col_sums[kBlocks][16], old_part[8][C], new_part[8][C], across_part[8];
+  __shared__ float row_sums[kBlocks][16], col_sums[kBlocks][16], all_sums[kBlocks], old_part[8][C], new_part[8][C], across_part[8];
   constexpr int warps = 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, gc = lane & 3;
   int64_t unit = blockIdx.x;
@@ -912,7 +916,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
       join(x, xl);
       join(y, yl);
     }
-    float rs[2] = {}, cs[2][2] = {};
+    float w[2][4];
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -924,9 +928,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
           const float z = u + f <= t ? a.scale * exp2_fast(d.between(d.at[t], d.at[u + f])) : 0.f;
           p[f] = u + f <= t ? x[j][e + f] * z : 0.f;
           q[f] = u + f <= t ? y[j][e + f] * z : 0.f;
-          const float w = u + f < t ? p[f] * y[j][e + f] : 0.f;
-          rs[e >> 1] += w;
-          cs[j][f] += w;
+          w[j][e + f] = u + f < t ? p[f] * y[j][e + f] : 0.f;
         }
         uint32_t pp[Pl::out], pq[Pl::out];
         split<Pl::out>(p[0], p[1], pp);
@@ -937,11 +939,44 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
           asm volatile("st.shared.b32 [%0], %1;" ::"r"(te.piece(t, u / 8, z) + (u & 7) * 2), "r"(pq[z]) : "memory");
         }
       }
+    float cs[2][2];
+    if (row == col) {
+      // of each row u, the pairs before t = its columns 2 gc, 2 gc + 1 and 8 more, where t <= u
+      cs[0][0] = cs[0][1] = cs[1][0] = cs[1][1] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      rs[e] += __shfl_xor_sync(0xffffffffu, rs[e], 1);
-      rs[e] += __shfl_xor_sync(0xffffffffu, rs[e], 2);
-      if (gc == 0) row_sums[blk][gr + e * 8] = rs[e];
+      for (int e = 0; e < 2; ++e) {
+        float upto[2], left = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          upto[j] = w[j][2 * e] + w[j][2 * e + 1];
+#pragma unroll
+          for (int o = 1; o < 4; o <<= 1) {
+            const float v = __shfl_up_sync(0xffffffffu, upto[j], o, 4);
+            if (gc >= o) upto[j] += v;
+          }
+          float before = __shfl_up_sync(0xffffffffu, upto[j], 1, 4);
+          before = gc == 0 ? left : left + before;
+          left = __shfl_sync(0xffffffffu, upto[j], 3, 4);
+          const int u = gr + e * 8, t = j * 8 + 2 * gc;
+          cs[j][0] += t <= u ? before : 0.f;
+          cs[j][1] += t + 1 <= u ? before + w[j][2 * e] : 0.f;
+        }
+      }
+    } else {
+      float rs[2], all;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        rs[e] = (w[0][2 * e] + w[0][2 * e + 1]) + (w[1][2 * e] + w[1][2 * e + 1]);
+        rs[e] += __shfl_xor_sync(0xffffffffu, rs[e], 1);
+        rs[e] += __shfl_xor_sync(0xffffffffu, rs[e], 2);
+        if (gc == 0) row_sums[blk][gr + e * 8] = rs[e];
+      }
+      all = column_sum(rs[0] + rs[1]);
+      if (lane == 0) all_sums[blk] = all;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) cs[j][f] = w[j][f] + w[j][2 + f];
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -1100,48 +1135,72 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) linattn_backward_
   }
   __syncthreads();
   if (warp == 0) {
-    // dg_t = sum_(u >= t) (late_u) + sum_(u < t) new_u + across, with late = row sums - column sums + old
-    constexpr int M = C / 32;
-    float late[M], fresh[M], late_sum = 0.f, fresh_sum = 0.f;
+    // dg_t = sum_(u >= t) old_u + sum_(s < t) new_s + across + the pairs' share: the diagonal block's, whole blocks,
+    // and in t's block of 16 tokens the sums of rows from t on and of columns before t
+    constexpr int M = C / 32, W = 16 / M;  // tokens of a lane, lanes of a block
+    const int tb = lane / W;
+    float old[M], fresh[M], rows[M], cols[M], pairs[M], old_sum = 0.f, fresh_sum = 0.f, row_sum = 0.f, col_sum = 0.f;
+    float whole = 0.f;
+#pragma unroll
+    for (int o = 0; o < B16; ++o)
+#pragma unroll
+      for (int u = o + 2; u < B16; ++u)
+        if (o < tb && tb < u) whole += all_sums[u * (u + 1) / 2 + o];
 #pragma unroll
     for (int i = 0; i < M; ++i) {
-      const int t = lane * M + i, tb = t / 16;
+      const int t = lane * M + i;
       float x = 0.f, y = 0.f;
+      pairs[i] = col_sums[tb * (tb + 1) / 2 + tb][t % 16] + whole;
+#pragma unroll
       for (int o = 0; o < B16; ++o) {
-        if (o <= tb) x += row_sums[tb * (tb + 1) / 2 + o][t % 16];
-        if (o >= tb) x -= col_sums[o * (o + 1) / 2 + tb][t % 16];
+        if (o < tb) x += row_sums[tb * (tb + 1) / 2 + o][t % 16];
+        if (o > tb) y += col_sums[o * (o + 1) / 2 + tb][t % 16];
       }
+      rows[i] = x;
+      cols[i] = y;
+      row_sum += x;
+      col_sum += y;
+      x = y = 0.f;
       for (int w = 0; w < key_tiles; ++w) {
         x += old_part[w][t];
         y += new_part[w][t];
       }
-      late[i] = x;
+      old[i] = x;
       fresh[i] = y;
-      late_sum += x;
+      old_sum += x;
       fresh_sum += y;
     }
-    // sums from this lane's tokens on, and up to them (neither as a difference, that what is not finite stays on
-    // its side)
-    float from = late_sum, before = fresh_sum;
+    // sums over the lanes behind this one and before it, of all or of its block
+    auto behind = [&](float v, int width) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const float x = __shfl_down_sync(0xffffffffu, from, o), y = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane + o < 32) from += x;
-      if (lane >= o) before += y;
-    }
-    from = __shfl_down_sync(0xffffffffu, from, 1);  // behind this lane's
-    before = __shfl_up_sync(0xffffffffu, before, 1);
-    if (lane == 31) from = 0.f;
-    if (lane == 0) before = 0.f;
+      for (int o = 1; o < 32; o <<= 1) {
+        if (o >= width) break;
+        const float x = __shfl_down_sync(0xffffffffu, v, o, width);
+        if (lane % width + o < width) v += x;
+      }
+      v = __shfl_down_sync(0xffffffffu, v, 1, width);
+      return lane % width == width - 1 ? 0.f : v;
+    };
+    auto before = [&](float v, int width) {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        if (o >= width) break;
+        const float x = __shfl_up_sync(0xffffffffu, v, o, width);
+        if (lane % width >= o) v += x;
+      }
+      v = __shfl_up_sync(0xffffffffu, v, 1, width);
+      return lane % width == 0 ? 0.f : v;
+    };
+    float sum = behind(old_sum, 32) + before(fresh_sum, 32) + behind(row_sum, W) + before(col_sum, W);
     float across = 0.f;
     for (int w = 0; w < warps; ++w) across += across_part[w];
-    across *= d.whole;
+    sum += across * d.whole;
 #pragma unroll
     for (int i = 0; i < M; ++i) {
       const int t = lane * M + i;
-      float x = from + before + across;
+      float x = sum + pairs[i];
 #pragma unroll
-      for (int j = 0; j < M; ++j) x += j < i ? fresh[j] : late[j];
+      for (int j = 0; j < M; ++j) x += j < i ? fresh[j] + cols[j] : old[j] + rows[j];
       if (t < kept) dg[t] = t < n ? x : 0.f;
     }
   }
