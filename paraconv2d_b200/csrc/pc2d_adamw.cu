@@ -103,7 +103,7 @@ __device__ __forceinline__ int find_item(const Items<N> &a, int block) {
 }
 
 struct Rates {
-  float keep_first, keep_rest, lr_first, lr_rest, root, scale;
+  float drop_first, drop_rest, lr_first, lr_rest, root, scale;  // drop: what the decay takes of a weight
   int64_t split;
 };
 
@@ -116,7 +116,11 @@ __device__ __forceinline__ float weight(float w, float m, float v, bool first, c
   float s;
   asm("sqrt.approx.f32 %0, %1;" : "=f"(s) : "f"(v));
   const float step = __fdividef(m, fmaf(s, r.root, b.eps));
-  return (first ? r.keep_first : r.keep_rest) * w - (first ? r.lr_first : r.lr_rest) * step;
+  const float by = (first ? r.lr_first : r.lr_rest) * step;
+  // What goes off, and then off the weight: 1 - lr wd in 32 bits would be lr wd rounded to a multiple of 2^-24, nothing
+  // at all for lr wd = 1e-8.  (An infinite weight stays one.)
+  const float decayed = fmaf(first ? r.drop_first : r.drop_rest, w, by);
+  return w - (fabsf(w) == __int_as_float(0x7f800000) ? by : decayed);
 }
 
 // ------------------------------------------------------------- 8-bit moments
@@ -201,8 +205,8 @@ __device__ __forceinline__ void put(const float (&x)[N], T *p, bool whole, int l
 __device__ __forceinline__ Rates rates_of(const Item &it, const Coef *coef, const float *grad_scale, const Betas &b) {
   const float lr = coef->lr, lr1 = coef->lr1;
   Rates r;
-  r.keep_first = 1.f - lr * it.rate_first * b.wd * it.decay;
-  r.keep_rest = 1.f - lr * it.rate_rest * b.wd * it.decay;
+  r.drop_first = lr * it.rate_first * b.wd * it.decay;
+  r.drop_rest = lr * it.rate_rest * b.wd * it.decay;
   r.lr_first = lr1 * it.rate_first;
   r.lr_rest = lr1 * it.rate_rest;
   r.root = coef->root;
@@ -268,7 +272,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
 // Moments in 8 bits: a warp takes a block of 256 at a time, eight a lane (the
 // generator's 16 bytes are for eight elements; the largest values meet in one
 // instruction a warp).  Instructions bound it, not memory: 46 million bfloat16
-// parameters, 10 bytes each, take 184 us, 2.5 TB/s.  Codes by comparisons and
+// parameters, 10 bytes each, take 187 us, 2.5 TB/s.  Codes by comparisons and
 // shifts instead of products took 242, two blocks an SM instead of three
 // included.
 template <typename P, typename G, int N>
