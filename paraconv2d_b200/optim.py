@@ -200,8 +200,10 @@ class ParaboloidAdamW(Optimizer):
     parameters need the same one.  ``lr`` may be a float32 tensor on the GPU.
     Steps are counted on the GPU, for all parameters that have had the same
     gradients together (one that gets none is left as it is and goes on at its
-    own count), so that ``step`` can be captured into a CUDA graph after a first
-    one outside; the gradients must then stay the same tensors."""
+    own count), so that ``step`` can be captured into a CUDA graph after one
+    outside of the same parameters' gradients (a capture that would have to make
+    a state or a count raises); the gradients must then stay the same tensors,
+    and a step outside of other parameters ends the graph's use."""
 
     def __init__(self, params, lr: Union[float, Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32, masters: bool = False,
@@ -215,10 +217,17 @@ class ParaboloidAdamW(Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
                                       state_bits=state_bits, masters=bool(masters), seed=int(seed)))
 
+    @staticmethod
+    def _not_captured(why):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"ParaboloidAdamW: a parameter cannot be stepped in a capture yet: {why}; take a step with "
+                               "the same gradients outside it")
+
     def _new_state(self, p, group):
         if not p.is_cuda or p.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             raise NotImplementedError("ParaboloidAdamW: float32, float16 and bfloat16 parameters on the GPU only, got "
                                       f"{p.dtype} on {p.device}")
+        self._not_captured("its first step makes its state, which a graph would clear at every replay")
         state = self.state[p]
         state["exp_avg"], state["exp_avg_sq"], scales = adamw_new_state(p, group["state_bits"])
         if scales is not None:
@@ -248,7 +257,9 @@ class ParaboloidAdamW(Optimizer):
                 else:
                     count = self.state[members[0]]["step"]
                     if any(self.state[q].get("step") is count for q in group["params"] if q.grad is None):
-                        count = count.clone()  # the others stay where they are
+                        # the others stay where they are
+                        self._not_captured("it gets a count of its own, which a graph would start anew at every replay")
+                        count = count.clone()
                 for p in members:
                     self.state[p]["step"] = count
                 states = [self.state[p] for p in members]

@@ -45,3 +45,66 @@ def test_infinite_weights_stay_infinite(decay, bits):
     assert p[3] == float("inf") and p[270] == -float("inf")
     p[3] = p[270] = 0.0
     assert p.isfinite().all()
+
+
+# ------------------------------------------------------------------ optimizer
+
+def pair(bits, n=1000, **kw):
+    """Two parameters of the same values, and the optimizer of them."""
+    w = torch.randn(n, generator=gen(2))
+    params = [torch.nn.Parameter(w.to(DEV)) for _ in range(2)]
+    return params, pc.ParaboloidAdamW(params, lr=1e-2, state_bits=bits, seed=7, **kw)
+
+
+def give(params, on, grad):
+    for p, g in zip(params, on):
+        p.grad = grad.clone() if g else None
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_count_is_not_split_in_a_capture(bits):
+    """A parameter that lost its gradient since the first step would need a count of its own, which a graph would start
+    from the same number at every replay: refused; after a step outside it can be captured."""
+    (a, b), opt = pair(bits)
+    grad = torch.randn(1000, generator=gen(3)).to(DEV)
+    give((a, b), (1, 1), grad)
+    opt.step()
+    b.grad = None
+    with pytest.raises(RuntimeError, match="captur"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    opt.step()
+    assert opt.state[a]["step"].tolist() == [2] and opt.state[b]["step"].tolist() == [1]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+    (c, d), eager = pair(bits)
+    give((c, d), (1, 1), grad)
+    eager.step()
+    d.grad = None
+    for _ in range(4):
+        eager.step()
+    assert opt.state[a]["step"].tolist() == eager.state[c]["step"].tolist() == [5]
+    assert opt.state[b]["step"].tolist() == [1]
+    assert torch.equal(a, c) and torch.equal(b, d)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_no_state_is_made_in_a_capture(bits):
+    """A graph would clear the moments at every replay."""
+    (a, b), opt = pair(bits)
+    grad = torch.ones(1000, device=DEV)
+    give((a, b), (1, 1), grad)
+    with pytest.raises(RuntimeError, match="captur"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    give((a, b), (1, 0), grad)
+    opt.step()
+    give((a, b), (1, 1), grad)
+    with pytest.raises(RuntimeError, match="captur"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    opt.step()
+    assert opt.state[a]["step"].tolist() == [2] and opt.state[b]["step"].tolist() == [1]
