@@ -41,7 +41,7 @@ class AdamWTensor(ctypes.Structure):
                 ("grad", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p), ("exp_avg_sq", ctypes.c_void_p),
                 ("master", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("n", ctypes.c_int64),
                 ("split", ctypes.c_int64), ("rate_first", ctypes.c_double), ("rate_rest", ctypes.c_double),
-                ("decay", ctypes.c_double)]
+                ("decay", ctypes.c_double), ("shift", ctypes.c_int64)]
 
 
 _lock = threading.Lock()

@@ -54,7 +54,7 @@ struct Item {
   unsigned char *scales;
   int64_t n, split;
   float rate_first, rate_rest, decay;
-  int index;  // in the caller's list
+  int index;  // in the caller's list, and shifted: the tensor's number in the counter
   int vec;    // every array on the boundary that vectors need
 };
 
@@ -418,7 +418,7 @@ int in_launches(const pc2d_adamw_tensor *tensors, int count, Take &&take, Fill &
     it.v = tensors[i].exp_avg_sq;
     it.scales = tensors[i].scales;
     it.n = tensors[i].n;
-    it.index = i;
+    it.index = (int)(i + tensors[i].shift);
     fill(it, tensors[i]);
     items[used] = it;
     first[used++] = (int)blocks;
@@ -483,6 +483,8 @@ extern "C" int pc2d_adamw_step(int state_bits, const pc2d_adamw_tensor *tensors,
       return refuse("pc2d_adamw_step: tensor %d: parameters of float32, float16 or bfloat16, gradients of the same or "
                     "float32", i);
     if (t.n < 0 || t.n > (int64_t)1 << 34 || t.split < 0) return refuse("pc2d_adamw_step: tensor %d: invalid size", i);
+    if (state_bits == 8 && (t.shift < -i || t.shift > 0x7fffffff - i))
+      return refuse("pc2d_adamw_step: tensor %d: its number must be from 0 to 2^31 - 1", i);
     if (!isfinite(t.rate_first) || !isfinite(t.rate_rest) || !isfinite(t.decay))
       return refuse("pc2d_adamw_step: tensor %d: factors must be finite", i);
     if (t.master && t.dtype == PC2D_DTYPE_F32) return refuse("pc2d_adamw_step: tensor %d: a float32 parameter needs no "

@@ -45,7 +45,8 @@ struct Ranges {
 void adamw_step_cuda(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs, at::TensorList exp_avg_sqs,
                      at::TensorList masters, at::TensorList scales, const Tensor &step, const OptTensor &lr_tensor,
                      double lr, double beta1, double beta2, double eps, double weight_decay,
-                     const OptTensor &grad_scale_, at::IntArrayRef splits, at::ArrayRef<double> factors, int64_t seed) {
+                     const OptTensor &grad_scale_, at::IntArrayRef splits, at::ArrayRef<double> factors, int64_t seed,
+                     at::IntArrayRef numbers) {
   const Call call{"paraconv2d_b200.adamw_step", step.device()};
   const c10::cuda::CUDAGuard guard(step.device());
   const size_t count = params.size();
@@ -55,6 +56,7 @@ void adamw_step_cuda(at::TensorList params, at::TensorList grads, at::TensorList
               ": masters and scales must be as many as params, or none");
   TORCH_CHECK((splits.empty() && factors.empty()) || (splits.size() == count && factors.size() == 3 * count), call.what,
               ": a split and three factors for each of params, or none");
+  TORCH_CHECK(numbers.empty() || numbers.size() == count, call.what, ": a number for each of params, or none");
   TORCH_CHECK(count <= INT_MAX, call.what, ": too many tensors");
   call.in_place_any(step, "step", at::kLong, {1});
   Ranges ranges;
@@ -130,6 +132,11 @@ void adamw_step_cuda(at::TensorList params, at::TensorList grads, at::TensorList
     it.rate_first = factors.empty() ? 1.0 : factors[3 * i];
     it.rate_rest = factors.empty() ? 1.0 : factors[3 * i + 1];
     it.decay = factors.empty() ? 1.0 : factors[3 * i + 2];
+    if (!numbers.empty()) {
+      TORCH_CHECK(numbers[i] >= 0 && numbers[i] <= INT_MAX, call.what, ": numbers must be from 0 to 2^31 - 1, got ",
+                  numbers[i]);
+      it.shift = numbers[i] - (int64_t)i;
+    }
   }
   ranges.check(call.what);
   const size_t bytes = pc2d_adamw_workspace_size();
@@ -148,12 +155,12 @@ void adamw_step_autograd(at::TensorList params, at::TensorList grads, at::Tensor
                          at::TensorList exp_avg_sqs, at::TensorList masters, at::TensorList scales, const Tensor &step,
                          const OptTensor &lr_tensor, double lr, double beta1, double beta2, double eps,
                          double weight_decay, const OptTensor &grad_scale, at::IntArrayRef splits,
-                         at::ArrayRef<double> factors, int64_t seed) {
+                         at::ArrayRef<double> factors, int64_t seed, at::IntArrayRef numbers) {
   check_cuda(step, "adamw_step");
   at::AutoDispatchBelowADInplaceOrView below;
   PC2D_BELOW(adamw_step)
       .call(params, grads, exp_avgs, exp_avg_sqs, masters, scales, step, lr_tensor, lr, beta1, beta2, eps, weight_decay,
-            grad_scale, splits, factors, seed);
+            grad_scale, splits, factors, seed, numbers);
 }
 
 std::vector<Tensor> adamw_state_values_cuda(at::TensorList exp_avgs, at::TensorList exp_avg_sqs, at::TensorList scales,
@@ -490,7 +497,8 @@ TORCH_LIBRARY_FRAGMENT(paraconv2d_b200, m) {
   m.def(
       "adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avgs, Tensor(c!)[] exp_avg_sqs, "
       "Tensor(d!)[] masters, Tensor(e!)[] scales, Tensor(f!) step, Tensor? lr_tensor, float lr, float beta1, "
-      "float beta2, float eps, float weight_decay, Tensor? grad_scale, int[] splits, float[] factors, int seed) -> ()");
+      "float beta2, float eps, float weight_decay, Tensor? grad_scale, int[] splits, float[] factors, int seed, "
+      "int[] numbers=[]) -> ()");
   m.def(
       "group_norm_forward(Tensor input, Tensor? weight, Tensor? bias, Tensor? lengths, int groups, float eps, bool "
       "silu, bool keep_stats) -> Tensor[]");

@@ -118,7 +118,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
                betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                masters: Optional[Sequence[Optional[Tensor]]] = None, scales: Optional[Sequence[Tensor]] = None,
                factors: Optional[Sequence[Optional[Tuple[int, float, float, float]]]] = None,
-               grad_scale: Optional[Tensor] = None, seed: int = 0) -> None:
+               grad_scale: Optional[Tensor] = None, seed: int = 0, numbers: Optional[Sequence[int]] = None) -> None:
     """One AdamW step over many tensors, in place, in two launches (and one
     more for every further combination of types, and beyond 320 tensors)::
 
@@ -140,7 +140,8 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     The moments are float32 of their parameter's shape and strides, or uint8
     [n] with ``scales`` (uint8 [ceil(n/256), 2]): codes of 8-bit floats with
     3 bits of mantissa under an exponent for every 256 elements, rounded
-    stochastically by ``seed``, the step and the element's place (see
+    stochastically by ``seed``, the step, the tensor's number (``numbers``, or
+    its place in the list) and the element's place in it (see
     :func:`adamw_new_state`, :func:`adamw_state_values`).  The update is
     computed from the moments before they are rounded.  Where a moment is not
     finite, the state of its 256 elements becomes NaN.
@@ -162,7 +163,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
             splits.append(split)
             rates += (first, rest, decay)
     _adamw_step(params, grads, exp_avgs, exp_avg_sqs, masters or [], scales or [], step, rate_tensor, rate, betas[0],
-                betas[1], eps, weight_decay, grad_scale, splits, rates, seed)
+                betas[1], eps, weight_decay, grad_scale, splits, rates, seed, numbers or [])
 
 
 def adamw_new_state(param: Tensor, bits: int = 32):
@@ -196,8 +197,8 @@ class ParaboloidAdamW(Optimizer):
 
     ``state_bits``: 32, or 8 for moments of two bytes and a 128th per element
     instead of eight.  ``masters``: keep float32 copies of 16-bit parameters.  ``seed``:
-    of the stochastic rounding of 8-bit moments; ranks that hold the same
-    parameters need the same one.  ``lr`` may be a float32 tensor on the GPU.
+    of the stochastic rounding of 8-bit moments, with a parameter's place among
+    all of the optimizer's; ranks that hold the same parameters need the same one.  ``lr`` may be a float32 tensor on the GPU.
     Steps are counted on the GPU, for all parameters that have had the same
     gradients together (one that gets none is left as it is and goes on at its
     own count), so that ``step`` can be captured into a CUDA graph after one
@@ -241,9 +242,12 @@ class ParaboloidAdamW(Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for index, group in enumerate(self.param_groups):
+        number, numbers = 0, {}  # places among all parameters: what their random numbers go by
+        for group in self.param_groups:
             cohorts = {}  # parameters by the counter that they share
             for p in group["params"]:
+                numbers[p] = number
+                number += 1
                 if p.grad is None:
                     continue
                 if "step" not in self.state[p]:
@@ -277,7 +281,8 @@ class ParaboloidAdamW(Optimizer):
                            eps=group["eps"], weight_decay=group["weight_decay"],
                            masters=[s.get("master") for s in states] if group["masters"] else None,
                            scales=[s["scales"] for s in states] if group["state_bits"] == 8 else None,
-                           factors=factors, grad_scale=grad_scale, seed=group["seed"] + index)
+                           factors=factors, grad_scale=grad_scale, seed=group["seed"],
+                           numbers=[numbers[p] for p in members] if group["state_bits"] == 8 else None)
         return loss
 
     def load_state_dict(self, state_dict):

@@ -1,8 +1,11 @@
 """The AdamW step on the GPU: small decays, infinite weights, and the optimizer's
 counts and random numbers."""
+import copy
+
 import pytest
 import torch
 
+import train_ref as ref
 import paraconv2d_b200 as pc
 
 pytestmark = pytest.mark.gpu
@@ -108,3 +111,77 @@ def test_no_state_is_made_in_a_capture(bits):
             opt.step()
     opt.step()
     assert opt.state[a]["step"].tolist() == [2] and opt.state[b]["step"].tolist() == [1]
+
+
+def codes_of(params, opt):
+    return [[opt.state[p][k].cpu() for k in ("exp_avg", "exp_avg_sq", "scales")] for p in params]
+
+
+@pytest.mark.parametrize("how", ["together", "one by one", "groups"])
+def test_random_numbers_belong_to_the_parameter(how):
+    """Each parameter's moments are rounded by the numbers of its place among all parameters, whichever others a step
+    takes and whatever group it is in."""
+    (a, b), opt = pair(8)
+    if how == "groups":
+        opt = pc.ParaboloidAdamW([{"params": [a]}, {"params": [b], "weight_decay": 0.0}], lr=1e-2, state_bits=8, seed=7)
+    grad = torch.randn(1000, generator=gen(4))
+    for on in ((1, 0), (0, 1)) if how == "one by one" else ((1, 1),):
+        give((a, b), on, grad.to(DEV))
+        opt.step()
+    new = [pc.adamw_new_state(torch.empty(1000), 8) for _ in range(2)]
+    c = dict(params=[a.detach().cpu()] * 2, grads=[grad] * 2, masters=None, m=[s[0] for s in new], v=[s[1] for s in new],
+             scales=[s[2] for s in new])
+    want = ref.adamw(c, 1, lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, seed=7)
+    got = codes_of((a, b), opt)
+    for (m, v, s), w in zip(got, want):
+        assert torch.equal(m, w["m_code"]) and torch.equal(v, w["v_code"]) and torch.equal(s, w["scales"])
+    assert not torch.equal(got[0][0], got[1][0]) and not torch.equal(got[0][1], got[1][1])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_checkpoint_of_counts_that_met(bits):
+    """Parameters that missed different steps and have equal counts go on alike, reloaded or not."""
+    grads = torch.randn(8, 1000, generator=gen(5)).to(DEV)
+
+    def run(params, opt, steps):
+        for i, on in steps:
+            give(params, on, grads[i])
+            opt.step()
+
+    params, opt = pair(bits)
+    run(params, opt, [(0, (1, 0)), (1, (0, 1))])
+    values, kept = [p.detach().clone() for p in params], copy.deepcopy(opt.state_dict())
+    more = [(i, (1, 1)) for i in range(2, 6)]
+    run(params, opt, more)
+    others, opt2 = pair(bits)
+    with torch.no_grad():
+        for p, v in zip(others, values):
+            p.copy_(v)
+    opt2.load_state_dict(kept)
+    run(others, opt2, more)
+    for p, q in zip(params, others):
+        assert torch.equal(p, q)
+        for k in opt.state[p]:
+            assert torch.equal(opt.state[p][k], opt2.state[q][k]), k
+
+
+def test_numbers_of_the_function():
+    """adamw_step's own numbers: the list's places unless given."""
+    n = 600
+    grad = torch.randn(n, generator=gen(6))
+
+    def call(**kw):
+        states = [[t.to(DEV) for t in pc.adamw_new_state(torch.empty(n), 8)] for _ in range(3)]
+        pc.adamw_step([torch.zeros(n, device=DEV) for _ in range(3)], [grad.to(DEV)] * 3, [s[0] for s in states],
+                      [s[1] for s in states], torch.zeros(1, dtype=torch.int64, device=DEV), lr=0.1,
+                      scales=[s[2] for s in states], seed=3, **kw)
+        return [s[0].cpu() for s in states]
+
+    plain, moved = call(), call(numbers=[2, 7, 0])
+    assert torch.equal(moved[0], plain[2]) and torch.equal(moved[2], plain[0])
+    low = ref.adamw_random(n, 3, 1, 7)[0]
+    want, _ = ref.adamw_encode((grad * float(torch.tensor(1 - 0.9))).double(), low, True)
+    assert torch.equal(moved[1], want)
+    for bad in ([0, 1], [0, 1, -1], [0, 1, 2 ** 31]):
+        with pytest.raises((RuntimeError, ValueError)):
+            call(numbers=bad)
