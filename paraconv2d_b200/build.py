@@ -51,6 +51,19 @@ def _run(cmd, verbose):
     return res
 
 
+def _compile(cmd, obj, verbose):
+    """Runs cmd with the output `obj`, which is there whole or not at all: an interrupted build leaves no part of one
+    that a later build would take as up to date, and one beside it none that it would link half written."""
+    tmp = f"{obj}.tmp{os.getpid()}"
+    try:
+        res = _run([*cmd, "-o", tmp], verbose)
+        os.replace(tmp, obj)
+    finally:
+        if os.path.exists(tmp):
+            os.remove(tmp)
+    return res
+
+
 def kernel_sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.cu")))
 
@@ -72,7 +85,7 @@ def build_kernel_lib(force=False, verbose=False, ptxas_verbose=False):
         obj = os.path.join(BUILD, os.path.basename(src) + ".o")
         if not (force or ptxas_verbose) and os.path.exists(obj) and os.path.getmtime(obj) >= max(newest, os.path.getmtime(src)):
             return obj
-        _run([NVCC, *ARCH_FLAGS, *NVCC_FLAGS, *extra, "-c", src, "-o", obj], verbose or ptxas_verbose)
+        _compile([NVCC, *ARCH_FLAGS, *NVCC_FLAGS, *extra, "-c", src], obj, verbose or ptxas_verbose)
         return obj
 
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
@@ -100,11 +113,11 @@ def build_op_lib(force=False, verbose=False):
 
     def compile_one(src):
         obj = os.path.join(BUILD, os.path.basename(src) + ".o")
-        _run([cxx, "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-              "-isystem", os.path.join(tdir, "include"),
-              "-isystem", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
-              "-isystem", sysconfig.get_path("include"), "-I" + os.path.join(CUDA_HOME, "include"), "-I" + INCLUDE,
-              "-c", src, "-o", obj], verbose)
+        _compile([cxx, "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+                  "-isystem", os.path.join(tdir, "include"),
+                  "-isystem", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
+                  "-isystem", sysconfig.get_path("include"), "-I" + os.path.join(CUDA_HOME, "include"), "-I" + INCLUDE,
+                  "-c", src], obj, verbose)
         return obj
 
     with cf.ThreadPoolExecutor(max_workers=len(srcs)) as ex:
