@@ -34,10 +34,10 @@
 // (tcgen05) it would be read, scaled, split and written again for each.
 //
 // Measured (one B200).  4 rows of 32 heads of 64 at 2048 tokens, bfloat16, a
-// training step: 438 us, of these outputs 89, states of the segments 37,
-// gradients' states 38 + 45, gradients 232.  16 heads of 128 at 16384 tokens:
-// 283 us, states of the segments 100 (tensor pipe half busy: it multiplies
-// three planes), outputs 187.  Everywhere the steps from one product to the
+// training step: 474 us, of these outputs 101, states of the segments 37,
+// gradients' states 38 + 44, gradients 250.  16 heads of 128 at 16384 tokens:
+// 337 us, states of the segments 100 (tensor pipe half busy: it multiplies
+// three planes), outputs 242 (each kernel's time from a cold cache).  Everywhere the steps from one product to the
 // next (loads from shared memory, splits, exponentials) leave the tensor pipe
 // idle; what helped was more warps for an SM, fewer instructions between
 // products (no calls, fixed strides) and no 64-bit arithmetic.
@@ -1330,8 +1330,9 @@ Plan make_plan(int dtype, int batch, int heads, int length, int dk, int dv) {
   };
   p.segments = segments(4);
   // Five fit with up to 64 keys: taken where their segments are shorter by as much as they share the SM more (70 heads
-  // of 48x80 at 777 tokens: 5 segments of 5 chunks 70 us, 4 of up to 7 84; 128 heads of 64 at 2048 tokens, where they
-  // would be 5 of up to 7 chunks for 4 of 8: 449 us for 438).
+  // of 48x80 at 777 tokens in float16: 5 segments of 5 chunks 96 us, 4 of up to 7 112; 128 heads of 64 at 2048 tokens in
+  // bfloat16, where they would be 5 of up to 7 chunks for 4 of 8: 154 us for 146, a training step 508 for 493; from a
+  // cold cache, in turn).
   if (dk <= 64 && ceil_div(p.chunks, segments(5)) * 5 <= ceil_div(p.chunks, p.segments) * 4) p.segments = segments(5);
   p.per_segment = ceil_div(p.chunks, p.segments);
   p.segments = std::max(1, ceil_div(p.chunks, std::max(1, p.per_segment)));

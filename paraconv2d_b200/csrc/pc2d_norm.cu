@@ -15,7 +15,7 @@
 // and go over it again there; what does not fit is read again, from the L2
 // cache as a rule.  Each thread reads only what it has copied.
 // Measured (one B200; of a training step, forwards / backwards): 64x128x56x56
-// float32 43 / 71 us, 4.8 and 4.3 TB/s of the three or five passes over the map
+// float32 43 / 71 us, 4.8 and 4.3 TB/s of the two or three passes over the map
 // that have to be; 16x512x64x64 bfloat16 channels last 50 / 86 us, 2.7 and 2.3
 // TB/s.  The first is near the memory's time; the second is bound by the
 // exponentials and reciprocals of the sigmoid (two an element forwards, four
