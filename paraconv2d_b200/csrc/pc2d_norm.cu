@@ -16,7 +16,7 @@
 // cache as a rule.  Each thread reads only what it has copied.
 // Measured (one B200; of a training step, forwards / backwards): 64x128x56x56
 // float32 43 / 71 us, 4.8 and 4.3 TB/s of the two or three passes over the map
-// that have to be; 16x512x64x64 bfloat16 channels last 50 / 86 us, 2.7 and 2.3
+// that have to be; 16x512x64x64 bfloat16 channels last 51 / 87 us, 2.6 and 2.3
 // TB/s.  The first is near the memory's time; the second is bound by the
 // exponentials and reciprocals of the sigmoid (two an element forwards, four
 // backwards: at least 15 and 30 us) and by the chain load, sum, exchange, go
@@ -28,8 +28,10 @@
 // the channel, channels last), and the (count, mean, M2) of threads, warps and
 // blocks are joined by M2 = sum M2_i + n_i (mean_i - mean)^2.  Neither a large
 // mean nor a single outlier cancels: a thread's sums are off by 2^-24 of
-// squares that the slab's M2 holds too, once per element of the thread.
-// All joins go by fixed orders.
+// squares that the slab's M2 holds too, once per element of a run of the thread.
+// Runs are at most kRun vectors: a sum over tens of thousands of squares rounds
+// the small ones among them away, all to one side (65,536 a thread: 7e-5 of the
+// variance).  All joins go by fixed orders.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -45,6 +47,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
+constexpr int kRun = 256;             // vectors of a thread that are summed before they are joined with those before
 constexpr int kMaxSplit = 64;         // blocks of a slab that exchange through device memory
 constexpr int kMaxChannels = 8192;    // of a slab: its sums are in shared memory
 constexpr int kCacheBytes = 64 * 1024;  // of a slab's share that a block keeps, x and dy together
@@ -409,49 +412,59 @@ struct Norm {
         });
         arrived();
       }
-      columns([&](int col, int slot, int n) {
-        float2 k[P] = {}, s[P] = {}, q[P] = {};
-        each<kFlight>(a, kept, slot, x + place(col), stride, n, [&](const Vec &v, int j) {
-          if (j == 0)
+      columns([&](int col, int slot, int all_mine) {
+        for (int run = 0; run == 0 || run < l.slots(); run += kRun) {
+          const int n = min(max(all_mine - run, 0), kRun);
+          float2 k[P] = {}, s[P] = {}, q[P] = {};
+          each<kFlight>(a, kept, slot + run, x + place(col) + run * stride, stride, n, [&](const Vec &v, int j) {
+            if (j == 0)
 #pragma unroll
-            for (int i = 0; i < P; ++i) k[i] = mul2(get(v, i), both(-1.f));
-#pragma unroll
-          for (int i = 0; i < P; ++i) {
-            const float2 d = add2(get(v, i), k[i]);
-            s[i] = add2(s[i], d);
-            q[i] = fma2(d, d, q[i]);
-          }
-        });
-        const float inv = n > 0 ? 1.f / n : 0.f;
-#pragma unroll
-        for (int i = 0; i < P; ++i) {  // s: the mean, q: M2
-          const float2 m = mul2(s[i], both(inv));
-          q[i] = fma2(s[i], mul2(m, both(-1.f)), q[i]);
-          s[i] = n > 0 ? fma2(k[i], both(-1.f), m) : both(0.f);
-        }
-        if (l.folds()) {
-          float count = n;
-          for (int o = l.cols; o < 32; o <<= 1) {
-            const float other = __shfl_xor_sync(0xffffffffu, count, o), sum = count + other;
-            const float share = sum > 0.f ? other / sum : 0.f;
+              for (int i = 0; i < P; ++i) k[i] = mul2(get(v, i), both(-1.f));
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-              const float2 m = make_float2(__shfl_xor_sync(0xffffffffu, s[i].x, o), __shfl_xor_sync(0xffffffffu, s[i].y, o));
-              const float2 v = make_float2(__shfl_xor_sync(0xffffffffu, q[i].x, o), __shfl_xor_sync(0xffffffffu, q[i].y, o));
-              const float2 d = fma2(s[i], both(-1.f), m);
-              s[i] = fma2(d, both(share), s[i]);
-              q[i] = add2(add2(q[i], v), mul2(mul2(d, d), both(count * share)));
+              const float2 d = add2(get(v, i), k[i]);
+              s[i] = add2(s[i], d);
+              q[i] = fma2(d, d, q[i]);
             }
-            count = sum;
-          }
-        }
-        if (l.sums_here() && col < l.sv)
+          });
+          const float inv = n > 0 ? 1.f / n : 0.f;
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            float *e = red + 2 * ((size_t)l.sum_row(ty) * l.sc + col * V + i);
-            e[0] = Norm::at(s, i);
-            e[1] = Norm::at(q, i);
+          for (int i = 0; i < P; ++i) {  // s: the mean, q: M2
+            const float2 m = mul2(s[i], both(inv));
+            q[i] = fma2(s[i], mul2(m, both(-1.f)), q[i]);
+            s[i] = n > 0 ? fma2(k[i], both(-1.f), m) : both(0.f);
           }
+          float count = n;
+          if (l.folds()) {
+            for (int o = l.cols; o < 32; o <<= 1) {
+              const float other = __shfl_xor_sync(0xffffffffu, count, o), sum = count + other;
+              const float share = sum > 0.f ? other / sum : 0.f;
+#pragma unroll
+              for (int i = 0; i < P; ++i) {
+                const float2 m = make_float2(__shfl_xor_sync(0xffffffffu, s[i].x, o), __shfl_xor_sync(0xffffffffu, s[i].y, o));
+                const float2 v = make_float2(__shfl_xor_sync(0xffffffffu, q[i].x, o), __shfl_xor_sync(0xffffffffu, q[i].y, o));
+                const float2 d = fma2(s[i], both(-1.f), m);
+                s[i] = fma2(d, both(share), s[i]);
+                q[i] = add2(add2(q[i], v), mul2(mul2(d, d), both(count * share)));
+              }
+              count = sum;
+            }
+          }
+          if (l.sums_here() && col < l.sv)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              float *e = red + 2 * ((size_t)l.sum_row(ty) * l.sc + col * V + i);
+              if (run == 0) {
+                e[0] = Norm::at(s, i);
+                e[1] = Norm::at(q, i);
+              } else {  // (all rows of threads had the tokens of the runs before)
+                const float had = (float)run * (l.folds() ? 32 >> l.log : 1), share = count / (had + count);
+                const float d = Norm::at(s, i) - e[0];
+                e[0] = fmaf(d, share, e[0]);
+                e[1] += Norm::at(q, i) + d * d * (had * share);
+              }
+            }
+        }
       });
       __syncthreads();
       // few groups of many sums: several warps share one's rows
@@ -591,32 +604,36 @@ struct Norm {
       columns([&](int col, int slot, int n) {
         if (n) channel(col);
         if (slot == 0) arrived();
-        float2 s[P] = {}, q[P] = {};
-        by_silu(a, [&](auto silu) {
-          each_two<kFlightTwo>(a, kept, slot, x + place(col), dy + place(col), stride, n, [&](const Two &v, int) {
+        for (int run = 0; run == 0 || run < l.slots(); run += kRun) {
+          float2 s[P] = {}, q[P] = {};
+          by_silu(a, [&](auto silu) {
+            const int64_t from = place(col) + run * stride;
+            const int here = min(max(n - run, 0), kRun);
+            each_two<kFlightTwo>(a, kept, slot + run, x + from, dy + from, stride, here, [&](const Two &v, int) {
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-              float2 xhat;
-              const float2 h = slope(silu, v, i, xhat);
-              s[i] = add2(s[i], h);
-              q[i] = fma2(h, xhat, q[i]);
-            }
+              for (int i = 0; i < P; ++i) {
+                float2 xhat;
+                const float2 h = slope(silu, v, i, xhat);
+                s[i] = add2(s[i], h);
+                q[i] = fma2(h, xhat, q[i]);
+              }
+            });
           });
-        });
-        if (l.folds())
-          for (int o = l.cols; o < 32; o <<= 1)
+          if (l.folds())
+            for (int o = l.cols; o < 32; o <<= 1)
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-              s[i] = add2(s[i], make_float2(__shfl_xor_sync(0xffffffffu, s[i].x, o), __shfl_xor_sync(0xffffffffu, s[i].y, o)));
-              q[i] = add2(q[i], make_float2(__shfl_xor_sync(0xffffffffu, q[i].x, o), __shfl_xor_sync(0xffffffffu, q[i].y, o)));
+              for (int i = 0; i < P; ++i) {
+                s[i] = add2(s[i], make_float2(__shfl_xor_sync(0xffffffffu, s[i].x, o), __shfl_xor_sync(0xffffffffu, s[i].y, o)));
+                q[i] = add2(q[i], make_float2(__shfl_xor_sync(0xffffffffu, q[i].x, o), __shfl_xor_sync(0xffffffffu, q[i].y, o)));
+              }
+          if (l.sums_here() && col < l.sv)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              float *e = red + 2 * ((size_t)l.sum_row(ty) * l.sc + col * V + i);
+              e[0] = run == 0 ? Norm::at(s, i) : e[0] + Norm::at(s, i);
+              e[1] = run == 0 ? Norm::at(q, i) : e[1] + Norm::at(q, i);
             }
-        if (l.sums_here() && col < l.sv)
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            float *e = red + 2 * ((size_t)l.sum_row(ty) * l.sc + col * V + i);
-            e[0] = Norm::at(s, i);
-            e[1] = Norm::at(q, i);
-          }
+        }
       });
       __syncthreads();
       // a number's rows over up to 32 lanes
@@ -757,19 +774,25 @@ struct Norm {
       int count = 0;
       pieces(a, f, p.len, [&](int row, int t0, int t1, int slot, int n) {
         const T *at = x + f.base + (int64_t)row * a.P + t0;
-        each<kFlight>(a, kept, slot, at, step, n, [&](const Vec &v, int j) {
-          // all of a vector's tokens, or (at a row's last) some
-          const int left = min(t1 - t0 - j * step, V);
-          if (count == 0) k = v.f(0);
-          count += left;
+        for (int run = 0; run < n; run += kRun) {
+          const int here = min(n - run, kRun);
+          float2 s1 = {}, q1 = {};
+          each<kFlight>(a, kept, slot + run, at + (int64_t)run * step, step, here, [&](const Vec &v, int j) {
+            // all of a vector's tokens, or (at a row's last) some
+            const int left = min(t1 - t0 - (run + j) * step, V);
+            if (count == 0) k = v.f(0);
+            count += left;
 #pragma unroll
-          for (int i = 0; i < P; ++i) {
-            float2 d = add2(get(v, i), both(-k));
-            if (left < V || V == 1) d = make_float2(2 * i < left ? d.x : 0.f, 2 * i + 1 < left ? d.y : 0.f);
-            s2 = add2(s2, d);
-            q2 = fma2(d, d, q2);
-          }
-        });
+            for (int i = 0; i < P; ++i) {
+              float2 d = add2(get(v, i), both(-k));
+              if (left < V || V == 1) d = make_float2(2 * i < left ? d.x : 0.f, 2 * i + 1 < left ? d.y : 0.f);
+              s1 = add2(s1, d);
+              q1 = fma2(d, d, q1);
+            }
+          });
+          s2 = add2(s2, s1);
+          q2 = add2(q2, q1);
+        }
       });
       const float s = s2.x + s2.y, q = q2.x + q2.y, m = count ? s / count : 0.f;
       float *e = red + 3 * threadIdx.x;
@@ -864,19 +887,26 @@ struct Norm {
           channel(row);
           const int64_t at = f.base + (int64_t)row * a.P + t0;
           by_silu(a, [&](auto silu) {
-            each_two<kFlightTwo>(a, kept, slot, x + at, dy + at, step, n, [&](const Two &v, int j) {
-              float2 h[P];
+            for (int run = 0; run < n; run += kRun) {
+              const int64_t from = at + (int64_t)run * step;
+              const int here = min(n - run, kRun);
+              float2 s1 = {}, q1 = {};
+              each_two<kFlightTwo>(a, kept, slot + run, x + from, dy + from, step, here, [&](const Two &v, int j) {
+                float2 h[P];
 #pragma unroll
-              for (int e = 0; e < P; ++e) {
-                float2 xhat;
-                h[e] = held(slope(silu, v, e, xhat), e, t1 - t0 - j * step);
-                s2 = add2(s2, h[e]);
-                q2 = add2(q2, held(mul2(h[e], xhat), e, t1 - t0 - j * step));
-              }
-              // (in 32 bits, what the second pass needs of dy is kept in its place)
-              if (kReuse && slot + j < a.cache)
-                write(reinterpret_cast<T *>(kept_d + ((size_t)(slot + j) * kThreads + threadIdx.x) * 16), h);
-            });
+                for (int e = 0; e < P; ++e) {
+                  float2 xhat;
+                  h[e] = held(slope(silu, v, e, xhat), e, t1 - t0 - (run + j) * step);
+                  s1 = add2(s1, h[e]);
+                  q1 = add2(q1, held(mul2(h[e], xhat), e, t1 - t0 - (run + j) * step));
+                }
+                // (in 32 bits, what the second pass needs of dy is kept in its place)
+                if (kReuse && slot + run + j < a.cache)
+                  write(reinterpret_cast<T *>(kept_d + ((size_t)(slot + run + j) * kThreads + threadIdx.x) * 16), h);
+              });
+              s2 = add2(s2, s1);
+              q2 = add2(q2, q1);
+            }
           });
           slot += n;
         }
