@@ -61,3 +61,37 @@ def test_adamw(bits, ptype, gtype, masters):
     c = adamw.case(adamw.SIZES, ptype, gtype, bits, masters, seed=46)
     got, want = adamw.step_both(c, 6, 99, grad_scale=0.7)
     adamw.check(got, want, c)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("name", ["q", "k", "v", "g"])
+def test_attention_beside_infinities(name, value, dtype):
+    attention.test_values_that_are_not_finite_reach_no_earlier_token(name, value, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_gradients_beside_infinities(dtype):
+    attention.test_gradients_that_are_not_finite_reach_no_later_token(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_attention_states(dtype):
+    attention.test_large_states(dtype)
+    attention.test_step((3, 2, 1, 33, 65), dtype)
+    if dtype != F16:
+        attention.test_steps_go_on_from_a_prompt(dtype)
+
+
+def test_attention_forgets_all():
+    attention.test_forgetting()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_beside_infinities(bits):
+    adamw.test_values_that_are_not_finite(bits)
+
+
+@pytest.mark.parametrize("last", [False, True])
+def test_norm_of_large_means_and_outliers(last):
+    norm.test_large_means_and_outliers(last)
