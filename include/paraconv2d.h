@@ -384,9 +384,10 @@ int pc2d_linear_attention_step(int dtype, const void *q, const void *k, const vo
  * value, rounded up to a code, into the topmost binade, and values are rounded up with the
  * probability of what is cut off: size/step + (r + 1/2)/256, rounded down,
  * where r is byte j of the first (m) or of the last (v) two words that
- * Philox4x32-10 gives for the counter (element/8, i + shift, t low, t high)
- * under the key `seed`, j = element % 8 (`shift` lets a tensor keep its numbers
- * whatever its place in the list; 0 <= i + shift < 2^31); a v that is not zero gets code 1 at least.  Per call: two launches, and more beyond 320 tensors
+ * Philox4x32-10 gives for the counter (element/8, i, t low, t high) under the
+ * key `seed`, j = element % 8 (pc2d_adamw_step_numbered takes numbers[i], from 0
+ * to 2^31 - 1, in the place of i: a tensor's random numbers then do not depend on its
+ * place in the list; numbers is read before the call returns); a v that is not zero gets code 1 at least.  Per call: two launches, and more beyond 320 tensors
  * or for more types.  workspace: pc2d_adamw_workspace_size() bytes.
  * pc2d_adamw_state_values writes the values of 8-bit moments (exp_avg,
  * exp_avg_sq, scales and n of each tensor) as F32 or BF16, both exact. */
@@ -399,12 +400,15 @@ typedef struct {
   unsigned char *scales; /* 8 bits only */
   int64_t n, split;
   double rate_first, rate_rest, decay;
-  int64_t shift;         /* of its number in the random numbers' counter; 8 bits only */
 } pc2d_adamw_tensor;
 size_t pc2d_adamw_workspace_size(void);
 int pc2d_adamw_step(int state_bits, const pc2d_adamw_tensor *tensors, int count, int64_t *step, const float *lr_device,
                     double lr, double beta1, double beta2, double eps, double weight_decay, const float *grad_scale,
                     int64_t seed, void *workspace, size_t workspace_bytes, void *stream);
+int pc2d_adamw_step_numbered(int state_bits, const pc2d_adamw_tensor *tensors, int count, const int64_t *numbers,
+                             int64_t *step, const float *lr_device, double lr, double beta1, double beta2, double eps,
+                             double weight_decay, const float *grad_scale, int64_t seed, void *workspace,
+                             size_t workspace_bytes, void *stream);
 int pc2d_adamw_state_values(int dtype, const pc2d_adamw_tensor *tensors, int count, void *const *exp_avgs,
                             void *const *exp_avg_sqs, void *stream);
 

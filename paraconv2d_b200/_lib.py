@@ -41,7 +41,7 @@ class AdamWTensor(ctypes.Structure):
                 ("grad", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p), ("exp_avg_sq", ctypes.c_void_p),
                 ("master", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("n", ctypes.c_int64),
                 ("split", ctypes.c_int64), ("rate_first", ctypes.c_double), ("rate_rest", ctypes.c_double),
-                ("decay", ctypes.c_double), ("shift", ctypes.c_int64)]
+                ("decay", ctypes.c_double)]
 
 
 _lock = threading.Lock()
@@ -123,6 +123,7 @@ def cabi() -> ctypes.CDLL:
             "pc2d_linear_attention_step": ([I] + [P] * 4 + [I, P, P] + [I] * 6 + [D, P, P], I),
             "pc2d_adamw_workspace_size": ([], S),
             "pc2d_adamw_step": ([I, ctypes.POINTER(AdamWTensor), I, P, P] + [D] * 5 + [P, L, P, S, P], I),
+            "pc2d_adamw_step_numbered": ([I, ctypes.POINTER(AdamWTensor), I, P, P, P] + [D] * 5 + [P, L, P, S, P], I),
             "pc2d_adamw_state_values": ([I, ctypes.POINTER(AdamWTensor), I, ctypes.POINTER(P), ctypes.POINTER(P), P],
                                         I),
             "pc2d_status_string": ([I], ctypes.c_char_p),

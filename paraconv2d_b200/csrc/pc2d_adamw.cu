@@ -54,7 +54,7 @@ struct Item {
   unsigned char *scales;
   int64_t n, split;
   float rate_first, rate_rest, decay;
-  int index;  // in the caller's list, and shifted: the tensor's number in the counter
+  int index;  // the tensor's number in the counter
   int vec;    // every array on the boundary that vectors need
 };
 
@@ -418,7 +418,7 @@ int in_launches(const pc2d_adamw_tensor *tensors, int count, Take &&take, Fill &
     it.v = tensors[i].exp_avg_sq;
     it.scales = tensors[i].scales;
     it.n = tensors[i].n;
-    it.index = (int)(i + tensors[i].shift);
+    it.index = i;
     fill(it, tensors[i]);
     items[used] = it;
     first[used++] = (int)blocks;
@@ -428,14 +428,15 @@ int in_launches(const pc2d_adamw_tensor *tensors, int count, Take &&take, Fill &
 }
 
 template <typename P, typename G>
-int launch_group(int bits, const pc2d_adamw_tensor *tensors, int count, int dtype, int grad_dtype, const Coef *coef,
-                 const float *grad_scale, const Betas &b, cudaStream_t stream) {
+int launch_group(int bits, const pc2d_adamw_tensor *tensors, int count, const int64_t *numbers, int dtype,
+                 int grad_dtype, const Coef *coef, const float *grad_scale, const Betas &b, cudaStream_t stream) {
   auto take = [&](const pc2d_adamw_tensor &t) { return t.n > 0 && t.dtype == dtype && t.grad_dtype == grad_dtype; };
   auto fill = [&](Item &it, const pc2d_adamw_tensor &t) {
     it.param = t.param;
     it.grad = t.grad;
     it.master = t.master;
     it.split = t.split;
+    if (numbers) it.index = (int)numbers[&t - tensors];
     it.rate_first = (float)t.rate_first;
     it.rate_rest = (float)t.rate_rest;
     it.decay = (float)t.decay;
@@ -469,6 +470,15 @@ extern "C" int pc2d_adamw_step(int state_bits, const pc2d_adamw_tensor *tensors,
                                const float *lr_device, double lr, double beta1, double beta2, double eps,
                                double weight_decay, const float *grad_scale, int64_t seed, void *workspace,
                                size_t workspace_bytes, void *stream) {
+  return pc2d_adamw_step_numbered(state_bits, tensors, count, nullptr, step, lr_device, lr, beta1, beta2, eps,
+                                  weight_decay, grad_scale, seed, workspace, workspace_bytes, stream);
+}
+
+extern "C" int pc2d_adamw_step_numbered(int state_bits, const pc2d_adamw_tensor *tensors, int count,
+                                        const int64_t *numbers, int64_t *step, const float *lr_device, double lr,
+                                        double beta1, double beta2, double eps, double weight_decay,
+                                        const float *grad_scale, int64_t seed, void *workspace, size_t workspace_bytes,
+                                        void *stream) {
   NvtxRange range("pc2d_adamw_step");
   if (state_bits != 8 && state_bits != 32) return refuse("pc2d_adamw_step: states of 32 or 8 bits, got %d", state_bits);
   if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) || !(weight_decay >= 0.0) ||
@@ -483,7 +493,7 @@ extern "C" int pc2d_adamw_step(int state_bits, const pc2d_adamw_tensor *tensors,
       return refuse("pc2d_adamw_step: tensor %d: parameters of float32, float16 or bfloat16, gradients of the same or "
                     "float32", i);
     if (t.n < 0 || t.n > (int64_t)1 << 34 || t.split < 0) return refuse("pc2d_adamw_step: tensor %d: invalid size", i);
-    if (state_bits == 8 && (t.shift < -i || t.shift > 0x7fffffff - i))
+    if (numbers && (numbers[i] < 0 || numbers[i] > 0x7fffffff))
       return refuse("pc2d_adamw_step: tensor %d: its number must be from 0 to 2^31 - 1", i);
     if (!isfinite(t.rate_first) || !isfinite(t.rate_rest) || !isfinite(t.decay))
       return refuse("pc2d_adamw_step: tensor %d: factors must be finite", i);
@@ -514,13 +524,17 @@ extern "C" int pc2d_adamw_step(int state_bits, const pc2d_adamw_tensor *tensors,
   PC2D_LAUNCH_CHECK("adamw_coef_kernel");
   const Betas b{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)weight_decay,
                 (uint64_t)seed};
+  auto group = [&](auto p, auto g, int dtype, int grad_dtype) -> int {
+    return launch_group<decltype(p), decltype(g)>(state_bits, tensors, count, numbers, dtype, grad_dtype, coef, grad_scale,
+                                                  b, s);
+  };
   const int F = PC2D_DTYPE_F32, H = PC2D_DTYPE_F16, B = PC2D_DTYPE_BF16;
-  if ((st = launch_group<float, float>(state_bits, tensors, count, F, F, coef, grad_scale, b, s)) != PC2D_OK ||
-      (st = launch_group<__half, __half>(state_bits, tensors, count, H, H, coef, grad_scale, b, s)) != PC2D_OK ||
-      (st = launch_group<__half, float>(state_bits, tensors, count, H, F, coef, grad_scale, b, s)) != PC2D_OK ||
-      (st = launch_group<__nv_bfloat16, __nv_bfloat16>(state_bits, tensors, count, B, B, coef, grad_scale, b, s)) !=
-          PC2D_OK ||
-      (st = launch_group<__nv_bfloat16, float>(state_bits, tensors, count, B, F, coef, grad_scale, b, s)) != PC2D_OK)
+  const float f32{};
+  const __half f16{};
+  const __nv_bfloat16 bf16{};
+  if ((st = group(f32, f32, F, F)) != PC2D_OK || (st = group(f16, f16, H, H)) != PC2D_OK ||
+      (st = group(f16, f32, H, F)) != PC2D_OK || (st = group(bf16, bf16, B, B)) != PC2D_OK ||
+      (st = group(bf16, f32, B, F)) != PC2D_OK)
     return st;
   return PC2D_OK;
 }

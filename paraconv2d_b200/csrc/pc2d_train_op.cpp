@@ -132,18 +132,14 @@ void adamw_step_cuda(at::TensorList params, at::TensorList grads, at::TensorList
     it.rate_first = factors.empty() ? 1.0 : factors[3 * i];
     it.rate_rest = factors.empty() ? 1.0 : factors[3 * i + 1];
     it.decay = factors.empty() ? 1.0 : factors[3 * i + 2];
-    if (!numbers.empty()) {
-      TORCH_CHECK(numbers[i] >= 0 && numbers[i] <= INT_MAX, call.what, ": numbers must be from 0 to 2^31 - 1, got ",
-                  numbers[i]);
-      it.shift = numbers[i] - (int64_t)i;
-    }
   }
   ranges.check(call.what);
   const size_t bytes = pc2d_adamw_workspace_size();
   const Tensor ws = workspace(bytes, step);
-  check_status(pc2d_adamw_step(bits8 ? 8 : 32, items.data(), (int)count, ptr<int64_t>(step), ptr<float>(rate), lr,
-                               beta1, beta2, eps, weight_decay, ptr<float>(grad_scale), seed, ptr(ws), bytes,
-                               stream_now()),
+  check_status(pc2d_adamw_step_numbered(bits8 ? 8 : 32, items.data(), (int)count,
+                                        numbers.empty() ? nullptr : numbers.data(), ptr<int64_t>(step), ptr<float>(rate),
+                                        lr, beta1, beta2, eps, weight_decay, ptr<float>(grad_scale), seed, ptr(ws),
+                                        bytes, stream_now()),
                call.what);
   changed(step);
   for (const auto &list : {params, exp_avgs, exp_avg_sqs, masters, scales})
